@@ -16,6 +16,8 @@ LIB_PATH = os.path.join(HERE, "libfmb200.so")
 MAX_ROW = 1024
 MAX_LAYERS = 2
 MAX_SPECIES = 8
+MAX_GROUPS = 1024
+ADAMW_BLOCK = 256
 IMAGES, IMAGE_ONCHIP, IMAGE_FIRST_PADDED = 0x464d4200, 1, 2   # LayerStruct.extra_images: mark and bits
 
 STATUS_CAND_OVERFLOW = 1
@@ -31,7 +33,9 @@ EXPORTS = ("fmb_version", "fmb_last_error", "fmb_sizeof", "fmb_launch_count", "f
            "fmb_forces", "fmb_forces_phase", "fmb_halo_gather_rows", "fmb_halo_add_rows", "fmb_halo_local_positions",
            "fmb_halo_owned_forces", "fmb_edge_features", "fmb_harmonics_probe", "fmb_forward", "fmb_backward", "fmb_gemm", "fmb_langevin_first_half",
            "fmb_langevin_second_half", "fmb_langevin_device_noise", "fmb_langevin_device_noise_ids",
-           "fmb_langevin_noise_sums", "fmb_langevin_first_half_global", "fmb_commit_forces", "fmb_profile_enable", "fmb_profile_read")
+           "fmb_langevin_noise_sums", "fmb_langevin_first_half_global", "fmb_commit_forces", "fmb_profile_enable", "fmb_profile_read",
+           "fmb_group_rows_scratch", "fmb_group_rows", "fmb_grouped_scratch", "fmb_grouped_linear", "fmb_grouped_input_gradient",
+           "fmb_grouped_weight_gradient", "fmb_adamw_step")
 
 
 class Fmb200Error(RuntimeError):
@@ -102,6 +106,29 @@ class LangevinStruct(ctypes.Structure):
     ]
 
 
+class GroupedStruct(ctypes.Structure):
+    _fields_ = [
+        ("type", c_int32), ("groups", c_int32), ("rows", c_int32), ("k", c_int32), ("n", c_int32), ("zero_rest", c_int32),
+        ("accumulate", c_int32), ("reserved", c_int32), ("order", c_void_p), ("offsets", c_void_p), ("x", c_void_p),
+        ("y", c_void_p), ("w", c_void_p), ("x_stride", ctypes.c_longlong), ("y_stride", ctypes.c_longlong),
+        ("w_row_stride", ctypes.c_longlong), ("w_group_stride", ctypes.c_longlong), ("scratch", c_void_p),
+        ("status", c_void_p),
+    ]
+
+
+class AdamwTensorStruct(ctypes.Structure):
+    _fields_ = [("p", c_void_p), ("g", c_void_p), ("copy", c_void_p), ("values", ctypes.c_longlong),
+                ("block", ctypes.c_longlong)]
+
+
+class AdamwStruct(ctypes.Structure):
+    _fields_ = [
+        ("moment_bits", c_int32), ("grad_type", c_int32), ("copy_type", c_int32), ("reserved", c_int32),
+        ("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
+        ("m", c_void_p), ("v", c_void_p), ("m_scale", c_void_p), ("v_scale", c_void_p), ("state", c_void_p),
+    ]
+
+
 STAGES = ("edge_features", "radial_gemm", "tp_forward_l0", "tp_forward_l1", "node_linears", "symcon_forward",
           "symcon_backward", "tp_backward_l1", "tp_backward_l0", "readout_reduce")
 
@@ -123,7 +150,8 @@ def load() -> ctypes.CDLL:
     lib.fmb_launch_count.restype = ctypes.c_longlong
     if lib.fmb_version() != VERSION:
         raise Fmb200Error(f"the library has version {lib.fmb_version()}, this binding {VERSION}: rebuild the library")
-    for which, struct in enumerate((NlStruct, ModelStruct, WorkStruct, LangevinStruct)):
+    for which, struct in enumerate((NlStruct, ModelStruct, WorkStruct, LangevinStruct, GroupedStruct, AdamwTensorStruct,
+                                    AdamwStruct)):
         if lib.fmb_sizeof(which) != ctypes.sizeof(struct):
             raise Fmb200Error(f"struct {struct.__name__} is {ctypes.sizeof(struct)} bytes here, "
                               f"{lib.fmb_sizeof(which)} in the library: rebuild the library")
@@ -152,6 +180,14 @@ def load() -> ctypes.CDLL:
     lib.fmb_commit_forces.argtypes = [POINTER(WorkStruct), P, P, P, P]
     lib.fmb_profile_enable.argtypes = [c_int]
     lib.fmb_profile_read.argtypes = [POINTER(c_float), POINTER(c_int), c_int]
+    lib.fmb_group_rows_scratch.argtypes = [ctypes.c_longlong, c_int]
+    lib.fmb_group_rows_scratch.restype = ctypes.c_longlong
+    lib.fmb_group_rows.argtypes = [P, c_int, ctypes.c_longlong, c_int, P, P, P, P]
+    lib.fmb_grouped_scratch.argtypes = [POINTER(GroupedStruct)]
+    lib.fmb_grouped_scratch.restype = ctypes.c_longlong
+    for name in ("fmb_grouped_linear", "fmb_grouped_input_gradient", "fmb_grouped_weight_gradient"):
+        getattr(lib, name).argtypes = [POINTER(GroupedStruct), P]
+    lib.fmb_adamw_step.argtypes = [POINTER(AdamwStruct), POINTER(AdamwTensorStruct), c_int, P]
     _LIB = lib
     return lib
 

@@ -58,6 +58,9 @@ extern "C" FMB_API int fmb_sizeof(int which) {
         case 1: return (int)sizeof(fmb_model_t);
         case 2: return (int)sizeof(fmb_work_t);
         case 3: return (int)sizeof(fmb_langevin_t);
+        case 4: return (int)sizeof(fmb_grouped_t);
+        case 5: return (int)sizeof(fmb_adamw_tensor_t);
+        case 6: return (int)sizeof(fmb_adamw_t);
         default: return -1;
     }
 }

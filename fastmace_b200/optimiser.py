@@ -1,0 +1,156 @@
+"""``AdamW`` over a model's weights: one launch per step for the whole list of tensors (``csrc/adamw.cu``), first and second
+moments in 32 or in 8 bits.
+
+    weights = {name: w.cuda() for name, w in init_weights(spec, seed).items()}
+    optimiser = AdamW(weights, lr=1e-3, state_bits=8)
+    optimiser.step(gradients)                       # {name: gradient}; tensors without one stay as they are
+
+With t the number of the step:
+
+    m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
+    p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+
+Weights and arithmetic are float32; gradients float32, bfloat16 or float16; ``copies`` are optional bfloat16 or float16
+tensors that a step leaves with the new weights (for products in 16 bits). With ``state_bits=8`` each 256 values of a tensor
+share a scale s per moment, the largest of them / 448: m is held as e4m3(m / s), v as e4m3(sqrt(v) / s), never as zero
+where v is not. A gradient that is not finite makes the moments of its value (with 8 bits: of its 256 values) not finite, and
+with them the weights.
+
+A step runs on the current stream of the weights' device, allocates nothing and can be captured: the number of the step is
+counted on the device, the learning rate and the other constants are those at capture. There is no CPU path.
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+from .grouped import TYPES
+
+BLOCK = _lib.ADAMW_BLOCK
+
+
+class AdamW:
+    def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                 state_bits: int = 32, copies=None):
+        self.names = list(params) if isinstance(params, dict) else list(range(len(params)))
+        self.params = [params[k] for k in self.names]
+        if not self.params:
+            raise ValueError("AdamW: no tensors")
+        if state_bits not in (8, 32):
+            raise ValueError("AdamW: state_bits is 8 or 32")
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+            raise ValueError("AdamW: betas in [0, 1)")
+        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
+            raise ValueError("AdamW: lr, eps and weight_decay must not be negative")
+        self.lr, self.betas, self.eps, self.weight_decay = float(lr), tuple(float(b) for b in betas), float(eps), float(weight_decay)
+        self.state_bits = int(state_bits)
+        self.device = self.params[0].device
+        for p in self.params:
+            if not p.is_cuda:
+                raise ValueError("AdamW: the weights must be CUDA tensors, there is no CPU path")
+            if p.dtype != torch.float32 or not p.is_contiguous() or p.device != self.device:
+                raise ValueError("AdamW: the weights must be contiguous float32 tensors on one device")
+        self.copies = [None] * len(self.params) if copies is None else [copies[k] for k in self.names]
+        self._copy_type = 0
+        for p, c in zip(self.params, self.copies):
+            if c is None:
+                continue
+            if c.dtype not in (torch.bfloat16, torch.float16) or not c.is_contiguous() or c.device != self.device or c.shape != p.shape:
+                raise ValueError("AdamW: a copy must be a contiguous bfloat16 or float16 tensor of its weights' shape")
+            if self._copy_type not in (0, TYPES[c.dtype]):
+                raise ValueError("AdamW: the copies must have one type")
+            self._copy_type = TYPES[c.dtype]
+        self.lib = _lib.load()
+        self.blocks, blocks = [], 0
+        for p in self.params:
+            self.blocks.append(blocks)
+            blocks += -(-p.numel() // BLOCK)
+        held = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
+        with torch.cuda.device(self.device):
+            # first moments, and second moments (their square roots in 8 bits), each tensor from the start of a block
+            self.m = torch.zeros(blocks * BLOCK, dtype=torch.float32, device=self.device).to(held)
+            self.v = torch.zeros(blocks * BLOCK, dtype=torch.float32, device=self.device).to(held)
+            scale = lambda: torch.full((blocks,), 2.0 ** -126, device=self.device) if self.state_bits == 8 else None  # noqa: E731
+            self.m_scale, self.v_scale = scale(), scale()
+            self._state = torch.tensor([0.0, 1.0, 1.0, 0.0], dtype=torch.float64, device=self.device)
+        self._tensors = (_lib.AdamwTensorStruct * len(self.params))()
+        for k, p in enumerate(self.params):
+            t = self._tensors[k]
+            t.p, t.values, t.block = p.data_ptr(), p.numel(), self.blocks[k]
+            t.copy = None if self.copies[k] is None else self.copies[k].data_ptr()
+        self._args = _lib.AdamwStruct()
+
+    def _fill_args(self) -> None:
+        a = self._args
+        a.moment_bits, a.copy_type = self.state_bits, self._copy_type
+        a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = self.lr, *self.betas, self.eps, self.weight_decay
+        a.m, a.v, a.state = self.m.data_ptr(), self.v.data_ptr(), self._state.data_ptr()
+        if self.state_bits == 8:
+            a.m_scale, a.v_scale = self.m_scale.data_ptr(), self.v_scale.data_ptr()
+
+    def step(self, grads) -> None:
+        """One step along ``grads`` (a dictionary or sequence like the weights; a missing or ``None`` gradient leaves its
+        tensor and its moments as they are). Counts as a step if any tensor has a gradient."""
+        if isinstance(grads, dict):
+            unknown = set(grads) - set(self.names)
+            if unknown:
+                raise ValueError(f"AdamW.step: gradients of unknown tensors: {sorted(map(str, unknown))}")
+            grads = [grads.get(k) for k in self.names]
+        elif len(grads) != len(self.params):
+            raise ValueError(f"AdamW.step: {len(grads)} gradients for {len(self.params)} tensors")
+        kind = None
+        for t, p, g in zip(self._tensors, self.params, grads):
+            if g is None:
+                t.g = None
+                continue
+            if g.dtype != kind:
+                if kind is not None or g.dtype not in TYPES:
+                    raise ValueError("AdamW.step: the gradients must have one type, float32, bfloat16 or float16")
+                kind = g.dtype
+            if g.shape != p.shape or not g.is_contiguous() or g.device != self.device:
+                raise ValueError("AdamW.step: a gradient must be contiguous, of its weights' shape and on their device")
+            t.g = g.data_ptr()
+        if kind is None:
+            return
+        self._fill_args()
+        self._args.grad_type = TYPES[kind]
+        with torch.cuda.device(self.device):
+            _lib.check(self.lib.fmb_adamw_step(ctypes.byref(self._args), self._tensors, len(self.params),
+                                               _lib.current_stream()), "fmb_adamw_step")
+
+    @property
+    def steps(self) -> int:
+        """Steps done (synchronises)."""
+        return int(self._state[0].item())
+
+    def load_moments(self, steps: int, *moments: torch.Tensor) -> None:
+        """Continue from the moments of a run of ``steps`` steps: ``m, v`` (32 bits) or ``m, m_scale, v, v_scale`` (8 bits), as
+        this class holds them under these names. The optimiser uses the tensors given, it does not copy them."""
+        names = ("m", "v") if self.state_bits == 32 else ("m", "m_scale", "v", "v_scale")
+        if len(moments) != len(names) or steps < 0:
+            raise ValueError(f"AdamW.load_moments: steps and {', '.join(names)}")
+        for name, t in zip(names, moments):
+            like = getattr(self, name)
+            if t.shape != like.shape or t.dtype != like.dtype or t.device != like.device or not t.is_contiguous():
+                raise ValueError(f"AdamW.load_moments: {name} must be a contiguous {like.dtype} tensor {tuple(like.shape)}")
+            if t.data_ptr() % 16:
+                raise ValueError(f"AdamW.load_moments: {name} must start at a multiple of 16 bytes")
+        for name, t in zip(names, moments):
+            setattr(self, name, t)
+        self._state.copy_(torch.tensor([steps, self.betas[0] ** steps, self.betas[1] ** steps, 0.0], dtype=torch.float64))
+
+    def moments(self, name) -> tuple[torch.Tensor, torch.Tensor]:
+        """First and second moments of one tensor in float32, in its shape."""
+        k = self.names.index(name)
+        p, b = self.params[k], self.blocks[k]
+        n = -(-p.numel() // BLOCK)
+        m, v = (t[b * BLOCK:(b + n) * BLOCK].float().view(n, BLOCK) for t in (self.m, self.v))
+        if self.state_bits == 8:
+            m, v = m * self.m_scale[b:b + n, None], (v * self.v_scale[b:b + n, None]) ** 2
+        return tuple(t.reshape(-1)[:p.numel()].view(p.shape).clone() for t in (m, v))
+
+
+__all__ = ["AdamW", "BLOCK"]

@@ -59,7 +59,7 @@ typedef void* fmb_stream_t;           /* a cudaStream_t */
 FMB_API int fmb_version(void);
 FMB_API const char* fmb_last_error(void);
 /* sizeof of the structs below, for the host binding to verify its mirror: which = 0 fmb_nl_t, 1 fmb_model_t,
- * 2 fmb_work_t, 3 fmb_langevin_t */
+ * 2 fmb_work_t, 3 fmb_langevin_t, 4 fmb_grouped_t, 5 fmb_adamw_tensor_t, 6 fmb_adamw_t */
 FMB_API int fmb_sizeof(int which);
 /* kernels this library has launched (or captured into a graph) in this process so far */
 FMB_API long long fmb_launch_count(void);
@@ -402,6 +402,89 @@ FMB_API int fmb_langevin_first_half_global(const fmb_langevin_t* lv, const doubl
 /* state.forces/energy/stress <- ForceOutput (fastmace/engine/graph.py:1125-1131): fp32 -> float64 copies. */
 FMB_API int fmb_commit_forces(const fmb_work_t* work, double* forces64, double* energy64, double* stress64,
                       fmb_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------ training of weights
+ * No counterpart in the reference, which evaluates trained models only. The products of a species-dependent linear (one
+ * matrix per group of rows, as in the skip of an interaction) over any number of groups, their two gradients, and the AdamW
+ * step over a model's weights. */
+#define FMB_MAX_GROUPS 1024
+#define FMB_TYPE_F32 0
+#define FMB_TYPE_BF16 1
+#define FMB_TYPE_F16 2
+
+/* Which rows belong to which group. order [rows]: the rows of group 0, then of group 1, ... in ascending order within a
+ * group, then the rows whose key is no group (negative, or >= groups). offsets [groups + 1]: where each group starts;
+ * offsets[groups] is the number of rows that have a group. keys: int32 or int64 (key_bytes 4 or 8). 1 <= groups <=
+ * FMB_MAX_GROUPS, 0 <= rows. scratch: fmb_group_rows_scratch(rows, groups) int32, written before it is read. */
+FMB_API long long fmb_group_rows_scratch(long long rows, int groups);
+FMB_API int fmb_group_rows(const void* keys, int key_bytes, long long rows, int groups, int32_t* order, int32_t* offsets,
+                           int32_t* scratch, fmb_stream_t stream);
+
+/* One call of the grouped products. Matrices are row-major with the strides given, in elements; the last index is
+ * contiguous. `order` and `offsets` as fmb_group_rows writes them; entries out of range are skipped. Weights of a group:
+ * w + g * w_group_stride, k rows w_row_stride apart, n columns. type: of x, w, y (FMB_TYPE_*). */
+typedef struct {
+    int32_t type;
+    int32_t groups;
+    int32_t rows;                     /* rows of x and y, and entries of `order` */
+    int32_t k;
+    int32_t n;
+    int32_t zero_rest;                /* linear, input gradient: rows of no group become zero instead of staying as they are */
+    int32_t accumulate;               /* weight gradient: add to dw */
+    int32_t reserved;
+    const int32_t* order;
+    const int32_t* offsets;
+    void* x;                          /* [rows][k]: output of the input gradient */
+    void* y;                          /* [rows][n]: output of the linear */
+    void* w;                          /* [groups][k][n]: weights; of the weight gradient its output, always fp32 */
+    long long x_stride;
+    long long y_stride;
+    long long w_row_stride;
+    long long w_group_stride;
+    float* scratch;                   /* weight gradient: fmb_grouped_scratch(...) floats, written before they are read */
+    uint32_t* status;                 /* device word, may be null: receives FMB_STATUS_TENSOR_TIMEOUT */
+} fmb_grouped_t;
+
+/* y[r] = x[r] W[g(r)] */
+FMB_API int fmb_grouped_linear(const fmb_grouped_t* args, fmb_stream_t stream);
+/* x[r] = y[r] W[g(r)]^T */
+FMB_API int fmb_grouped_input_gradient(const fmb_grouped_t* args, fmb_stream_t stream);
+/* W[g] (+)= sum of x[r]^T y[r] over the rows of group g, in fp32, summed in an order that depends on the sizes alone; zero
+ * for groups without rows */
+FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* args, fmb_stream_t stream);
+/* floats of scratch that fmb_grouped_weight_gradient needs for these sizes (fields type, groups, rows, k, n are read) */
+FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* args);
+
+#define FMB_ADAMW_BLOCK 256           /* values that share a scale where moments are held in 8 bits */
+
+/* A tensor of an AdamW step. The moments of its `values` values start at `block` * FMB_ADAMW_BLOCK in the moment arrays of
+ * the step (a tensor begins a block, its last block is filled up with values that are never read for a weight). */
+typedef struct {
+    float* p;                         /* weights */
+    const void* g;                    /* gradient; null: the tensor is left as it is */
+    void* copy;                       /* optional copy of the weights in 16 bits */
+    long long values;
+    long long block;
+} fmb_adamw_tensor_t;
+
+typedef struct {
+    int32_t moment_bits;              /* 32: m and v are fp32; 8: m and r are e4m3 in units of m_scale / r_scale per block */
+    int32_t grad_type;                /* FMB_TYPE_* of every g */
+    int32_t copy_type;                /* FMB_TYPE_BF16 or FMB_TYPE_F16 of every copy */
+    int32_t reserved;
+    double lr, beta1, beta2, eps, weight_decay;
+    void* m;                          /* first moments */
+    void* v;                          /* second moments; with 8 bits their square roots r */
+    float* m_scale;                   /* [blocks], 8 bits only */
+    float* v_scale;
+    double* state;                    /* [4] on the device: steps done, beta1^steps, beta2^steps, 0 */
+} fmb_adamw_t;
+
+/* One step over all tensors:
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2,
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * The number of the step t is read from `state` and advanced on the device, so a captured step can be replayed. */
+FMB_API int fmb_adamw_step(const fmb_adamw_t* args, const fmb_adamw_tensor_t* tensors, int count, fmb_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,184 @@
+"""AdamW on the GPU against the formula in float64.
+
+Tolerances of one step. With moments in 32 bits m and v are one product and one fused or rounded sum of two terms: 4 roundings,
+2^-22 of the terms' magnitudes. A weight moves by at most a few lr, computed with about ten roundings and an approximate
+division (2^-22): 2^-20 of the update, and one rounding of the weight, 2^-24 of it (plus 2^-24 for the decay's). Moments in 8 bits: the
+new moment is within half a step of e4m3 of the formula's, 2^-4 of itself or 2^-10 of the block's scale (below its smallest normal
+number), and the scale is off by a rounding or two, 2^-22.
+"""
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+SIZES = [[1], [5, 300, 256, 255, 257, 1000], [16_384, 4096, 512, 2, 33_000], [3] * 450, [200_001]]
+
+
+def _formula(p, g, m, v, t, lr, b1, b2, eps, wd):
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    update = lr / (1 - b1 ** t) * m / (torch.sqrt(v) / (1 - b2 ** t) ** 0.5 + eps)
+    return p * (1 - lr * wd) - update, m, v, update
+
+
+def _case(sizes, grad, seed, offset=0):
+    """Weights and gradients of the sizes, views of one buffer each that start `offset` elements off its alignment."""
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    total = sum(sizes)
+
+    def views(t):
+        out, at = [], offset
+        for n in sizes:
+            out.append(t[at:at + n])
+            at += n
+        return out
+
+    p = torch.randn(total + offset, generator=g, device="cuda")
+    size = torch.exp(3 * torch.randn(total + offset, generator=g, device="cuda")) * 1e-3
+    gr = (torch.randn(total + offset, generator=g, device="cuda") * size).to(grad)
+    return views(p), views(gr), views(torch.zeros(total + offset, dtype=torch.bfloat16, device="cuda"))
+
+
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("grad", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{s[0]}")
+def test_steps_against_the_formula(sizes, bits, grad, offset):
+    from fastmace_b200.optimiser import BLOCK, AdamW
+    hyper = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.02)
+    params, _, copies = _case(sizes, grad, 1, offset)
+    opt = AdamW(params, state_bits=bits, copies=copies, **hyper)
+    for t in range(1, 4):
+        grads = _case(sizes, grad, 10 + t, offset)[1]
+        before = [(p.double(), *(x.double() for x in opt.moments(k))) for k, p in enumerate(params)]
+        opt.step(grads)
+        for k, (p, g, c) in enumerate(zip(params, grads, copies)):
+            p0, m0, v0 = before[k]
+            rp, rm, rv, update = _formula(p0, g.double(), m0, v0, t, 3e-3, 0.9, 0.99, 1e-8, 0.02)
+            assert bool(((p.double() - rp).abs() <= 2.0 ** -20 * update.abs() + 2.0 ** -23 * p0.abs() + 1e-30).all())
+            assert torch.equal(c, p.to(torch.bfloat16))
+            m, v = (x.double() for x in opt.moments(k))
+            if bits == 32:
+                assert bool(((m - rm).abs() <= 2.0 ** -22 * (0.9 * m0.abs() + 0.1 * g.double().abs()) + 1e-37).all())
+                assert bool(((v - rv).abs() <= 2.0 ** -22 * rv + 1e-37).all())
+                continue
+            blocks = -(-p.numel() // BLOCK)
+            for got, ref in ((m, rm), (v.sqrt(), rv.sqrt())):
+                pad = torch.zeros(blocks * BLOCK, dtype=torch.float64, device="cuda")
+                pad[:p.numel()] = ref.view(-1)
+                scale = (pad.view(-1, BLOCK).abs().amax(1) / 448).repeat_interleave(BLOCK)[:p.numel()]
+                tol = torch.maximum(2.0 ** -4 * ref.abs(), 2.0 ** -10 * scale) * (1 + 2.0 ** -18) + 2.0 ** -135
+                # a root too small for the type is held as the smallest number, 2^-9 of the scale, instead of zero
+                if got is not m:
+                    tol = torch.where((ref > 0) & (ref < 2.0 ** -9 * scale), 2.0 ** -9 * scale, tol)
+                assert bool(((got - ref).abs() <= tol).all()), float(((got - ref).abs() - tol).max())
+            assert bool((v[rv > 0] > 0).all())
+    assert opt.steps == 3
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_without_a_gradient_stay(bits):
+    from fastmace_b200.optimiser import AdamW
+    g = torch.Generator(device="cuda").manual_seed(3)
+    weights = {n: torch.randn(s, generator=g, device="cuda") for n, s in (("a", (7, 90)), ("b", (300,)), ("c", (4, 5, 6)), ("d", (0,)))}
+    opt = AdamW(weights, lr=0.1, state_bits=bits)
+    opt.step({n: torch.ones_like(w) for n, w in weights.items()})
+    kept = [weights["b"].clone(), *opt.moments("b")]
+    old = weights["a"].clone()
+    opt.step({"a": torch.ones(7, 90, device="cuda"), "c": torch.ones(4, 5, 6, device="cuda"), "b": None})
+    assert all(torch.equal(x, y) for x, y in zip(kept, (weights["b"], *opt.moments("b"))))
+    assert not torch.equal(old, weights["a"]) and opt.steps == 2
+    opt.step({})
+    assert opt.steps == 2
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps_count_on(bits):
+    """A captured step replayed with new gradients gives the bits of the same steps taken one by one, and two optimisers' graphs
+    replayed on two streams do not meet."""
+    from fastmace_b200.optimiser import AdamW
+    g = torch.Generator(device="cuda").manual_seed(4)
+    start = [torch.randn(n, generator=g, device="cuda") for n in (5000, 77, 300)]
+    grads = [[torch.randn(n, generator=g, device="cuda") for n in (5000, 77, 300)] for _ in range(6)]
+
+    def fresh():
+        params = [p.clone() for p in start]
+        return params, AdamW(params, lr=1e-2, state_bits=bits)
+
+    params, opt = fresh()
+    for step in grads:
+        opt.step(step)
+    runs = []
+    for _ in range(2):
+        p, o = fresh()
+        held = [x.clone() for x in grads[0]]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o.step(held)
+        runs.append((p, o, held, graph, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for step in grads:
+        for p, o, held, graph, stream in runs:
+            with torch.cuda.stream(stream):
+                for h, x in zip(held, step):
+                    h.copy_(x)
+                graph.replay()
+    torch.cuda.synchronize()
+    for p, o, *_ in runs:
+        assert o.steps == 6 and all(torch.equal(a, b) for a, b in zip(p, params))
+        assert torch.equal(o.m.view(torch.uint8), opt.m.view(torch.uint8)) and torch.equal(o.v.view(torch.uint8), opt.v.view(torch.uint8))
+
+
+def test_continued_from_given_moments():
+    from fastmace_b200.optimiser import AdamW
+    for bits in (32, 8):
+        g = torch.Generator(device="cuda").manual_seed(5)
+        a = [torch.randn(1000, generator=g, device="cuda")]
+        b = [a[0].clone()]
+        grads = [[torch.randn(1000, generator=g, device="cuda")] for _ in range(4)]
+        one, two = AdamW(a, state_bits=bits), AdamW(b, state_bits=bits)
+        for x in grads:
+            one.step(x)
+        for x in grads[:2]:
+            two.step(x)
+        held = (two.m.clone(), two.v.clone()) if bits == 32 else (two.m.clone(), two.m_scale.clone(), two.v.clone(), two.v_scale.clone())
+        two = AdamW(b, state_bits=bits)
+        two.load_moments(2, *held)
+        for x in grads[2:]:
+            two.step(x)
+        assert torch.equal(a[0], b[0]) and two.steps == 4
+
+
+def test_values_that_are_not_finite_or_zero():
+    from fastmace_b200.optimiser import AdamW
+    for bits in (32, 8):
+        p = [torch.ones(1024, device="cuda")]
+        opt = AdamW(p, lr=0.1, weight_decay=0.0, state_bits=bits)
+        opt.step([torch.zeros(1024, device="cuda")])
+        assert bool((p[0] == 1).all())
+        bad = torch.ones(1024, device="cuda")
+        bad[300] = float("nan")
+        bad[800] = float("inf")
+        opt.step([bad])
+        fine = torch.ones(1024, dtype=torch.bool, device="cuda")
+        fine[[300, 800]] = False
+        assert bool(torch.isfinite(p[0][fine]).all()) and bool(torch.isnan(p[0][300]))
+        opt.step([torch.ones(1024, device="cuda")])
+        if bits == 8:
+            fine[256:512] = False
+            fine[768:] = False
+        assert bool(torch.isfinite(p[0][fine]).all()) and bool(torch.isnan(p[0][300])) and not bool(torch.isfinite(p[0][800]))
+
+
+def test_refusals_on_the_device():
+    from fastmace_b200.optimiser import AdamW
+    w = torch.zeros(8, 8, device="cuda")
+    for bad in (lambda: AdamW([]), lambda: AdamW([w.half()]), lambda: AdamW([w.t()[:4]]), lambda: AdamW([w], state_bits=16),
+                lambda: AdamW([w], betas=(1.0, 0.9)), lambda: AdamW([w], lr=-1.0), lambda: AdamW([w], copies=[w]),
+                lambda: AdamW([w], copies=[w.half()[:4]]), lambda: AdamW([w]).step([w, w]), lambda: AdamW([w]).step([w.double()]),
+                lambda: AdamW([w]).step([w[:4]]), lambda: AdamW([w]).step([w.t()]), lambda: AdamW({"a": w}).step({"b": w}),
+                lambda: AdamW([w, w.clone()]).step([w, w.half()]), lambda: AdamW([w]).step([w.cpu()]),
+                lambda: AdamW([w]).load_moments(1, w), lambda: AdamW([w]).load_moments(1, w, w)):
+        with pytest.raises(ValueError):
+            bad()
