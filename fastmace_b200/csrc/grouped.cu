@@ -1,29 +1,14 @@
 // Products of a grouped linear and its gradients: one matrix per group of rows (fmb_grouped_linear and the calls beside it).
 
-#include "fmb_common.cuh"
-
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
+#include "grouped.cuh"
 
 namespace fmb {
 
 namespace {
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-template <typename T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+using namespace grp;
 
 constexpr int kT = 64, kK = 16, kThreads = 256;
-
-// the rows [begin, end) of group g in `order`, whatever offsets holds
-__device__ __forceinline__ void group_span(const int32_t* offsets, int g, int rows, int& begin, int& end) {
-    begin = min(max(offsets[g], 0), rows);
-    end = min(max(offsets[g + 1], begin), rows);
-}
 
 // out[r] = in[r] W[g] (or W[g]^T): a CTA takes 64 rows of a group and 64 columns
 template <typename T, bool TRANSPOSED>
@@ -150,6 +135,8 @@ int rows_launch(const fmb_grouped_t* a, cudaStream_t stream) {
     const int rc = check(a, 0, 0);
     if (rc) return rc;
     if (a->rows == 0) return FMB_OK;
+    const int by_tma = tma_launch(a, TRANSPOSED ? kInputGradient : kLinear, stream);
+    if (by_tma != FMB_ERR_UNSUPPORTED) return by_tma;
     const dim3 grid(ceil_div(a->rows, kT) + a->groups + 1, ceil_div(TRANSPOSED ? a->k : a->n, kT));
     if (a->type == FMB_TYPE_F32) k_grouped_rows<float, TRANSPOSED><<<grid, kThreads, 0, stream>>>(*a);
     else if (a->type == FMB_TYPE_BF16) k_grouped_rows<__nv_bfloat16, TRANSPOSED><<<grid, kThreads, 0, stream>>>(*a);
@@ -173,14 +160,17 @@ extern "C" FMB_API int fmb_grouped_input_gradient(const fmb_grouped_t* a, fmb_st
 }
 
 extern "C" FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* a) {
-    (void)a;
-    return 0;
+    return a && a->groups >= 1 && a->k >= 1 && a->n >= 1 ? scratch_floats(a) : 0;
 }
 
 extern "C" FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* a, fmb_stream_t stream_) {
     const int rc = check(a, 0, 0);
     if (rc) return rc;
     cudaStream_t stream = (cudaStream_t)stream_;
+    if (a->rows) {
+        const int by_tma = tma_launch(a, kWeightGradient, stream);
+        if (by_tma != FMB_ERR_UNSUPPORTED) return by_tma;
+    }
     const dim3 grid(ceil_div(a->k, kT), ceil_div(a->n, kT), a->groups);
     if (a->type == FMB_TYPE_F32) k_grouped_weights<float><<<grid, kThreads, 0, stream>>>(*a);
     else if (a->type == FMB_TYPE_BF16) k_grouped_weights<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(*a);

@@ -1,0 +1,74 @@
+// What the kernels of the grouped products share: spans of the groups, units of work, conversions.
+#pragma once
+
+#include "fmb_common.cuh"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+namespace fmb {
+namespace grp {
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T from_float(float x);
+template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// the entries [begin, end) of group g in `order`, whatever offsets holds
+__device__ __forceinline__ void group_span(const int32_t* offsets, int g, int rows, int& begin, int& end) {
+    begin = min(max(offsets[g], 0), rows);
+    end = min(max(offsets[g + 1], begin), rows);
+}
+
+// A unit is up to `size` entries of one group. first[g] = units of the groups before g, first[groups] = all; groups without
+// rows have `empty` units. By the whole CTA (THREADS threads, a multiple of 32); ends with a barrier.
+template <int THREADS>
+__device__ __forceinline__ void count_units(const int32_t* offsets, int groups, int rows, int size, int empty, int* first) {
+    __shared__ int warp_total[THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int per = (groups + THREADS - 1) / THREADS, from = min(groups, (int)threadIdx.x * per), to = min(groups, from + per);
+    int sum = 0;
+    for (int g = from; g < to; ++g) {
+        int begin, end;
+        group_span(offsets, g, rows, begin, end);
+        const int units = end > begin ? (end - begin - 1) / size + 1 : empty;
+        first[g] = sum;
+        sum += units;
+    }
+    int inclusive = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, inclusive, o);
+        if (lane >= o) inclusive += up;
+    }
+    if (lane == 31) warp_total[warp] = inclusive;
+    __syncthreads();
+    int before = inclusive - sum;
+    for (int w = 0; w < warp; ++w) before += warp_total[w];
+    for (int g = from; g < to; ++g) first[g] += before;
+    if (threadIdx.x == THREADS - 1) first[groups] = before + sum;
+    __syncthreads();
+}
+
+// the group that unit u belongs to: the last one that begins at or before it
+__device__ __forceinline__ int group_of_unit(const int* first, int groups, int u) {
+    int low = 0, high = groups - 1;
+    while (low < high) {
+        const int mid = (low + high + 1) >> 1;
+        if (first[mid] <= u) low = mid; else high = mid - 1;
+    }
+    return low;
+}
+
+enum Mode { kLinear = 0, kInputGradient = 1, kWeightGradient = 2 };
+
+// tcgen05 kernels with operands by TMA (grouped_tc.cu): FMB_ERR_UNSUPPORTED for types and alignments that TMA does not take
+int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
+// floats of scratch of the weight gradient
+long long scratch_floats(const fmb_grouped_t* a);
+
+}  // namespace grp
+}  // namespace fmb

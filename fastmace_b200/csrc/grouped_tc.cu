@@ -1,0 +1,585 @@
+// Grouped products of 16-bit operands on tcgen05 with operands by TMA.
+//
+// All three products are tiles D[128 features][TN rows of the output] of sums over `depth`:
+//   linear           features: columns of W, rows: gathered rows of x, depth: k
+//   input gradient   features: rows of W,    rows: gathered rows of y, depth: n
+//   weight gradient  features: columns of y, rows: columns of x,       depth: the rows of a group, gathered
+// The features lie on the 128 accumulator lanes because they are many whatever the group: the other side of the tile shrinks to
+// the rows a group has (multiples of 16), so a group of one row costs an MMA of 16 columns, and an accumulator column is
+// a run of the output row: 32 lanes store 64 or 128 consecutive bytes.
+//
+// Rows are where the groups' order says: they come by TMA gather (four row numbers an instruction), which fills what is no row
+// with zeros; nothing is permuted in memory. Weights come by TMA tiles from the caller's layout. Operands whose depth runs along
+// memory are K-major tiles, the others MN-major ones; both with the 128-byte swizzle.
+
+#include "grouped.cuh"
+#include "tc_common.cuh"
+
+#include <cuda.h>
+
+#include <algorithm>
+
+namespace fmb {
+namespace grp {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kDepth = 64;                       // depth of a stage: 128 bytes of 16-bit values
+constexpr unsigned kSpin = 1u << 20;
+constexpr int kProducerWarps = 4, kEpilogueWarps = 8;
+constexpr int kThreads = 32 * (kProducerWarps + kEpilogueWarps);
+constexpr int kChunk = 512;                      // weight gradient: depth after which an accumulator moves to registers
+
+template <int TN> struct Shape {
+    static constexpr int kFeatureBytes = 128 * kDepth * 2, kRowBytes = TN * kDepth * 2;
+    static constexpr int kStageBytes = kFeatureBytes + kRowBytes;
+    static constexpr int kStages = (200 * 1024) / kStageBytes < 8 ? (200 * 1024) / kStageBytes : 8;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + (FMB_MAX_GROUPS + 1) * 4 + 256;
+    static constexpr int kTmem = 2 * TN < 32 ? 32 : 2 * TN;
+};
+
+struct Args {
+    fmb_grouped_t a;
+    int feature_tiles, row_tiles;                // of the output; row_tiles 1 where rows are gathered
+    int unit_rows;                               // entries of a group per unit
+    int wide_store;                              // output rows may be written 4 bytes at a time
+};
+
+__device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                 :: "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int col, int r0, int r1, int r2, int r3, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+                 :: "r"(dst), "l"(map), "r"(col), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n"
+        :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// MN-major tile with the 128-byte swizzle: 64 depths of 64 features each, 8 KB apart, 1024 bytes between 8 depths
+__device__ __forceinline__ uint64_t make_desc_mn(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3ffff) >> 4);
+    d |= (uint64_t)(kDepth * 128 >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]), "=&r"(r[4]), "=&r"(r[5]), "=&r"(r[6]), "=&r"(r[7]),
+          "=&r"(r[8]), "=&r"(r[9]), "=&r"(r[10]), "=&r"(r[11]), "=&r"(r[12]), "=&r"(r[13]), "=&r"(r[14]), "=&r"(r[15]),
+          "=&r"(r[16]), "=&r"(r[17]), "=&r"(r[18]), "=&r"(r[19]), "=&r"(r[20]), "=&r"(r[21]), "=&r"(r[22]), "=&r"(r[23]),
+          "=&r"(r[24]), "=&r"(r[25]), "=&r"(r[26]), "=&r"(r[27]), "=&r"(r[28]), "=&r"(r[29]), "=&r"(r[30]), "=&r"(r[31])
+        : "r"(taddr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Tile t of the launch: its unit (entries [first, first + count) of group g in `order`), features and output rows.
+struct Tile {
+    int unit, g, first, count, feature0, row0, units_of_group;
+};
+
+template <int MODE>
+__device__ __forceinline__ Tile locate(const Args& p, const int* first_unit, int t, int tn) {
+    Tile w;
+    const int per_unit = p.feature_tiles * p.row_tiles;
+    w.unit = t / per_unit;
+    const int rest = t - w.unit * per_unit, rt = rest / p.feature_tiles;
+    w.row0 = rt * tn;
+    w.feature0 = (rest - rt * p.feature_tiles) * 128;
+    w.g = group_of_unit(first_unit, p.a.groups, w.unit);
+    int begin, end;
+    group_span(p.a.offsets, w.g, p.a.rows, begin, end);
+    // offsets that are none could make a unit that lies outside its group: it has no entries
+    const int skip = w.unit - first_unit[w.g];
+    const long long first = begin + (long long)skip * p.unit_rows;
+    // (in 64 bits: as the minimum of a 32-bit difference and unit_rows the count came out as end + first, CUDA 12.9)
+    const long long left = skip >= 0 ? end - first : 0;
+    w.first = left > 0 ? (int)first : end;
+    w.count = left <= 0 ? 0 : left < p.unit_rows ? (int)left : p.unit_rows;
+    w.units_of_group = first_unit[w.g + 1] - first_unit[w.g];
+    return w;
+}
+
+// a row number that TMA fills with zeros stands for everything that is no row
+__device__ __forceinline__ int row_at(const Args& p, int entry, int end) {
+    const int row = entry < end ? __ldg(p.a.order + entry) : p.a.rows;
+    return (unsigned)row < (unsigned)p.a.rows ? row : p.a.rows;
+}
+
+template <typename T, int MODE, int TN>
+__global__ void __launch_bounds__(kThreads, 1)
+k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap feature_map, const __grid_constant__ CUtensorMap row_map) {
+    using S = Shape<TN>;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    int* const first_unit = reinterpret_cast<int*>(smem + S::kStages * S::kStageBytes);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStageBytes + ((FMB_MAX_GROUPS + 1) * 4 + 7) / 8 * 8);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 4);
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const uint32_t bar0 = smem_u32(bars), stage0 = smem_u32(smem);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (S::kStages + s); };
+    auto acc_full = [&](int b) { return bar0 + 8u * (2 * S::kStages + b); };
+    auto acc_empty = [&](int b) { return bar0 + 8u * (2 * S::kStages + 2 + b); };
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+    constexpr bool kWeights = MODE == kWeightGradient;
+    constexpr int kGatherWarps = 2;              // bring the rows of the output; warp 0 brings the features, warp 3 issues the MMAs
+
+    if (warp == 0) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
+    if (warp == 3 && elect_one()) {
+        for (int s = 0; s < S::kStages; ++s) {
+            mbar_init(full(s), 1 + kGatherWarps);
+            mbar_init(empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full(b), 1);
+            mbar_init(acc_empty(b), kEpilogueWarps);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    count_units<kThreads>(p.a.offsets, p.a.groups, p.a.rows, p.unit_rows, kWeights ? 1 : 0, first_unit);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const int tiles = first_unit[p.a.groups] * p.feature_tiles * p.row_tiles;
+    const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n;        // not of the weight gradient
+
+    if (warp < 3) {
+        // ---------------------------------------------------------------- producers
+        int at = 0;
+        uint32_t phase = 0;
+        const int part = warp - 1;               // of the gather
+        bool alive = true;
+        for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
+            const Tile w = locate<MODE>(p, first_unit, t, TN);
+            const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
+            const int end = w.first + w.count;
+            // rows of the output this warp gathers: lane l holds the row numbers 4 (part * TN / 8 + l) and on
+            int rows[4];
+            constexpr int kPerWarp = TN / 4 / kGatherWarps;
+            if (!kWeights && warp > 0) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) rows[i] = lane < kPerWarp ? row_at(p, w.first + 4 * (part * kPerWarp + lane) + i, end) : 0;
+            }
+            int next[4];
+            if (kWeights) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) next[i] = row_at(p, w.first + 4 * (lane & 15) + i, end);
+            }
+            for (int b = 0; b < blocks; ++b) {
+                const int d0 = b * kDepth;
+                if (kWeights) {
+                    // the depths of this block, and those of the next on their way
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        rows[i] = next[i];
+                        next[i] = row_at(p, w.first + d0 + kDepth + 4 * (lane & 15) + i, end);
+                    }
+                }
+                alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
+                if (!alive) break;
+                const uint32_t base = stage0 + at * S::kStageBytes, bar = full(at);
+                // depths past the end are filled with zeros up to a multiple of 16
+                const int quads = kWeights ? min(16, (w.count - d0 + 15) / 16 * 4) : 0;
+                if (warp == 0) {
+                    if constexpr (kWeights) {
+                        if (elect_one()) mbar_expect_tx(bar, quads * 2 * 512);
+                        __syncwarp();
+                        for (int q = 0; q < quads; ++q) {
+                            const int r0 = __shfl_sync(0xffffffffu, rows[0], q), r1 = __shfl_sync(0xffffffffu, rows[1], q);
+                            const int r2 = __shfl_sync(0xffffffffu, rows[2], q), r3 = __shfl_sync(0xffffffffu, rows[3], q);
+                            if (elect_one()) {
+                                tma_gather4(base + q * 512, &feature_map, w.feature0, r0, r1, r2, r3, bar);
+                                tma_gather4(base + 8192 + q * 512, &feature_map, w.feature0 + 64, r0, r1, r2, r3, bar);
+                            }
+                            __syncwarp();
+                        }
+                    } else if (elect_one()) {
+                        mbar_expect_tx(bar, S::kFeatureBytes);
+                        if constexpr (MODE == kLinear) {
+                            tma_tile_3d(base, &feature_map, w.feature0, d0, w.g, bar);
+                            tma_tile_3d(base + 8192, &feature_map, w.feature0 + 64, d0, w.g, bar);
+                        } else {
+                            tma_tile_3d(base, &feature_map, d0, w.feature0, w.g, bar);
+                        }
+                    }
+                    __syncwarp();
+                } else if constexpr (kWeights) {
+                    constexpr int kChunks = TN / 64 / kGatherWarps;          // of 64 output rows
+                    const uint32_t dst = base + S::kFeatureBytes + part * kChunks * 8192;
+                    if (elect_one()) mbar_expect_tx(bar, quads * kChunks * 512);
+                    __syncwarp();
+                    for (int q = 0; q < quads; ++q) {
+                        const int r0 = __shfl_sync(0xffffffffu, rows[0], q), r1 = __shfl_sync(0xffffffffu, rows[1], q);
+                        const int r2 = __shfl_sync(0xffffffffu, rows[2], q), r3 = __shfl_sync(0xffffffffu, rows[3], q);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int c = 0; c < kChunks; ++c)
+                                tma_gather4(dst + c * 8192 + q * 512, &row_map, w.row0 + (part * kChunks + c) * 64, r0, r1, r2, r3, bar);
+                        }
+                        __syncwarp();
+                    }
+                } else {
+                    const int mine = min(kPerWarp, max(0, (w.count + 3) / 4 - part * kPerWarp));
+                    const uint32_t dst = base + S::kFeatureBytes + part * kPerWarp * 512;
+                    if (elect_one()) {
+                        if (mine) mbar_expect_tx(bar, mine * 512);
+                        else mbar_arrive(bar);
+                    }
+                    __syncwarp();
+                    for (int q = 0; q < mine; ++q) {
+                        const int r0 = __shfl_sync(0xffffffffu, rows[0], q), r1 = __shfl_sync(0xffffffffu, rows[1], q);
+                        const int r2 = __shfl_sync(0xffffffffu, rows[2], q), r3 = __shfl_sync(0xffffffffu, rows[3], q);
+                        if (elect_one()) tma_gather4(dst + q * 512, &row_map, d0, r0, r1, r2, r3, bar);
+                        __syncwarp();
+                    }
+                }
+                if (++at == S::kStages) {
+                    at = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 3) {
+        // ---------------------------------------------------------------- MMAs
+        int at = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        constexpr uint32_t kType = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1 : 0;
+        constexpr uint32_t kMajor = MODE == kLinear ? 1u << 15 : MODE == kWeightGradient ? 3u << 15 : 0;
+        constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | kMajor | ((uint32_t)(128 >> 4) << 24);
+        bool alive = true;
+        for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
+            const Tile w = locate<MODE>(p, first_unit, t, TN);
+            const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
+            const int columns = kWeights ? TN : max(16, min(TN, (w.count + 15) / 16 * 16));
+            const uint32_t idesc = kDesc | ((uint32_t)(columns >> 3) << 17);
+            for (int b = 0; b < blocks; ++b) {
+                const bool fresh = b == 0 || (kWeights && b % (kChunk / kDepth) == 0);
+                if (fresh) alive = mbar_wait(acc_empty(acc), acc_phase ^ 1, abort_flag, kSpin);
+                alive = alive && mbar_wait(full(at), phase, abort_flag, kSpin);
+                if (!alive) break;
+                fence_after_sync();
+                const uint32_t base = stage0 + at * S::kStageBytes;
+                const uint64_t fd = MODE == kInputGradient ? make_desc(base) : make_desc_mn(base);
+                const uint64_t rd = kWeights ? make_desc_mn(base + S::kFeatureBytes) : make_desc(base + S::kFeatureBytes);
+                const int steps = min(4, (depth - b * kDepth + 15) / 16);
+                const uint32_t d = tmem + acc * TN;
+                if (elect_one()) {
+                    for (int k = 0; k < steps; ++k) {
+                        constexpr uint64_t kF = MODE == kInputGradient ? 2 : 128, kR = kWeights ? 128 : 2;
+                        mma_f16(d, fd + k * kF, rd + k * kR, idesc, k > 0 || !fresh);
+                    }
+                    mma_commit(empty(at));
+                    const bool last = b == blocks - 1 || (kWeights && (b + 1) % (kChunk / kDepth) == 0);
+                    if (last) mma_commit(acc_full(acc));
+                }
+                __syncwarp();
+                if (b == blocks - 1 || (kWeights && (b + 1) % (kChunk / kDepth) == 0)) {
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1;
+                }
+                if (++at == S::kStages) {
+                    at = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- epilogue
+        const int ew = warp - kProducerWarps, quarter = ew & 3, half = ew >> 2;      // lanes 32 quarter + [0, 32), half of the columns
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        const int width = MODE == kInputGradient ? p.a.k : p.a.n;
+        if (!kWeights && p.a.zero_rest) {
+            // rows of no group
+            T* const out = (T*)(MODE == kLinear ? p.a.y : p.a.x);
+            const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
+            const int from = min(max(p.a.offsets[p.a.groups], 0), p.a.rows);
+            for (int i = from + blockIdx.x * kEpilogueWarps + ew; i < p.a.rows; i += gridDim.x * kEpilogueWarps) {
+                const int row = row_at(p, i, p.a.rows);
+                if (row < p.a.rows)
+                    for (int c = lane; c < width; c += 32) out[row * stride + c] = from_float<T>(0.0f);
+            }
+        }
+        bool alive = true;
+        for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
+            const Tile w = locate<MODE>(p, first_unit, t, TN);
+            const int feature = w.feature0 + quarter * 32 + lane;
+            if constexpr (kWeights) {
+                constexpr int kCols = TN / 2;
+                const int chunks = (w.count + kChunk - 1) / kChunk;
+                float sum[kCols];
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
+                for (int c = 0; c < chunks; ++c) {
+                    alive = mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
+                    if (!alive) break;
+                    fence_after_sync();
+#pragma unroll
+                    for (int j0 = 0; j0 < kCols; j0 += 32) {
+                        float v[32];
+                        tmem_load_32(tmem + lanes + acc * TN + half * kCols + j0, v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[j0 + j] += v[j];
+                    }
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty(acc));
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1;
+                }
+                const bool direct = w.units_of_group <= 1;
+                const long long stride = direct ? p.a.w_row_stride : p.a.n;
+                float* const out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + (long long)w.unit * p.a.k * p.a.n) + feature;
+                const int row0 = w.row0 + half * kCols;
+                if (feature < p.a.n) {
+#pragma unroll
+                    for (int j = 0; j < kCols; ++j) {
+                        if (row0 + j >= p.a.k) break;
+                        float* const at = out + (row0 + j) * stride;
+                        *at = direct && p.a.accumulate ? *at + sum[j] : sum[j];
+                    }
+                }
+            } else {
+                T* const out = (T*)(MODE == kLinear ? p.a.y : p.a.x);
+                const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
+                alive = mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
+                if (!alive) break;
+                fence_after_sync();
+                // the halves take turns at blocks of 32 columns
+#pragma unroll 1
+                for (int j0 = half * 32; j0 < w.count; j0 += 64) {
+                    float v[32];
+                    tmem_load_32(tmem + lanes + acc * TN + j0, v);
+                    const int row = row_at(p, w.first + j0 + lane, w.first + w.count);
+                    if (p.wide_store) {
+                        // a lane and its neighbour exchange a value, so that each holds two features of one row
+                        const int odd = lane & 1;
+                        T* const at = out + (feature - odd);
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+                            const int r0 = __shfl_sync(0xffffffffu, row, j), r1 = __shfl_sync(0xffffffffu, row, j + 1);
+                            const int r = odd ? r1 : r0;
+                            const T two[2] = {from_float<T>(odd ? got : v[j]), from_float<T>(odd ? v[j + 1] : got)};
+                            if (r < p.a.rows && feature - odd < width)
+                                *reinterpret_cast<uint32_t*>(at + r * stride) = *reinterpret_cast<const uint32_t*>(two);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const int r = __shfl_sync(0xffffffffu, row, j);
+                            if (r < p.a.rows && feature < width) out[r * stride + feature] = from_float<T>(v[j]);
+                        }
+                    }
+                }
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty(acc));
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1;
+            }
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 0) {
+        fence_after_sync();
+        if (*abort_flag) {
+            // a wait ran out: what was requested lands before the CTA gives its memory back
+            for (int i = 0; i < 20000; ++i) __nanosleep(1000);
+            if (lane == 0 && p.a.status) atomicOr(p.a.status, FMB_STATUS_TENSOR_TIMEOUT);
+        }
+        __syncwarp();
+        tmem_free(tmem, S::kTmem);
+    }
+}
+
+// sums of the units of every group that has more than one, in the order of its entries
+__global__ void __launch_bounds__(256)
+k_sum_units(fmb_grouped_t a, int unit_rows) {
+    const int g = blockIdx.y;
+    __shared__ int first[2];
+    if (threadIdx.x < 32) {
+        int before = 0;
+        for (int q = threadIdx.x; q < g; q += 32) {
+            int begin, end;
+            group_span(a.offsets, q, a.rows, begin, end);
+            before += end > begin ? (end - begin - 1) / unit_rows + 1 : 1;
+        }
+        before = warp_sum(before);
+        int begin, end;
+        group_span(a.offsets, g, a.rows, begin, end);
+        if (threadIdx.x == 0) {
+            first[0] = before;
+            first[1] = end > begin ? (end - begin - 1) / unit_rows + 1 : 1;
+        }
+    }
+    __syncthreads();
+    if (first[1] <= 1) return;
+    const long long size = (long long)a.k * a.n, i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= size) return;
+    const float* at = a.scratch + first[0] * size + i;
+    float sum = 0.0f;
+    for (int u = 0; u < first[1]; ++u, at += size) sum += *at;
+    float* const out = (float*)a.w + g * a.w_group_stride + (i / a.n) * a.w_row_stride + i % a.n;
+    *out = a.accumulate ? *out + sum : sum;
+}
+
+typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                           const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                           CUtensorMapFloatOOBfill);
+
+Encode encoder() {
+    static Encode found = [] {
+        void* fn = nullptr;
+        cudaDriverEntryPointQueryResult result;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &result) != cudaSuccess ||
+            result != cudaDriverEntryPointSuccess)
+            fn = nullptr;
+        return (Encode)fn;
+    }();
+    return found;
+}
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// [groups][rows][columns] with the strides given, in boxes of 1 x box_rows x 64
+bool encode_map(CUtensorMap* map, int type, const void* base, int columns, int rows, int groups, long long row_stride,
+                long long group_stride, int box_rows, int dims) {
+    const Encode encode = encoder();
+    if (!encode || !aligned16(base)) return false;
+    if (rows == 1) row_stride = std::max<long long>(row_stride, (columns + 7) / 8 * 8);     // never used
+    if (groups == 1) group_stride = 8;
+    if (row_stride <= 0 || row_stride % 8 || row_stride >= (1ll << 38)) return false;
+    if (dims == 3 && (group_stride <= 0 || group_stride % 8 || group_stride >= (1ll << 38))) return false;
+    const cuuint64_t size[3] = {(cuuint64_t)columns, (cuuint64_t)rows, (cuuint64_t)groups};
+    const cuuint64_t stride[2] = {(cuuint64_t)row_stride * 2, (cuuint64_t)group_stride * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    return encode(map, type == FMB_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims,
+                  const_cast<void*>(base), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 1;
+    return sms;
+}
+
+template <typename T, int MODE, int TN>
+int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, long long tiles, cudaStream_t stream) {
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN>, Shape<TN>::kSmem));
+    const int grid = (int)std::min<long long>(tiles, sm_count());
+    k_grouped_tc<T, MODE, TN><<<grid, kThreads, Shape<TN>::kSmem, stream>>>(p, features, rows);
+    FMB_LAUNCH_CHECK();
+    return FMB_OK;
+}
+
+// most units a launch can have
+long long most_units(const fmb_grouped_t* a, int unit_rows) { return (long long)a->rows / unit_rows + a->groups; }
+
+template <typename T, int MODE>
+int launch_rows(Args& p, const CUtensorMap& features, const CUtensorMap& rows, cudaStream_t stream) {
+    // the widest tile that still leaves a tile per SM, but none much wider than the groups are on average
+    const fmb_grouped_t* a = &p.a;
+    const int average = a->rows / a->groups;
+    int tn = 256;
+    while (tn > 32 && (tn > std::max(32, 2 * average) || most_units(a, tn) * p.feature_tiles < 148)) tn /= 2;
+    p.unit_rows = tn;
+    const long long tiles = most_units(a, tn) * p.feature_tiles;
+    if (tn == 256) return launch<T, MODE, 256>(p, features, rows, tiles, stream);
+    if (tn == 128) return launch<T, MODE, 128>(p, features, rows, tiles, stream);
+    if (tn == 64) return launch<T, MODE, 64>(p, features, rows, tiles, stream);
+    return launch<T, MODE, 32>(p, features, rows, tiles, stream);
+}
+
+// weight gradient: columns of a tile, and rows per unit -- all of a group's, or fewer where there are few tiles
+void weight_plan(const fmb_grouped_t* a, int& tn, int& unit_rows) {
+    tn = a->k > 128 ? 256 : 128;
+    const long long tiles = (long long)a->groups * ((a->n + 127) / 128) * ((a->k + tn - 1) / tn);
+    unit_rows = 1 << 30;
+    if (tiles < 2 * 148 && a->rows > 128) {
+        const long long wanted = (2 * 148 + tiles - 1) / tiles * a->groups;      // units in all
+        unit_rows = (int)std::max<long long>(128, (a->rows / wanted + 63) / 64 * 64);
+        if (unit_rows >= a->rows) unit_rows = 1 << 30;
+    }
+}
+
+template <typename T>
+int tma_typed(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
+    Args p;
+    p.a = *a;
+    p.row_tiles = 1;
+    CUtensorMap features, rows;
+    if (mode == kWeightGradient) {
+        int tn;
+        weight_plan(a, tn, p.unit_rows);
+        p.feature_tiles = ceil_div(a->n, 128);
+        p.row_tiles = ceil_div(a->k, tn);
+        p.wide_store = 0;
+        if (!encode_map(&features, a->type, a->y, a->n, a->rows, 1, a->y_stride, 0, 1, 2) ||
+            !encode_map(&rows, a->type, a->x, a->k, a->rows, 1, a->x_stride, 0, 1, 2))
+            return FMB_ERR_UNSUPPORTED;
+        const long long tiles = most_units(a, p.unit_rows) * p.feature_tiles * p.row_tiles;
+        FMB_REQUIRE(p.unit_rows >= a->rows || a->scratch, "fmb_grouped_weight_gradient: null scratch");
+        const int rc = tn == 256 ? launch<T, kWeightGradient, 256>(p, features, rows, tiles, stream)
+                                 : launch<T, kWeightGradient, 128>(p, features, rows, tiles, stream);
+        if (rc || p.unit_rows >= a->rows) return rc;
+        k_sum_units<<<dim3(ceil_div((long long)a->k * a->n, 256), a->groups), 256, 0, stream>>>(*a, p.unit_rows);
+        FMB_LAUNCH_CHECK();
+        return FMB_OK;
+    }
+    const bool forward = mode == kLinear;
+    const int width = forward ? a->n : a->k, depth = forward ? a->k : a->n;
+    const void* in = forward ? a->x : a->y;
+    const void* out = forward ? a->y : a->x;
+    const long long in_stride = forward ? a->x_stride : a->y_stride, out_stride = forward ? a->y_stride : a->x_stride;
+    p.feature_tiles = ceil_div(width, 128);
+    p.wide_store = ((uintptr_t)out & 3) == 0 && out_stride % 2 == 0 && width % 2 == 0;
+    if (!encode_map(&features, a->type, a->w, a->n, a->k, a->groups, a->w_row_stride, a->w_group_stride, forward ? 64 : 128, 3) ||
+        !encode_map(&rows, a->type, in, depth, a->rows, 1, in_stride, 0, 1, 2))
+        return FMB_ERR_UNSUPPORTED;
+    return forward ? launch_rows<T, kLinear>(p, features, rows, stream) : launch_rows<T, kInputGradient>(p, features, rows, stream);
+}
+
+}  // namespace
+
+int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
+    if (a->type == FMB_TYPE_BF16) return tma_typed<__nv_bfloat16>(a, mode, stream);
+    if (a->type == FMB_TYPE_F16) return tma_typed<__half>(a, mode, stream);
+    return FMB_ERR_UNSUPPORTED;
+}
+
+long long scratch_floats(const fmb_grouped_t* a) {
+    if (a->type == FMB_TYPE_F32) return 0;
+    int tn, unit_rows;
+    weight_plan(a, tn, unit_rows);
+    return unit_rows >= a->rows ? 0 : most_units(a, unit_rows) * a->k * a->n;
+}
+
+}  // namespace grp
+}  // namespace fmb
