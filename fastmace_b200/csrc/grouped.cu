@@ -1,121 +1,49 @@
-// Products of a grouped linear and its gradients: one matrix per group of rows (fmb_grouped_linear and the calls beside it).
+// Entry points of the grouped products (fmb_grouped_linear and the calls beside it): checks, and which kernel runs.
+//
+// 16-bit operands whose rows start at multiples of 16 bytes go by TMA (grouped_tc.cu); threads bring the others
+// (grouped_split.cu): fp32, which has to be split into bf16 parts on its way, and odd sizes.
 
 #include "grouped.cuh"
 
+#include <algorithm>
+
 namespace fmb {
+namespace grp {
 
 namespace {
 
-using namespace grp;
-
-constexpr int kT = 64, kK = 16, kThreads = 256;
-
-// out[r] = in[r] W[g] (or W[g]^T): a CTA takes 64 rows of a group and 64 columns
-template <typename T, bool TRANSPOSED>
-__global__ void __launch_bounds__(kThreads)
-k_grouped_rows(fmb_grouped_t a) {
-    __shared__ float sx[kK][kT + 4], sw[kK][kT + 4];
-    __shared__ int32_t row_of[kT];
-    const int depth = TRANSPOSED ? a.n : a.k, width = TRANSPOSED ? a.k : a.n;
-    const T* const in = (const T*)(TRANSPOSED ? a.y : a.x);
-    T* const out = (T*)(TRANSPOSED ? a.x : a.y);
-    const long long in_stride = TRANSPOSED ? a.y_stride : a.x_stride, out_stride = TRANSPOSED ? a.x_stride : a.y_stride;
-    int unit = blockIdx.x, g = 0, begin = 0, end = 0;
-    for (; g <= a.groups; ++g) {
-        if (g == a.groups) {
-            begin = min(max(a.offsets[g], 0), a.rows);
-            end = a.zero_rest ? a.rows : begin;
-        } else {
-            group_span(a.offsets, g, a.rows, begin, end);
+// sums of the units of every group that has more than one, in the order of its entries
+__global__ void __launch_bounds__(256)
+k_sum_units(fmb_grouped_t a, int unit_rows) {
+    const int g = blockIdx.y;
+    __shared__ int first[2];
+    if (threadIdx.x < 32) {
+        int before = 0;
+        for (int q = threadIdx.x; q < g; q += 32) {
+            int begin, end;
+            group_span(a.offsets, q, a.rows, begin, end);
+            before += end > begin ? (end - begin - 1) / unit_rows + 1 : 1;
         }
-        const int units = (end - begin + kT - 1) / kT;
-        if (unit < units) break;
-        unit -= units;
-    }
-    if (g > a.groups) return;
-    const int first = begin + unit * kT, col0 = blockIdx.y * kT;
-    if (threadIdx.x < kT) {
-        const int at = first + threadIdx.x;
-        int row = at < end ? a.order[at] : -1;
-        if (row >= a.rows) row = -1;
-        row_of[threadIdx.x] = row;
+        before = warp_sum(before);
+        int begin, end;
+        group_span(a.offsets, g, a.rows, begin, end);
+        if (threadIdx.x == 0) {
+            first[0] = before;
+            first[1] = end > begin ? (end - begin - 1) / unit_rows + 1 : 1;
+        }
     }
     __syncthreads();
-    float acc[4][4] = {};
-    const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
-    if (g < a.groups) {
-        const T* const w = (const T*)a.w + (long long)g * a.w_group_stride;
-        for (int k0 = 0; k0 < depth; k0 += kK) {
-            for (int i = threadIdx.x; i < kT * kK; i += kThreads) {
-                const int r = i / kK, k = i % kK;
-                const int row = row_of[r];
-                sx[k][r] = row >= 0 && k0 + k < depth ? to_float(in[(long long)row * in_stride + k0 + k]) : 0.0f;
-                const int kk = TRANSPOSED ? i % kK : i / kT, c = TRANSPOSED ? i / kK : i % kT;
-                const bool live = k0 + kk < depth && col0 + c < width;
-                const long long at = TRANSPOSED ? (long long)(col0 + c) * a.w_row_stride + k0 + kk
-                                                : (long long)(k0 + kk) * a.w_row_stride + col0 + c;
-                sw[kk][c] = live ? to_float(w[at]) : 0.0f;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kK; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sx[k][tr * 4 + i], sw[k][tc + 16 * j], acc[i][j]);
-            __syncthreads();
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = row_of[tr * 4 + i];
-        if (row < 0) continue;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (col0 + tc + 16 * j < width) out[(long long)row * out_stride + col0 + tc + 16 * j] = from_float<T>(acc[i][j]);
-    }
+    if (first[1] <= 1) return;
+    const long long size = (long long)a.k * a.n, i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= size) return;
+    const float* at = a.scratch + first[0] * size + i;
+    float sum = 0.0f;
+    for (int u = 0; u < first[1]; ++u, at += size) sum += *at;
+    float* const out = (float*)a.w + g * a.w_group_stride + (i / a.n) * a.w_row_stride + i % a.n;
+    *out = a.accumulate ? *out + sum : sum;
 }
 
-// dW[g] (+)= sum x[r]^T y[r]: a CTA takes 64 x 64 of a group's matrix
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-k_grouped_weights(fmb_grouped_t a) {
-    __shared__ float sx[kK][kT + 4], sy[kK][kT + 4];
-    const int g = blockIdx.z, k0 = blockIdx.x * kT, n0 = blockIdx.y * kT;
-    int begin, end;
-    group_span(a.offsets, g, a.rows, begin, end);
-    float acc[4][4] = {};
-    const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
-    for (int r0 = begin; r0 < end; r0 += kK) {
-        for (int i = threadIdx.x; i < kT * kK; i += kThreads) {
-            const int r = i / kT, c = i % kT;
-            int row = r0 + r < end ? a.order[r0 + r] : -1;
-            if (row >= a.rows) row = -1;
-            sx[r][c] = row >= 0 && k0 + c < a.k ? to_float(((const T*)a.x)[(long long)row * a.x_stride + k0 + c]) : 0.0f;
-            sy[r][c] = row >= 0 && n0 + c < a.n ? to_float(((const T*)a.y)[(long long)row * a.y_stride + n0 + c]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < kK; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sx[r][tr * 4 + i], sy[r][tc + 16 * j], acc[i][j]);
-        __syncthreads();
-    }
-    float* const w = (float*)a.w + (long long)g * a.w_group_stride;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int k = k0 + tr * 4 + i, n = n0 + tc + 16 * j;
-            if (k >= a.k || n >= a.n) continue;
-            float* const at = w + (long long)k * a.w_row_stride + n;
-            *at = a.accumulate ? *at + acc[i][j] : acc[i][j];
-        }
-}
-
-int check(const fmb_grouped_t* a, int wide_in, int wide_out) {
+int check(const fmb_grouped_t* a) {
     FMB_REQUIRE(a, "grouped product: null argument");
     FMB_REQUIRE(a->type >= FMB_TYPE_F32 && a->type <= FMB_TYPE_F16, "grouped product: type");
     FMB_REQUIRE(a->groups >= 1 && a->groups <= FMB_MAX_GROUPS, "grouped product: 1 to FMB_MAX_GROUPS groups");
@@ -125,56 +53,52 @@ int check(const fmb_grouped_t* a, int wide_in, int wide_out) {
     FMB_REQUIRE(a->offsets && a->w, "grouped product: null argument");
     FMB_REQUIRE(a->rows == 0 || (a->order && a->x && a->y), "grouped product: null argument");
     FMB_REQUIRE(a->rows <= 1 || (a->x_stride >= a->k && a->y_stride >= a->n), "grouped product: rows overlap");
-    (void)wide_in;
-    (void)wide_out;
     return FMB_OK;
 }
 
-template <bool TRANSPOSED>
-int rows_launch(const fmb_grouped_t* a, cudaStream_t stream) {
-    const int rc = check(a, 0, 0);
+int run(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
+    const int rc = check(a);
     if (rc) return rc;
-    if (a->rows == 0) return FMB_OK;
-    const int by_tma = tma_launch(a, TRANSPOSED ? kInputGradient : kLinear, stream);
-    if (by_tma != FMB_ERR_UNSUPPORTED) return by_tma;
-    const dim3 grid(ceil_div(a->rows, kT) + a->groups + 1, ceil_div(TRANSPOSED ? a->k : a->n, kT));
-    if (a->type == FMB_TYPE_F32) k_grouped_rows<float, TRANSPOSED><<<grid, kThreads, 0, stream>>>(*a);
-    else if (a->type == FMB_TYPE_BF16) k_grouped_rows<__nv_bfloat16, TRANSPOSED><<<grid, kThreads, 0, stream>>>(*a);
-    else k_grouped_rows<__half, TRANSPOSED><<<grid, kThreads, 0, stream>>>(*a);
-    FMB_LAUNCH_CHECK();
-    return FMB_OK;
+    if (a->rows == 0 && mode != kWeightGradient) return FMB_OK;
+    const int by_tma = tma_launch(a, mode, stream);
+    return by_tma != FMB_ERR_UNSUPPORTED ? by_tma : split_launch(a, mode, stream);
 }
 
 }  // namespace
 
+int sum_units(const fmb_grouped_t* a, int unit_rows, cudaStream_t stream) {
+    k_sum_units<<<dim3(ceil_div((long long)a->k * a->n, 256), a->groups), 256, 0, stream>>>(*a, unit_rows);
+    FMB_LAUNCH_CHECK();
+    return FMB_OK;
+}
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 1;
+    return sms;
+}
+
+}  // namespace grp
 }  // namespace fmb
 
 using namespace fmb;
+using namespace fmb::grp;
 
-extern "C" FMB_API int fmb_grouped_linear(const fmb_grouped_t* a, fmb_stream_t stream) {
-    return rows_launch<false>(a, (cudaStream_t)stream);
-}
+extern "C" FMB_API int fmb_grouped_linear(const fmb_grouped_t* a, fmb_stream_t stream) { return run(a, kLinear, (cudaStream_t)stream); }
 
 extern "C" FMB_API int fmb_grouped_input_gradient(const fmb_grouped_t* a, fmb_stream_t stream) {
-    return rows_launch<true>(a, (cudaStream_t)stream);
+    return run(a, kInputGradient, (cudaStream_t)stream);
+}
+
+extern "C" FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* a, fmb_stream_t stream) {
+    return run(a, kWeightGradient, (cudaStream_t)stream);
 }
 
 extern "C" FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* a) {
-    return a && a->groups >= 1 && a->k >= 1 && a->n >= 1 ? scratch_floats(a) : 0;
-}
-
-extern "C" FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* a, fmb_stream_t stream_) {
-    const int rc = check(a, 0, 0);
-    if (rc) return rc;
-    cudaStream_t stream = (cudaStream_t)stream_;
-    if (a->rows) {
-        const int by_tma = tma_launch(a, kWeightGradient, stream);
-        if (by_tma != FMB_ERR_UNSUPPORTED) return by_tma;
-    }
-    const dim3 grid(ceil_div(a->k, kT), ceil_div(a->n, kT), a->groups);
-    if (a->type == FMB_TYPE_F32) k_grouped_weights<float><<<grid, kThreads, 0, stream>>>(*a);
-    else if (a->type == FMB_TYPE_BF16) k_grouped_weights<__nv_bfloat16><<<grid, kThreads, 0, stream>>>(*a);
-    else k_grouped_weights<__half><<<grid, kThreads, 0, stream>>>(*a);
-    FMB_LAUNCH_CHECK();
-    return FMB_OK;
+    if (!a || a->groups < 1 || a->k < 1 || a->n < 1 || a->rows < 1) return 0;
+    // whichever kernel the pointers' alignment selects
+    long long most = 0;
+    for (int unit_rows : {tma_unit_rows(a), split_unit_rows(a)})
+        if (unit_rows < a->rows) most = std::max(most, most_units(a, unit_rows) * a->k * a->n);
+    return most;
 }

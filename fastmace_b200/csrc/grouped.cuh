@@ -67,8 +67,16 @@ enum Mode { kLinear = 0, kInputGradient = 1, kWeightGradient = 2 };
 
 // tcgen05 kernels with operands by TMA (grouped_tc.cu): FMB_ERR_UNSUPPORTED for types and alignments that TMA does not take
 int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
-// floats of scratch of the weight gradient
-long long scratch_floats(const fmb_grouped_t* a);
+// tcgen05 kernels whose threads bring the operands (grouped_split.cu): fp32, and every alignment
+int split_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
+
+// weight gradient: rows per unit of either kernel (2^30 where units are whole groups), the most units there can be, and the sum
+// over the units of the groups that have several
+int tma_unit_rows(const fmb_grouped_t* a);
+int split_unit_rows(const fmb_grouped_t* a);
+inline long long most_units(const fmb_grouped_t* a, int unit_rows) { return (long long)a->rows / unit_rows + a->groups; }
+int sum_units(const fmb_grouped_t* a, int unit_rows, cudaStream_t stream);
+int sm_count();
 
 }  // namespace grp
 }  // namespace fmb

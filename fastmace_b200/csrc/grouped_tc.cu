@@ -418,37 +418,6 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     }
 }
 
-// sums of the units of every group that has more than one, in the order of its entries
-__global__ void __launch_bounds__(256)
-k_sum_units(fmb_grouped_t a, int unit_rows) {
-    const int g = blockIdx.y;
-    __shared__ int first[2];
-    if (threadIdx.x < 32) {
-        int before = 0;
-        for (int q = threadIdx.x; q < g; q += 32) {
-            int begin, end;
-            group_span(a.offsets, q, a.rows, begin, end);
-            before += end > begin ? (end - begin - 1) / unit_rows + 1 : 1;
-        }
-        before = warp_sum(before);
-        int begin, end;
-        group_span(a.offsets, g, a.rows, begin, end);
-        if (threadIdx.x == 0) {
-            first[0] = before;
-            first[1] = end > begin ? (end - begin - 1) / unit_rows + 1 : 1;
-        }
-    }
-    __syncthreads();
-    if (first[1] <= 1) return;
-    const long long size = (long long)a.k * a.n, i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= size) return;
-    const float* at = a.scratch + first[0] * size + i;
-    float sum = 0.0f;
-    for (int u = 0; u < first[1]; ++u, at += size) sum += *at;
-    float* const out = (float*)a.w + g * a.w_group_stride + (i / a.n) * a.w_row_stride + i % a.n;
-    *out = a.accumulate ? *out + sum : sum;
-}
-
 typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                            const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
                            CUtensorMapFloatOOBfill);
@@ -484,12 +453,6 @@ bool encode_map(CUtensorMap* map, int type, const void* base, int columns, int r
                   CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int sm_count() {
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 1;
-    return sms;
-}
-
 template <typename T, int MODE, int TN>
 int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, long long tiles, cudaStream_t stream) {
     FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN>, Shape<TN>::kSmem));
@@ -498,9 +461,6 @@ int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, 
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
-
-// most units a launch can have
-long long most_units(const fmb_grouped_t* a, int unit_rows) { return (long long)a->rows / unit_rows + a->groups; }
 
 template <typename T, int MODE>
 int launch_rows(Args& p, const CUtensorMap& features, const CUtensorMap& rows, cudaStream_t stream) {
@@ -529,56 +489,54 @@ void weight_plan(const fmb_grouped_t* a, int& tn, int& unit_rows) {
     }
 }
 
+bool maps(const fmb_grouped_t* a, Mode mode, CUtensorMap* features, CUtensorMap* rows) {
+    if (a->type == FMB_TYPE_F32 || a->rows == 0) return false;
+    if (mode == kWeightGradient)
+        return encode_map(features, a->type, a->y, a->n, a->rows, 1, a->y_stride, 0, 1, 2) &&
+               encode_map(rows, a->type, a->x, a->k, a->rows, 1, a->x_stride, 0, 1, 2);
+    const bool forward = mode == kLinear;
+    return encode_map(features, a->type, a->w, a->n, a->k, a->groups, a->w_row_stride, a->w_group_stride, forward ? 64 : 128, 3) &&
+           encode_map(rows, a->type, forward ? a->x : a->y, forward ? a->k : a->n, a->rows, 1, forward ? a->x_stride : a->y_stride, 0, 1, 2);
+}
+
 template <typename T>
-int tma_typed(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
+int tma_typed(const fmb_grouped_t* a, Mode mode, const CUtensorMap& features, const CUtensorMap& rows, cudaStream_t stream) {
     Args p;
     p.a = *a;
     p.row_tiles = 1;
-    CUtensorMap features, rows;
+    p.wide_store = 0;
     if (mode == kWeightGradient) {
         int tn;
         weight_plan(a, tn, p.unit_rows);
         p.feature_tiles = ceil_div(a->n, 128);
         p.row_tiles = ceil_div(a->k, tn);
-        p.wide_store = 0;
-        if (!encode_map(&features, a->type, a->y, a->n, a->rows, 1, a->y_stride, 0, 1, 2) ||
-            !encode_map(&rows, a->type, a->x, a->k, a->rows, 1, a->x_stride, 0, 1, 2))
-            return FMB_ERR_UNSUPPORTED;
         const long long tiles = most_units(a, p.unit_rows) * p.feature_tiles * p.row_tiles;
         FMB_REQUIRE(p.unit_rows >= a->rows || a->scratch, "fmb_grouped_weight_gradient: null scratch");
         const int rc = tn == 256 ? launch<T, kWeightGradient, 256>(p, features, rows, tiles, stream)
                                  : launch<T, kWeightGradient, 128>(p, features, rows, tiles, stream);
-        if (rc || p.unit_rows >= a->rows) return rc;
-        k_sum_units<<<dim3(ceil_div((long long)a->k * a->n, 256), a->groups), 256, 0, stream>>>(*a, p.unit_rows);
-        FMB_LAUNCH_CHECK();
-        return FMB_OK;
+        return rc || p.unit_rows >= a->rows ? rc : sum_units(a, p.unit_rows, stream);
     }
     const bool forward = mode == kLinear;
-    const int width = forward ? a->n : a->k, depth = forward ? a->k : a->n;
-    const void* in = forward ? a->x : a->y;
+    const int width = forward ? a->n : a->k;
     const void* out = forward ? a->y : a->x;
-    const long long in_stride = forward ? a->x_stride : a->y_stride, out_stride = forward ? a->y_stride : a->x_stride;
     p.feature_tiles = ceil_div(width, 128);
-    p.wide_store = ((uintptr_t)out & 3) == 0 && out_stride % 2 == 0 && width % 2 == 0;
-    if (!encode_map(&features, a->type, a->w, a->n, a->k, a->groups, a->w_row_stride, a->w_group_stride, forward ? 64 : 128, 3) ||
-        !encode_map(&rows, a->type, in, depth, a->rows, 1, in_stride, 0, 1, 2))
-        return FMB_ERR_UNSUPPORTED;
+    p.wide_store = ((uintptr_t)out & 3) == 0 && (forward ? a->y_stride : a->x_stride) % 2 == 0 && width % 2 == 0;
     return forward ? launch_rows<T, kLinear>(p, features, rows, stream) : launch_rows<T, kInputGradient>(p, features, rows, stream);
 }
 
 }  // namespace
 
-int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
-    if (a->type == FMB_TYPE_BF16) return tma_typed<__nv_bfloat16>(a, mode, stream);
-    if (a->type == FMB_TYPE_F16) return tma_typed<__half>(a, mode, stream);
-    return FMB_ERR_UNSUPPORTED;
-}
-
-long long scratch_floats(const fmb_grouped_t* a) {
-    if (a->type == FMB_TYPE_F32) return 0;
+int tma_unit_rows(const fmb_grouped_t* a) {
     int tn, unit_rows;
     weight_plan(a, tn, unit_rows);
-    return unit_rows >= a->rows ? 0 : most_units(a, unit_rows) * a->k * a->n;
+    return unit_rows;
+}
+
+int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
+    CUtensorMap features, rows;
+    if (!maps(a, mode, &features, &rows)) return FMB_ERR_UNSUPPORTED;
+    return a->type == FMB_TYPE_BF16 ? tma_typed<__nv_bfloat16>(a, mode, features, rows, stream)
+                                    : tma_typed<__half>(a, mode, features, rows, stream);
 }
 
 }  // namespace grp

@@ -37,43 +37,52 @@ class RowGroups(NamedTuple):
     offsets: torch.Tensor
 
 
-_status: dict[torch.device, torch.Tensor] = {}
+_status: dict[int, torch.Tensor] = {}         # a status word per device, read by check_status
 
 
-def _status_of(device: torch.device) -> torch.Tensor:
-    if device not in _status:
+def _status_pointer(index: int) -> int:
+    word = _status.get(index)
+    if word is None:
         if torch.cuda.is_current_stream_capturing():
-            raise _lib.Fmb200Error("call grouped.prepare_device() before capturing the first grouped product")
-        _status[device] = torch.zeros((), dtype=torch.int32, device=device)
-        torch.cuda.current_stream(device).synchronize()       # other streams may use it from here on
-    return _status[device]
+            raise _lib.Fmb200Error("call grouped.prepare_device() before capturing the first grouped product of a device")
+        word = torch.zeros((), dtype=torch.int32, device=torch.device("cuda", index))
+        torch.cuda.current_stream(word.device).synchronize()       # other streams may use it from here on
+        _status[index] = word
+    return word.data_ptr()
+
+
+def _index(device) -> int:
+    device = torch.device(device)
+    return device.index if device.index is not None else torch.cuda.current_device()
 
 
 def prepare_device(device="cuda") -> None:
-    """Makes the device's status word; needed only where the first call on a device would be a captured one."""
-    device = torch.device(device)
-    _status_of(device if device.index is not None else torch.device("cuda", torch.cuda.current_device()))
+    """Makes the device's status word; needed only where the first product on a device would be a captured one."""
+    _status_pointer(_index(device))
 
 
 def check_status(device="cuda") -> None:
     """Raises if a grouped product on ``device`` gave up waiting since the last check (synchronises)."""
-    device = torch.device(device)
-    if device.index is None:
-        device = torch.device("cuda", torch.cuda.current_device())
-    word = _status.get(device)
+    word = _status.get(_index(device))
     if word is not None and int(word.item()) & _lib.STATUS_TENSOR_TIMEOUT:
         word.zero_()
         raise _lib.Fmb200Error("a tensor-core kernel gave up waiting (FMB_STATUS_TENSOR_TIMEOUT)")
 
 
-def _on_device(what: str, *tensors: torch.Tensor) -> torch.device:
-    device = tensors[0].device
+def _on_device(what: str, *tensors: torch.Tensor) -> int:
+    index = tensors[0].get_device()
     for t in tensors:
-        if not t.is_cuda:
-            raise ValueError(f"{what}: the operands must be CUDA tensors, there is no CPU path")
-        if t.device != device:
-            raise ValueError(f"{what}: the operands are on different devices")
-    return device
+        if t.get_device() != index or index < 0:
+            raise ValueError(f"{what}: the operands must be CUDA tensors on one device, there is no CPU path")
+    return index
+
+
+def _launch(index: int, call, *arguments):
+    """``call(*arguments, stream)`` with the device current and its current stream."""
+    if torch.cuda.current_device() == index:
+        return call(*arguments, torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(index):
+        return call(*arguments, torch.cuda.current_stream().cuda_stream)
 
 
 def group_rows(keys: torch.Tensor, n_groups: int) -> RowGroups:
@@ -83,91 +92,80 @@ def group_rows(keys: torch.Tensor, n_groups: int) -> RowGroups:
         raise ValueError("group_rows: keys must be one int32 or int64 per row")
     if not 1 <= int(n_groups) <= MAX_GROUPS:
         raise ValueError(f"group_rows: 1 to {MAX_GROUPS} groups")
-    device = _on_device("group_rows", keys)
+    index = _on_device("group_rows", keys)
     if keys.shape[0] > 1 and keys.stride(0) != 1:
         keys = keys.contiguous()
-    rows = keys.shape[0]
-    lib = _lib.load()
-    with torch.cuda.device(device):
-        out = RowGroups(torch.empty(rows, dtype=torch.int32, device=device),
-                        torch.empty(int(n_groups) + 1, dtype=torch.int32, device=device))
-        need = lib.fmb_group_rows_scratch(rows, int(n_groups))
-        scratch = torch.empty(need, dtype=torch.int32, device=device) if need else None
-        _lib.check(lib.fmb_group_rows(keys.data_ptr(), keys.element_size(), rows, int(n_groups), out.rows.data_ptr(),
-                                      out.offsets.data_ptr(), scratch.data_ptr() if need else None, _lib.current_stream()),
-                   "fmb_group_rows")
+    rows, lib, device = keys.shape[0], _lib.load(), keys.device
+    out = RowGroups(torch.empty(rows, dtype=torch.int32, device=device),
+                    torch.empty(int(n_groups) + 1, dtype=torch.int32, device=device))
+    need = lib.fmb_group_rows_scratch(rows, int(n_groups))
+    scratch = torch.empty(need, dtype=torch.int32, device=device) if need else None
+    _lib.check(_launch(index, lib.fmb_group_rows, keys.data_ptr(), keys.element_size(), rows, int(n_groups), out.rows.data_ptr(),
+                       out.offsets.data_ptr(), scratch.data_ptr() if need else None), "fmb_group_rows")
     return out
 
 
-def _matrix(what: str, name: str, t: torch.Tensor, shape: tuple | None = None) -> torch.Tensor:
-    if t.dim() != 2 or (shape is not None and tuple(t.shape) != shape):
-        raise ValueError(f"{what}: {name} must be {shape if shape else 'a matrix'}, got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+def _matrix(what: str, name: str, t: torch.Tensor, columns: int | None = None, rows: int | None = None):
+    """(rows, columns, row stride) of a matrix with contiguous rows."""
+    if t.dim() != 2:
+        raise ValueError(f"{what}: {name} must be a matrix, got {tuple(t.shape)}")
+    (m, n), (far, near) = t.shape, t.stride()
+    if (columns is not None and n != columns) or (rows is not None and m != rows):
+        raise ValueError(f"{what}: {name} is {m} x {n}, expected {m if rows is None else rows} x {n if columns is None else columns}")
+    if n < 1:
+        raise ValueError(f"{what}: {name} has empty rows")
+    if (n > 1 and near != 1) or (m > 1 and far < n):
         raise ValueError(f"{what}: {name} must have contiguous rows that do not overlap")
-    return t
+    return m, n, far if m > 1 else n
 
 
-def _weights(what: str, name: str, t: torch.Tensor) -> torch.Tensor:
+def _weights(what: str, name: str, t: torch.Tensor):
+    """(groups, k, n, group stride, row stride) of the matrices of all groups."""
     if t.dim() != 3:
         raise ValueError(f"{what}: {name} must be [groups, k, n], got {tuple(t.shape)}")
-    if t.shape[2] > 1 and t.stride(2) != 1:
+    (g, k, n), (between, far, near) = t.shape, t.stride()
+    if n > 1 and near != 1:
         raise ValueError(f"{what}: the columns of {name} must be contiguous")
-    return t
+    return g, k, n, between, far
 
 
-def _groups(what: str, groups: RowGroups, rows: int, n_groups: int | None) -> int:
+def _groups(what: str, groups: RowGroups, rows: int, n_groups: int | None = None) -> int:
     order, offsets = groups
-    for t in (order, offsets):
-        if t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous():
-            raise ValueError(f"{what}: groups must be as group_rows returns them")
-    if order.shape[0] != rows:
-        raise ValueError(f"{what}: groups of {order.shape[0]} rows for {rows} rows")
+    if order.dtype != torch.int32 or offsets.dtype != torch.int32 or order.dim() != 1 or offsets.dim() != 1 or \
+            not order.is_contiguous() or not offsets.is_contiguous():
+        raise ValueError(f"{what}: groups must be as group_rows returns them")
     count = offsets.shape[0] - 1
-    if not 1 <= count <= MAX_GROUPS:
-        raise ValueError(f"{what}: 1 to {MAX_GROUPS} groups")
-    if n_groups is not None and count != n_groups:
-        raise ValueError(f"{what}: {count} groups for {n_groups} matrices")
+    if order.shape[0] != rows or not 1 <= count <= MAX_GROUPS or (n_groups is not None and count != n_groups):
+        raise ValueError(f"{what}: {count} groups of {order.shape[0]} rows, expected {n_groups or f'1 to {MAX_GROUPS}'} of {rows}")
     return count
 
 
-def _struct(groups: RowGroups, x, y, w, device) -> _lib.GroupedStruct:
-    a = _lib.GroupedStruct()
-    a.type = TYPES[x.dtype]
-    a.groups, a.rows, a.k, a.n = groups.offsets.shape[0] - 1, x.shape[0], x.shape[1], y.shape[1]
-    a.order, a.offsets = groups.rows.data_ptr(), groups.offsets.data_ptr()
-    a.x, a.y, a.w = x.data_ptr(), y.data_ptr(), w.data_ptr()
-    a.x_stride, a.y_stride = max(x.stride(0), x.shape[1]), max(y.stride(0), y.shape[1])
-    a.w_group_stride, a.w_row_stride = w.stride(0), w.stride(1)
-    a.status = _status_of(device).data_ptr()
-    return a
-
-
 def _rows_product(what: str, entry: str, source, weight, groups, out, transposed: bool):
-    _matrix(what, "the input", source)
-    _weights(what, "weight", weight)
-    if source.dtype not in TYPES or weight.dtype != source.dtype:
+    count, k, n, w_group, w_row = _weights(what, "weight", weight)
+    rows, width, stride = _matrix(what, "the input", source, n if transposed else k)
+    dtype = source.dtype
+    kind = TYPES.get(dtype)
+    if kind is None or weight.dtype != dtype:
         raise ValueError(f"{what}: input and weight must have the same type, float32, bfloat16 or float16")
-    wide_in, wide_out = (weight.shape[2], weight.shape[1]) if transposed else (weight.shape[1], weight.shape[2])
-    if source.shape[1] != wide_in:
-        raise ValueError(f"{what}: rows of {source.shape[1]} values for matrices that take {wide_in}")
-    if wide_in < 1 or wide_out < 1:
+    if k < 1 or n < 1:
         raise ValueError(f"{what}: empty matrices")
-    rows = source.shape[0]
-    _groups(what, groups, rows, weight.shape[0])
+    _groups(what, groups, rows, count)
+    index = _on_device(what, source, weight, *groups)
+    wide_out = k if transposed else n
     given = out is not None
-    device = _on_device(what, source, weight, *groups, *((out,) if given else ()))
     if given:
-        _matrix(what, "out", out, (rows, wide_out))
-        if out.dtype != source.dtype:
+        out_stride = _matrix(what, "out", out, wide_out, rows)[2]
+        if out.dtype != dtype:
             raise ValueError(f"{what}: out must have the input's type")
-    with torch.cuda.device(device):
-        if not given:
-            out = torch.empty(rows, wide_out, dtype=source.dtype, device=device)
-        if rows:
-            x, y = (out, source) if transposed else (source, out)
-            a = _struct(groups, x, y, weight, device)
-            a.zero_rest = int(not given)
-            _lib.check(getattr(_lib.load(), entry)(ctypes.byref(a), _lib.current_stream()), entry)
+        _on_device(what, source, out)
+    else:
+        out, out_stride = source.new_empty((rows, wide_out)), wide_out
+    if rows:
+        lib, here, there = _lib.load(), source.data_ptr(), out.data_ptr()
+        x, y, x_stride, y_stride = (there, here, out_stride, stride) if transposed else (here, there, stride, out_stride)
+        a = _lib.GroupedStruct(kind, count, rows, k, n, not given, 0, 0, groups[0].data_ptr(), groups[1].data_ptr(), x, y,
+                               weight.data_ptr(), x_stride, y_stride, w_row, w_group, None, _status_pointer(index))
+        _lib.check(_launch(index, getattr(lib, entry), ctypes.byref(a)), entry)
     return out
 
 
@@ -187,34 +185,30 @@ def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: Ro
     """``dW[g] = sum of x[r]^T dy[r]`` over the rows of g, float32 ``[groups, k, n]``; zero for a group without rows.
     ``accumulate=True`` adds to ``out``. The sums run in an order that depends on the sizes alone."""
     what = "grouped_linear_weight_gradient"
-    _matrix(what, "x", x)
-    _matrix(what, "dy", dy)
-    if x.dtype not in TYPES or dy.dtype != x.dtype:
+    rows, k, x_stride = _matrix(what, "x", x)
+    _, n, y_stride = _matrix(what, "dy", dy, rows=rows)
+    kind = TYPES.get(x.dtype)
+    if kind is None or dy.dtype != x.dtype:
         raise ValueError(f"{what}: x and dy must have the same type, float32, bfloat16 or float16")
-    if x.shape[0] != dy.shape[0]:
-        raise ValueError(f"{what}: {x.shape[0]} rows of x for {dy.shape[0]} of dy")
-    if x.shape[1] < 1 or dy.shape[1] < 1:
-        raise ValueError(f"{what}: empty rows")
-    count = _groups(what, groups, x.shape[0], None)
-    shape = (count, x.shape[1], dy.shape[1])
-    given = out is not None
-    if accumulate and not given:
-        raise ValueError(f"{what}: accumulate needs out")
-    device = _on_device(what, x, dy, *groups, *((out,) if given else ()))
-    if given:
-        _weights(what, "out", out)
-        if tuple(out.shape) != shape or out.dtype != torch.float32:
-            raise ValueError(f"{what}: out must be float32 {shape}")
-    with torch.cuda.device(device):
-        if not given:
-            out = torch.empty(shape, dtype=torch.float32, device=device)
-        lib = _lib.load()
-        a = _struct(groups, x, dy, out, device)
-        a.accumulate = int(bool(accumulate))
-        need = lib.fmb_grouped_scratch(ctypes.byref(a))
-        scratch = torch.empty(need, dtype=torch.float32, device=device) if need else None
-        a.scratch = scratch.data_ptr() if need else None
-        _lib.check(lib.fmb_grouped_weight_gradient(ctypes.byref(a), _lib.current_stream()), "fmb_grouped_weight_gradient")
+    count = _groups(what, groups, rows)
+    index = _on_device(what, x, dy, *groups)
+    if out is None:
+        if accumulate:
+            raise ValueError(f"{what}: accumulate needs out")
+        out = torch.empty((count, k, n), dtype=torch.float32, device=x.device)
+    elif out.dtype != torch.float32 or tuple(out.shape) != (count, k, n):
+        raise ValueError(f"{what}: out must be float32 {(count, k, n)}")
+    else:
+        _on_device(what, x, out)
+    _, _, _, w_group, w_row = _weights(what, "out", out)
+    lib = _lib.load()
+    a = _lib.GroupedStruct(kind, count, rows, k, n, 0, bool(accumulate), 0, groups[0].data_ptr(), groups[1].data_ptr(), x.data_ptr(),
+                           dy.data_ptr(), out.data_ptr(), x_stride, y_stride, w_row, w_group, None, _status_pointer(index))
+    need = lib.fmb_grouped_scratch(ctypes.byref(a))
+    if need:
+        scratch = torch.empty(need, dtype=torch.float32, device=x.device)
+        a.scratch = scratch.data_ptr()
+    _lib.check(_launch(index, lib.fmb_grouped_weight_gradient, ctypes.byref(a)), "fmb_grouped_weight_gradient")
     return out
 
 

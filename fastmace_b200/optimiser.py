@@ -24,10 +24,11 @@ from __future__ import annotations
 
 import ctypes
 
+import numpy as np
 import torch
 
 from . import _lib
-from .grouped import TYPES
+from .grouped import TYPES, _launch
 
 BLOCK = _lib.ADAMW_BLOCK
 
@@ -76,11 +77,14 @@ class AdamW:
             scale = lambda: torch.full((blocks,), 2.0 ** -126, device=self.device) if self.state_bits == 8 else None  # noqa: E731
             self.m_scale, self.v_scale = scale(), scale()
             self._state = torch.tensor([0.0, 1.0, 1.0, 0.0], dtype=torch.float64, device=self.device)
+        self._shapes, self._index = [p.shape for p in self.params], self.device.index
         self._tensors = (_lib.AdamwTensorStruct * len(self.params))()
         for k, p in enumerate(self.params):
             t = self._tensors[k]
             t.p, t.values, t.block = p.data_ptr(), p.numel(), self.blocks[k]
             t.copy = None if self.copies[k] is None else self.copies[k].data_ptr()
+        # the gradients' pointers of the list above, as one column
+        self._pointers = np.frombuffer(self._tensors, dtype=np.int64).reshape(len(self.params), -1)[:, 1]
         self._args = _lib.AdamwStruct()
 
     def _fill_args(self) -> None:
@@ -101,25 +105,25 @@ class AdamW:
             grads = [grads.get(k) for k in self.names]
         elif len(grads) != len(self.params):
             raise ValueError(f"AdamW.step: {len(grads)} gradients for {len(self.params)} tensors")
-        kind = None
-        for t, p, g in zip(self._tensors, self.params, grads):
-            if g is None:
-                t.g = None
-                continue
-            if g.dtype != kind:
-                if kind is not None or g.dtype not in TYPES:
-                    raise ValueError("AdamW.step: the gradients must have one type, float32, bfloat16 or float16")
-                kind = g.dtype
-            if g.shape != p.shape or not g.is_contiguous() or g.device != self.device:
-                raise ValueError("AdamW.step: a gradient must be contiguous, of its weights' shape and on their device")
-            t.g = g.data_ptr()
-        if kind is None:
-            return
+        shapes = self._shapes
+        if any(g is None for g in grads):
+            self._pointers[:] = [0 if g is None else g.data_ptr() for g in grads]
+            shapes = [s for s, g in zip(shapes, grads) if g is not None]
+            grads = [g for g in grads if g is not None]
+            if not grads:
+                return
+        else:
+            self._pointers[:] = [g.data_ptr() for g in grads]
+        kind = grads[0].dtype
+        if kind not in TYPES or any(g.dtype is not kind for g in grads):
+            raise ValueError("AdamW.step: the gradients must have one type, float32, bfloat16 or float16")
+        if [g.shape for g in grads] != shapes or not all([g.is_contiguous() for g in grads]) or \
+                any([g.get_device() != self._index for g in grads]):
+            raise ValueError("AdamW.step: a gradient must be contiguous, of its weights' shape and on their device")
         self._fill_args()
         self._args.grad_type = TYPES[kind]
-        with torch.cuda.device(self.device):
-            _lib.check(self.lib.fmb_adamw_step(ctypes.byref(self._args), self._tensors, len(self.params),
-                                               _lib.current_stream()), "fmb_adamw_step")
+        _lib.check(_launch(self._index, self.lib.fmb_adamw_step, ctypes.byref(self._args), self._tensors, len(self.params)),
+                   "fmb_adamw_step")
 
     @property
     def steps(self) -> int:
