@@ -57,11 +57,11 @@ int check(const fmb_grouped_t* a) {
 }
 
 int run(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
-    const int rc = check(a);
+    int rc = check(a);
     if (rc) return rc;
     if (a->rows == 0 && mode != kWeightGradient) return FMB_OK;
-    const int by_tma = tma_launch(a, mode, stream);
-    return by_tma != FMB_ERR_UNSUPPORTED ? by_tma : split_launch(a, mode, stream);
+    rc = a->type == FMB_TYPE_F32 ? resident_launch(a, mode, stream) : tma_launch(a, mode, stream);
+    return rc != FMB_ERR_UNSUPPORTED ? rc : split_launch(a, mode, stream);
 }
 
 }  // namespace

@@ -70,6 +70,15 @@ int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
 // tcgen05 kernels whose threads bring the operands (grouped_split.cu): fp32, and every alignment
 int split_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
 
+// tcgen05 kernel that keeps the split weights in tensor memory (grouped_resident.cu): FMB_ERR_UNSUPPORTED unless fp32, a depth of
+// at most 128 and rows that TMA takes
+int resident_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
+
+// rows that start at multiples of four values, so that they can be read four at a time
+inline bool four_at_a_time(const void* base, long long stride, int bytes) {
+    return ((uintptr_t)base & (uintptr_t)(4 * bytes - 1)) == 0 && stride % 4 == 0;
+}
+
 // weight gradient: rows per unit of either kernel (2^30 where units are whole groups), the most units there can be, and the sum
 // over the units of the groups that have several
 int tma_unit_rows(const fmb_grouped_t* a);

@@ -1,0 +1,328 @@
+// Grouped linear and its input gradient in fp32 for a depth of up to 128, the linears of a model of 128 channels: the
+// split weights of 128 features stay in tensor memory while a CTA goes through the rows of their group.
+//
+// The numbers and their six products are those of grouped_split.cu. What bounds the work here is memory, 8 bytes per row and
+// channel, so the SM's own paths are kept short of that:
+//   * rows come by TMA gather, 4 whole rows an instruction, into a ring of three tiles of 64 rows: 64 KB on their way while
+//     one is worked on (threads' own loads, 32 KB and waits in between, brought 2.2 TB/s);
+//   * eight warps split a tile into three K-major planes (48 KB, two of them);
+//   * the weights, as the MMAs' first operand in TMEM (three planes of 64 columns), take no shared-memory reads: a tile
+//     costs 96 KB of reads there instead of 192. Two accumulators, hi hi and the five others, twice (448 columns in all);
+//   * the result turns through shared memory, so that a store writes 512 bytes of a row. A lane that stored its own
+//     feature row by row took longer than everything else together.
+
+#include "grouped_tc.cuh"
+
+#include <algorithm>
+
+namespace fmb {
+namespace grp {
+
+namespace {
+
+using namespace tc;
+
+constexpr int kTN = 64, kK = 128;                          // rows of a tile, depth
+constexpr int kRaw = 3, kRawBytes = kTN * kK * 4;
+constexpr int kPlanes = 2, kPlaneTile = kTN * kDepth * 2, kPlaneBytes = 3 * 2 * kPlaneTile;      // [part][half of the depth]
+constexpr int kTurnBytes = 32 * 128 * 4;                   // half a tile of results
+constexpr int kPlane0 = kRaw * kRawBytes, kTurn0 = kPlane0 + kPlanes * kPlaneBytes, kUnits0 = kTurn0 + kTurnBytes;
+constexpr int kSmem = 1024 + kUnits0 + (FMB_MAX_GROUPS + 1) * 4 + 256;
+constexpr int kEpilogueWarps = 4, kSplitWarps = 8, kThreads = 32 * (4 + kEpilogueWarps + kSplitWarps);
+constexpr uint32_t kAccumulators = 192;                    // TMEM columns before them: the weights
+static_assert(kSmem <= 227 * 1024, "fits an SM");
+
+__device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t (&v)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 :: "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+}
+
+// this lane's feature of the tile's weights, split, into the TMEM columns of the three planes (two values a column)
+template <int MODE>
+__device__ __forceinline__ void bring_weights(const SplitArgs& p, const Tile& w, int feature, int depth, uint32_t tmem) {
+    const int width = MODE == kInputGradient ? p.a.k : p.a.n;
+    const float* const from = (const float*)p.a.w + w.g * p.a.w_group_stride + (MODE == kInputGradient ? feature * p.a.w_row_stride : feature);
+    const bool live = feature < width;
+#pragma unroll 1
+    for (int d0 = 0; d0 < depth; d0 += 16) {
+        float v[16];
+        if constexpr (MODE == kInputGradient) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+                const Quad<float> q = load_quad(from + d0 + i, live ? depth - d0 - i : 0, p.wide_features);
+                v[i] = q.v.x; v[i + 1] = q.v.y; v[i + 2] = q.v.z; v[i + 3] = q.v.w;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = live && d0 + i < depth ? __ldg(from + (d0 + i) * p.a.w_row_stride) : 0.0f;
+        }
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            uint32_t two[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) two[i] = upper_halves(v[2 * i], v[2 * i + 1]);
+            tmem_store_8(tmem + part * 64 + d0 / 2, two);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] = without_upper(v[i]);
+        }
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+template <int MODE>
+__global__ void __launch_bounds__(kThreads, 1)
+k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ CUtensorMap row_map, int wide_out) {
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    int* const first_unit = reinterpret_cast<int*>(smem + kUnits0);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + kUnits0 + ((FMB_MAX_GROUPS + 1) * 4 + 7) / 8 * 8);
+    uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kRaw + 2 * kPlanes + 5);
+    volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const uint32_t bar0 = smem_u32(bars);
+    auto raw_full = [&](int s) { return bar0 + 8u * s; };
+    auto raw_empty = [&](int s) { return bar0 + 8u * (kRaw + s); };
+    auto plane_full = [&](int s) { return bar0 + 8u * (2 * kRaw + s); };
+    auto plane_empty = [&](int s) { return bar0 + 8u * (2 * kRaw + kPlanes + s); };
+    auto acc_full = [&](int b) { return bar0 + 8u * (2 * kRaw + 2 * kPlanes + b); };
+    auto acc_empty = [&](int b) { return bar0 + 8u * (2 * kRaw + 2 * kPlanes + 2 + b); };
+    const uint32_t w_full = bar0 + 8u * (2 * kRaw + 2 * kPlanes + 4);
+    const int warp = uniform_warp(), lane = threadIdx.x & 31;
+
+    if (warp == 2) tmem_alloc(smem_u32(tmem_slot), 512);
+    if (warp == 1 && elect_one()) {
+        for (int s = 0; s < kRaw; ++s) {
+            mbar_init(raw_full(s), 1);
+            mbar_init(raw_empty(s), kSplitWarps);
+        }
+        for (int s = 0; s < kPlanes; ++s) {
+            mbar_init(plane_full(s), kSplitWarps);
+            mbar_init(plane_empty(s), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            mbar_init(acc_full(b), 1);
+            mbar_init(acc_empty(b), kEpilogueWarps);
+        }
+        mbar_init(w_full, kEpilogueWarps);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    count_units<kThreads>(p.a.offsets, p.a.groups, p.a.rows, kTN, 0, first_unit);
+    fence_before_sync();
+    __syncthreads();
+    fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const long long tiles = (long long)first_unit[p.a.groups] * p.feature_tiles;
+    const int t_begin = (int)(tiles * blockIdx.x / gridDim.x), t_end = (int)(tiles * (blockIdx.x + 1) / gridDim.x);
+    const int depth = MODE == kLinear ? p.a.k : p.a.n, width = MODE == kLinear ? p.a.n : p.a.k;
+    const int columns = depth <= 64 ? 64 : 128;              // of a row in the ring
+    bool alive = true;
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- rows
+        for (int t = t_begin, at = 0, phase = 0; t < t_end; ++t) {
+            const Tile w = locate(p, first_unit, t, kTN);
+            const int end = w.first + w.count, quads = (w.count + 3) / 4;
+            int rows[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = lane < 16 ? row_at(p, w.first + 4 * lane + i, end) : -1;
+                rows[i] = row < 0 ? p.a.rows : row;           // what is no row is filled with zeros
+            }
+            alive = mbar_wait(raw_empty(at), phase ^ 1, abort_flag, kSpin);
+            if (!alive) break;
+            const uint32_t dst = smem_u32(smem) + at * kRawBytes, bar = raw_full(at);
+            if (elect_one()) mbar_expect_tx(bar, quads * columns * 16);
+            __syncwarp();
+            for (int q = 0; q < quads; ++q) {
+                const int r0 = __shfl_sync(0xffffffffu, rows[0], q), r1 = __shfl_sync(0xffffffffu, rows[1], q);
+                const int r2 = __shfl_sync(0xffffffffu, rows[2], q), r3 = __shfl_sync(0xffffffffu, rows[3], q);
+                if (elect_one()) tma_gather4(dst + q * columns * 16, &row_map, 0, r0, r1, r2, r3, bar);
+                __syncwarp();
+            }
+            if (++at == kRaw) {
+                at = 0;
+                phase ^= 1;
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMAs
+        constexpr uint32_t kDesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+        int held_g = -1, held_f = -1;
+        uint32_t w_phase = 0;
+        const int steps = (depth + 15) / 16;
+        for (int t = t_begin, n = 0; t < t_end; ++t, ++n) {
+            const Tile w = locate(p, first_unit, t, kTN);
+            const int s = n & 1;
+            const uint32_t phase = (n >> 1) & 1;
+            if (w.g != held_g || w.feature0 != held_f) {
+                held_g = w.g;
+                held_f = w.feature0;
+                alive = mbar_wait(w_full, w_phase, abort_flag, kSpin);
+                w_phase ^= 1;
+            }
+            alive = alive && mbar_wait(acc_empty(s), phase ^ 1, abort_flag, kSpin);
+            alive = alive && mbar_wait(plane_full(s), phase, abort_flag, kSpin);
+            if (!alive) break;
+            fence_after_sync();
+            const uint64_t plane = make_desc(smem_u32(smem) + kPlane0 + s * kPlaneBytes);
+            const uint32_t main = tmem + kAccumulators + s * 2 * kTN, rest = main + kTN;
+            if (elect_one()) {
+                for (int k = 0; k < steps; ++k) {
+                    const uint64_t b = plane + (uint64_t)((k >> 2) * kPlaneTile + (k & 3) * 32) / 16;
+                    constexpr uint64_t kPart = 2 * kPlaneTile / 16;
+                    const uint32_t a = tmem + k * 8;
+                    mma_f16_ts(rest, a + 128, b, kDesc, k > 0);              // lo hi
+                    mma_f16_ts(rest, a + 64, b + kPart, kDesc, 1);           // mid mid
+                    mma_f16_ts(rest, a, b + 2 * kPart, kDesc, 1);            // hi lo
+                    mma_f16_ts(rest, a + 64, b, kDesc, 1);                   // mid hi
+                    mma_f16_ts(rest, a, b + kPart, kDesc, 1);                // hi mid
+                    mma_f16_ts(main, a, b, kDesc, k > 0);                    // hi hi
+                }
+                mma_commit(plane_empty(s));
+                mma_commit(acc_full(s));
+            }
+            __syncwarp();
+        }
+    } else if (warp >= 4 && warp < 4 + kEpilogueWarps) {
+        // ---------------------------------------------------------------- weights in, results out
+        const int quarter = warp & 3, id = quarter * 32 + lane;
+        float* const out = (float*)(MODE == kLinear ? p.a.y : p.a.x);
+        const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        float* const turn = reinterpret_cast<float*>(smem + kTurn0);                 // [32 rows][128 features]
+        if (p.a.zero_rest) {
+            const int from = min(max(p.a.offsets[p.a.groups], 0), p.a.rows);
+            for (int e = from + blockIdx.x * kEpilogueWarps + quarter; e < p.a.rows; e += gridDim.x * kEpilogueWarps) {
+                const int row = row_at(p, e, p.a.rows);
+                if (row >= 0)
+                    for (int c = lane; c < width; c += 32) out[row * stride + c] = 0.0f;
+            }
+        }
+        int held_g = -1, held_f = -1;
+        for (int t = t_begin, n = 0; t < t_end; ++t, ++n) {
+            const Tile w = locate(p, first_unit, t, kTN);
+            if (w.g != held_g || w.feature0 != held_f) {
+                // the accumulators of every tile before have been waited for: nobody reads the old weights
+                held_g = w.g;
+                held_f = w.feature0;
+                bring_weights<MODE>(p, w, w.feature0 + id, depth, tmem + lanes);
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(w_full);
+            }
+            const int s = n & 1;
+            const int row_low = row_at(p, w.first + lane, w.first + w.count), row_high = row_at(p, w.first + 32 + lane, w.first + w.count);
+            alive = mbar_wait(acc_full(s), (n >> 1) & 1, abort_flag, kSpin);
+            if (!alive) break;
+            fence_after_sync();
+            const uint32_t main = tmem + lanes + kAccumulators + s * 2 * kTN;
+#pragma unroll 1
+            for (int half = 0; half < 2; ++half) {
+                float v[32], u[32];
+                tmem_load_32(main + half * 32, v);
+                tmem_load_32(main + kTN + half * 32, u);
+                if (half == 1) {
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(acc_empty(s));
+                }
+                named_barrier(1, 128);                       // the half before has been read
+#pragma unroll
+                for (int j = 0; j < 32; ++j) turn[j * 128 + id] = v[j] + u[j];
+                named_barrier(1, 128);
+                const int mine = half ? row_high : row_low;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int at = quarter + 4 * j, row = __shfl_sync(0xffffffffu, mine, at);
+                    if (row < 0) continue;
+                    float* const to = out + row * stride + w.feature0;
+                    if (wide_out) {
+                        if (w.feature0 + 4 * lane < width)
+                            *reinterpret_cast<float4*>(to + 4 * lane) = *reinterpret_cast<const float4*>(turn + at * 128 + 4 * lane);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 128; c += 32)
+                            if (w.feature0 + c + lane < width) to[c + lane] = turn[at * 128 + c + lane];
+                    }
+                }
+            }
+        }
+    } else if (warp >= 4 + kEpilogueWarps) {
+        // ---------------------------------------------------------------- split
+        const int i = threadIdx.x - 32 * (4 + kEpilogueWarps);
+        const int row_shift = columns == 64 ? 4 : 5;           // quads of a row
+        for (int t = t_begin, n = 0, at = 0, raw_phase = 0; t < t_end; ++t, ++n) {
+            const int s = n & 1;
+            alive = mbar_wait(raw_full(at), raw_phase, abort_flag, kSpin);
+            if (!alive) break;
+            Quad<float> q[8];
+            const float4* const raw = reinterpret_cast<const float4*>(smem + at * kRawBytes);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < 4 || columns == 128) q[j].v = raw[i + j * 256];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(raw_empty(at));
+            alive = mbar_wait(plane_empty(s), ((n >> 1) & 1) ^ 1, abort_flag, kSpin);
+            if (!alive) break;
+            uint8_t* const plane = smem + kPlane0 + s * kPlaneBytes;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (j < 4 || columns == 128) {
+                    const int idx = i + j * 256, row = idx >> row_shift, quad = idx & ((1 << row_shift) - 1);
+                    store_quad<float, 2 * kPlaneTile>(plane, (quad >> 4) * kPlaneTile + quad_offset(row, quad & 15), q[j]);
+                }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(plane_full(s));
+            if (++at == kRaw) {
+                at = 0;
+                raw_phase ^= 1;
+            }
+        }
+    }
+    fence_before_sync();
+    __syncthreads();
+    if (warp == 2) {
+        fence_after_sync();
+        if (*abort_flag) {
+            // a wait ran out: copies and MMAs under way end before the CTA gives its memory back
+            for (int n = 0; n < 20000; ++n) __nanosleep(1000);
+            if (lane == 0 && p.a.status) atomicOr(p.a.status, FMB_STATUS_TENSOR_TIMEOUT);
+        }
+        __syncwarp();
+        tmem_free(tmem, 512);
+    }
+}
+
+template <int MODE>
+int launch(const SplitArgs& p, const CUtensorMap& rows, int wide_out, cudaStream_t stream) {
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_resident<MODE>, kSmem));
+    const long long tiles = most_units(&p.a, kTN) * p.feature_tiles;
+    k_grouped_resident<MODE><<<(int)std::min<long long>(tiles, sm_count()), kThreads, kSmem, stream>>>(p, rows, wide_out);
+    FMB_LAUNCH_CHECK();
+    return FMB_OK;
+}
+
+}  // namespace
+
+int resident_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
+    const bool forward = mode == kLinear;
+    const int depth = forward ? a->k : a->n, width = forward ? a->n : a->k;
+    if (a->type != FMB_TYPE_F32 || mode == kWeightGradient || depth > kK) return FMB_ERR_UNSUPPORTED;
+    CUtensorMap rows;
+    if (!encode_map(&rows, a->type, forward ? a->x : a->y, depth, a->rows, 1, forward ? a->x_stride : a->y_stride, 0, 1, 2,
+                    depth <= 64 ? 64 : 128, false))
+        return FMB_ERR_UNSUPPORTED;
+    SplitArgs p;
+    p.a = *a;
+    p.feature_tiles = ceil_div(width, 128);
+    p.row_tiles = 1;
+    p.unit_rows = kTN;
+    p.wide_features = four_at_a_time(a->w, a->w_row_stride, 4) && a->w_group_stride % 4 == 0;
+    p.wide_rows = 1;
+    const int wide_out = width % 4 == 0 && four_at_a_time(forward ? a->y : a->x, forward ? a->y_stride : a->x_stride, 4);
+    return forward ? launch<kLinear>(p, rows, wide_out, stream) : launch<kInputGradient>(p, rows, wide_out, stream);
+}
+
+}  // namespace grp
+}  // namespace fmb

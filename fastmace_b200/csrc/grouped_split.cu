@@ -15,8 +15,7 @@
 //
 // Two groups of eight warps bring blocks of 64 of the depth in turn, one's loads under way while the other splits.
 
-#include "grouped.cuh"
-#include "tc_common.cuh"
+#include "grouped_tc.cuh"
 
 #include <algorithm>
 
@@ -27,8 +26,7 @@ namespace {
 
 using namespace tc;
 
-constexpr int kDepth = 64, kTN = 64;
-constexpr unsigned kSpin = 1u << 20;
+constexpr int kTN = 64;
 constexpr int kGroupWarps = 8, kLoaderWarps = 2 * kGroupWarps, kEpilogueWarps = 4;
 constexpr int kMmaWarp = kLoaderWarps + kEpilogueWarps;
 constexpr int kThreads = 32 * (kMmaWarp + 1);
@@ -47,125 +45,10 @@ template <typename T, bool RESIDENT> struct Shape {
     static constexpr int kTmem = kParts == 3 ? 512 : 128;
 };
 
-struct Args {
-    fmb_grouped_t a;
-    int feature_tiles, row_tiles, unit_rows;
-    int wide_features, wide_rows;                // operands that may be read four values at a time
-};
-
-struct Tile {
-    int unit, g, feature0, row0, first, count, units_of_group;
-};
-
-// Tile t: group by group, all units of a group for the same features and output rows one after the other
-__device__ __forceinline__ Tile locate(const Args& p, const int* first_unit, int t) {
-    Tile w;
-    const int per_unit = p.feature_tiles * p.row_tiles;
-    w.g = group_of_unit(first_unit, p.a.groups, t / per_unit);
-    const int before = first_unit[w.g];
-    w.units_of_group = max(1, first_unit[w.g + 1] - before);
-    const int local = t - before * per_unit, rest = local / w.units_of_group, skip = local - rest * w.units_of_group;
-    w.unit = before + skip;
-    const int rt = rest / p.feature_tiles;
-    w.row0 = rt * kTN;
-    w.feature0 = (rest - rt * p.feature_tiles) * 128;
-    int begin, end;
-    group_span(p.a.offsets, w.g, p.a.rows, begin, end);
-    // offsets that are none could make a unit that lies outside its group: it has no entries (64 bits: see grouped_tc.cu)
-    const long long first = begin + (long long)skip * p.unit_rows, left = skip >= 0 ? end - first : 0;
-    w.first = left > 0 ? (int)first : end;
-    w.count = left <= 0 ? 0 : left < p.unit_rows ? (int)left : p.unit_rows;
-    return w;
-}
-
-__device__ __forceinline__ int row_at(const Args& p, int entry, int end) {
-    const int row = entry < end ? __ldg(p.a.order + entry) : -1;
-    return (unsigned)row < (unsigned)p.a.rows ? row : -1;
-}
-
-template <typename T> struct Quad { uint2 v; };
-template <> struct Quad<float> { float4 v; };
-
-// four values from p on, of which `live` (at most four) exist
-template <typename T>
-__device__ __forceinline__ Quad<T> load_quad(const T* p, int live, bool wide) {
-    Quad<T> q;
-    if constexpr (sizeof(T) == 4) {
-        if (wide && live >= 4) {
-            q.v = __ldg(reinterpret_cast<const float4*>(p));
-        } else {
-            q.v.x = live > 0 ? __ldg(p) : 0.0f;
-            q.v.y = live > 1 ? __ldg(p + 1) : 0.0f;
-            q.v.z = live > 2 ? __ldg(p + 2) : 0.0f;
-            q.v.w = live > 3 ? __ldg(p + 3) : 0.0f;
-        }
-    } else {
-        if (wide && live >= 4) {
-            q.v = __ldg(reinterpret_cast<const uint2*>(p));
-        } else {
-            const unsigned short* const h = reinterpret_cast<const unsigned short*>(p);
-            const uint32_t a = live > 0 ? __ldg(h) : 0, b = live > 1 ? __ldg(h + 1) : 0;
-            const uint32_t c = live > 2 ? __ldg(h + 2) : 0, d = live > 3 ? __ldg(h + 3) : 0;
-            q.v = make_uint2(a | b << 16, c | d << 16);
-        }
-    }
-    return q;
-}
-
-// upper halves of two floats side by side
-__device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
-__device__ __forceinline__ float without_upper(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
-
-// four consecutive values at byte `offset` of every part
-template <typename T, int PART_BYTES>
-__device__ __forceinline__ void store_quad(uint8_t* tile, uint32_t offset, const Quad<T>& q) {
-    if constexpr (sizeof(T) == 4) {
-        float a = q.v.x, b = q.v.y, c = q.v.z, d = q.v.w;
-#pragma unroll
-        for (int part = 0; part < 3; ++part) {
-            *reinterpret_cast<uint2*>(tile + part * PART_BYTES + offset) = make_uint2(upper_halves(a, b), upper_halves(c, d));
-            if (part < 2) {
-                a = without_upper(a);
-                b = without_upper(b);
-                c = without_upper(c);
-                d = without_upper(d);
-            }
-        }
-    } else {
-        *reinterpret_cast<uint2*>(tile + offset) = q.v;
-    }
-}
-
-// byte of quad q of row r in a tile of 128-byte rows with the 128-byte swizzle
-__device__ __forceinline__ uint32_t quad_offset(int r, int q) {
-    return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + (((q >> 1) ^ (r & 7)) << 4) + (q & 1) * 8);
-}
-
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-        "}\n"
-        :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-
-// MN-major tile: 64 depths of 64 features each, 8 KB apart, 1024 bytes between 8 depths
-__device__ __forceinline__ uint64_t make_desc_mn(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3ffff) >> 4);
-    d |= (uint64_t)(kDepth * 128 >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-
 // The features' side of a block: `count` quads per thread from thread `i` of `step` threads on.
 // LINEAR: W[g] rows are the depth. INPUT GRADIENT: W[g] rows are the features. WEIGHT GRADIENT: rows of y, by number.
 template <typename T, int MODE, int N, int THREADS, typename RowOf>
-__device__ __forceinline__ void load_features(const Args& p, const Tile& w, int d0, int depth, int i, RowOf row_of, Quad<T> (&q)[N]) {
+__device__ __forceinline__ void load_features(const SplitArgs& p, const Tile& w, int d0, int depth, int i, RowOf row_of, Quad<T> (&q)[N]) {
     const int width = MODE == kInputGradient ? p.a.k : p.a.n;
     const T* const weights = (const T*)p.a.w + (MODE == kWeightGradient ? 0 : w.g * p.a.w_group_stride);
 #pragma unroll
@@ -196,7 +79,7 @@ __device__ __forceinline__ void store_features(uint8_t* tile, int i, const Quad<
 
 template <typename T, int MODE, bool RESIDENT>
 __global__ void __launch_bounds__(kThreads, 1)
-k_grouped_split(const __grid_constant__ Args p) {
+k_grouped_split(const __grid_constant__ SplitArgs p) {
     using S = Shape<T, RESIDENT>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -247,7 +130,7 @@ k_grouped_split(const __grid_constant__ Args p) {
         uint32_t phase = 0, w_phase = 0;
         bool alive = true;
         for (int t = t_begin; alive && t < t_end; ++t) {
-            const Tile w = locate(p, first_unit, t);
+            const Tile w = locate(p, first_unit, t, kTN);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
             const int end = w.first + w.count;
             if constexpr (RESIDENT) {
@@ -322,7 +205,7 @@ k_grouped_split(const __grid_constant__ Args p) {
         constexpr int kChunkBlocks = S::kChunk / kDepth;
         bool alive = true;
         for (int t = t_begin; alive && t < t_end; ++t) {
-            const Tile w = locate(p, first_unit, t);
+            const Tile w = locate(p, first_unit, t, kTN);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
             bool release = false;
             if constexpr (RESIDENT) {
@@ -334,7 +217,7 @@ k_grouped_split(const __grid_constant__ Args p) {
                     if (!alive) break;
                 }
                 if (t + 1 < t_end) {
-                    const Tile next = locate(p, first_unit, t + 1);
+                    const Tile next = locate(p, first_unit, t + 1, kTN);
                     release = next.g != held_g || next.feature0 != held_f;
                 }
             }
@@ -399,7 +282,7 @@ k_grouped_split(const __grid_constant__ Args p) {
         }
         bool alive = true;
         for (int t = t_begin; alive && t < t_end; ++t) {
-            const Tile w = locate(p, first_unit, t);
+            const Tile w = locate(p, first_unit, t, kTN);
             const int feature = w.feature0 + quarter * 32 + lane;
             const int depth = kWeights ? w.count : depth_of_row, chunks = (depth + S::kChunk - 1) / S::kChunk;
             float sum[kTN];
@@ -473,12 +356,8 @@ k_grouped_split(const __grid_constant__ Args p) {
     }
 }
 
-bool four_at_a_time(const void* base, long long stride, int bytes) {
-    return ((uintptr_t)base & (uintptr_t)(4 * bytes - 1)) == 0 && stride % 4 == 0;
-}
-
 template <typename T, int MODE, bool RESIDENT>
-int launch(const Args& p, long long tiles, cudaStream_t stream) {
+int launch(const SplitArgs& p, long long tiles, cudaStream_t stream) {
     using S = Shape<T, RESIDENT>;
     FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_split<T, MODE, RESIDENT>, S::kSmem));
     k_grouped_split<T, MODE, RESIDENT><<<(int)std::min<long long>(tiles, sm_count()), kThreads, S::kSmem, stream>>>(p);
@@ -488,7 +367,7 @@ int launch(const Args& p, long long tiles, cudaStream_t stream) {
 
 template <typename T>
 int typed(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
-    Args p;
+    SplitArgs p;
     p.a = *a;
     const int bytes = (int)sizeof(T);
     const bool x_wide = four_at_a_time(a->x, a->x_stride, bytes), y_wide = four_at_a_time(a->y, a->y_stride, bytes);

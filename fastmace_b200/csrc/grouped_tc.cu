@@ -12,10 +12,7 @@
 // with zeros; nothing is permuted in memory. Weights come by TMA tiles from the caller's layout. Operands whose depth runs along
 // memory are K-major tiles, the others MN-major ones; both with the 128-byte swizzle.
 
-#include "grouped.cuh"
-#include "tc_common.cuh"
-
-#include <cuda.h>
+#include "grouped_tc.cuh"
 
 #include <algorithm>
 
@@ -26,8 +23,6 @@ namespace {
 
 using namespace tc;
 
-constexpr int kDepth = 64;                       // depth of a stage: 128 bytes of 16-bit values
-constexpr unsigned kSpin = 1u << 20;
 constexpr int kProducerWarps = 4, kEpilogueWarps = 8;
 constexpr int kThreads = 32 * (kProducerWarps + kEpilogueWarps);
 constexpr int kChunk = 512;                      // weight gradient: depth after which an accumulator moves to registers
@@ -52,55 +47,14 @@ __device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map
                  :: "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
 
-__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int col, int r0, int r1, int r2, int r3, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-                 :: "r"(dst), "l"(map), "r"(col), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar) : "memory");
-}
-
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-        "}\n"
-        :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-
-// MN-major tile with the 128-byte swizzle: 64 depths of 64 features each, 8 KB apart, 1024 bytes between 8 depths
-__device__ __forceinline__ uint64_t make_desc_mn(uint32_t smem_addr) {
-    uint64_t d = 0;
-    d |= (uint64_t)((smem_addr & 0x3ffff) >> 4);
-    d |= (uint64_t)(kDepth * 128 >> 4) << 16;
-    d |= (uint64_t)(1024 >> 4) << 32;
-    d |= (uint64_t)1 << 46;
-    d |= (uint64_t)2 << 61;
-    return d;
-}
-
-__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&v)[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
-        "tcgen05.wait::ld.sync.aligned;"
-        : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]), "=&r"(r[4]), "=&r"(r[5]), "=&r"(r[6]), "=&r"(r[7]),
-          "=&r"(r[8]), "=&r"(r[9]), "=&r"(r[10]), "=&r"(r[11]), "=&r"(r[12]), "=&r"(r[13]), "=&r"(r[14]), "=&r"(r[15]),
-          "=&r"(r[16]), "=&r"(r[17]), "=&r"(r[18]), "=&r"(r[19]), "=&r"(r[20]), "=&r"(r[21]), "=&r"(r[22]), "=&r"(r[23]),
-          "=&r"(r[24]), "=&r"(r[25]), "=&r"(r[26]), "=&r"(r[27]), "=&r"(r[28]), "=&r"(r[29]), "=&r"(r[30]), "=&r"(r[31])
-        : "r"(taddr) : "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-
 // Tile t of the launch: its unit (entries [first, first + count) of group g in `order`), features and output rows.
-struct Tile {
+struct TmaTile {
     int unit, g, first, count, feature0, row0, units_of_group;
 };
 
 template <int MODE>
-__device__ __forceinline__ Tile locate(const Args& p, const int* first_unit, int t, int tn) {
-    Tile w;
+__device__ __forceinline__ TmaTile locate(const Args& p, const int* first_unit, int t, int tn) {
+    TmaTile w;
     const int per_unit = p.feature_tiles * p.row_tiles;
     w.unit = t / per_unit;
     const int rest = t - w.unit * per_unit, rt = rest / p.feature_tiles;
@@ -173,7 +127,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         const int part = warp - 1;               // of the gather
         bool alive = true;
         for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
-            const Tile w = locate<MODE>(p, first_unit, t, TN);
+            const TmaTile w = locate<MODE>(p, first_unit, t, TN);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
             const int end = w.first + w.count;
             // rows of the output this warp gathers: lane l holds the row numbers 4 (part * TN / 8 + l) and on
@@ -271,7 +225,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | kMajor | ((uint32_t)(128 >> 4) << 24);
         bool alive = true;
         for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
-            const Tile w = locate<MODE>(p, first_unit, t, TN);
+            const TmaTile w = locate<MODE>(p, first_unit, t, TN);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
             const int columns = kWeights ? TN : max(16, min(TN, (w.count + 15) / 16 * 16));
             const uint32_t idesc = kDesc | ((uint32_t)(columns >> 3) << 17);
@@ -326,7 +280,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         }
         bool alive = true;
         for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
-            const Tile w = locate<MODE>(p, first_unit, t, TN);
+            const TmaTile w = locate<MODE>(p, first_unit, t, TN);
             const int feature = w.feature0 + quarter * 32 + lane;
             if constexpr (kWeights) {
                 constexpr int kCols = TN / 2;
@@ -434,25 +388,6 @@ Encode encoder() {
     return found;
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
-
-// [groups][rows][columns] with the strides given, in boxes of 1 x box_rows x 64
-bool encode_map(CUtensorMap* map, int type, const void* base, int columns, int rows, int groups, long long row_stride,
-                long long group_stride, int box_rows, int dims) {
-    const Encode encode = encoder();
-    if (!encode || !aligned16(base)) return false;
-    if (rows == 1) row_stride = std::max<long long>(row_stride, (columns + 7) / 8 * 8);     // never used
-    if (groups == 1) group_stride = 8;
-    if (row_stride <= 0 || row_stride % 8 || row_stride >= (1ll << 38)) return false;
-    if (dims == 3 && (group_stride <= 0 || group_stride % 8 || group_stride >= (1ll << 38))) return false;
-    const cuuint64_t size[3] = {(cuuint64_t)columns, (cuuint64_t)rows, (cuuint64_t)groups};
-    const cuuint64_t stride[2] = {(cuuint64_t)row_stride * 2, (cuuint64_t)group_stride * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
-    return encode(map, type == FMB_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims,
-                  const_cast<void*>(base), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <typename T, int MODE, int TN>
 int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, long long tiles, cudaStream_t stream) {
     FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN>, Shape<TN>::kSmem));
@@ -492,11 +427,11 @@ void weight_plan(const fmb_grouped_t* a, int& tn, int& unit_rows) {
 bool maps(const fmb_grouped_t* a, Mode mode, CUtensorMap* features, CUtensorMap* rows) {
     if (a->type == FMB_TYPE_F32 || a->rows == 0) return false;
     if (mode == kWeightGradient)
-        return encode_map(features, a->type, a->y, a->n, a->rows, 1, a->y_stride, 0, 1, 2) &&
-               encode_map(rows, a->type, a->x, a->k, a->rows, 1, a->x_stride, 0, 1, 2);
+        return encode_map(features, a->type, a->y, a->n, a->rows, 1, a->y_stride, 0, 1, 2, 64, true) &&
+               encode_map(rows, a->type, a->x, a->k, a->rows, 1, a->x_stride, 0, 1, 2, 64, true);
     const bool forward = mode == kLinear;
-    return encode_map(features, a->type, a->w, a->n, a->k, a->groups, a->w_row_stride, a->w_group_stride, forward ? 64 : 128, 3) &&
-           encode_map(rows, a->type, forward ? a->x : a->y, forward ? a->k : a->n, a->rows, 1, forward ? a->x_stride : a->y_stride, 0, 1, 2);
+    return encode_map(features, a->type, a->w, a->n, a->k, a->groups, a->w_row_stride, a->w_group_stride, forward ? 64 : 128, 3, 64, true) &&
+           encode_map(rows, a->type, forward ? a->x : a->y, forward ? a->k : a->n, a->rows, 1, forward ? a->x_stride : a->y_stride, 0, 1, 2, 64, true);
 }
 
 template <typename T>
@@ -525,6 +460,25 @@ int tma_typed(const fmb_grouped_t* a, Mode mode, const CUtensorMap& features, co
 }
 
 }  // namespace
+
+bool encode_map(CUtensorMap* map, int type, const void* base, int columns, int rows, int groups, long long row_stride,
+                long long group_stride, int box_rows, int dims, int box_columns, bool swizzled) {
+    const Encode encode = encoder();
+    const int bytes = type == FMB_TYPE_F32 ? 4 : 2, unit = 16 / bytes;           // values in 16 bytes
+    if (!encode || ((uintptr_t)base & 15) != 0) return false;
+    if (rows == 1) row_stride = std::max<long long>(row_stride, (columns + unit - 1) / unit * unit);     // never used
+    if (groups == 1) group_stride = unit;
+    if (row_stride <= 0 || row_stride % unit || row_stride >= (1ll << 37)) return false;
+    if (dims == 3 && (group_stride <= 0 || group_stride % unit || group_stride >= (1ll << 37))) return false;
+    const cuuint64_t size[3] = {(cuuint64_t)columns, (cuuint64_t)rows, (cuuint64_t)groups};
+    const cuuint64_t stride[2] = {(cuuint64_t)row_stride * bytes, (cuuint64_t)group_stride * bytes};
+    const cuuint32_t box[3] = {(cuuint32_t)box_columns, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    const CUtensorMapDataType kind = type == FMB_TYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : type == FMB_TYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return encode(map, kind, dims, const_cast<void*>(base), size, stride, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 int tma_unit_rows(const fmb_grouped_t* a) {
     int tn, unit_rows;

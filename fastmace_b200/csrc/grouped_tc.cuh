@@ -1,0 +1,169 @@
+// Tensor-core side of the grouped products: TMA, MMAs of 16-bit operands, tiles, and the split of fp32 into bf16 parts.
+#pragma once
+
+#include "grouped.cuh"
+#include "tc_common.cuh"
+
+#include <cuda.h>
+
+namespace fmb {
+namespace grp {
+
+constexpr int kDepth = 64;                       // depth of a stage: 128 bytes of 16-bit values
+constexpr unsigned kSpin = 1u << 20;
+
+__device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map, int col, int r0, int r1, int r2, int r3, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+                 :: "r"(dst), "l"(map), "r"(col), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar) : "memory");
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n"
+        :: "r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// the same with the first operand in tensor memory
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n"
+        :: "r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
+}
+
+// MN-major tile with the 128-byte swizzle: 64 depths of 64 features each, 8 KB apart, 1024 bytes between 8 depths
+__device__ __forceinline__ uint64_t make_desc_mn(uint32_t smem_addr) {
+    uint64_t d = 0;
+    d |= (uint64_t)((smem_addr & 0x3ffff) >> 4);
+    d |= (uint64_t)(kDepth * 128 >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+__device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&v)[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=&r"(r[0]), "=&r"(r[1]), "=&r"(r[2]), "=&r"(r[3]), "=&r"(r[4]), "=&r"(r[5]), "=&r"(r[6]), "=&r"(r[7]),
+          "=&r"(r[8]), "=&r"(r[9]), "=&r"(r[10]), "=&r"(r[11]), "=&r"(r[12]), "=&r"(r[13]), "=&r"(r[14]), "=&r"(r[15]),
+          "=&r"(r[16]), "=&r"(r[17]), "=&r"(r[18]), "=&r"(r[19]), "=&r"(r[20]), "=&r"(r[21]), "=&r"(r[22]), "=&r"(r[23]),
+          "=&r"(r[24]), "=&r"(r[25]), "=&r"(r[26]), "=&r"(r[27]), "=&r"(r[28]), "=&r"(r[29]), "=&r"(r[30]), "=&r"(r[31])
+        : "r"(taddr) : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// ------------------------------------------------------------------------------------------------ operands brought by threads
+
+struct SplitArgs {
+    fmb_grouped_t a;
+    int feature_tiles, row_tiles, unit_rows;
+    int wide_features, wide_rows;                // operands that may be read four values at a time
+};
+
+struct Tile {
+    int unit, g, feature0, row0, first, count, units_of_group;
+};
+
+// Tile t: group by group, all units of a group for the same features and output rows one after the other
+__device__ __forceinline__ Tile locate(const SplitArgs& p, const int* first_unit, int t, int tile_rows) {
+    Tile w;
+    const int per_unit = p.feature_tiles * p.row_tiles;
+    w.g = group_of_unit(first_unit, p.a.groups, t / per_unit);
+    const int before = first_unit[w.g];
+    w.units_of_group = max(1, first_unit[w.g + 1] - before);
+    const int local = t - before * per_unit, rest = local / w.units_of_group, skip = local - rest * w.units_of_group;
+    w.unit = before + skip;
+    const int rt = rest / p.feature_tiles;
+    w.row0 = rt * tile_rows;
+    w.feature0 = (rest - rt * p.feature_tiles) * 128;
+    int begin, end;
+    group_span(p.a.offsets, w.g, p.a.rows, begin, end);
+    // offsets that are none could make a unit that lies outside its group: it has no entries (64 bits: see grouped_tc.cu)
+    const long long first = begin + (long long)skip * p.unit_rows, left = skip >= 0 ? end - first : 0;
+    w.first = left > 0 ? (int)first : end;
+    w.count = left <= 0 ? 0 : left < p.unit_rows ? (int)left : p.unit_rows;
+    return w;
+}
+
+__device__ __forceinline__ int row_at(const SplitArgs& p, int entry, int end) {
+    const int row = entry < end ? __ldg(p.a.order + entry) : -1;
+    return (unsigned)row < (unsigned)p.a.rows ? row : -1;
+}
+
+template <typename T> struct Quad { uint2 v; };
+template <> struct Quad<float> { float4 v; };
+
+// four values from p on, of which `live` (at most four) exist
+template <typename T>
+__device__ __forceinline__ Quad<T> load_quad(const T* p, int live, bool wide) {
+    Quad<T> q;
+    if constexpr (sizeof(T) == 4) {
+        if (wide && live >= 4) {
+            q.v = __ldg(reinterpret_cast<const float4*>(p));
+        } else {
+            q.v.x = live > 0 ? __ldg(p) : 0.0f;
+            q.v.y = live > 1 ? __ldg(p + 1) : 0.0f;
+            q.v.z = live > 2 ? __ldg(p + 2) : 0.0f;
+            q.v.w = live > 3 ? __ldg(p + 3) : 0.0f;
+        }
+    } else {
+        if (wide && live >= 4) {
+            q.v = __ldg(reinterpret_cast<const uint2*>(p));
+        } else {
+            const unsigned short* const h = reinterpret_cast<const unsigned short*>(p);
+            const uint32_t a = live > 0 ? __ldg(h) : 0, b = live > 1 ? __ldg(h + 1) : 0;
+            const uint32_t c = live > 2 ? __ldg(h + 2) : 0, d = live > 3 ? __ldg(h + 3) : 0;
+            q.v = make_uint2(a | b << 16, c | d << 16);
+        }
+    }
+    return q;
+}
+
+// upper halves of two floats side by side
+__device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
+__device__ __forceinline__ float without_upper(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
+
+// four consecutive values at byte `offset` of every part
+template <typename T, int PART_BYTES>
+__device__ __forceinline__ void store_quad(uint8_t* tile, uint32_t offset, const Quad<T>& q) {
+    if constexpr (sizeof(T) == 4) {
+        float a = q.v.x, b = q.v.y, c = q.v.z, d = q.v.w;
+#pragma unroll
+        for (int part = 0; part < 3; ++part) {
+            *reinterpret_cast<uint2*>(tile + part * PART_BYTES + offset) = make_uint2(upper_halves(a, b), upper_halves(c, d));
+            if (part < 2) {
+                a = without_upper(a);
+                b = without_upper(b);
+                c = without_upper(c);
+                d = without_upper(d);
+            }
+        }
+    } else {
+        *reinterpret_cast<uint2*>(tile + offset) = q.v;
+    }
+}
+
+// byte of quad q of row r in a tile of 128-byte rows with the 128-byte swizzle
+__device__ __forceinline__ uint32_t quad_offset(int r, int q) {
+    return (uint32_t)((r >> 3) * 1024 + (r & 7) * 128 + (((q >> 1) ^ (r & 7)) << 4) + (q & 1) * 8);
+}
+
+// A tensor map of [groups][rows][columns] with the strides given (in elements), in boxes of 1 x box_rows x box_columns; false
+// where TMA does not take the alignment. dims 2: one group.
+bool encode_map(CUtensorMap* map, int type, const void* base, int columns, int rows, int groups, long long row_stride,
+                long long group_stride, int box_rows, int dims, int box_columns, bool swizzled);
+
+}  // namespace grp
+}  // namespace fmb
