@@ -25,10 +25,11 @@ using namespace tc;
 constexpr int kTN = 64, kK = 128;                          // rows of a tile, depth
 constexpr int kRaw = 3, kRawBytes = kTN * kK * 4;
 constexpr int kPlanes = 2, kPlaneTile = kTN * kDepth * 2, kPlaneBytes = 3 * 2 * kPlaneTile;      // [part][half of the depth]
-constexpr int kTurnBytes = 32 * 128 * 4;                   // half a tile of results
-constexpr int kPlane0 = kRaw * kRawBytes, kTurn0 = kPlane0 + kPlanes * kPlaneBytes, kUnits0 = kTurn0 + kTurnBytes;
+constexpr int kTurnRows = 16, kTurnBytes = kTurnRows * 128 * 4;      // rows of results that turn at a time, one buffer per set
+constexpr int kPlane0 = kRaw * kRawBytes, kTurn0 = kPlane0 + kPlanes * kPlaneBytes, kUnits0 = kTurn0 + 2 * kTurnBytes;
 constexpr int kSmem = 1024 + kUnits0 + (FMB_MAX_GROUPS + 1) * 4 + 256;
-constexpr int kEpilogueWarps = 4, kSplitWarps = 8, kThreads = 32 * (4 + kEpilogueWarps + kSplitWarps);
+constexpr int kEpilogueWarps = 8, kSplitWarps = 8,           // two sets of four, which take the tiles in turn; eight that split
+              kThreads = 32 * (4 + kEpilogueWarps + kSplitWarps);
 constexpr uint32_t kAccumulators = 192;                    // TMEM columns before them: the weights
 static_assert(kSmem <= 227 * 1024, "fits an SM");
 
@@ -100,9 +101,9 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
-            mbar_init(acc_empty(b), kEpilogueWarps);
+            mbar_init(acc_empty(b), 4);
         }
-        mbar_init(w_full, kEpilogueWarps);
+        mbar_init(w_full, 4);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -185,64 +186,73 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
         }
     } else if (warp >= 4 && warp < 4 + kEpilogueWarps) {
         // ---------------------------------------------------------------- weights in, results out
-        const int quarter = warp & 3, id = quarter * 32 + lane;
+        const int quarter = warp & 3, set = (warp - 4) >> 2, id = quarter * 32 + lane;
         float* const out = (float*)(MODE == kLinear ? p.a.y : p.a.x);
         const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        float* const turn = reinterpret_cast<float*>(smem + kTurn0);                 // [32 rows][128 features]
+        float* const turn = reinterpret_cast<float*>(smem + kTurn0 + set * kTurnBytes);      // [rows][128 features]
         if (p.a.zero_rest) {
             const int from = min(max(p.a.offsets[p.a.groups], 0), p.a.rows);
-            for (int e = from + blockIdx.x * kEpilogueWarps + quarter; e < p.a.rows; e += gridDim.x * kEpilogueWarps) {
+            for (int e = from + blockIdx.x * kEpilogueWarps + warp - 4; e < p.a.rows; e += gridDim.x * kEpilogueWarps) {
                 const int row = row_at(p, e, p.a.rows);
                 if (row >= 0)
                     for (int c = lane; c < width; c += 32) out[row * stride + c] = 0.0f;
             }
         }
-        int held_g = -1, held_f = -1;
-        for (int t = t_begin, n = 0; t < t_end; ++t, ++n) {
-            const Tile w = locate(p, first_unit, t, kTN);
-            if (w.g != held_g || w.feature0 != held_f) {
-                // the accumulators of every tile before have been waited for: nobody reads the old weights
-                held_g = w.g;
-                held_f = w.feature0;
+        Tile w;
+        int row_low = -1, row_high = -1;
+        auto find = [&](int t) {
+            if (t >= t_end) return;
+            w = locate(p, first_unit, t, kTN);
+            row_low = row_at(p, w.first + lane, w.first + w.count);
+            row_high = row_at(p, w.first + 32 + lane, w.first + w.count);
+        };
+        find(t_begin + set);
+        for (int t = t_begin + set, n = set; t < t_end; t += 2, n += 2) {
+            if (t == t_begin || w.unit == first_unit[w.g]) {
+                // other weights: nobody reads the old ones once the tile before, the other set's, has its accumulators
+                if (n > 0) alive = mbar_wait(acc_full(set ^ 1), ((n - 1) >> 1) & 1, abort_flag, kSpin);
+                if (!alive) break;
+                fence_after_sync();
                 bring_weights<MODE>(p, w, w.feature0 + id, depth, tmem + lanes);
                 fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(w_full);
             }
-            const int s = n & 1;
-            const int row_low = row_at(p, w.first + lane, w.first + w.count), row_high = row_at(p, w.first + 32 + lane, w.first + w.count);
-            alive = mbar_wait(acc_full(s), (n >> 1) & 1, abort_flag, kSpin);
+            alive = mbar_wait(acc_full(set), (n >> 1) & 1, abort_flag, kSpin);
             if (!alive) break;
             fence_after_sync();
-            const uint32_t main = tmem + lanes + kAccumulators + s * 2 * kTN;
+            const uint32_t main = tmem + lanes + kAccumulators + set * 2 * kTN;
+            const int low = row_low, high = row_high, feature0 = w.feature0;
 #pragma unroll 1
-            for (int half = 0; half < 2; ++half) {
-                float v[32], u[32];
-                tmem_load_32(main + half * 32, v);
-                tmem_load_32(main + kTN + half * 32, u);
-                if (half == 1) {
+            for (int r0 = 0; r0 < kTN; r0 += kTurnRows) {
+                float v[16], u[16];
+                tmem_load_16x2(main + r0, main + kTN + r0, v, u);
+                if (r0 == kTN - kTurnRows) {
                     fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty(s));
+                    if (lane == 0) mbar_arrive(acc_empty(set));
+                    find(t + 2);
                 }
-                named_barrier(1, 128);                       // the half before has been read
+                named_barrier(1 + set, 128);                 // what was here has been read
 #pragma unroll
-                for (int j = 0; j < 32; ++j) turn[j * 128 + id] = v[j] + u[j];
-                named_barrier(1, 128);
-                const int mine = half ? row_high : row_low;
+                for (int j = 0; j < kTurnRows; ++j) turn[j * 128 + id] = v[j] + u[j];
+                named_barrier(1 + set, 128);
+                float4 q[4];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int at = quarter + 4 * j, row = __shfl_sync(0xffffffffu, mine, at);
-                    if (row < 0) continue;
-                    float* const to = out + row * stride + w.feature0;
+                for (int j = 0; j < 4; ++j) q[j] = *reinterpret_cast<const float4*>(turn + (quarter * 4 + j) * 128 + 4 * lane);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = r0 + quarter * 4 + j, row = __shfl_sync(0xffffffffu, r0 < 32 ? low : high, at & 31);
+                    float* const to = out + row * stride + feature0 + 4 * lane;
+                    const int live = row < 0 ? 0 : width - feature0 - 4 * lane;
                     if (wide_out) {
-                        if (w.feature0 + 4 * lane < width)
-                            *reinterpret_cast<float4*>(to + 4 * lane) = *reinterpret_cast<const float4*>(turn + at * 128 + 4 * lane);
+                        if (live > 0) *reinterpret_cast<float4*>(to) = q[j];
                     } else {
-#pragma unroll
-                        for (int c = 0; c < 128; c += 32)
-                            if (w.feature0 + c + lane < width) to[c + lane] = turn[at * 128 + c + lane];
+                        if (live > 0) to[0] = q[j].x;
+                        if (live > 1) to[1] = q[j].y;
+                        if (live > 2) to[2] = q[j].z;
+                        if (live > 3) to[3] = q[j].w;
                     }
                 }
             }
