@@ -40,7 +40,7 @@ __device__ __forceinline__ void tmem_store_8(uint32_t taddr, const uint32_t (&v)
 
 // this lane's feature of the tile's weights, split, into the TMEM columns of the three planes (two values a column)
 template <int MODE>
-__device__ __forceinline__ void bring_weights(const SplitArgs& p, const Tile& w, int feature, int depth, uint32_t tmem) {
+__device__ __forceinline__ void bring_weights(const SplitArgs& p, const Walk& w, int feature, int depth, uint32_t tmem) {
     const int width = MODE == kInputGradient ? p.a.k : p.a.n;
     const float* const from = (const float*)p.a.w + w.g * p.a.w_group_stride + (MODE == kInputGradient ? feature * p.a.w_row_stride : feature);
     const bool live = feature < width;
@@ -117,47 +117,49 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
     const int depth = MODE == kLinear ? p.a.k : p.a.n, width = MODE == kLinear ? p.a.n : p.a.k;
     const int columns = depth <= 64 ? 64 : 128;              // of a row in the ring
     bool alive = true;
+    Walk w(p.a, first_unit, kTN, p.feature_tiles, 1, kTN);
 
-    if (warp == 0) {
-        // ---------------------------------------------------------------- rows
-        for (int t = t_begin, at = 0, phase = 0; t < t_end; ++t) {
-            const Tile w = locate(p, first_unit, t, kTN);
-            const int end = w.first + w.count, quads = (w.count + 3) / 4;
-            int rows[4];
+    if (warp == 0 || warp == 2 || warp == 3) {
+        // ---------------------------------------------------------------- rows: a warp per tile of the ring
+        const int at = warp == 0 ? 0 : warp - 1;
+        int rows[4], quads = 0;
+        auto find = [&] {
+            quads = (w.count + 3) / 4;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = lane < 16 ? row_at(p, w.first + 4 * lane + i, end) : -1;
+                const int row = lane < 16 ? row_at(p, w.first + 4 * lane + i, w.first + w.count) : -1;
                 rows[i] = row < 0 ? p.a.rows : row;           // what is no row is filled with zeros
             }
+        };
+        if (t_begin + at < t_end) {
+            w.start(t_begin + at);
+            find();
+        }
+        uint32_t phase = 0;
+        for (int t = t_begin + at; t < t_end; t += kRaw, phase ^= 1) {
             alive = mbar_wait(raw_empty(at), phase ^ 1, abort_flag, kSpin);
             if (!alive) break;
             const uint32_t dst = smem_u32(smem) + at * kRawBytes, bar = raw_full(at);
             if (elect_one()) mbar_expect_tx(bar, quads * columns * 16);
             __syncwarp();
-            for (int q = 0; q < quads; ++q) {
-                const int r0 = __shfl_sync(0xffffffffu, rows[0], q), r1 = __shfl_sync(0xffffffffu, rows[1], q);
-                const int r2 = __shfl_sync(0xffffffffu, rows[2], q), r3 = __shfl_sync(0xffffffffu, rows[3], q);
-                if (elect_one()) tma_gather4(dst + q * columns * 16, &row_map, 0, r0, r1, r2, r3, bar);
-                __syncwarp();
-            }
-            if (++at == kRaw) {
-                at = 0;
-                phase ^= 1;
+            if (lane < quads) tma_gather4(dst + lane * columns * 16, &row_map, 0, rows[0], rows[1], rows[2], rows[3], bar);
+            __syncwarp();
+            if (t + kRaw < t_end) {
+                w.step(kRaw);
+                find();
             }
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMAs
         constexpr uint32_t kDesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(kTN >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-        int held_g = -1, held_f = -1;
         uint32_t w_phase = 0;
         const int steps = (depth + 15) / 16;
         for (int t = t_begin, n = 0; t < t_end; ++t, ++n) {
-            const Tile w = locate(p, first_unit, t, kTN);
             const int s = n & 1;
             const uint32_t phase = (n >> 1) & 1;
-            if (w.g != held_g || w.feature0 != held_f) {
-                held_g = w.g;
-                held_f = w.feature0;
+            if (n == 0) w.start(t);
+            else w.step(1);
+            if (n == 0 || w.leads()) {
                 alive = mbar_wait(w_full, w_phase, abort_flag, kSpin);
                 w_phase ^= 1;
             }
@@ -199,17 +201,17 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
                     for (int c = lane; c < width; c += 32) out[row * stride + c] = 0.0f;
             }
         }
-        Tile w;
         int row_low = -1, row_high = -1;
-        auto find = [&](int t) {
-            if (t >= t_end) return;
-            w = locate(p, first_unit, t, kTN);
+        auto find = [&] {
             row_low = row_at(p, w.first + lane, w.first + w.count);
             row_high = row_at(p, w.first + 32 + lane, w.first + w.count);
         };
-        find(t_begin + set);
+        if (t_begin + set < t_end) {
+            w.start(t_begin + set);
+            find();
+        }
         for (int t = t_begin + set, n = set; t < t_end; t += 2, n += 2) {
-            if (t == t_begin || w.unit == first_unit[w.g]) {
+            if (n == 0 || w.leads()) {
                 // other weights: nobody reads the old ones once the tile before, the other set's, has its accumulators
                 if (n > 0) alive = mbar_wait(acc_full(set ^ 1), ((n - 1) >> 1) & 1, abort_flag, kSpin);
                 if (!alive) break;
@@ -232,7 +234,10 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
                     fence_before_sync();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(acc_empty(set));
-                    find(t + 2);
+                    if (t + 2 < t_end) {
+                        w.step(2);
+                        find();
+                    }
                 }
                 named_barrier(1 + set, 128);                 // what was here has been read
 #pragma unroll

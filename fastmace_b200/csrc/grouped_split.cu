@@ -48,7 +48,7 @@ template <typename T, bool RESIDENT> struct Shape {
 // The features' side of a block: `count` quads per thread from thread `i` of `step` threads on.
 // LINEAR: W[g] rows are the depth. INPUT GRADIENT: W[g] rows are the features. WEIGHT GRADIENT: rows of y, by number.
 template <typename T, int MODE, int N, int THREADS, typename RowOf>
-__device__ __forceinline__ void load_features(const SplitArgs& p, const Tile& w, int d0, int depth, int i, RowOf row_of, Quad<T> (&q)[N]) {
+__device__ __forceinline__ void load_features(const SplitArgs& p, const Walk& w, int d0, int depth, int i, RowOf row_of, Quad<T> (&q)[N]) {
     const int width = MODE == kInputGradient ? p.a.k : p.a.n;
     const T* const weights = (const T*)p.a.w + (MODE == kWeightGradient ? 0 : w.g * p.a.w_group_stride);
 #pragma unroll
@@ -122,6 +122,8 @@ k_grouped_split(const __grid_constant__ SplitArgs p) {
     const T* const row_source = (const T*)(MODE == kInputGradient ? p.a.y : p.a.x);
     const long long row_stride = MODE == kInputGradient ? p.a.y_stride : p.a.x_stride;
 
+    Walk w(p.a, first_unit, p.unit_rows, p.feature_tiles, p.row_tiles, kTN);
+
     if (warp < kLoaderWarps) {
         // ---------------------------------------------------------------- loaders
         const int group = warp / kGroupWarps, gw = warp % kGroupWarps, i = gw * 32 + lane;
@@ -130,7 +132,8 @@ k_grouped_split(const __grid_constant__ SplitArgs p) {
         uint32_t phase = 0, w_phase = 0;
         bool alive = true;
         for (int t = t_begin; alive && t < t_end; ++t) {
-            const Tile w = locate(p, first_unit, t, kTN);
+            if (t == t_begin) w.start(t);
+            else w.step(1);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
             const int end = w.first + w.count;
             if constexpr (RESIDENT) {
@@ -205,7 +208,8 @@ k_grouped_split(const __grid_constant__ SplitArgs p) {
         constexpr int kChunkBlocks = S::kChunk / kDepth;
         bool alive = true;
         for (int t = t_begin; alive && t < t_end; ++t) {
-            const Tile w = locate(p, first_unit, t, kTN);
+            if (t == t_begin) w.start(t);
+            else w.step(1);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
             bool release = false;
             if constexpr (RESIDENT) {
@@ -217,7 +221,8 @@ k_grouped_split(const __grid_constant__ SplitArgs p) {
                     if (!alive) break;
                 }
                 if (t + 1 < t_end) {
-                    const Tile next = locate(p, first_unit, t + 1, kTN);
+                    Walk next = w;
+                    next.step(1);
                     release = next.g != held_g || next.feature0 != held_f;
                 }
             }
@@ -282,7 +287,8 @@ k_grouped_split(const __grid_constant__ SplitArgs p) {
         }
         bool alive = true;
         for (int t = t_begin; alive && t < t_end; ++t) {
-            const Tile w = locate(p, first_unit, t, kTN);
+            if (t == t_begin) w.start(t);
+            else w.step(1);
             const int feature = w.feature0 + quarter * 32 + lane;
             const int depth = kWeights ? w.count : depth_of_row, chunks = (depth + S::kChunk - 1) / S::kChunk;
             float sum[kTN];
@@ -318,7 +324,7 @@ k_grouped_split(const __grid_constant__ SplitArgs p) {
             }
             if (!alive) break;
             if constexpr (kWeights) {
-                const bool direct = w.units_of_group <= 1;
+                const bool direct = w.units <= 1;
                 const long long stride = direct ? p.a.w_row_stride : p.a.n;
                 float* const to = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + (long long)w.unit * p.a.k * p.a.n) + feature;
                 if (feature < p.a.n) {

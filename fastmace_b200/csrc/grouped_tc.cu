@@ -47,33 +47,6 @@ __device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map
                  :: "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
 
-// Tile t of the launch: its unit (entries [first, first + count) of group g in `order`), features and output rows.
-struct TmaTile {
-    int unit, g, first, count, feature0, row0, units_of_group;
-};
-
-template <int MODE>
-__device__ __forceinline__ TmaTile locate(const Args& p, const int* first_unit, int t, int tn) {
-    TmaTile w;
-    const int per_unit = p.feature_tiles * p.row_tiles;
-    w.unit = t / per_unit;
-    const int rest = t - w.unit * per_unit, rt = rest / p.feature_tiles;
-    w.row0 = rt * tn;
-    w.feature0 = (rest - rt * p.feature_tiles) * 128;
-    w.g = group_of_unit(first_unit, p.a.groups, w.unit);
-    int begin, end;
-    group_span(p.a.offsets, w.g, p.a.rows, begin, end);
-    // offsets that are none could make a unit that lies outside its group: it has no entries
-    const int skip = w.unit - first_unit[w.g];
-    const long long first = begin + (long long)skip * p.unit_rows;
-    // (in 64 bits: as the minimum of a 32-bit difference and unit_rows the count came out as end + first, CUDA 12.9)
-    const long long left = skip >= 0 ? end - first : 0;
-    w.first = left > 0 ? (int)first : end;
-    w.count = left <= 0 ? 0 : left < p.unit_rows ? (int)left : p.unit_rows;
-    w.units_of_group = first_unit[w.g + 1] - first_unit[w.g];
-    return w;
-}
-
 // a row number that TMA fills with zeros stands for everything that is no row
 __device__ __forceinline__ int row_at(const Args& p, int entry, int end) {
     const int row = entry < end ? __ldg(p.a.order + entry) : p.a.rows;
@@ -120,6 +93,8 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     const int tiles = first_unit[p.a.groups] * p.feature_tiles * p.row_tiles;
     const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n;        // not of the weight gradient
 
+    Walk w(p.a, first_unit, p.unit_rows, p.feature_tiles, p.row_tiles, TN);
+
     if (warp < 3) {
         // ---------------------------------------------------------------- producers
         int at = 0;
@@ -127,7 +102,8 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         const int part = warp - 1;               // of the gather
         bool alive = true;
         for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
-            const TmaTile w = locate<MODE>(p, first_unit, t, TN);
+            if (t == (int)blockIdx.x) w.start(t);
+            else w.step(gridDim.x);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
             const int end = w.first + w.count;
             // rows of the output this warp gathers: lane l holds the row numbers 4 (part * TN / 8 + l) and on
@@ -225,7 +201,8 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | kMajor | ((uint32_t)(128 >> 4) << 24);
         bool alive = true;
         for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
-            const TmaTile w = locate<MODE>(p, first_unit, t, TN);
+            if (t == (int)blockIdx.x) w.start(t);
+            else w.step(gridDim.x);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
             const int columns = kWeights ? TN : max(16, min(TN, (w.count + 15) / 16 * 16));
             const uint32_t idesc = kDesc | ((uint32_t)(columns >> 3) << 17);
@@ -280,7 +257,8 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         }
         bool alive = true;
         for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
-            const TmaTile w = locate<MODE>(p, first_unit, t, TN);
+            if (t == (int)blockIdx.x) w.start(t);
+            else w.step(gridDim.x);
             const int feature = w.feature0 + quarter * 32 + lane;
             if constexpr (kWeights) {
                 constexpr int kCols = TN / 2;
@@ -305,7 +283,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1;
                 }
-                const bool direct = w.units_of_group <= 1;
+                const bool direct = w.units <= 1;
                 const long long stride = direct ? p.a.w_row_stride : p.a.n;
                 float* const out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + (long long)w.unit * p.a.k * p.a.n) + feature;
                 const int row0 = w.row0 + half * kCols;

@@ -72,30 +72,55 @@ struct SplitArgs {
     int wide_features, wide_rows;                // operands that may be read four values at a time
 };
 
-struct Tile {
-    int unit, g, feature0, row0, first, count, units_of_group;
-};
+// The tiles of a launch, group by group; of a group all units (entries [first, first + count) of `order`) for the same features
+// and output rows, then the next features, then the next output rows. A Walk goes through them in steps: the search
+// for the group and the reads of its span happen once per group, not per tile (as much as 2,000 cycles).
+struct Walk {
+    const int32_t* offsets;
+    const int* first_unit;
+    int groups, rows, unit_rows, feature_tiles, per_unit, tile_rows;
+    int g, local, units, begin, end;             // group, tile of it, its units, its span
+    int unit, feature0, row0, first, count;      // the tile
 
-// Tile t: group by group, all units of a group for the same features and output rows one after the other
-__device__ __forceinline__ Tile locate(const SplitArgs& p, const int* first_unit, int t, int tile_rows) {
-    Tile w;
-    const int per_unit = p.feature_tiles * p.row_tiles;
-    w.g = group_of_unit(first_unit, p.a.groups, t / per_unit);
-    const int before = first_unit[w.g];
-    w.units_of_group = max(1, first_unit[w.g + 1] - before);
-    const int local = t - before * per_unit, rest = local / w.units_of_group, skip = local - rest * w.units_of_group;
-    w.unit = before + skip;
-    const int rt = rest / p.feature_tiles;
-    w.row0 = rt * tile_rows;
-    w.feature0 = (rest - rt * p.feature_tiles) * 128;
-    int begin, end;
-    group_span(p.a.offsets, w.g, p.a.rows, begin, end);
-    // offsets that are none could make a unit that lies outside its group: it has no entries (64 bits: see grouped_tc.cu)
-    const long long first = begin + (long long)skip * p.unit_rows, left = skip >= 0 ? end - first : 0;
-    w.first = left > 0 ? (int)first : end;
-    w.count = left <= 0 ? 0 : left < p.unit_rows ? (int)left : p.unit_rows;
-    return w;
-}
+    __device__ __forceinline__ Walk(const fmb_grouped_t& a, const int* first_unit, int unit_rows, int feature_tiles, int row_tiles, int tile_rows)
+        : offsets(a.offsets), first_unit(first_unit), groups(a.groups), rows(a.rows), unit_rows(unit_rows), feature_tiles(feature_tiles),
+          per_unit(feature_tiles * row_tiles), tile_rows(tile_rows), g(0), local(0), units(1), begin(0), end(0),
+          unit(0), feature0(0), row0(0), first(0), count(0) {}
+
+    __device__ __forceinline__ void enter() {
+        units = max(1, first_unit[g + 1] - first_unit[g]);
+        group_span(offsets, g, rows, begin, end);
+    }
+    __device__ __forceinline__ void place() {
+        const int rest = local / units, skip = local - rest * units, rt = rest / feature_tiles;
+        unit = first_unit[g] + skip;
+        row0 = rt * tile_rows;
+        feature0 = (rest - rt * feature_tiles) * 128;
+        // offsets that are none could make a unit that lies outside its group: it has no entries. (In 64 bits: as the minimum of
+        // a 32-bit difference and unit_rows the count came out as end + first, CUDA 12.9.)
+        const long long at = begin + (long long)skip * unit_rows, left = end - at;
+        first = left > 0 ? (int)at : end;
+        count = left <= 0 ? 0 : left < unit_rows ? (int)left : unit_rows;
+    }
+    __device__ __forceinline__ void start(int t) {
+        g = group_of_unit(first_unit, groups, t / per_unit);
+        local = t - first_unit[g] * per_unit;
+        enter();
+        place();
+    }
+    // n tiles on; the caller has made sure that the launch has them
+    __device__ __forceinline__ void step(int n) {
+        local += n;
+        while (local >= units * per_unit && g + 1 < groups) {
+            local -= (first_unit[g + 1] - first_unit[g]) * per_unit;
+            do ++g; while (g + 1 < groups && first_unit[g + 1] == first_unit[g]);
+            enter();
+        }
+        place();
+    }
+    // first tile of its group with these features and output rows
+    __device__ __forceinline__ bool leads() const { return unit == first_unit[g]; }
+};
 
 __device__ __forceinline__ int row_at(const SplitArgs& p, int entry, int end) {
     const int row = entry < end ? __ldg(p.a.order + entry) : -1;
