@@ -7,7 +7,8 @@
 //           the row numbers
 //
 // Rows whose key is no group come behind all groups. Up to kRowsPerCta rows `place` alone does it: one launch.
-// Bound by latency: 8 bytes move per row and key reads hit L2 the second time.
+// Bound by latency: 8 bytes move per row and the second pass reads keys from L2. A lane asks for its keys all at once and keeps them for
+// both passes of `place`; one at a time, each waited for, 1,944 rows took 14 us.
 
 #include "fmb_common.cuh"
 
@@ -15,43 +16,65 @@ namespace fmb {
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kRowsPerWarp = 1024;
+constexpr int kWarps = 32, kThreads = kWarps * 32;
+constexpr int kKeys = 8;                                  // per lane
+constexpr int kRowsPerWarp = 32 * kKeys;
 constexpr int kRowsPerCta = kWarps * kRowsPerWarp;
 
-// `groups` stands for "no group"
+// the groups of this lane's rows begin + 32 i + lane: `groups` stands for "no group", -1 for rows past the end
 template <typename K>
-__device__ __forceinline__ int group_of(const K* __restrict__ keys, long long row, int groups) {
-    const K key = keys[row];
-    return key < 0 || key >= (K)groups ? groups : (int)key;
+__device__ __forceinline__ void load_keys(const K* __restrict__ keys, long long begin, long long rows, int groups, int (&g)[kKeys]) {
+    const int lane = threadIdx.x & 31;
+    K key[kKeys];
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+        const long long row = begin + 32 * i + lane;
+        key[i] = row < rows ? keys[row] : (K)-1;
+    }
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i)
+        g[i] = begin + 32 * i + lane >= rows ? -1 : key[i] < 0 || key[i] >= (K)groups ? groups : (int)key[i];
 }
 
-// counts[warp][g] of the rows of every warp of this CTA, in shared memory
-template <typename K>
-__device__ __forceinline__ void count_warp(const K* __restrict__ keys, long long begin, long long end, int groups, int* counts) {
+// counts[g] of this warp's rows
+__device__ __forceinline__ void count_warp(const int (&g)[kKeys], int* counts) {
     const int lane = threadIdx.x & 31;
-    for (long long row = begin + lane; row - lane < end; row += 32) {
-        const int g = row < end ? group_of(keys, row, groups) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, g);
-        if (g >= 0 && lane == __ffs(same) - 1) counts[g] += __popc(same);
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+        const unsigned same = __match_any_sync(0xffffffffu, g[i]);
+        if (g[i] >= 0 && lane == __ffs(same) - 1) counts[g[i]] += __popc(same);
         __syncwarp();
     }
+}
+
+// of the 32 warps' counts of group g: what the warps before lane `w`'s have, and all of them (lane = warp)
+__device__ __forceinline__ int warps_before(int mine, int& all) {
+    const int lane = threadIdx.x & 31;
+    int inclusive = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, inclusive, o);
+        if (lane >= o) inclusive += up;
+    }
+    all = __shfl_sync(0xffffffffu, inclusive, 31);
+    return inclusive - mine;
 }
 
 template <typename K>
 __global__ void __launch_bounds__(kThreads)
 k_group_count(const K* __restrict__ keys, long long rows, int groups, int32_t* __restrict__ table) {
     extern __shared__ int counts[];                       // [kWarps][groups + 1]
-    const int width = groups + 1, warp = threadIdx.x >> 5;
+    const int width = groups + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int g[kKeys];
+    load_keys(keys, (long long)blockIdx.x * kRowsPerCta + warp * kRowsPerWarp, rows, groups, g);
     for (int i = threadIdx.x; i < kWarps * width; i += kThreads) counts[i] = 0;
     __syncthreads();
-    const long long begin = (long long)blockIdx.x * kRowsPerCta + warp * kRowsPerWarp;
-    count_warp(keys, begin, min(rows, begin + kRowsPerWarp), groups, counts + warp * width);
+    count_warp(g, counts + warp * width);
     __syncthreads();
-    for (int g = threadIdx.x; g < width; g += kThreads) {
-        int sum = 0;
-        for (int w = 0; w < kWarps; ++w) sum += counts[w * width + g];
-        table[(long long)blockIdx.x * width + g] = sum;
+    for (int q = warp; q < width; q += kWarps) {
+        int all;
+        warps_before(counts[lane * width + q], all);
+        if (lane == 0) table[(long long)blockIdx.x * width + q] = all;
     }
 }
 
@@ -63,41 +86,42 @@ k_group_scan(int32_t* __restrict__ table, int32_t* __restrict__ totals, int ctas
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.x * 32 + lane;
     const int share = (ctas + 31) / 32, begin = warp * share, end = min(ctas, begin + share);
     int sum = 0;
-    if (g < width)
+    if (g < width) {
+#pragma unroll 8
         for (int c = begin; c < end; ++c) sum += table[(long long)c * width + g];
+    }
     part[warp][lane] = sum;
     __syncthreads();
     int before = 0;
     for (int w = 0; w < warp; ++w) before += part[w][lane];
     if (g >= width) return;
-    for (int c = begin; c < end; ++c) {
-        int32_t* at = table + (long long)c * width + g;
-        const int here = *at;
-        *at = before;
-        before += here;
+    for (int c0 = begin; c0 < end; c0 += 8) {
+        int here[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) here[i] = c0 + i < end ? table[(long long)(c0 + i) * width + g] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (c0 + i < end) table[(long long)(c0 + i) * width + g] = before;
+            before += here[i];
+        }
     }
     if (warp == 31) totals[g] = before;
 }
 
-// starts[g] = sum of totals[0 .. g) for g <= width, by the whole CTA; `totals` and `starts` may be the same array
-__device__ __forceinline__ void exclusive_starts(const int* totals, int* starts, int width) {
-    __shared__ int warp_sum_of[kWarps];
-    const int per = (width + kThreads - 1) / kThreads, begin = threadIdx.x * per, end = min(width, begin + per);
-    int sum = 0;
-    for (int i = begin; i < end; ++i) sum += totals[i];
-    int inclusive = sum;
+// starts[g] = sum of starts[0 .. g) for g < width, by the whole CTA
+__device__ __forceinline__ void exclusive_starts(int* starts, int width) {
+    __shared__ int warp_total[kWarps];
+    const int per = (width + kThreads - 1) / kThreads, begin = min(width, (int)threadIdx.x * per), end = min(width, begin + per);
+    int sum = 0, all;
+    for (int i = begin; i < end; ++i) sum += starts[i];
+    int before = warps_before(sum, all);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, inclusive, o);
-        if (lane >= o) inclusive += up;
-    }
-    if (lane == 31) warp_sum_of[warp] = inclusive;
+    if (lane == 31) warp_total[warp] = all;
     __syncthreads();
-    int before = inclusive - sum;
-    for (int w = 0; w < warp; ++w) before += warp_sum_of[w];
+    int ahead = lane < warp ? warp_total[lane] : 0;
+    before += warp_sum(ahead);
     for (int i = begin; i < end; ++i) {
-        const int here = totals[i];
+        const int here = starts[i];
         starts[i] = before;
         before += here;
     }
@@ -112,48 +136,55 @@ k_group_place(const K* __restrict__ keys, long long rows, int groups, const int3
     extern __shared__ int counts[];                       // [kWarps][groups + 1], then [groups + 1] starts
     const int width = groups + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int* const starts = counts + kWarps * width;
+    const long long begin = (long long)blockIdx.x * kRowsPerCta + warp * kRowsPerWarp;
+    int g[kKeys];
+    load_keys(keys, begin, rows, groups, g);
     for (int i = threadIdx.x; i < kWarps * width; i += kThreads) counts[i] = 0;
+    if (!ALONE)
+        for (int q = threadIdx.x; q < width; q += kThreads) starts[q] = totals[q];
     __syncthreads();
-    const long long begin = (long long)blockIdx.x * kRowsPerCta + warp * kRowsPerWarp, end = min(rows, begin + kRowsPerWarp);
-    count_warp(keys, begin, end, groups, counts + warp * width);
+    count_warp(g, counts + warp * width);
     __syncthreads();
-    for (int g = threadIdx.x; g < width; g += kThreads) {
-        int sum = 0;
-        for (int w = 0; w < kWarps; ++w) {
-            const int here = counts[w * width + g];
-            counts[w * width + g] = sum;
-            sum += here;
-        }
-        starts[g] = ALONE ? sum : totals[g];
+    for (int q = warp; q < width; q += kWarps) {
+        int all;
+        const int before = warps_before(counts[lane * width + q], all);
+        counts[lane * width + q] = before;
+        if (ALONE && lane == 0) starts[q] = all;
     }
     __syncthreads();
-    exclusive_starts(starts, starts, width);
+    exclusive_starts(starts, width);
     if (blockIdx.x == 0)
-        for (int g = threadIdx.x; g < width; g += kThreads) offsets[g] = starts[g];
-    for (int g = threadIdx.x; g < width; g += kThreads) {
-        const int first = starts[g] + (ALONE ? 0 : table[(long long)blockIdx.x * width + g]);
-        for (int w = 0; w < kWarps; ++w) counts[w * width + g] += first;
+        for (int q = threadIdx.x; q < width; q += kThreads) offsets[q] = starts[q];
+    if (!ALONE) {
+        for (int q = threadIdx.x; q < width; q += kThreads) starts[q] += table[(long long)blockIdx.x * width + q];
+        __syncthreads();
     }
-    __syncthreads();
     int* const next = counts + warp * width;
-    for (long long row = begin + lane; row - lane < end; row += 32) {
-        const int g = row < end ? group_of(keys, row, groups) : -1;
-        const unsigned same = __match_any_sync(0xffffffffu, g);
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+        const unsigned same = __match_any_sync(0xffffffffu, g[i]);
         const int rank = __popc(same & ((1u << lane) - 1u));
-        const int base = g >= 0 ? next[g] : 0;
+        const int base = g[i] >= 0 ? next[g[i]] : 0;
         __syncwarp();
-        if (g >= 0) {
-            order[base + rank] = (int32_t)row;
-            if (rank == 0) next[g] = base + __popc(same);
+        if (g[i] >= 0) {
+            order[starts[g[i]] + base + rank] = (int32_t)(begin + 32 * i + lane);
+            if (rank == 0) next[g[i]] = base + __popc(same);
         }
         __syncwarp();
     }
 }
 
+constexpr int kMostSmem = (kWarps + 1) * (FMB_MAX_GROUPS + 1) * 4;
+
 template <typename K>
 int group_rows(const K* keys, long long rows, int groups, int32_t* order, int32_t* offsets, int32_t* scratch, cudaStream_t stream) {
     const int width = groups + 1, ctas = ceil_div(rows, kRowsPerCta);
     const int smem = (kWarps + 1) * width * (int)sizeof(int);
+    if (smem > 48 * 1024) {
+        FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, true>, kMostSmem));
+        FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, false>, kMostSmem));
+        FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_count<K>, kMostSmem));
+    }
     if (ctas <= 1) {
         k_group_place<K, true><<<1, kThreads, smem, stream>>>(keys, rows, groups, nullptr, nullptr, order, offsets);
         FMB_LAUNCH_CHECK();

@@ -79,10 +79,11 @@ def _on_device(what: str, *tensors: torch.Tensor) -> int:
 
 def _launch(index: int, call, *arguments):
     """``call(*arguments, stream)`` with the device current and its current stream."""
+    stream = torch._C._cuda_getCurrentRawStream(index)       # what torch.cuda.current_stream holds, a twentieth of its time
     if torch.cuda.current_device() == index:
-        return call(*arguments, torch.cuda.current_stream().cuda_stream)
+        return call(*arguments, stream)
     with torch.cuda.device(index):
-        return call(*arguments, torch.cuda.current_stream().cuda_stream)
+        return call(*arguments, stream)
 
 
 def group_rows(keys: torch.Tensor, n_groups: int) -> RowGroups:
