@@ -38,7 +38,13 @@ k_sum_units(fmb_grouped_t a, int unit_rows) {
     if (i >= size) return;
     const float* at = a.scratch + first[0] * size + i;
     float sum = 0.0f;
-    for (int u = 0; u < first[1]; ++u, at += size) sum += *at;
+    for (int u = 0; u < first[1]; u += 8) {
+        float v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = u + j < first[1] ? at[(u + j) * size] : 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum += v[j];
+    }
     float* const out = (float*)a.w + g * a.w_group_stride + (i / a.n) * a.w_row_stride + i % a.n;
     *out = a.accumulate ? *out + sum : sum;
 }

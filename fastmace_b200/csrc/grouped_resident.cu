@@ -213,16 +213,15 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
         for (int t = t_begin + set, n = set; t < t_end; t += 2, n += 2) {
             if (n == 0 || w.leads()) {
                 // other weights: nobody reads the old ones once the tile before, the other set's, has its accumulators
-                if (n > 0) alive = mbar_wait(acc_full(set ^ 1), ((n - 1) >> 1) & 1, abort_flag, kSpin);
-                if (!alive) break;
+                if (n > 0) mbar_wait(acc_full(set ^ 1), ((n - 1) >> 1) & 1, abort_flag, kSpin);
                 fence_after_sync();
                 bring_weights<MODE>(p, w, w.feature0 + id, depth, tmem + lanes);
                 fence_before_sync();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(w_full);
             }
-            alive = mbar_wait(acc_full(set), (n >> 1) & 1, abort_flag, kSpin);
-            if (!alive) break;
+            // (one that runs out does not end the loop: the set's warps meet at barriers, and all have to come)
+            mbar_wait(acc_full(set), (n >> 1) & 1, abort_flag, kSpin);
             fence_after_sync();
             const uint32_t main = tmem + lanes + kAccumulators + set * 2 * kTN;
             const int low = row_low, high = row_high, feature0 = w.feature0;

@@ -23,23 +23,36 @@ namespace {
 
 using namespace tc;
 
-constexpr int kProducerWarps = 4, kEpilogueWarps = 8;
-constexpr int kThreads = 32 * (kProducerWarps + kEpilogueWarps);
+constexpr int kEpilogueWarps = 8;
 constexpr int kChunk = 512;                      // weight gradient: depth after which an accumulator moves to registers
 
-template <int TN> struct Shape {
+template <int MODE, int TN> struct Shape {
+    static constexpr bool kWeights = MODE == kWeightGradient;
     static constexpr int kFeatureBytes = 128 * kDepth * 2, kRowBytes = TN * kDepth * 2;
     static constexpr int kStageBytes = kFeatureBytes + kRowBytes;
-    static constexpr int kStages = (200 * 1024) / kStageBytes < 8 ? (200 * 1024) / kStageBytes : 8;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + (FMB_MAX_GROUPS + 1) * 4 + 256;
+    // Warps that issue copies: of the linears warp 0 for the features, the others for rows, 32 each; of the weight gradient one
+    // per 64 columns of y or x. One warp takes 30 cycles a gather, and 64 (96) of them feed 512 cycles of MMAs. Then the warp
+    // that issues MMAs, and eight that take results out, two sets of four.
+    static constexpr int kGathers = kWeights ? 2 + TN / 64 : TN / 32, kCopyWarps = kWeights ? kGathers : 1 + kGathers;
+    static constexpr int kMmaWarp = kCopyWarps;
+    static constexpr int kFirstEpilogue = kWeights ? 8 : kMmaWarp + 1;             // whole warpgroups, so that registers can be dealt
+    static constexpr int kThreads = 32 * (kFirstEpilogue + kEpilogueWarps);
+    // results turn through shared memory, 32 rows of 128 features at a time and set
+    static constexpr int kTurnBytes = 32 * 128 * (kWeights ? 4 : 2);
+    static constexpr int kRoom = 226 * 1024 - 2 * kTurnBytes - 1024 - (FMB_MAX_GROUPS + 1) * 4 - 256 - kCopyWarps * 256;
+    static constexpr int kStages = kRoom / kStageBytes < 8 ? kRoom / kStageBytes : 8;
+    static constexpr int kTurn0 = kStages * kStageBytes, kRows0 = kTurn0 + 2 * kTurnBytes, kUnits0 = kRows0 + kCopyWarps * 256,
+                         kBars0 = kUnits0 + ((FMB_MAX_GROUPS + 1) * 4 + 7) / 8 * 8;
+    static constexpr int kSmem = 1024 + kBars0 + 256;
     static constexpr int kTmem = 2 * TN < 32 ? 32 : 2 * TN;
+    static_assert(kStages >= 3 && kSmem <= 227 * 1024 && kMmaWarp < kFirstEpilogue, "fits an SM");
 };
 
 struct Args {
     fmb_grouped_t a;
     int feature_tiles, row_tiles;                // of the output; row_tiles 1 where rows are gathered
     int unit_rows;                               // entries of a group per unit
-    int wide_store;                              // output rows may be written 4 bytes at a time
+    int wide_store;                              // output rows may be written 16 bytes at a time
 };
 
 __device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
@@ -47,20 +60,14 @@ __device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map
                  :: "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
 
-// a row number that TMA fills with zeros stands for everything that is no row
-__device__ __forceinline__ int row_at(const Args& p, int entry, int end) {
-    const int row = entry < end ? __ldg(p.a.order + entry) : p.a.rows;
-    return (unsigned)row < (unsigned)p.a.rows ? row : p.a.rows;
-}
-
 template <typename T, int MODE, int TN>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Shape<MODE, TN>::kThreads, 1)
 k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap feature_map, const __grid_constant__ CUtensorMap row_map) {
-    using S = Shape<TN>;
+    using S = Shape<MODE, TN>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    int* const first_unit = reinterpret_cast<int*>(smem + S::kStages * S::kStageBytes);
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::kStages * S::kStageBytes + ((FMB_MAX_GROUPS + 1) * 4 + 7) / 8 * 8);
+    int* const first_unit = reinterpret_cast<int*>(smem + S::kUnits0);
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(smem + S::kBars0);
     uint32_t* const tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::kStages + 4);
     volatile int* const abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const uint32_t bar0 = smem_u32(bars), stage0 = smem_u32(smem);
@@ -69,13 +76,13 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     auto acc_full = [&](int b) { return bar0 + 8u * (2 * S::kStages + b); };
     auto acc_empty = [&](int b) { return bar0 + 8u * (2 * S::kStages + 2 + b); };
     const int warp = uniform_warp(), lane = threadIdx.x & 31;
-    constexpr bool kWeights = MODE == kWeightGradient;
-    constexpr int kGatherWarps = 2;              // bring the rows of the output; warp 0 brings the features, warp 3 issues the MMAs
+    constexpr bool kWeights = S::kWeights;
+    constexpr int kMmaWarp = S::kMmaWarp;
 
     if (warp == 0) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
-    if (warp == 3 && elect_one()) {
+    if (warp == kMmaWarp && elect_one()) {
         for (int s = 0; s < S::kStages; ++s) {
-            mbar_init(full(s), 1 + kGatherWarps);
+            mbar_init(full(s), S::kCopyWarps);
             mbar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -85,7 +92,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    count_units<kThreads>(p.a.offsets, p.a.groups, p.a.rows, p.unit_rows, kWeights ? 1 : 0, first_unit);
+    count_units<S::kThreads>(p.a.offsets, p.a.groups, p.a.rows, p.unit_rows, kWeights ? 1 : 0, first_unit);
     fence_before_sync();
     __syncthreads();
     fence_after_sync();
@@ -94,109 +101,116 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n;        // not of the weight gradient
 
     Walk w(p.a, first_unit, p.unit_rows, p.feature_tiles, p.row_tiles, TN);
+    if constexpr (kWeights) {
+        // eight warps with 56 registers a thread, eight with 200: 256 x 256 as at the launch
+        if (warp < 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    }
 
-    if (warp < 3) {
-        // ---------------------------------------------------------------- producers
+    if (warp < S::kCopyWarps) {
+        // ---------------------------------------------------------------- copies
         int at = 0;
         uint32_t phase = 0;
-        const int part = warp - 1;               // of the gather
         bool alive = true;
+        // The row numbers of this warp's gathers, in shared memory: read four at a time at an address the whole warp shares,
+        // they get to the gather on the short way (with shuffles 47 cycles a gather, lanes that issue their own 62).
+        int4* const rows = reinterpret_cast<int4*>(smem + S::kRows0 + warp * 256);
+        int* const my_rows = reinterpret_cast<int*>(rows) + 2 * lane;
+        auto row_or_zeros = [&](int entry, int end) {
+            const int row = row_at(p, entry, end);
+            return row < 0 ? p.a.rows : row;               // TMA fills what is past the last row with zeros
+        };
         for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
             if (t == (int)blockIdx.x) w.start(t);
             else w.step(gridDim.x);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
             const int end = w.first + w.count;
-            // rows of the output this warp gathers: lane l holds the row numbers 4 (part * TN / 8 + l) and on
-            int rows[4];
-            constexpr int kPerWarp = TN / 4 / kGatherWarps;
-            if (!kWeights && warp > 0) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) rows[i] = lane < kPerWarp ? row_at(p, w.first + 4 * (part * kPerWarp + lane) + i, end) : 0;
-            }
-            int next[4];
-            if (kWeights) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) next[i] = row_at(p, w.first + 4 * (lane & 15) + i, end);
-            }
-            for (int b = 0; b < blocks; ++b) {
-                const int d0 = b * kDepth;
-                if (kWeights) {
-                    // the depths of this block, and those of the next on their way
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        rows[i] = next[i];
-                        next[i] = row_at(p, w.first + d0 + kDepth + 4 * (lane & 15) + i, end);
-                    }
-                }
-                alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
-                if (!alive) break;
-                const uint32_t base = stage0 + at * S::kStageBytes, bar = full(at);
-                // depths past the end are filled with zeros up to a multiple of 16
-                const int quads = kWeights ? min(16, (w.count - d0 + 15) / 16 * 4) : 0;
-                if (warp == 0) {
-                    if constexpr (kWeights) {
-                        if (elect_one()) mbar_expect_tx(bar, quads * 2 * 512);
-                        __syncwarp();
-                        for (int q = 0; q < quads; ++q) {
-                            const int r0 = __shfl_sync(0xffffffffu, rows[0], q), r1 = __shfl_sync(0xffffffffu, rows[1], q);
-                            const int r2 = __shfl_sync(0xffffffffu, rows[2], q), r3 = __shfl_sync(0xffffffffu, rows[3], q);
-                            if (elect_one()) {
-                                tma_gather4(base + q * 512, &feature_map, w.feature0, r0, r1, r2, r3, bar);
-                                tma_gather4(base + 8192 + q * 512, &feature_map, w.feature0 + 64, r0, r1, r2, r3, bar);
-                            }
-                            __syncwarp();
-                        }
-                    } else if (elect_one()) {
-                        mbar_expect_tx(bar, S::kFeatureBytes);
-                        if constexpr (MODE == kLinear) {
-                            tma_tile_3d(base, &feature_map, w.feature0, d0, w.g, bar);
-                            tma_tile_3d(base + 8192, &feature_map, w.feature0 + 64, d0, w.g, bar);
-                        } else {
-                            tma_tile_3d(base, &feature_map, d0, w.feature0, w.g, bar);
-                        }
+            if constexpr (!kWeights) {
+                if (warp > 0) {
+                    const int quads = min(8, max(0, (w.count + 3) / 4 - (warp - 1) * 8));
+                    __syncwarp();
+                    if (lane < 16) {
+                        my_rows[0] = row_or_zeros(w.first + (warp - 1) * 32 + 2 * lane, end);
+                        my_rows[1] = row_or_zeros(w.first + (warp - 1) * 32 + 2 * lane + 1, end);
                     }
                     __syncwarp();
-                } else if constexpr (kWeights) {
-                    constexpr int kChunks = TN / 64 / kGatherWarps;          // of 64 output rows
-                    const uint32_t dst = base + S::kFeatureBytes + part * kChunks * 8192;
-                    if (elect_one()) mbar_expect_tx(bar, quads * kChunks * 512);
-                    __syncwarp();
-                    for (int q = 0; q < quads; ++q) {
-                        const int r0 = __shfl_sync(0xffffffffu, rows[0], q), r1 = __shfl_sync(0xffffffffu, rows[1], q);
-                        const int r2 = __shfl_sync(0xffffffffu, rows[2], q), r3 = __shfl_sync(0xffffffffu, rows[3], q);
+                    for (int b = 0; b < blocks; ++b) {
+                        alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
+                        if (!alive) break;
+                        const uint32_t dst = stage0 + at * S::kStageBytes + S::kFeatureBytes + (warp - 1) * 8 * 512, bar = full(at);
                         if (elect_one()) {
+                            if (quads) mbar_expect_tx(bar, quads * 512);
+                            else mbar_arrive(bar);
 #pragma unroll
-                            for (int c = 0; c < kChunks; ++c)
-                                tma_gather4(dst + c * 8192 + q * 512, &row_map, w.row0 + (part * kChunks + c) * 64, r0, r1, r2, r3, bar);
+                            for (int q = 0; q < 8; ++q) {
+                                const int4 r = rows[q];
+                                if (q < quads) tma_gather4(dst + q * 512, &row_map, b * kDepth, r.x, r.y, r.z, r.w, bar);
+                            }
                         }
                         __syncwarp();
+                        if (++at == S::kStages) {
+                            at = 0;
+                            phase ^= 1;
+                        }
                     }
                 } else {
-                    const int mine = min(kPerWarp, max(0, (w.count + 3) / 4 - part * kPerWarp));
-                    const uint32_t dst = base + S::kFeatureBytes + part * kPerWarp * 512;
-                    if (elect_one()) {
-                        if (mine) mbar_expect_tx(bar, mine * 512);
-                        else mbar_arrive(bar);
-                    }
-                    __syncwarp();
-                    for (int q = 0; q < mine; ++q) {
-                        const int r0 = __shfl_sync(0xffffffffu, rows[0], q), r1 = __shfl_sync(0xffffffffu, rows[1], q);
-                        const int r2 = __shfl_sync(0xffffffffu, rows[2], q), r3 = __shfl_sync(0xffffffffu, rows[3], q);
-                        if (elect_one()) tma_gather4(dst + q * 512, &row_map, d0, r0, r1, r2, r3, bar);
+                    for (int b = 0; b < blocks; ++b) {
+                        alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
+                        if (!alive) break;
+                        const uint32_t dst = stage0 + at * S::kStageBytes, bar = full(at);
+                        if (elect_one()) {
+                            mbar_expect_tx(bar, S::kFeatureBytes);
+                            if constexpr (MODE == kLinear) {
+                                tma_tile_3d(dst, &feature_map, w.feature0, b * kDepth, w.g, bar);
+                                tma_tile_3d(dst + 8192, &feature_map, w.feature0 + 64, b * kDepth, w.g, bar);
+                            } else {
+                                tma_tile_3d(dst, &feature_map, b * kDepth, w.feature0, w.g, bar);
+                            }
+                        }
                         __syncwarp();
+                        if (++at == S::kStages) {
+                            at = 0;
+                            phase ^= 1;
+                        }
                     }
                 }
-                if (++at == S::kStages) {
-                    at = 0;
-                    phase ^= 1;
+            } else {
+                const CUtensorMap* const map = warp < 2 ? &feature_map : &row_map;
+                const int column = warp < 2 ? w.feature0 + warp * 64 : w.row0 + (warp - 2) * 64;
+                int next0 = row_or_zeros(w.first + 2 * lane, end), next1 = row_or_zeros(w.first + 2 * lane + 1, end);
+                for (int b = 0; b < blocks; ++b) {
+                    // the depths of this block, and those of the next on their way
+                    __syncwarp();
+                    my_rows[0] = next0;
+                    my_rows[1] = next1;
+                    next0 = row_or_zeros(w.first + (b + 1) * kDepth + 2 * lane, end);
+                    next1 = row_or_zeros(w.first + (b + 1) * kDepth + 2 * lane + 1, end);
+                    __syncwarp();
+                    alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
+                    if (!alive) break;
+                    const uint32_t dst = stage0 + at * S::kStageBytes + warp * 8192, bar = full(at);
+                    const int quads = min(16, (w.count - b * kDepth + 15) / 16 * 4);     // depths past the end, up to a multiple of 16, are zeros
+                    if (elect_one()) {
+                        mbar_expect_tx(bar, quads * 512);
+#pragma unroll 4
+                        for (int q = 0; q < quads; ++q) {
+                            const int4 r = rows[q];
+                            tma_gather4(dst + q * 512, map, column, r.x, r.y, r.z, r.w, bar);
+                        }
+                    }
+                    __syncwarp();
+                    if (++at == S::kStages) {
+                        at = 0;
+                        phase ^= 1;
+                    }
                 }
             }
         }
-    } else if (warp == 3) {
+    } else if (warp == kMmaWarp) {
         // ---------------------------------------------------------------- MMAs
         int at = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
-        constexpr uint32_t kType = sizeof(T) == 2 && __is_same(T, __nv_bfloat16) ? 1 : 0;
+        constexpr uint32_t kType = __is_same(T, __nv_bfloat16) ? 1 : 0;
         constexpr uint32_t kMajor = MODE == kLinear ? 1u << 15 : MODE == kWeightGradient ? 3u << 15 : 0;
         constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | kMajor | ((uint32_t)(128 >> 4) << 24);
         bool alive = true;
@@ -237,43 +251,30 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 }
             }
         }
-    } else {
-        // ---------------------------------------------------------------- epilogue
-        const int ew = warp - kProducerWarps, quarter = ew & 3, half = ew >> 2;      // lanes 32 quarter + [0, 32), half of the columns
+    } else if (warp >= S::kFirstEpilogue) {
+        // ---------------------------------------------------------------- results
+        const int quarter = warp & 3, set = (warp - S::kFirstEpilogue) >> 2, id = quarter * 32 + lane;     // lanes 32 quarter + [0, 32)
         int acc = 0;
         uint32_t acc_phase = 0;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        const int width = MODE == kInputGradient ? p.a.k : p.a.n;
-        if (!kWeights && p.a.zero_rest) {
-            // rows of no group
-            T* const out = (T*)(MODE == kLinear ? p.a.y : p.a.x);
-            const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
-            const int from = min(max(p.a.offsets[p.a.groups], 0), p.a.rows);
-            for (int i = from + blockIdx.x * kEpilogueWarps + ew; i < p.a.rows; i += gridDim.x * kEpilogueWarps) {
-                const int row = row_at(p, i, p.a.rows);
-                if (row < p.a.rows)
-                    for (int c = lane; c < width; c += 32) out[row * stride + c] = from_float<T>(0.0f);
-            }
-        }
-        bool alive = true;
-        for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
-            if (t == (int)blockIdx.x) w.start(t);
-            else w.step(gridDim.x);
-            const int feature = w.feature0 + quarter * 32 + lane;
-            if constexpr (kWeights) {
-                constexpr int kCols = TN / 2;
+        // a wait that runs out does not end these loops: the set's warps meet at barriers, and all have to come
+        if constexpr (kWeights) {
+            constexpr int kCols = TN / 2;                        // of a set
+            float* const turn = reinterpret_cast<float*>(smem + S::kTurn0 + set * S::kTurnBytes);
+            for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+                if (t == (int)blockIdx.x) w.start(t);
+                else w.step(gridDim.x);
                 const int chunks = (w.count + kChunk - 1) / kChunk;
                 float sum[kCols];
 #pragma unroll
                 for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
                 for (int c = 0; c < chunks; ++c) {
-                    alive = mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
-                    if (!alive) break;
+                    mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
                     fence_after_sync();
 #pragma unroll
                     for (int j0 = 0; j0 < kCols; j0 += 32) {
                         float v[32];
-                        tmem_load_32(tmem + lanes + acc * TN + half * kCols + j0, v);
+                        tmem_load_32(tmem + lanes + acc * TN + set * kCols + j0, v);
 #pragma unroll
                         for (int j = 0; j < 32; ++j) sum[j0 + j] += v[j];
                     }
@@ -285,46 +286,85 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 }
                 const bool direct = w.units <= 1;
                 const long long stride = direct ? p.a.w_row_stride : p.a.n;
+                const int feature = w.feature0 + 4 * lane, live = p.a.n - feature;
                 float* const out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + (long long)w.unit * p.a.k * p.a.n) + feature;
-                const int row0 = w.row0 + half * kCols;
-                if (feature < p.a.n) {
+                const bool add = direct && p.a.accumulate, wide = direct ? p.wide_store : p.a.n % 4 == 0;
+                const int row0 = w.row0 + set * kCols;
 #pragma unroll
-                    for (int j = 0; j < kCols; ++j) {
-                        if (row0 + j >= p.a.k) break;
-                        float* const at = out + (row0 + j) * stride;
-                        *at = direct && p.a.accumulate ? *at + sum[j] : sum[j];
+                for (int j0 = 0; j0 < kCols; j0 += 32) {
+                    named_barrier(1 + set, 128);                  // what was here has been read
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) turn[j * 128 + id] = sum[j0 + j];
+                    named_barrier(1 + set, 128);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int r = j * 4 + quarter, row = row0 + j0 + r;
+                        float4 v = *reinterpret_cast<const float4*>(turn + r * 128 + 4 * lane);
+                        if (row >= p.a.k) continue;
+                        float* const to = out + row * stride;
+                        if (wide) {
+                            if (live > 0) {
+                                if (add) {
+                                    const float4 old = *reinterpret_cast<const float4*>(to);
+                                    v.x += old.x; v.y += old.y; v.z += old.z; v.w += old.w;
+                                }
+                                *reinterpret_cast<float4*>(to) = v;
+                            }
+                        } else {
+                            if (live > 0) to[0] = add ? to[0] + v.x : v.x;
+                            if (live > 1) to[1] = add ? to[1] + v.y : v.y;
+                            if (live > 2) to[2] = add ? to[2] + v.z : v.z;
+                            if (live > 3) to[3] = add ? to[3] + v.w : v.w;
+                        }
                     }
                 }
-            } else {
-                T* const out = (T*)(MODE == kLinear ? p.a.y : p.a.x);
-                const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
-                alive = mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
-                if (!alive) break;
+            }
+        } else {
+            T* const out = (T*)(MODE == kLinear ? p.a.y : p.a.x);
+            const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
+            const int width = MODE == kLinear ? p.a.n : p.a.k;
+            T* const turn = reinterpret_cast<T*>(smem + S::kTurn0 + set * S::kTurnBytes);      // [32 rows][128 features]
+            if (p.a.zero_rest) {
+                // rows of no group
+                const int from = min(max(p.a.offsets[p.a.groups], 0), p.a.rows), first = blockIdx.x * kEpilogueWarps + warp - S::kFirstEpilogue;
+                for (int i = from + first; i < p.a.rows; i += gridDim.x * kEpilogueWarps) {
+                    const int row = row_at(p, i, p.a.rows);
+                    if (row >= 0)
+                        for (int c = lane; c < width; c += 32) out[row * stride + c] = from_float<T>(0.0f);
+                }
+            }
+            for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+                if (t == (int)blockIdx.x) w.start(t);
+                else w.step(gridDim.x);
+                mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
                 fence_after_sync();
-                // the halves take turns at blocks of 32 columns
+                const int feature = w.feature0 + 8 * (lane & 15), live = width - feature;
+                // the sets take turns at blocks of 32 rows
 #pragma unroll 1
-                for (int j0 = half * 32; j0 < w.count; j0 += 64) {
+                for (int j0 = set * 32; j0 < w.count; j0 += 64) {
+                    const int mine = row_at(p, w.first + j0 + lane, w.first + w.count);
                     float v[32];
                     tmem_load_32(tmem + lanes + acc * TN + j0, v);
-                    const int row = row_at(p, w.first + j0 + lane, w.first + w.count);
-                    if (p.wide_store) {
-                        // a lane and its neighbour exchange a value, so that each holds two features of one row
-                        const int odd = lane & 1;
-                        T* const at = out + (feature - odd);
+                    named_barrier(1 + set, 128);                  // what was here has been read
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
-                            const int r0 = __shfl_sync(0xffffffffu, row, j), r1 = __shfl_sync(0xffffffffu, row, j + 1);
-                            const int r = odd ? r1 : r0;
-                            const T two[2] = {from_float<T>(odd ? got : v[j]), from_float<T>(odd ? v[j + 1] : got)};
-                            if (r < p.a.rows && feature - odd < width)
-                                *reinterpret_cast<uint32_t*>(at + r * stride) = *reinterpret_cast<const uint32_t*>(two);
-                        }
-                    } else {
+                    for (int j = 0; j < 32; ++j) turn[j * 128 + id] = from_float<T>(v[j]);
+                    named_barrier(1 + set, 128);
+                    uint4 q[4];
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int r = __shfl_sync(0xffffffffu, row, j);
-                            if (r < p.a.rows && feature < width) out[r * stride + feature] = from_float<T>(v[j]);
+                    for (int j = 0; j < 4; ++j)
+                        q[j] = *reinterpret_cast<const uint4*>(turn + (j * 8 + quarter * 2 + (lane >> 4)) * 128 + 8 * (lane & 15));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int row = __shfl_sync(0xffffffffu, mine, j * 8 + quarter * 2 + (lane >> 4));
+                        T* const to = out + row * stride + feature;
+                        if (row < 0) continue;
+                        if (p.wide_store) {
+                            if (live > 0) *reinterpret_cast<uint4*>(to) = q[j];
+                        } else {
+                            const T* const each = reinterpret_cast<const T*>(&q[j]);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (i < live) to[i] = each[i];
                         }
                     }
                 }
@@ -368,9 +408,9 @@ Encode encoder() {
 
 template <typename T, int MODE, int TN>
 int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, long long tiles, cudaStream_t stream) {
-    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN>, Shape<TN>::kSmem));
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN>, Shape<MODE, TN>::kSmem));
     const int grid = (int)std::min<long long>(tiles, sm_count());
-    k_grouped_tc<T, MODE, TN><<<grid, kThreads, Shape<TN>::kSmem, stream>>>(p, features, rows);
+    k_grouped_tc<T, MODE, TN><<<grid, Shape<MODE, TN>::kThreads, Shape<MODE, TN>::kSmem, stream>>>(p, features, rows);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
@@ -417,8 +457,8 @@ int tma_typed(const fmb_grouped_t* a, Mode mode, const CUtensorMap& features, co
     Args p;
     p.a = *a;
     p.row_tiles = 1;
-    p.wide_store = 0;
     if (mode == kWeightGradient) {
+        p.wide_store = four_at_a_time(a->w, a->w_row_stride, 4) && a->w_group_stride % 4 == 0 && a->n % 4 == 0;
         int tn;
         weight_plan(a, tn, p.unit_rows);
         p.feature_tiles = ceil_div(a->n, 128);
@@ -433,7 +473,7 @@ int tma_typed(const fmb_grouped_t* a, Mode mode, const CUtensorMap& features, co
     const int width = forward ? a->n : a->k;
     const void* out = forward ? a->y : a->x;
     p.feature_tiles = ceil_div(width, 128);
-    p.wide_store = ((uintptr_t)out & 3) == 0 && (forward ? a->y_stride : a->x_stride) % 2 == 0 && width % 2 == 0;
+    p.wide_store = ((uintptr_t)out & 15) == 0 && (forward ? a->y_stride : a->x_stride) % 8 == 0 && width % 8 == 0;
     return forward ? launch_rows<T, kLinear>(p, features, rows, stream) : launch_rows<T, kInputGradient>(p, features, rows, stream);
 }
 

@@ -122,7 +122,9 @@ struct Walk {
     __device__ __forceinline__ bool leads() const { return unit == first_unit[g]; }
 };
 
-__device__ __forceinline__ int row_at(const SplitArgs& p, int entry, int end) {
+// the row that `entry` of the order names; -1 where there is none
+template <typename ARGS>
+__device__ __forceinline__ int row_at(const ARGS& p, int entry, int end) {
     const int row = entry < end ? __ldg(p.a.order + entry) : -1;
     return (unsigned)row < (unsigned)p.a.rows ? row : -1;
 }
