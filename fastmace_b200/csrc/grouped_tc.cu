@@ -26,14 +26,16 @@ using namespace tc;
 constexpr int kEpilogueWarps = 8;
 constexpr int kChunk = 512;                      // weight gradient: depth after which an accumulator moves to registers
 
-template <int MODE, int TN> struct Shape {
+template <int MODE, int TN, bool PAIR> struct Shape {
     static constexpr bool kWeights = MODE == kWeightGradient;
-    static constexpr int kFeatureBytes = 128 * kDepth * 2, kRowBytes = TN * kDepth * 2;
+    static constexpr int kCtas = PAIR ? 2 : 1, kRows = TN / kCtas;                 // rows of the tile that a CTA brings
+    static constexpr int kFeatureBytes = 128 * kDepth * 2, kRowBytes = kRows * kDepth * 2;
     static constexpr int kStageBytes = kFeatureBytes + kRowBytes;
+    static constexpr int kRowsPerWarp = PAIR ? 16 : 32, kQuads = kRowsPerWarp / 4;
     // Warps that issue copies: of the linears warp 0 for the features, the others for rows, 32 each; of the weight gradient one
     // per 64 columns of y or x. One warp takes 30 cycles a gather, and 64 (96) of them feed 512 cycles of MMAs. Then the warp
     // that issues MMAs, and eight that take results out, two sets of four.
-    static constexpr int kGathers = kWeights ? 2 + TN / 64 : TN / 32, kCopyWarps = kWeights ? kGathers : 1 + kGathers;
+    static constexpr int kGathers = kWeights ? 2 + kRows / 64 : kRows / kRowsPerWarp, kCopyWarps = kWeights ? kGathers : 1 + kGathers;
     static constexpr int kMmaWarp = kCopyWarps;
     static constexpr int kFirstEpilogue = kWeights ? 8 : kMmaWarp + 1;             // whole warpgroups, so that registers can be dealt
     static constexpr int kThreads = 32 * (kFirstEpilogue + kEpilogueWarps);
@@ -60,10 +62,10 @@ __device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map
                  :: "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
 
-template <typename T, int MODE, int TN>
-__global__ void __launch_bounds__(Shape<MODE, TN>::kThreads, 1)
+template <typename T, int MODE, int TN, bool PAIR>
+__global__ void __launch_bounds__(Shape<MODE, TN, PAIR>::kThreads, 1)
 k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap feature_map, const __grid_constant__ CUtensorMap row_map) {
-    using S = Shape<MODE, TN>;
+    using S = Shape<MODE, TN, PAIR>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     int* const first_unit = reinterpret_cast<int*>(smem + S::kUnits0);
@@ -79,15 +81,43 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     constexpr bool kWeights = S::kWeights;
     constexpr int kMmaWarp = S::kMmaWarp;
 
-    if (warp == 0) tmem_alloc(smem_u32(tmem_slot), S::kTmem);
+    // of a pair: CTA 0 leads; both walk the same tiles, each with its own 128 features and half of the rows to bring
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0, t_first = blockIdx.x / S::kCtas, t_step = gridDim.x / S::kCtas;
+    auto copy_bar = [&](int s) { return PAIR ? in_leader(full(s)) : full(s); };
+    auto expect = [&](uint32_t bar, uint32_t bytes) {
+        if constexpr (PAIR) {
+            if (bytes) remote_expect_tx(bar, bytes);
+            else remote_arrive(bar);
+        } else {
+            if (bytes) mbar_expect_tx(bar, bytes);
+            else mbar_arrive(bar);
+        }
+    };
+    auto gather = [&](uint32_t dst, const CUtensorMap* map, int column, const int4& r, uint32_t bar) {
+        if constexpr (PAIR) tma_gather4_pair(dst, map, column, r.x, r.y, r.z, r.w, bar);
+        else tma_gather4(dst, map, column, r.x, r.y, r.z, r.w, bar);
+    };
+    auto box = [&](uint32_t dst, int c0, int c1, int c2, uint32_t bar) {
+        if constexpr (PAIR) tma_tile_3d_pair(dst, &feature_map, c0, c1, c2, bar);
+        else tma_tile_3d(dst, &feature_map, c0, c1, c2, bar);
+    };
+
+    if (warp == 0) {
+        if constexpr (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(smem_u32(tmem_slot)), "r"(S::kTmem) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            tmem_alloc(smem_u32(tmem_slot), S::kTmem);
+        }
+    }
     if (warp == kMmaWarp && elect_one()) {
         for (int s = 0; s < S::kStages; ++s) {
-            mbar_init(full(s), S::kCopyWarps);
+            mbar_init(full(s), S::kCopyWarps * S::kCtas);
             mbar_init(empty(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
-            mbar_init(acc_empty(b), kEpilogueWarps);
+            mbar_init(acc_empty(b), kEpilogueWarps * S::kCtas);
         }
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -95,6 +125,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     count_units<S::kThreads>(p.a.offsets, p.a.groups, p.a.rows, p.unit_rows, kWeights ? 1 : 0, first_unit);
     fence_before_sync();
     __syncthreads();
+    if constexpr (PAIR) cluster_sync();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const int tiles = first_unit[p.a.groups] * p.feature_tiles * p.row_tiles;
@@ -120,31 +151,33 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
             const int row = row_at(p, entry, end);
             return row < 0 ? p.a.rows : row;               // TMA fills what is past the last row with zeros
         };
-        for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
-            if (t == (int)blockIdx.x) w.start(t);
-            else w.step(gridDim.x);
+        for (int t = t_first; alive && t < tiles; t += t_step) {
+            if (t == t_first) w.start(t);
+            else w.step(t_step);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
-            const int end = w.first + w.count;
+            const int end = w.first + w.count, feature0 = w.feature0 * S::kCtas + rank * 128;
             if constexpr (!kWeights) {
                 if (warp > 0) {
-                    const int quads = min(8, max(0, (w.count + 3) / 4 - (warp - 1) * 8));
+                    // of a pair's MMA columns the first half are CTA 0's rows
+                    const int half = PAIR ? (w.count + 31) / 32 * 16 : TN, mine = min(half, max(0, w.count - rank * half));
+                    const int quads = min(S::kQuads, max(0, (mine + 3) / 4 - (warp - 1) * S::kQuads));
+                    const int entry = w.first + rank * half + (warp - 1) * S::kRowsPerWarp + 2 * lane;
                     __syncwarp();
-                    if (lane < 16) {
-                        my_rows[0] = row_or_zeros(w.first + (warp - 1) * 32 + 2 * lane, end);
-                        my_rows[1] = row_or_zeros(w.first + (warp - 1) * 32 + 2 * lane + 1, end);
+                    if (lane < S::kRowsPerWarp / 2) {
+                        my_rows[0] = row_or_zeros(entry, end);
+                        my_rows[1] = row_or_zeros(entry + 1, end);
                     }
                     __syncwarp();
                     for (int b = 0; b < blocks; ++b) {
                         alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
                         if (!alive) break;
-                        const uint32_t dst = stage0 + at * S::kStageBytes + S::kFeatureBytes + (warp - 1) * 8 * 512, bar = full(at);
+                        const uint32_t dst = stage0 + at * S::kStageBytes + S::kFeatureBytes + (warp - 1) * S::kQuads * 512, bar = copy_bar(at);
                         if (elect_one()) {
-                            if (quads) mbar_expect_tx(bar, quads * 512);
-                            else mbar_arrive(bar);
+                            expect(bar, quads * 512);
 #pragma unroll
-                            for (int q = 0; q < 8; ++q) {
+                            for (int q = 0; q < S::kQuads; ++q) {
                                 const int4 r = rows[q];
-                                if (q < quads) tma_gather4(dst + q * 512, &row_map, b * kDepth, r.x, r.y, r.z, r.w, bar);
+                                if (q < quads) gather(dst + q * 512, &row_map, b * kDepth, r, bar);
                             }
                         }
                         __syncwarp();
@@ -157,14 +190,14 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                     for (int b = 0; b < blocks; ++b) {
                         alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
                         if (!alive) break;
-                        const uint32_t dst = stage0 + at * S::kStageBytes, bar = full(at);
+                        const uint32_t dst = stage0 + at * S::kStageBytes, bar = copy_bar(at);
                         if (elect_one()) {
-                            mbar_expect_tx(bar, S::kFeatureBytes);
+                            expect(bar, S::kFeatureBytes);
                             if constexpr (MODE == kLinear) {
-                                tma_tile_3d(dst, &feature_map, w.feature0, b * kDepth, w.g, bar);
-                                tma_tile_3d(dst + 8192, &feature_map, w.feature0 + 64, b * kDepth, w.g, bar);
+                                box(dst, feature0, b * kDepth, w.g, bar);
+                                box(dst + 8192, feature0 + 64, b * kDepth, w.g, bar);
                             } else {
-                                tma_tile_3d(dst, &feature_map, b * kDepth, w.feature0, w.g, bar);
+                                box(dst, b * kDepth, feature0, w.g, bar);
                             }
                         }
                         __syncwarp();
@@ -176,7 +209,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 }
             } else {
                 const CUtensorMap* const map = warp < 2 ? &feature_map : &row_map;
-                const int column = warp < 2 ? w.feature0 + warp * 64 : w.row0 + (warp - 2) * 64;
+                const int column = warp < 2 ? feature0 + warp * 64 : w.row0 + rank * S::kRows + (warp - 2) * 64;
                 int next0 = row_or_zeros(w.first + 2 * lane, end), next1 = row_or_zeros(w.first + 2 * lane + 1, end);
                 for (int b = 0; b < blocks; ++b) {
                     // the depths of this block, and those of the next on their way
@@ -188,14 +221,14 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                     __syncwarp();
                     alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
                     if (!alive) break;
-                    const uint32_t dst = stage0 + at * S::kStageBytes + warp * 8192, bar = full(at);
+                    const uint32_t dst = stage0 + at * S::kStageBytes + warp * 8192, bar = copy_bar(at);
                     const int quads = min(16, (w.count - b * kDepth + 15) / 16 * 4);     // depths past the end, up to a multiple of 16, are zeros
                     if (elect_one()) {
-                        mbar_expect_tx(bar, quads * 512);
+                        expect(bar, quads * 512);
 #pragma unroll 4
                         for (int q = 0; q < quads; ++q) {
                             const int4 r = rows[q];
-                            tma_gather4(dst + q * 512, map, column, r.x, r.y, r.z, r.w, bar);
+                            gather(dst + q * 512, map, column, r, bar);
                         }
                     }
                     __syncwarp();
@@ -206,19 +239,20 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 }
             }
         }
-    } else if (warp == kMmaWarp) {
+    } else if (warp == kMmaWarp && rank == 0) {
         // ---------------------------------------------------------------- MMAs
         int at = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         constexpr uint32_t kType = __is_same(T, __nv_bfloat16) ? 1 : 0;
         constexpr uint32_t kMajor = MODE == kLinear ? 1u << 15 : MODE == kWeightGradient ? 3u << 15 : 0;
-        constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | kMajor | ((uint32_t)(128 >> 4) << 24);
+        constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | kMajor | ((uint32_t)(128 * S::kCtas >> 4) << 24);
         bool alive = true;
-        for (int t = blockIdx.x; alive && t < tiles; t += gridDim.x) {
-            if (t == (int)blockIdx.x) w.start(t);
-            else w.step(gridDim.x);
+        for (int t = t_first; alive && t < tiles; t += t_step) {
+            if (t == t_first) w.start(t);
+            else w.step(t_step);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
-            const int columns = kWeights ? TN : max(16, min(TN, (w.count + 15) / 16 * 16));
+            constexpr int kUnit = 16 * S::kCtas;
+            const int columns = kWeights ? TN : max(kUnit, min(TN, (w.count + kUnit - 1) / kUnit * kUnit));
             const uint32_t idesc = kDesc | ((uint32_t)(columns >> 3) << 17);
             for (int b = 0; b < blocks; ++b) {
                 const bool fresh = b == 0 || (kWeights && b % (kChunk / kDepth) == 0);
@@ -234,11 +268,17 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 if (elect_one()) {
                     for (int k = 0; k < steps; ++k) {
                         constexpr uint64_t kF = MODE == kInputGradient ? 2 : 128, kR = kWeights ? 128 : 2;
-                        mma_f16(d, fd + k * kF, rd + k * kR, idesc, k > 0 || !fresh);
+                        if constexpr (PAIR) mma_f16_pair(d, fd + k * kF, rd + k * kR, idesc, k > 0 || !fresh);
+                        else mma_f16(d, fd + k * kF, rd + k * kR, idesc, k > 0 || !fresh);
                     }
-                    mma_commit(empty(at));
                     const bool last = b == blocks - 1 || (kWeights && (b + 1) % (kChunk / kDepth) == 0);
-                    if (last) mma_commit(acc_full(acc));
+                    if constexpr (PAIR) {
+                        mma_commit_pair(empty(at));
+                        if (last) mma_commit_pair(acc_full(acc));
+                    } else {
+                        mma_commit(empty(at));
+                        if (last) mma_commit(acc_full(acc));
+                    }
                 }
                 __syncwarp();
                 if (b == blocks - 1 || (kWeights && (b + 1) % (kChunk / kDepth) == 0)) {
@@ -257,13 +297,17 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         int acc = 0;
         uint32_t acc_phase = 0;
         const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        auto accumulator_read = [&](int b) {
+            if constexpr (PAIR) remote_arrive(in_leader(acc_empty(b)));
+            else mbar_arrive(acc_empty(b));
+        };
         // a wait that runs out does not end these loops: the set's warps meet at barriers, and all have to come
         if constexpr (kWeights) {
             constexpr int kCols = TN / 2;                        // of a set
             float* const turn = reinterpret_cast<float*>(smem + S::kTurn0 + set * S::kTurnBytes);
-            for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-                if (t == (int)blockIdx.x) w.start(t);
-                else w.step(gridDim.x);
+            for (int t = t_first; t < tiles; t += t_step) {
+                if (t == t_first) w.start(t);
+                else w.step(t_step);
                 const int chunks = (w.count + kChunk - 1) / kChunk;
                 float sum[kCols];
 #pragma unroll
@@ -280,13 +324,13 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                     }
                     fence_before_sync();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(acc_empty(acc));
+                    if (lane == 0) accumulator_read(acc);
                     acc ^= 1;
                     if (acc == 0) acc_phase ^= 1;
                 }
                 const bool direct = w.units <= 1;
                 const long long stride = direct ? p.a.w_row_stride : p.a.n;
-                const int feature = w.feature0 + 4 * lane, live = p.a.n - feature;
+                const int feature = w.feature0 * S::kCtas + rank * 128 + 4 * lane, live = p.a.n - feature;
                 float* const out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + (long long)w.unit * p.a.k * p.a.n) + feature;
                 const bool add = direct && p.a.accumulate, wide = direct ? p.wide_store : p.a.n % 4 == 0;
                 const int row0 = w.row0 + set * kCols;
@@ -333,12 +377,12 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                         for (int c = lane; c < width; c += 32) out[row * stride + c] = from_float<T>(0.0f);
                 }
             }
-            for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
-                if (t == (int)blockIdx.x) w.start(t);
-                else w.step(gridDim.x);
+            for (int t = t_first; t < tiles; t += t_step) {
+                if (t == t_first) w.start(t);
+                else w.step(t_step);
                 mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
                 fence_after_sync();
-                const int feature = w.feature0 + 8 * (lane & 15), live = width - feature;
+                const int feature = w.feature0 * S::kCtas + rank * 128 + 8 * (lane & 15), live = width - feature;
                 // the sets take turns at blocks of 32 rows
 #pragma unroll 1
                 for (int j0 = set * 32; j0 < w.count; j0 += 64) {
@@ -370,7 +414,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 }
                 fence_before_sync();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty(acc));
+                if (lane == 0) accumulator_read(acc);
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1;
             }
@@ -386,7 +430,12 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
             if (lane == 0 && p.a.status) atomicOr(p.a.status, FMB_STATUS_TENSOR_TIMEOUT);
         }
         __syncwarp();
-        tmem_free(tmem, S::kTmem);
+    }
+    // neither CTA of a pair gives up its memory while the other's copies and arrivals may still come
+    if constexpr (PAIR) cluster_sync();
+    if (warp == 0) {
+        if constexpr (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(tmem), "r"(S::kTmem) : "memory");
+        else tmem_free(tmem, S::kTmem);
     }
 }
 
@@ -406,28 +455,50 @@ Encode encoder() {
     return found;
 }
 
-template <typename T, int MODE, int TN>
+template <typename T, int MODE, int TN, bool PAIR>
 int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, long long tiles, cudaStream_t stream) {
-    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN>, Shape<MODE, TN>::kSmem));
-    const int grid = (int)std::min<long long>(tiles, sm_count());
-    k_grouped_tc<T, MODE, TN><<<grid, Shape<MODE, TN>::kThreads, Shape<MODE, TN>::kSmem, stream>>>(p, features, rows);
+    using S = Shape<MODE, TN, PAIR>;
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN, PAIR>, S::kSmem));
+    const int grid = (int)std::min<long long>(tiles, sm_count() / S::kCtas) * S::kCtas;
+    if constexpr (PAIR) {
+        cudaLaunchConfig_t config = {};
+        cudaLaunchAttribute pair;
+        pair.id = cudaLaunchAttributeClusterDimension;
+        pair.val.clusterDim.x = 2;
+        pair.val.clusterDim.y = pair.val.clusterDim.z = 1;
+        config.gridDim = dim3(grid);
+        config.blockDim = dim3(S::kThreads);
+        config.dynamicSmemBytes = S::kSmem;
+        config.stream = stream;
+        config.attrs = &pair;
+        config.numAttrs = 1;
+        FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_grouped_tc<T, MODE, TN, PAIR>, p, features, rows));
+    } else {
+        k_grouped_tc<T, MODE, TN, PAIR><<<grid, S::kThreads, S::kSmem, stream>>>(p, features, rows);
+    }
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
 
 template <typename T, int MODE>
 int launch_rows(Args& p, const CUtensorMap& features, const CUtensorMap& rows, cudaStream_t stream) {
-    // the widest tile that still leaves a tile per SM, but none much wider than the groups are on average
     const fmb_grouped_t* a = &p.a;
-    const int average = a->rows / a->groups;
+    const int average = a->rows / a->groups, width = MODE == kLinear ? a->n : a->k;
+    // pairs of CTAs where there is a tile of 256 x 256 for each, and the groups fill half of one
+    if (average >= 128 && width > 128 && most_units(a, 256) * ((width + 255) / 256) >= 74) {
+        p.unit_rows = 256;
+        p.feature_tiles = ceil_div(width, 256);
+        return launch<T, MODE, 256, true>(p, features, rows, most_units(a, 256) * p.feature_tiles, stream);
+    }
+    // else the widest tile that still leaves one per SM, but none much wider than the groups are on average
     int tn = 256;
     while (tn > 32 && (tn > std::max(32, 2 * average) || most_units(a, tn) * p.feature_tiles < 148)) tn /= 2;
     p.unit_rows = tn;
     const long long tiles = most_units(a, tn) * p.feature_tiles;
-    if (tn == 256) return launch<T, MODE, 256>(p, features, rows, tiles, stream);
-    if (tn == 128) return launch<T, MODE, 128>(p, features, rows, tiles, stream);
-    if (tn == 64) return launch<T, MODE, 64>(p, features, rows, tiles, stream);
-    return launch<T, MODE, 32>(p, features, rows, tiles, stream);
+    if (tn == 256) return launch<T, MODE, 256, false>(p, features, rows, tiles, stream);
+    if (tn == 128) return launch<T, MODE, 128, false>(p, features, rows, tiles, stream);
+    if (tn == 64) return launch<T, MODE, 64, false>(p, features, rows, tiles, stream);
+    return launch<T, MODE, 32, false>(p, features, rows, tiles, stream);
 }
 
 // weight gradient: columns of a tile, and rows per unit -- all of a group's, or fewer where there are few tiles
@@ -461,12 +532,15 @@ int tma_typed(const fmb_grouped_t* a, Mode mode, const CUtensorMap& features, co
         p.wide_store = four_at_a_time(a->w, a->w_row_stride, 4) && a->w_group_stride % 4 == 0 && a->n % 4 == 0;
         int tn;
         weight_plan(a, tn, p.unit_rows);
-        p.feature_tiles = ceil_div(a->n, 128);
         p.row_tiles = ceil_div(a->k, tn);
-        const long long tiles = most_units(a, p.unit_rows) * p.feature_tiles * p.row_tiles;
         FMB_REQUIRE(p.unit_rows >= a->rows || a->scratch, "fmb_grouped_weight_gradient: null scratch");
-        const int rc = tn == 256 ? launch<T, kWeightGradient, 256>(p, features, rows, tiles, stream)
-                                 : launch<T, kWeightGradient, 128>(p, features, rows, tiles, stream);
+        const long long units = most_units(a, p.unit_rows);
+        const bool pair = tn == 256 && a->n > 128 && units * p.row_tiles * ((a->n + 255) / 256) >= 74;
+        p.feature_tiles = ceil_div(a->n, pair ? 256 : 128);
+        const long long tiles = units * p.feature_tiles * p.row_tiles;
+        const int rc = pair        ? launch<T, kWeightGradient, 256, true>(p, features, rows, tiles, stream)
+                       : tn == 256 ? launch<T, kWeightGradient, 256, false>(p, features, rows, tiles, stream)
+                                   : launch<T, kWeightGradient, 128, false>(p, features, rows, tiles, stream);
         return rc || p.unit_rows >= a->rows ? rc : sum_units(a, p.unit_rows, stream);
     }
     const bool forward = mode == kLinear;

@@ -79,7 +79,7 @@ SHAPES = [(1, 1, 1, 1, "even", 1), (1, 3, 128, 128, "one", 1), (7, 64, 64, 32, "
           (200, 5, 128, 128, "even", 4), (257, 3, 65, 129, "uneven", 1), (100, 9, 1, 200, "even", 1), (90, 4, 200, 1, "even", 3),
           (513, 17, 100, 72, "uneven", 1), (1000, 7, 130, 515, "even", 1), (640, 2, 264, 384, "one", 2),
           (300, 6, 128, 64, "none", 1), (5000, 8, 128, 128, "uneven", 4), (129, 1024, 48, 56, "even", 1),
-          (2500, 3, 1024, 256, "even", 1), (700, 2, 2056, 136, "uneven", 1), (16, 4, 4096, 512, "even", 1)]
+          (20_000, 7, 200, 1096, "uneven", 1), (9000, 30, 520, 264, "even", 1), (2500, 3, 1024, 256, "even", 1), (700, 2, 2056, 136, "uneven", 1), (16, 4, 4096, 512, "even", 1)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
