@@ -132,12 +132,138 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n;        // not of the weight gradient
 
     Walk w(p.a, first_unit, p.unit_rows, p.feature_tiles, p.row_tiles, TN);
-    if constexpr (kWeights) {
-        // eight warps with 56 registers a thread, eight with 200: 256 x 256 as at the launch
-        if (warp < 8) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
-        else asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    }
-
+    if (warp >= S::kFirstEpilogue) {
+        // of the weight gradient eight warps with 72 registers a thread and eight with 184: 256 x 256, as at the launch
+        if constexpr (kWeights) asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        // ---------------------------------------------------------------- results
+        const int quarter = warp & 3, set = (warp - S::kFirstEpilogue) >> 2, id = quarter * 32 + lane;     // lanes 32 quarter + [0, 32)
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+        auto accumulator_read = [&](int b) {
+            if constexpr (PAIR) remote_arrive(in_leader(acc_empty(b)));
+            else mbar_arrive(acc_empty(b));
+        };
+        // a wait that runs out does not end these loops: the set's warps meet at barriers, and all have to come
+        if constexpr (kWeights) {
+            constexpr int kCols = TN / 2;                        // of a set
+            float* const turn = reinterpret_cast<float*>(smem + S::kTurn0 + set * S::kTurnBytes);
+            for (int t = t_first; t < tiles; t += t_step) {
+                if (t == t_first) w.start(t);
+                else w.step(t_step);
+                const int chunks = (w.count + kChunk - 1) / kChunk;
+                float sum[kCols];
+#pragma unroll
+                for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
+                for (int c = 0; c < chunks; ++c) {
+                    mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
+                    fence_after_sync();
+#pragma unroll
+                    for (int j0 = 0; j0 < kCols; j0 += 32) {
+                        float v[32];
+                        tmem_load_32(tmem + lanes + acc * TN + set * kCols + j0, v);
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) sum[j0 + j] += v[j];
+                    }
+                    fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) accumulator_read(acc);
+                    acc ^= 1;
+                    if (acc == 0) acc_phase ^= 1;
+                }
+                const bool direct = w.units <= 1;
+                const long long stride = direct ? p.a.w_row_stride : p.a.n;
+                const int feature = w.feature0 * S::kCtas + rank * 128 + 4 * lane, live = p.a.n - feature;
+                float* const out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + (long long)w.unit * p.a.k * p.a.n) + feature;
+                const bool add = direct && p.a.accumulate, wide = direct ? p.wide_store : p.a.n % 4 == 0;
+                const int row0 = w.row0 + set * kCols;
+#pragma unroll
+                for (int j0 = 0; j0 < kCols; j0 += 32) {
+                    named_barrier(1 + set, 128);                  // what was here has been read
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) turn[j * 128 + id] = sum[j0 + j];
+                    named_barrier(1 + set, 128);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int r = j * 4 + quarter, row = row0 + j0 + r;
+                        float4 v = *reinterpret_cast<const float4*>(turn + r * 128 + 4 * lane);
+                        if (row >= p.a.k) continue;
+                        float* const to = out + row * stride;
+                        if (wide) {
+                            if (live > 0) {
+                                if (add) {
+                                    const float4 old = *reinterpret_cast<const float4*>(to);
+                                    v.x += old.x; v.y += old.y; v.z += old.z; v.w += old.w;
+                                }
+                                *reinterpret_cast<float4*>(to) = v;
+                            }
+                        } else {
+                            if (live > 0) to[0] = add ? to[0] + v.x : v.x;
+                            if (live > 1) to[1] = add ? to[1] + v.y : v.y;
+                            if (live > 2) to[2] = add ? to[2] + v.z : v.z;
+                            if (live > 3) to[3] = add ? to[3] + v.w : v.w;
+                        }
+                    }
+                }
+            }
+        } else {
+            T* const out = (T*)(MODE == kLinear ? p.a.y : p.a.x);
+            const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
+            const int width = MODE == kLinear ? p.a.n : p.a.k;
+            T* const turn = reinterpret_cast<T*>(smem + S::kTurn0 + set * S::kTurnBytes);      // [32 rows][128 features]
+            if (p.a.zero_rest) {
+                // rows of no group
+                const int from = min(max(p.a.offsets[p.a.groups], 0), p.a.rows), first = blockIdx.x * kEpilogueWarps + warp - S::kFirstEpilogue;
+                for (int i = from + first; i < p.a.rows; i += gridDim.x * kEpilogueWarps) {
+                    const int row = row_at(p, i, p.a.rows);
+                    if (row >= 0)
+                        for (int c = lane; c < width; c += 32) out[row * stride + c] = from_float<T>(0.0f);
+                }
+            }
+            for (int t = t_first; t < tiles; t += t_step) {
+                if (t == t_first) w.start(t);
+                else w.step(t_step);
+                mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
+                fence_after_sync();
+                const int feature = w.feature0 * S::kCtas + rank * 128 + 8 * (lane & 15), live = width - feature;
+                // the sets take turns at blocks of 32 rows
+#pragma unroll 1
+                for (int j0 = set * 32; j0 < w.count; j0 += 64) {
+                    const int mine = row_at(p, w.first + j0 + lane, w.first + w.count);
+                    float v[32];
+                    tmem_load_32(tmem + lanes + acc * TN + j0, v);
+                    named_barrier(1 + set, 128);                  // what was here has been read
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) turn[j * 128 + id] = from_float<T>(v[j]);
+                    named_barrier(1 + set, 128);
+                    uint4 q[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        q[j] = *reinterpret_cast<const uint4*>(turn + (j * 8 + quarter * 2 + (lane >> 4)) * 128 + 8 * (lane & 15));
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int row = __shfl_sync(0xffffffffu, mine, j * 8 + quarter * 2 + (lane >> 4));
+                        T* const to = out + row * stride + feature;
+                        if (row < 0) continue;
+                        if (p.wide_store) {
+                            if (live > 0) *reinterpret_cast<uint4*>(to) = q[j];
+                        } else {
+                            const T* const each = reinterpret_cast<const T*>(&q[j]);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (i < live) to[i] = each[i];
+                        }
+                    }
+                }
+                fence_before_sync();
+                __syncwarp();
+                if (lane == 0) accumulator_read(acc);
+                acc ^= 1;
+                if (acc == 0) acc_phase ^= 1;
+            }
+        }
+    } else {
+    if constexpr (kWeights) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     if (warp < S::kCopyWarps) {
         // ---------------------------------------------------------------- copies
         int at = 0;
@@ -291,134 +417,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 }
             }
         }
-    } else if (warp >= S::kFirstEpilogue) {
-        // ---------------------------------------------------------------- results
-        const int quarter = warp & 3, set = (warp - S::kFirstEpilogue) >> 2, id = quarter * 32 + lane;     // lanes 32 quarter + [0, 32)
-        int acc = 0;
-        uint32_t acc_phase = 0;
-        const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-        auto accumulator_read = [&](int b) {
-            if constexpr (PAIR) remote_arrive(in_leader(acc_empty(b)));
-            else mbar_arrive(acc_empty(b));
-        };
-        // a wait that runs out does not end these loops: the set's warps meet at barriers, and all have to come
-        if constexpr (kWeights) {
-            constexpr int kCols = TN / 2;                        // of a set
-            float* const turn = reinterpret_cast<float*>(smem + S::kTurn0 + set * S::kTurnBytes);
-            for (int t = t_first; t < tiles; t += t_step) {
-                if (t == t_first) w.start(t);
-                else w.step(t_step);
-                const int chunks = (w.count + kChunk - 1) / kChunk;
-                float sum[kCols];
-#pragma unroll
-                for (int j = 0; j < kCols; ++j) sum[j] = 0.0f;
-                for (int c = 0; c < chunks; ++c) {
-                    mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
-                    fence_after_sync();
-#pragma unroll
-                    for (int j0 = 0; j0 < kCols; j0 += 32) {
-                        float v[32];
-                        tmem_load_32(tmem + lanes + acc * TN + set * kCols + j0, v);
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) sum[j0 + j] += v[j];
-                    }
-                    fence_before_sync();
-                    __syncwarp();
-                    if (lane == 0) accumulator_read(acc);
-                    acc ^= 1;
-                    if (acc == 0) acc_phase ^= 1;
-                }
-                const bool direct = w.units <= 1;
-                const long long stride = direct ? p.a.w_row_stride : p.a.n;
-                const int feature = w.feature0 * S::kCtas + rank * 128 + 4 * lane, live = p.a.n - feature;
-                float* const out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + (long long)w.unit * p.a.k * p.a.n) + feature;
-                const bool add = direct && p.a.accumulate, wide = direct ? p.wide_store : p.a.n % 4 == 0;
-                const int row0 = w.row0 + set * kCols;
-#pragma unroll
-                for (int j0 = 0; j0 < kCols; j0 += 32) {
-                    named_barrier(1 + set, 128);                  // what was here has been read
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) turn[j * 128 + id] = sum[j0 + j];
-                    named_barrier(1 + set, 128);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const int r = j * 4 + quarter, row = row0 + j0 + r;
-                        float4 v = *reinterpret_cast<const float4*>(turn + r * 128 + 4 * lane);
-                        if (row >= p.a.k) continue;
-                        float* const to = out + row * stride;
-                        if (wide) {
-                            if (live > 0) {
-                                if (add) {
-                                    const float4 old = *reinterpret_cast<const float4*>(to);
-                                    v.x += old.x; v.y += old.y; v.z += old.z; v.w += old.w;
-                                }
-                                *reinterpret_cast<float4*>(to) = v;
-                            }
-                        } else {
-                            if (live > 0) to[0] = add ? to[0] + v.x : v.x;
-                            if (live > 1) to[1] = add ? to[1] + v.y : v.y;
-                            if (live > 2) to[2] = add ? to[2] + v.z : v.z;
-                            if (live > 3) to[3] = add ? to[3] + v.w : v.w;
-                        }
-                    }
-                }
-            }
-        } else {
-            T* const out = (T*)(MODE == kLinear ? p.a.y : p.a.x);
-            const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
-            const int width = MODE == kLinear ? p.a.n : p.a.k;
-            T* const turn = reinterpret_cast<T*>(smem + S::kTurn0 + set * S::kTurnBytes);      // [32 rows][128 features]
-            if (p.a.zero_rest) {
-                // rows of no group
-                const int from = min(max(p.a.offsets[p.a.groups], 0), p.a.rows), first = blockIdx.x * kEpilogueWarps + warp - S::kFirstEpilogue;
-                for (int i = from + first; i < p.a.rows; i += gridDim.x * kEpilogueWarps) {
-                    const int row = row_at(p, i, p.a.rows);
-                    if (row >= 0)
-                        for (int c = lane; c < width; c += 32) out[row * stride + c] = from_float<T>(0.0f);
-                }
-            }
-            for (int t = t_first; t < tiles; t += t_step) {
-                if (t == t_first) w.start(t);
-                else w.step(t_step);
-                mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
-                fence_after_sync();
-                const int feature = w.feature0 * S::kCtas + rank * 128 + 8 * (lane & 15), live = width - feature;
-                // the sets take turns at blocks of 32 rows
-#pragma unroll 1
-                for (int j0 = set * 32; j0 < w.count; j0 += 64) {
-                    const int mine = row_at(p, w.first + j0 + lane, w.first + w.count);
-                    float v[32];
-                    tmem_load_32(tmem + lanes + acc * TN + j0, v);
-                    named_barrier(1 + set, 128);                  // what was here has been read
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) turn[j * 128 + id] = from_float<T>(v[j]);
-                    named_barrier(1 + set, 128);
-                    uint4 q[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        q[j] = *reinterpret_cast<const uint4*>(turn + (j * 8 + quarter * 2 + (lane >> 4)) * 128 + 8 * (lane & 15));
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int row = __shfl_sync(0xffffffffu, mine, j * 8 + quarter * 2 + (lane >> 4));
-                        T* const to = out + row * stride + feature;
-                        if (row < 0) continue;
-                        if (p.wide_store) {
-                            if (live > 0) *reinterpret_cast<uint4*>(to) = q[j];
-                        } else {
-                            const T* const each = reinterpret_cast<const T*>(&q[j]);
-#pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (i < live) to[i] = each[i];
-                        }
-                    }
-                }
-                fence_before_sync();
-                __syncwarp();
-                if (lane == 0) accumulator_read(acc);
-                acc ^= 1;
-                if (acc == 0) acc_phase ^= 1;
-            }
-        }
+    }
     }
     fence_before_sync();
     __syncthreads();
