@@ -41,10 +41,10 @@ template <int MODE, int TN, bool PAIR> struct Shape {
     static constexpr int kThreads = 32 * (kFirstEpilogue + kEpilogueWarps);
     // results turn through shared memory, 32 rows of 128 features at a time and set
     static constexpr int kTurnBytes = 32 * 128 * (kWeights ? 4 : 2);
-    static constexpr int kRoom = 226 * 1024 - 2 * kTurnBytes - 1024 - (FMB_MAX_GROUPS + 1) * 4 - 256 - kCopyWarps * 256;
+    static constexpr int kRoom = 226 * 1024 - 2 * kTurnBytes - 1024 - (FMB_MAX_GROUPS + 1) * 4 - 256 - kCopyWarps * 512 - (kWeights ? (FMB_MAX_GROUPS + 1) * 8 : 0);
     static constexpr int kStages = kRoom / kStageBytes < 8 ? kRoom / kStageBytes : 8;
-    static constexpr int kTurn0 = kStages * kStageBytes, kRows0 = kTurn0 + 2 * kTurnBytes, kUnits0 = kRows0 + kCopyWarps * 256,
-                         kBars0 = kUnits0 + ((FMB_MAX_GROUPS + 1) * 4 + 7) / 8 * 8;
+    static constexpr int kTurn0 = kStages * kStageBytes, kRows0 = kTurn0 + 2 * kTurnBytes, kUnits0 = kRows0 + kCopyWarps * 512,
+                         kCosts0 = kUnits0 + ((FMB_MAX_GROUPS + 1) * 4 + 7) / 8 * 8, kBars0 = kCosts0 + (kWeights ? (FMB_MAX_GROUPS + 1) * 8 : 0);
     static constexpr int kSmem = 1024 + kBars0 + 256;
     static constexpr int kTmem = 2 * TN < 32 ? 32 : 2 * TN;
     static_assert(kStages >= 3 && kSmem <= 227 * 1024 && kMmaWarp < kFirstEpilogue, "fits an SM");
@@ -82,7 +82,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     constexpr int kMmaWarp = S::kMmaWarp;
 
     // of a pair: CTA 0 leads; both walk the same tiles, each with its own 128 features and half of the rows to bring
-    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0, t_first = blockIdx.x / S::kCtas, t_step = gridDim.x / S::kCtas;
+    const int rank = PAIR ? (int)(blockIdx.x & 1) : 0;
     auto copy_bar = [&](int s) { return PAIR ? in_leader(full(s)) : full(s); };
     auto expect = [&](uint32_t bar, uint32_t bytes) {
         if constexpr (PAIR) {
@@ -128,7 +128,52 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     if constexpr (PAIR) cluster_sync();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const int tiles = first_unit[p.a.groups] * p.feature_tiles * p.row_tiles;
+    // Tiles of the linears cost the same, and go round. Those of the weight gradient cost what their group has rows: every CTA (pair)
+    // takes consecutive tiles of the same cost in all (sizes that differ by a factor of three cost 40 % where tiles went round).
+    const int walkers = gridDim.x / S::kCtas, walker = blockIdx.x / S::kCtas, all_tiles = first_unit[p.a.groups] * p.feature_tiles * p.row_tiles;
+    int t_first = walker, t_end = all_tiles;
+    constexpr bool kRound = !kWeights;
+    const int t_step = kRound ? walkers : 1;
+    if constexpr (kWeights) {
+        long long* const cost = reinterpret_cast<long long*>(smem + S::kCosts0);
+        if (warp == 0) {
+            long long before = 0;
+            for (int g0 = 0; g0 < p.a.groups; g0 += 32) {
+                const int g = g0 + lane;
+                long long mine = 0;
+                if (g < p.a.groups) {
+                    int begin, end;
+                    group_span(p.a.offsets, g, p.a.rows, begin, end);
+                    const int units = first_unit[g + 1] - first_unit[g];
+                    mine = ((end - begin + kDepth - 1) / kDepth + 2ll * units) * p.feature_tiles * p.row_tiles;
+                }
+                long long inclusive = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const long long up = __shfl_up_sync(0xffffffffu, inclusive, o);
+                    if (lane >= o) inclusive += up;
+                }
+                if (g < p.a.groups) cost[g] = before + inclusive - mine;
+                before += __shfl_sync(0xffffffffu, inclusive, 31);
+            }
+            if (lane == 0) cost[p.a.groups] = before;
+        }
+        __syncthreads();
+        auto first_tile = [&](int c) {
+            if (c >= walkers) return all_tiles;
+            const long long target = cost[p.a.groups] / walkers * c + cost[p.a.groups] % walkers * c / walkers;
+            int low = 0, high = p.a.groups - 1;
+            while (low < high) {
+                const int mid = (low + high + 1) >> 1;
+                if (cost[mid] <= target) low = mid; else high = mid - 1;
+            }
+            const long long tiles_of = (long long)(first_unit[low + 1] - first_unit[low]) * p.feature_tiles * p.row_tiles, span = cost[low + 1] - cost[low];
+            const long long skip = span > 0 ? ((target - cost[low]) * tiles_of + span / 2) / span : 0;
+            return first_unit[low] * p.feature_tiles * p.row_tiles + (int)min(skip, tiles_of);
+        };
+        t_first = first_tile(walker);
+        t_end = first_tile(walker + 1);
+    }
     const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n;        // not of the weight gradient
 
     Walk w(p.a, first_unit, p.unit_rows, p.feature_tiles, p.row_tiles, TN);
@@ -148,7 +193,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         if constexpr (kWeights) {
             constexpr int kCols = TN / 2;                        // of a set
             float* const turn = reinterpret_cast<float*>(smem + S::kTurn0 + set * S::kTurnBytes);
-            for (int t = t_first; t < tiles; t += t_step) {
+            for (int t = t_first; t < t_end; t += t_step) {
                 if (t == t_first) w.start(t);
                 else w.step(t_step);
                 const int chunks = (w.count + kChunk - 1) / kChunk;
@@ -220,7 +265,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                         for (int c = lane; c < width; c += 32) out[row * stride + c] = from_float<T>(0.0f);
                 }
             }
-            for (int t = t_first; t < tiles; t += t_step) {
+            for (int t = t_first; t < t_end; t += t_step) {
                 if (t == t_first) w.start(t);
                 else w.step(t_step);
                 mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
@@ -271,13 +316,35 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         bool alive = true;
         // The row numbers of this warp's gathers, in shared memory: read four at a time at an address the whole warp shares,
         // they get to the gather on the short way (with shuffles 47 cycles a gather, lanes that issue their own 62).
-        int4* const rows = reinterpret_cast<int4*>(smem + S::kRows0 + warp * 256);
+        int4* const rows = reinterpret_cast<int4*>(smem + S::kRows0 + warp * 512);
         int* const my_rows = reinterpret_cast<int*>(rows) + 2 * lane;
         auto row_or_zeros = [&](int entry, int end) {
             const int row = row_at(p, entry, end);
             return row < 0 ? p.a.rows : row;               // TMA fills what is past the last row with zeros
         };
-        for (int t = t_first; alive && t < tiles; t += t_step) {
+        // weight gradient: the tile and block whose row numbers come next
+        Walk ahead = w;
+        int ahead_tile = t_first, ahead_block = -1, next0 = p.a.rows, next1 = p.a.rows, buffer = 0;
+        auto look_ahead = [&] {
+            ++ahead_block;
+            while (ahead_tile < t_end && ahead_block * kDepth >= ahead.count) {
+                ahead_block = 0;
+                if (++ahead_tile < t_end) ahead.step(1);
+            }
+            if (ahead_tile >= t_end) return;
+            const int end = ahead.first + ahead.count;
+            next0 = row_or_zeros(ahead.first + ahead_block * kDepth + 2 * lane, end);
+            next1 = row_or_zeros(ahead.first + ahead_block * kDepth + 2 * lane + 1, end);
+        };
+        if (kWeights && t_first < t_end) {
+            // row numbers are asked for two blocks ahead, and put in place one ahead, across tiles
+            ahead.start(t_first);
+            look_ahead();
+            my_rows[0] = next0;
+            my_rows[1] = next1;
+            look_ahead();
+        }
+        for (int t = t_first; alive && t < t_end; t += t_step) {
             if (t == t_first) w.start(t);
             else w.step(t_step);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
@@ -336,24 +403,21 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
             } else {
                 const CUtensorMap* const map = warp < 2 ? &feature_map : &row_map;
                 const int column = warp < 2 ? feature0 + warp * 64 : w.row0 + rank * S::kRows + (warp - 2) * 64;
-                int next0 = row_or_zeros(w.first + 2 * lane, end), next1 = row_or_zeros(w.first + 2 * lane + 1, end);
-                for (int b = 0; b < blocks; ++b) {
-                    // the depths of this block, and those of the next on their way
-                    __syncwarp();
-                    my_rows[0] = next0;
-                    my_rows[1] = next1;
-                    next0 = row_or_zeros(w.first + (b + 1) * kDepth + 2 * lane, end);
-                    next1 = row_or_zeros(w.first + (b + 1) * kDepth + 2 * lane + 1, end);
+                for (int b = 0; b < blocks; ++b, buffer ^= 64) {
+                    my_rows[(buffer ^ 64)] = next0;
+                    my_rows[(buffer ^ 64) + 1] = next1;
+                    look_ahead();
                     __syncwarp();
                     alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
                     if (!alive) break;
                     const uint32_t dst = stage0 + at * S::kStageBytes + warp * 8192, bar = copy_bar(at);
                     const int quads = min(16, (w.count - b * kDepth + 15) / 16 * 4);     // depths past the end, up to a multiple of 16, are zeros
+                    const int4* const mine = rows + buffer / 4;
                     if (elect_one()) {
                         expect(bar, quads * 512);
 #pragma unroll 4
                         for (int q = 0; q < quads; ++q) {
-                            const int4 r = rows[q];
+                            const int4 r = mine[q];
                             gather(dst + q * 512, map, column, r, bar);
                         }
                     }
@@ -373,7 +437,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         constexpr uint32_t kMajor = MODE == kLinear ? 1u << 15 : MODE == kWeightGradient ? 3u << 15 : 0;
         constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | kMajor | ((uint32_t)(128 * S::kCtas >> 4) << 24);
         bool alive = true;
-        for (int t = t_first; alive && t < tiles; t += t_step) {
+        for (int t = t_first; alive && t < t_end; t += t_step) {
             if (t == t_first) w.start(t);
             else w.step(t_step);
             const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
