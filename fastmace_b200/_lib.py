@@ -183,7 +183,7 @@ def load() -> ctypes.CDLL:
     lib.fmb_group_rows_scratch.argtypes = [ctypes.c_longlong, c_int]
     lib.fmb_group_rows_scratch.restype = ctypes.c_longlong
     lib.fmb_group_rows.argtypes = [P, c_int, ctypes.c_longlong, c_int, P, P, P, P]
-    lib.fmb_grouped_scratch.argtypes = [POINTER(GroupedStruct)]
+    lib.fmb_grouped_scratch.argtypes = [POINTER(GroupedStruct), c_int]
     lib.fmb_grouped_scratch.restype = ctypes.c_longlong
     for name in ("fmb_grouped_linear", "fmb_grouped_input_gradient", "fmb_grouped_weight_gradient"):
         getattr(lib, name).argtypes = [POINTER(GroupedStruct), P]

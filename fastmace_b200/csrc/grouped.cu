@@ -1,7 +1,7 @@
 // Entry points of the grouped products (fmb_grouped_linear and the calls beside it): checks, and which kernel runs.
 //
-// 16-bit operands whose rows start at multiples of 16 bytes go by TMA (grouped_tc.cu); threads bring the others
-// (grouped_split.cu): fp32, which has to be split into bf16 parts on its way, and odd sizes.
+// 16-bit operands go by TMA (grouped_tc.cu). fp32 operands are split into bf16 parts on their way (grouped_split.cu); linears of
+// a depth of up to 128 keep the split weights in tensor memory (grouped_resident.cu).
 
 #include "grouped.cuh"
 
@@ -33,7 +33,7 @@ k_sum_units(fmb_grouped_t a, int unit_rows) {
         }
     }
     __syncthreads();
-    if (first[1] <= 1) return;
+    if (first[1] <= 1 || first[0] + first[1] > most_units(a.rows, a.groups, unit_rows)) return;
     const long long size = (long long)a.k * a.n, i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= size) return;
     const float* at = a.scratch + first[0] * size + i;
@@ -66,7 +66,8 @@ int run(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
     int rc = check(a);
     if (rc) return rc;
     if (a->rows == 0 && mode != kWeightGradient) return FMB_OK;
-    rc = a->type == FMB_TYPE_F32 ? resident_launch(a, mode, stream) : tma_launch(a, mode, stream);
+    if (a->rows > 0 && a->type != FMB_TYPE_F32) return tma_launch(a, mode, stream);
+    rc = a->rows > 0 ? resident_launch(a, mode, stream) : FMB_ERR_UNSUPPORTED;
     return rc != FMB_ERR_UNSUPPORTED ? rc : split_launch(a, mode, stream);
 }
 
@@ -100,11 +101,9 @@ extern "C" FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* a, fmb_s
     return run(a, kWeightGradient, (cudaStream_t)stream);
 }
 
-extern "C" FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* a) {
-    if (!a || a->groups < 1 || a->k < 1 || a->n < 1 || a->rows < 1) return 0;
-    // whichever kernel the pointers' alignment selects
-    long long most = 0;
-    for (int unit_rows : {tma_unit_rows(a), split_unit_rows(a)})
-        if (unit_rows < a->rows) most = std::max(most, most_units(a, unit_rows) * a->k * a->n);
-    return most;
+extern "C" FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* a, int which) {
+    if (!a || which < 0 || which > 2 || a->groups < 1 || a->k < 1 || a->n < 1 || a->rows < 1) return 0;
+    if (a->type != FMB_TYPE_F32) return tma_scratch_bytes(a, (Mode)which) / 4;
+    const int unit_rows = split_unit_rows(a);
+    return which == 2 && unit_rows < a->rows ? most_units(a, unit_rows) * a->k * a->n : 0;
 }

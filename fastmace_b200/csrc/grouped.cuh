@@ -53,6 +53,13 @@ __device__ __forceinline__ void count_units(const int32_t* offsets, int groups, 
     __syncthreads();
 }
 
+// Units that `rows` entries can make at most. Offsets that are none can add up to more: what is past this is left out, so that
+// buffers of this many units are never left.
+__host__ __device__ __forceinline__ long long most_units(int rows, int groups, int size) { return (long long)rows / size + groups; }
+__device__ __forceinline__ int units_in_all(const int* first, int groups, int rows, int size) {
+    return (int)min((long long)max(0, first[groups]), most_units(rows, groups, size));
+}
+
 // the group that unit u belongs to: the last one that begins at or before it
 __device__ __forceinline__ int group_of_unit(const int* first, int groups, int u) {
     int low = 0, high = groups - 1;
@@ -65,9 +72,11 @@ __device__ __forceinline__ int group_of_unit(const int* first, int groups, int u
 
 enum Mode { kLinear = 0, kInputGradient = 1, kWeightGradient = 2 };
 
-// tcgen05 kernels with operands by TMA (grouped_tc.cu): FMB_ERR_UNSUPPORTED for types and alignments that TMA does not take
+// tcgen05 kernels of 16-bit operands, brought by TMA (grouped_tc.cu), and the bytes of scratch that a call with these sizes,
+// strides and pointers needs
 int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
-// tcgen05 kernels whose threads bring the operands (grouped_split.cu): fp32, and every alignment
+long long tma_scratch_bytes(const fmb_grouped_t* a, Mode mode);
+// tcgen05 kernels whose threads bring the operands (grouped_split.cu): fp32 at any alignment
 int split_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
 
 // tcgen05 kernel that keeps the split weights in tensor memory (grouped_resident.cu): FMB_ERR_UNSUPPORTED unless fp32, a depth of
@@ -79,13 +88,17 @@ inline bool four_at_a_time(const void* base, long long stride, int bytes) {
     return ((uintptr_t)base & (uintptr_t)(4 * bytes - 1)) == 0 && stride % 4 == 0;
 }
 
-// weight gradient: rows per unit of either kernel (2^30 where units are whole groups), the most units there can be, and the sum
+// fp32 weight gradient: rows per unit (2^30 where units are whole groups), the most units there can be, and the sum
 // over the units of the groups that have several
-int tma_unit_rows(const fmb_grouped_t* a);
 int split_unit_rows(const fmb_grouped_t* a);
-inline long long most_units(const fmb_grouped_t* a, int unit_rows) { return (long long)a->rows / unit_rows + a->groups; }
+inline long long most_units(const fmb_grouped_t* a, int unit_rows) { return most_units(a->rows, a->groups, unit_rows); }
 int sum_units(const fmb_grouped_t* a, int unit_rows, cudaStream_t stream);
 int sm_count();
+
+// copies into the layouts that TMA takes (grouped_pack.cu)
+int pack_rows(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream);
+int pack_weights(const fmb_grouped_t* a, void* dst, cudaStream_t stream);
+int sort_rows(const fmb_grouped_t* a, void* x, void* y, int32_t* first_block, cudaStream_t stream);
 
 }  // namespace grp
 }  // namespace fmb

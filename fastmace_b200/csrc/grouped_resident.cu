@@ -112,7 +112,7 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const long long tiles = (long long)first_unit[p.a.groups] * p.feature_tiles;
+    const long long tiles = (long long)units_in_all(first_unit, p.a.groups, p.a.rows, kTN) * p.feature_tiles;
     const int t_begin = (int)(tiles * blockIdx.x / gridDim.x), t_end = (int)(tiles * (blockIdx.x + 1) / gridDim.x);
     const int depth = MODE == kLinear ? p.a.k : p.a.n, width = MODE == kLinear ? p.a.n : p.a.k;
     const int columns = depth <= 64 ? 64 : 128;              // of a row in the ring

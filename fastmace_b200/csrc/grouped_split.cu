@@ -116,7 +116,7 @@ k_grouped_split(const __grid_constant__ SplitArgs p) {
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const long long tiles = (long long)first_unit[p.a.groups] * p.feature_tiles * p.row_tiles;
+    const long long tiles = (long long)units_in_all(first_unit, p.a.groups, p.a.rows, p.unit_rows) * p.feature_tiles * p.row_tiles;
     const int t_begin = (int)(tiles * blockIdx.x / gridDim.x), t_end = (int)(tiles * (blockIdx.x + 1) / gridDim.x);
     const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n;
     const T* const row_source = (const T*)(MODE == kInputGradient ? p.a.y : p.a.x);
@@ -410,11 +410,7 @@ int split_unit_rows(const fmb_grouped_t* a) {
     return unit_rows < a->rows ? unit_rows : 1 << 30;
 }
 
-int split_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
-    if (a->type == FMB_TYPE_F32) return typed<float>(a, mode, stream);
-    if (a->type == FMB_TYPE_BF16) return typed<__nv_bfloat16>(a, mode, stream);
-    return typed<__half>(a, mode, stream);
-}
+int split_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) { return typed<float>(a, mode, stream); }
 
 }  // namespace grp
 }  // namespace fmb

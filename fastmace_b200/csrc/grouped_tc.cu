@@ -26,7 +26,8 @@ using namespace tc;
 constexpr int kEpilogueWarps = 8;
 constexpr int kChunk = 512;                      // weight gradient: depth after which an accumulator moves to registers
 
-template <int MODE, int TN, bool PAIR> struct Shape {
+// SORTED, of the weight gradient: the rows lie by groups (sort_rows)
+template <int MODE, int TN, bool PAIR, bool SORTED> struct Shape {
     static constexpr bool kWeights = MODE == kWeightGradient;
     static constexpr int kCtas = PAIR ? 2 : 1, kRows = TN / kCtas;                 // rows of the tile that a CTA brings
     static constexpr int kFeatureBytes = 128 * kDepth * 2, kRowBytes = kRows * kDepth * 2;
@@ -35,7 +36,7 @@ template <int MODE, int TN, bool PAIR> struct Shape {
     // Warps that issue copies: of the linears warp 0 for the features, the others for rows, 32 each; of the weight gradient one
     // per 64 columns of y or x. One warp takes 30 cycles a gather, and 64 (96) of them feed 512 cycles of MMAs. Then the warp
     // that issues MMAs, and eight that take results out, two sets of four.
-    static constexpr int kGathers = kWeights ? 2 + kRows / 64 : kRows / kRowsPerWarp, kCopyWarps = kWeights ? kGathers : 1 + kGathers;
+    static constexpr int kGathers = kWeights ? 2 + kRows / 64 : kRows / kRowsPerWarp, kCopyWarps = SORTED ? 1 : kWeights ? kGathers : 1 + kGathers;
     static constexpr int kMmaWarp = kCopyWarps;
     static constexpr int kFirstEpilogue = kWeights ? 8 : kMmaWarp + 1;             // whole warpgroups, so that registers can be dealt
     static constexpr int kThreads = 32 * (kFirstEpilogue + kEpilogueWarps);
@@ -55,6 +56,7 @@ struct Args {
     int feature_tiles, row_tiles;                // of the output; row_tiles 1 where rows are gathered
     int unit_rows;                               // entries of a group per unit
     int wide_store;                              // output rows may be written 16 bytes at a time
+    const int32_t* first_block;                  // SORTED: blocks of 64 rows of the groups before each
 };
 
 __device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
@@ -62,10 +64,10 @@ __device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map
                  :: "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
 }
 
-template <typename T, int MODE, int TN, bool PAIR>
-__global__ void __launch_bounds__(Shape<MODE, TN, PAIR>::kThreads, 1)
+template <typename T, int MODE, int TN, bool PAIR, bool SORTED>
+__global__ void __launch_bounds__(Shape<MODE, TN, PAIR, SORTED>::kThreads, 1)
 k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap feature_map, const __grid_constant__ CUtensorMap row_map) {
-    using S = Shape<MODE, TN, PAIR>;
+    using S = Shape<MODE, TN, PAIR, SORTED>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     int* const first_unit = reinterpret_cast<int*>(smem + S::kUnits0);
@@ -96,6 +98,10 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     auto gather = [&](uint32_t dst, const CUtensorMap* map, int column, const int4& r, uint32_t bar) {
         if constexpr (PAIR) tma_gather4_pair(dst, map, column, r.x, r.y, r.z, r.w, bar);
         else tma_gather4(dst, map, column, r.x, r.y, r.z, r.w, bar);
+    };
+    auto tile = [&](uint32_t dst, const CUtensorMap* map, int column, int row, uint32_t bar) {
+        if constexpr (PAIR) tma_tile_2d_pair(dst, map, column, row, bar);
+        else tma_tile_2d(dst, map, column, row, bar);
     };
     auto box = [&](uint32_t dst, int c0, int c1, int c2, uint32_t bar) {
         if constexpr (PAIR) tma_tile_3d_pair(dst, &feature_map, c0, c1, c2, bar);
@@ -130,7 +136,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     // Tiles of the linears cost the same, and go round. Those of the weight gradient cost what their group has rows: every CTA (pair)
     // takes consecutive tiles of the same cost in all (sizes that differ by a factor of three cost 40 % where tiles went round).
-    const int walkers = gridDim.x / S::kCtas, walker = blockIdx.x / S::kCtas, all_tiles = first_unit[p.a.groups] * p.feature_tiles * p.row_tiles;
+    const int walkers = gridDim.x / S::kCtas, walker = blockIdx.x / S::kCtas, all_tiles = units_in_all(first_unit, p.a.groups, p.a.rows, p.unit_rows) * p.feature_tiles * p.row_tiles;
     int t_first = walker, t_end = all_tiles;
     constexpr bool kRound = !kWeights;
     const int t_step = kRound ? walkers : 1;
@@ -171,8 +177,8 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
             const long long skip = span > 0 ? ((target - cost[low]) * tiles_of + span / 2) / span : 0;
             return first_unit[low] * p.feature_tiles * p.row_tiles + (int)min(skip, tiles_of);
         };
-        t_first = first_tile(walker);
-        t_end = first_tile(walker + 1);
+        t_first = min(first_tile(walker), all_tiles);
+        t_end = min(first_tile(walker + 1), all_tiles);
     }
     const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n;        // not of the weight gradient
 
@@ -336,7 +342,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
             next0 = row_or_zeros(ahead.first + ahead_block * kDepth + 2 * lane, end);
             next1 = row_or_zeros(ahead.first + ahead_block * kDepth + 2 * lane + 1, end);
         };
-        if (kWeights && t_first < t_end) {
+        if (kWeights && !SORTED && t_first < t_end) {
             // row numbers are asked for two blocks ahead, and put in place one ahead, across tiles
             ahead.start(t_first);
             look_ahead();
@@ -398,6 +404,26 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                             at = 0;
                             phase ^= 1;
                         }
+                    }
+                }
+            } else if constexpr (SORTED) {
+                const int from = __ldg(p.first_block + w.g) * kDepth + w.first - w.begin;
+                for (int b = 0; b < blocks; ++b) {
+                    alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
+                    if (!alive) break;
+                    const uint32_t dst = stage0 + at * S::kStageBytes, bar = copy_bar(at);
+                    if (elect_one()) {
+                        expect(bar, S::kStageBytes);
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) tile(dst + c * 8192, &feature_map, feature0 + c * 64, from + b * kDepth, bar);
+#pragma unroll
+                        for (int c = 0; c < S::kRows / 64; ++c)
+                            tile(dst + S::kFeatureBytes + c * 8192, &row_map, w.row0 + rank * S::kRows + c * 64, from + b * kDepth, bar);
+                    }
+                    __syncwarp();
+                    if (++at == S::kStages) {
+                        at = 0;
+                        phase ^= 1;
                     }
                 }
             } else {
@@ -518,10 +544,10 @@ Encode encoder() {
     return found;
 }
 
-template <typename T, int MODE, int TN, bool PAIR>
+template <typename T, int MODE, int TN, bool PAIR, bool SORTED = false>
 int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, long long tiles, cudaStream_t stream) {
-    using S = Shape<MODE, TN, PAIR>;
-    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN, PAIR>, S::kSmem));
+    using S = Shape<MODE, TN, PAIR, SORTED>;
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN, PAIR, SORTED>, S::kSmem));
     const int grid = (int)std::min<long long>(tiles, sm_count() / S::kCtas) * S::kCtas;
     if constexpr (PAIR) {
         cudaLaunchConfig_t config = {};
@@ -535,9 +561,9 @@ int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, 
         config.stream = stream;
         config.attrs = &pair;
         config.numAttrs = 1;
-        FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_grouped_tc<T, MODE, TN, PAIR>, p, features, rows));
+        FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_grouped_tc<T, MODE, TN, PAIR, SORTED>, p, features, rows));
     } else {
-        k_grouped_tc<T, MODE, TN, PAIR><<<grid, S::kThreads, S::kSmem, stream>>>(p, features, rows);
+        k_grouped_tc<T, MODE, TN, PAIR, SORTED><<<grid, S::kThreads, S::kSmem, stream>>>(p, features, rows);
     }
     FMB_LAUNCH_CHECK();
     return FMB_OK;
@@ -564,54 +590,133 @@ int launch_rows(Args& p, const CUtensorMap& features, const CUtensorMap& rows, c
     return launch<T, MODE, 32, false>(p, features, rows, tiles, stream);
 }
 
-// weight gradient: columns of a tile, and rows per unit -- all of a group's, or fewer where there are few tiles
-void weight_plan(const fmb_grouped_t* a, int& tn, int& unit_rows) {
-    tn = a->k > 128 ? 256 : 128;
-    const long long tiles = (long long)a->groups * ((a->n + 127) / 128) * ((a->k + tn - 1) / tn);
-    unit_rows = 1 << 30;
+bool by_sixteen(const void* base, long long stride) { return ((uintptr_t)base & 15) == 0 && stride % 8 == 0 && stride > 0; }
+
+// What a call does before its products, and where in its scratch (byte offsets; -1: not needed).
+struct Plan {
+    long long x = -1, y = -1, w = -1, units = -1, first_block = -1, bytes = 0;
+    int tn = 0, unit_rows = 1 << 30;             // weight gradient
+    bool pair = false, sorted = false;
+
+    long long take(long long size) {
+        const long long at = bytes;
+        bytes += (size + 255) / 256 * 256;
+        return at;
+    }
+};
+
+Plan plan_of(const fmb_grouped_t* a, Mode mode) {
+    Plan p;
+    const long long k8 = (a->k + 7) / 8 * 8, n8 = (a->n + 7) / 8 * 8;
+    const bool x_fits = by_sixteen(a->x, a->x_stride), y_fits = by_sixteen(a->y, a->y_stride);
+    if (mode != kWeightGradient) {
+        // the input, and the weights (their strides may be anything where there is one row, or one matrix)
+        if (mode == kLinear && !x_fits) p.x = p.take(a->rows * k8 * 2);
+        if (mode == kInputGradient && !y_fits) p.y = p.take(a->rows * n8 * 2);
+        if (!by_sixteen(a->w, a->k > 1 ? a->w_row_stride : 8) || (a->groups > 1 && (a->w_group_stride % 8 || a->w_group_stride <= 0)))
+            p.w = p.take(a->groups * a->k * n8 * 2);
+        return p;
+    }
+    // Units: all rows of a group, or fewer where that makes few tiles
+    p.tn = a->k > 128 ? 256 : 128;
+    const long long row_tiles = (a->k + p.tn - 1) / p.tn, tiles = a->groups * ((a->n + 127) / 128) * row_tiles;
     if (tiles < 2 * 148 && a->rows > 128) {
         const long long wanted = (2 * 148 + tiles - 1) / tiles * a->groups;      // units in all
-        unit_rows = (int)std::max<long long>(128, (a->rows / wanted + 63) / 64 * 64);
-        if (unit_rows >= a->rows) unit_rows = 1 << 30;
+        const int unit_rows = (int)std::max<long long>(128, (a->rows / wanted + 63) / 64 * 64);
+        if (unit_rows < a->rows) p.unit_rows = unit_rows;
     }
-}
-
-bool maps(const fmb_grouped_t* a, Mode mode, CUtensorMap* features, CUtensorMap* rows) {
-    if (a->type == FMB_TYPE_F32 || a->rows == 0) return false;
-    if (mode == kWeightGradient)
-        return encode_map(features, a->type, a->y, a->n, a->rows, 1, a->y_stride, 0, 1, 2, 64, true) &&
-               encode_map(rows, a->type, a->x, a->k, a->rows, 1, a->x_stride, 0, 1, 2, 64, true);
-    const bool forward = mode == kLinear;
-    return encode_map(features, a->type, a->w, a->n, a->k, a->groups, a->w_row_stride, a->w_group_stride, forward ? 64 : 128, 3, 64, true) &&
-           encode_map(rows, a->type, forward ? a->x : a->y, forward ? a->k : a->n, a->rows, 1, forward ? a->x_stride : a->y_stride, 0, 1, 2, 64, true);
+    if (p.unit_rows < a->rows) p.units = p.take(most_units(a, p.unit_rows) * a->k * a->n * 4);
+    p.pair = p.tn == 256 && a->n > 128 && most_units(a, p.unit_rows) * row_tiles * ((a->n + 255) / 256) >= 74;
+    // Sorting reads and writes every row once, at the rate of memory; gathering costs a CTA pair 1,000 cycles more per 64 rows of a tile.
+    // Against each other per row: 256 (n / 256 + k / 256) x 4 bytes, 1.6e-4 us per 256 columns, and 1.1e-4 us per tile of 256 x 256
+    const long long n_tiles = (a->n + 255) / 256, k_tiles = (a->k + 255) / 256;
+    p.sorted = !x_fits || !y_fits || 2 * n_tiles * k_tiles > 3 * (n_tiles + k_tiles);
+    if (p.sorted) {
+        const long long rows = a->rows + 64ll * a->groups;
+        p.x = p.take(rows * k8 * 2);
+        p.y = p.take(rows * n8 * 2);
+        p.first_block = p.take((a->groups + 1) * 4);
+    }
+    return p;
 }
 
 template <typename T>
-int tma_typed(const fmb_grouped_t* a, Mode mode, const CUtensorMap& features, const CUtensorMap& rows, cudaStream_t stream) {
+int weight_gradient(const fmb_grouped_t* a, const Plan& plan, cudaStream_t stream) {
     Args p;
     p.a = *a;
-    p.row_tiles = 1;
-    if (mode == kWeightGradient) {
-        p.wide_store = four_at_a_time(a->w, a->w_row_stride, 4) && a->w_group_stride % 4 == 0 && a->n % 4 == 0;
-        int tn;
-        weight_plan(a, tn, p.unit_rows);
-        p.row_tiles = ceil_div(a->k, tn);
-        FMB_REQUIRE(p.unit_rows >= a->rows || a->scratch, "fmb_grouped_weight_gradient: null scratch");
-        const long long units = most_units(a, p.unit_rows);
-        const bool pair = tn == 256 && a->n > 128 && units * p.row_tiles * ((a->n + 255) / 256) >= 74;
-        p.feature_tiles = ceil_div(a->n, pair ? 256 : 128);
-        const long long tiles = units * p.feature_tiles * p.row_tiles;
-        const int rc = pair        ? launch<T, kWeightGradient, 256, true>(p, features, rows, tiles, stream)
-                       : tn == 256 ? launch<T, kWeightGradient, 256, false>(p, features, rows, tiles, stream)
-                                   : launch<T, kWeightGradient, 128, false>(p, features, rows, tiles, stream);
-        return rc || p.unit_rows >= a->rows ? rc : sum_units(a, p.unit_rows, stream);
+    p.a.scratch = plan.units >= 0 ? (float*)((char*)a->scratch + plan.units) : nullptr;
+    p.first_block = nullptr;
+    p.wide_store = four_at_a_time(a->w, a->w_row_stride, 4) && a->w_group_stride % 4 == 0 && a->n % 4 == 0;
+    p.unit_rows = plan.unit_rows;
+    p.row_tiles = ceil_div(a->k, plan.tn);
+    p.feature_tiles = ceil_div(a->n, plan.pair ? 256 : 128);
+    const long long tiles = most_units(a, plan.unit_rows) * p.feature_tiles * p.row_tiles;
+    CUtensorMap features, rows;
+    int rc;
+    if (plan.sorted) {
+        void* const x = (char*)a->scratch + plan.x;
+        void* const y = (char*)a->scratch + plan.y;
+        int32_t* const first_block = (int32_t*)((char*)a->scratch + plan.first_block);
+        rc = sort_rows(a, x, y, first_block, stream);
+        if (rc) return rc;
+        p.first_block = first_block;
+        const int all = a->rows + 64 * a->groups;
+        FMB_REQUIRE(encode_map(&features, a->type, y, a->n, all, 1, (a->n + 7) / 8 * 8, 0, 64, 2, 64, true) &&
+                        encode_map(&rows, a->type, x, a->k, all, 1, (a->k + 7) / 8 * 8, 0, 64, 2, 64, true),
+                    "fmb_grouped_weight_gradient: tensor maps");
+        rc = plan.pair        ? launch<T, kWeightGradient, 256, true, true>(p, features, rows, tiles, stream)
+             : plan.tn == 256 ? launch<T, kWeightGradient, 256, false, true>(p, features, rows, tiles, stream)
+                              : launch<T, kWeightGradient, 128, false, true>(p, features, rows, tiles, stream);
+    } else {
+        FMB_REQUIRE(encode_map(&features, a->type, a->y, a->n, a->rows, 1, a->y_stride, 0, 1, 2, 64, true) &&
+                        encode_map(&rows, a->type, a->x, a->k, a->rows, 1, a->x_stride, 0, 1, 2, 64, true),
+                    "fmb_grouped_weight_gradient: tensor maps");
+        rc = plan.pair        ? launch<T, kWeightGradient, 256, true>(p, features, rows, tiles, stream)
+             : plan.tn == 256 ? launch<T, kWeightGradient, 256, false>(p, features, rows, tiles, stream)
+                              : launch<T, kWeightGradient, 128, false>(p, features, rows, tiles, stream);
     }
-    const bool forward = mode == kLinear;
-    const int width = forward ? a->n : a->k;
-    const void* out = forward ? a->y : a->x;
+    return rc || plan.units < 0 ? rc : sum_units(&p.a, plan.unit_rows, stream);
+}
+
+template <typename T>
+int linear(const fmb_grouped_t* a, bool forward, const Plan& plan, cudaStream_t stream) {
+    Args p;
+    p.a = *a;
+    p.first_block = nullptr;
+    p.row_tiles = 1;
+    const int width = forward ? a->n : a->k, depth = forward ? a->k : a->n;
+    const void* const out = forward ? a->y : a->x;
+    const void* in = forward ? a->x : a->y;
+    const void* w = a->w;
+    long long in_stride = forward ? a->x_stride : a->y_stride, w_row = a->w_row_stride, w_group = a->w_group_stride;
     p.feature_tiles = ceil_div(width, 128);
     p.wide_store = ((uintptr_t)out & 15) == 0 && (forward ? a->y_stride : a->x_stride) % 8 == 0 && width % 8 == 0;
+    const long long packed = forward ? plan.x : plan.y;
+    if (packed >= 0) {
+        void* const to = (char*)a->scratch + packed;
+        const int rc = pack_rows(in, in_stride, depth, a->rows, to, stream);
+        if (rc) return rc;
+        in = to;
+        in_stride = (depth + 7) / 8 * 8;
+    }
+    if (plan.w >= 0) {
+        void* const to = (char*)a->scratch + plan.w;
+        const int rc = pack_weights(a, to, stream);
+        if (rc) return rc;
+        w = to;
+        w_row = (a->n + 7) / 8 * 8;
+        w_group = a->k * w_row;
+    }
+    CUtensorMap features, rows;
+    FMB_REQUIRE(encode_map(&features, a->type, w, a->n, a->k, a->groups, w_row, w_group, forward ? 64 : 128, 3, 64, true) &&
+                    encode_map(&rows, a->type, in, depth, a->rows, 1, in_stride, 0, 1, 2, 64, true),
+                "grouped product: tensor maps");
     return forward ? launch_rows<T, kLinear>(p, features, rows, stream) : launch_rows<T, kInputGradient>(p, features, rows, stream);
+}
+
+template <typename T>
+int typed(const fmb_grouped_t* a, Mode mode, const Plan& plan, cudaStream_t stream) {
+    return mode == kWeightGradient ? weight_gradient<T>(a, plan, stream) : linear<T>(a, mode == kLinear, plan, stream);
 }
 
 }  // namespace
@@ -635,17 +740,13 @@ bool encode_map(CUtensorMap* map, int type, const void* base, int columns, int r
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int tma_unit_rows(const fmb_grouped_t* a) {
-    int tn, unit_rows;
-    weight_plan(a, tn, unit_rows);
-    return unit_rows;
-}
+long long tma_scratch_bytes(const fmb_grouped_t* a, Mode mode) { return plan_of(a, mode).bytes; }
 
 int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
-    CUtensorMap features, rows;
-    if (!maps(a, mode, &features, &rows)) return FMB_ERR_UNSUPPORTED;
-    return a->type == FMB_TYPE_BF16 ? tma_typed<__nv_bfloat16>(a, mode, features, rows, stream)
-                                    : tma_typed<__half>(a, mode, features, rows, stream);
+    const Plan plan = plan_of(a, mode);
+    FMB_REQUIRE(plan.bytes == 0 || a->scratch, "grouped product: null scratch");
+    FMB_REQUIRE(((uintptr_t)a->scratch & 255) == 0, "grouped product: scratch starts at a multiple of 256 bytes");
+    return a->type == FMB_TYPE_BF16 ? typed<__nv_bfloat16>(a, mode, plan, stream) : typed<__half>(a, mode, plan, stream);
 }
 
 }  // namespace grp

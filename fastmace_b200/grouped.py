@@ -166,7 +166,12 @@ def _rows_product(what: str, entry: str, source, weight, groups, out, transposed
         x, y, x_stride, y_stride = (there, here, out_stride, stride) if transposed else (here, there, stride, out_stride)
         a = _lib.GroupedStruct(kind, count, rows, k, n, not given, 0, 0, groups[0].data_ptr(), groups[1].data_ptr(), x, y,
                                weight.data_ptr(), x_stride, y_stride, w_row, w_group, None, _status_pointer(index))
-        _lib.check(_launch(index, getattr(lib, entry), ctypes.byref(a)), entry)
+        call = ctypes.byref(a)
+        need = lib.fmb_grouped_scratch(call, int(transposed))
+        if need:
+            scratch = torch.empty(need, dtype=torch.float32, device=source.device)
+            a.scratch = scratch.data_ptr()
+        _lib.check(_launch(index, getattr(lib, entry), call), entry)
     return out
 
 
@@ -205,7 +210,7 @@ def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: Ro
     lib = _lib.load()
     a = _lib.GroupedStruct(kind, count, rows, k, n, 0, bool(accumulate), 0, groups[0].data_ptr(), groups[1].data_ptr(), x.data_ptr(),
                            dy.data_ptr(), out.data_ptr(), x_stride, y_stride, w_row, w_group, None, _status_pointer(index))
-    need = lib.fmb_grouped_scratch(ctypes.byref(a))
+    need = lib.fmb_grouped_scratch(ctypes.byref(a), 2)
     if need:
         scratch = torch.empty(need, dtype=torch.float32, device=x.device)
         a.scratch = scratch.data_ptr()

@@ -441,7 +441,8 @@ typedef struct {
     long long y_stride;
     long long w_row_stride;
     long long w_group_stride;
-    float* scratch;                   /* weight gradient: fmb_grouped_scratch(...) floats, written before they are read */
+    float* scratch;                   /* fmb_grouped_scratch(...) floats from a multiple of 256 bytes on, written before they are
+                                       * read; may be null where that is 0 */
     uint32_t* status;                 /* device word, may be null: receives FMB_STATUS_TENSOR_TIMEOUT */
 } fmb_grouped_t;
 
@@ -452,8 +453,10 @@ FMB_API int fmb_grouped_input_gradient(const fmb_grouped_t* args, fmb_stream_t s
 /* W[g] (+)= sum of x[r]^T y[r] over the rows of group g, in fp32, summed in an order that depends on the sizes alone; zero
  * for groups without rows */
 FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* args, fmb_stream_t stream);
-/* floats of scratch that fmb_grouped_weight_gradient needs for these sizes (fields type, groups, rows, k, n are read) */
-FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* args);
+/* floats of scratch that a call with these arguments needs (all fields but scratch as in the call); which: 0 linear,
+ * 1 input gradient, 2 weight gradient. Operands of 16 bits whose rows do not start at multiples of 16 bytes are copied there, and
+ * the sums of parts of a group's rows held. */
+FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* args, int which);
 
 #define FMB_ADAMW_BLOCK 256           /* values that share a scale where moments are held in 8 bits */
 
