@@ -151,7 +151,8 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                     int begin, end;
                     group_span(p.a.offsets, g, p.a.rows, begin, end);
                     const int units = first_unit[g + 1] - first_unit[g];
-                    mine = ((end - begin + kDepth - 1) / kDepth + 2ll * units) * p.feature_tiles * p.row_tiles;
+                    // a tile takes as long as its blocks or, 128 KB written per CTA, as nine of them
+                    mine = (max((long long)(end - begin + kDepth - 1) / kDepth, 9ll * units) + units) * p.feature_tiles * p.row_tiles;
                 }
                 long long inclusive = mine;
 #pragma unroll
