@@ -5,8 +5,7 @@
 // array. With moments in 8 bits the block shares a scale per moment: first moments are held as e4m3 of m / s, second
 // moments as e4m3 of sqrt(v) / s, s = (largest of the block) / 448. Relative steps of 2^-4 over 2^15 and the root's smaller
 // range keep the quotient m / sqrt(v) to a few per cent of itself; a v that is not zero is never held as zero, which would make
-// the next quotient m / eps. All arithmetic is in fp32, rounded as written: the moments come out with the same bits
-// whatever the compiler contracts, so their 8-bit codes do not depend on it either.
+// the next quotient m / eps. Arithmetic is in fp32.
 //
 // Bound by HBM: 28 bytes a value with fp32 gradients and moments, 16 with 8-bit moments.
 
@@ -16,30 +15,34 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
+#include <type_traits>
+
 namespace fmb {
 
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kBlock = FMB_ADAMW_BLOCK;
-constexpr int kBlocksPerWarp = 2;
-constexpr int kCtaBlocks = kWarps * kBlocksPerWarp;
-constexpr int kMaxTensors = 400;
+constexpr int kCtaBlocks = 16;
+constexpr int kMaxTensors = 400, kFewTensors = 64;        // of a launch: the list is 48 bytes a tensor of kernel arguments
 
 struct Entry {
     float* p;
     const void* g;
     void* copy;
     long long values, block;
-    int cta_begin;               // first CTA of this tensor
+    long long first;             // first block of this tensor among those of the launch
     int wide;                    // every array of the tensor may be read four values at a time
 };
 
+template <int CAPACITY>
 struct Table {
-    Entry entry[kMaxTensors];
+    Entry entry[CAPACITY];
     int count;
     int advance;                 // the last launch of a step counts it
     int copy_type;
+    long long blocks;            // of the launch
     float decay, lr, b1, c1, b2, c2, eps;
     double beta1, beta2;
     void* m;
@@ -53,16 +56,13 @@ __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
-template <typename T> __device__ __forceinline__ void load_four(const T* p, float (&out)[4]) {
-    if constexpr (sizeof(T) == 4) {
-        const float4 q = *reinterpret_cast<const float4*>(p);
-        out[0] = q.x; out[1] = q.y; out[2] = q.z; out[3] = q.w;
-    } else {
-        const uint2 q = *reinterpret_cast<const uint2*>(p);
-        const T* e = reinterpret_cast<const T*>(&q);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) out[i] = to_float(e[i]);
-    }
+template <typename G> __device__ __forceinline__ G zero_of() { return G(0.0f); }
+
+// off by 2^-23 of itself at most, where a code keeps 2^-4; the rounded root takes eight instructions more
+__device__ __forceinline__ float fast_root(float x) {
+    float r;
+    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
 }
 
 __device__ __forceinline__ void decode_four(uint32_t codes, float scale, float (&out)[4]) {
@@ -90,12 +90,13 @@ __device__ __forceinline__ float block_scale(float largest) {
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
 
+// codes of x times 1 / scale; KEEP: what is positive does not become zero
 template <bool KEEP>
-__device__ __forceinline__ uint32_t encode_four(const float (&x)[4], float scale) {
+__device__ __forceinline__ uint32_t encode_four(const float (&x)[4], float inverse) {
     uint32_t out = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const float2 q = make_float2(__fdiv_rn(x[2 * i], scale), __fdiv_rn(x[2 * i + 1], scale));
+        const float2 q = make_float2(x[2 * i] * inverse, x[2 * i + 1] * inverse);
         uint32_t two = __nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3);
         if constexpr (KEEP) {
             if (x[2 * i] > 0.0f && (two & 0xffu) == 0) two |= 1u;
@@ -106,118 +107,172 @@ __device__ __forceinline__ uint32_t encode_four(const float (&x)[4], float scale
     return out;
 }
 
+// What a warp reads of a block: two times four values per lane of every array, as they are held.
 template <typename G, bool EIGHT>
-__global__ void __launch_bounds__(kThreads)
-k_adamw(const __grid_constant__ Table t) {
-    __shared__ float corrections[2];
-    // the tensor of this CTA: the last one that begins at or before it
-    int low = 0, high = t.count - 1;
-    while (low < high) {
-        const int mid = (low + high + 1) >> 1;
-        if (t.entry[mid].cta_begin <= (int)blockIdx.x) low = mid; else high = mid - 1;
+struct Raw {
+    using Four = typename std::conditional<sizeof(G) == 4, float4, uint2>::type;
+    using Moment = typename std::conditional<EIGHT, uint32_t, float4>::type;
+    float4 p[2];
+    Four g[2];
+    Moment m[2], v[2];
+    float m_scale, v_scale;
+    int entry;                   // of the table
+    long long at;                // first value of the block in its tensor
+    bool whole;
+};
+
+template <typename G, bool EIGHT, int CAPACITY>
+__device__ __forceinline__ void load_block(const Table<CAPACITY>& t, long long b, int& entry, Raw<G, EIGHT>& r) {
+    const int lane = threadIdx.x & 31;
+    while (entry + 1 < t.count && t.entry[entry + 1].first <= b) ++entry;
+    const Entry& e = t.entry[entry];
+    r.entry = entry;
+    r.at = (b - e.first) * kBlock;
+    r.whole = e.wide && r.at + kBlock <= e.values;
+    const long long moment = e.block * kBlock + r.at;
+    if constexpr (EIGHT) {
+        r.m_scale = t.m_scale[e.block + r.at / kBlock];
+        r.v_scale = t.v_scale[e.block + r.at / kBlock];
     }
-    const Entry e = t.entry[low];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    using Moment = typename Raw<G, EIGHT>::Moment;
+    constexpr int kHeld = EIGHT ? 1 : 4;                 // bytes of a moment
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = h * 128 + lane * 4;
+        r.m[h] = *reinterpret_cast<const Moment*>((const uint8_t*)t.m + (moment + i) * kHeld);
+        r.v[h] = *reinterpret_cast<const Moment*>((const uint8_t*)t.v + (moment + i) * kHeld);
+        if (r.whole) {
+            r.p[h] = *reinterpret_cast<const float4*>(e.p + r.at + i);
+            r.g[h] = *reinterpret_cast<const typename Raw<G, EIGHT>::Four*>((const G*)e.g + r.at + i);
+        } else {
+            float* const p = reinterpret_cast<float*>(&r.p[h]);
+            G* const g = reinterpret_cast<G*>(&r.g[h]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool live = r.at + i + j < e.values;
+                p[j] = live ? e.p[r.at + i + j] : 0.0f;
+                g[j] = live ? ((const G*)e.g)[r.at + i + j] : zero_of<G>();
+            }
+        }
+    }
+}
+
+template <typename G, bool EIGHT, int CAPACITY>
+__device__ __forceinline__ void step_block(const Table<CAPACITY>& t, const Raw<G, EIGHT>& r, float step, float root_scale) {
+    const int lane = threadIdx.x & 31;
+    const Entry& e = t.entry[r.entry];
+    const long long block = e.block + r.at / kBlock, moment = block * kBlock;
+    float p[2][4], m[2][4], v[2][4], root[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const float* const rp = reinterpret_cast<const float*>(&r.p[h]);
+        const G* const rg = reinterpret_cast<const G*>(&r.g[h]);
+        if constexpr (EIGHT) {
+            decode_four(r.m[h], r.m_scale, m[h]);
+            decode_four(r.v[h], r.v_scale, v[h]);
+        } else {
+            const float* const rm = reinterpret_cast<const float*>(&r.m[h]);
+            const float* const rv = reinterpret_cast<const float*>(&r.v[h]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                m[h][j] = rm[j];
+                v[h][j] = rv[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!r.whole && r.at + h * 128 + lane * 4 + j >= e.values) m[h][j] = v[h][j] = 0.0f;
+            if constexpr (EIGHT) v[h][j] *= v[h][j];
+            const float gr = to_float(rg[j]);
+            m[h][j] = m[h][j] * t.b1 + gr * t.c1;
+            v[h][j] = v[h][j] * t.b2 + gr * t.c2 * gr;
+            root[h][j] = EIGHT ? fast_root(v[h][j]) : __fsqrt_rn(v[h][j]);
+            p[h][j] = rp[j] * t.decay - __fdividef(m[h][j] * step, root[h][j] * root_scale + t.eps);
+        }
+    }
+    float ms = 1.0f, vs = 1.0f;
+    if constexpr (EIGHT) {
+        ms = block_scale(warp_largest(m[0], m[1]));
+        vs = block_scale(warp_largest(root[0], root[1]));
+        if (lane == 0) {
+            t.m_scale[block] = ms;
+            t.v_scale[block] = vs;
+        }
+        ms = __fdiv_rn(1.0f, ms);
+        vs = __fdiv_rn(1.0f, vs);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int i = h * 128 + lane * 4;
+        if constexpr (EIGHT) {
+            *reinterpret_cast<uint32_t*>((uint8_t*)t.m + moment + i) = encode_four<false>(m[h], ms);
+            *reinterpret_cast<uint32_t*>((uint8_t*)t.v + moment + i) = encode_four<true>(root[h], vs);
+        } else {
+            *reinterpret_cast<float4*>((float*)t.m + moment + i) = make_float4(m[h][0], m[h][1], m[h][2], m[h][3]);
+            *reinterpret_cast<float4*>((float*)t.v + moment + i) = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
+        }
+        uint32_t half_bits[2] = {0, 0};
+        if (e.copy) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                if (t.copy_type == FMB_TYPE_BF16) {
+                    const __nv_bfloat162 two = __floats2bfloat162_rn(p[h][2 * q], p[h][2 * q + 1]);
+                    half_bits[q] = *reinterpret_cast<const uint32_t*>(&two);
+                } else {
+                    const __half2 two = __floats2half2_rn(p[h][2 * q], p[h][2 * q + 1]);
+                    half_bits[q] = *reinterpret_cast<const uint32_t*>(&two);
+                }
+            }
+        }
+        if (r.whole) {
+            *reinterpret_cast<float4*>(e.p + r.at + i) = make_float4(p[h][0], p[h][1], p[h][2], p[h][3]);
+            if (e.copy) *reinterpret_cast<uint2*>((uint16_t*)e.copy + r.at + i) = make_uint2(half_bits[0], half_bits[1]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (r.at + i + j < e.values) {
+                    e.p[r.at + i + j] = p[h][j];
+                    if (e.copy) ((uint16_t*)e.copy)[r.at + i + j] = (uint16_t)(half_bits[j >> 1] >> (16 * (j & 1)));
+                }
+        }
+    }
+}
+
+// Moments in 8 bits: as many CTAs as the device holds, whose warps take blocks in turn, so that the whole GPU is at one place of every
+// array; in 32 bits, where a block has twice the bytes to wait for, CTAs of 16 blocks that come and go (200 M values 906 us against
+// 990; the other way round 64 M values in 8 bits 220 against 330). With 8 bits a warp asks for its next block before it works on
+// the one it has; with 32 the registers that takes cost more warps than it gains (1,070 us).
+template <typename G, bool EIGHT, int CAPACITY>
+__global__ void __launch_bounds__(kThreads)
+k_adamw(const __grid_constant__ Table<CAPACITY> t) {
+    __shared__ float corrections[2];
+    const int warp = threadIdx.x >> 5;
+    const long long begin = (long long)blockIdx.x * (EIGHT ? kWarps : kCtaBlocks);
+    const long long end = EIGHT ? t.blocks : min(t.blocks, begin + kCtaBlocks), stride = EIGHT ? (long long)gridDim.x * kWarps : kWarps;
+    long long b = begin + warp;
+    int entry = 0, high = t.count - 1;
+    while (entry < high) {
+        const int mid = (entry + high + 1) >> 1;
+        if (t.entry[mid].first <= b) entry = mid; else high = mid - 1;
+    }
+    Raw<G, EIGHT> raw;
+    if (EIGHT && b < end) load_block<G, EIGHT, CAPACITY>(t, b, entry, raw);
     if (threadIdx.x == 0) {
         corrections[0] = (float)(1.0 / (1.0 - t.state[1] * t.beta1));
         corrections[1] = (float)(1.0 / sqrt(1.0 - t.state[2] * t.beta2));
     }
     __syncthreads();
     const float step = t.lr * corrections[0], root_scale = corrections[1];
-    const G* const grad = (const G*)e.g;
-    const long long first = ((long long)(blockIdx.x - e.cta_begin) * kCtaBlocks + warp) * kBlock;
 #pragma unroll 1
-    for (int b = 0; b < kBlocksPerWarp; ++b) {
-        const long long at = first + (long long)b * kWarps * kBlock;
-        if (at >= e.values) break;
-        const long long block = e.block + at / kBlock, moment = block * kBlock;
-        const bool whole = e.wide && at + kBlock <= e.values;
-        float p[2][4], g[2][4], m[2][4], v[2][4];
-        float ms = 0.0f, vs = 0.0f;
+    for (; b < end; b += stride) {
         if constexpr (EIGHT) {
-            ms = t.m_scale[block];
-            vs = t.v_scale[block];
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int i = h * 128 + lane * 4;
-            if constexpr (EIGHT) {
-                const uint32_t mc = *reinterpret_cast<const uint32_t*>((const uint8_t*)t.m + moment + i);
-                const uint32_t vc = *reinterpret_cast<const uint32_t*>((const uint8_t*)t.v + moment + i);
-                decode_four(mc, ms, m[h]);
-                decode_four(vc, vs, v[h]);
-            } else {
-                load_four((const float*)t.m + moment + i, m[h]);
-                load_four((const float*)t.v + moment + i, v[h]);
-            }
-            if (whole) {
-                load_four((const float*)e.p + at + i, p[h]);
-                load_four(grad + at + i, g[h]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const bool live = at + i + j < e.values;
-                    p[h][j] = live ? e.p[at + i + j] : 0.0f;
-                    g[h][j] = live ? to_float(grad[at + i + j]) : 0.0f;
-                    if (!live) m[h][j] = v[h][j] = 0.0f;
-                }
-            }
-        }
-        float root[2][4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if constexpr (EIGHT) v[h][j] = __fmul_rn(v[h][j], v[h][j]);
-                const float gr = g[h][j];
-                m[h][j] = __fadd_rn(__fmul_rn(m[h][j], t.b1), __fmul_rn(gr, t.c1));
-                v[h][j] = __fadd_rn(__fmul_rn(v[h][j], t.b2), __fmul_rn(__fmul_rn(gr, t.c2), gr));
-                root[h][j] = __fsqrt_rn(v[h][j]);
-                p[h][j] = p[h][j] * t.decay - __fdividef(m[h][j] * step, root[h][j] * root_scale + t.eps);
-            }
-        if constexpr (EIGHT) {
-            const float new_ms = block_scale(warp_largest(m[0], m[1])), new_vs = block_scale(warp_largest(root[0], root[1]));
-            if (lane == 0) {
-                t.m_scale[block] = new_ms;
-                t.v_scale[block] = new_vs;
-            }
-            ms = new_ms;
-            vs = new_vs;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int i = h * 128 + lane * 4;
-            if constexpr (EIGHT) {
-                *reinterpret_cast<uint32_t*>((uint8_t*)t.m + moment + i) = encode_four<false>(m[h], ms);
-                *reinterpret_cast<uint32_t*>((uint8_t*)t.v + moment + i) = encode_four<true>(root[h], vs);
-            } else {
-                *reinterpret_cast<float4*>((float*)t.m + moment + i) = make_float4(m[h][0], m[h][1], m[h][2], m[h][3]);
-                *reinterpret_cast<float4*>((float*)t.v + moment + i) = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
-            }
-            uint32_t half_bits[2] = {0, 0};
-            if (e.copy) {
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    if (t.copy_type == FMB_TYPE_BF16) {
-                        const __nv_bfloat162 two = __floats2bfloat162_rn(p[h][2 * q], p[h][2 * q + 1]);
-                        half_bits[q] = *reinterpret_cast<const uint32_t*>(&two);
-                    } else {
-                        const __half2 two = __floats2half2_rn(p[h][2 * q], p[h][2 * q + 1]);
-                        half_bits[q] = *reinterpret_cast<const uint32_t*>(&two);
-                    }
-                }
-            }
-            if (whole) {
-                *reinterpret_cast<float4*>(e.p + at + i) = make_float4(p[h][0], p[h][1], p[h][2], p[h][3]);
-                if (e.copy) *reinterpret_cast<uint2*>((uint16_t*)e.copy + at + i) = make_uint2(half_bits[0], half_bits[1]);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (at + i + j < e.values) {
-                        e.p[at + i + j] = p[h][j];
-                        if (e.copy) ((uint16_t*)e.copy)[at + i + j] = (uint16_t)(half_bits[j >> 1] >> (16 * (j & 1)));
-                    }
-            }
+            Raw<G, EIGHT> next;
+            if (b + stride < end) load_block<G, EIGHT, CAPACITY>(t, b + stride, entry, next);
+            step_block<G, EIGHT, CAPACITY>(t, raw, step, root_scale);
+            raw = next;
+        } else {
+            load_block<G, EIGHT, CAPACITY>(t, b, entry, raw);
+            step_block<G, EIGHT, CAPACITY>(t, raw, step, root_scale);
         }
     }
     if (!t.advance) return;
@@ -235,15 +290,68 @@ k_adamw(const __grid_constant__ Table t) {
     }
 }
 
-template <typename G>
-int launch(const Table& t, int ctas, bool eight, cudaStream_t stream) {
-    if (eight) k_adamw<G, true><<<ctas, kThreads, 0, stream>>>(t);
-    else k_adamw<G, false><<<ctas, kThreads, 0, stream>>>(t);
+template <typename G, bool EIGHT, int CAPACITY>
+int launch(const Table<CAPACITY>& t, cudaStream_t stream) {
+    long long ctas = (t.blocks + kCtaBlocks - 1) / kCtaBlocks;
+    if (EIGHT) {
+        int dev = 0, sms = 0;
+        static const int per_sm = [] {
+            int n = 0;
+            return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_adamw<G, EIGHT, CAPACITY>, kThreads, 0) == cudaSuccess && n > 0 ? n : 1;
+        }();
+        FMB_CUDA_CHECK(cudaGetDevice(&dev));
+        FMB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+        ctas = std::min<long long>((t.blocks + kWarps - 1) / kWarps, (long long)per_sm * sms);
+    }
+    FMB_REQUIRE(ctas < (1ll << 31), "fmb_adamw_step: too many values");
+    k_adamw<G, EIGHT, CAPACITY><<<(unsigned)ctas, kThreads, 0, stream>>>(t);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
 
+template <typename G, int CAPACITY>
+int launch(const Table<CAPACITY>& t, bool eight, cudaStream_t stream) {
+    return eight ? launch<G, true, CAPACITY>(t, stream) : launch<G, false, CAPACITY>(t, stream);
+}
+
 bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
+
+// the tensors up to `last` that have a gradient
+template <int CAPACITY>
+int step(const fmb_adamw_t* a, const fmb_adamw_tensor_t* tensors, int last, cudaStream_t stream) {
+    const int grad_bytes = a->grad_type == FMB_TYPE_F32 ? 4 : 2;
+    Table<CAPACITY> t;
+    t.copy_type = a->copy_type;
+    t.decay = (float)(1.0 - a->lr * a->weight_decay);
+    t.lr = (float)a->lr;
+    t.b1 = (float)a->beta1; t.c1 = (float)(1.0 - a->beta1);
+    t.b2 = (float)a->beta2; t.c2 = (float)(1.0 - a->beta2);
+    t.eps = (float)a->eps;
+    t.beta1 = a->beta1; t.beta2 = a->beta2;
+    t.m = a->m; t.v = a->v; t.m_scale = a->m_scale; t.v_scale = a->v_scale; t.state = a->state;
+    t.count = 0;
+    t.blocks = 0;
+    for (int i = 0; i <= last; ++i) {
+        const fmb_adamw_tensor_t& s = tensors[i];
+        if (!s.g || s.values == 0) continue;
+        Entry& e = t.entry[t.count++];
+        e.p = s.p; e.g = s.g; e.copy = s.copy; e.values = s.values; e.block = s.block;
+        e.first = t.blocks;
+        e.wide = aligned(s.p, 16) && aligned(s.g, 4 * grad_bytes) && aligned(s.copy, 8);
+        t.blocks += (s.values + kBlock - 1) / kBlock;
+        if (t.count == CAPACITY || i == last) {
+            t.advance = i == last;
+            const bool eight = a->moment_bits == 8;
+            const int rc = a->grad_type == FMB_TYPE_F32    ? launch<float, CAPACITY>(t, eight, stream)
+                           : a->grad_type == FMB_TYPE_BF16 ? launch<__nv_bfloat16, CAPACITY>(t, eight, stream)
+                                                           : launch<__half, CAPACITY>(t, eight, stream);
+            if (rc) return rc;
+            t.count = 0;
+            t.blocks = 0;
+        }
+    }
+    return FMB_OK;
+}
 
 }  // namespace
 
@@ -270,36 +378,6 @@ extern "C" FMB_API int fmb_adamw_step(const fmb_adamw_t* a, const fmb_adamw_tens
         last = i;
     }
     if (last < 0) return FMB_OK;
-    Table t;
-    t.copy_type = a->copy_type;
-    t.decay = (float)(1.0 - a->lr * a->weight_decay);
-    t.lr = (float)a->lr;
-    t.b1 = (float)a->beta1; t.c1 = (float)(1.0 - a->beta1);
-    t.b2 = (float)a->beta2; t.c2 = (float)(1.0 - a->beta2);
-    t.eps = (float)a->eps;
-    t.beta1 = a->beta1; t.beta2 = a->beta2;
-    t.m = a->m; t.v = a->v; t.m_scale = a->m_scale; t.v_scale = a->v_scale; t.state = a->state;
-    t.count = 0;
-    long long ctas = 0;
-    for (int i = 0; i <= last; ++i) {
-        const fmb_adamw_tensor_t& s = tensors[i];
-        if (!s.g || s.values == 0) continue;
-        Entry& e = t.entry[t.count++];
-        e.p = s.p; e.g = s.g; e.copy = s.copy; e.values = s.values; e.block = s.block;
-        e.cta_begin = (int)ctas;
-        e.wide = aligned(s.p, 16) && aligned(s.g, 4 * grad_bytes) && aligned(s.copy, 8);
-        ctas += (s.values + (long long)kCtaBlocks * kBlock - 1) / ((long long)kCtaBlocks * kBlock);
-        FMB_REQUIRE(ctas < (1ll << 31), "fmb_adamw_step: too many values");
-        if (t.count == kMaxTensors || i == last) {
-            t.advance = i == last;
-            const bool eight = a->moment_bits == 8;
-            const int rc = a->grad_type == FMB_TYPE_F32    ? launch<float>(t, (int)ctas, eight, (cudaStream_t)stream)
-                           : a->grad_type == FMB_TYPE_BF16 ? launch<__nv_bfloat16>(t, (int)ctas, eight, (cudaStream_t)stream)
-                                                           : launch<__half>(t, (int)ctas, eight, (cudaStream_t)stream);
-            if (rc) return rc;
-            t.count = 0;
-            ctas = 0;
-        }
-    }
-    return FMB_OK;
+    return last < kFewTensors ? step<kFewTensors>(a, tensors, last, (cudaStream_t)stream)
+                              : step<kMaxTensors>(a, tensors, last, (cudaStream_t)stream);
 }
