@@ -1,7 +1,8 @@
 // Entry points of the grouped products (fmb_grouped_linear and the calls beside it): checks, and which kernel runs.
 //
-// 16-bit operands go by TMA (grouped_tc.cu). fp32 operands are split into bf16 parts on their way (grouped_split.cu); linears of
-// a depth of up to 128 keep the split weights in tensor memory (grouped_resident.cu).
+// 16-bit operands go by TMA (grouped_tc.cu). fp32 operands are split into bf16 parts on their way: the weight gradient in
+// grouped_weights.cu, linears of a depth of up to 128, whose split weights fit in tensor memory, in grouped_resident.cu, the others, and
+// rows that do not start at multiples of 16 bytes, in grouped_split.cu.
 
 #include "grouped.cuh"
 
@@ -49,6 +50,13 @@ k_sum_units(fmb_grouped_t a, int unit_rows) {
     *out = a.accumulate ? *out + sum : sum;
 }
 
+__global__ void __launch_bounds__(256)
+k_zero_weights(fmb_grouped_t a) {
+    const long long size = (long long)a.k * a.n;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < size; i += gridDim.x * 256ll)
+        ((float*)a.w)[blockIdx.y * a.w_group_stride + (i / a.n) * a.w_row_stride + i % a.n] = 0.0f;
+}
+
 int check(const fmb_grouped_t* a) {
     FMB_REQUIRE(a, "grouped product: null argument");
     FMB_REQUIRE(a->type >= FMB_TYPE_F32 && a->type <= FMB_TYPE_F16, "grouped product: type");
@@ -66,8 +74,15 @@ int run(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
     int rc = check(a);
     if (rc) return rc;
     if (a->rows == 0 && mode != kWeightGradient) return FMB_OK;
-    if (a->rows > 0 && a->type != FMB_TYPE_F32) return tma_launch(a, mode, stream);
-    rc = a->rows > 0 ? resident_launch(a, mode, stream) : FMB_ERR_UNSUPPORTED;
+    if (a->rows == 0) {
+        if (a->accumulate) return FMB_OK;
+        k_zero_weights<<<dim3(std::min(ceil_div((long long)a->k * a->n, 256), 4096), a->groups), 256, 0, stream>>>(*a);
+        FMB_LAUNCH_CHECK();
+        return FMB_OK;
+    }
+    if (a->type != FMB_TYPE_F32) return tma_launch(a, mode, stream);
+    if (mode == kWeightGradient) return weights_launch(a, stream);
+    rc = resident_launch(a, mode, stream);
     return rc != FMB_ERR_UNSUPPORTED ? rc : split_launch(a, mode, stream);
 }
 
@@ -104,6 +119,5 @@ extern "C" FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* a, fmb_s
 extern "C" FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* a, int which) {
     if (!a || which < 0 || which > 2 || a->groups < 1 || a->k < 1 || a->n < 1 || a->rows < 1) return 0;
     if (a->type != FMB_TYPE_F32) return tma_scratch_bytes(a, (Mode)which) / 4;
-    const int unit_rows = split_unit_rows(a);
-    return which == 2 && unit_rows < a->rows ? most_units(a, unit_rows) * a->k * a->n : 0;
+    return which == 2 ? weights_scratch(a) : 0;
 }

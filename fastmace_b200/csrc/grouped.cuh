@@ -88,15 +88,18 @@ inline bool four_at_a_time(const void* base, long long stride, int bytes) {
     return ((uintptr_t)base & (uintptr_t)(4 * bytes - 1)) == 0 && stride % 4 == 0;
 }
 
-// fp32 weight gradient: rows per unit (2^30 where units are whole groups), the most units there can be, and the sum
-// over the units of the groups that have several
-int split_unit_rows(const fmb_grouped_t* a);
+// fp32 weight gradient (grouped_weights.cu), and the floats of scratch it needs
+int weights_launch(const fmb_grouped_t* a, cudaStream_t stream);
+long long weights_scratch(const fmb_grouped_t* a);
+
 inline long long most_units(const fmb_grouped_t* a, int unit_rows) { return most_units(a->rows, a->groups, unit_rows); }
+// sums of the units of every group that has more than one, from scratch to w
 int sum_units(const fmb_grouped_t* a, int unit_rows, cudaStream_t stream);
 int sm_count();
 
 // copies into the layouts that TMA takes (grouped_pack.cu)
 int pack_rows(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream);
+int pack_rows_32(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream);
 int pack_weights(const fmb_grouped_t* a, void* dst, cudaStream_t stream);
 int sort_rows(const fmb_grouped_t* a, void* x, void* y, int32_t* first_block, cudaStream_t stream);
 

@@ -45,6 +45,14 @@ k_pack_rows(RowsArgs a, int rows) {
         copy_row(a.dst + r * a.dst_stride, a.src + r * a.src_stride, a.columns, (int)a.dst_stride, a.wide);
 }
 
+// rows of 32-bit values, filled up with zeros to a multiple of four
+__global__ void __launch_bounds__(kThreads)
+k_pack_rows_32(const float* src, long long stride, int columns, float* dst, int rows) {
+    const int lane = threadIdx.x & 31, width = (columns + 3) / 4 * 4;
+    for (int r = (blockIdx.x * kThreads + threadIdx.x) >> 5; r < rows; r += gridDim.x * (kThreads / 32))
+        for (int c = lane; c < width; c += 32) dst[(long long)r * width + c] = c < columns ? __ldg(src + r * stride + c) : 0.0f;
+}
+
 // the matrices of the groups that have rows
 __global__ void __launch_bounds__(kThreads)
 k_pack_weights(fmb_grouped_t a, uint16_t* dst, int width, int wide) {
@@ -94,6 +102,13 @@ RowsArgs rows_args(const void* src, long long stride, int columns, void* dst) {
 int pack_rows(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream) {
     const int grid = std::min(ceil_div(rows, kThreads / 32), 8 * sm_count());
     k_pack_rows<<<grid, kThreads, 0, stream>>>(rows_args(src, stride, columns, dst), rows);
+    FMB_LAUNCH_CHECK();
+    return FMB_OK;
+}
+
+int pack_rows_32(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream) {
+    const int grid = std::min(ceil_div(rows, kThreads / 32), 8 * sm_count());
+    k_pack_rows_32<<<grid, kThreads, 0, stream>>>((const float*)src, stride, columns, (float*)dst, rows);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
