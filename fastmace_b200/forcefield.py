@@ -13,12 +13,14 @@ are simply never read), and forces come from analytic backward kernels, not auto
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import NamedTuple
 
 import numpy as np
 import torch
 
 from . import _lib
+from .grouped import group_rows, grouped_linear_weight_gradient
 from .model import MaceSpec
 from .neighbours import CellListNeighbours, NeighbourConfig
 from .packing import PackedModel
@@ -363,6 +365,38 @@ class B200ForceField:
         _lib.check(self.lib.fmb_forces_phase(self.packed.pointer(), self.neighbours.pointer(), ctypes.byref(self.work),
                                              positions.data_ptr() if positions is not None else None, int(index),
                                              _lib.current_stream()), "fmb_forces_phase")
+
+    def weight_gradients(self) -> dict[str, torch.Tensor]:
+        """Gradient of the last call's energy in the linears of the last interaction: its species-dependent skip
+        (``l{t}.skip.{l}``) and ``linear_up`` (``l{t}.up.{l}``), float32 in the shapes of the weights' dictionary (``model.py``), as
+        ``optimiser.AdamW`` takes them. Elements that no atom has get zeros. The features and gradients that the call left in its
+        workspace are read, so nothing else may have used this force field since. On the current stream; no counterpart in the
+        reference, which evaluates trained models only."""
+        if self.work is None or self.calls == 0:
+            raise _lib.Fmb200Error("weight_gradients: no force call has been made")
+        if self.halo_exchange or not self._same_rows() or 0 <= self.n_owned < self.natoms:
+            raise _lib.Fmb200Error("weight_gradients: the force field must own all of its atoms")
+        spec, n, t = self.spec, self.natoms, self.spec.num_interactions - 1
+        c, hid, elements = spec.channels, (spec.hidden_lmax + 1) ** 2, spec.num_elements
+        # features of the interaction before, the gradient in linear_up's output, and the gradient in the last layer's scalars, which the
+        # forward pass parks in `basis`
+        h = self.buf["h"].view(-1)[:n * hid * c].view(n, hid, c)
+        d_x = self.buf["d_x"][:n]
+        d_out = self.buf["basis"].view(-1)[:n * c].view(n, c)
+        element = torch.tensor(self.packed.species_z, dtype=torch.int32, device=self._device) - 1
+        by_element = group_rows(element[self.species[:n].long()], elements)
+        everyone = group_rows(torch.zeros(n, dtype=torch.int32, device=self._device), 1)
+        out = {}
+        for l in range(spec.skip_lmax(t) + 1):          # the last layer has scalars only
+            g = torch.empty(c, elements, c, dtype=torch.float32, device=self._device)
+            grouped_linear_weight_gradient(h[:, 0], d_out, by_element, out=g.permute(1, 0, 2))
+            out[f"l{t}.skip.{l}"] = g.mul_(1.0 / math.sqrt(c * elements))
+        for l in range(spec.l_in_max(t) + 1):
+            g = torch.empty(c, c, dtype=torch.float32, device=self._device)
+            for m in range(l * l, (l + 1) ** 2):
+                grouped_linear_weight_gradient(h[:, m], d_x[:, m], everyone, out=g[None], accumulate=m > l * l)
+            out[f"l{t}.up.{l}"] = g.mul_(1.0 / math.sqrt(c))
+        return out
 
     def evaluate(self, atoms, stress: bool = False):
         """One-off evaluation (``ForceField.evaluate``): rebuilds the list, synchronises, returns host values:
