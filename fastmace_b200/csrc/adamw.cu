@@ -5,7 +5,9 @@
 // array. With moments in 8 bits the block shares a scale per moment: first moments are held as e4m3 of m / s, second
 // moments as e4m3 of sqrt(v) / s, s = (largest of the block) / 448. Relative steps of 2^-4 over 2^15 and the root's smaller
 // range keep the quotient m / sqrt(v) to a few per cent of itself; a v that is not zero is never held as zero, which would make
-// the next quotient m / eps. Arithmetic is in fp32.
+// the next quotient m / eps. Arithmetic is in fp32, and
+// that of the moments is rounded operation by operation, as it is written here: a moment that came out a bit
+// apart could take the next code, 2^-4 away, and with the block's largest the scale would follow a step later.
 //
 // Bound by HBM: 28 bytes a value with fp32 gradients and moments, 16 with 8-bit moments.
 
@@ -58,13 +60,6 @@ __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 
 template <typename G> __device__ __forceinline__ G zero_of() { return G(0.0f); }
 
-// off by 2^-23 of itself at most, where a code keeps 2^-4; the rounded root takes eight instructions more
-__device__ __forceinline__ float fast_root(float x) {
-    float r;
-    asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
 __device__ __forceinline__ void decode_four(uint32_t codes, float scale, float (&out)[4]) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -86,17 +81,23 @@ __device__ __forceinline__ float warp_largest(const float (&a)[4], const float (
 
 // scale of a block: its largest value becomes 448; blocks of zeros and of the tiniest numbers have a scale all the same
 __device__ __forceinline__ float block_scale(float largest) {
-    const float s = __fdiv_rn(largest, 448.0f);
+    const float s = __fmul_rn(largest, 1.0f / 448.0f);
     return s < 1.17549435e-38f ? 1.17549435e-38f : s;
 }
 
-// codes of x times 1 / scale; KEEP: what is positive does not become zero
+// x / scale from the rounded inverse of the scale, the quotient corrected by its residual (Markstein, 1990)
+__device__ __forceinline__ float quotient(float x, float scale, float inverse) {
+    const float q = __fmul_rn(x, inverse);
+    return fmaf(fmaf(-q, scale, x), inverse, q);
+}
+
+// codes of x / scale; KEEP: what is positive does not become zero
 template <bool KEEP>
-__device__ __forceinline__ uint32_t encode_four(const float (&x)[4], float inverse) {
+__device__ __forceinline__ uint32_t encode_four(const float (&x)[4], float scale, float inverse) {
     uint32_t out = 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const float2 q = make_float2(x[2 * i] * inverse, x[2 * i + 1] * inverse);
+        const float2 q = make_float2(quotient(x[2 * i], scale, inverse), quotient(x[2 * i + 1], scale, inverse));
         uint32_t two = __nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3);
         if constexpr (KEEP) {
             if (x[2 * i] > 0.0f && (two & 0xffu) == 0) two |= 1u;
@@ -182,15 +183,15 @@ __device__ __forceinline__ void step_block(const Table<CAPACITY>& t, const Raw<G
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             if (!r.whole && r.at + h * 128 + lane * 4 + j >= e.values) m[h][j] = v[h][j] = 0.0f;
-            if constexpr (EIGHT) v[h][j] *= v[h][j];
+            if constexpr (EIGHT) v[h][j] = __fmul_rn(v[h][j], v[h][j]);
             const float gr = to_float(rg[j]);
-            m[h][j] = m[h][j] * t.b1 + gr * t.c1;
-            v[h][j] = v[h][j] * t.b2 + gr * t.c2 * gr;
-            root[h][j] = EIGHT ? fast_root(v[h][j]) : __fsqrt_rn(v[h][j]);
+            m[h][j] = __fadd_rn(__fmul_rn(m[h][j], t.b1), __fmul_rn(gr, t.c1));
+            v[h][j] = __fadd_rn(__fmul_rn(v[h][j], t.b2), __fmul_rn(__fmul_rn(gr, t.c2), gr));
+            root[h][j] = __fsqrt_rn(v[h][j]);
             p[h][j] = rp[j] * t.decay - __fdividef(m[h][j] * step, root[h][j] * root_scale + t.eps);
         }
     }
-    float ms = 1.0f, vs = 1.0f;
+    float ms = 1.0f, vs = 1.0f, m_inverse = 1.0f, v_inverse = 1.0f;
     if constexpr (EIGHT) {
         ms = block_scale(warp_largest(m[0], m[1]));
         vs = block_scale(warp_largest(root[0], root[1]));
@@ -198,15 +199,15 @@ __device__ __forceinline__ void step_block(const Table<CAPACITY>& t, const Raw<G
             t.m_scale[block] = ms;
             t.v_scale[block] = vs;
         }
-        ms = __fdiv_rn(1.0f, ms);
-        vs = __fdiv_rn(1.0f, vs);
+        m_inverse = __fdiv_rn(1.0f, ms);
+        v_inverse = __fdiv_rn(1.0f, vs);
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int i = h * 128 + lane * 4;
         if constexpr (EIGHT) {
-            *reinterpret_cast<uint32_t*>((uint8_t*)t.m + moment + i) = encode_four<false>(m[h], ms);
-            *reinterpret_cast<uint32_t*>((uint8_t*)t.v + moment + i) = encode_four<true>(root[h], vs);
+            *reinterpret_cast<uint32_t*>((uint8_t*)t.m + moment + i) = encode_four<false>(m[h], ms, m_inverse);
+            *reinterpret_cast<uint32_t*>((uint8_t*)t.v + moment + i) = encode_four<true>(root[h], vs, v_inverse);
         } else {
             *reinterpret_cast<float4*>((float*)t.m + moment + i) = make_float4(m[h][0], m[h][1], m[h][2], m[h][3]);
             *reinterpret_cast<float4*>((float*)t.v + moment + i) = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
