@@ -1,8 +1,7 @@
 // Entry points of the grouped products (fmb_grouped_linear and the calls beside it): checks, and which kernel runs.
 //
-// 16-bit operands go by TMA (grouped_tc.cu). fp32 operands are split into bf16 parts on their way: the weight gradient in
-// grouped_weights.cu, linears of a depth of up to 128, whose split weights fit in tensor memory, in grouped_resident.cu, the others, and
-// rows that do not start at multiples of 16 bytes, in grouped_split.cu.
+// 16-bit operands: grouped_tc.cu. fp32 operands, split into bf16 parts on their way: grouped_parts.cu, and linears of a depth of up to
+// 128, whose split weights fit in tensor memory, grouped_resident.cu.
 
 #include "grouped.cuh"
 
@@ -71,7 +70,7 @@ int check(const fmb_grouped_t* a) {
 }
 
 int run(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
-    int rc = check(a);
+    const int rc = check(a);
     if (rc) return rc;
     if (a->rows == 0 && mode != kWeightGradient) return FMB_OK;
     if (a->rows == 0) {
@@ -80,10 +79,7 @@ int run(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
         FMB_LAUNCH_CHECK();
         return FMB_OK;
     }
-    if (a->type != FMB_TYPE_F32) return tma_launch(a, mode, stream);
-    if (mode == kWeightGradient) return weights_launch(a, stream);
-    rc = resident_launch(a, mode, stream);
-    return rc != FMB_ERR_UNSUPPORTED ? rc : split_launch(a, mode, stream);
+    return a->type == FMB_TYPE_F32 ? parts_launch(a, mode, stream) : tma_launch(a, mode, stream);
 }
 
 }  // namespace
@@ -118,6 +114,5 @@ extern "C" FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* a, fmb_s
 
 extern "C" FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* a, int which) {
     if (!a || which < 0 || which > 2 || a->groups < 1 || a->k < 1 || a->n < 1 || a->rows < 1) return 0;
-    if (a->type != FMB_TYPE_F32) return tma_scratch_bytes(a, (Mode)which) / 4;
-    return which == 2 ? weights_scratch(a) : 0;
+    return a->type == FMB_TYPE_F32 ? parts_scratch(a, (Mode)which) : tma_scratch_bytes(a, (Mode)which) / 4;
 }

@@ -76,11 +76,8 @@ enum Mode { kLinear = 0, kInputGradient = 1, kWeightGradient = 2 };
 // strides and pointers needs
 int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
 long long tma_scratch_bytes(const fmb_grouped_t* a, Mode mode);
-// tcgen05 kernels whose threads bring the operands (grouped_split.cu): fp32 at any alignment
-int split_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
-
-// tcgen05 kernel that keeps the split weights in tensor memory (grouped_resident.cu): FMB_ERR_UNSUPPORTED unless fp32, a depth of
-// at most 128 and rows that TMA takes
+// tcgen05 kernel that keeps the split weights in tensor memory (grouped_resident.cu): fp32 linears of a depth of at most 128, rows
+// that TMA takes
 int resident_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
 
 // rows that start at multiples of four values, so that they can be read four at a time
@@ -88,9 +85,9 @@ inline bool four_at_a_time(const void* base, long long stride, int bytes) {
     return ((uintptr_t)base & (uintptr_t)(4 * bytes - 1)) == 0 && stride % 4 == 0;
 }
 
-// fp32 weight gradient (grouped_weights.cu), and the floats of scratch it needs
-int weights_launch(const fmb_grouped_t* a, cudaStream_t stream);
-long long weights_scratch(const fmb_grouped_t* a);
+// all fp32 products, and the floats of scratch they need (grouped_parts.cu)
+int parts_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
+long long parts_scratch(const fmb_grouped_t* a, Mode mode);
 
 inline long long most_units(const fmb_grouped_t* a, int unit_rows) { return most_units(a->rows, a->groups, unit_rows); }
 // sums of the units of every group that has more than one, from scratch to w
@@ -101,6 +98,7 @@ int sm_count();
 int pack_rows(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream);
 int pack_rows_32(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream);
 int pack_weights(const fmb_grouped_t* a, void* dst, cudaStream_t stream);
+int pack_weights_32(const fmb_grouped_t* a, void* dst, cudaStream_t stream);
 int sort_rows(const fmb_grouped_t* a, void* x, void* y, int32_t* first_block, cudaStream_t stream);
 
 }  // namespace grp

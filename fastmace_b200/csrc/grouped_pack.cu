@@ -53,6 +53,19 @@ k_pack_rows_32(const float* src, long long stride, int columns, float* dst, int 
         for (int c = lane; c < width; c += 32) dst[(long long)r * width + c] = c < columns ? __ldg(src + r * stride + c) : 0.0f;
 }
 
+__global__ void __launch_bounds__(kThreads)
+k_pack_weights_32(fmb_grouped_t a, float* dst) {
+    const int g = blockIdx.y, lane = threadIdx.x & 31, width = (a.n + 3) / 4 * 4;
+    int begin, end;
+    group_span(a.offsets, g, a.rows, begin, end);
+    if (begin == end) return;
+    for (int r = (blockIdx.x * kThreads + threadIdx.x) >> 5; r < a.k; r += gridDim.x * (kThreads / 32)) {
+        const float* const from = (const float*)a.w + g * a.w_group_stride + r * a.w_row_stride;
+        float* const to = dst + ((long long)g * a.k + r) * width;
+        for (int c = lane; c < width; c += 32) to[c] = c < a.n ? __ldg(from + c) : 0.0f;
+    }
+}
+
 // the matrices of the groups that have rows
 __global__ void __launch_bounds__(kThreads)
 k_pack_weights(fmb_grouped_t a, uint16_t* dst, int width, int wide) {
@@ -109,6 +122,13 @@ int pack_rows(const void* src, long long stride, int columns, int rows, void* ds
 int pack_rows_32(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream) {
     const int grid = std::min(ceil_div(rows, kThreads / 32), 8 * sm_count());
     k_pack_rows_32<<<grid, kThreads, 0, stream>>>((const float*)src, stride, columns, (float*)dst, rows);
+    FMB_LAUNCH_CHECK();
+    return FMB_OK;
+}
+
+int pack_weights_32(const fmb_grouped_t* a, void* dst, cudaStream_t stream) {
+    const int grid = std::min(ceil_div(a->k, kThreads / 32), std::max(1, 16 * sm_count() / a->groups));
+    k_pack_weights_32<<<dim3(grid, a->groups), kThreads, 0, stream>>>(*a, (float*)dst);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }

@@ -1,7 +1,7 @@
 // Grouped linear and its input gradient in fp32 for a depth of up to 128, the linears of a model of 128 channels: the
 // split weights of 128 features stay in tensor memory while a CTA goes through the rows of their group.
 //
-// The numbers and their six products are those of grouped_split.cu. What bounds the work here is memory, 8 bytes per row and
+// The numbers and their six products are those of grouped_parts.cu. What bounds the work here is memory, 8 bytes per row and
 // channel, so the SM's own paths are kept short of that:
 //   * rows come by TMA gather, 4 whole rows an instruction, into a ring of three tiles of 64 rows: 64 KB on their way while
 //     one is worked on (threads' own loads, 32 KB and waits in between, brought 2.2 TB/s);
@@ -333,11 +333,10 @@ int launch(const SplitArgs& p, const CUtensorMap& rows, int wide_out, cudaStream
 int resident_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
     const bool forward = mode == kLinear;
     const int depth = forward ? a->k : a->n, width = forward ? a->n : a->k;
-    if (a->type != FMB_TYPE_F32 || mode == kWeightGradient || depth > kK) return FMB_ERR_UNSUPPORTED;
     CUtensorMap rows;
-    if (!encode_map(&rows, a->type, forward ? a->x : a->y, depth, a->rows, 1, forward ? a->x_stride : a->y_stride, 0, 1, 2,
-                    depth <= 64 ? 64 : 128, false))
-        return FMB_ERR_UNSUPPORTED;
+    FMB_REQUIRE(encode_map(&rows, a->type, forward ? a->x : a->y, depth, a->rows, 1, forward ? a->x_stride : a->y_stride, 0, 1, 2,
+                           depth <= 64 ? 64 : 128, false),
+                "grouped product: tensor maps");
     SplitArgs p;
     p.a = *a;
     p.feature_tiles = ceil_div(width, 128);

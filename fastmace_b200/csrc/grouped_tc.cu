@@ -59,11 +59,6 @@ struct Args {
     const int32_t* first_block;                  // SORTED: blocks of 64 rows of the groups before each
 };
 
-__device__ __forceinline__ void tma_tile_3d(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-                 :: "r"(dst), "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(bar) : "memory");
-}
-
 template <typename T, int MODE, int TN, bool PAIR, bool SORTED>
 __global__ void __launch_bounds__(Shape<MODE, TN, PAIR, SORTED>::kThreads, 1)
 k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap feature_map, const __grid_constant__ CUtensorMap row_map) {
