@@ -17,6 +17,7 @@ __global__ void __launch_bounds__(256)
 k_sum_units(fmb_grouped_t a, int unit_rows) {
     const int g = blockIdx.y;
     __shared__ int first[2];
+    __shared__ float parts[4][64];
     if (threadIdx.x < 32) {
         int before = 0;
         for (int q = threadIdx.x; q < g; q += 32) {
@@ -33,18 +34,26 @@ k_sum_units(fmb_grouped_t a, int unit_rows) {
         }
     }
     __syncthreads();
-    if (first[1] <= 1 || first[0] + first[1] > most_units(a.rows, a.groups, unit_rows)) return;
-    const long long size = (long long)a.k * a.n, i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= size) return;
-    const float* at = a.scratch + first[0] * size + i;
+    const int units = first[1];
+    if (units <= 1 || first[0] + units > most_units(a.rows, a.groups, unit_rows)) return;
+    // four threads share a sum: with one each, 49,152 values of 37 units took 11 us for their round trips
+    const long long size = (long long)a.k * a.n, i = (long long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int part = threadIdx.x >> 6, from = units * part / 4, to = units * (part + 1) / 4;
     float sum = 0.0f;
-    for (int u = 0; u < first[1]; u += 8) {
-        float v[8];
+    if (i < size) {
+        const float* const at = a.scratch + first[0] * size + i;
+        for (int u = from; u < to; u += 8) {
+            float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = u + j < first[1] ? at[(u + j) * size] : 0.0f;
+            for (int j = 0; j < 8; ++j) v[j] = u + j < to ? at[(u + j) * size] : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum += v[j];
+            for (int j = 0; j < 8; ++j) sum += v[j];
+        }
     }
+    parts[part][threadIdx.x & 63] = sum;
+    __syncthreads();
+    if (part > 0 || i >= size) return;
+    sum = (sum + parts[1][threadIdx.x]) + (parts[2][threadIdx.x] + parts[3][threadIdx.x]);
     float* const out = (float*)a.w + g * a.w_group_stride + (i / a.n) * a.w_row_stride + i % a.n;
     *out = a.accumulate ? *out + sum : sum;
 }
@@ -85,7 +94,7 @@ int run(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
 }  // namespace
 
 int sum_units(const fmb_grouped_t* a, int unit_rows, cudaStream_t stream) {
-    k_sum_units<<<dim3(ceil_div((long long)a->k * a->n, 256), a->groups), 256, 0, stream>>>(*a, unit_rows);
+    k_sum_units<<<dim3(ceil_div((long long)a->k * a->n, 64), a->groups), 256, 0, stream>>>(*a, unit_rows);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
