@@ -14,7 +14,9 @@ is float32 whatever the operands'. A row of no group (key negative or >= the num
 allocates, left as it was in one that is given, and takes no part in a weight gradient.
 
 Calls run on the current stream of the operands' device and allocate their outputs and scratch from torch's allocator, so
-they can be captured. There is no autograd and no CPU path.
+they can be captured, after one call of the same kind outside a capture. The groups are read on the device: nothing synchronises,
+and a captured call may be replayed on other groups. A kernel that gives up waiting raises nothing by itself: ``check_status``.
+There is no autograd and no CPU path.
 """
 
 from __future__ import annotations
@@ -207,6 +209,10 @@ def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: Ro
     else:
         _on_device(what, x, out)
     _, _, _, w_group, w_row = _weights(what, "out", out)
+    far, near, inner = (max(w_row, w_group), min(w_row, w_group), k if w_group >= w_row else count)
+    if k > 1 and count > 1 and (near < n or far < (inner - 1) * near + n) or k > 1 and count == 1 and w_row < n or \
+            k == 1 and count > 1 and w_group < n:
+        raise ValueError(f"{what}: the matrices of out overlap")
     lib = _lib.load()
     a = _lib.GroupedStruct(kind, count, rows, k, n, 0, bool(accumulate), 0, groups[0].data_ptr(), groups[1].data_ptr(), x.data_ptr(),
                            dy.data_ptr(), out.data_ptr(), x_stride, y_stride, w_row, w_group, None, _status_pointer(index))

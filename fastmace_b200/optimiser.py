@@ -54,6 +54,9 @@ class AdamW:
                 raise ValueError("AdamW: the weights must be CUDA tensors, there is no CPU path")
             if p.dtype != torch.float32 or not p.is_contiguous() or p.device != self.device:
                 raise ValueError("AdamW: the weights must be contiguous float32 tensors on one device")
+        held = [p.data_ptr() for p in self.params if p.numel()]
+        if len(set(held)) < len(held):
+            raise ValueError("AdamW: a tensor is listed twice")
         self.copies = [None] * len(self.params) if copies is None else [copies[k] for k in self.names]
         self._copy_type = 0
         for p, c in zip(self.params, self.copies):
@@ -132,7 +135,8 @@ class AdamW:
 
     def load_moments(self, steps: int, *moments: torch.Tensor) -> None:
         """Continue from the moments of a run of ``steps`` steps: ``m, v`` (32 bits) or ``m, m_scale, v, v_scale`` (8 bits), as
-        this class holds them under these names. The optimiser uses the tensors given, it does not copy them."""
+        this class holds them under these names. The optimiser uses the tensors given, it does not copy them; a step captured before
+        goes on with the ones it had."""
         names = ("m", "v") if self.state_bits == 32 else ("m", "m_scale", "v", "v_scale")
         if len(moments) != len(names) or steps < 0:
             raise ValueError(f"AdamW.load_moments: steps and {', '.join(names)}")

@@ -174,7 +174,7 @@ def test_values_that_are_not_finite_or_zero():
 def test_refusals_on_the_device():
     from fastmace_b200.optimiser import AdamW
     w = torch.zeros(8, 8, device="cuda")
-    for bad in (lambda: AdamW([]), lambda: AdamW([w.half()]), lambda: AdamW([w.t()[:4]]), lambda: AdamW([w], state_bits=16),
+    for bad in (lambda: AdamW([]), lambda: AdamW([w.half()]), lambda: AdamW([w.t()[:4]]), lambda: AdamW([w], state_bits=16), lambda: AdamW([w, w]),
                 lambda: AdamW([w], betas=(1.0, 0.9)), lambda: AdamW([w], lr=-1.0), lambda: AdamW([w], copies=[w]),
                 lambda: AdamW([w], copies=[w.half()[:4]]), lambda: AdamW([w]).step([w, w]), lambda: AdamW([w]).step([w.double()]),
                 lambda: AdamW([w]).step([w[:4]]), lambda: AdamW([w]).step([w.t()]), lambda: AdamW({"a": w}).step({"b": w}),

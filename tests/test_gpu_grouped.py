@@ -79,7 +79,7 @@ SHAPES = [(1, 1, 1, 1, "even", 1), (1, 3, 128, 128, "one", 1), (7, 64, 64, 32, "
           (200, 5, 128, 128, "even", 4), (257, 3, 65, 129, "uneven", 1), (100, 9, 1, 200, "even", 1), (90, 4, 200, 1, "even", 3),
           (513, 17, 100, 72, "uneven", 1), (1000, 7, 130, 515, "even", 1), (640, 2, 264, 384, "one", 2),
           (300, 6, 128, 64, "none", 1), (5000, 8, 128, 128, "uneven", 4), (129, 1024, 48, 56, "even", 1),
-          (20_000, 7, 200, 1096, "uneven", 1), (9000, 30, 520, 264, "even", 1), (2500, 3, 1024, 256, "even", 1), (700, 2, 2056, 136, "uneven", 1), (16, 4, 4096, 512, "even", 1)]
+          (20_000, 7, 200, 1096, "uneven", 1), (9000, 30, 520, 264, "even", 1), (6000, 5, 1032, 1040, "uneven", 2), (2500, 3, 1024, 256, "even", 1), (700, 2, 2056, 136, "uneven", 1), (16, 4, 4096, 512, "even", 1)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
@@ -275,16 +275,17 @@ def test_row_numbers_out_of_range_are_skipped():
         _check_weights(grouped.grouped_linear_weight_gradient(x, dy, bad), x, dy, keys)
 
 
-def test_captured_calls_and_another_stream():
+@pytest.mark.parametrize("dtype,rows,k,n", [(F32, 9000, 96, 160), (F32, 9000, 300, 260), (BF16, 20_000, 264, 1096), (F16, 9000, 1025, 515)])
+def test_captured_calls_and_another_stream(dtype, rows, k, n):
     """A captured run of grouping, product and gradients, replayed on new inputs while another stream runs its own."""
     from fastmace_b200 import grouped
     grouped.prepare_device()
     g = torch.Generator(device="cuda").manual_seed(9)
 
     def inputs():
-        return (torch.randint(0, 6, (9000,), generator=g, device="cuda", dtype=torch.int32),
-                torch.randn(9000, 96, generator=g, device="cuda"), torch.randn(6, 96, 160, generator=g, device="cuda"),
-                torch.randn(9000, 160, generator=g, device="cuda"))
+        return (torch.randint(0, 6, (rows,), generator=g, device="cuda", dtype=torch.int32),
+                torch.randn(rows, k, generator=g, device="cuda").to(dtype), torch.randn(6, k, n, generator=g, device="cuda").to(dtype),
+                torch.randn(rows, n, generator=g, device="cuda").to(dtype))
 
     def calls(keys, x, w, dy):
         plan = grouped.group_rows(keys, 6)
@@ -314,6 +315,24 @@ def test_captured_calls_and_another_stream():
             assert torch.equal(a, c) and torch.equal(b, c)
         for a, c in zip(beside, calls(*other)):
             assert torch.equal(a, c)
+    grouped.check_status()
+
+
+@pytest.mark.parametrize("dtype,k,n", [(F32, 128, 128), (F32, 200, 140), (BF16, 1032, 1040), (BF16, 264, 1096), (BF16, 130, 515)])
+def test_weight_gradients_add_up(dtype, k, n):
+    """accumulate=True over groups of one unit, of several and of none."""
+    from fastmace_b200 import grouped
+    g = torch.Generator(device="cuda").manual_seed(12)
+    keys = torch.cat([torch.zeros(3, dtype=torch.int32), torch.full((2990,), 2, dtype=torch.int32), torch.full((7,), 4, dtype=torch.int32)]).cuda()
+    keys = keys[torch.randperm(3000, generator=g, device="cuda")]
+    plan = grouped.group_rows(keys, 5)
+    x = torch.randn(3000, k, generator=g, device="cuda").to(dtype)
+    dy = torch.randn(3000, n, generator=g, device="cuda").to(dtype)
+    base = torch.randn(5, k, n, generator=g, device="cuda")
+    out = base.clone()
+    assert grouped.grouped_linear_weight_gradient(x, dy, plan, out=out, accumulate=True) is out
+    _check_weights(out, x, dy, keys, base=base)
+    assert torch.equal(out[[1, 3]], base[[1, 3]])
 
 
 def test_offsets_beyond_32_bits():
@@ -350,6 +369,8 @@ def test_refusals_on_the_device():
                 lambda: grouped.grouped_linear_weight_gradient(x, x[:7], plan),
                 lambda: grouped.grouped_linear_weight_gradient(x, x, plan, accumulate=True),
                 lambda: grouped.grouped_linear_weight_gradient(x, x, plan, out=torch.zeros(2, 16, 15, device="cuda")),
+                lambda: grouped.grouped_linear_weight_gradient(x, x, plan, out=torch.zeros(1, 16, 16, device="cuda").expand(2, 16, 16)),
+                lambda: grouped.grouped_linear_weight_gradient(x, x, plan, out=torch.zeros(40, device="cuda").as_strided((2, 16, 16), (1, 1, 1))),
                 lambda: grouped.group_rows(torch.zeros(8, device="cuda"), 2),
                 lambda: grouped.group_rows(torch.zeros(8, dtype=torch.int32, device="cuda"), 1025)):
         with pytest.raises(ValueError):
