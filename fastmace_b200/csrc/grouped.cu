@@ -12,50 +12,61 @@ namespace grp {
 
 namespace {
 
-// sums of the units of every group that has more than one, in the order of its entries
+// Sums of the units of every group that has more than one, in the order of its entries. A thread has four values, side by side where
+// `wide`; 4 or 16 threads share the units of a value where there are many (49,152 values of 37 units took 11 us with one each, for
+// their round trips, and 6 with four). Groups of one unit cost their blocks only, and of those there is a bounded number.
 __global__ void __launch_bounds__(256)
-k_sum_units(fmb_grouped_t a, int unit_rows) {
+k_sum_units(fmb_grouped_t a, int unit_rows, int wide) {
     const int g = blockIdx.y;
-    __shared__ int first[2];
-    __shared__ float parts[4][64];
-    if (threadIdx.x < 32) {
-        int before = 0;
-        for (int q = threadIdx.x; q < g; q += 32) {
-            int begin, end;
-            group_span(a.offsets, q, a.rows, begin, end);
-            before += end > begin ? (end - begin - 1) / unit_rows + 1 : 1;
+    int begin, end;
+    group_span(a.offsets, g, a.rows, begin, end);
+    const int units = end > begin ? (end - begin - 1) / unit_rows + 1 : 1;
+    if (units <= 1) return;
+    __shared__ float4 parts[256];
+    const int share = units > 64 ? 16 : units > 12 ? 4 : 1, threads = 256 / share;
+    const int thread = threadIdx.x % threads, part = threadIdx.x / threads, from = units * part / share, to = units * (part + 1) / share;
+    const long long size = (long long)a.k * a.n;
+    const int step = wide ? 1 : threads;
+    for (long long first = (long long)blockIdx.x * 4 * threads; first < size; first += (long long)gridDim.x * 4 * threads) {
+        // this thread's values: i, i + step, ...
+        const long long i = first + (wide ? 4 * thread : thread);
+        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int u = from; u < to; u += 4) {
+            float v[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float* const at = a.scratch + unit_slot(begin, u + j, units, unit_rows) * size + i;
+                if (wide) {
+                    const float4 q = u + j < to && i < size ? *reinterpret_cast<const float4*>(at) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    v[j][0] = q.x; v[j][1] = q.y; v[j][2] = q.z; v[j][3] = q.w;
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) v[j][c] = u + j < to && i + c * step < size ? at[c * step] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) sum[c] += v[j][c];
         }
-        before = warp_sum(before);
-        int begin, end;
-        group_span(a.offsets, g, a.rows, begin, end);
-        if (threadIdx.x == 0) {
-            first[0] = before;
-            first[1] = end > begin ? (end - begin - 1) / unit_rows + 1 : 1;
+        if (share > 1) {
+            __syncthreads();                                      // what was here has been read
+            parts[threadIdx.x] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+            __syncthreads();
+            if (part > 0) continue;
+            for (int q = 1; q < share; ++q) {
+                const float4 v = parts[q * threads + thread];
+                sum[0] += v.x; sum[1] += v.y; sum[2] += v.z; sum[3] += v.w;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const long long one = i + c * step;
+            if (one >= size) break;
+            float* const out = (float*)a.w + g * a.w_group_stride + (one / a.n) * a.w_row_stride + one % a.n;
+            *out = a.accumulate ? *out + sum[c] : sum[c];
         }
     }
-    __syncthreads();
-    const int units = first[1];
-    if (units <= 1 || first[0] + units > most_units(a.rows, a.groups, unit_rows)) return;
-    // four threads share a sum: with one each, 49,152 values of 37 units took 11 us for their round trips
-    const long long size = (long long)a.k * a.n, i = (long long)blockIdx.x * 64 + (threadIdx.x & 63);
-    const int part = threadIdx.x >> 6, from = units * part / 4, to = units * (part + 1) / 4;
-    float sum = 0.0f;
-    if (i < size) {
-        const float* const at = a.scratch + first[0] * size + i;
-        for (int u = from; u < to; u += 8) {
-            float v[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = u + j < to ? at[(u + j) * size] : 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) sum += v[j];
-        }
-    }
-    parts[part][threadIdx.x & 63] = sum;
-    __syncthreads();
-    if (part > 0 || i >= size) return;
-    sum = (sum + parts[1][threadIdx.x]) + (parts[2][threadIdx.x] + parts[3][threadIdx.x]);
-    float* const out = (float*)a.w + g * a.w_group_stride + (i / a.n) * a.w_row_stride + i % a.n;
-    *out = a.accumulate ? *out + sum : sum;
 }
 
 __global__ void __launch_bounds__(256)
@@ -94,7 +105,9 @@ int run(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
 }  // namespace
 
 int sum_units(const fmb_grouped_t* a, int unit_rows, cudaStream_t stream) {
-    k_sum_units<<<dim3(ceil_div((long long)a->k * a->n, 64), a->groups), 256, 0, stream>>>(*a, unit_rows);
+    const long long size = (long long)a->k * a->n;
+    const int wide = size % 4 == 0 && ((uintptr_t)a->scratch & 15) == 0, blocks = std::max(1, 32 * sm_count() / a->groups);
+    k_sum_units<<<dim3(std::min(ceil_div(size, 64), blocks), a->groups), 256, 0, stream>>>(*a, unit_rows, wide);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }

@@ -60,6 +60,14 @@ __device__ __forceinline__ int units_in_all(const int* first, int groups, int ro
     return (int)min((long long)max(0, first[groups]), most_units(rows, groups, size));
 }
 
+// Where the sums of unit u of a group's `units` lie, in units: at its first entry's multiple of the size, behind the end of the group
+// before. No two are alike: units that begin within one size of each other are the last of a group and one of the next group that is
+// not the last, or that group has one unit and is not kept.
+__host__ __device__ __forceinline__ long long unit_slot(int begin, int u, int units, int size) {
+    return 2ll * (begin / size + u) + (u == units - 1);
+}
+__host__ __device__ __forceinline__ long long unit_slots(int rows, int size) { return 2ll * (rows / size + 1); }
+
 // the group that unit u belongs to: the last one that begins at or before it
 __device__ __forceinline__ int group_of_unit(const int* first, int groups, int u) {
     int low = 0, high = groups - 1;

@@ -262,7 +262,7 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
             float* out;
             if constexpr (kWeights) {
                 stride = direct ? p.a.w_row_stride : p.a.n;
-                out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + (long long)w.unit * p.a.k * p.a.n) + feature;
+                out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + w.slot * p.a.k * p.a.n) + feature;
             } else {
                 stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
                 out = (float*)(MODE == kLinear ? p.a.y : p.a.x) + feature;
@@ -370,14 +370,12 @@ Plan plan_of(const fmb_grouped_t* a, Mode mode) {
             p.w = whole(a->groups * a->k * n4);
         return p;
     }
-    // a unit per SM where there is not a tile for each; none of less than 64 rows
-    const long long tiles = a->groups * ((a->n + 127) / 128) * (long long)((a->k + 127) / 128);
-    if (tiles < 148) {
-        const long long wanted = std::max<long long>(1, 148 * a->groups / tiles - a->groups);
-        const int unit_rows = (int)std::max<long long>(64, (a->rows / wanted + 31) / 32 * 32);
-        if (unit_rows < a->rows) p.unit_rows = unit_rows;
-    }
-    if (p.unit_rows < a->rows) p.units = whole(most_units(a, p.unit_rows) * a->k * a->n);
+    // a unit per SM where there is not a tile for each; else a group's rows, cut at an SM's share of the work; none of less than 64
+    const long long of_group = ((a->n + 127) / 128) * (long long)((a->k + 127) / 128), tiles = a->groups * of_group;
+    const long long units = tiles < 148 ? std::max<long long>(1, 148 * a->groups / tiles - a->groups) : std::max<long long>(1, 148 / of_group);
+    const long long unit_rows = std::max<long long>(64, (a->rows / units + 31) / 32 * 32);
+    if (unit_rows < a->rows) p.unit_rows = (int)unit_rows;
+    if (p.unit_rows < a->rows) p.units = whole(unit_slots(a->rows, p.unit_rows) * a->k * a->n);
     return p;
 }
 

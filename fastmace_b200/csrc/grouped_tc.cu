@@ -221,7 +221,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 const bool direct = w.units <= 1;
                 const long long stride = direct ? p.a.w_row_stride : p.a.n;
                 const int feature = w.feature0 * S::kCtas + rank * 128 + 4 * lane, live = p.a.n - feature;
-                float* const out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + (long long)w.unit * p.a.k * p.a.n) + feature;
+                float* const out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + w.slot * p.a.k * p.a.n) + feature;
                 const bool add = direct && p.a.accumulate, wide = direct ? p.wide_store : p.a.n % 4 == 0;
                 const int row0 = w.row0 + set * kCols;
 #pragma unroll
@@ -613,15 +613,15 @@ Plan plan_of(const fmb_grouped_t* a, Mode mode) {
             p.w = p.take(a->groups * a->k * n8 * 2);
         return p;
     }
-    // Units: all rows of a group, or fewer where that makes few tiles
+    // Units: a group's rows, cut at half an SM's share of the work, so that every SM has some and one long group does not keep the
+    // others waiting (208,333 rows of 64 x 512 in 103 groups, the largest of 40,000: 173 us, and 305 uncut). Where the tiles of one
+    // group are enough for a quarter of the SMs, a launch for sums costs more than balance gives (16,384 rows of 2,048 x 1,024 in 32
+    // groups: 155 us, and 160 with it)
     p.tn = a->k > 128 ? 256 : 128;
-    const long long row_tiles = (a->k + p.tn - 1) / p.tn, tiles = a->groups * ((a->n + 127) / 128) * row_tiles;
-    if (tiles < 2 * 148 && a->rows > 128) {
-        const long long wanted = (2 * 148 + tiles - 1) / tiles * a->groups;      // units in all
-        const int unit_rows = (int)std::max<long long>(128, (a->rows / wanted + 63) / 64 * 64);
-        if (unit_rows < a->rows) p.unit_rows = unit_rows;
-    }
-    if (p.unit_rows < a->rows) p.units = p.take(most_units(a, p.unit_rows) * a->k * a->n * 4);
+    const long long row_tiles = (a->k + p.tn - 1) / p.tn, of_group = ((a->n + 127) / 128) * row_tiles;
+    const long long unit_rows = std::max<long long>(128, (a->rows * of_group / (2 * 148) + 63) / 64 * 64);
+    if (unit_rows < a->rows && (a->groups * of_group < 2 * 148 || of_group < 148 / 4)) p.unit_rows = (int)unit_rows;
+    if (p.unit_rows < a->rows) p.units = p.take(unit_slots(a->rows, p.unit_rows) * a->k * a->n * 4);
     p.pair = p.tn == 256 && a->n > 128 && most_units(a, p.unit_rows) * row_tiles * ((a->n + 255) / 256) >= 74;
     // Sorting reads and writes every row once, at the rate of memory; gathering costs a CTA pair 1,000 cycles more per 64 rows of a tile.
     // Against each other per row: 256 (n / 256 + k / 256) x 4 bytes, 1.6e-4 us per 256 columns, and 1.1e-4 us per tile of 256 x 256

@@ -144,11 +144,12 @@ struct Walk {
     int groups, rows, unit_rows, feature_tiles, per_unit, tile_rows;
     int g, local, units, begin, end;             // group, tile of it, its units, its span
     int unit, feature0, row0, first, count;      // the tile
+    long long slot;                              // of its unit in the scratch
 
     __device__ __forceinline__ Walk(const fmb_grouped_t& a, const int* first_unit, int unit_rows, int feature_tiles, int row_tiles, int tile_rows)
         : offsets(a.offsets), first_unit(first_unit), groups(a.groups), rows(a.rows), unit_rows(unit_rows), feature_tiles(feature_tiles),
           per_unit(feature_tiles * row_tiles), tile_rows(tile_rows), g(0), local(0), units(1), begin(0), end(0),
-          unit(0), feature0(0), row0(0), first(0), count(0) {}
+          unit(0), feature0(0), row0(0), first(0), count(0), slot(0) {}
 
     __device__ __forceinline__ void enter() {
         units = max(1, first_unit[g + 1] - first_unit[g]);
@@ -157,6 +158,7 @@ struct Walk {
     __device__ __forceinline__ void place() {
         const int rest = local / units, skip = local - rest * units, rt = rest / feature_tiles;
         unit = first_unit[g] + skip;
+        slot = min(unit_slot(begin, skip, units, unit_rows), unit_slots(rows, unit_rows) - 1);
         row0 = rt * tile_rows;
         feature0 = (rest - rt * feature_tiles) * 128;
         // offsets that are none could make a unit that lies outside its group: it has no entries. (In 64 bits: as the minimum of

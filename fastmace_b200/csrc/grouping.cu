@@ -147,7 +147,8 @@ k_group_place(const K* __restrict__ keys, long long rows, int groups, int bits, 
     const long long first = (long long)blockIdx.x * kRowsPerCta;
     int g[kKeys], rank[kKeys];
     load_keys(keys, first + warp * kRowsPerWarp, rows, groups, g);
-    for (int i = threadIdx.x; i < kWarps * width; i += kThreads) counts[i] = 0;
+    const int warps = ALONE ? (int)((rows + kRowsPerWarp - 1) / kRowsPerWarp) : kWarps;        // that have rows
+    for (int i = threadIdx.x; i < warps * width; i += kThreads) counts[i] = 0;
     if (!ALONE)
         for (int q = threadIdx.x; q < width; q += kThreads) starts[q] = totals[q];
     unsigned same[kKeys];
@@ -165,7 +166,8 @@ k_group_place(const K* __restrict__ keys, long long rows, int groups, int bits, 
     __syncthreads();
     for (int q = warp; q < width; q += kWarps) {
         int all;
-        counts[lane * width + q] = warps_before(counts[lane * width + q], all);
+        const int before = warps_before(lane < warps ? counts[lane * width + q] : 0, all);
+        if (lane < warps) counts[lane * width + q] = before;
         if (lane == 0) here[q] = all;
     }
     __syncthreads();

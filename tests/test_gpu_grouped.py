@@ -126,6 +126,30 @@ def test_long_groups_against_float64(shape, dtype):
     _check_rows(grouped.grouped_linear(x, w, plan), x, w, keys)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("groups,k,n", [(310, 100, 60), (170, 130, 190), (60, 264, 600), (1024, 8, 3)])
+def test_weight_gradient_of_a_long_group_among_short_ones(groups, k, n, dtype):
+    """Many groups, of which one has two rows in three and another a fifth: these are cut, the others are not."""
+    from fastmace_b200 import grouped
+    rows = 24_001
+    rng = np.random.default_rng(groups)
+    keys = rng.integers(-1, groups, rows)
+    draw = rng.random(rows)
+    keys[draw < 0.66], keys[draw > 0.8] = groups // 2, groups - 1
+    keys = torch.tensor(keys, dtype=torch.int32, device="cuda")
+    plan = grouped.group_rows(keys, groups)
+    g = torch.Generator(device="cuda").manual_seed(groups)
+    x = torch.randn(rows, k, generator=g, device="cuda").to(dtype)
+    dy = torch.randn(rows, n, generator=g, device="cuda").to(dtype)
+    dw = grouped.grouped_linear_weight_gradient(x, dy, plan)
+    _check_weights(dw, x, dy, keys)
+    base = torch.randn(groups, k, n, generator=g, device="cuda")
+    added = grouped.grouped_linear_weight_gradient(x, dy, plan, out=base.clone(), accumulate=True)
+    _check_weights(added, x, dy, keys, base)
+    assert torch.equal(dw, grouped.grouped_linear_weight_gradient(x, dy, plan))
+    grouped.check_status()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_order_of_magnitude_extremes(dtype):
     """Values from 2^-60 to 2^60 of one matrix: float32 operands keep their 24 bits at every size."""
