@@ -1,4 +1,4 @@
-// What the kernels of the grouped products share: spans of the groups, units of work, conversions.
+// What the kernels of the grouped products share: spans of the groups, units of work.
 #pragma once
 
 #include "fmb_common.cuh"
@@ -9,11 +9,7 @@
 namespace fmb {
 namespace grp {
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 template <typename T> __device__ __forceinline__ T from_float(float x);
-template <> __device__ __forceinline__ float from_float<float>(float x) { return x; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 template <> __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 

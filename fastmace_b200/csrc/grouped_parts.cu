@@ -54,18 +54,18 @@ __device__ __forceinline__ uint64_t plane_desc(uint32_t smem_addr) {
 // one side of a block, 128 x 32 values in rows of memory, by 128 threads into its planes
 template <bool K_MAJOR>
 __device__ __forceinline__ void split_side(const float4* raw, uint8_t* plane, int i) {
-    Quad<float> q[8];
+    float4 q[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) q[j].v = raw[i + j * 128];
+    for (int j = 0; j < 8; ++j) q[j] = raw[i + j * 128];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const int idx = i + j * 128;
         if constexpr (K_MAJOR) {
             const int row = idx >> 3, quad = idx & 7;
-            store_quad<float, kPart>(plane, (uint32_t)(row * 64 + (((quad >> 1) ^ ((row >> 1) & 3)) << 4) + (quad & 1) * 8), q[j]);
+            store_quad<kPart>(plane, (uint32_t)(row * 64 + (((quad >> 1) ^ ((row >> 1) & 3)) << 4) + (quad & 1) * 8), q[j]);
         } else {
             const int depth = idx >> 5, quad = idx & 31;
-            store_quad<float, kPart>(plane, (quad >> 4) * kChunkTile + quad_offset(depth, quad & 15), q[j]);
+            store_quad<kPart>(plane, (quad >> 4) * kChunkTile + quad_offset(depth, quad & 15), q[j]);
         }
     }
 }
@@ -421,7 +421,6 @@ int parts_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
     if (rc) return rc;
     if (mode != kWeightGradient && (mode == kLinear ? a->k : a->n) <= 128) return resident_launch(&p.a, mode, stream);
     CUtensorMap features, rows;
-    p.wide_features = p.wide_rows = 1;
     if (mode == kWeightGradient) {
         FMB_REQUIRE(encode_map(&features, a->type, p.a.y, a->n, a->rows, 1, p.a.y_stride, 0, 1, 2, 128, false) &&
                         encode_map(&rows, a->type, p.a.x, a->k, a->rows, 1, p.a.x_stride, 0, 1, 2, 128, false),

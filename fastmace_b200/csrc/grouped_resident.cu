@@ -49,8 +49,8 @@ __device__ __forceinline__ void bring_weights(const SplitArgs& p, const Walk& w,
         if constexpr (MODE == kInputGradient) {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-                const Quad<float> q = load_quad(from + d0 + i, live ? depth - d0 - i : 0, p.wide_features);
-                v[i] = q.v.x; v[i + 1] = q.v.y; v[i + 2] = q.v.z; v[i + 3] = q.v.w;
+                const float4 q = load_quad(from + d0 + i, live ? depth - d0 - i : 0, p.wide_features);
+                v[i] = q.x; v[i + 1] = q.y; v[i + 2] = q.z; v[i + 3] = q.w;
             }
         } else {
 #pragma unroll
@@ -280,11 +280,11 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
             const int s = n & 1;
             alive = mbar_wait(raw_full(at), raw_phase, abort_flag, kSpin);
             if (!alive) break;
-            Quad<float> q[8];
+            float4 q[8];
             const float4* const raw = reinterpret_cast<const float4*>(smem + at * kRawBytes);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                if (j < 4 || columns == 128) q[j].v = raw[i + j * 256];
+                if (j < 4 || columns == 128) q[j] = raw[i + j * 256];
             __syncwarp();
             if (lane == 0) mbar_arrive(raw_empty(at));
             alive = mbar_wait(plane_empty(s), ((n >> 1) & 1) ^ 1, abort_flag, kSpin);
@@ -294,7 +294,7 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
             for (int j = 0; j < 8; ++j)
                 if (j < 4 || columns == 128) {
                     const int idx = i + j * 256, row = idx >> row_shift, quad = idx & ((1 << row_shift) - 1);
-                    store_quad<float, 2 * kPlaneTile>(plane, (quad >> 4) * kPlaneTile + quad_offset(row, quad & 15), q[j]);
+                    store_quad<2 * kPlaneTile>(plane, (quad >> 4) * kPlaneTile + quad_offset(row, quad & 15), q[j]);
                 }
             fence_async_smem();
             __syncwarp();
@@ -343,7 +343,6 @@ int resident_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
     p.row_tiles = 1;
     p.unit_rows = kTN;
     p.wide_features = four_at_a_time(a->w, a->w_row_stride, 4) && a->w_group_stride % 4 == 0;
-    p.wide_rows = 1;
     const int wide_out = width % 4 == 0 && four_at_a_time(forward ? a->y : a->x, forward ? a->y_stride : a->x_stride, 4);
     return forward ? launch<kLinear>(p, rows, wide_out, stream) : launch<kInputGradient>(p, rows, wide_out, stream);
 }

@@ -9,8 +9,13 @@
 // a run of the output row: 32 lanes store 64 or 128 consecutive bytes.
 //
 // Rows are where the groups' order says: they come by TMA gather (four row numbers an instruction), which fills what is no row
-// with zeros; nothing is permuted in memory. Weights come by TMA tiles from the caller's layout. Operands whose depth runs along
-// memory are K-major tiles, the others MN-major ones; both with the 128-byte swizzle.
+// with zeros, so that the linears permute nothing in memory. Of the weight gradient the same holds where it has few tiles; where
+// it has many, each of which would gather its rows anew, both matrices are first laid by groups (plan_of). Weights come by TMA
+// tiles from the caller's layout. Operands whose depth runs along memory are K-major tiles, the others MN-major ones; both with
+// the 128-byte swizzle. What TMA cannot take (rows or weights at no multiple of 16 bytes) is copied to aligned rows first.
+//
+// What bounds it: few rows, the bytes of the weights (8 rows, 8 groups of 2,048 x 2,048: see launch_rows); many, the tensor cores
+// (16,384 rows of 4,096 x 4,096 in 4 groups: 1.52 PFLOP/s) and with deep gathers the 30 cycles that one takes.
 
 #include "grouped_tc.cuh"
 
@@ -33,9 +38,10 @@ template <int MODE, int TN, bool PAIR, bool SORTED> struct Shape {
     static constexpr int kFeatureBytes = 128 * kDepth * 2, kRowBytes = kRows * kDepth * 2;
     static constexpr int kStageBytes = kFeatureBytes + kRowBytes;
     static constexpr int kRowsPerWarp = PAIR ? 16 : 32, kQuads = kRowsPerWarp / 4;
-    // Warps that issue copies: of the linears warp 0 for the features, the others for rows, 32 each; of the weight gradient one
-    // per 64 columns of y or x. One warp takes 30 cycles a gather, and 64 (96) of them feed 512 cycles of MMAs. Then the warp
-    // that issues MMAs, and eight that take results out, two sets of four.
+    // Warps that issue copies: of the linears warp 0 for the features, the others for rows, 32 (16 of a pair) each; of the weight
+    // gradient one per 64 columns of y or x, or one in all where the rows are sorted. An SM takes in a gather (512 bytes) every 18
+    // cycles at best, one warp issues one every 30. Then the warp that issues MMAs, and eight that take results out, two sets of
+    // four.
     static constexpr int kGathers = kWeights ? 2 + kRows / 64 : kRows / kRowsPerWarp, kCopyWarps = SORTED ? 1 : kWeights ? kGathers : 1 + kGathers;
     static constexpr int kMmaWarp = kCopyWarps;
     static constexpr int kFirstEpilogue = kWeights ? 8 : kMmaWarp + 1;             // whole warpgroups, so that registers can be dealt
@@ -131,10 +137,10 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     // Tiles of the linears cost the same, and go round. Those of the weight gradient cost what their group has rows: every CTA (pair)
     // takes consecutive tiles of the same cost in all (sizes that differ by a factor of three cost 40 % where tiles went round).
-    const int walkers = gridDim.x / S::kCtas, walker = blockIdx.x / S::kCtas, all_tiles = units_in_all(first_unit, p.a.groups, p.a.rows, p.unit_rows) * p.feature_tiles * p.row_tiles;
+    const int walkers = gridDim.x / S::kCtas, walker = blockIdx.x / S::kCtas;
+    const int all_tiles = units_in_all(first_unit, p.a.groups, p.a.rows, p.unit_rows) * p.feature_tiles * p.row_tiles;
     int t_first = walker, t_end = all_tiles;
-    constexpr bool kRound = !kWeights;
-    const int t_step = kRound ? walkers : 1;
+    const int t_step = kWeights ? 1 : walkers;
     if constexpr (kWeights) {
         long long* const cost = reinterpret_cast<long long*>(smem + S::kCosts0);
         if (warp == 0) {
@@ -310,200 +316,197 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
             }
         }
     } else {
-    if constexpr (kWeights) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-    if (warp < S::kCopyWarps) {
-        // ---------------------------------------------------------------- copies
-        int at = 0;
-        uint32_t phase = 0;
-        bool alive = true;
-        // The row numbers of this warp's gathers, in shared memory: read four at a time at an address the whole warp shares,
-        // they get to the gather on the short way (with shuffles 47 cycles a gather, lanes that issue their own 62).
-        int4* const rows = reinterpret_cast<int4*>(smem + S::kRows0 + warp * 512);
-        int* const my_rows = reinterpret_cast<int*>(rows) + 2 * lane;
-        auto row_or_zeros = [&](int entry, int end) {
-            const int row = row_at(p, entry, end);
-            return row < 0 ? p.a.rows : row;               // TMA fills what is past the last row with zeros
-        };
-        // weight gradient: the tile and block whose row numbers come next
-        Walk ahead = w;
-        int ahead_tile = t_first, ahead_block = -1, next0 = p.a.rows, next1 = p.a.rows, buffer = 0;
-        auto look_ahead = [&] {
-            ++ahead_block;
-            while (ahead_tile < t_end && ahead_block * kDepth >= ahead.count) {
-                ahead_block = 0;
-                if (++ahead_tile < t_end) ahead.step(1);
+        if constexpr (kWeights) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp < S::kCopyWarps) {
+            // ---------------------------------------------------------------- copies
+            int at = 0;
+            uint32_t phase = 0;
+            bool alive = true;
+            auto advance = [&] {
+                if (++at == S::kStages) {
+                    at = 0;
+                    phase ^= 1;
+                }
+            };
+            // The row numbers of this warp's gathers, in shared memory: read four at a time at an address the whole warp shares,
+            // they get to the gather on the short way (with shuffles 47 cycles a gather, lanes that issue their own 62).
+            int4* const rows = reinterpret_cast<int4*>(smem + S::kRows0 + warp * 512);
+            int* const my_rows = reinterpret_cast<int*>(rows) + 2 * lane;
+            auto row_or_zeros = [&](int entry, int end) {
+                const int row = row_at(p, entry, end);
+                return row < 0 ? p.a.rows : row;               // TMA fills what is past the last row with zeros
+            };
+            // weight gradient: the tile and block whose row numbers come next
+            Walk ahead = w;
+            int ahead_tile = t_first, ahead_block = -1, next0 = p.a.rows, next1 = p.a.rows, buffer = 0;
+            auto look_ahead = [&] {
+                ++ahead_block;
+                while (ahead_tile < t_end && ahead_block * kDepth >= ahead.count) {
+                    ahead_block = 0;
+                    if (++ahead_tile < t_end) ahead.step(1);
+                }
+                if (ahead_tile >= t_end) return;
+                const int end = ahead.first + ahead.count;
+                next0 = row_or_zeros(ahead.first + ahead_block * kDepth + 2 * lane, end);
+                next1 = row_or_zeros(ahead.first + ahead_block * kDepth + 2 * lane + 1, end);
+            };
+            if (kWeights && !SORTED && t_first < t_end) {
+                // row numbers are asked for two blocks ahead, and put in place one ahead, across tiles
+                ahead.start(t_first);
+                look_ahead();
+                my_rows[0] = next0;
+                my_rows[1] = next1;
+                look_ahead();
             }
-            if (ahead_tile >= t_end) return;
-            const int end = ahead.first + ahead.count;
-            next0 = row_or_zeros(ahead.first + ahead_block * kDepth + 2 * lane, end);
-            next1 = row_or_zeros(ahead.first + ahead_block * kDepth + 2 * lane + 1, end);
-        };
-        if (kWeights && !SORTED && t_first < t_end) {
-            // row numbers are asked for two blocks ahead, and put in place one ahead, across tiles
-            ahead.start(t_first);
-            look_ahead();
-            my_rows[0] = next0;
-            my_rows[1] = next1;
-            look_ahead();
-        }
-        for (int t = t_first; alive && t < t_end; t += t_step) {
-            if (t == t_first) w.start(t);
-            else w.step(t_step);
-            const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
-            const int end = w.first + w.count, feature0 = w.feature0 * S::kCtas + rank * 128;
-            if constexpr (!kWeights) {
-                if (warp > 0) {
-                    // of a pair's MMA columns the first half are CTA 0's rows
-                    const int half = PAIR ? (w.count + 31) / 32 * 16 : TN, mine = min(half, max(0, w.count - rank * half));
-                    const int quads = min(S::kQuads, max(0, (mine + 3) / 4 - (warp - 1) * S::kQuads));
-                    const int entry = w.first + rank * half + (warp - 1) * S::kRowsPerWarp + 2 * lane;
-                    __syncwarp();
-                    if (lane < S::kRowsPerWarp / 2) {
-                        my_rows[0] = row_or_zeros(entry, end);
-                        my_rows[1] = row_or_zeros(entry + 1, end);
-                    }
-                    __syncwarp();
-                    for (int b = 0; b < blocks; ++b) {
-                        alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
-                        if (!alive) break;
-                        const uint32_t dst = stage0 + at * S::kStageBytes + S::kFeatureBytes + (warp - 1) * S::kQuads * 512, bar = copy_bar(at);
-                        if (elect_one()) {
-                            expect(bar, quads * 512);
-#pragma unroll
-                            for (int q = 0; q < S::kQuads; ++q) {
-                                const int4 r = rows[q];
-                                if (q < quads) gather(dst + q * 512, &row_map, b * kDepth, r, bar);
-                            }
+            for (int t = t_first; alive && t < t_end; t += t_step) {
+                if (t == t_first) w.start(t);
+                else w.step(t_step);
+                const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
+                const int end = w.first + w.count, feature0 = w.feature0 * S::kCtas + rank * 128;
+                if constexpr (!kWeights) {
+                    if (warp > 0) {
+                        // of a pair's MMA columns the first half are CTA 0's rows
+                        const int half = PAIR ? (w.count + 31) / 32 * 16 : TN, mine = min(half, max(0, w.count - rank * half));
+                        const int quads = min(S::kQuads, max(0, (mine + 3) / 4 - (warp - 1) * S::kQuads));
+                        const int entry = w.first + rank * half + (warp - 1) * S::kRowsPerWarp + 2 * lane;
+                        __syncwarp();
+                        if (lane < S::kRowsPerWarp / 2) {
+                            my_rows[0] = row_or_zeros(entry, end);
+                            my_rows[1] = row_or_zeros(entry + 1, end);
                         }
                         __syncwarp();
-                        if (++at == S::kStages) {
-                            at = 0;
-                            phase ^= 1;
+                        for (int b = 0; b < blocks; ++b) {
+                            alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
+                            if (!alive) break;
+                            const uint32_t dst = stage0 + at * S::kStageBytes + S::kFeatureBytes + (warp - 1) * S::kQuads * 512, bar = copy_bar(at);
+                            if (elect_one()) {
+                                expect(bar, quads * 512);
+#pragma unroll
+                                for (int q = 0; q < S::kQuads; ++q) {
+                                    const int4 r = rows[q];
+                                    if (q < quads) gather(dst + q * 512, &row_map, b * kDepth, r, bar);
+                                }
+                            }
+                            __syncwarp();
+                            advance();
+                        }
+                    } else {
+                        for (int b = 0; b < blocks; ++b) {
+                            alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
+                            if (!alive) break;
+                            const uint32_t dst = stage0 + at * S::kStageBytes, bar = copy_bar(at);
+                            if (elect_one()) {
+                                expect(bar, S::kFeatureBytes);
+                                if constexpr (MODE == kLinear) {
+                                    box(dst, feature0, b * kDepth, w.g, bar);
+                                    box(dst + 8192, feature0 + 64, b * kDepth, w.g, bar);
+                                } else {
+                                    box(dst, b * kDepth, feature0, w.g, bar);
+                                }
+                            }
+                            __syncwarp();
+                            advance();
                         }
                     }
-                } else {
+                } else if constexpr (SORTED) {
+                    const int from = __ldg(p.first_block + w.g) * kDepth + w.first - w.begin;
                     for (int b = 0; b < blocks; ++b) {
                         alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
                         if (!alive) break;
                         const uint32_t dst = stage0 + at * S::kStageBytes, bar = copy_bar(at);
                         if (elect_one()) {
-                            expect(bar, S::kFeatureBytes);
-                            if constexpr (MODE == kLinear) {
-                                box(dst, feature0, b * kDepth, w.g, bar);
-                                box(dst + 8192, feature0 + 64, b * kDepth, w.g, bar);
-                            } else {
-                                box(dst, b * kDepth, feature0, w.g, bar);
+                            expect(bar, S::kStageBytes);
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) tile(dst + c * 8192, &feature_map, feature0 + c * 64, from + b * kDepth, bar);
+#pragma unroll
+                            for (int c = 0; c < S::kRows / 64; ++c)
+                                tile(dst + S::kFeatureBytes + c * 8192, &row_map, w.row0 + rank * S::kRows + c * 64, from + b * kDepth, bar);
+                        }
+                        __syncwarp();
+                        advance();
+                    }
+                } else {
+                    const CUtensorMap* const map = warp < 2 ? &feature_map : &row_map;
+                    const int column = warp < 2 ? feature0 + warp * 64 : w.row0 + rank * S::kRows + (warp - 2) * 64;
+                    for (int b = 0; b < blocks; ++b, buffer ^= 64) {
+                        my_rows[(buffer ^ 64)] = next0;
+                        my_rows[(buffer ^ 64) + 1] = next1;
+                        look_ahead();
+                        __syncwarp();
+                        alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
+                        if (!alive) break;
+                        const uint32_t dst = stage0 + at * S::kStageBytes + warp * 8192, bar = copy_bar(at);
+                        const int quads = min(16, (w.count - b * kDepth + 15) / 16 * 4);     // depths past the end, up to a multiple of 16, are zeros
+                        const int4* const mine = rows + buffer / 4;
+                        if (elect_one()) {
+                            expect(bar, quads * 512);
+#pragma unroll 4
+                            for (int q = 0; q < quads; ++q) {
+                                const int4 r = mine[q];
+                                gather(dst + q * 512, map, column, r, bar);
                             }
                         }
                         __syncwarp();
-                        if (++at == S::kStages) {
-                            at = 0;
-                            phase ^= 1;
-                        }
-                    }
-                }
-            } else if constexpr (SORTED) {
-                const int from = __ldg(p.first_block + w.g) * kDepth + w.first - w.begin;
-                for (int b = 0; b < blocks; ++b) {
-                    alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
-                    if (!alive) break;
-                    const uint32_t dst = stage0 + at * S::kStageBytes, bar = copy_bar(at);
-                    if (elect_one()) {
-                        expect(bar, S::kStageBytes);
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) tile(dst + c * 8192, &feature_map, feature0 + c * 64, from + b * kDepth, bar);
-#pragma unroll
-                        for (int c = 0; c < S::kRows / 64; ++c)
-                            tile(dst + S::kFeatureBytes + c * 8192, &row_map, w.row0 + rank * S::kRows + c * 64, from + b * kDepth, bar);
-                    }
-                    __syncwarp();
-                    if (++at == S::kStages) {
-                        at = 0;
-                        phase ^= 1;
-                    }
-                }
-            } else {
-                const CUtensorMap* const map = warp < 2 ? &feature_map : &row_map;
-                const int column = warp < 2 ? feature0 + warp * 64 : w.row0 + rank * S::kRows + (warp - 2) * 64;
-                for (int b = 0; b < blocks; ++b, buffer ^= 64) {
-                    my_rows[(buffer ^ 64)] = next0;
-                    my_rows[(buffer ^ 64) + 1] = next1;
-                    look_ahead();
-                    __syncwarp();
-                    alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
-                    if (!alive) break;
-                    const uint32_t dst = stage0 + at * S::kStageBytes + warp * 8192, bar = copy_bar(at);
-                    const int quads = min(16, (w.count - b * kDepth + 15) / 16 * 4);     // depths past the end, up to a multiple of 16, are zeros
-                    const int4* const mine = rows + buffer / 4;
-                    if (elect_one()) {
-                        expect(bar, quads * 512);
-#pragma unroll 4
-                        for (int q = 0; q < quads; ++q) {
-                            const int4 r = mine[q];
-                            gather(dst + q * 512, map, column, r, bar);
-                        }
-                    }
-                    __syncwarp();
-                    if (++at == S::kStages) {
-                        at = 0;
-                        phase ^= 1;
+                        advance();
                     }
                 }
             }
-        }
-    } else if (warp == kMmaWarp && rank == 0) {
-        // ---------------------------------------------------------------- MMAs
-        int at = 0, acc = 0;
-        uint32_t phase = 0, acc_phase = 0;
-        constexpr uint32_t kType = __is_same(T, __nv_bfloat16) ? 1 : 0;
-        constexpr uint32_t kMajor = MODE == kLinear ? 1u << 15 : MODE == kWeightGradient ? 3u << 15 : 0;
-        constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | kMajor | ((uint32_t)(128 * S::kCtas >> 4) << 24);
-        bool alive = true;
-        for (int t = t_first; alive && t < t_end; t += t_step) {
-            if (t == t_first) w.start(t);
-            else w.step(t_step);
-            const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
-            constexpr int kUnit = 16 * S::kCtas;
-            const int columns = kWeights ? TN : max(kUnit, min(TN, (w.count + kUnit - 1) / kUnit * kUnit));
-            const uint32_t idesc = kDesc | ((uint32_t)(columns >> 3) << 17);
-            for (int b = 0; b < blocks; ++b) {
-                const bool fresh = b == 0 || (kWeights && b % (kChunk / kDepth) == 0);
-                if (fresh) alive = mbar_wait(acc_empty(acc), acc_phase ^ 1, abort_flag, kSpin);
-                alive = alive && mbar_wait(full(at), phase, abort_flag, kSpin);
-                if (!alive) break;
-                fence_after_sync();
-                const uint32_t base = stage0 + at * S::kStageBytes;
-                const uint64_t fd = MODE == kInputGradient ? make_desc(base) : make_desc_mn(base);
-                const uint64_t rd = kWeights ? make_desc_mn(base + S::kFeatureBytes) : make_desc(base + S::kFeatureBytes);
-                const int steps = min(4, (depth - b * kDepth + 15) / 16);
-                const uint32_t d = tmem + acc * TN;
-                if (elect_one()) {
-                    for (int k = 0; k < steps; ++k) {
-                        constexpr uint64_t kF = MODE == kInputGradient ? 2 : 128, kR = kWeights ? 128 : 2;
-                        if constexpr (PAIR) mma_f16_pair(d, fd + k * kF, rd + k * kR, idesc, k > 0 || !fresh);
-                        else mma_f16(d, fd + k * kF, rd + k * kR, idesc, k > 0 || !fresh);
-                    }
-                    const bool last = b == blocks - 1 || (kWeights && (b + 1) % (kChunk / kDepth) == 0);
-                    if constexpr (PAIR) {
-                        mma_commit_pair(empty(at));
-                        if (last) mma_commit_pair(acc_full(acc));
-                    } else {
-                        mma_commit(empty(at));
-                        if (last) mma_commit(acc_full(acc));
-                    }
-                }
-                __syncwarp();
-                if (b == blocks - 1 || (kWeights && (b + 1) % (kChunk / kDepth) == 0)) {
-                    acc ^= 1;
-                    if (acc == 0) acc_phase ^= 1;
-                }
+        } else if (warp == kMmaWarp && rank == 0) {
+            // ---------------------------------------------------------------- MMAs
+            int at = 0, acc = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            auto advance = [&] {
                 if (++at == S::kStages) {
                     at = 0;
                     phase ^= 1;
                 }
+            };
+            constexpr uint32_t kType = __is_same(T, __nv_bfloat16) ? 1 : 0;
+            constexpr uint32_t kMajor = MODE == kLinear ? 1u << 15 : MODE == kWeightGradient ? 3u << 15 : 0;
+            constexpr uint32_t kDesc = (1u << 4) | (kType << 7) | (kType << 10) | kMajor | ((uint32_t)(128 * S::kCtas >> 4) << 24);
+            bool alive = true;
+            for (int t = t_first; alive && t < t_end; t += t_step) {
+                if (t == t_first) w.start(t);
+                else w.step(t_step);
+                const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
+                constexpr int kUnit = 16 * S::kCtas;
+                const int columns = kWeights ? TN : max(kUnit, min(TN, (w.count + kUnit - 1) / kUnit * kUnit));
+                const uint32_t idesc = kDesc | ((uint32_t)(columns >> 3) << 17);
+                for (int b = 0; b < blocks; ++b) {
+                    const bool fresh = b == 0 || (kWeights && b % (kChunk / kDepth) == 0);
+                    if (fresh) alive = mbar_wait(acc_empty(acc), acc_phase ^ 1, abort_flag, kSpin);
+                    alive = alive && mbar_wait(full(at), phase, abort_flag, kSpin);
+                    if (!alive) break;
+                    fence_after_sync();
+                    const uint32_t base = stage0 + at * S::kStageBytes;
+                    const uint64_t fd = MODE == kInputGradient ? make_desc(base) : make_desc_mn(base);
+                    const uint64_t rd = kWeights ? make_desc_mn(base + S::kFeatureBytes) : make_desc(base + S::kFeatureBytes);
+                    const int steps = min(4, (depth - b * kDepth + 15) / 16);
+                    const uint32_t d = tmem + acc * TN;
+                    if (elect_one()) {
+                        for (int k = 0; k < steps; ++k) {
+                            constexpr uint64_t kF = MODE == kInputGradient ? 2 : 128, kR = kWeights ? 128 : 2;
+                            if constexpr (PAIR) mma_f16_pair(d, fd + k * kF, rd + k * kR, idesc, k > 0 || !fresh);
+                            else mma_f16(d, fd + k * kF, rd + k * kR, idesc, k > 0 || !fresh);
+                        }
+                        const bool last = b == blocks - 1 || (kWeights && (b + 1) % (kChunk / kDepth) == 0);
+                        if constexpr (PAIR) {
+                            mma_commit_pair(empty(at));
+                            if (last) mma_commit_pair(acc_full(acc));
+                        } else {
+                            mma_commit(empty(at));
+                            if (last) mma_commit(acc_full(acc));
+                        }
+                    }
+                    __syncwarp();
+                    if (b == blocks - 1 || (kWeights && (b + 1) % (kChunk / kDepth) == 0)) {
+                        acc ^= 1;
+                        if (acc == 0) acc_phase ^= 1;
+                    }
+                    advance();
+                }
             }
         }
-    }
     }
     fence_before_sync();
     __syncthreads();
@@ -623,8 +626,10 @@ Plan plan_of(const fmb_grouped_t* a, Mode mode) {
     if (unit_rows < a->rows && (a->groups * of_group < 2 * 148 || of_group < 148 / 4)) p.unit_rows = (int)unit_rows;
     if (p.unit_rows < a->rows) p.units = p.take(unit_slots(a->rows, p.unit_rows) * a->k * a->n * 4);
     p.pair = p.tn == 256 && a->n > 128 && most_units(a, p.unit_rows) * row_tiles * ((a->n + 255) / 256) >= 74;
-    // Sorting reads and writes every row once, at the rate of memory; gathering costs a CTA pair 1,000 cycles more per 64 rows of a tile.
-    // Against each other per row: 256 (n / 256 + k / 256) x 4 bytes, 1.6e-4 us per 256 columns, and 1.1e-4 us per tile of 256 x 256
+    // Sorting reads and writes every row once, at the rate of memory; gathering costs a CTA pair 1,000 cycles more per 64 rows of a
+    // tile. Against each other per row: 256 (n / 256 + k / 256) x 4 bytes, 1.6e-4 us per 256 columns, and 1.1e-4 us per tile of
+    // 256 x 256. In us, sorted and gathered: 16,384 rows of 2,048 x 1,024: 155, 217; 65,536 of 2,048 x 2,048: 626, 1,111; 30,000 of
+    // 1,024 x 1,024: 132, 189; 30,000 of 256 x 512: 77, 71; 300,000 of 128 x 128: 132, 89.
     const long long n_tiles = (a->n + 255) / 256, k_tiles = (a->k + 255) / 256;
     p.sorted = !x_fits || !y_fits || 2 * n_tiles * k_tiles > 3 * (n_tiles + k_tiles);
     if (p.sorted) {

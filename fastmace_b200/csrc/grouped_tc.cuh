@@ -127,12 +127,12 @@ __device__ __forceinline__ void tmem_load_32(uint32_t taddr, float (&v)[32]) {
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
 
-// ------------------------------------------------------------------------------------------------ operands brought by threads
+// ------------------------------------------------------------------------------------------------ fp32 as three bf16 parts
 
 struct SplitArgs {
     fmb_grouped_t a;
     int feature_tiles, row_tiles, unit_rows;
-    int wide_features, wide_rows;                // operands that may be read four values at a time
+    int wide_features;                           // weights that may be read four values at a time (grouped_resident.cu)
 };
 
 // The tiles of a launch, group by group; of a group all units (entries [first, first + count) of `order`) for the same features
@@ -194,56 +194,23 @@ __device__ __forceinline__ int row_at(const ARGS& p, int entry, int end) {
     return (unsigned)row < (unsigned)p.a.rows ? row : -1;
 }
 
-template <typename T> struct Quad { uint2 v; };
-template <> struct Quad<float> { float4 v; };
-
 // four values from p on, of which `live` (at most four) exist
-template <typename T>
-__device__ __forceinline__ Quad<T> load_quad(const T* p, int live, bool wide) {
-    Quad<T> q;
-    if constexpr (sizeof(T) == 4) {
-        if (wide && live >= 4) {
-            q.v = __ldg(reinterpret_cast<const float4*>(p));
-        } else {
-            q.v.x = live > 0 ? __ldg(p) : 0.0f;
-            q.v.y = live > 1 ? __ldg(p + 1) : 0.0f;
-            q.v.z = live > 2 ? __ldg(p + 2) : 0.0f;
-            q.v.w = live > 3 ? __ldg(p + 3) : 0.0f;
-        }
-    } else {
-        if (wide && live >= 4) {
-            q.v = __ldg(reinterpret_cast<const uint2*>(p));
-        } else {
-            const unsigned short* const h = reinterpret_cast<const unsigned short*>(p);
-            const uint32_t a = live > 0 ? __ldg(h) : 0, b = live > 1 ? __ldg(h + 1) : 0;
-            const uint32_t c = live > 2 ? __ldg(h + 2) : 0, d = live > 3 ? __ldg(h + 3) : 0;
-            q.v = make_uint2(a | b << 16, c | d << 16);
-        }
-    }
-    return q;
+__device__ __forceinline__ float4 load_quad(const float* p, int live, bool wide) {
+    if (wide && live >= 4) return __ldg(reinterpret_cast<const float4*>(p));
+    return make_float4(live > 0 ? __ldg(p) : 0.0f, live > 1 ? __ldg(p + 1) : 0.0f, live > 2 ? __ldg(p + 2) : 0.0f, live > 3 ? __ldg(p + 3) : 0.0f);
 }
 
 // upper halves of two floats side by side
 __device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
 __device__ __forceinline__ float without_upper(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
-// four consecutive values at byte `offset` of every part
-template <typename T, int PART_BYTES>
-__device__ __forceinline__ void store_quad(uint8_t* tile, uint32_t offset, const Quad<T>& q) {
-    if constexpr (sizeof(T) == 4) {
-        float a = q.v.x, b = q.v.y, c = q.v.z, d = q.v.w;
+// the three bf16 parts of four consecutive values, at byte `offset` of each part's tile
+template <int PART_BYTES>
+__device__ __forceinline__ void store_quad(uint8_t* tile, uint32_t offset, float4 q) {
 #pragma unroll
-        for (int part = 0; part < 3; ++part) {
-            *reinterpret_cast<uint2*>(tile + part * PART_BYTES + offset) = make_uint2(upper_halves(a, b), upper_halves(c, d));
-            if (part < 2) {
-                a = without_upper(a);
-                b = without_upper(b);
-                c = without_upper(c);
-                d = without_upper(d);
-            }
-        }
-    } else {
-        *reinterpret_cast<uint2*>(tile + offset) = q.v;
+    for (int part = 0; part < 3; ++part) {
+        *reinterpret_cast<uint2*>(tile + part * PART_BYTES + offset) = make_uint2(upper_halves(q.x, q.y), upper_halves(q.z, q.w));
+        if (part < 2) q = make_float4(without_upper(q.x), without_upper(q.y), without_upper(q.z), without_upper(q.w));
     }
 }
 
