@@ -35,6 +35,7 @@ constexpr int kChunk = 512;                      // weight gradient: depth after
 template <int MODE, int TN, bool PAIR, bool SORTED> struct Shape {
     static constexpr bool kWeights = MODE == kWeightGradient;
     static constexpr int kCtas = PAIR ? 2 : 1, kRows = TN / kCtas;                 // rows of the tile that a CTA brings
+    static constexpr bool kSplits = !kWeights && TN == 32;                         // may share the depth of a tile (Args::split)
     static constexpr int kFeatureBytes = 128 * kDepth * 2, kRowBytes = kRows * kDepth * 2;
     static constexpr int kStageBytes = kFeatureBytes + kRowBytes;
     static constexpr int kRowsPerWarp = PAIR ? 16 : 32, kQuads = kRowsPerWarp / 4;
@@ -54,6 +55,7 @@ template <int MODE, int TN, bool PAIR, bool SORTED> struct Shape {
                          kCosts0 = kUnits0 + ((FMB_MAX_GROUPS + 1) * 4 + 7) / 8 * 8, kBars0 = kCosts0 + (kWeights ? (FMB_MAX_GROUPS + 1) * 8 : 0);
     static constexpr int kSmem = 1024 + kBars0 + 256;
     static constexpr int kTmem = 2 * TN < 32 ? 32 : 2 * TN;
+    static_assert(!kSplits || 7 * TN * 128 * 4 <= kStages * kStageBytes, "room for the sums of seven CTAs");
     static_assert(kStages >= 3 && kSmem <= 227 * 1024 && kMmaWarp < kFirstEpilogue, "fits an SM");
 };
 
@@ -61,6 +63,7 @@ struct Args {
     fmb_grouped_t a;
     int feature_tiles, row_tiles;                // of the output; row_tiles 1 where rows are gathered
     int unit_rows;                               // entries of a group per unit
+    int split = 1;                               // linears of few rows: CTAs, a cluster, that share the depth of a tile; one tile each
     int wide_store;                              // output rows may be written 16 bytes at a time
     const int32_t* first_block;                  // SORTED: blocks of 64 rows of the groups before each
 };
@@ -137,9 +140,10 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     // Tiles of the linears cost the same, and go round. Those of the weight gradient cost what their group has rows: every CTA (pair)
     // takes consecutive tiles of the same cost in all (sizes that differ by a factor of three cost 40 % where tiles went round).
-    const int walkers = gridDim.x / S::kCtas, walker = blockIdx.x / S::kCtas;
+    const bool split = S::kSplits && p.split > 1;
+    const int ctas = split ? p.split : S::kCtas, walkers = gridDim.x / ctas, walker = blockIdx.x / ctas, part = split ? blockIdx.x % p.split : 0;
     const int all_tiles = units_in_all(first_unit, p.a.groups, p.a.rows, p.unit_rows) * p.feature_tiles * p.row_tiles;
-    int t_first = walker, t_end = all_tiles;
+    int t_first = walker, t_end = split ? min(all_tiles, walkers) : all_tiles;
     const int t_step = kWeights ? 1 : walkers;
     if constexpr (kWeights) {
         long long* const cost = reinterpret_cast<long long*>(smem + S::kCosts0);
@@ -182,7 +186,9 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
         t_first = min(first_tile(walker), all_tiles);
         t_end = min(first_tile(walker + 1), all_tiles);
     }
-    const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n;        // not of the weight gradient
+    // not of the weight gradient
+    const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n, row_blocks = (depth_of_row + kDepth - 1) / kDepth;
+    const int first_block = split ? row_blocks * part / p.split : 0, last_block = split ? row_blocks * (part + 1) / p.split : row_blocks;
 
     Walk w(p.a, first_unit, p.unit_rows, p.feature_tiles, p.row_tiles, TN);
     if (warp >= S::kFirstEpilogue) {
@@ -278,6 +284,25 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 else w.step(t_step);
                 mbar_wait(acc_full(acc), acc_phase, abort_flag, kSpin);
                 fence_after_sync();
+                if constexpr (S::kSplits) {
+                    __syncwarp();
+                    if (split) cluster_sync();       // every CTA's products are done, and the stages of the first one free
+                    if (split && part > 0) {
+                        // its sums [32 rows][128 features] into the place of this one in the first CTA's stages
+                        float v[32];
+                        const uint32_t to = in_leader(stage0) + (uint32_t)((part - 1) * 32 * 128 + id) * 4;
+                        if (set == 0) {
+                            tmem_load_32(tmem + lanes, v);
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (j < w.count) asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(to + j * 512), "f"(v[j]) : "memory");
+                        }
+                        __syncwarp();
+                        cluster_sync();
+                        break;
+                    }
+                    if (split) cluster_sync();
+                }
                 const int feature = w.feature0 * S::kCtas + rank * 128 + 8 * (lane & 15), live = width - feature;
                 // the sets take turns at blocks of 32 rows
 #pragma unroll 1
@@ -285,6 +310,13 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                     const int mine = row_at(p, w.first + j0 + lane, w.first + w.count);
                     float v[32];
                     tmem_load_32(tmem + lanes + acc * TN + j0, v);
+                    if constexpr (S::kSplits) {
+                        for (int q = 1; q < ctas; ++q) {
+                            const float* const from = reinterpret_cast<const float*>(smem) + (q - 1) * 32 * 128 + id;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] += j < w.count ? from[j * 128] : 0.0f;
+                        }
+                    }
                     named_barrier(1 + set, 128);                  // what was here has been read
 #pragma unroll
                     for (int j = 0; j < 32; ++j) turn[j * 128 + id] = from_float<T>(v[j]);
@@ -361,7 +393,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
             for (int t = t_first; alive && t < t_end; t += t_step) {
                 if (t == t_first) w.start(t);
                 else w.step(t_step);
-                const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
+                const int depth = kWeights ? w.count : depth_of_row, blocks = kWeights ? (depth + kDepth - 1) / kDepth : last_block;
                 const int end = w.first + w.count, feature0 = w.feature0 * S::kCtas + rank * 128;
                 if constexpr (!kWeights) {
                     if (warp > 0) {
@@ -375,7 +407,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                             my_rows[1] = row_or_zeros(entry + 1, end);
                         }
                         __syncwarp();
-                        for (int b = 0; b < blocks; ++b) {
+                        for (int b = first_block; b < blocks; ++b) {
                             alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
                             if (!alive) break;
                             const uint32_t dst = stage0 + at * S::kStageBytes + S::kFeatureBytes + (warp - 1) * S::kQuads * 512, bar = copy_bar(at);
@@ -391,7 +423,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                             advance();
                         }
                     } else {
-                        for (int b = 0; b < blocks; ++b) {
+                        for (int b = first_block; b < blocks; ++b) {
                             alive = mbar_wait(empty(at), phase ^ 1, abort_flag, kSpin);
                             if (!alive) break;
                             const uint32_t dst = stage0 + at * S::kStageBytes, bar = copy_bar(at);
@@ -468,12 +500,12 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
             for (int t = t_first; alive && t < t_end; t += t_step) {
                 if (t == t_first) w.start(t);
                 else w.step(t_step);
-                const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kDepth - 1) / kDepth;
+                const int depth = kWeights ? w.count : depth_of_row, blocks = kWeights ? (depth + kDepth - 1) / kDepth : last_block;
                 constexpr int kUnit = 16 * S::kCtas;
                 const int columns = kWeights ? TN : max(kUnit, min(TN, (w.count + kUnit - 1) / kUnit * kUnit));
                 const uint32_t idesc = kDesc | ((uint32_t)(columns >> 3) << 17);
-                for (int b = 0; b < blocks; ++b) {
-                    const bool fresh = b == 0 || (kWeights && b % (kChunk / kDepth) == 0);
+                for (int b = kWeights ? 0 : first_block; b < blocks; ++b) {
+                    const bool fresh = b == (kWeights ? 0 : first_block) || (kWeights && b % (kChunk / kDepth) == 0);
                     if (fresh) alive = mbar_wait(acc_empty(acc), acc_phase ^ 1, abort_flag, kSpin);
                     alive = alive && mbar_wait(full(at), phase, abort_flag, kSpin);
                     if (!alive) break;
@@ -506,6 +538,12 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                     advance();
                 }
             }
+        }
+        if (split && t_first < t_end) {
+            // (as the warps that join the sums)
+            __syncwarp();
+            cluster_sync();
+            cluster_sync();
         }
     }
     fence_before_sync();
@@ -547,18 +585,18 @@ template <typename T, int MODE, int TN, bool PAIR, bool SORTED = false>
 int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, long long tiles, cudaStream_t stream) {
     using S = Shape<MODE, TN, PAIR, SORTED>;
     FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN, PAIR, SORTED>, S::kSmem));
-    const int grid = (int)std::min<long long>(tiles, sm_count() / S::kCtas) * S::kCtas;
-    if constexpr (PAIR) {
+    const int ctas = S::kSplits ? p.split : S::kCtas, grid = (int)(p.split > 1 ? tiles : std::min<long long>(tiles, sm_count() / ctas)) * ctas;
+    if (ctas > 1) {
         cudaLaunchConfig_t config = {};
-        cudaLaunchAttribute pair;
-        pair.id = cudaLaunchAttributeClusterDimension;
-        pair.val.clusterDim.x = 2;
-        pair.val.clusterDim.y = pair.val.clusterDim.z = 1;
+        cudaLaunchAttribute cluster;
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = ctas;
+        cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
         config.gridDim = dim3(grid);
         config.blockDim = dim3(S::kThreads);
         config.dynamicSmemBytes = S::kSmem;
         config.stream = stream;
-        config.attrs = &pair;
+        config.attrs = &cluster;
         config.numAttrs = 1;
         FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_grouped_tc<T, MODE, TN, PAIR, SORTED>, p, features, rows));
     } else {
@@ -582,7 +620,17 @@ int launch_rows(Args& p, const CUtensorMap& features, const CUtensorMap& rows, c
     int tn = 256;
     while (tn > 32 && (tn > std::max(32, 2 * average) || most_units(a, tn) * p.feature_tiles < 148)) tn /= 2;
     p.unit_rows = tn;
-    const long long tiles = most_units(a, tn) * p.feature_tiles;
+    long long tiles = most_units(a, tn) * p.feature_tiles;
+    if (tn == 32) {
+        // Few rows: as many CTAs as there is room for share the depth of a tile, at least four blocks each, and the first adds up.
+        // (8 rows in 8 groups of 2,048 x 1,024, two CTAs a tile: 16.4 us, 18.5 with one; one row, eight: 12.3, 16.4; 30 rows
+        // of 4,096 x 4,096 in one group, four: 18.4, 34.8)
+        const long long with_rows = std::min<long long>(a->rows, most_units(a, tn)) * p.feature_tiles;
+        const int blocks = ((MODE == kLinear ? a->k : a->n) + kDepth - 1) / kDepth;
+        for (int split = 2; split <= 8; split *= 2)
+            if (with_rows * split <= (split == 2 ? 148 : 128) && blocks >= 4 * split) p.split = split;
+        if (p.split > 1) tiles = with_rows;
+    }
     if (tn == 256) return launch<T, MODE, 256, false>(p, features, rows, tiles, stream);
     if (tn == 128) return launch<T, MODE, 128, false>(p, features, rows, tiles, stream);
     if (tn == 64) return launch<T, MODE, 64, false>(p, features, rows, tiles, stream);

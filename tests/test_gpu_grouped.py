@@ -150,6 +150,39 @@ def test_weight_gradient_of_a_long_group_among_short_ones(groups, k, n, dtype):
     grouped.check_status()
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,groups,k,n", [(1, 1, 4096, 40), (1, 64, 2056, 1024), (2, 2, 512, 512), (8, 64, 2048, 1024), (9, 70, 1100, 515),
+                                             (30, 1, 515, 300), (31, 2, 640, 96), (5, 1024, 1096, 200), (40, 1, 2100, 136), (70, 3, 2048, 128)])
+def test_single_tokens(rows, groups, k, n, dtype):
+    """Few rows of deep products, where several blocks share the depth of a tile; some rows belong to no group."""
+    from fastmace_b200 import grouped
+    rng = np.random.default_rng(rows + k)
+    keys = rng.integers(0, groups, rows)
+    keys[rng.random(rows) < 0.15] = -1
+    keys = torch.tensor(keys, device="cuda")
+    plan = grouped.group_rows(keys, groups)
+    g = torch.Generator(device="cuda").manual_seed(k)
+    w = (torch.randn(groups, k, n, generator=g, device="cuda") / k ** 0.5).to(dtype)
+    x = torch.randn(rows, k, generator=g, device="cuda").to(dtype)
+    dy = torch.randn(rows, n, generator=g, device="cuda").to(dtype)
+    y = grouped.grouped_linear(x, w, plan)
+    dx = grouped.grouped_linear_input_gradient(dy, w, plan)
+    _check_rows(y, x, w, keys)
+    _check_rows(dx, dy, w, keys, transposed=True)
+    # captured, with other values and other groups at each replay
+    slots, inputs = torch.full_like(keys, groups - 1), torch.zeros_like(x)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        later = grouped.grouped_linear(inputs, w, grouped.group_rows(slots, groups))
+    for shift in range(3):
+        slots.copy_((keys + shift) % groups)
+        inputs.copy_(x * (shift + 1))
+        graph.replay()
+        _check_rows(later, inputs, w, slots)
+    assert torch.equal(y, grouped.grouped_linear(x, w, plan))
+    grouped.check_status()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_order_of_magnitude_extremes(dtype):
     """Values from 2^-60 to 2^60 of one matrix: float32 operands keep their 24 bits at every size."""
