@@ -65,12 +65,14 @@ struct Args {
     int unit_rows;                               // entries of a group per unit
     int split = 1;                               // linears of few rows: CTAs, a cluster, that share the depth of a tile; one tile each
     int wide_store;                              // output rows may be written 16 bytes at a time
+    int by_tma;                                  // weight gradient: as boxes of 16 rows, by weight_map
     const int32_t* first_block;                  // SORTED: blocks of 64 rows of the groups before each
 };
 
 template <typename T, int MODE, int TN, bool PAIR, bool SORTED>
 __global__ void __launch_bounds__(Shape<MODE, TN, PAIR, SORTED>::kThreads, 1)
-k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap feature_map, const __grid_constant__ CUtensorMap row_map) {
+k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap feature_map, const __grid_constant__ CUtensorMap row_map,
+             const __grid_constant__ CUtensorMap weight_map) {
     using S = Shape<MODE, TN, PAIR, SORTED>;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* const smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -156,8 +158,9 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                     int begin, end;
                     group_span(p.a.offsets, g, p.a.rows, begin, end);
                     const int units = first_unit[g + 1] - first_unit[g];
-                    // a tile takes as long as its blocks or, 128 KB written per CTA, as nine of them
-                    mine = (max((long long)(end - begin + kDepth - 1) / kDepth, 9ll * units) + units) * p.feature_tiles * p.row_tiles;
+                    // a tile takes as long as its blocks or, 128 KB written per CTA, as four of them (0, 4, 6, 9: 160, 147, 152, 154 us
+                    // for 16,384 rows of 2,048 x 1,024 in 32 groups)
+                    mine = (max((long long)(end - begin + kDepth - 1) / kDepth, 4ll * units) + units) * p.feature_tiles * p.row_tiles;
                 }
                 long long inclusive = mine;
 #pragma unroll
@@ -236,6 +239,27 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                 float* const out = (direct ? (float*)p.a.w + w.g * p.a.w_group_stride : p.a.scratch + w.slot * p.a.k * p.a.n) + feature;
                 const bool add = direct && p.a.accumulate, wide = direct ? p.wide_store : p.a.n % 4 == 0;
                 const int row0 = w.row0 + set * kCols;
+                if (direct && p.by_tma) {
+                    // 16 rows at a time through two buffers, and on by TMA (threads that wrote the rows themselves, 32 at a time, as
+                    // below: 269 us for 100,000 rows of 768 x 768 in 128 groups, and 223 so)
+#pragma unroll
+                    for (int j0 = 0; j0 < kCols; j0 += 16) {
+                        float* const box = turn + (j0 & 16) * 128;
+                        if (id == 0) bulk_wait_read<1>();
+                        named_barrier(1 + set, 128);              // what was in the box has been read
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) box[j * 128 + id] = sum[j0 + j];
+                        fence_to_async();
+                        named_barrier(1 + set, 128);
+                        if (id == 0) {
+                            const int column = w.feature0 * S::kCtas + rank * 128;
+                            if (row0 + j0 < p.a.k && column < p.a.n) tma_store_3d(&weight_map, smem_u32(box), column, row0 + j0, w.g);
+                            bulk_commit();
+                        }
+                    }
+                    continue;
+                }
+                if (id == 0) bulk_wait_read<0>();
 #pragma unroll
                 for (int j0 = 0; j0 < kCols; j0 += 32) {
                     named_barrier(1 + set, 128);                  // what was here has been read
@@ -265,6 +289,7 @@ k_grouped_tc(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap
                     }
                 }
             }
+            if (id == 0) bulk_wait();
         } else {
             T* const out = (T*)(MODE == kLinear ? p.a.y : p.a.x);
             const long long stride = MODE == kLinear ? p.a.y_stride : p.a.x_stride;
@@ -582,7 +607,7 @@ Encode encoder() {
 }
 
 template <typename T, int MODE, int TN, bool PAIR, bool SORTED = false>
-int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, long long tiles, cudaStream_t stream) {
+int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, const CUtensorMap& weights, long long tiles, cudaStream_t stream) {
     using S = Shape<MODE, TN, PAIR, SORTED>;
     FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_tc<T, MODE, TN, PAIR, SORTED>, S::kSmem));
     const int ctas = S::kSplits ? p.split : S::kCtas, grid = (int)(p.split > 1 ? tiles : std::min<long long>(tiles, sm_count() / ctas)) * ctas;
@@ -598,9 +623,9 @@ int launch(const Args& p, const CUtensorMap& features, const CUtensorMap& rows, 
         config.stream = stream;
         config.attrs = &cluster;
         config.numAttrs = 1;
-        FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_grouped_tc<T, MODE, TN, PAIR, SORTED>, p, features, rows));
+        FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_grouped_tc<T, MODE, TN, PAIR, SORTED>, p, features, rows, weights));
     } else {
-        k_grouped_tc<T, MODE, TN, PAIR, SORTED><<<grid, S::kThreads, S::kSmem, stream>>>(p, features, rows);
+        k_grouped_tc<T, MODE, TN, PAIR, SORTED><<<grid, S::kThreads, S::kSmem, stream>>>(p, features, rows, weights);
     }
     FMB_LAUNCH_CHECK();
     return FMB_OK;
@@ -614,7 +639,7 @@ int launch_rows(Args& p, const CUtensorMap& features, const CUtensorMap& rows, c
     if (average >= 128 && width > 128 && most_units(a, 256) * ((width + 255) / 256) >= 74) {
         p.unit_rows = 256;
         p.feature_tiles = ceil_div(width, 256);
-        return launch<T, MODE, 256, true>(p, features, rows, most_units(a, 256) * p.feature_tiles, stream);
+        return launch<T, MODE, 256, true>(p, features, rows, rows, most_units(a, 256) * p.feature_tiles, stream);
     }
     // else the widest tile that still leaves one per SM, but none much wider than the groups are on average
     int tn = 256;
@@ -631,10 +656,10 @@ int launch_rows(Args& p, const CUtensorMap& features, const CUtensorMap& rows, c
             if (with_rows * split <= (split == 2 ? 148 : 128) && blocks >= 4 * split) p.split = split;
         if (p.split > 1) tiles = with_rows;
     }
-    if (tn == 256) return launch<T, MODE, 256, false>(p, features, rows, tiles, stream);
-    if (tn == 128) return launch<T, MODE, 128, false>(p, features, rows, tiles, stream);
-    if (tn == 64) return launch<T, MODE, 64, false>(p, features, rows, tiles, stream);
-    return launch<T, MODE, 32, false>(p, features, rows, tiles, stream);
+    if (tn == 256) return launch<T, MODE, 256, false>(p, features, rows, rows, tiles, stream);
+    if (tn == 128) return launch<T, MODE, 128, false>(p, features, rows, rows, tiles, stream);
+    if (tn == 64) return launch<T, MODE, 64, false>(p, features, rows, rows, tiles, stream);
+    return launch<T, MODE, 32, false>(p, features, rows, rows, tiles, stream);
 }
 
 bool by_sixteen(const void* base, long long stride) { return ((uintptr_t)base & 15) == 0 && stride % 8 == 0 && stride > 0; }
@@ -667,7 +692,7 @@ Plan plan_of(const fmb_grouped_t* a, Mode mode) {
     // Units: a group's rows, cut at half an SM's share of the work, so that every SM has some and one long group does not keep the
     // others waiting (208,333 rows of 64 x 512 in 103 groups, the largest of 40,000: 173 us, and 305 uncut). Where the tiles of one
     // group are enough for a quarter of the SMs, a launch for sums costs more than balance gives (16,384 rows of 2,048 x 1,024 in 32
-    // groups: 155 us, and 160 with it)
+    // groups: 5 us more with it)
     p.tn = a->k > 128 ? 256 : 128;
     const long long row_tiles = (a->k + p.tn - 1) / p.tn, of_group = ((a->n + 127) / 128) * row_tiles;
     const long long unit_rows = std::max<long long>(128, (a->rows * of_group / (2 * 148) + 63) / 64 * 64);
@@ -676,7 +701,7 @@ Plan plan_of(const fmb_grouped_t* a, Mode mode) {
     p.pair = p.tn == 256 && a->n > 128 && most_units(a, p.unit_rows) * row_tiles * ((a->n + 255) / 256) >= 74;
     // Sorting reads and writes every row once, at the rate of memory; gathering costs a CTA pair 1,000 cycles more per 64 rows of a
     // tile. Against each other per row: 256 (n / 256 + k / 256) x 4 bytes, 1.6e-4 us per 256 columns, and 1.1e-4 us per tile of
-    // 256 x 256. In us, sorted and gathered: 16,384 rows of 2,048 x 1,024: 155, 217; 65,536 of 2,048 x 2,048: 626, 1,111; 30,000 of
+    // 256 x 256. In us, sorted and gathered: 16,384 rows of 2,048 x 1,024: 147, 217; 65,536 of 2,048 x 2,048: 626, 1,111; 30,000 of
     // 1,024 x 1,024: 132, 189; 30,000 of 256 x 512: 77, 71; 300,000 of 128 x 128: 132, 89.
     const long long n_tiles = (a->n + 255) / 256, k_tiles = (a->k + 255) / 256;
     p.sorted = !x_fits || !y_fits || 2 * n_tiles * k_tiles > 3 * (n_tiles + k_tiles);
@@ -700,7 +725,8 @@ int weight_gradient(const fmb_grouped_t* a, const Plan& plan, cudaStream_t strea
     p.row_tiles = ceil_div(a->k, plan.tn);
     p.feature_tiles = ceil_div(a->n, plan.pair ? 256 : 128);
     const long long tiles = most_units(a, plan.unit_rows) * p.feature_tiles * p.row_tiles;
-    CUtensorMap features, rows;
+    CUtensorMap features, rows, weights = {};
+    p.by_tma = !a->accumulate && encode_map(&weights, FMB_TYPE_F32, a->w, a->n, a->k, a->groups, a->w_row_stride, a->w_group_stride, 16, 3, 128, false);
     int rc;
     if (plan.sorted) {
         void* const x = (char*)a->scratch + plan.x;
@@ -713,16 +739,16 @@ int weight_gradient(const fmb_grouped_t* a, const Plan& plan, cudaStream_t strea
         FMB_REQUIRE(encode_map(&features, a->type, y, a->n, all, 1, (a->n + 7) / 8 * 8, 0, 64, 2, 64, true) &&
                         encode_map(&rows, a->type, x, a->k, all, 1, (a->k + 7) / 8 * 8, 0, 64, 2, 64, true),
                     "fmb_grouped_weight_gradient: tensor maps");
-        rc = plan.pair        ? launch<T, kWeightGradient, 256, true, true>(p, features, rows, tiles, stream)
-             : plan.tn == 256 ? launch<T, kWeightGradient, 256, false, true>(p, features, rows, tiles, stream)
-                              : launch<T, kWeightGradient, 128, false, true>(p, features, rows, tiles, stream);
+        rc = plan.pair        ? launch<T, kWeightGradient, 256, true, true>(p, features, rows, weights, tiles, stream)
+             : plan.tn == 256 ? launch<T, kWeightGradient, 256, false, true>(p, features, rows, weights, tiles, stream)
+                              : launch<T, kWeightGradient, 128, false, true>(p, features, rows, weights, tiles, stream);
     } else {
         FMB_REQUIRE(encode_map(&features, a->type, a->y, a->n, a->rows, 1, a->y_stride, 0, 1, 2, 64, true) &&
                         encode_map(&rows, a->type, a->x, a->k, a->rows, 1, a->x_stride, 0, 1, 2, 64, true),
                     "fmb_grouped_weight_gradient: tensor maps");
-        rc = plan.pair        ? launch<T, kWeightGradient, 256, true>(p, features, rows, tiles, stream)
-             : plan.tn == 256 ? launch<T, kWeightGradient, 256, false>(p, features, rows, tiles, stream)
-                              : launch<T, kWeightGradient, 128, false>(p, features, rows, tiles, stream);
+        rc = plan.pair        ? launch<T, kWeightGradient, 256, true>(p, features, rows, weights, tiles, stream)
+             : plan.tn == 256 ? launch<T, kWeightGradient, 256, false>(p, features, rows, weights, tiles, stream)
+                              : launch<T, kWeightGradient, 128, false>(p, features, rows, weights, tiles, stream);
     }
     return rc || plan.units < 0 ? rc : sum_units(&p.a, plan.unit_rows, stream);
 }
