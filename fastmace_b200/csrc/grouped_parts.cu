@@ -112,8 +112,13 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
     __syncthreads();
     fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const int tiles = units_in_all(first_unit, p.a.groups, p.a.rows, p.unit_rows) * p.feature_tiles * p.row_tiles;
-    const int t_first = blockIdx.x, t_step = gridDim.x, depth_of_row = MODE == kLinear ? p.a.k : p.a.n;       // (not of the weight gradient)
+    const bool split = !kWeights && p.split > 1;
+    const int t_first = split ? blockIdx.x / p.split : blockIdx.x, t_step = split ? gridDim.x / p.split : gridDim.x, part = split ? blockIdx.x % p.split : 0;
+    const int all_tiles = units_in_all(first_unit, p.a.groups, p.a.rows, p.unit_rows) * p.feature_tiles * p.row_tiles;
+    const int tiles = split ? min(all_tiles, t_step) : all_tiles;
+    // not of the weight gradient: depth, and the blocks of it that are this CTA's
+    const int depth_of_row = MODE == kLinear ? p.a.k : p.a.n, row_blocks = (depth_of_row + kStep - 1) / kStep;
+    const int first_block = split ? row_blocks * part / p.split : 0, my_blocks = split ? row_blocks * (part + 1) / p.split - first_block : row_blocks;
     bool alive = true;
     Walk w(p.a, first_unit, p.unit_rows, p.feature_tiles, p.row_tiles, 128);
 
@@ -125,7 +130,7 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
         for (int t = t_first; alive && t < tiles; t += t_step) {
             if (t == t_first) w.start(t);
             else w.step(t_step);
-            const int blocks = ((kWeights ? w.count : depth_of_row) + kStep - 1) / kStep, end = w.first + w.count;
+            const int blocks = kWeights ? (w.count + kStep - 1) / kStep : my_blocks, end = w.first + w.count;
             int b = mine - slot;                              // this warp's first block of the tile
             if (b < 0) b += kRaw;
             slot = (slot + blocks) % kRaw;
@@ -151,14 +156,14 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
                     if (lane >= 8 && lane < 8 + quads)
                         tma_gather4(dst + kRawSide + (lane - 8) * 2048, &row_map, w.row0, rows[0], rows[1], rows[2], rows[3], bar);
                 } else {
-                    const int quads = (w.count + 3) / 4;
+                    const int quads = (w.count + 3) / 4, column = (first_block + b) * kStep;
                     if (elect_one()) {
                         mbar_expect_tx(bar, kRawSide + quads * 512);
-                        if constexpr (MODE == kLinear) tma_tile_3d(dst, &feature_map, w.feature0, b * kStep, w.g, bar);
-                        else tma_tile_3d(dst, &feature_map, b * kStep, w.feature0, w.g, bar);
+                        if constexpr (MODE == kLinear) tma_tile_3d(dst, &feature_map, w.feature0, column, w.g, bar);
+                        else tma_tile_3d(dst, &feature_map, column, w.feature0, w.g, bar);
                     }
                     __syncwarp();
-                    if (lane < quads) tma_gather4(dst + kRawSide + lane * 512, &row_map, b * kStep, rows[0], rows[1], rows[2], rows[3], bar);
+                    if (lane < quads) tma_gather4(dst + kRawSide + lane * 512, &row_map, column, rows[0], rows[1], rows[2], rows[3], bar);
                 }
                 __syncwarp();
             }
@@ -173,7 +178,7 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
         for (int t = t_first; alive && t < tiles; t += t_step) {
             if (t == t_first) w.start(t);
             else w.step(t_step);
-            const int depth = kWeights ? w.count : depth_of_row, blocks = (depth + kStep - 1) / kStep;
+            const int depth = kWeights ? w.count : depth_of_row - first_block * kStep, blocks = kWeights ? (depth + kStep - 1) / kStep : my_blocks;
             for (int b = 0; b < blocks; ++b) {
                 const bool fresh = b % kChunkBlocks == 0, last = b == blocks - 1 || (b + 1) % kChunkBlocks == 0;
                 if (fresh) alive = mbar_wait(acc_empty(acc), acc_phase ^ 1, abort_flag, kSpin);
@@ -230,7 +235,7 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
         for (int t = t_first; t < tiles; t += t_step) {
             if (t == t_first) w.start(t);
             else w.step(t_step);
-            const int chunks = ((kWeights ? w.count : depth_of_row) + kChunk - 1) / kChunk;
+            const int chunks = kWeights ? (w.count + kChunk - 1) / kChunk : (my_blocks + kChunkBlocks - 1) / kChunkBlocks;
             int low = -1, high = -1;                         // rows of the output of a linear
             if (!kWeights) {
                 low = row_at(p, w.first + set * 64 + lane, w.first + w.count);
@@ -255,6 +260,28 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
                 if (lane == 0) mbar_arrive(acc_empty(acc));
                 acc ^= 1;
                 if (acc == 0) acc_phase ^= 1;
+            }
+            if constexpr (!kWeights) {
+                if (split) {
+                    // every CTA's products are done, and the ring and planes of the first one free; the sums [row][128 features] of the
+                    // others go there, and it adds them up in order
+                    __syncwarp();
+                    cluster_sync();
+                    if (part > 0) {
+                        const uint32_t to = in_leader(smem_u32(smem)) + (uint32_t)((((part - 1) * p.slot_rows + set * 64) * 128 + id) * 4);
+#pragma unroll
+                        for (int j = 0; j < 64; ++j)
+                            if (set * 64 + j < w.count) asm volatile("st.shared::cluster.f32 [%0], %1;" :: "r"(to + j * 512), "f"(sum[j]) : "memory");
+                    }
+                    __syncwarp();
+                    cluster_sync();
+                    if (part > 0) break;
+                    for (int q = 1; q < p.split; ++q) {
+                        const float* const from = reinterpret_cast<const float*>(smem) + ((q - 1) * p.slot_rows + set * 64) * 128 + id;
+#pragma unroll
+                        for (int j = 0; j < 64; ++j) sum[j] += set * 64 + j < w.count ? from[j * 128] : 0.0f;
+                    }
+                }
             }
             const bool direct = !kWeights || w.units <= 1, add = kWeights && direct && p.a.accumulate, wide = direct ? wide_out : p.a.n % 4 == 0;
             const int feature = w.feature0 + 4 * lane, live = width - feature;
@@ -309,7 +336,7 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
         for (int t = t_first; alive && t < tiles; t += t_step) {
             if (t == t_first) w.start(t);
             else w.step(t_step);
-            const int blocks = ((kWeights ? w.count : depth_of_row) + kStep - 1) / kStep;
+            const int blocks = kWeights ? (w.count + kStep - 1) / kStep : my_blocks;
             for (int b = 0; b < blocks; ++b) {
                 alive = mbar_wait(raw_full(at), raw_phase, abort_flag, kSpin);
                 alive = alive && mbar_wait(plane_empty(s), phase ^ 1, abort_flag, kSpin);
@@ -334,6 +361,12 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
                 }
             }
         }
+    }
+    if (split && t_first < tiles && (warp < 4 || warp >= 4 + kEpilogueWarps)) {
+        // (as the warps that join the sums)
+        __syncwarp();
+        cluster_sync();
+        cluster_sync();
     }
     fence_before_sync();
     __syncthreads();
@@ -379,9 +412,27 @@ Plan plan_of(const fmb_grouped_t* a, Mode mode) {
     return p;
 }
 
+// of a linear
+long long tiles_with_rows(const fmb_grouped_t* a, int feature_tiles) { return std::min<long long>(a->rows, most_units(a, 128)) * feature_tiles; }
+
 template <int MODE>
 int launch(const SplitArgs& p, const CUtensorMap& features, const CUtensorMap& rows, int wide_out, cudaStream_t stream) {
     FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_grouped_parts<MODE>, kSmem));
+    if (p.split > 1) {
+        cudaLaunchConfig_t config = {};
+        cudaLaunchAttribute cluster;
+        cluster.id = cudaLaunchAttributeClusterDimension;
+        cluster.val.clusterDim.x = p.split;
+        cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+        config.gridDim = dim3((int)tiles_with_rows(&p.a, p.feature_tiles) * p.split);
+        config.blockDim = dim3(kThreads);
+        config.dynamicSmemBytes = kSmem;
+        config.stream = stream;
+        config.attrs = &cluster;
+        config.numAttrs = 1;
+        FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_grouped_parts<MODE>, p, features, rows, wide_out));
+        return FMB_OK;
+    }
     const long long tiles = most_units(&p.a, p.unit_rows) * p.feature_tiles * p.row_tiles;
     k_grouped_parts<MODE><<<(int)std::min<long long>(tiles, sm_count()), kThreads, kSmem, stream>>>(p, features, rows, wide_out);
     FMB_LAUNCH_CHECK();
@@ -441,6 +492,14 @@ int parts_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
     p.feature_tiles = ceil_div(width, 128);
     p.row_tiles = 1;
     p.unit_rows = 128;
+    // Few rows: as many CTAs as there is room for share the depth of a tile, at least eight blocks each (285 rows of 4,096 x 256 in
+    // one group: 44 us, and 115 with one CTA a tile; 8 rows in 8 groups of 2,048 x 1,024: 37, 53; with four blocks each 100 rows of
+    // 256 x 256 take 17.4, and 16.4)
+    p.slot_rows = std::min(128, a->rows);
+    for (int split = 2; split <= 8; split *= 2)
+        if (tiles_with_rows(a, p.feature_tiles) * split <= (split == 2 ? 148 : 128) && ceil_div(depth, kStep) >= 8 * split &&
+            (split - 1) * p.slot_rows * 512 <= kTurn0)
+            p.split = split;
     const int wide_out = width % 4 == 0 && four_at_a_time(forward ? a->y : a->x, forward ? a->y_stride : a->x_stride, 4);
     return forward ? launch<kLinear>(p, features, rows, wide_out, stream) : launch<kInputGradient>(p, features, rows, wide_out, stream);
 }

@@ -143,6 +143,8 @@ struct SplitArgs {
     fmb_grouped_t a;
     int feature_tiles, row_tiles, unit_rows;
     int wide_features;                           // weights that may be read four values at a time (grouped_resident.cu)
+    int split = 1;                               // linears of few rows: CTAs, a cluster, that share the depth of a tile; one tile each
+    int slot_rows = 0;                           // rows that a tile has at most
 };
 
 // The tiles of a launch, group by group; of a group all units (entries [first, first + count) of `order`) for the same features
