@@ -122,6 +122,23 @@ def _matrix(what: str, name: str, t: torch.Tensor, columns: int | None = None, r
     return m, n, far if m > 1 else n
 
 
+def _shares_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors may have elements in common: false for ones that lie apart, and for rows of the same distance that lie
+    side by side (two components of one array of features)."""
+    size_a, size_b = a.element_size(), b.element_size()
+    reach = lambda t: sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1  # noqa: E731
+    if not a.numel() or not b.numel():
+        return False
+    at_a, at_b = a.data_ptr(), b.data_ptr()
+    if at_a + size_a * reach(a) <= at_b or at_b + size_b * reach(b) <= at_a:
+        return False
+    if a.dim() == b.dim() == 2 and size_a == size_b and a.stride(0) == b.stride(0) and (at_b - at_a) % size_a == 0:
+        stride = a.stride(0)
+        apart = (at_b - at_a) // size_a % stride if stride else 0
+        return not (a.shape[1] <= apart and apart + b.shape[1] <= stride)
+    return True
+
+
 def _weights(what: str, name: str, t: torch.Tensor):
     """(groups, k, n, group stride, row stride) of the matrices of all groups."""
     if t.dim() != 3:
@@ -161,6 +178,8 @@ def _rows_product(what: str, entry: str, source, weight, groups, out, transposed
         if out.dtype != dtype:
             raise ValueError(f"{what}: out must have the input's type")
         _on_device(what, source, out)
+        if _shares_memory(out, source) or _shares_memory(out, weight):
+            raise ValueError(f"{what}: out shares memory with an operand")
     else:
         out, out_stride = source.new_empty((rows, wide_out)), wide_out
     if rows:
@@ -208,6 +227,8 @@ def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: Ro
         raise ValueError(f"{what}: out must be float32 {(count, k, n)}")
     else:
         _on_device(what, x, out)
+        if _shares_memory(out, x) or _shares_memory(out, dy):
+            raise ValueError(f"{what}: out shares memory with an operand")
     _, _, _, w_group, w_row = _weights(what, "out", out)
     far, near, inner = (max(w_row, w_group), min(w_row, w_group), k if w_group >= w_row else count)
     if k > 1 and count > 1 and (near < n or far < (inner - 1) * near + n) or k > 1 and count == 1 and w_row < n or \

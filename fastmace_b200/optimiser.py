@@ -16,7 +16,8 @@ share a scale s per moment, the largest of them / 448: m is held as e4m3(m / s),
 where v is not. A gradient that is not finite makes the moments of its value (with 8 bits: of its 256 values) not finite, and
 with them the weights.
 
-A step runs on the current stream of the weights' device, allocates nothing and can be captured: the number of the step is
+The list of tensors and where they lie are those of the construction. Steps of one optimiser follow one another: not two at once on
+two streams. A step runs on the current stream of the weights' device, allocates nothing and can be captured: the number of the step is
 counted on the device, the learning rate and the other constants are those at capture. There is no CPU path.
 """
 
@@ -54,10 +55,13 @@ class AdamW:
                 raise ValueError("AdamW: the weights must be CUDA tensors, there is no CPU path")
             if p.dtype != torch.float32 or not p.is_contiguous() or p.device != self.device:
                 raise ValueError("AdamW: the weights must be contiguous float32 tensors on one device")
-        held = [p.data_ptr() for p in self.params if p.numel()]
-        if len(set(held)) < len(held):
-            raise ValueError("AdamW: a tensor is listed twice")
-        self.copies = [None] * len(self.params) if copies is None else [copies[k] for k in self.names]
+        if isinstance(copies, dict):
+            if set(copies) - set(self.names):
+                raise ValueError(f"AdamW: copies of unknown tensors: {sorted(map(str, set(copies) - set(self.names)))}")
+            copies = [copies.get(k) for k in self.names]
+        elif copies is not None and len(copies) != len(self.params):
+            raise ValueError(f"AdamW: {len(copies)} copies for {len(self.params)} tensors")
+        self.copies = [None] * len(self.params) if copies is None else list(copies)
         self._copy_type = 0
         for p, c in zip(self.params, self.copies):
             if c is None:
@@ -67,6 +71,12 @@ class AdamW:
             if self._copy_type not in (0, TYPES[c.dtype]):
                 raise ValueError("AdamW: the copies must have one type")
             self._copy_type = TYPES[c.dtype]
+        held = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in [*self.params, *self.copies] if t is not None and t.numel())
+        if any(here + size > there for (here, size), (there, _) in zip(held, held[1:])):
+            raise ValueError("AdamW: a tensor is listed twice, or two share memory")
+        # where the weights lie, and what keeps that memory while the optimiser lives
+        self._places, self._held = [p.data_ptr() for p in self.params], [p.detach() for p in self.params]
+        self._tracked = [p for p in self.params if p.requires_grad]
         self.lib = _lib.load()
         self.blocks, blocks = [], 0
         for p in self.params:
@@ -108,6 +118,8 @@ class AdamW:
             grads = [grads.get(k) for k in self.names]
         elif len(grads) != len(self.params):
             raise ValueError(f"AdamW.step: {len(grads)} gradients for {len(self.params)} tensors")
+        if [p.data_ptr() for p in self.params] != self._places:
+            raise ValueError("AdamW.step: a tensor of the list has been given other memory since")
         shapes = self._shapes
         if any(g is None for g in grads):
             self._pointers[:] = [0 if g is None else g.data_ptr() for g in grads]
@@ -127,6 +139,8 @@ class AdamW:
         self._args.grad_type = TYPES[kind]
         _lib.check(_launch(self._index, self.lib.fmb_adamw_step, ctypes.byref(self._args), self._tensors, len(self.params)),
                    "fmb_adamw_step")
+        if self._tracked:
+            torch.autograd.graph.increment_version(self._tracked)        # the weights have changed in place
 
     @property
     def steps(self) -> int:

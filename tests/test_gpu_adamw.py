@@ -182,3 +182,23 @@ def test_refusals_on_the_device():
                 lambda: AdamW([w]).load_moments(1, w), lambda: AdamW([w]).load_moments(1, w, w)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_lists_that_share_memory_or_move():
+    from fastmace_b200.optimiser import AdamW
+    base = torch.zeros(1000, device="cuda")
+    for bad in (lambda: AdamW([base[:600], base[500:]]), lambda: AdamW([base[:10], base[:10]]),
+                lambda: AdamW([base[:500]], copies=[base[250:500].view(torch.bfloat16)]),
+                lambda: AdamW([base[:10]], copies=[None, None]), lambda: AdamW({"a": base[:10]}, copies={"b": None})):
+        with pytest.raises(ValueError):
+            bad()
+    optimiser = AdamW({"a": base[:500], "b": base[500:]}, copies={"b": torch.zeros(500, dtype=torch.float16, device="cuda")})
+    optimiser.step({"a": torch.ones(500, device="cuda"), "b": torch.ones(500, device="cuda")})
+    weight = torch.nn.Parameter(torch.ones(100, device="cuda"))
+    optimiser = AdamW([weight])
+    version = weight._version
+    optimiser.step([torch.ones(100, device="cuda")])
+    assert weight._version > version                      # a graph that saved the weights finds out
+    weight.data = torch.ones(100, device="cuda")
+    with pytest.raises(ValueError, match="other memory"):
+        optimiser.step([torch.ones(100, device="cuda")])

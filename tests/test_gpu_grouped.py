@@ -432,3 +432,21 @@ def test_refusals_on_the_device():
                 lambda: grouped.group_rows(torch.zeros(8, dtype=torch.int32, device="cuda"), 1025)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_outputs_that_share_memory_with_operands():
+    from fastmace_b200 import grouped
+    nodes = torch.randn(40, 4, 64, device="cuda")
+    w = torch.randn(2, 64, 64, device="cuda")
+    keys = torch.arange(40, device="cuda") % 2
+    plan = grouped.group_rows(keys, 2)
+    for call in (lambda: grouped.grouped_linear(nodes[:, 0], w, plan, out=nodes[:, 0]),
+                 lambda: grouped.grouped_linear_input_gradient(nodes[:, 0], w, plan, out=w.view(-1)[:2560].view(40, 64)),
+                 lambda: grouped.grouped_linear_weight_gradient(nodes[:, 0], nodes[:, 1], plan, out=nodes.view(-1)[:8192].view(2, 64, 64))):
+        with pytest.raises(ValueError, match="shares memory"):
+            call()
+    # another component of the same array is no overlap
+    before = nodes.clone()
+    grouped.grouped_linear(nodes[:, 0], w, plan, out=nodes[:, 2])
+    _check_rows(nodes[:, 2], before[:, 0], w, keys)
+    assert torch.equal(nodes[:, 0], before[:, 0]) and torch.equal(nodes[:, 1], before[:, 1]) and torch.equal(nodes[:, 3], before[:, 3])

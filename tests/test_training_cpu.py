@@ -74,3 +74,19 @@ def test_adamw_entry_refuses():
                    dict(tensor=dict(p=4097)), dict(tensor=dict(values=-1)), dict(tensor=dict(block=-1)), dict(tensor=dict(copy=4097))):
         assert call(**change) == 1, change
     assert call(tensor=dict(g=None)) == 0 and call(count=0) == 0 and call(tensor=dict(values=0)) == 0
+
+
+def test_what_shares_memory():
+    from fastmace_b200.grouped import _shares_memory
+    nodes = torch.zeros(10, 4, 16)
+    assert _shares_memory(nodes[:, 1], nodes[:, 1]) and _shares_memory(nodes[:, 1], nodes[:, 1, 8:])
+    assert not _shares_memory(nodes[:, 0], nodes[:, 1]) and not _shares_memory(nodes[:, 3], nodes[:, 0])
+    assert not _shares_memory(nodes[:, 1, :8], nodes[:, 1, 8:]) and _shares_memory(nodes[:, 1, :9], nodes[:, 1, 8:])
+    assert _shares_memory(nodes[:, 1], nodes.view(-1)[8:168].view(10, 16))
+    assert not _shares_memory(nodes[:5, 1], nodes[5:, 1]) and not _shares_memory(nodes[:, 0], torch.zeros(10, 16))
+    assert not _shares_memory(nodes[:0, 1], nodes[:, 1])
+    # a row that goes round the end of the distance between rows
+    wide = torch.zeros(200)
+    assert _shares_memory(wide.as_strided((5, 10), (16, 1), 0), wide.as_strided((5, 10), (16, 1), 12))
+    assert _shares_memory(wide[:64].view(8, 8), wide[8:72].view(2, 4, 8))
+    assert _shares_memory(wide[:64].view(8, 8), wide[:64].view(torch.float16).view(8, 16))
