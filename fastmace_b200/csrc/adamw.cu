@@ -9,7 +9,9 @@
 // that of the moments is rounded operation by operation, as it is written here: a moment that came out a bit
 // apart could take the next code, 2^-4 away, and with the block's largest the scale would follow a step later.
 //
-// Bound by HBM: 28 bytes a value with fp32 gradients and moments, 16 with 8-bit moments.
+// Bound by HBM: 28 bytes a value with fp32 gradients and moments, 16 with 8-bit moments. 200 M values in 32 bits with bf16 copies
+// take 910 us (6.6 TB/s, what a copy of as many bytes reaches), 64 M in 8 bits with bf16 gradients and copies 207 (5.0 TB/s: 24 warps'
+// conversions and exact quotients an SM keep it at 74 % of its rate), the 43 tensors of a medium model 27 (4.7 M values, 131 MB).
 
 #include "fmb_common.cuh"
 

@@ -10,6 +10,7 @@
 //     costs 96 KB of reads there instead of 192. Two accumulators, hi hi and the five others, twice (448 columns in all);
 //   * the result turns through shared memory, so that a store writes 512 bytes of a row. A lane that stored its own
 //     feature row by row took longer than everything else together.
+// 884,736 rows of 128 x 128 in 5 groups take 180 us (5.1 TB/s of 910 MB; 141 us at the rate of a copy), 1,944 rows in 2 groups 12.
 
 #include "grouped_tc.cuh"
 

@@ -3,12 +3,13 @@
 //   count:  a CTA counts the keys of kRowsPerCta consecutive rows
 //   scan:   per group, the counts of the CTAs before each CTA, and the total
 //   place:  every warp of a CTA owns consecutive rows; the warps' own counts give each its first place per group, and inside
-//           32 rows the lanes with the same key find their order by a match; no atomics on results, so the order is the one of
+//           32 rows the lanes with the same key find their order by votes; no atomics on results, so the order is the one of
 //           the row numbers
 //
 // Rows whose key is no group come behind all groups. Up to kRowsPerCta rows `place` alone does it: one launch.
 // Bound by latency: 8 bytes move per row and the second pass reads keys from L2. A lane asks for its keys all at once and keeps them for
-// both passes of `place`; one at a time, each waited for, 1,944 rows took 14 us.
+// both passes of `place`; one at a time, each waited for, 1,944 rows took 14 us. A call: 1,944 rows by 2 keys 11 us (one launch of
+// one CTA, of which the launch is most), 2,100,003 rows by 128 keys 35 us (three launches; 17 MB, 2.6 us of memory).
 
 #include "fmb_common.cuh"
 
