@@ -99,10 +99,9 @@ int sum_units(const fmb_grouped_t* a, int unit_rows, cudaStream_t stream);
 int sm_count();
 
 // copies into the layouts that TMA takes (grouped_pack.cu)
-int pack_rows(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream);
-int pack_rows_32(const void* src, long long stride, int columns, int rows, void* dst, cudaStream_t stream);
-int pack_weights(const fmb_grouped_t* a, void* dst, cudaStream_t stream);
-int pack_weights_32(const fmb_grouped_t* a, void* dst, cudaStream_t stream);
+// (rows, weights: where to, or null; in 32 bits the strides are multiples of four values, else of eight)
+int pack(const fmb_grouped_t* a, const void* src, long long stride, int columns, void* rows, void* weights, cudaStream_t stream);
+int pack_32(const fmb_grouped_t* a, const void* src, long long stride, int columns, void* rows, void* weights, cudaStream_t stream);
 int sort_rows(const fmb_grouped_t* a, void* x, void* y, int32_t* first_block, cudaStream_t stream);
 
 }  // namespace grp

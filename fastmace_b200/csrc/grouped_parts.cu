@@ -449,23 +449,23 @@ int parts_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
     FMB_REQUIRE(((uintptr_t)a->scratch & 255) == 0, "grouped product: scratch starts at a multiple of 256 bytes");
     SplitArgs p;
     p.a = *a;
-    float* at = a->scratch + plan.units;
+    float* const x = a->scratch + plan.units;
+    float* const y = x + plan.x;
+    float* const weights = y + plan.y;
     int rc = FMB_OK;
     if (plan.x) {
-        rc = pack_rows_32(a->x, a->x_stride, a->k, a->rows, at, stream);
-        p.a.x = at;
+        rc = pack_32(a, a->x, a->x_stride, a->k, x, plan.w ? weights : nullptr, stream);
+        p.a.x = x;
         p.a.x_stride = (a->k + 3) / 4 * 4;
-        at += plan.x;
     }
     if (!rc && plan.y) {
-        rc = pack_rows_32(a->y, a->y_stride, a->n, a->rows, at, stream);
-        p.a.y = at;
+        rc = pack_32(a, a->y, a->y_stride, a->n, y, plan.w ? weights : nullptr, stream);
+        p.a.y = y;
         p.a.y_stride = (a->n + 3) / 4 * 4;
-        at += plan.y;
     }
     if (!rc && plan.w) {
-        rc = pack_weights_32(a, at, stream);
-        p.a.w = at;
+        if (!plan.x && !plan.y) rc = pack_32(a, nullptr, 0, 0, nullptr, weights, stream);
+        p.a.w = weights;
         p.a.w_row_stride = (a->n + 3) / 4 * 4;
         p.a.w_group_stride = a->k * p.a.w_row_stride;
     }

@@ -770,18 +770,18 @@ int linear(const fmb_grouped_t* a, bool forward, const Plan& plan, cudaStream_t 
     p.feature_tiles = ceil_div(width, 128);
     p.wide_store = ((uintptr_t)out & 15) == 0 && (forward ? a->y_stride : a->x_stride) % 8 == 0 && width % 8 == 0;
     const long long packed = forward ? plan.x : plan.y;
-    if (packed >= 0) {
-        void* const to = (char*)a->scratch + packed;
-        const int rc = pack_rows(in, in_stride, depth, a->rows, to, stream);
+    void* const packed_rows = packed >= 0 ? (char*)a->scratch + packed : nullptr;
+    void* const packed_weights = plan.w >= 0 ? (char*)a->scratch + plan.w : nullptr;
+    if (packed_rows || packed_weights) {
+        const int rc = pack(a, in, in_stride, depth, packed_rows, packed_weights, stream);
         if (rc) return rc;
-        in = to;
+    }
+    if (packed_rows) {
+        in = packed_rows;
         in_stride = (depth + 7) / 8 * 8;
     }
-    if (plan.w >= 0) {
-        void* const to = (char*)a->scratch + plan.w;
-        const int rc = pack_weights(a, to, stream);
-        if (rc) return rc;
-        w = to;
+    if (packed_weights) {
+        w = packed_weights;
         w_row = (a->n + 7) / 8 * 8;
         w_group = a->k * w_row;
     }
