@@ -32,6 +32,7 @@ from . import _lib
 from .grouped import TYPES, _launch
 
 BLOCK = _lib.ADAMW_BLOCK
+_place = torch.Tensor.data_ptr
 
 
 class AdamW:
@@ -118,7 +119,8 @@ class AdamW:
             grads = [grads.get(k) for k in self.names]
         elif len(grads) != len(self.params):
             raise ValueError(f"AdamW.step: {len(grads)} gradients for {len(self.params)} tensors")
-        if [p.data_ptr() for p in self.params] != self._places:
+        # (mapped methods: looking over 117 small tensors takes the host longer than their step takes the device, 17 us)
+        if list(map(_place, self.params)) != self._places:
             raise ValueError("AdamW.step: a tensor of the list has been given other memory since")
         shapes = self._shapes
         if any(g is None for g in grads):
@@ -128,12 +130,12 @@ class AdamW:
             if not grads:
                 return
         else:
-            self._pointers[:] = [g.data_ptr() for g in grads]
+            self._pointers[:] = list(map(_place, grads))
         kind = grads[0].dtype
-        if kind not in TYPES or any(g.dtype is not kind for g in grads):
+        if kind not in TYPES or [g.dtype for g in grads].count(kind) != len(grads):
             raise ValueError("AdamW.step: the gradients must have one type, float32, bfloat16 or float16")
-        if [g.shape for g in grads] != shapes or not all([g.is_contiguous() for g in grads]) or \
-                any([g.get_device() != self._index for g in grads]):
+        if [g.shape for g in grads] != shapes or not all(map(torch.Tensor.is_contiguous, grads)) or \
+                set(map(torch.Tensor.get_device, grads)) != {self._index}:
             raise ValueError("AdamW.step: a gradient must be contiguous, of its weights' shape and on their device")
         self._fill_args()
         self._args.grad_type = TYPES[kind]
