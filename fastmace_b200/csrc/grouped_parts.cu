@@ -384,6 +384,9 @@ k_grouped_parts(const __grid_constant__ SplitArgs p, const __grid_constant__ CUt
 
 bool rows_fit(const void* base, long long stride) { return four_at_a_time(base, stride, 4) && stride > 0; }
 
+// linears whose split weights fit in tensor memory (grouped_resident.cu, whose threads read the weights from where they are)
+bool is_resident(const fmb_grouped_t* a, Mode mode) { return mode != kWeightGradient && (mode == kLinear ? a->k : a->n) <= 128; }
+
 // Scratch: sums of units of the weight gradient, then copies of rows and matrices that TMA does not take as they are (floats).
 struct Plan {
     int unit_rows = 1 << 30;
@@ -398,8 +401,8 @@ Plan plan_of(const fmb_grouped_t* a, Mode mode) {
     if (mode != kInputGradient && !rows_fit(a->x, a->x_stride)) p.x = whole(a->rows * k4);
     if (mode != kLinear && !rows_fit(a->y, a->y_stride)) p.y = whole(a->rows * n4);
     if (mode != kWeightGradient) {
-        // (the strides may be anything where there is one row, or one matrix)
-        if (!rows_fit(a->w, a->k > 1 ? a->w_row_stride : 4) || (a->groups > 1 && (a->w_group_stride % 4 || a->w_group_stride <= 0)))
+        // (the strides may be anything where there is one row, or one matrix, and where the weights do not come by TMA)
+        if (!is_resident(a, mode) && (!rows_fit(a->w, a->k > 1 ? a->w_row_stride : 4) || (a->groups > 1 && (a->w_group_stride % 4 || a->w_group_stride <= 0))))
             p.w = whole(a->groups * a->k * n4);
         return p;
     }
@@ -470,7 +473,7 @@ int parts_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
         p.a.w_group_stride = a->k * p.a.w_row_stride;
     }
     if (rc) return rc;
-    if (mode != kWeightGradient && (mode == kLinear ? a->k : a->n) <= 128) return resident_launch(&p.a, mode, stream);
+    if (is_resident(a, mode)) return resident_launch(&p.a, mode, stream);
     CUtensorMap features, rows;
     if (mode == kWeightGradient) {
         FMB_REQUIRE(encode_map(&features, a->type, p.a.y, a->n, a->rows, 1, p.a.y_stride, 0, 1, 2, 128, false) &&
