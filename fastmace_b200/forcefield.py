@@ -87,6 +87,7 @@ class B200ForceField:
         self.edge_adjoint = edge_adjoint
         self.num_edges = 0
         self.calls = 0
+        self._evaluated = False              # the workspace holds a finished call of these atoms (weight_gradients)
         self.data = {}
         self.work = None
         self._outputs()
@@ -154,6 +155,7 @@ class B200ForceField:
         self.n_owned, self.n_inner = int(n_owned), int(n_inner)
         if self.halo_exchange and self.n_inner != self.n_owned:
             raise ValueError("halo-exchange mode: n_inner == n_owned")
+        self._evaluated = False
         moved = False
         if self.natoms > self.atom_capacity:
             self.atom_capacity = int(self.natoms * 1.1) + 16
@@ -195,6 +197,7 @@ class B200ForceField:
 
     def _allocate_work(self):
         spec, n, cap, dev = self.spec, self.atom_capacity, self.neighbours.capacity, self._device
+        self._evaluated = False
         if getattr(self, "buf", None) is not None:
             # the edge capacity grew: give the old buffers back to the device before the new ones are sized, so that the
             # two sets never exist side by side (the per-edge buffers of a large brick are tens of GB each)
@@ -351,8 +354,10 @@ class B200ForceField:
         if positions.dtype != torch.float64 or not positions.is_cuda:
             raise ValueError("positions must be a float64 CUDA tensor")
         self.calls += 1
+        self._evaluated = False
         _lib.check(self.lib.fmb_forces(self.packed.pointer(), self.neighbours.pointer(), ctypes.byref(self.work),
                                        positions.data_ptr(), _lib.current_stream()), "fmb_forces")
+        self._evaluated = True
         return ForceOutput(self.energy, self.forces, self.stress if self._compute_stress else None)
 
     def phase(self, index: int, positions: torch.Tensor | None = None) -> None:
@@ -370,10 +375,11 @@ class B200ForceField:
         """Gradient of the last call's energy in the linears of the last interaction: its species-dependent skip
         (``l{t}.skip.{l}``) and ``linear_up`` (``l{t}.up.{l}``), float32 in the shapes of the weights' dictionary (``model.py``), as
         ``optimiser.AdamW`` takes them. Elements that no atom has get zeros. The features and gradients that the call left in its
-        workspace are read, so nothing else may have used this force field since. On the current stream; no counterpart in the
-        reference, which evaluates trained models only."""
-        if self.work is None or self.calls == 0:
-            raise _lib.Fmb200Error("weight_gradients: no force call has been made")
+        workspace are read, so nothing else may have used this force field since; after ``set_atoms``, or a ``rebuild`` that made the
+        buffers anew, there is none until the next call. On the current stream; no counterpart in the reference, which evaluates
+        trained models only."""
+        if self.work is None or not self._evaluated:
+            raise _lib.Fmb200Error("weight_gradients: no force call since the atoms were set and the buffers made")
         if self.halo_exchange or not self._same_rows() or 0 <= self.n_owned < self.natoms:
             raise _lib.Fmb200Error("weight_gradients: the force field must own all of its atoms")
         spec, n, t = self.spec, self.natoms, self.spec.num_interactions - 1

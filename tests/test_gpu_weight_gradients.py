@@ -119,3 +119,48 @@ def test_refusals():
     part.evaluate(s)
     with pytest.raises(_lib.Fmb200Error, match="own all"):
         part.weight_gradients()
+
+
+@pytest.mark.parametrize("change", ["fewer", "more", "others"])
+def test_a_workspace_without_a_call_of_these_atoms_is_refused(change):
+    """After ``set_atoms`` (with and without new buffers) the features are those of other atoms, or zeros."""
+    from fastmace_b200 import _lib
+    from fastmace_b200.forcefield import B200ForceField
+    spec, weights, s = _case("small")
+    ff = B200ForceField(spec, weights, s.numbers, s.cell)
+    ff.evaluate(s)
+    before = ff.weight_gradients()
+    numbers = {"fewer": s.numbers[:-2], "more": np.concatenate([s.numbers, s.numbers[:2]]), "others": s.numbers[::-1].copy()}[change]
+    positions = np.concatenate([s.positions, s.positions[:2] + 1.3])[:len(numbers)]
+    ff.set_atoms(numbers)
+    with pytest.raises(_lib.Fmb200Error, match="no force call"):
+        ff.weight_gradients()
+    x = torch.as_tensor(positions, device="cuda")
+    ff.rebuild(x)
+    ff.compact(x)
+    with pytest.raises(_lib.Fmb200Error, match="no force call"):
+        ff.weight_gradients()
+    ff(x)
+    ff.check_status()
+    fresh = B200ForceField(spec, weights, numbers, s.cell, positions=x)
+    fresh(x)
+    for (k, a), b, old in zip(ff.weight_gradients().items(), fresh.weight_gradients().values(), before.values()):
+        # the same sums of the same terms, in an order that may follow the buffers' sizes
+        assert float((a - b).norm()) <= 1e-5 * float(b.norm()) and not torch.equal(a, old), k
+
+
+def test_buffers_made_anew_hold_no_call():
+    """A list that outgrows its capacity moves every buffer."""
+    from fastmace_b200 import _lib
+    from fastmace_b200.forcefield import B200ForceField
+    spec, weights, s = _case("small")
+    at = np.arange(len(s.numbers))
+    far = torch.zeros(len(at), 3, dtype=torch.float64, device="cuda")                # pairs far from one another
+    far[:, 2] = torch.as_tensor(40.0 * (at // 2) + 2.5 * (at % 2), device="cuda")
+    ff = B200ForceField(spec, weights, s.numbers, np.diag([30.0, 30.0, 40.0 * len(s.numbers)]), positions=far)
+    ff(far)
+    ff.weight_gradients()
+    near = torch.as_tensor(s.positions, device="cuda")
+    assert ff.rebuild(near)
+    with pytest.raises(_lib.Fmb200Error, match="no force call"):
+        ff.weight_gradients()
