@@ -19,7 +19,7 @@ from typing import NamedTuple
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, grouped
 from .grouped import group_rows, grouped_linear_weight_gradient
 from .model import MaceSpec
 from .neighbours import CellListNeighbours, NeighbourConfig
@@ -376,8 +376,8 @@ class B200ForceField:
         (``l{t}.skip.{l}``) and ``linear_up`` (``l{t}.up.{l}``), float32 in the shapes of the weights' dictionary (``model.py``), as
         ``optimiser.AdamW`` takes them. Elements that no atom has get zeros. The features and gradients that the call left in its
         workspace are read, so nothing else may have used this force field since; after ``set_atoms``, or a ``rebuild`` that made the
-        buffers anew, there is none until the next call. On the current stream; no counterpart in the reference, which evaluates
-        trained models only."""
+        buffers anew, there is none until the next call. On the current stream, and synchronises, since it raises if a product gave up
+        waiting. No counterpart in the reference, which evaluates trained models only."""
         if self.work is None or not self._evaluated:
             raise _lib.Fmb200Error("weight_gradients: no force call since the atoms were set and the buffers made")
         if self.halo_exchange or not self._same_rows() or 0 <= self.n_owned < self.natoms:
@@ -402,6 +402,8 @@ class B200ForceField:
             for m in range(l * l, (l + 1) ** 2):
                 grouped_linear_weight_gradient(h[:, m], d_x[:, m], everyone, out=g[None], accumulate=m > l * l)
             out[f"l{t}.up.{l}"] = g.mul_(1.0 / math.sqrt(c))
+        if not torch.cuda.is_current_stream_capturing():
+            grouped.check_status(self._device)
         return out
 
     def evaluate(self, atoms, stress: bool = False):

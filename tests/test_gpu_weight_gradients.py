@@ -164,3 +164,17 @@ def test_buffers_made_anew_hold_no_call():
     assert ff.rebuild(near)
     with pytest.raises(_lib.Fmb200Error, match="no force call"):
         ff.weight_gradients()
+
+
+def test_products_that_gave_up_waiting_are_reported():
+    """The products' status word as a kernel whose wait has run out leaves it."""
+    from fastmace_b200 import _lib, grouped
+    from fastmace_b200.forcefield import B200ForceField
+    spec, weights, s = _case("small")
+    ff = B200ForceField(spec, weights, s.numbers, s.cell)
+    ff.evaluate(s)
+    good = ff.weight_gradients()
+    grouped._status[ff.device.index].fill_(_lib.STATUS_TENSOR_TIMEOUT)
+    with pytest.raises(_lib.Fmb200Error, match="gave up waiting"):
+        ff.weight_gradients()
+    assert all(torch.equal(a, b) for a, b in zip(good.values(), ff.weight_gradients().values()))
