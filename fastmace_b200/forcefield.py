@@ -65,6 +65,8 @@ class B200ForceField:
         # three phases (``phase``) between which the caller moves the halo rows of ``x`` and ``d_x``
         self.packed = packed if packed is not None else \
             PackedModel(spec, weights, sorted(set(int(z) for z in self.numbers)), self._device)
+        # element (atomic number less one) of each species index, for weight_gradients
+        self._elements = torch.tensor(self.packed.species_z, dtype=torch.int32, device=self._device) - 1
         self.n_owned, self.n_inner = int(n_owned), int(n_inner)
         self.halo_exchange = bool(halo_exchange)
         if self.halo_exchange and self.n_inner != self.n_owned:
@@ -377,7 +379,8 @@ class B200ForceField:
         ``optimiser.AdamW`` takes them. Elements that no atom has get zeros. The features and gradients that the call left in its
         workspace are read, so nothing else may have used this force field since; after ``set_atoms``, or a ``rebuild`` that made the
         buffers anew, there is none until the next call. On the current stream, and synchronises, since it raises if a product gave up
-        waiting. No counterpart in the reference, which evaluates trained models only."""
+        waiting. It can be captured after one call outside a capture, also behind the force call in one graph; it does not
+        synchronise then, and ``grouped.check_status`` tells. No counterpart in the reference, which evaluates trained models only."""
         if self.work is None or not self._evaluated:
             raise _lib.Fmb200Error("weight_gradients: no force call since the atoms were set and the buffers made")
         if self.halo_exchange or not self._same_rows() or 0 <= self.n_owned < self.natoms:
@@ -389,8 +392,7 @@ class B200ForceField:
         h = self.buf["h"].view(-1)[:n * hid * c].view(n, hid, c)
         d_x = self.buf["d_x"][:n]
         d_out = self.buf["basis"].view(-1)[:n * c].view(n, c)
-        element = torch.tensor(self.packed.species_z, dtype=torch.int32, device=self._device) - 1
-        by_element = group_rows(element[self.species[:n].long()], elements)
+        by_element = group_rows(self._elements[self.species[:n].long()], elements)
         everyone = group_rows(torch.zeros(n, dtype=torch.int32, device=self._device), 1)
         out = {}
         for l in range(spec.skip_lmax(t) + 1):          # the last layer has scalars only

@@ -178,3 +178,30 @@ def test_products_that_gave_up_waiting_are_reported():
     with pytest.raises(_lib.Fmb200Error, match="gave up waiting"):
         ff.weight_gradients()
     assert all(torch.equal(a, b) for a, b in zip(good.values(), ff.weight_gradients().values()))
+
+
+def test_captured_with_the_force_call():
+    """One graph of force call and gradients, replayed at other positions, gives the bits of the calls one by one."""
+    from fastmace_b200 import grouped
+    from fastmace_b200.forcefield import B200ForceField
+    spec, weights, s = _case("medium")
+    ff = B200ForceField(spec, weights, s.numbers, s.cell)
+    ff.evaluate(s)
+    ff.weight_gradients()
+    x = torch.as_tensor(s.positions, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ff(x)
+        captured = ff.weight_gradients()
+    g = torch.Generator(device="cuda").manual_seed(1)
+    for _ in range(2):
+        x.add_(0.01 * torch.randn(x.shape, generator=g, device="cuda", dtype=torch.float64))
+        ff.compact(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        seen = {k: v.clone() for k, v in captured.items()}
+        ff(x)
+        for k, v in ff.weight_gradients().items():
+            assert torch.equal(seen[k], v), k
+    grouped.check_status()
+    ff.check_status()
