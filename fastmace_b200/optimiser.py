@@ -77,7 +77,9 @@ class AdamW:
             raise ValueError("AdamW: a tensor is listed twice, or two share memory")
         # where the weights lie, and what keeps that memory while the optimiser lives
         self._places, self._held = [p.data_ptr() for p in self.params], [p.detach() for p in self.params]
-        self._tracked = [p for p in self.params if p.requires_grad]
+        # what a step writes to, for autograd, of each tensor (inference tensors have no version to count)
+        self._written = [[t for t in pair if t is not None and not t.is_inference()] for pair in zip(self.params, self.copies)]
+        self._all_written = sum(self._written, [])
         self.lib = _lib.load()
         self.blocks, blocks = [], 0
         for p in self.params:
@@ -122,8 +124,9 @@ class AdamW:
         # (mapped methods: looking over 117 small tensors takes the host longer than their step takes the device, 17 us)
         if list(map(_place, self.params)) != self._places:
             raise ValueError("AdamW.step: a tensor of the list has been given other memory since")
-        shapes = self._shapes
+        shapes, written = self._shapes, self._all_written
         if any(g is None for g in grads):
+            written = sum((w for w, g in zip(self._written, grads) if g is not None), [])
             self._pointers[:] = [0 if g is None else g.data_ptr() for g in grads]
             shapes = [s for s, g in zip(shapes, grads) if g is not None]
             grads = [g for g in grads if g is not None]
@@ -141,8 +144,9 @@ class AdamW:
         self._args.grad_type = TYPES[kind]
         _lib.check(_launch(self._index, self.lib.fmb_adamw_step, ctypes.byref(self._args), self._tensors, len(self.params)),
                    "fmb_adamw_step")
-        if self._tracked:
-            torch.autograd.graph.increment_version(self._tracked)        # the weights have changed in place
+        # weights and copies have changed in place: a graph that saved one, to go on to its activations, must not run with the new values
+        if written:
+            torch.autograd.graph.increment_version(written)
 
     @property
     def steps(self) -> int:

@@ -202,3 +202,32 @@ def test_lists_that_share_memory_or_move():
     weight.data = torch.ones(100, device="cuda")
     with pytest.raises(ValueError, match="other memory"):
         optimiser.step([torch.ones(100, device="cuda")])
+
+
+@pytest.mark.parametrize("saved", ["plain", "copy", "asked later"])
+def test_graphs_that_saved_a_weight_find_out(saved):
+    """The gradient in the activations needs the weight that the product was made with, whether or not that asks for one itself."""
+    from fastmace_b200.optimiser import AdamW
+    weights = {n: torch.randn(16, 16, device="cuda") for n in "ab"}
+    copies = {n: w.to(torch.bfloat16) for n, w in weights.items()}
+    optimiser = AdamW(weights, copies=copies)
+    if saved == "asked later":
+        weights["a"].requires_grad_()
+    used = {n: (copies if saved == "copy" else weights)[n] for n in "ab"}
+    x = torch.randn(4, 16, device="cuda", dtype=used["a"].dtype, requires_grad=True)
+    outputs = {n: (x @ w).sum() for n, w in used.items()}
+    optimiser.step({"a": torch.ones(16, 16, device="cuda")})
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        outputs["a"].backward()
+    outputs["b"].backward()                                # no gradient, no step
+    # sums of 16 products with ones: 16 additions in fp32 in an order that is the library's, and the result's own rounding
+    ref, size = used["b"].double().sum(1), used["b"].double().abs().sum(1)
+    assert bool(((x.grad.double() - ref).abs() <= 16 * 2.0 ** -24 * size * 1.01 + torch.finfo(x.dtype).eps / 2 * size).all())
+
+
+def test_tensors_of_inference_mode_are_stepped():
+    from fastmace_b200.optimiser import AdamW
+    with torch.inference_mode():
+        weight = torch.ones(300, device="cuda")
+        AdamW([weight]).step([torch.ones(300, device="cuda")])
+        assert bool((weight < 1).all())
