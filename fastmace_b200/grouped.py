@@ -88,6 +88,12 @@ def _launch(index: int, call, *arguments):
         return call(*arguments, stream)
 
 
+def _written(out: torch.Tensor) -> None:
+    """Tells autograd that a given output has changed in place (inference tensors have no version to count)."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+
+
 def group_rows(keys: torch.Tensor, n_groups: int) -> RowGroups:
     """Rows by group for ``keys`` (int32 or int64, one per row): a stable order, so equal keys keep the order of their rows.
     1 to 1,024 groups. Does not synchronise."""
@@ -193,6 +199,8 @@ def _rows_product(what: str, entry: str, source, weight, groups, out, transposed
             scratch = torch.empty(need, dtype=torch.float32, device=source.device)
             a.scratch = scratch.data_ptr()
         _lib.check(_launch(index, getattr(lib, entry), call), entry)
+        if given:
+            _written(out)
     return out
 
 
@@ -219,7 +227,8 @@ def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: Ro
         raise ValueError(f"{what}: x and dy must have the same type, float32, bfloat16 or float16")
     count = _groups(what, groups, rows)
     index = _on_device(what, x, dy, *groups)
-    if out is None:
+    given = out is not None
+    if not given:
         if accumulate:
             raise ValueError(f"{what}: accumulate needs out")
         out = torch.empty((count, k, n), dtype=torch.float32, device=x.device)
@@ -242,6 +251,8 @@ def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: Ro
         scratch = torch.empty(need, dtype=torch.float32, device=x.device)
         a.scratch = scratch.data_ptr()
     _lib.check(_launch(index, lib.fmb_grouped_weight_gradient, ctypes.byref(a)), "fmb_grouped_weight_gradient")
+    if given:
+        _written(out)
     return out
 
 

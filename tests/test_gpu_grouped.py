@@ -450,3 +450,21 @@ def test_outputs_that_share_memory_with_operands():
     grouped.grouped_linear(nodes[:, 0], w, plan, out=nodes[:, 2])
     _check_rows(nodes[:, 2], before[:, 0], w, keys)
     assert torch.equal(nodes[:, 0], before[:, 0]) and torch.equal(nodes[:, 1], before[:, 1]) and torch.equal(nodes[:, 3], before[:, 3])
+
+
+def test_graphs_that_saved_a_given_output_find_out():
+    from fastmace_b200 import grouped
+    x, dy, w = torch.ones(8, 16, device="cuda"), torch.ones(8, 8, device="cuda"), torch.ones(2, 16, 8, device="cuda")
+    plan = grouped.group_rows(torch.zeros(8, dtype=torch.int32, device="cuda"), 2)
+    for call, shape in ((lambda out: grouped.grouped_linear(x, w, plan, out=out), (8, 8)),
+                        (lambda out: grouped.grouped_linear_input_gradient(dy, w, plan, out=out), (8, 16)),
+                        (lambda out: grouped.grouped_linear_weight_gradient(x, dy, plan, out=out, accumulate=True), (2, 16, 8))):
+        out = torch.zeros(shape, device="cuda")
+        factor = torch.ones(shape, device="cuda", requires_grad=True)
+        saved = (factor * out).sum()
+        call(out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.backward()
+    with torch.inference_mode():
+        out = torch.zeros(8, 8, device="cuda")
+        assert bool((grouped.grouped_linear(x, w, plan, out=out) == 16).all())
