@@ -729,7 +729,8 @@ int weight_gradient(const fmb_grouped_t* a, const Plan& plan, cudaStream_t strea
     p.feature_tiles = ceil_div(a->n, plan.pair ? 256 : 128);
     const long long tiles = most_units(a, plan.unit_rows) * p.feature_tiles * p.row_tiles;
     CUtensorMap features, rows, weights = {};
-    p.by_tma = !a->accumulate && encode_map(&weights, FMB_TYPE_F32, a->w, a->n, a->k, a->groups, a->w_row_stride, a->w_group_stride, 16, 3, 128, false);
+    // (a store writes whole pieces of 16 bytes: of rows that end within one, it would write zeros over what lies beside them)
+    p.by_tma = !a->accumulate && a->n % 4 == 0 && encode_map(&weights, FMB_TYPE_F32, a->w, a->n, a->k, a->groups, a->w_row_stride, a->w_group_stride, 16, 3, 128, false);
     int rc;
     if (plan.sorted) {
         void* const x = (char*)a->scratch + plan.x;

@@ -27,7 +27,8 @@ __device__ __forceinline__ void tma_gather4(uint32_t dst, const CUtensorMap* map
                  :: "r"(dst), "l"(map), "r"(col), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar) : "memory");
 }
 
-// from shared memory, by threads that a proxy fence of the writers and a barrier precede; what lies outside the tensor is not written
+// from shared memory, by threads that a proxy fence of the writers and a barrier precede; what lies outside the tensor is not written,
+// apart from the rest of a row's last 16 bytes
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
     asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
                  :: "l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2) : "memory");

@@ -468,3 +468,35 @@ def test_graphs_that_saved_a_given_output_find_out():
     with torch.inference_mode():
         out = torch.zeros(8, 8, device="cuda")
         assert bool((grouped.grouped_linear(x, w, plan, out=out) == 16).all())
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,groups,k,n", [(90, 3, 13, 21), (300, 2, 65, 129), (700, 5, 130, 515), (9, 4, 515, 301), (5000, 2, 263, 391),
+                                             (3000, 40, 1026, 1030)])
+def test_what_lies_beside_operands_and_outputs(rows, groups, k, n, dtype):
+    """Rows at multiples of 16 bytes whose lengths are none: what is behind the end of a row of an operand (NaN here) takes no part,
+    and behind that of an output stays as it was."""
+    from fastmace_b200 import grouped
+    g = torch.Generator(device="cuda").manual_seed(k)
+    keys = torch.randint(-1, groups, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    plan = grouped.group_rows(keys, groups)
+
+    def room(*shape, fill, dtype=dtype):
+        return torch.full((*shape[:-1], (shape[-1] + 15) // 8 * 8), fill, dtype=dtype, device="cuda")
+
+    def within(*shape, scale=1.0):
+        t = room(*shape, fill=float("nan"))[..., :shape[-1]]
+        return t.copy_(torch.randn(*shape, generator=g, device="cuda") * scale)
+
+    x, dy, w = within(rows, k), within(rows, n), within(groups, k, n, scale=k ** -0.5)
+    y, dx, dw = room(rows, n, fill=7.0), room(rows, k, fill=7.0), room(groups, k, n, fill=7.0, dtype=F32)
+    grouped.grouped_linear(x, w, plan, out=y[:, :n])
+    grouped.grouped_linear_input_gradient(dy, w, plan, out=dx[:, :k])
+    grouped.grouped_linear_weight_gradient(x, dy, plan, out=dw[:, :, :n])
+    live = keys >= 0
+    _check_rows(y[live][:, :n], x[live], w, keys[live])
+    _check_rows(dx[live][:, :k], dy[live], w, keys[live], transposed=True)
+    _check_weights(dw[:, :, :n], x, dy, keys)
+    for t, width in ((y, n), (dx, k), (dw, n)):
+        assert bool((t[..., width:] == 7).all())
+    grouped.check_status()
