@@ -805,7 +805,8 @@ bool encode_map(CUtensorMap* map, int type, const void* base, int columns, int r
     const Encode encode = encoder();
     const int bytes = type == FMB_TYPE_F32 ? 4 : 2, unit = 16 / bytes;           // values in 16 bytes
     if (!encode || ((uintptr_t)base & 15) != 0) return false;
-    if (rows == 1) row_stride = std::max<long long>(row_stride, (columns + unit - 1) / unit * unit);     // never used
+    // (what is never used may have any value at the caller's: the stride of a single row, or of a single group)
+    if (rows == 1) row_stride = (columns + unit - 1) / unit * unit;
     if (groups == 1) group_stride = unit;
     if (row_stride <= 0 || row_stride % unit || row_stride >= (1ll << 37)) return false;
     if (dims == 3 && (group_stride <= 0 || group_stride % unit || group_stride >= (1ll << 37))) return false;

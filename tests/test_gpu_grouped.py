@@ -500,3 +500,25 @@ def test_what_lies_beside_operands_and_outputs(rows, groups, k, n, dtype):
     for t, width in ((y, n), (dx, k), (dw, n)):
         assert bool((t[..., width:] == 7).all())
     grouped.check_status()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("n", [13, 64, 200, 515])
+@pytest.mark.parametrize("wide", [(8, 21), (3, 2), (4, 0), (1, 8)])
+def test_weights_of_one_row_cut_from_wider_ones(dtype, n, wide):
+    """k == 1: the distance between the rows of a matrix, which nothing uses, may be anything; that between matrices as well."""
+    from fastmace_b200 import grouped
+    deep, more = wide
+    g = torch.Generator(device="cuda").manual_seed(n + deep)
+    keys = torch.randint(-1, 3, (70,), generator=g, device="cuda", dtype=torch.int32)
+    plan = grouped.group_rows(keys, 3)
+    w = torch.randn(3, deep, n + more, generator=g, device="cuda").to(dtype)[:, :1, :n]
+    x = torch.randn(70, 1, generator=g, device="cuda").to(dtype)
+    dy = torch.randn(70, n, generator=g, device="cuda").to(dtype)
+    _check_rows(grouped.grouped_linear(x, w, plan), x, w, keys)
+    _check_rows(grouped.grouped_linear_input_gradient(dy, w, plan), dy, w, keys, transposed=True)
+    room = torch.full((3, deep, n + more), 7.0, device="cuda")
+    dw = grouped.grouped_linear_weight_gradient(x, dy, plan, out=room[:, :1, :n])
+    _check_weights(dw, x, dy, keys)
+    assert bool((room[:, 1:] == 7).all()) and bool((room[:, :, n:] == 7).all())
+    grouped.check_status()
