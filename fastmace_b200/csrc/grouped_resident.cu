@@ -252,7 +252,7 @@ k_grouped_resident(const __grid_constant__ SplitArgs p, const __grid_constant__ 
                 }
                 named_barrier(1 + set, 128);                 // what was here has been read
 #pragma unroll
-                for (int j = 0; j < kTurnRows; ++j) turn[j * 128 + id] = v[j] + u[j];
+                for (int j = 0; j < kTurnRows; ++j) turn[j * 128 + id] = infinite(v[j]) ? v[j] : v[j] + u[j];
                 named_barrier(1 + set, 128);
                 float4 q[4];
 #pragma unroll

@@ -217,6 +217,12 @@ __device__ __forceinline__ float4 load_quad(const float* p, int live, bool wide)
 __device__ __forceinline__ uint32_t upper_halves(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }
 __device__ __forceinline__ float without_upper(float x) { return x - __uint_as_float(__float_as_uint(x) & 0xffff0000u); }
 
+// Infinities: all of one is in its upper half, and what it leaves there is no number. So where the products of the upper halves, hi hi,
+// are infinite, they alone are the result; the kernels leave out the five others there. (A signalling NaN that has nothing in its upper
+// half but the exponent, which no operation makes, counts as an infinity. Made the usual one while it is split, by an addition of -0 to
+// every value, it costs the deep products 5 %: 9,000 x 2,048 x 1,024 223 -> 234 us.)
+__device__ __forceinline__ bool infinite(float x) { return fabsf(x) == __uint_as_float(0x7f800000u); }
+
 // the three bf16 parts of four consecutive values, at byte `offset` of each part's tile
 template <int PART_BYTES>
 __device__ __forceinline__ void store_quad(uint8_t* tile, uint32_t offset, float4 q) {

@@ -522,3 +522,42 @@ def test_weights_of_one_row_cut_from_wider_ones(dtype, n, wide):
     _check_weights(dw, x, dy, keys)
     assert bool((room[:, 1:] == 7).all()) and bool((room[:, :, n:] == 7).all())
     grouped.check_status()
+
+
+@pytest.mark.parametrize("rows,k,n", [(200, 64, 96), (200, 128, 200), (200, 300, 96), (8, 4096, 136), (70, 13, 21)])
+def test_infinities_in_fp32_give_what_the_plain_product_gives(rows, k, n):
+    """Infinities of both signs, NaN and zeros opposite to them, in rows and in weights; half of the finite values have eight significant
+    bits at most, so that the lower parts of their splits are zeros. Where float64 has a number the others keep the usual bound."""
+    from fastmace_b200 import grouped
+    g = torch.Generator(device="cuda").manual_seed(k)
+    keys = torch.arange(rows, device="cuda") % 2
+    plan = grouped.group_rows(keys, 2)
+    inf, nan = float("inf"), float("nan")
+
+    def values(*shape):
+        t = torch.randn(*shape, generator=g, device="cuda")
+        t[..., ::2] = t[..., ::2].to(BF16).float()
+        return t
+
+    def check(got, a, b):
+        ref = a.double() @ b.double()
+        fine = torch.isfinite(ref)
+        assert torch.equal(torch.isnan(got), torch.isnan(ref)) and torch.equal(got.isinf(), ref.isinf())
+        assert torch.equal(got[got.isinf()].double(), ref[got.isinf()])
+        assert bool(((got.double() - ref).abs() <= (a.shape[1] + 8) * 2.0 ** -24 * (a.double().abs() @ b.double().abs()))[fine].all())
+
+    x, dy, w = values(rows, k), values(rows, n), values(2, k, n)
+    for t in (x, dy):
+        t[0, 2], t[1, 6], t[2, 7], t[3, 3], t[4, 5] = inf, -inf, nan, inf, -inf
+        t[5, 2], t[5, 4] = inf, inf
+        t[6, 2], t[6, 4] = inf, -inf
+    w[0, 2, :9:2], w[1, 6, 1:8:3], w[:, 3, 11], w[:, 10, 5] = 0.0, 0.0, inf, -inf
+    for each, kept in ((w, w.clone()), (torch.ones_like(w), torch.ones_like(w))):
+        y, dx = grouped.grouped_linear(x, each, plan), grouped.grouped_linear_input_gradient(dy, each, plan)
+        for q in range(2):
+            check(y[keys == q], x[keys == q], kept[q])
+            check(dx[keys == q], dy[keys == q], kept[q].t())
+    dw = grouped.grouped_linear_weight_gradient(x, dy, plan)
+    for q in range(2):
+        check(dw[q], x[keys == q].t(), dy[keys == q])
+    grouped.check_status()
