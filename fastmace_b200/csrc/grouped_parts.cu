@@ -1,7 +1,7 @@
 // Grouped products in fp32: linear, input gradient and weight gradient (linears of a depth of up to 128: grouped_resident.cu).
 //
-// x = hi + mid + lo with eight significant bits each, cut off rather than rounded, is exact, at every size a float has (no
-// scales). Of the nine products of two such triples of bf16 the six largest are taken,
+// x = hi + mid + lo with eight significant bits each, cut off rather than rounded, is exact from 2^-110 on, without scales: bf16 reaches
+// down to 2^-133, and what of a smaller x lies below that is lost. Of the nine products of two such triples of bf16 the six largest are taken,
 //     hi hi | hi mid + mid hi | hi lo + mid mid + lo hi        (what is left out is below 2^-21 of |x| |w|, 2^-24 on average)
 // The tensor core cuts its accumulator off at every instruction, so hi hi has columns of its own -- the others are 2^-8 of
 // it -- and accumulators move to fp32 registers every kChunk of the depth. Against tf32 pairs: the same tensor time (six products

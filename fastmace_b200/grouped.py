@@ -9,8 +9,8 @@ experts of a layer -- with any number of rows per group, and their gradients (``
 Rows keep their places: row r of ``y`` belongs to row r of ``x`` whatever the order of the groups. ``x`` and ``dy`` may be
 views whose rows are further apart than they are long (a component of ``[atom][component][channel]`` features), ``weight``
 any ``[groups, k, n]`` view with contiguous columns (``w["l1.skip.0"].permute(1, 0, 2)``). Types: float32, bfloat16, float16,
-the same for all operands of a call; sums are in float32 at least (float32 operands keep their 24 bits), the weight gradient
-is float32 whatever the operands'. A row of no group (key negative or >= the number of groups) is zero in an output the call
+the same for all operands of a call; sums are in float32 at least, the weight gradient is float32 whatever the operands'. float32
+operands keep their 24 bits from 2^-110 on, and less of smaller ones: what lies below 2^-133 is lost. A row of no group (key negative or >= the number of groups) is zero in an output the call
 allocates, left as it was in one that is given, and takes no part in a weight gradient.
 
 Calls run on the current stream of the operands' device and allocate their outputs and scratch from torch's allocator, so

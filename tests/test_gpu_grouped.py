@@ -561,3 +561,23 @@ def test_infinities_in_fp32_give_what_the_plain_product_gives(rows, k, n):
     for q in range(2):
         check(dw[q], x[keys == q].t(), dy[keys == q])
     grouped.check_status()
+
+
+@pytest.mark.parametrize("size", [-105, -112, -120, -126, -132])
+@pytest.mark.parametrize("k", [64, 300, 2100])
+def test_smallest_fp32_operands_against_large_ones(size, k):
+    """Products that are ordinary numbers of operands about 2^size and 2^60. The last of the three bf16 parts of a value ends at 2^-133,
+    bf16's smallest number: up to that much of each value is lost, times what it is multiplied by, beside the usual bound."""
+    from fastmace_b200 import grouped
+    g = torch.Generator(device="cuda").manual_seed(k)
+    keys = torch.arange(40, device="cuda") % 2
+    plan = grouped.group_rows(keys, 2)
+    small = torch.randn(40, k, generator=g, device="cuda") * 2.0 ** -60 * 2.0 ** (size + 60)
+    w = torch.randn(2, k, 200, generator=g, device="cuda") * 2.0 ** 60
+    large = torch.randn(40, 200, generator=g, device="cuda") * 2.0 ** 60
+    y, dw = grouped.grouped_linear(small, w, plan), grouped.grouped_linear_weight_gradient(small, large, plan)
+    for q in range(2):
+        for got, a, b in ((y[keys == q], small[keys == q], w[q]), (dw[q], small[keys == q].t(), large[keys == q])):
+            a, b = a.double(), b.double()
+            tol = (a.shape[1] + 8) * 2.0 ** -24 * (a.abs() @ b.abs()) + 2.0 ** -133 * b.abs().sum(0)
+            assert bool(((got.double() - a @ b).abs() <= tol).all())
