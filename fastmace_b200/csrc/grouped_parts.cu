@@ -447,6 +447,7 @@ int launch(const SplitArgs& p, const CUtensorMap& features, const CUtensorMap& r
         config.attrs = &cluster;
         config.numAttrs = 1;
         FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_grouped_parts<MODE>, p, features, rows, wide_out));
+        FMB_LAUNCH_CHECK();
         return FMB_OK;
     }
     const long long tiles = most_units(&p.a, p.unit_rows) * p.feature_tiles * p.row_tiles;

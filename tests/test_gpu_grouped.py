@@ -581,3 +581,15 @@ def test_smallest_fp32_operands_against_large_ones(size, k):
             a, b = a.double(), b.double()
             tol = (a.shape[1] + 8) * 2.0 ** -24 * (a.abs() @ b.abs()) + 2.0 ** -133 * b.abs().sum(0)
             assert bool(((got.double() - a @ b).abs() <= tol).all())
+
+
+@pytest.mark.parametrize("dtype,k", [(F32, 2048), (F32, 256), (F32, 64), (BF16, 2048), (BF16, 64)])
+def test_every_launch_is_counted(dtype, k):
+    """Single tokens, with and without clusters that share the depth: one kernel a linear."""
+    from fastmace_b200 import _lib, grouped
+    lib = _lib.load()
+    plan = grouped.group_rows(torch.arange(8, device="cuda"), 8)
+    x, w = torch.ones(8, k, dtype=dtype, device="cuda"), torch.ones(8, k, 1024, dtype=dtype, device="cuda")
+    before = lib.fmb_launch_count()
+    grouped.grouped_linear(x, w, plan)
+    assert lib.fmb_launch_count() == before + 1
