@@ -102,6 +102,8 @@ class AdamW:
         # the gradients' pointers of the list above, as one column
         self._pointers = np.frombuffer(self._tensors, dtype=np.int64).reshape(len(self.params), -1)[:, 1]
         self._args = _lib.AdamwStruct()
+        # whether a step has been captured, and the moments that captured steps go on with since others were loaded
+        self._captured, self._replaced = False, []
 
     def _fill_args(self) -> None:
         a = self._args
@@ -140,6 +142,7 @@ class AdamW:
         if [g.shape for g in grads] != shapes or not all(map(torch.Tensor.is_contiguous, grads)) or \
                 set(map(torch.Tensor.get_device, grads)) != {self._index}:
             raise ValueError("AdamW.step: a gradient must be contiguous, of its weights' shape and on their device")
+        self._captured = self._captured or torch.cuda.is_current_stream_capturing()
         self._fill_args()
         self._args.grad_type = TYPES[kind]
         _lib.check(_launch(self._index, self.lib.fmb_adamw_step, ctypes.byref(self._args), self._tensors, len(self.params)),
@@ -156,7 +159,7 @@ class AdamW:
     def load_moments(self, steps: int, *moments: torch.Tensor) -> None:
         """Continue from the moments of a run of ``steps`` steps: ``m, v`` (32 bits) or ``m, m_scale, v, v_scale`` (8 bits), as
         this class holds them under these names. The optimiser uses the tensors given, it does not copy them; a step captured before
-        goes on with the ones it had."""
+        goes on with the ones it had, which the optimiser keeps for it."""
         names = ("m", "v") if self.state_bits == 32 else ("m", "m_scale", "v", "v_scale")
         if len(moments) != len(names) or steps < 0:
             raise ValueError(f"AdamW.load_moments: steps and {', '.join(names)}")
@@ -166,6 +169,8 @@ class AdamW:
                 raise ValueError(f"AdamW.load_moments: {name} must be a contiguous {like.dtype} tensor {tuple(like.shape)}")
             if t.data_ptr() % 16:
                 raise ValueError(f"AdamW.load_moments: {name} must start at a multiple of 16 bytes")
+        if self._captured:
+            self._replaced.extend(getattr(self, name) for name in names)
         for name, t in zip(names, moments):
             setattr(self, name, t)
         self._state.copy_(torch.tensor([steps, self.betas[0] ** steps, self.betas[1] ** steps, 0.0], dtype=torch.float64))

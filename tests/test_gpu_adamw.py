@@ -231,3 +231,34 @@ def test_tensors_of_inference_mode_are_stepped():
         weight = torch.ones(300, device="cuda")
         AdamW([weight]).step([torch.ones(300, device="cuda")])
         assert bool((weight < 1).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_of_a_captured_step_live_on(bits):
+    """A captured step goes on with the moments it was captured with after others have been loaded: they stay allocated, and the loaded
+    ones are not its."""
+    import weakref
+
+    from fastmace_b200.optimiser import AdamW
+    weight, grad = torch.ones(1000, device="cuda"), torch.ones(1000, device="cuda")
+    optimiser = AdamW([weight], state_bits=bits)
+    optimiser.step([grad])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        optimiser.step([grad])
+    names = ("m", "v") if bits == 32 else ("m", "m_scale", "v", "v_scale")
+    old = [weakref.ref(getattr(optimiser, name)) for name in names]
+    loaded = [getattr(optimiser, name).clone() for name in names]
+    kept = [t.clone() for t in loaded]
+    optimiser.load_moments(1, *loaded)
+    assert all(ref() is not None for ref in old)
+    before = [ref().clone() for ref in old]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(loaded, kept))
+    assert any(not torch.equal(ref().view(torch.uint8), b.view(torch.uint8)) for ref, b in zip(old, before))
+    # without a captured step nothing is kept
+    other = AdamW([torch.ones(1000, device="cuda")], state_bits=bits)
+    gone = weakref.ref(other.m)
+    other.load_moments(1, *(t.clone() for t in loaded))
+    assert gone() is None
