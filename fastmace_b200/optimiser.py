@@ -75,8 +75,9 @@ class AdamW:
         held = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in [*self.params, *self.copies] if t is not None and t.numel())
         if any(here + size > there for (here, size), (there, _) in zip(held, held[1:])):
             raise ValueError("AdamW: a tensor is listed twice, or two share memory")
-        # where the weights lie, and what keeps that memory while the optimiser lives
-        self._places, self._held = [p.data_ptr() for p in self.params], [p.detach() for p in self.params]
+        # where weights and copies lie, and what keeps that memory while the optimiser lives
+        self._listed = [t for t in (*self.params, *self.copies) if t is not None]
+        self._places, self._held = [t.data_ptr() for t in self._listed], [t.detach() for t in self._listed]
         # what a step writes to, for autograd, of each tensor (inference tensors have no version to count)
         self._written = [[t for t in pair if t is not None and not t.is_inference()] for pair in zip(self.params, self.copies)]
         self._all_written = sum(self._written, [])
@@ -124,7 +125,7 @@ class AdamW:
         elif len(grads) != len(self.params):
             raise ValueError(f"AdamW.step: {len(grads)} gradients for {len(self.params)} tensors")
         # (mapped methods: looking over 117 small tensors takes the host longer than their step takes the device, 17 us)
-        if list(map(_place, self.params)) != self._places:
+        if list(map(_place, self._listed)) != self._places:
             raise ValueError("AdamW.step: a tensor of the list has been given other memory since")
         shapes, written = self._shapes, self._all_written
         if any(g is None for g in grads):

@@ -262,3 +262,19 @@ def test_moments_of_a_captured_step_live_on(bits):
     gone = weakref.ref(other.m)
     other.load_moments(1, *(t.clone() for t in loaded))
     assert gone() is None
+
+
+def test_a_copy_that_moved_is_refused():
+    """As a weight that moved: the step would write to where the copy was, which lives on all the same."""
+    from fastmace_b200.optimiser import AdamW
+    weights = [torch.ones(300, device="cuda"), torch.ones(5, device="cuda")]
+    copy = torch.zeros(300, dtype=torch.bfloat16, device="cuda")
+    optimiser = AdamW(weights, copies=[copy, None])
+    optimiser.step([torch.ones_like(w) for w in weights])
+    assert torch.equal(copy, weights[0].to(torch.bfloat16))
+    place, storage = copy.data_ptr(), torch.empty(300, dtype=torch.bfloat16, device="cuda")
+    copy.data = storage
+    taken = [torch.empty(300, dtype=torch.bfloat16, device="cuda") for _ in range(8)]
+    assert all(t.data_ptr() != place for t in taken)
+    with pytest.raises(ValueError, match="other memory"):
+        optimiser.step([torch.ones_like(w) for w in weights])
