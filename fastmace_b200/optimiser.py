@@ -35,6 +35,12 @@ BLOCK = _lib.ADAMW_BLOCK
 _place = torch.Tensor.data_ptr
 
 
+def _share_memory(tensors) -> bool:
+    """Whether two of these contiguous tensors overlap."""
+    held = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in tensors if t.numel())
+    return any(here + size > there for (here, size), (there, _) in zip(held, held[1:]))
+
+
 class AdamW:
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
                  state_bits: int = 32, copies=None):
@@ -72,8 +78,7 @@ class AdamW:
             if self._copy_type not in (0, TYPES[c.dtype]):
                 raise ValueError("AdamW: the copies must have one type")
             self._copy_type = TYPES[c.dtype]
-        held = sorted((t.data_ptr(), t.numel() * t.element_size()) for t in [*self.params, *self.copies] if t is not None and t.numel())
-        if any(here + size > there for (here, size), (there, _) in zip(held, held[1:])):
+        if _share_memory([t for t in (*self.params, *self.copies) if t is not None]):
             raise ValueError("AdamW: a tensor is listed twice, or two share memory")
         # where weights and copies lie, and what keeps that memory while the optimiser lives
         self._listed = [t for t in (*self.params, *self.copies) if t is not None]
@@ -162,7 +167,7 @@ class AdamW:
         this class holds them under these names. The optimiser uses the tensors given, it does not copy them; a step captured before
         goes on with the ones it had, which the optimiser keeps for it."""
         names = ("m", "v") if self.state_bits == 32 else ("m", "m_scale", "v", "v_scale")
-        if len(moments) != len(names) or steps < 0:
+        if len(moments) != len(names) or int(steps) != steps or steps < 0:
             raise ValueError(f"AdamW.load_moments: steps and {', '.join(names)}")
         for name, t in zip(names, moments):
             like = getattr(self, name)
@@ -170,6 +175,8 @@ class AdamW:
                 raise ValueError(f"AdamW.load_moments: {name} must be a contiguous {like.dtype} tensor {tuple(like.shape)}")
             if t.data_ptr() % 16:
                 raise ValueError(f"AdamW.load_moments: {name} must start at a multiple of 16 bytes")
+        if _share_memory([*moments, *self._listed]):
+            raise ValueError("AdamW.load_moments: two of the moments share memory, or one with a weight or copy")
         if self._captured:
             self._replaced.extend(getattr(self, name) for name in names)
         for name, t in zip(names, moments):

@@ -278,3 +278,24 @@ def test_a_copy_that_moved_is_refused():
     assert all(t.data_ptr() != place for t in taken)
     with pytest.raises(ValueError, match="other memory"):
         optimiser.step([torch.ones_like(w) for w in weights])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_moments_that_share_memory_are_refused(bits):
+    from fastmace_b200.optimiser import AdamW
+    weight = torch.ones(512, device="cuda")
+    optimiser = AdamW([weight], state_bits=bits)
+    names = ("m", "v") if bits == 32 else ("m", "m_scale", "v", "v_scale")
+    fine = {name: getattr(optimiser, name).clone() for name in names}
+    room = torch.zeros(1000, dtype=fine["m"].dtype, device="cuda")
+    bad = [{**fine, "v": fine["m"]}, {**fine, "m": room[:512], "v": room[256:768]}]
+    bad.append({**fine, "m": weight} if bits == 32 else {**fine, "v_scale": weight[:2]})
+    for moments in bad:
+        with pytest.raises(ValueError, match="share"):
+            optimiser.load_moments(1, *moments.values())
+    for steps in (-1, 2.5):
+        with pytest.raises(ValueError):
+            optimiser.load_moments(steps, *fine.values())
+    optimiser.load_moments(1, *fine.values())
+    optimiser.step([torch.ones(512, device="cuda")])
+    assert optimiser.steps == 2
