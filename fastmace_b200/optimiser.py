@@ -24,6 +24,7 @@ counted on the device, the learning rate and the other constants are those at ca
 from __future__ import annotations
 
 import ctypes
+import math
 
 import numpy as np
 import torch
@@ -52,8 +53,8 @@ class AdamW:
             raise ValueError("AdamW: state_bits is 8 or 32")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError("AdamW: betas in [0, 1)")
-        if lr < 0.0 or eps < 0.0 or weight_decay < 0.0:
-            raise ValueError("AdamW: lr, eps and weight_decay must not be negative")
+        if not all(0.0 <= x < math.inf for x in (lr, eps, weight_decay)):
+            raise ValueError("AdamW: lr, eps and weight_decay must be finite and not negative")
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), tuple(float(b) for b in betas), float(eps), float(weight_decay)
         self.state_bits = int(state_bits)
         self.device = self.params[0].device

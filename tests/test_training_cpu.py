@@ -90,3 +90,11 @@ def test_what_shares_memory():
     assert _shares_memory(wide.as_strided((5, 10), (16, 1), 0), wide.as_strided((5, 10), (16, 1), 12))
     assert _shares_memory(wide[:64].view(8, 8), wide[8:72].view(2, 4, 8))
     assert _shares_memory(wide[:64].view(8, 8), wide[:64].view(torch.float16).view(8, 16))
+
+
+@pytest.mark.parametrize("change", [dict(lr=float("nan")), dict(lr=float("inf")), dict(eps=float("nan")), dict(weight_decay=float("nan")),
+                                    dict(betas=(float("nan"), 0.9)), dict(betas=(0.9, float("nan"))), dict(weight_decay=-1.0)])
+def test_constants_that_are_no_numbers_are_refused(change):
+    from fastmace_b200.optimiser import AdamW
+    with pytest.raises(ValueError, match="finite|betas"):
+        AdamW([torch.zeros(4)], **change)
