@@ -123,7 +123,7 @@ class AdamwTensorStruct(ctypes.Structure):
 
 class AdamwStruct(ctypes.Structure):
     _fields_ = [
-        ("moment_bits", c_int32), ("grad_type", c_int32), ("copy_type", c_int32), ("reserved", c_int32),
+        ("moment_bits", c_int32), ("grad_type", c_int32), ("copy_type", c_int32), ("random", c_int32),
         ("lr", c_double), ("beta1", c_double), ("beta2", c_double), ("eps", c_double), ("weight_decay", c_double),
         ("m", c_void_p), ("v", c_void_p), ("m_scale", c_void_p), ("v_scale", c_void_p), ("state", c_void_p),
     ]

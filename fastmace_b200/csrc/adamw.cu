@@ -4,8 +4,13 @@
 // step is a device counter that the last CTA to finish advances. A warp takes a block of 256 values, two float4 per lane and
 // array. With moments in 8 bits the block shares a scale per moment: first moments are held as e4m3 of m / s, second
 // moments as e4m3 of sqrt(v) / s, s = (largest of the block) / 448. Relative steps of 2^-4 over 2^15 and the root's smaller
-// range keep the quotient m / sqrt(v) to a few per cent of itself; a v that is not zero is never held as zero, which would make
-// the next quotient m / eps. Arithmetic is in fp32, and
+// range keep the quotient m / sqrt(v) of one step to a few per cent of itself; a v that is not zero is never held as zero, which would
+// make the next quotient m / eps. Over many steps that is not enough: with beta2 = 0.999 a root moves by 0.05 % a step downwards and
+// codes are 6 to 12 % apart, so that rounded to the nearest a code stays and the value follows its block's largest instead of its own
+// gradients. Held at random (Table::random), as the code below or above with the chances that make the expected v the exact one, it follows
+// its moving average: the expectation of v is that of fp32 at every step, and its root spreads about that by a sixth, which codes a
+// twelfth apart and a memory of 2,000 steps make. The bits are Philox's, of the step, the place of the value and a key, 16 a
+// value. First moments move by a tenth a step and are rounded to the nearest. Arithmetic is in fp32, and
 // that of the moments is rounded operation by operation, as it is written here: a moment that came out a bit
 // apart could take the next code, 2^-4 away, and with the block's largest the scale would follow a step later.
 //
@@ -14,6 +19,7 @@
 // conversions and exact quotients an SM keep it at 74 % of its rate), the 43 tensors of a medium model 27 (4.7 M values, 131 MB).
 
 #include "fmb_common.cuh"
+#include "philox.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -46,6 +52,7 @@ struct Table {
     int count;
     int advance;                 // the last launch of a step counts it
     int copy_type;
+    uint32_t random;             // 8 bits: key of the random rounding of second moments
     long long blocks;            // of the launch
     float decay, lr, b1, c1, b2, c2, eps;
     double beta1, beta2;
@@ -91,6 +98,28 @@ __device__ __forceinline__ float block_scale(float largest) {
 __device__ __forceinline__ float quotient(float x, float scale, float inverse) {
     const float q = __fmul_rn(x, inverse);
     return fmaf(fmaf(-q, scale, x), inverse, q);
+}
+
+// code of x / scale for x >= 0: the number of the type below q or the one above, which has the chance (q^2 - below^2) / (above^2 - below^2).
+// Below 2^-6 the numbers are 2^-9 apart, as they are between 2^-6 and 2^-5, and q moves there.
+__device__ __forceinline__ float either(float q, uint32_t bits) {
+    const float u = (float)bits * (1.0f / 65536.0f) + (0.5f / 65536.0f), base = q < 0x1p-6f ? 0x1p-6f : 0.0f;
+    const uint32_t cut = __float_as_uint(q + base) & 0xfff00000u;
+    const float below = __uint_as_float(cut) - base, above = __uint_as_float(cut + 0x00100000u) - base;
+    return u * ((above - below) * (above + below)) < (q - below) * (q + below) ? above : below;
+}
+__device__ __forceinline__ uint32_t encode_four_either(const float (&x)[4], float scale, float inverse, uint32_t bits_low, uint32_t bits_high) {
+    uint32_t out = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t bits = i ? bits_high : bits_low;
+        const float2 q = make_float2(either(quotient(x[2 * i], scale, inverse), bits & 0xffffu), either(quotient(x[2 * i + 1], scale, inverse), bits >> 16));
+        uint32_t two = __nv_cvt_float2_to_fp8x2(q, __NV_SATFINITE, __NV_E4M3);
+        if (x[2 * i] > 0.0f && (two & 0xffu) == 0) two |= 1u;
+        if (x[2 * i + 1] > 0.0f && (two >> 8) == 0) two |= 0x100u;
+        out |= two << (16 * i);
+    }
+    return out;
 }
 
 // codes of x / scale; KEEP: what is positive does not become zero
@@ -160,8 +189,8 @@ __device__ __forceinline__ void load_block(const Table<CAPACITY>& t, long long b
     }
 }
 
-template <typename G, bool EIGHT, int CAPACITY>
-__device__ __forceinline__ void step_block(const Table<CAPACITY>& t, const Raw<G, EIGHT>& r, float step, float root_scale) {
+template <typename G, bool EIGHT, bool RANDOM, int CAPACITY>
+__device__ __forceinline__ void step_block(const Table<CAPACITY>& t, const Raw<G, EIGHT>& r, float step, float root_scale, uint32_t number) {
     const int lane = threadIdx.x & 31;
     const Entry& e = t.entry[r.entry];
     const long long block = e.block + r.at / kBlock, moment = block * kBlock;
@@ -204,12 +233,19 @@ __device__ __forceinline__ void step_block(const Table<CAPACITY>& t, const Raw<G
         m_inverse = __fdiv_rn(1.0f, ms);
         v_inverse = __fdiv_rn(1.0f, vs);
     }
+    uint32_t bits[4];
+    if constexpr (RANDOM) {
+        const unsigned long long at = block * 32 + lane;
+        bits[0] = (uint32_t)at; bits[1] = (uint32_t)(at >> 32); bits[2] = number; bits[3] = 0x61646d77u;
+        philox(bits, t.random, 0x6d616365u);
+    }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         const int i = h * 128 + lane * 4;
         if constexpr (EIGHT) {
             *reinterpret_cast<uint32_t*>((uint8_t*)t.m + moment + i) = encode_four<false>(m[h], ms, m_inverse);
-            *reinterpret_cast<uint32_t*>((uint8_t*)t.v + moment + i) = encode_four<true>(root[h], vs, v_inverse);
+            *reinterpret_cast<uint32_t*>((uint8_t*)t.v + moment + i) =
+                RANDOM ? encode_four_either(root[h], vs, v_inverse, bits[2 * h], bits[2 * h + 1]) : encode_four<true>(root[h], vs, v_inverse);
         } else {
             *reinterpret_cast<float4*>((float*)t.m + moment + i) = make_float4(m[h][0], m[h][1], m[h][2], m[h][3]);
             *reinterpret_cast<float4*>((float*)t.v + moment + i) = make_float4(v[h][0], v[h][1], v[h][2], v[h][3]);
@@ -244,11 +280,13 @@ __device__ __forceinline__ void step_block(const Table<CAPACITY>& t, const Raw<G
 // Moments in 8 bits: as many CTAs as the device holds, whose warps take blocks in turn, so that the whole GPU is at one place of every
 // array; in 32 bits, where a block has twice the bytes to wait for, CTAs of 16 blocks that come and go (200 M values 906 us against
 // 990; the other way round 64 M values in 8 bits 220 against 330). With 8 bits a warp asks for its next block before it works on
-// the one it has; with 32 the registers that takes cost more warps than it gains (1,070 us).
-template <typename G, bool EIGHT, int CAPACITY>
-__global__ void __launch_bounds__(kThreads)
+// the one it has; with 32 the registers that takes cost more warps than it gains (1,070 us). Random rounding takes the issue slots of ten
+// rounds and two squares a value: 64 M values 298 us, 202 to the nearest.
+template <typename G, bool EIGHT, bool RANDOM, int CAPACITY>
+__global__ void __launch_bounds__(kThreads, EIGHT ? 3 : 4)          // 80 registers, 64: what the plain ones take by themselves
 k_adamw(const __grid_constant__ Table<CAPACITY> t) {
     __shared__ float corrections[2];
+    __shared__ uint32_t steps_before;
     const int warp = threadIdx.x >> 5;
     const long long begin = (long long)blockIdx.x * (EIGHT ? kWarps : kCtaBlocks);
     const long long end = EIGHT ? t.blocks : min(t.blocks, begin + kCtaBlocks), stride = EIGHT ? (long long)gridDim.x * kWarps : kWarps;
@@ -263,19 +301,21 @@ k_adamw(const __grid_constant__ Table<CAPACITY> t) {
     if (threadIdx.x == 0) {
         corrections[0] = (float)(1.0 / (1.0 - t.state[1] * t.beta1));
         corrections[1] = (float)(1.0 / sqrt(1.0 - t.state[2] * t.beta2));
+        if (RANDOM) steps_before = (uint32_t)(unsigned long long)t.state[0];
     }
     __syncthreads();
     const float step = t.lr * corrections[0], root_scale = corrections[1];
+    const uint32_t number = RANDOM ? steps_before : 0;
 #pragma unroll 1
     for (; b < end; b += stride) {
         if constexpr (EIGHT) {
             Raw<G, EIGHT> next;
             if (b + stride < end) load_block<G, EIGHT, CAPACITY>(t, b + stride, entry, next);
-            step_block<G, EIGHT, CAPACITY>(t, raw, step, root_scale);
+            step_block<G, EIGHT, RANDOM, CAPACITY>(t, raw, step, root_scale, number);
             raw = next;
         } else {
             load_block<G, EIGHT, CAPACITY>(t, b, entry, raw);
-            step_block<G, EIGHT, CAPACITY>(t, raw, step, root_scale);
+            step_block<G, EIGHT, RANDOM, CAPACITY>(t, raw, step, root_scale, number);
         }
     }
     if (!t.advance) return;
@@ -293,28 +333,29 @@ k_adamw(const __grid_constant__ Table<CAPACITY> t) {
     }
 }
 
-template <typename G, bool EIGHT, int CAPACITY>
+template <typename G, bool EIGHT, bool RANDOM, int CAPACITY>
 int launch(const Table<CAPACITY>& t, cudaStream_t stream) {
     long long ctas = (t.blocks + kCtaBlocks - 1) / kCtaBlocks;
     if (EIGHT) {
         int dev = 0, sms = 0;
         static const int per_sm = [] {
             int n = 0;
-            return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_adamw<G, EIGHT, CAPACITY>, kThreads, 0) == cudaSuccess && n > 0 ? n : 1;
+            return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, k_adamw<G, EIGHT, RANDOM, CAPACITY>, kThreads, 0) == cudaSuccess && n > 0 ? n : 1;
         }();
         FMB_CUDA_CHECK(cudaGetDevice(&dev));
         FMB_CUDA_CHECK(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
         ctas = std::min<long long>((t.blocks + kWarps - 1) / kWarps, (long long)per_sm * sms);
     }
     FMB_REQUIRE(ctas < (1ll << 31), "fmb_adamw_step: too many values");
-    k_adamw<G, EIGHT, CAPACITY><<<(unsigned)ctas, kThreads, 0, stream>>>(t);
+    k_adamw<G, EIGHT, RANDOM, CAPACITY><<<(unsigned)ctas, kThreads, 0, stream>>>(t);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
 
 template <typename G, int CAPACITY>
 int launch(const Table<CAPACITY>& t, bool eight, cudaStream_t stream) {
-    return eight ? launch<G, true, CAPACITY>(t, stream) : launch<G, false, CAPACITY>(t, stream);
+    if (!eight) return launch<G, false, false, CAPACITY>(t, stream);
+    return t.random ? launch<G, true, true, CAPACITY>(t, stream) : launch<G, true, false, CAPACITY>(t, stream);
 }
 
 bool aligned(const void* p, int bytes) { return ((uintptr_t)p & (uintptr_t)(bytes - 1)) == 0; }
@@ -325,6 +366,7 @@ int step(const fmb_adamw_t* a, const fmb_adamw_tensor_t* tensors, int last, cuda
     const int grad_bytes = a->grad_type == FMB_TYPE_F32 ? 4 : 2;
     Table<CAPACITY> t;
     t.copy_type = a->copy_type;
+    t.random = (uint32_t)a->random;
     t.decay = (float)(1.0 - a->lr * a->weight_decay);
     t.lr = (float)a->lr;
     t.b1 = (float)a->beta1; t.c1 = (float)(1.0 - a->beta1);
@@ -369,6 +411,7 @@ extern "C" FMB_API int fmb_adamw_step(const fmb_adamw_t* a, const fmb_adamw_tens
     FMB_REQUIRE(a->m && a->v && a->state, "fmb_adamw_step: null moments or state");
     FMB_REQUIRE(aligned(a->m, 16) && aligned(a->v, 16), "fmb_adamw_step: moments start at a multiple of 16 bytes");
     FMB_REQUIRE(a->moment_bits == 32 || (a->m_scale && a->v_scale), "fmb_adamw_step: 8-bit moments need their scales");
+    FMB_REQUIRE(a->moment_bits == 8 || !a->random, "fmb_adamw_step: random rounding is of 8-bit moments");
     FMB_REQUIRE(a->beta1 >= 0.0 && a->beta1 < 1.0 && a->beta2 >= 0.0 && a->beta2 < 1.0, "fmb_adamw_step: betas in [0, 1)");
     const int grad_bytes = a->grad_type == FMB_TYPE_F32 ? 4 : 2;
     int last = -1;

@@ -8,6 +8,7 @@
 // new noise without host involvement.
 
 #include "fmb_common.cuh"
+#include "philox.cuh"
 
 #include <algorithm>
 
@@ -125,21 +126,6 @@ k_second_half(fmb_langevin_t lv) {
 // Counter-based normal deviates (Philox4x32-10 + Box-Muller in float64): one (seed, step, atom) triple always yields
 // the same six numbers, so every rank of a domain-decomposed run draws identical noise without communication and
 // without the host generator, whose draw of 6 N normals per step is the bottleneck beyond ~10^5 atoms.
-__device__ __forceinline__ void philox_round(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
-    const uint64_t p0 = (uint64_t)0xD2511F53u * c[0], p1 = (uint64_t)0xCD9E8D57u * c[2];
-    const uint32_t n0 = (uint32_t)(p1 >> 32) ^ c[1] ^ k0, n2 = (uint32_t)(p0 >> 32) ^ c[3] ^ k1;
-    c[0] = n0; c[1] = (uint32_t)p1; c[2] = n2; c[3] = (uint32_t)p0;
-}
-
-__device__ __forceinline__ void philox(uint32_t (&c)[4], uint32_t k0, uint32_t k1) {
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        philox_round(c, k0, k1);
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
-    }
-}
-
 __device__ __forceinline__ void box_muller(uint32_t a, uint32_t b, uint32_t c, uint32_t d, double& z0, double& z1) {
     const double u1 = ((double)(((uint64_t)(a >> 5) << 26) | (uint64_t)(b >> 6)) + 0.5) * (1.0 / 9007199254740992.0);
     const double u2 = ((double)(((uint64_t)(c >> 5) << 26) | (uint64_t)(d >> 6)) + 0.5) * (1.0 / 9007199254740992.0);

@@ -16,6 +16,15 @@ share a scale s per moment, the largest of them / 448: m is held as e4m3(m / s),
 where v is not. A gradient that is not finite makes the moments of its value (with 8 bits: of its 256 values) not finite, and
 with them the weights.
 
+Moments in 8 bits are rounded to the nearest or, with ``rounding="random"``, v at random (m always to the nearest). To the nearest each
+step is the best it can be, but v does not follow its moving average over many: what a step changes, 0.05 % of the root with beta2 =
+0.999, is less than half of the 6 to 12 % between two codes, so a value keeps its ratio to the largest of its 256. Where the sizes of
+gradients change while weights are trained, that is off by factors: at 3,000 steps after all sizes were drawn anew, from lognormals
+of e^0.5, the roots of 90 % of the values were 0.3 to 1.8 of the true ones and updates twice as large; of values whose gradients fell to
+a tenth many stayed 9 times too large. At random the expected v is the one of 32 bits at every step, and roots are 0.71 to 1.32 of the true
+ones (90 %) in both cases. So: ``rounding="random"`` for runs of more than a few hundred steps. The random bits are those of ``seed``, the
+number of the step and the place of the value: runs repeat bit by bit, also captured or continued from loaded moments.
+
 The list of tensors and where they lie are those of the construction. Steps of one optimiser follow one another: not two at once on
 two streams. A step runs on the current stream of the weights' device, allocates nothing and can be captured: the number of the step is
 counted on the device, the learning rate and the other constants are those at capture. There is no CPU path.
@@ -44,19 +53,24 @@ def _share_memory(tensors) -> bool:
 
 class AdamW:
     def __init__(self, params, lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
-                 state_bits: int = 32, copies=None):
+                 state_bits: int = 32, copies=None, rounding: str = "nearest", seed: int = 0):
         self.names = list(params) if isinstance(params, dict) else list(range(len(params)))
         self.params = [params[k] for k in self.names]
         if not self.params:
             raise ValueError("AdamW: no tensors")
         if state_bits not in (8, 32):
             raise ValueError("AdamW: state_bits is 8 or 32")
+        if rounding not in ("nearest", "random") or (rounding == "random" and state_bits != 8):
+            raise ValueError("AdamW: rounding is 'nearest' or, with state_bits=8, 'random'")
+        if not 0 <= int(seed) < 2 ** 31 - 1:
+            raise ValueError("AdamW: seed is a number from 0 to 2^31 - 2")
         if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
             raise ValueError("AdamW: betas in [0, 1)")
         if not all(0.0 <= x < math.inf for x in (lr, eps, weight_decay)):
             raise ValueError("AdamW: lr, eps and weight_decay must be finite and not negative")
         self.lr, self.betas, self.eps, self.weight_decay = float(lr), tuple(float(b) for b in betas), float(eps), float(weight_decay)
         self.state_bits = int(state_bits)
+        self.rounding, self.seed = rounding, int(seed)
         self.device = self.params[0].device
         for p in self.params:
             if not p.is_cuda:
@@ -115,6 +129,7 @@ class AdamW:
     def _fill_args(self) -> None:
         a = self._args
         a.moment_bits, a.copy_type = self.state_bits, self._copy_type
+        a.random = 1 + self.seed if self.rounding == "random" else 0
         a.lr, a.beta1, a.beta2, a.eps, a.weight_decay = self.lr, *self.betas, self.eps, self.weight_decay
         a.m, a.v, a.state = self.m.data_ptr(), self.v.data_ptr(), self._state.data_ptr()
         if self.state_bits == 8:

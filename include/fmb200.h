@@ -474,7 +474,8 @@ typedef struct {
     int32_t moment_bits;              /* 32: m and v are fp32; 8: m and r are e4m3 in units of m_scale / r_scale per block */
     int32_t grad_type;                /* FMB_TYPE_* of every g */
     int32_t copy_type;                /* FMB_TYPE_BF16 or FMB_TYPE_F16 of every copy */
-    int32_t reserved;
+    int32_t random;                   /* 8 bits: 0 = moments are rounded to the nearest; else r is rounded up or down at random, with the
+                                       * chances that make the expected r^2 the exact one, by bits that this number keys */
     double lr, beta1, beta2, eps, weight_decay;
     void* m;                          /* first moments */
     void* v;                          /* second moments; with 8 bits their square roots r */

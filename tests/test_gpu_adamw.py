@@ -299,3 +299,131 @@ def test_moments_that_share_memory_are_refused(bits):
     optimiser.load_moments(1, *fine.values())
     optimiser.step([torch.ones(512, device="cuda")])
     assert optimiser.steps == 2
+
+
+@pytest.mark.parametrize("course", ["steady", "sizes drawn anew", "half fall to a tenth"])
+def test_second_moments_in_8_bits_follow_those_in_32(course):
+    """Thousands of steps of random gradients, whose sizes change on the way. At random rounding the expected v is that of 32 bits. A
+    root changes by no more than 1/2,000 of itself a step downwards (and as much upwards on average); a change of c between codes d apart, d at most
+    1/8 of the value, adds a variance of d c at most, which fades by 1/1,000 a step: 1/8 x 1/2,000 x 1,000 = 1/16, a spread of a quarter
+    at most, and nine values in ten within 1.65 of that. The sum of v over 262,144 values whose sizes are lognormals of e^0.5 then spreads by
+    0.2 %. First moments are rounded to the nearest: they are compared with nothing here."""
+    from fastmace_b200.optimiser import AdamW
+    n = 262_144
+    g = torch.Generator(device="cuda").manual_seed(7)
+    sizes = [torch.exp(0.5 * torch.randn(n, generator=g, device="cuda"))]
+    if course == "steady":
+        sizes.append(sizes[0])
+    elif course == "sizes drawn anew":
+        sizes.append(torch.exp(0.5 * torch.randn(n, generator=g, device="cuda")))
+    else:
+        sizes.append(sizes[0] * torch.where(torch.rand(n, generator=g, device="cuda") < 0.5, 0.1, 1.0))
+    weights = [torch.zeros(n, device="cuda") for _ in range(2)]
+    optimisers = [AdamW([weights[0]], state_bits=8, rounding="random", seed=3), AdamW([weights[1]])]
+    for step in range(5000):
+        grad = torch.randn(n, generator=g, device="cuda") * sizes[step >= 1000]
+        for optimiser in optimisers:
+            optimiser.step([grad])
+        if step in (100, 999, 4999):
+            held, true = (optimiser.moments(0)[1].double() for optimiser in optimisers)
+            low, high = torch.quantile((held / true).sqrt(), torch.tensor([0.05, 0.95], dtype=torch.float64, device="cuda")).tolist()
+            assert 1 - 1.65 / 4 < low and high < 1 + 1.65 / 4, (step, low, high)
+            assert abs(float(held.sum() / true.sum()) - 1) < 0.01, step
+
+
+@pytest.mark.parametrize("grad", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{s[0]}")
+def test_one_step_rounded_at_random(sizes, grad):
+    """Weights, first moments and scales are those of rounding to the nearest, bit by bit; a root is one of the two numbers of the type
+    that its exact value lies between; v is exact on average over the seeds."""
+    from fastmace_b200.optimiser import BLOCK, AdamW
+    hyper = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.02, state_bits=8)
+    params, grads, copies = _case(sizes, grad, 1)
+    start, first = [p.clone() for p in params], _case(sizes, grad, 5)[1]
+
+    def run(**more):
+        for p, s in zip(params, start):
+            p.copy_(s)
+        optimiser = AdamW(params, copies=copies, **hyper)
+        optimiser.step(first)
+        held = [t.clone() for t in (optimiser.m, optimiser.m_scale, optimiser.v, optimiser.v_scale)]
+        optimiser = AdamW(params, copies=copies, **hyper, **more)
+        optimiser.load_moments(1, *held)
+        before = [optimiser.moments(k)[1].double() for k in range(len(params))]
+        optimiser.step(grads)
+        return optimiser, before, [p.clone() for p in params], [c.clone() for c in copies]
+
+    nearest, before, weights, bf16 = run()
+    total, seeds = 0.0, 24
+    exact = torch.cat([0.99 * v + 0.01 * g.double().view(-1) ** 2 for v, g in zip(before, grads)])
+    for seed in range(seeds):
+        other, _, w, c = run(rounding="random", seed=seed)
+        assert all(torch.equal(a, b) for a, b in zip(weights + bf16, w + c))
+        assert torch.equal(nearest.m.view(torch.uint8), other.m.view(torch.uint8))
+        assert torch.equal(nearest.m_scale, other.m_scale) and torch.equal(nearest.v_scale, other.v_scale)
+        codes = torch.cat([other.v[b * BLOCK:b * BLOCK + p.numel()] for b, p in zip(other.blocks, params)]).double()
+        scale = torch.cat([other.v_scale[b:b - (-p.numel() // BLOCK)].repeat_interleave(BLOCK)[:p.numel()]
+                           for b, p in zip(other.blocks, params)]).double()
+        unit = exact.sqrt() / scale
+        gap = torch.exp2(torch.floor(torch.log2(torch.maximum(unit, codes).clamp(min=2.0 ** -6))) - 3)
+        tiny = (unit < 2.0 ** -9) & (unit > 0)                      # held as the smallest number
+        # (2^-21: the roots are fp32, and so are their quotients)
+        assert bool(((codes - unit).abs() < gap + 2.0 ** -21 * unit)[~tiny].all()) and bool((codes[tiny] == 2.0 ** -9).all())
+        total = total + torch.where(tiny, unit, codes) ** 2
+    # independent errors of v in units of its scale: each spreads by half of what the squares of its two codes are apart, 2 unit gap, at most
+    off, spread = (total / seeds - unit ** 2).sum(), float(((unit + gap) * gap).norm()) / seeds ** 0.5
+    assert abs(float(off)) <= 6 * spread + 2.0 ** -20 * float((unit ** 2).sum())
+
+
+def test_random_rounding_repeats_itself():
+    """By seed, step and place: again, captured, continued, and whatever else is in the list behind."""
+    from fastmace_b200.optimiser import AdamW
+    g = torch.Generator(device="cuda").manual_seed(4)
+    start = [torch.randn(n, generator=g, device="cuda") for n in (5000, 77, 300)]
+    grads = [[torch.randn(n, generator=g, device="cuda") for n in (5000, 77, 300)] for _ in range(6)]
+
+    def run(seed, mode="plain", count=3):
+        params = [p.clone() for p in start[:count]]
+        optimiser = AdamW(params, state_bits=8, rounding="random", seed=seed)
+        if mode == "captured":
+            held = [x.clone() for x in grads[0]]
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                optimiser.step(held)
+        for k, step in enumerate(grads):
+            if mode == "captured":
+                for h, x in zip(held, step):
+                    h.copy_(x)
+                graph.replay()
+                continue
+            if mode == "continued" and k == 3:
+                held = [t.clone() for t in (optimiser.m, optimiser.m_scale, optimiser.v, optimiser.v_scale)]
+                optimiser = AdamW(params, state_bits=8, rounding="random", seed=seed)
+                optimiser.load_moments(3, *held)
+            optimiser.step(step[:count])
+        return params, optimiser.v.view(torch.uint8).clone()
+
+    params, codes = run(5)
+    for mode in ("plain", "captured", "continued"):
+        p, c = run(5, mode)
+        assert torch.equal(c, codes) and all(torch.equal(a, b) for a, b in zip(p, params)), mode
+    p, c = run(5, count=1)
+    assert torch.equal(c, codes[:len(c)]) and torch.equal(p[0], params[0])
+    assert not torch.equal(run(6)[1], codes)
+
+
+def test_random_rounding_of_values_that_are_not_finite_or_zero():
+    from fastmace_b200.optimiser import AdamW
+    weight = torch.ones(1024, device="cuda")
+    optimiser = AdamW([weight], lr=0.1, weight_decay=0.0, state_bits=8, rounding="random")
+    optimiser.step([torch.zeros(1024, device="cuda")])
+    assert bool((weight == 1).all()) and bool((optimiser.v.float() == 0).all())
+    bad = torch.ones(1024, device="cuda")
+    bad[300], bad[800] = float("nan"), float("inf")
+    for _ in range(2):
+        optimiser.step([bad])
+        bad = torch.ones(1024, device="cuda")
+    fine = torch.ones(1024, dtype=torch.bool, device="cuda")
+    fine[256:512], fine[768:] = False, False
+    assert bool(torch.isfinite(weight[fine]).all()) and not bool(torch.isfinite(weight[[300, 800]]).any())
+    assert bool(torch.isnan(optimiser.moments(0)[1][~fine]).all()) and bool(torch.isfinite(optimiser.moments(0)[1][fine]).all())

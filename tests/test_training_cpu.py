@@ -98,3 +98,19 @@ def test_constants_that_are_no_numbers_are_refused(change):
     from fastmace_b200.optimiser import AdamW
     with pytest.raises(ValueError, match="finite|betas"):
         AdamW([torch.zeros(4)], **change)
+
+
+def test_random_rounding_is_of_8_bit_moments():
+    from fastmace_b200.optimiser import AdamW
+    for change in (dict(rounding="random"), dict(rounding="down", state_bits=8), dict(rounding="random", state_bits=8, seed=-1),
+                   dict(rounding="random", state_bits=8, seed=2 ** 31 - 1)):
+        with pytest.raises(ValueError, match="rounding|seed"):
+            AdamW([torch.zeros(4)], **change)
+    mod, lib = _lib()
+    a = mod.AdamwStruct()
+    a.moment_bits, a.copy_type, a.beta1, a.beta2, a.random = 32, 1, 0.9, 0.999, 1
+    a.m = a.v = a.state = 4096
+    t = (mod.AdamwTensorStruct * 1)()
+    assert lib.fmb_adamw_step(ctypes.byref(a), t, 1, None) == 1 and b"random" in lib.fmb_last_error()
+    a.random = 0
+    assert lib.fmb_adamw_step(ctypes.byref(a), t, 1, None) == 0
