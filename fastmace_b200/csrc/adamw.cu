@@ -35,7 +35,7 @@ namespace {
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kBlock = FMB_ADAMW_BLOCK;
 constexpr int kCtaBlocks = 16;
-constexpr int kMaxTensors = 400, kFewTensors = 64;        // of a launch: the list is 48 bytes a tensor of kernel arguments
+constexpr int kMaxTensors = 400, kFewTensors = 64;        // of a launch: the list is 56 bytes a tensor of kernel arguments
 
 struct Entry {
     float* p;
@@ -62,6 +62,8 @@ struct Table {
     float* v_scale;
     double* state;
 };
+
+static_assert(sizeof(Entry) == 56 && sizeof(Table<kMaxTensors>) <= 32764, "fits what a kernel takes as arguments");
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }

@@ -454,8 +454,8 @@ FMB_API int fmb_grouped_input_gradient(const fmb_grouped_t* args, fmb_stream_t s
  * for groups without rows */
 FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* args, fmb_stream_t stream);
 /* floats of scratch that a call with these arguments needs (all fields but scratch as in the call); which: 0 linear,
- * 1 input gradient, 2 weight gradient. Operands of 16 bits whose rows do not start at multiples of 16 bytes are copied there, and
- * the sums of parts of a group's rows held. */
+ * 1 input gradient, 2 weight gradient. Operands whose rows or matrices do not start at multiples of 16 bytes are copied there, the
+ * rows of a 16-bit weight gradient laid by groups, and the sums of parts of a group's rows held. */
 FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* args, int which);
 
 #define FMB_ADAMW_BLOCK 256           /* values that share a scale where moments are held in 8 bits */
