@@ -205,3 +205,57 @@ def test_captured_with_the_force_call():
             assert torch.equal(seen[k], v), k
     grouped.check_status()
     ff.check_status()
+
+
+def _close(got, ref):
+    """The same fp32 terms from other kernels, summed in another order: 1e-5 of the norm, as for the forces of those paths."""
+    assert list(got) == list(ref)
+    for k in ref:
+        assert float((got[k].double() - ref[k].double()).norm()) <= 1e-5 * float(ref[k].double().norm()), k
+
+
+@pytest.mark.parametrize("name", ["small", "medium", "large"])
+@pytest.mark.parametrize("chunk,edge_adjoint,mirror", [(37, None, True), (1000, None, True), (37, False, True), (1000, False, True),
+                                                       (1000, False, False), (None, None, False)])
+def test_other_paths_leave_the_same_gradients(name, chunk, edge_adjoint, mirror):
+    """Lists in chunks, sender gradients of one chunk at a time, every edge from both ends; atoms without neighbours among them."""
+    from fastmace_b200.forcefield import B200ForceField
+    from fastmace_b200.model import SPECS, init_weights
+    spec = SPECS[name]
+    weights = init_weights(spec, 4)
+    rng = np.random.default_rng(5)
+    edge = (150 * 50.0) ** (1 / 3)
+    cell, positions = np.diag([edge, edge, edge + 30.0]), rng.uniform(0, edge, (150, 3))
+    positions[[0, 70, 149], :] = [[1, 1, edge + 15.0], [1, 9, edge + 15.0], [9, 1, edge + 15.0]]
+    numbers, x = rng.choice([11, 17], 150), torch.tensor(positions, device="cuda")
+    whole = B200ForceField(spec, weights, numbers, cell, positions=x)
+    whole(x)
+    ff = B200ForceField(spec, weights, numbers, cell, positions=x, chunk_edges=chunk, edge_adjoint=edge_adjoint)
+    if not mirror:
+        ff.work.mirror, ff.work.edge_q, ff.work.edge_dx = None, None, None
+    for _ in range(2):
+        ff(x)
+        ff.check_status()
+        _close(ff.weight_gradients(), whole.weight_gradients())
+
+
+@pytest.mark.parametrize("mode", ["checked", "graph"])
+@pytest.mark.parametrize("repeat", [(2, 2, 2), (4, 4, 3)])
+def test_gradients_after_the_steps_of_an_engine(mode, repeat):
+    """The last force call is that of the last step, captured or not; 384 atoms take the kernels with the radial layer on the SM."""
+    from fastmace_b200.engine import B200Engine
+    from fastmace_b200.forcefield import B200ForceField
+    from fastmace_b200.langevin import IntegratorConfig, Langevin
+    from fastmace_b200.model import MEDIUM, init_weights
+    from fastmace_b200.state import SimulationState
+    from fastmace_b200.structures import nacl
+    s = nacl(repeat, 0.05, 1)
+    weights = init_weights(MEDIUM, 1)
+    ff = B200ForceField(MEDIUM, weights, s.numbers, s.cell)
+    state = SimulationState.from_structure(s.with_velocities(300.0, 2), "cuda", seed=3)
+    engine = B200Engine(ff, Langevin(state, IntegratorConfig(), temperature_K=300.0), state, mode=mode)
+    for steps in (1, 7):
+        engine.run(steps)
+        fresh = B200ForceField(MEDIUM, weights, s.numbers, s.cell, positions=state.positions)
+        fresh(state.positions)
+        _close(ff.weight_gradients(), fresh.weight_gradients())
