@@ -34,6 +34,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import numpy as np
 import torch
@@ -42,7 +43,7 @@ from . import _lib
 from .grouped import TYPES, _launch
 
 BLOCK = _lib.ADAMW_BLOCK
-_place = torch.Tensor.data_ptr
+_place, _type = torch.Tensor.data_ptr, operator.attrgetter("dtype")
 
 
 def _share_memory(tensors) -> bool:
@@ -149,24 +150,24 @@ class AdamW:
         if list(map(_place, self._listed)) != self._places:
             raise ValueError("AdamW.step: a tensor of the list has been given other memory since")
         shapes, written = self._shapes, self._all_written
-        if any(g is None for g in grads):
-            written = sum((w for w, g in zip(self._written, grads) if g is not None), [])
+        try:
+            self._pointers[:] = list(map(_place, grads))
+        except TypeError:                                # a gradient is None
             self._pointers[:] = [0 if g is None else g.data_ptr() for g in grads]
+            written = sum((w for w, g in zip(self._written, grads) if g is not None), [])
             shapes = [s for s, g in zip(shapes, grads) if g is not None]
             grads = [g for g in grads if g is not None]
             if not grads:
                 return
-        else:
-            self._pointers[:] = list(map(_place, grads))
-        kind = grads[0].dtype
-        if kind not in TYPES or [g.dtype for g in grads].count(kind) != len(grads):
+        kinds = set(map(_type, grads))
+        if len(kinds) != 1 or not kinds <= set(TYPES):
             raise ValueError("AdamW.step: the gradients must have one type, float32, bfloat16 or float16")
         if [g.shape for g in grads] != shapes or not all(map(torch.Tensor.is_contiguous, grads)) or \
                 set(map(torch.Tensor.get_device, grads)) != {self._index}:
             raise ValueError("AdamW.step: a gradient must be contiguous, of its weights' shape and on their device")
         self._captured = self._captured or torch.cuda.is_current_stream_capturing()
         self._fill_args()
-        self._args.grad_type = TYPES[kind]
+        self._args.grad_type = TYPES[kinds.pop()]
         _lib.check(_launch(self._index, self.lib.fmb_adamw_step, ctypes.byref(self._args), self._tensors, len(self.params)),
                    "fmb_adamw_step")
         # weights and copies have changed in place: a graph that saved one, to go on to its activations, must not run with the new values
