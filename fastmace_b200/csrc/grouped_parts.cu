@@ -76,7 +76,7 @@ __device__ __forceinline__ void finite_rest(const float (&main)[16], float (&res
     float top = 0.0f;
 #pragma unroll
     for (int j = 0; j < 16; j += 2) top = fmaxf(fmaxf(fabsf(main[j]), fabsf(main[j + 1])), top);
-    if (infinite(top)) {
+    if (__any_sync(0xffffffffu, infinite(top))) {        // (by the whole warp: what follows is too)
 #pragma unroll
         for (int j = 0; j < 16; ++j) rest[j] = infinite(main[j]) ? 0.0f : rest[j];
     }
