@@ -2,7 +2,7 @@
 moments in 32 or in 8 bits.
 
     weights = {name: w.cuda() for name, w in init_weights(spec, seed).items()}
-    optimiser = AdamW(weights, lr=1e-3, state_bits=8)
+    optimiser = AdamW(weights, lr=1e-3, state_bits=8, rounding="random")
     optimiser.step(gradients)                       # {name: gradient}; tensors without one stay as they are
 
 With t the number of the step:
@@ -25,9 +25,10 @@ a tenth many stayed 9 times too large. At random the expected v is the one of 32
 ones (90 %) in both cases. So: ``rounding="random"`` for runs of more than a few hundred steps. The random bits are those of ``seed``, the
 number of the step and the place of the value: runs repeat bit by bit, also captured or continued from loaded moments.
 
-The list of tensors and where they lie are those of the construction. Steps of one optimiser follow one another: not two at once on
-two streams. A step runs on the current stream of the weights' device, allocates nothing and can be captured: the number of the step is
-counted on the device, the learning rate and the other constants are those at capture. There is no CPU path.
+The list of tensors and where they lie are those of the construction; gradients share no memory with weights, copies or moments.
+Steps of one optimiser follow one another: not two at once on two streams. A step runs on the current stream of the weights' device,
+allocates nothing and can be captured: the number of the step is counted on the device, the learning rate and the other constants are
+those at capture. There is no CPU path.
 """
 
 from __future__ import annotations
