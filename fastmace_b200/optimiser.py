@@ -108,6 +108,7 @@ class AdamW:
         for p in self.params:
             self.blocks.append(blocks)
             blocks += -(-p.numel() // BLOCK)
+        blocks = max(1, blocks)                          # (a list of empty tensors has somewhere to point to as well)
         held = torch.float32 if self.state_bits == 32 else torch.float8_e4m3fn
         with torch.cuda.device(self.device):
             # first moments, and second moments (their square roots in 8 bits), each tensor from the start of a block
@@ -139,7 +140,7 @@ class AdamW:
 
     def step(self, grads) -> None:
         """One step along ``grads`` (a dictionary or sequence like the weights; a missing or ``None`` gradient leaves its
-        tensor and its moments as they are). Counts as a step if any tensor has a gradient."""
+        tensor and its moments as they are). Counts as a step if any tensor that has values has a gradient."""
         if isinstance(grads, dict):
             unknown = set(grads) - set(self.names)
             if unknown:

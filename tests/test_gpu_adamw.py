@@ -427,3 +427,17 @@ def test_random_rounding_of_values_that_are_not_finite_or_zero():
     fine[256:512], fine[768:] = False, False
     assert bool(torch.isfinite(weight[fine]).all()) and not bool(torch.isfinite(weight[[300, 800]]).any())
     assert bool(torch.isnan(optimiser.moments(0)[1][~fine]).all()) and bool(torch.isfinite(optimiser.moments(0)[1][fine]).all())
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_lists_of_empty_tensors(bits):
+    from fastmace_b200.optimiser import AdamW
+    empty, weight = torch.zeros(0, 7, device="cuda"), torch.ones(3, device="cuda")
+    optimiser = AdamW([empty, torch.zeros(0, device="cuda")], state_bits=bits)
+    optimiser.step([torch.zeros(0, 7, device="cuda"), None])
+    assert optimiser.steps == 0 and optimiser.moments(0)[0].shape == (0, 7)
+    optimiser = AdamW([empty, weight], state_bits=bits)
+    optimiser.step([torch.zeros(0, 7, device="cuda"), None])
+    assert optimiser.steps == 0 and bool((weight == 1).all())
+    optimiser.step([torch.zeros(0, 7, device="cuda"), torch.ones(3, device="cuda")])
+    assert optimiser.steps == 1 and bool((weight < 1).all())
