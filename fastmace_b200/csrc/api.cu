@@ -61,6 +61,7 @@ extern "C" FMB_API int fmb_sizeof(int which) {
         case 4: return (int)sizeof(fmb_grouped_t);
         case 5: return (int)sizeof(fmb_adamw_tensor_t);
         case 6: return (int)sizeof(fmb_adamw_t);
+        case 7: return (int)sizeof(fmb_embedding_t);
         default: return -1;
     }
 }

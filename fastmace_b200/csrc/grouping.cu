@@ -13,6 +13,8 @@
 
 #include "fmb_common.cuh"
 
+#include <algorithm>
+
 namespace fmb {
 
 namespace {
@@ -22,19 +24,36 @@ constexpr int kKeys = 8;                                  // per lane
 constexpr int kRowsPerWarp = 32 * kKeys;
 constexpr int kRowsPerCta = kWarps * kRowsPerWarp;
 
-// the groups of this lane's rows begin + 32 i + lane: `groups` stands for "no group", -1 for rows past the end
+// A pass over some bits of keys that are too many for one table (sort_tokens): the row in place i is from[i], or i; a key that
+// is no token counts as `vocabulary`, behind all others; the groups are the values of its bits from `shift` on.
+struct Digit {
+    const int32_t* from;
+    int32_t* sorted_keys;                                 // of the last pass: the keys in their order
+    int vocabulary, shift, mask;
+};
+
+// as kept: `groups` stands for "no group"
 template <typename K>
-__device__ __forceinline__ void load_keys(const K* __restrict__ keys, long long begin, long long rows, int groups, int (&g)[kKeys]) {
+__device__ __forceinline__ int group_of(K key, int groups) { return key < 0 || key >= (K)groups ? groups : (int)key; }
+
+// the groups of this lane's rows begin + 32 i + lane, -1 for rows past the end
+template <typename K, bool DIGIT>
+__device__ __forceinline__ void load_keys(const K* __restrict__ keys, const Digit& d, long long begin, long long rows, int groups, int (&g)[kKeys]) {
     const int lane = threadIdx.x & 31;
     K key[kKeys];
+    int at[kKeys];
+    if (DIGIT && d.from) {
+#pragma unroll
+        for (int i = 0; i < kKeys; ++i) at[i] = begin + 32 * i + lane < rows ? d.from[begin + 32 * i + lane] : 0;
+    }
 #pragma unroll
     for (int i = 0; i < kKeys; ++i) {
         const long long row = begin + 32 * i + lane;
-        key[i] = row < rows ? keys[row] : (K)-1;
+        key[i] = row < rows ? keys[DIGIT && d.from ? at[i] : row] : (K)-1;
     }
 #pragma unroll
     for (int i = 0; i < kKeys; ++i)
-        g[i] = begin + 32 * i + lane >= rows ? -1 : key[i] < 0 || key[i] >= (K)groups ? groups : (int)key[i];
+        g[i] = begin + 32 * i + lane >= rows ? -1 : DIGIT ? group_of(key[i], d.vocabulary) >> d.shift & d.mask : group_of(key[i], groups);
 }
 
 // Lanes whose rows have this lane's group, for each of its rows, by a vote per bit of the group's number: 3 instructions a bit,
@@ -68,13 +87,13 @@ __device__ __forceinline__ int warps_before(int mine, int& all) {
     return inclusive - mine;
 }
 
-template <typename K>
+template <typename K, bool DIGIT>
 __global__ void __launch_bounds__(kThreads)
-k_group_count(const K* __restrict__ keys, long long rows, int groups, int32_t* __restrict__ table) {
+k_group_count(const K* __restrict__ keys, Digit d, long long rows, int groups, int32_t* __restrict__ table) {
     __shared__ int counts[FMB_MAX_GROUPS + 1];
     const int width = groups + 1;
     int g[kKeys];
-    load_keys(keys, (long long)blockIdx.x * kRowsPerCta + (threadIdx.x >> 5) * kRowsPerWarp, rows, groups, g);
+    load_keys<K, DIGIT>(keys, d, (long long)blockIdx.x * kRowsPerCta + (threadIdx.x >> 5) * kRowsPerWarp, rows, groups, g);
     for (int q = threadIdx.x; q < width; q += kThreads) counts[q] = 0;
     __syncthreads();
 #pragma unroll
@@ -136,9 +155,9 @@ __device__ __forceinline__ void exclusive_starts(int* starts, int width) {
 
 // ALONE: the only CTA, which takes its own counts for the totals. The CTA's rows are put in order in shared memory first, so
 // that the rows of a group leave in one run.
-template <typename K, bool ALONE>
+template <typename K, bool ALONE, bool DIGIT>
 __global__ void __launch_bounds__(kThreads, ALONE ? 1 : 2)
-k_group_place(const K* __restrict__ keys, long long rows, int groups, int bits, const int32_t* __restrict__ table,
+k_group_place(const K* __restrict__ keys, Digit d, long long rows, int groups, int bits, const int32_t* __restrict__ table,
               const int32_t* __restrict__ totals, int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
     extern __shared__ int counts[];                       // [kWarps][groups + 1], [groups + 1] starts of the CTA, [groups + 1] of all, rows
     const int width = groups + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -147,7 +166,7 @@ k_group_place(const K* __restrict__ keys, long long rows, int groups, int bits, 
     int* const sorted = here + 2 * width;                 // row of the CTA | group << 13
     const long long first = (long long)blockIdx.x * kRowsPerCta;
     int g[kKeys], rank[kKeys];
-    load_keys(keys, first + warp * kRowsPerWarp, rows, groups, g);
+    load_keys<K, DIGIT>(keys, d, first + warp * kRowsPerWarp, rows, groups, g);
     const int warps = ALONE ? (int)((rows + kRowsPerWarp - 1) / kRowsPerWarp) : kWarps;        // that have rows
     for (int i = threadIdx.x; i < warps * width; i += kThreads) counts[i] = 0;
     if (!ALONE)
@@ -174,7 +193,7 @@ k_group_place(const K* __restrict__ keys, long long rows, int groups, int bits, 
     __syncthreads();
     exclusive_starts(here, width);
     if (!ALONE) exclusive_starts(starts, width);
-    if (blockIdx.x == 0)
+    if (!DIGIT && blockIdx.x == 0)
         for (int q = threadIdx.x; q < width; q += kThreads) offsets[q] = starts[q];
 #pragma unroll
     for (int i = 0; i < kKeys; ++i)
@@ -189,31 +208,51 @@ k_group_place(const K* __restrict__ keys, long long rows, int groups, int bits, 
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
         const int i = threadIdx.x + j * kThreads, v = i < count ? sorted[i] : 0;
-        if (i < count) order[(ALONE ? 0 : starts[v >> 13]) + i] = (int32_t)(first + (v & (kRowsPerCta - 1)));
+        if (i >= count) continue;
+        const int to = (ALONE ? 0 : starts[v >> 13]) + i;
+        int32_t row = (int32_t)(first + (v & (kRowsPerCta - 1)));
+        if (DIGIT && d.from) row = d.from[row];
+        order[to] = row;
+        if (DIGIT && d.sorted_keys) d.sorted_keys[to] = group_of(keys[row], d.vocabulary);
     }
 }
 
 constexpr int place_smem(int width) { return ((kWarps + 2) * width + kRowsPerCta) * 4; }
 
-template <typename K>
-int group_rows(const K* keys, long long rows, int groups, int32_t* order, int32_t* offsets, int32_t* scratch, cudaStream_t stream) {
+// one stable pass: counts, their sums over the CTAs, places; a launch alone where one CTA takes all rows
+template <typename K, bool DIGIT>
+int sort_pass(const K* keys, const Digit& d, long long rows, int groups, int32_t* order, int32_t* offsets, int32_t* scratch, cudaStream_t stream) {
     const int width = groups + 1, ctas = ceil_div(rows, kRowsPerCta);
     const int smem = place_smem(width), bits = 32 - __builtin_clz(groups);
-    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, true>, place_smem(FMB_MAX_GROUPS + 1)));
-    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, false>, place_smem(FMB_MAX_GROUPS + 1)));
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, true, DIGIT>, place_smem(FMB_MAX_GROUPS + 1)));
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, false, DIGIT>, place_smem(FMB_MAX_GROUPS + 1)));
     if (ctas <= 1) {
-        k_group_place<K, true><<<1, kThreads, smem, stream>>>(keys, rows, groups, bits, nullptr, nullptr, order, offsets);
+        k_group_place<K, true, DIGIT><<<1, kThreads, smem, stream>>>(keys, d, rows, groups, bits, nullptr, nullptr, order, offsets);
         FMB_LAUNCH_CHECK();
         return FMB_OK;
     }
     int32_t* const totals = scratch + (long long)ctas * width;
-    k_group_count<K><<<ctas, kThreads, 0, stream>>>(keys, rows, groups, scratch);
+    k_group_count<K, DIGIT><<<ctas, kThreads, 0, stream>>>(keys, d, rows, groups, scratch);
     FMB_LAUNCH_CHECK();
     k_group_scan<<<ceil_div(width, 32), 1024, 0, stream>>>(scratch, totals, ctas, width);
     FMB_LAUNCH_CHECK();
-    k_group_place<K, false><<<ctas, kThreads, smem, stream>>>(keys, rows, groups, bits, scratch, totals, order, offsets);
+    k_group_place<K, false, DIGIT><<<ctas, kThreads, smem, stream>>>(keys, d, rows, groups, bits, scratch, totals, order, offsets);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
+}
+
+// Tokens by value: one pass where the table holds every value, else one over the lower half of their bits and one over the upper half,
+// which keeps the order that the first has made.
+int lower_bits(int vocabulary) { return vocabulary <= FMB_MAX_GROUPS ? 0 : (33 - __builtin_clz(vocabulary)) / 2; }
+long long table_size(long long rows, int width) { return rows <= kRowsPerCta ? 0 : ((rows + kRowsPerCta - 1) / kRowsPerCta + 1) * width; }
+
+template <typename K>
+int sort_tokens(const K* tokens, long long rows, int vocabulary, int32_t* order, int32_t* keys, int32_t* scratch, cudaStream_t stream) {
+    const int low = lower_bits(vocabulary);
+    if (low == 0) return sort_pass<K, true>(tokens, Digit{nullptr, keys, vocabulary, 0, -1}, rows, vocabulary, order, nullptr, scratch, stream);
+    int32_t* const table = scratch + rows;
+    const int rc = sort_pass<K, true>(tokens, Digit{nullptr, nullptr, vocabulary, 0, (1 << low) - 1}, rows, (1 << low) - 1, scratch, nullptr, table, stream);
+    return rc ? rc : sort_pass<K, true>(tokens, Digit{scratch, keys, vocabulary, low, -1}, rows, vocabulary >> low, order, nullptr, table, stream);
 }
 
 }  // namespace
@@ -235,6 +274,25 @@ extern "C" FMB_API int fmb_group_rows(const void* keys, int key_bytes, long long
     FMB_REQUIRE(scratch || fmb_group_rows_scratch(rows, groups) == 0, "fmb_group_rows: null scratch");
     FMB_REQUIRE(key_bytes == 4 || key_bytes == 8, "fmb_group_rows: keys of 4 or 8 bytes");
     if (key_bytes == 4)
-        return group_rows((const int32_t*)keys, rows, groups, order, offsets, scratch, (cudaStream_t)stream);
-    return group_rows((const long long*)keys, rows, groups, order, offsets, scratch, (cudaStream_t)stream);
+        return sort_pass<int32_t, false>((const int32_t*)keys, Digit{}, rows, groups, order, offsets, scratch, (cudaStream_t)stream);
+    return sort_pass<long long, false>((const long long*)keys, Digit{}, rows, groups, order, offsets, scratch, (cudaStream_t)stream);
+}
+
+extern "C" FMB_API long long fmb_sort_tokens_scratch(long long rows, int vocabulary) {
+    if (rows < 1 || vocabulary < 1 || vocabulary > FMB_MAX_VOCABULARY) return 0;
+    const int low = lower_bits(vocabulary);
+    if (low == 0) return table_size(rows, vocabulary + 1);
+    return rows + table_size(rows, std::max(1 << low, (vocabulary >> low) + 1));
+}
+
+extern "C" FMB_API int fmb_sort_tokens(const void* tokens, int token_bytes, long long rows, int vocabulary, int32_t* order,
+                                       int32_t* keys, int32_t* scratch, fmb_stream_t stream) {
+    FMB_REQUIRE(vocabulary >= 1 && vocabulary <= FMB_MAX_VOCABULARY, "fmb_sort_tokens: 1 to FMB_MAX_VOCABULARY tokens");
+    FMB_REQUIRE(rows >= 0 && rows < (1ll << 31) - kRowsPerCta, "fmb_sort_tokens: too many rows");
+    FMB_REQUIRE(token_bytes == 4 || token_bytes == 8, "fmb_sort_tokens: tokens of 4 or 8 bytes");
+    if (rows == 0) return FMB_OK;
+    FMB_REQUIRE(tokens && order && keys, "fmb_sort_tokens: null argument");
+    FMB_REQUIRE(scratch || fmb_sort_tokens_scratch(rows, vocabulary) == 0, "fmb_sort_tokens: null scratch");
+    if (token_bytes == 4) return sort_tokens((const int32_t*)tokens, rows, vocabulary, order, keys, scratch, (cudaStream_t)stream);
+    return sort_tokens((const long long*)tokens, rows, vocabulary, order, keys, scratch, (cudaStream_t)stream);
 }

@@ -490,6 +490,45 @@ typedef struct {
  * The number of the step t is read from `state` and advanced on the device, so a captured step can be replayed. */
 FMB_API int fmb_adamw_step(const fmb_adamw_t* args, const fmb_adamw_tensor_t* tensors, int count, fmb_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------------ embeddings
+ * No counterpart in the reference. Rows of a table by token (the element of an atom), scaled, and the table's gradient from
+ * tokens that have been sorted. */
+#define FMB_MAX_VOCABULARY 1048575
+
+/* order [rows]: the rows by token, in ascending order within a token, then the rows whose token is none (negative, or >=
+ * vocabulary); keys [rows]: their tokens, `vocabulary` for none. tokens: int32 or int64 (token_bytes 4 or 8).
+ * scratch: fmb_sort_tokens_scratch(rows, vocabulary) int32, written before it is read. */
+FMB_API long long fmb_sort_tokens_scratch(long long rows, int vocabulary);
+FMB_API int fmb_sort_tokens(const void* tokens, int token_bytes, long long rows, int vocabulary, int32_t* order, int32_t* keys,
+                            int32_t* scratch, fmb_stream_t stream);
+
+typedef struct {
+    int32_t type;                     /* FMB_TYPE_* of the table, or of dy */
+    int32_t out_type;                 /* lookup: of the rows; the gradient is always fp32 */
+    int32_t rows;
+    int32_t vocabulary;
+    int32_t width;
+    int32_t token_bytes;              /* lookup: 4 or 8 */
+    int32_t zero_rest;                /* lookup: rows of no token become zero instead of staying as they are */
+    int32_t accumulate;               /* gradient: add to the table's */
+    double scale;
+    const void* tokens;               /* lookup [rows]; gradient: `keys` of fmb_sort_tokens */
+    const int32_t* order;             /* gradient: of fmb_sort_tokens */
+    const void* source;               /* lookup: the table [vocabulary][width]; gradient: dy [rows][width] */
+    void* out;                        /* lookup: rows [rows][width]; gradient: fp32 [vocabulary][width] */
+    long long source_stride;          /* in elements; the last index is contiguous */
+    long long out_stride;
+    float* scratch;                   /* gradient: fmb_embedding_gradient_scratch(...) floats from a multiple of 16 bytes on, written
+                                       * before they are read; may be null where that is 0 */
+} fmb_embedding_t;
+
+/* out[r] = scale source[tokens[r]], computed in fp32 and rounded once */
+FMB_API int fmb_embedding(const fmb_embedding_t* args, fmb_stream_t stream);
+/* out[v] (+)= scale * sum of source[r] over the rows r of token v, summed in fp32 in an order that the sizes and the tokens fix; zero
+ * for a token without rows. Entries of order and keys that are out of range are skipped. */
+FMB_API int fmb_embedding_gradient(const fmb_embedding_t* args, fmb_stream_t stream);
+FMB_API long long fmb_embedding_gradient_scratch(const fmb_embedding_t* args);
+
 #ifdef __cplusplus
 }
 #endif
