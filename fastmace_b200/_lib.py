@@ -19,6 +19,7 @@ MAX_SPECIES = 8
 MAX_GROUPS = 1024
 ADAMW_BLOCK = 256
 MAX_VOCABULARY = 1048575
+HELD_BLOCK = 32
 IMAGES, IMAGE_ONCHIP, IMAGE_FIRST_PADDED = 0x464d4200, 1, 2   # LayerStruct.extra_images: mark and bits
 
 STATUS_CAND_OVERFLOW = 1
@@ -37,7 +38,9 @@ EXPORTS = ("fmb_version", "fmb_last_error", "fmb_sizeof", "fmb_launch_count", "f
            "fmb_langevin_noise_sums", "fmb_langevin_first_half_global", "fmb_commit_forces", "fmb_profile_enable", "fmb_profile_read",
            "fmb_group_rows_scratch", "fmb_group_rows", "fmb_grouped_scratch", "fmb_grouped_linear", "fmb_grouped_input_gradient",
            "fmb_grouped_weight_gradient", "fmb_adamw_step",
-           "fmb_sort_tokens_scratch", "fmb_sort_tokens", "fmb_embedding", "fmb_embedding_gradient", "fmb_embedding_gradient_scratch")
+           "fmb_sort_tokens_scratch", "fmb_sort_tokens", "fmb_embedding", "fmb_embedding_gradient", "fmb_embedding_gradient_scratch",
+           "fmb_hold_rows", "fmb_release_rows", "fmb_gated_rows", "fmb_gated_rows_gradient", "fmb_held_weight_gradient",
+           "fmb_held_weight_gradient_scratch")
 
 
 class Fmb200Error(RuntimeError):
@@ -140,6 +143,14 @@ class EmbeddingStruct(ctypes.Structure):
     ]
 
 
+class HeldStruct(ctypes.Structure):
+    _fields_ = [
+        ("type", c_int32), ("rows", c_int32), ("columns", c_int32), ("parts", c_int32), ("x", c_void_p), ("codes", c_void_p),
+        ("exponents", c_void_p), ("h", c_void_p), ("dh", c_void_p), ("du", c_void_p), ("x_stride", ctypes.c_longlong),
+        ("h_stride", ctypes.c_longlong), ("dh_stride", ctypes.c_longlong), ("du_stride", ctypes.c_longlong),
+    ]
+
+
 STAGES = ("edge_features", "radial_gemm", "tp_forward_l0", "tp_forward_l1", "node_linears", "symcon_forward",
           "symcon_backward", "tp_backward_l1", "tp_backward_l0", "readout_reduce")
 
@@ -162,7 +173,7 @@ def load() -> ctypes.CDLL:
     if lib.fmb_version() != VERSION:
         raise Fmb200Error(f"the library has version {lib.fmb_version()}, this binding {VERSION}: rebuild the library")
     for which, struct in enumerate((NlStruct, ModelStruct, WorkStruct, LangevinStruct, GroupedStruct, AdamwTensorStruct,
-                                    AdamwStruct, EmbeddingStruct)):
+                                    AdamwStruct, EmbeddingStruct, HeldStruct)):
         if lib.fmb_sizeof(which) != ctypes.sizeof(struct):
             raise Fmb200Error(f"struct {struct.__name__} is {ctypes.sizeof(struct)} bytes here, "
                               f"{lib.fmb_sizeof(which)} in the library: rebuild the library")
@@ -201,10 +212,17 @@ def load() -> ctypes.CDLL:
     lib.fmb_sort_tokens_scratch.argtypes = [ctypes.c_longlong, c_int]
     lib.fmb_sort_tokens.argtypes = [P, c_int, ctypes.c_longlong, c_int, P, P, P, P]
     lib.fmb_embedding_gradient_scratch.argtypes = [POINTER(EmbeddingStruct)]
-    for name in ("fmb_sort_tokens_scratch", "fmb_embedding_gradient_scratch"):
+    for name in ("fmb_sort_tokens_scratch", "fmb_embedding_gradient_scratch",
+           "fmb_hold_rows", "fmb_release_rows", "fmb_gated_rows", "fmb_gated_rows_gradient", "fmb_held_weight_gradient",
+           "fmb_held_weight_gradient_scratch"):
         getattr(lib, name).restype = ctypes.c_longlong
     for name in ("fmb_embedding", "fmb_embedding_gradient"):
         getattr(lib, name).argtypes = [POINTER(EmbeddingStruct), P]
+    for name in ("fmb_hold_rows", "fmb_release_rows", "fmb_gated_rows", "fmb_gated_rows_gradient"):
+        getattr(lib, name).argtypes = [POINTER(HeldStruct), P]
+    lib.fmb_held_weight_gradient.argtypes = [POINTER(GroupedStruct), P, P]
+    lib.fmb_held_weight_gradient_scratch.argtypes = [POINTER(GroupedStruct)]
+    lib.fmb_held_weight_gradient_scratch.restype = ctypes.c_longlong
     lib.fmb_adamw_step.argtypes = [POINTER(AdamwStruct), POINTER(AdamwTensorStruct), c_int, P]
     _LIB = lib
     return lib

@@ -62,6 +62,7 @@ extern "C" FMB_API int fmb_sizeof(int which) {
         case 5: return (int)sizeof(fmb_adamw_tensor_t);
         case 6: return (int)sizeof(fmb_adamw_t);
         case 7: return (int)sizeof(fmb_embedding_t);
+        case 8: return (int)sizeof(fmb_held_t);
         default: return -1;
     }
 }

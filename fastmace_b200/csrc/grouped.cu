@@ -3,7 +3,7 @@
 // 16-bit operands: grouped_tc.cu. fp32 operands, split into bf16 parts on their way: grouped_parts.cu, and linears of a depth of up to
 // 128, whose split weights fit in tensor memory, grouped_resident.cu.
 
-#include "grouped.cuh"
+#include "held.cuh"
 
 #include <algorithm>
 
@@ -102,6 +102,16 @@ int run(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
     return a->type == FMB_TYPE_F32 ? parts_launch(a, mode, stream) : tma_launch(a, mode, stream);
 }
 
+// fp32 rows that are held in 8 bits are read back first, into the front of the scratch: the call that is left
+fmb_grouped_t released(const fmb_grouped_t& a, long long& front) {
+    fmb_grouped_t b = a;
+    b.x_stride = (a.k + 3) / 4 * 4;
+    front = (a.rows * b.x_stride + 63) / 64 * 64;
+    b.x = a.scratch ? (void*)a.scratch : (void*)256;         // (what a plan asks of it is where rows begin)
+    b.scratch = a.scratch ? a.scratch + front : nullptr;
+    return b;
+}
+
 }  // namespace
 
 int sum_units(const fmb_grouped_t* a, int unit_rows, cudaStream_t stream) {
@@ -137,4 +147,26 @@ extern "C" FMB_API int fmb_grouped_weight_gradient(const fmb_grouped_t* a, fmb_s
 extern "C" FMB_API long long fmb_grouped_scratch(const fmb_grouped_t* a, int which) {
     if (!a || which < 0 || which > 2 || a->groups < 1 || a->k < 1 || a->n < 1 || a->rows < 1) return 0;
     return a->type == FMB_TYPE_F32 ? parts_scratch(a, (Mode)which) : tma_scratch_bytes(a, (Mode)which) / 4;
+}
+
+extern "C" FMB_API int fmb_held_weight_gradient(const fmb_grouped_t* a, const uint8_t* exponents, fmb_stream_t stream) {
+    const int rc = check(a);
+    if (rc) return rc;
+    if (a->rows == 0) return run(a, kWeightGradient, (cudaStream_t)stream);
+    FMB_REQUIRE(exponents, "fmb_held_weight_gradient: null argument");
+    FMB_REQUIRE(a->rows == 1 || a->x_stride == a->k, "fmb_held_weight_gradient: codes must be contiguous");
+    if (a->type != FMB_TYPE_F32) return tma_launch(a, kWeightGradient, (cudaStream_t)stream, exponents);
+    FMB_REQUIRE(a->scratch && ((uintptr_t)a->scratch & 255) == 0, "grouped product: scratch starts at a multiple of 256 bytes");
+    long long front;
+    const fmb_grouped_t b = released(*a, front);
+    const int rc2 = held::release(a->type, (const uint8_t*)a->x, exponents, a->rows, a->k, 1, b.x, b.x_stride, (cudaStream_t)stream);
+    return rc2 ? rc2 : run(&b, kWeightGradient, (cudaStream_t)stream);
+}
+
+extern "C" FMB_API long long fmb_held_weight_gradient_scratch(const fmb_grouped_t* a) {
+    if (!a || a->groups < 1 || a->k < 1 || a->n < 1 || a->rows < 1) return 0;
+    if (a->type != FMB_TYPE_F32) return tma_scratch_bytes(a, kWeightGradient, true) / 4;
+    long long front;
+    const fmb_grouped_t b = released(*a, front);
+    return front + parts_scratch(&b, kWeightGradient);
 }

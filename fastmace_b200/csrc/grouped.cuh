@@ -78,8 +78,9 @@ enum Mode { kLinear = 0, kInputGradient = 1, kWeightGradient = 2 };
 
 // tcgen05 kernels of 16-bit operands, brought by TMA (grouped_tc.cu), and the bytes of scratch that a call with these sizes,
 // strides and pointers needs
-int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
-long long tma_scratch_bytes(const fmb_grouped_t* a, Mode mode);
+// exponents, of the weight gradient: x is held in 8 bits (held.cuh), a->x points at the codes
+int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream, const uint8_t* exponents = nullptr);
+long long tma_scratch_bytes(const fmb_grouped_t* a, Mode mode, bool held = false);
 // tcgen05 kernel that keeps the split weights in tensor memory (grouped_resident.cu): fp32 linears of a depth of at most 128, rows
 // that TMA takes
 int resident_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream);
@@ -102,7 +103,7 @@ int sm_count();
 // (rows, weights: where to, or null; in 32 bits the strides are multiples of four values, else of eight)
 int pack(const fmb_grouped_t* a, const void* src, long long stride, int columns, void* rows, void* weights, cudaStream_t stream);
 int pack_32(const fmb_grouped_t* a, const void* src, long long stride, int columns, void* rows, void* weights, cudaStream_t stream);
-int sort_rows(const fmb_grouped_t* a, void* x, void* y, int32_t* first_block, cudaStream_t stream);
+int sort_rows(const fmb_grouped_t* a, void* x, void* y, int32_t* first_block, const uint8_t* exponents, cudaStream_t stream);
 
 }  // namespace grp
 }  // namespace fmb

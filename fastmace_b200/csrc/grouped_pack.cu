@@ -5,7 +5,7 @@
 //     64 rows: TMA brings rows that lie side by side at 64 bytes a cycle and SM, rows gathered by number at 30. Each row is read
 //     once here and n / 256 or k / 256 times by the products.
 
-#include "grouped.cuh"
+#include "held.cuh"
 
 #include <algorithm>
 
@@ -99,9 +99,47 @@ k_pack_32(fmb_grouped_t a, float* weights, const float* src, long long stride, i
         copy_row_32(weights + ((long long)g * a.k + r) * width, (const float*)a.w + g * a.w_group_stride + r * a.w_row_stride, a.n);
 }
 
-// x and y by groups; first_block[g]: blocks of 64 rows of the groups before g
+// Eight values from column c of a row that is held in 8 bits, in T; what is past the columns is zero.
+template <typename T>
+__device__ __forceinline__ uint4 held_eight(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, int c, int columns, bool wide) {
+    if (c >= columns) return make_uint4(0, 0, 0, 0);
+    uint32_t v[2] = {0, 0};
+    if (wide) {
+        const uint2 eight = __ldg(reinterpret_cast<const uint2*>(codes + c));
+        v[0] = eight.x;
+        v[1] = eight.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (c + i < columns) v[i / 4] |= (uint32_t)__ldg(codes + c + i) << (8 * (i % 4));
+    }
+    const float unit = held::unit_of(__ldg(exponents + c / held::kBlock));
+    uint32_t out[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 two = held::two_values(v[i / 2] >> (16 * (i % 2)));
+        out[i] = held::two_of<T>(two.x * unit, two.y * unit);
+    }
+    return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ void release_row(uint16_t* __restrict__ dst, const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents,
+                                            int columns, int width, bool wide) {
+    for (int c0 = 8 * (threadIdx.x & 31); c0 < width; c0 += 1024) {
+        uint4 v[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = held_eight<T>(codes, exponents, c0 + 256 * j, codes ? columns : 0, wide);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (c0 + 256 * j < width) *reinterpret_cast<uint4*>(dst + c0 + 256 * j) = v[j];
+    }
+}
+
+// x and y by groups; first_block[g]: blocks of 64 rows of the groups before g. HELD: x is held in 8 bits, and read back in T on its way
+template <typename T, bool HELD>
 __global__ void __launch_bounds__(kThreads)
-k_sort_rows(fmb_grouped_t a, RowsArgs x, RowsArgs y, int32_t* first_block) {
+k_sort_rows(fmb_grouped_t a, RowsArgs x, RowsArgs y, int32_t* first_block, const uint8_t* __restrict__ exponents) {
     extern __shared__ int first[];
     count_units<kThreads>(a.offsets, a.groups, a.rows, 64, 0, first);
     if (blockIdx.x == 0)
@@ -114,7 +152,11 @@ k_sort_rows(fmb_grouped_t a, RowsArgs x, RowsArgs y, int32_t* first_block) {
         const long long entry = begin + (long long)(block - first[g]) * 64 + (r & 63);
         int row = entry < end ? __ldg(a.order + entry) : -1;
         if (row >= a.rows) row = -1;
-        copy_row(x.dst + r * x.dst_stride, row >= 0 ? x.src + row * x.src_stride : nullptr, x.columns, (int)x.dst_stride, x.wide);
+        if constexpr (HELD)
+            release_row<T>(x.dst + r * x.dst_stride, row >= 0 ? (const uint8_t*)x.src + row * (long long)x.columns : nullptr,
+                           exponents + row * (long long)held::blocks_of(x.columns), x.columns, (int)x.dst_stride, x.wide);
+        else
+            copy_row(x.dst + r * x.dst_stride, row >= 0 ? x.src + row * x.src_stride : nullptr, x.columns, (int)x.dst_stride, x.wide);
         copy_row(y.dst + r * y.dst_stride, row >= 0 ? y.src + row * y.src_stride : nullptr, y.columns, (int)y.dst_stride, y.wide);
     }
 }
@@ -161,10 +203,13 @@ int pack_32(const fmb_grouped_t* a, const void* src, long long stride, int colum
     return FMB_OK;
 }
 
-int sort_rows(const fmb_grouped_t* a, void* x, void* y, int32_t* first_block, cudaStream_t stream) {
-    const int grid = std::min(ceil_div(a->rows + 64ll * a->groups, kThreads / 32), 8 * sm_count());
-    k_sort_rows<<<grid, kThreads, (a->groups + 1) * (int)sizeof(int), stream>>>(
-        *a, rows_args(a->x, a->x_stride, a->k, x), rows_args(a->y, a->y_stride, a->n, y), first_block);
+int sort_rows(const fmb_grouped_t* a, void* x, void* y, int32_t* first_block, const uint8_t* exponents, cudaStream_t stream) {
+    const int grid = std::min(ceil_div(a->rows + 64ll * a->groups, kThreads / 32), 8 * sm_count()), smem = (a->groups + 1) * (int)sizeof(int);
+    RowsArgs from_x = rows_args(a->x, a->x_stride, a->k, x), from_y = rows_args(a->y, a->y_stride, a->n, y);
+    if (exponents) from_x.wide = a->k % 8 == 0 && ((uintptr_t)a->x & 7) == 0;
+    if (!exponents) k_sort_rows<uint16_t, false><<<grid, kThreads, smem, stream>>>(*a, from_x, from_y, first_block, nullptr);
+    else if (a->type == FMB_TYPE_BF16) k_sort_rows<__nv_bfloat16, true><<<grid, kThreads, smem, stream>>>(*a, from_x, from_y, first_block, exponents);
+    else k_sort_rows<__half, true><<<grid, kThreads, smem, stream>>>(*a, from_x, from_y, first_block, exponents);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }

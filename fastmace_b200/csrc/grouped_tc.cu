@@ -18,6 +18,7 @@
 // (16,384 rows of 4,096 x 4,096 in 4 groups: 1.52 PFLOP/s) and with deep gathers the 30 cycles that one takes.
 
 #include "grouped_tc.cuh"
+#include "held.cuh"
 
 #include <algorithm>
 
@@ -669,7 +670,7 @@ bool by_sixteen(const void* base, long long stride) { return ((uintptr_t)base & 
 
 // What a call does before its products, and where in its scratch (byte offsets; -1: not needed).
 struct Plan {
-    long long x = -1, y = -1, w = -1, units = -1, first_block = -1, bytes = 0;
+    long long x = -1, y = -1, w = -1, units = -1, first_block = -1, bytes = 0;      // x: also rows read back from 8 bits
     int tn = 0, unit_rows = 1 << 30;             // weight gradient
     bool pair = false, sorted = false;
 
@@ -680,10 +681,10 @@ struct Plan {
     }
 };
 
-Plan plan_of(const fmb_grouped_t* a, Mode mode) {
+Plan plan_of(const fmb_grouped_t* a, Mode mode, bool held) {
     Plan p;
     const long long k8 = (a->k + 7) / 8 * 8, n8 = (a->n + 7) / 8 * 8;
-    const bool x_fits = by_sixteen(a->x, a->x_stride), y_fits = by_sixteen(a->y, a->y_stride);
+    const bool x_fits = held || by_sixteen(a->x, a->x_stride), y_fits = by_sixteen(a->y, a->y_stride);
     if (mode != kWeightGradient) {
         // the input, and the weights (their strides may be anything where there is one row, or one matrix)
         if (mode == kLinear && !x_fits) p.x = p.take(a->rows * k8 * 2);
@@ -713,12 +714,14 @@ Plan plan_of(const fmb_grouped_t* a, Mode mode) {
         p.x = p.take(rows * k8 * 2);
         p.y = p.take(rows * n8 * 2);
         p.first_block = p.take((a->groups + 1) * 4);
+    } else if (held) {
+        p.x = p.take(a->rows * k8 * 2);
     }
     return p;
 }
 
 template <typename T>
-int weight_gradient(const fmb_grouped_t* a, const Plan& plan, cudaStream_t stream) {
+int weight_gradient(const fmb_grouped_t* a, const Plan& plan, const uint8_t* exponents, cudaStream_t stream) {
     Args p;
     p.a = *a;
     p.a.scratch = plan.units >= 0 ? (float*)((char*)a->scratch + plan.units) : nullptr;
@@ -736,7 +739,7 @@ int weight_gradient(const fmb_grouped_t* a, const Plan& plan, cudaStream_t strea
         void* const x = (char*)a->scratch + plan.x;
         void* const y = (char*)a->scratch + plan.y;
         int32_t* const first_block = (int32_t*)((char*)a->scratch + plan.first_block);
-        rc = sort_rows(a, x, y, first_block, stream);
+        rc = sort_rows(a, x, y, first_block, exponents, stream);
         if (rc) return rc;
         p.first_block = first_block;
         const int all = a->rows + 64 * a->groups;
@@ -747,8 +750,16 @@ int weight_gradient(const fmb_grouped_t* a, const Plan& plan, cudaStream_t strea
              : plan.tn == 256 ? launch<T, kWeightGradient, 256, false, true>(p, features, rows, weights, tiles, stream)
                               : launch<T, kWeightGradient, 128, false, true>(p, features, rows, weights, tiles, stream);
     } else {
+        const void* x = a->x;
+        long long x_stride = a->x_stride;
+        if (exponents) {
+            x = (char*)a->scratch + plan.x;
+            x_stride = (a->k + 7) / 8 * 8;
+            rc = held::release(a->type, (const uint8_t*)a->x, exponents, a->rows, a->k, 1, (char*)a->scratch + plan.x, x_stride, stream);
+            if (rc) return rc;
+        }
         FMB_REQUIRE(encode_map(&features, a->type, a->y, a->n, a->rows, 1, a->y_stride, 0, 1, 2, 64, true) &&
-                        encode_map(&rows, a->type, a->x, a->k, a->rows, 1, a->x_stride, 0, 1, 2, 64, true),
+                        encode_map(&rows, a->type, x, a->k, a->rows, 1, x_stride, 0, 1, 2, 64, true),
                     "fmb_grouped_weight_gradient: tensor maps");
         rc = plan.pair        ? launch<T, kWeightGradient, 256, true>(p, features, rows, weights, tiles, stream)
              : plan.tn == 256 ? launch<T, kWeightGradient, 256, false>(p, features, rows, weights, tiles, stream)
@@ -794,8 +805,8 @@ int linear(const fmb_grouped_t* a, bool forward, const Plan& plan, cudaStream_t 
 }
 
 template <typename T>
-int typed(const fmb_grouped_t* a, Mode mode, const Plan& plan, cudaStream_t stream) {
-    return mode == kWeightGradient ? weight_gradient<T>(a, plan, stream) : linear<T>(a, mode == kLinear, plan, stream);
+int typed(const fmb_grouped_t* a, Mode mode, const Plan& plan, const uint8_t* exponents, cudaStream_t stream) {
+    return mode == kWeightGradient ? weight_gradient<T>(a, plan, exponents, stream) : linear<T>(a, mode == kLinear, plan, stream);
 }
 
 }  // namespace
@@ -820,13 +831,13 @@ bool encode_map(CUtensorMap* map, int type, const void* base, int columns, int r
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-long long tma_scratch_bytes(const fmb_grouped_t* a, Mode mode) { return plan_of(a, mode).bytes; }
+long long tma_scratch_bytes(const fmb_grouped_t* a, Mode mode, bool held) { return plan_of(a, mode, held).bytes; }
 
-int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream) {
-    const Plan plan = plan_of(a, mode);
+int tma_launch(const fmb_grouped_t* a, Mode mode, cudaStream_t stream, const uint8_t* exponents) {
+    const Plan plan = plan_of(a, mode, exponents);
     FMB_REQUIRE(plan.bytes == 0 || a->scratch, "grouped product: null scratch");
     FMB_REQUIRE(((uintptr_t)a->scratch & 255) == 0, "grouped product: scratch starts at a multiple of 256 bytes");
-    return a->type == FMB_TYPE_BF16 ? typed<__nv_bfloat16>(a, mode, plan, stream) : typed<__half>(a, mode, plan, stream);
+    return a->type == FMB_TYPE_BF16 ? typed<__nv_bfloat16>(a, mode, plan, exponents, stream) : typed<__half>(a, mode, plan, exponents, stream);
 }
 
 }  // namespace grp

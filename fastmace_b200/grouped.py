@@ -215,15 +215,13 @@ def grouped_linear_input_gradient(dy: torch.Tensor, weight: torch.Tensor, groups
     return _rows_product("grouped_linear_input_gradient", "fmb_grouped_input_gradient", dy, weight, groups, out, True)
 
 
-def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: RowGroups, out: torch.Tensor | None = None,
-                                   accumulate: bool = False) -> torch.Tensor:
-    """``dW[g] = sum of x[r]^T dy[r]`` over the rows of g, float32 ``[groups, k, n]``; zero for a group without rows.
-    ``accumulate=True`` adds to ``out``. The sums run in an order that depends on the sizes alone."""
-    what = "grouped_linear_weight_gradient"
-    rows, k, x_stride = _matrix(what, "x", x)
+def _weight_gradient(what: str, x: torch.Tensor, x_stride: int, dtype: torch.dtype, dy: torch.Tensor, groups: RowGroups,
+                     out: torch.Tensor | None, accumulate: bool, exponents: torch.Tensor | None = None) -> torch.Tensor:
+    """The weight gradient of rows x, or of the codes x and exponents of rows of type ``dtype`` that are held in 8 bits."""
+    rows, k = x.shape
     _, n, y_stride = _matrix(what, "dy", dy, rows=rows)
-    kind = TYPES.get(x.dtype)
-    if kind is None or dy.dtype != x.dtype:
+    kind = TYPES.get(dtype)
+    if kind is None or dy.dtype != dtype:
         raise ValueError(f"{what}: x and dy must have the same type, float32, bfloat16 or float16")
     count = _groups(what, groups, rows)
     index = _on_device(what, x, dy, *groups)
@@ -236,7 +234,7 @@ def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: Ro
         raise ValueError(f"{what}: out must be float32 {(count, k, n)}")
     else:
         _on_device(what, x, out)
-        if _shares_memory(out, x) or _shares_memory(out, dy):
+        if _shares_memory(out, x) or _shares_memory(out, dy) or (exponents is not None and _shares_memory(out, exponents)):
             raise ValueError(f"{what}: out shares memory with an operand")
     _, _, _, w_group, w_row = _weights(what, "out", out)
     far, near, inner = (max(w_row, w_group), min(w_row, w_group), k if w_group >= w_row else count)
@@ -246,14 +244,28 @@ def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: Ro
     lib = _lib.load()
     a = _lib.GroupedStruct(kind, count, rows, k, n, 0, bool(accumulate), 0, groups[0].data_ptr(), groups[1].data_ptr(), x.data_ptr(),
                            dy.data_ptr(), out.data_ptr(), x_stride, y_stride, w_row, w_group, None, _status_pointer(index))
-    need = lib.fmb_grouped_scratch(ctypes.byref(a), 2)
+    call = ctypes.byref(a)
+    need = lib.fmb_grouped_scratch(call, 2) if exponents is None else lib.fmb_held_weight_gradient_scratch(call)
     if need:
         scratch = torch.empty(need, dtype=torch.float32, device=x.device)
         a.scratch = scratch.data_ptr()
-    _lib.check(_launch(index, lib.fmb_grouped_weight_gradient, ctypes.byref(a)), "fmb_grouped_weight_gradient")
+    if exponents is None:
+        _lib.check(_launch(index, lib.fmb_grouped_weight_gradient, call), "fmb_grouped_weight_gradient")
+    else:
+        _lib.check(_launch(index, lib.fmb_held_weight_gradient, call, exponents.data_ptr()), "fmb_held_weight_gradient")
     if given:
         _written(out)
     return out
+
+
+def grouped_linear_weight_gradient(x: torch.Tensor, dy: torch.Tensor, groups: RowGroups, out: torch.Tensor | None = None,
+                                   accumulate: bool = False) -> torch.Tensor:
+    """``dW[g] = sum of x[r]^T dy[r]`` over the rows of g, float32 ``[groups, k, n]``; zero for a group without rows.
+    ``accumulate=True`` adds to ``out``. The sums run in an order that depends on the sizes alone. Rows x that are held in 8 bits:
+    ``checkpoints.held_weight_gradient``."""
+    what = "grouped_linear_weight_gradient"
+    stride = _matrix(what, "x", x)[2]
+    return _weight_gradient(what, x, stride, x.dtype, dy, groups, out, accumulate)
 
 
 __all__ = ["RowGroups", "group_rows", "grouped_linear", "grouped_linear_input_gradient", "grouped_linear_weight_gradient",

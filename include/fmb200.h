@@ -529,6 +529,44 @@ FMB_API int fmb_embedding(const fmb_embedding_t* args, fmb_stream_t stream);
 FMB_API int fmb_embedding_gradient(const fmb_embedding_t* args, fmb_stream_t stream);
 FMB_API long long fmb_embedding_gradient_scratch(const fmb_embedding_t* args);
 
+/* ------------------------------------------------------------------------------------------------ rows held in 8 bits
+ * No counterpart in the reference. What a backward pass needs of a forward one, kept as e4m3 codes in units of a power of two per
+ * FMB_HELD_BLOCK columns: exact in the rows' own type when read back. The exponent of a block is the smallest e with |x| <= 448 2^e for
+ * all of its finite values, between -117 and 120 (FMB_TYPE_F16: -15 and 8; codes end at 240 in the highest); what is not finite is held
+ * as NaN. */
+#define FMB_HELD_BLOCK 32
+
+typedef struct {
+    int32_t type;                     /* FMB_TYPE_* of x, h, dh and du */
+    int32_t rows;
+    int32_t columns;                  /* of x and du; h and dh of a gate have half as many */
+    int32_t parts;                    /* 1, or 2: each half of a row has blocks of its own. The gate's rows u = (a | b) have 2 */
+    const void* x;                    /* [rows][columns] */
+    uint8_t* codes;                   /* [rows][columns], contiguous */
+    uint8_t* exponents;               /* [rows][parts][ceil(columns / parts / FMB_HELD_BLOCK)], contiguous: e + 127 */
+    void* h;
+    const void* dh;
+    void* du;
+    long long x_stride;               /* in elements; the last index is contiguous */
+    long long h_stride;
+    long long dh_stride;
+    long long du_stride;
+} fmb_held_t;
+
+/* codes and exponents of x */
+FMB_API int fmb_hold_rows(const fmb_held_t* args, fmb_stream_t stream);
+/* h [rows][columns] = the rows that codes and exponents hold */
+FMB_API int fmb_release_rows(const fmb_held_t* args, fmb_stream_t stream);
+/* h = silu(a) b for x = (a | b); codes and exponents of x with it where they are given */
+FMB_API int fmb_gated_rows(const fmb_held_t* args, fmb_stream_t stream);
+/* du = (dh b s (1 + a (1 - s)) | dh a s), s = 1 / (1 + exp(-a)), from codes and exponents or, where they are null, from x; h anew where it
+ * is given */
+FMB_API int fmb_gated_rows_gradient(const fmb_held_t* args, fmb_stream_t stream);
+/* fmb_grouped_weight_gradient with x held in 8 bits: args->x points at the codes (contiguous, x_stride = k), exponents [rows][ceil(k /
+ * FMB_HELD_BLOCK)]. Scratch as fmb_held_weight_gradient_scratch says, in floats. */
+FMB_API int fmb_held_weight_gradient(const fmb_grouped_t* args, const uint8_t* exponents, fmb_stream_t stream);
+FMB_API long long fmb_held_weight_gradient_scratch(const fmb_grouped_t* args);
+
 #ifdef __cplusplus
 }
 #endif
