@@ -20,6 +20,8 @@ MAX_GROUPS = 1024
 ADAMW_BLOCK = 256
 MAX_VOCABULARY = 1048575
 HELD_BLOCK = 32
+MAX_TOP = 16
+MAX_LAYER_TOKENS = 128
 IMAGES, IMAGE_ONCHIP, IMAGE_FIRST_PADDED = 0x464d4200, 1, 2   # LayerStruct.extra_images: mark and bits
 
 STATUS_CAND_OVERFLOW = 1
@@ -40,7 +42,7 @@ EXPORTS = ("fmb_version", "fmb_last_error", "fmb_sizeof", "fmb_launch_count", "f
            "fmb_grouped_weight_gradient", "fmb_adamw_step",
            "fmb_sort_tokens_scratch", "fmb_sort_tokens", "fmb_embedding", "fmb_embedding_gradient", "fmb_embedding_gradient_scratch",
            "fmb_hold_rows", "fmb_release_rows", "fmb_gated_rows", "fmb_gated_rows_gradient", "fmb_held_weight_gradient",
-           "fmb_held_weight_gradient_scratch")
+           "fmb_held_weight_gradient_scratch", "fmb_route_rows", "fmb_expert_layer", "fmb_expert_layer_scratch")
 
 
 class Fmb200Error(RuntimeError):
@@ -151,6 +153,24 @@ class HeldStruct(ctypes.Structure):
     ]
 
 
+class RouteStruct(ctypes.Structure):
+    _fields_ = [
+        ("type", c_int32), ("tokens", c_int32), ("width", c_int32), ("experts", c_int32), ("top", c_int32), ("normalise", c_int32),
+        ("x", c_void_p), ("router", c_void_p), ("chosen", c_void_p), ("weights", c_void_p), ("x_stride", ctypes.c_longlong),
+        ("router_stride", ctypes.c_longlong),
+    ]
+
+
+class ExpertsStruct(ctypes.Structure):
+    _fields_ = [
+        ("type", c_int32), ("tokens", c_int32), ("experts", c_int32), ("top", c_int32), ("width", c_int32), ("inner", c_int32),
+        ("x", c_void_p), ("w_up", c_void_p), ("w_down", c_void_p), ("chosen", c_void_p), ("weights", c_void_p), ("y", c_void_p),
+        ("x_stride", ctypes.c_longlong), ("y_stride", ctypes.c_longlong), ("up_group_stride", ctypes.c_longlong),
+        ("up_row_stride", ctypes.c_longlong), ("down_group_stride", ctypes.c_longlong), ("down_row_stride", ctypes.c_longlong),
+        ("scratch", c_void_p), ("status", c_void_p),
+    ]
+
+
 STAGES = ("edge_features", "radial_gemm", "tp_forward_l0", "tp_forward_l1", "node_linears", "symcon_forward",
           "symcon_backward", "tp_backward_l1", "tp_backward_l0", "readout_reduce")
 
@@ -173,7 +193,7 @@ def load() -> ctypes.CDLL:
     if lib.fmb_version() != VERSION:
         raise Fmb200Error(f"the library has version {lib.fmb_version()}, this binding {VERSION}: rebuild the library")
     for which, struct in enumerate((NlStruct, ModelStruct, WorkStruct, LangevinStruct, GroupedStruct, AdamwTensorStruct,
-                                    AdamwStruct, EmbeddingStruct, HeldStruct)):
+                                    AdamwStruct, EmbeddingStruct, HeldStruct, RouteStruct, ExpertsStruct)):
         if lib.fmb_sizeof(which) != ctypes.sizeof(struct):
             raise Fmb200Error(f"struct {struct.__name__} is {ctypes.sizeof(struct)} bytes here, "
                               f"{lib.fmb_sizeof(which)} in the library: rebuild the library")
@@ -214,7 +234,7 @@ def load() -> ctypes.CDLL:
     lib.fmb_embedding_gradient_scratch.argtypes = [POINTER(EmbeddingStruct)]
     for name in ("fmb_sort_tokens_scratch", "fmb_embedding_gradient_scratch",
            "fmb_hold_rows", "fmb_release_rows", "fmb_gated_rows", "fmb_gated_rows_gradient", "fmb_held_weight_gradient",
-           "fmb_held_weight_gradient_scratch"):
+           "fmb_held_weight_gradient_scratch", "fmb_route_rows", "fmb_expert_layer", "fmb_expert_layer_scratch"):
         getattr(lib, name).restype = ctypes.c_longlong
     for name in ("fmb_embedding", "fmb_embedding_gradient"):
         getattr(lib, name).argtypes = [POINTER(EmbeddingStruct), P]
@@ -223,6 +243,10 @@ def load() -> ctypes.CDLL:
     lib.fmb_held_weight_gradient.argtypes = [POINTER(GroupedStruct), P, P]
     lib.fmb_held_weight_gradient_scratch.argtypes = [POINTER(GroupedStruct)]
     lib.fmb_held_weight_gradient_scratch.restype = ctypes.c_longlong
+    lib.fmb_route_rows.argtypes = [POINTER(RouteStruct), P]
+    lib.fmb_expert_layer.argtypes = [POINTER(ExpertsStruct), P]
+    lib.fmb_expert_layer_scratch.argtypes = [POINTER(ExpertsStruct)]
+    lib.fmb_expert_layer_scratch.restype = ctypes.c_longlong
     lib.fmb_adamw_step.argtypes = [POINTER(AdamwStruct), POINTER(AdamwTensorStruct), c_int, P]
     _LIB = lib
     return lib

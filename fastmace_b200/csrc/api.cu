@@ -63,6 +63,8 @@ extern "C" FMB_API int fmb_sizeof(int which) {
         case 6: return (int)sizeof(fmb_adamw_t);
         case 7: return (int)sizeof(fmb_embedding_t);
         case 8: return (int)sizeof(fmb_held_t);
+        case 9: return (int)sizeof(fmb_route_t);
+        case 10: return (int)sizeof(fmb_experts_t);
         default: return -1;
     }
 }

@@ -567,6 +567,57 @@ FMB_API int fmb_gated_rows_gradient(const fmb_held_t* args, fmb_stream_t stream)
 FMB_API int fmb_held_weight_gradient(const fmb_grouped_t* args, const uint8_t* exponents, fmb_stream_t stream);
 FMB_API long long fmb_held_weight_gradient_scratch(const fmb_grouped_t* args);
 
+/* ------------------------------------------------------------------------------------------------ expert layers for a few tokens
+ * No counterpart in the reference. The routing of tokens to experts, and the experts' gated pair of matrices for so few tokens that the
+ * weights' bytes are what counts; for many, fmb_grouped_linear. */
+#define FMB_MAX_TOP 16
+#define FMB_MAX_LAYER_TOKENS 128
+
+typedef struct {
+    int32_t type;                     /* FMB_TYPE_* of x and router */
+    int32_t tokens;
+    int32_t width;
+    int32_t experts;                  /* 1 to FMB_MAX_GROUPS */
+    int32_t top;                      /* 1 to FMB_MAX_TOP */
+    int32_t normalise;                /* weights: softmax over the chosen logits, instead of over all */
+    const void* x;                    /* [tokens][width] */
+    const void* router;               /* [width][experts] */
+    int32_t* chosen;                  /* [tokens][top], contiguous */
+    float* weights;                   /* [tokens][top], contiguous */
+    long long x_stride;               /* in elements; the last index is contiguous */
+    long long router_stride;
+} fmb_route_t;
+
+/* The `top` largest of the logits x router of each token in falling order, equal ones by number, NaN last, and their weights; sums in fp32 */
+FMB_API int fmb_route_rows(const fmb_route_t* args, fmb_stream_t stream);
+
+typedef struct {
+    int32_t type;                     /* FMB_TYPE_* of x, the weights and y */
+    int32_t tokens;                   /* 0 to FMB_MAX_LAYER_TOKENS */
+    int32_t experts;
+    int32_t top;
+    int32_t width;
+    int32_t inner;
+    const void* x;                    /* [tokens][width] */
+    const void* w_up;                 /* [experts][width][2 inner]: the gate's columns, then those it multiplies */
+    const void* w_down;               /* [experts][inner][width] */
+    const int32_t* chosen;            /* [tokens][top], contiguous; one that is no expert gives nothing */
+    const float* weights;             /* [tokens][top], contiguous */
+    void* y;                          /* [tokens][width] */
+    long long x_stride;               /* in elements; the last index is contiguous */
+    long long y_stride;
+    long long up_group_stride;
+    long long up_row_stride;
+    long long down_group_stride;
+    long long down_row_stride;
+    float* scratch;                   /* fmb_expert_layer_scratch(...) floats from a multiple of 16 bytes on, written before they are read */
+    uint32_t* status;                 /* device word, may be null: receives FMB_STATUS_TENSOR_TIMEOUT */
+} fmb_experts_t;
+
+/* y[t] = sum over j of weights[t][j] (silu(a) b) w_down[e], (a | b) = x[t] w_up[e], e = chosen[t][j]; summed in fp32, rounded once */
+FMB_API int fmb_expert_layer(const fmb_experts_t* args, fmb_stream_t stream);
+FMB_API long long fmb_expert_layer_scratch(const fmb_experts_t* args);
+
 #ifdef __cplusplus
 }
 #endif
