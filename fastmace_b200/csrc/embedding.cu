@@ -96,110 +96,178 @@ int lookup(const fmb_embedding_t& a, cudaStream_t stream) {
 
 // ------------------------------------------------------------------------------------------------------------ gradient
 
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr int kUnroll = 8;                       // rows on their way
 
 // Columns of a slab: of every lane N side by side (VEC), or N that are 32 apart, where rows do not start at multiples of a pack
-template <typename T, bool VEC, int N>
+template <bool VEC, int N>
 __device__ __forceinline__ int column(int slab, int i) {
     const int lane = threadIdx.x & 31;
     return slab * 32 * N + (VEC ? lane * N + i : lane + 32 * i);
 }
 
+// A lane's N values of a row as they are in memory, 16 bytes (fp32, four) or up to 16, so that a row waits in few registers
 template <typename T, bool VEC, int N>
-__device__ __forceinline__ void load_columns(const T* __restrict__ row, int slab, int width, float (&x)[N]) {
-    const int c0 = column<T, VEC, N>(slab, 0);
-    if (VEC && c0 + N <= width) {
-        const Pack<T, N> in = *reinterpret_cast<const Pack<T, N>*>(row + c0);
+__device__ __forceinline__ uint4 load_columns(const T* __restrict__ row, int slab, int width) {
+    const int c0 = column<VEC, N>(slab, 0);
+    if (VEC && c0 + N <= width) return __ldg(reinterpret_cast<const uint4*>(row + c0));
+    uint32_t v[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = to_float(in.v[i]);
+    for (int i = 0; i < N; ++i) {
+        const int c = column<VEC, N>(slab, i);
+        if constexpr (sizeof(T) == 4) v[i] = c < width ? __ldg(reinterpret_cast<const uint32_t*>(row) + c) : 0u;
+        else v[i / 2] |= (c < width ? (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(row) + c) : 0u) << (16 * (i % 2));
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+template <typename T> __device__ __forceinline__ float2 two_of(uint32_t v);
+template <> __device__ __forceinline__ float2 two_of<__nv_bfloat16>(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }
+template <> __device__ __forceinline__ float2 two_of<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+
+template <typename T, int N>
+__device__ __forceinline__ void add_columns(float (&sum)[N], const uint4& x) {
+    if constexpr (sizeof(T) == 4) {
+        sum[0] += __uint_as_float(x.x);
+        sum[1] += __uint_as_float(x.y);
+        sum[2] += __uint_as_float(x.z);
+        sum[3] += __uint_as_float(x.w);
     } else {
+        const uint32_t v[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = column<T, VEC, N>(slab, i) < width ? to_float(row[column<T, VEC, N>(slab, i)]) : 0.0f;
+        for (int i = 0; i < N; i += 2) {
+            const float2 two = two_of<T>(v[i / 2]);
+            sum[i] += two.x;
+            sum[i + 1] += two.y;
+        }
     }
 }
 
 struct Sums {
     fmb_embedding_t a;
-    int chunk, chunks, slabs;
+    int chunk, chunks, slabs;                    // rows of a CTA's chunk, kWarps shares of them
     int wide_out;                                // rows of the table start at multiples of 16 bytes
     long long part_stride;                       // floats of a part in scratch: the width, filled up to a multiple of four
-    long long sum_ctas;                          // CTAs before those that write zeros
+    unsigned zero_ctas;                          // CTAs that write zeros, before those that sum
 };
 
-// first place whose key is not less than v
-__device__ __forceinline__ int lower_bound(const int32_t* __restrict__ keys, int rows, int v) {
-    int low = 0, high = rows;
+// first place from `low` on whose key is not less than v, by a warp: 32 places of what is left at a time
+__device__ __forceinline__ int lower_bound(const int32_t* __restrict__ keys, int low, int high, int v) {
+    const int lane = threadIdx.x & 31;
     while (low < high) {
-        const int mid = (int)(((unsigned)low + (unsigned)high) >> 1);
-        if (__ldg(keys + mid) < v) low = mid + 1; else high = mid;
+        const int step = (high - low + 31) / 32, at = min(low + lane * step, high - 1);
+        // of falling runs of "less", the last probe that is
+        const int less = __popc(__ballot_sync(0xffffffffu, low + lane * step < high && __ldg(keys + at) < v));
+        if (less == 0) return low;
+        const int last = low + (less - 1) * step;
+        high = min(high, last + step);
+        low = last + 1;
     }
     return low;
 }
 
+// Zeros for the tokens without rows, of 256 at a time: the rows' keys from the first of them on say which have some.
 __device__ __forceinline__ void write_zeros(const Sums& p) {
+    __shared__ uint32_t present[kWarps];
     const fmb_embedding_t& a = p.a;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int32_t* const keys = (const int32_t*)a.tokens;
-    const long long first = ((blockIdx.x - p.sum_ctas) * 8 + (threadIdx.x >> 5)) * 32;
-    const int v = (int)min(first + lane, (long long)a.vocabulary);
-    bool absent = false;
-    if (v < a.vocabulary) {
-        const int at = lower_bound(keys, a.rows, v);
-        absent = at == a.rows || keys[at] != v;
+    const int first = (int)blockIdx.x * 256, last = min(first + 256, a.vocabulary);
+    if (threadIdx.x < kWarps) present[threadIdx.x] = 0;
+    __syncthreads();
+    // every warp takes 32 of them: its rows lie between two bounds, and a lane looks at every 32nd
+    const int mine = first + 32 * warp;
+    if (mine < last) {
+        const int from = lower_bound(keys, 0, a.rows, mine), to = lower_bound(keys, from, a.rows, min(mine + 32, last));
+        uint32_t seen = 0;
+        if (to - from > 256) {
+            // tokens of many rows: a lane looks for its own
+            int low = from, high = mine + lane < last ? to : from;
+            while (low < high) {
+                const int mid = (int)(((unsigned)low + (unsigned)high) >> 1);
+                if (__ldg(keys + mid) < mine + lane) low = mid + 1; else high = mid;
+            }
+            seen = __ballot_sync(0xffffffffu, mine + lane < last && low < to && __ldg(keys + low) == mine + lane);
+        } else {
+            for (int at = from + lane; at < to; at += 32) seen |= 1u << ((__ldg(keys + at) - mine) & 31);
+            seen = __reduce_or_sync(0xffffffffu, seen);
+        }
+        if (lane == 0) present[warp] = seen;
     }
-    for (unsigned left = __ballot_sync(0xffffffffu, absent); left; left &= left - 1) {
-        float* const out = (float*)a.out + (first + __ffs(left) - 1) * a.out_stride;
+    __syncthreads();
+    for (int v = first + warp; v < last; v += kWarps) {
+        if (present[(v - first) >> 5] >> ((v - first) & 31) & 1) continue;
+        float* const out = (float*)a.out + v * a.out_stride;
         const int packs = p.wide_out ? a.width / 4 : 0;
         for (int c = lane; c < packs; c += 32) reinterpret_cast<float4*>(out)[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int c = 4 * packs + lane; c < a.width; c += 32) out[c] = 0.0f;
     }
 }
 
+// out (+)= scale sum, or a part as it is
+template <bool VEC, int N>
+__device__ __forceinline__ void write_sums(const Sums& p, int slab, float* out, bool part, const float (&sum)[N]) {
+    const fmb_embedding_t& a = p.a;
+    const float scale = (float)a.scale;
+    const bool wide = VEC && (part || p.wide_out);
+#pragma unroll
+    for (int i0 = 0; i0 < N; i0 += 4) {
+        const int c0 = column<VEC, N>(slab, i0);
+        if (wide && c0 + 4 <= a.width) {
+            float4* const to = reinterpret_cast<float4*>(out + c0);
+            float4 s = make_float4(sum[i0], sum[i0 + 1], sum[i0 + 2], sum[i0 + 3]);
+            if (!part) {
+                const float4 old = a.accumulate ? *to : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                s = make_float4(old.x + scale * s.x, old.y + scale * s.y, old.z + scale * s.z, old.w + scale * s.w);
+            }
+            *to = s;
+        } else {
+#pragma unroll
+            for (int i = i0; i < i0 + 4; ++i) {
+                const int c = column<VEC, N>(slab, i);
+                if (c < a.width) out[c] = part ? sum[i] : (a.accumulate ? out[c] : 0.0f) + scale * sum[i];
+            }
+        }
+    }
+}
+
+// A chunk's places are shared by the CTA's warps in kWarps runs of their own. The parts of a run of equal keys that goes over a warp's
+// end meet in shared memory; the parts of one that goes over the chunk's end go to scratch, the first of a chunk's two places
+// holding what a run has that began before it, the other what one has that begins in it and goes on.
 template <typename T, bool VEC, int N>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kThreads, 3)
 k_embedding_sums(Sums p) {
-    if (blockIdx.x >= p.sum_ctas) {
+    if (blockIdx.x < p.zero_ctas) {              // the first, since their searches take long and their writes little
         write_zeros(p);
         return;
     }
+    __shared__ float parts[2][kWarps][N][32];    // of each warp: of the run that it begins with, of the one that it ends with
+    __shared__ int states[kWarps][2];
     const fmb_embedding_t& a = p.a;
     const int32_t* const keys = (const int32_t*)a.tokens;
-    const int lane = threadIdx.x & 31;
-    const long long unit = blockIdx.x * 8ll + (threadIdx.x >> 5);
-    if (unit >= (long long)p.chunks * p.slabs) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const unsigned unit = blockIdx.x - p.zero_ctas;
     const int chunk = (int)(unit / p.slabs), slab = (int)(unit % p.slabs);
-    const int begin = chunk * p.chunk, end = min(a.rows, begin + p.chunk);
-    const float scale = (float)a.scale;
-    // of a run: its key, and whether it began in the chunk before
-    int key = __ldg(keys + begin);
-    bool before = begin > 0 && __ldg(keys + begin - 1) == key;
+    const int chunk_begin = chunk * p.chunk, chunk_end = min(a.rows, chunk_begin + p.chunk), share = p.chunk / kWarps;
+    const int begin = min(chunk_end, chunk_begin + warp * share), end = min(chunk_end, begin + share);
+    // of a run: its key, and whether it began before this warp's rows
+    int key = begin < end ? __ldg(keys + begin) : a.vocabulary;
+    bool before = begin > 0 && begin < end && __ldg(keys + begin - 1) == key;
+    const bool has_first = before;
+    bool first_ends = false;                     // the run that began before ends here
     float sum[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) sum[i] = 0.0f;
-
-    auto flush = [&](bool after) {
-        if (key < 0 || key >= a.vocabulary) return;
-        const bool part = before || after;
-        float* const out = part ? a.scratch + (2ll * chunk + (before ? 0 : 1)) * p.part_stride : (float*)a.out + key * a.out_stride;
-        const bool wide = VEC && (part || p.wide_out);
+    auto keep = [&](int which) {
 #pragma unroll
-        for (int i0 = 0; i0 < N; i0 += 4) {
-            const int c0 = column<T, VEC, N>(slab, i0);
-            if (wide && c0 + 4 <= a.width) {
-                float4* const to = reinterpret_cast<float4*>(out + c0);
-                float4 s = make_float4(sum[i0], sum[i0 + 1], sum[i0 + 2], sum[i0 + 3]);
-                if (!part) {
-                    const float4 old = a.accumulate ? *to : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    s = make_float4(old.x + scale * s.x, old.y + scale * s.y, old.z + scale * s.z, old.w + scale * s.w);
-                }
-                *to = s;
-            } else {
-#pragma unroll
-                for (int i = i0; i < i0 + 4; ++i) {
-                    const int c = column<T, VEC, N>(slab, i);
-                    if (c < a.width) out[c] = part ? sum[i] : (a.accumulate ? out[c] : 0.0f) + scale * sum[i];
-                }
-            }
+        for (int i = 0; i < N; ++i) parts[which][warp][i][lane] = sum[i];
+    };
+    auto flush = [&]() {
+        if (before) {
+            keep(0);
+            first_ends = true;
+        } else if (key >= 0 && key < a.vocabulary) {
+            write_sums<VEC, N>(p, slab, (float*)a.out + key * a.out_stride, false, sum);
         }
     };
 
@@ -208,33 +276,75 @@ k_embedding_sums(Sums p) {
         int row = p0 + lane < end ? __ldg(a.order + p0 + lane) : -1;
         if (row >= a.rows || mine < 0 || mine >= a.vocabulary) row = -1;
         for (int j0 = 0; j0 < count; j0 += kUnroll) {
-            float x[kUnroll][N];
+            uint4 x[kUnroll];
 #pragma unroll
             for (int j = 0; j < kUnroll; ++j) {
                 const int r = __shfl_sync(0xffffffffu, row, j0 + j);
-                if (r >= 0) {
-                    load_columns<T, VEC, N>((const T*)a.source + r * a.source_stride, slab, a.width, x[j]);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < N; ++i) x[j][i] = 0.0f;
-                }
+                x[j] = r >= 0 ? load_columns<T, VEC, N>((const T*)a.source + r * a.source_stride, slab, a.width) : make_uint4(0, 0, 0, 0);
             }
 #pragma unroll
             for (int j = 0; j < kUnroll; ++j) {
                 const int next = __shfl_sync(0xffffffffu, mine, j0 + j);
                 if (j0 + j < count && next != key) {
-                    flush(false);
+                    flush();
                     key = next;
                     before = false;
 #pragma unroll
                     for (int i = 0; i < N; ++i) sum[i] = 0.0f;
                 }
-#pragma unroll
-                for (int i = 0; i < N; ++i) sum[i] += x[j][i];
+                add_columns<T, N>(sum, x[j]);
             }
         }
     }
-    flush(end < a.rows && __ldg(keys + end) == key);
+    const bool after = begin < end && end < a.rows && __ldg(keys + end) == key;
+    bool has_last = false;
+    if (begin < end) {
+        if (before) {
+            keep(0);
+            first_ends = !after;
+        } else if (after) {
+            keep(1);
+            has_last = true;
+        } else {
+            flush();
+        }
+    }
+    // bits: a run that began before, which ends here; one that goes on
+    if (lane == 0) {
+        states[warp][0] = (has_first ? 1 : 0) | (first_ends ? 2 : 0) | (has_last ? 4 : 0);
+        states[warp][1] = key;
+    }
+    __syncthreads();
+    // The warps' parts in their order. Each warp adds up the runs that end in the warps of its turn: the run that a warp ends with is
+    // followed through the ones behind it, by that warp; the run that the chunk begins with by warp 0.
+    auto follow = [&](int w0) {
+        // (sum holds what the run has so far)
+        bool ended = false;
+        int w = w0;
+        for (; w < kWarps && !ended && (states[w][0] & 1); ++w) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) sum[i] += parts[0][w][i][lane];
+            ended = states[w][0] & 2;
+        }
+        return ended;
+    };
+    if (warp == 0 && (states[0][0] & 1)) {
+        const int run = __ldg(keys + chunk_begin);
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] = 0.0f;
+        follow(0);
+        if (run >= 0 && run < a.vocabulary) write_sums<VEC, N>(p, slab, a.scratch + 2ll * chunk * p.part_stride, true, sum);
+    }
+    if (states[warp][0] & 4) {
+        const int run = states[warp][1];
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] = parts[1][warp][i][lane];
+        const bool ended = follow(warp + 1);
+        if (run >= 0 && run < a.vocabulary) {
+            if (ended) write_sums<VEC, N>(p, slab, (float*)a.out + run * a.out_stride, false, sum);
+            else write_sums<VEC, N>(p, slab, a.scratch + (2ll * chunk + 1) * p.part_stride, true, sum);
+        }
+    }
 }
 
 // The runs that go over the end of the chunk in which they begin: their parts, added in the order of the chunks. A CTA has every
@@ -267,13 +377,13 @@ k_embedding_join(Sums p) {
         }
         __syncthreads();
         for (int q = 0; q < count; ++q) {
-            const int chunk = list[q], key = __ldg(keys + (chunk + 1) * p.chunk - 1);
-            const int parts = (lower_bound(keys, a.rows, key + 1) - 1) / p.chunk - chunk + 1;
+            const int chunk = list[q], end = (chunk + 1) * p.chunk, key = __ldg(keys + end - 1);
+            const int parts = (lower_bound(keys, end, a.rows, key + 1) - 1) / p.chunk - chunk + 1;
             for (int s0 = 0; s0 < slabs; s0 += kJoinWarps / shares) {
-                const int slab = s0 + warp / shares, share = warp % shares, c = slab * 128 + 4 * lane;
+                const int slab = s0 + warp / shares, part = warp % shares, c = slab * 128 + 4 * lane;
                 float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                 if (c < a.width) {
-                    const int from = (int)((long long)parts * share / shares), to = (int)((long long)parts * (share + 1) / shares);
+                    const int from = (int)((long long)parts * part / shares), to = (int)((long long)parts * (part + 1) / shares);
                     for (int u0 = from; u0 < to; u0 += 8) {
                         float4 x[8];
 #pragma unroll
@@ -292,7 +402,7 @@ k_embedding_join(Sums p) {
                 __syncthreads();
                 sums[warp][lane] = sum;
                 __syncthreads();
-                if (share > 0 || c >= a.width) continue;
+                if (part > 0 || c >= a.width) continue;
                 for (int w = 1; w < shares; ++w) {
                     const float4 x = sums[warp + w][lane];
                     sum.x += x.x; sum.y += x.y; sum.z += x.z; sum.w += x.w;
@@ -307,11 +417,11 @@ k_embedding_join(Sums p) {
     }
 }
 
-// Rows per chunk: enough chunks for 24 warps on every SM, and as few parts as that leaves; between 16 rows, under which parts cost more
-// than they spread, and 256.
+// Rows per chunk: kWarps shares that make enough warps for 24 on every SM, and as few parts as that leaves; a share has between 8 rows,
+// what a warp has on their way, and 256.
 int chunk_rows(const fmb_embedding_t& a, int slabs) {
     const long long rows = (long long)a.rows * slabs / (148 * 24) + 1;
-    return (int)std::min(256ll, std::max(16ll, (rows + 15) / 16 * 16));
+    return kWarps * (int)std::min(256ll, std::max(8ll, (rows + 7) / 8 * 8));
 }
 
 bool packed(const fmb_embedding_t& a) {
@@ -330,11 +440,12 @@ int gradient(const fmb_embedding_t& a, cudaStream_t stream) {
     p.chunks = ceil_div(a.rows, p.chunk);
     p.wide_out = starts_at(a.out, a.out_stride, 4, 4);
     p.part_stride = (a.width + 3) / 4 * 4;
-    p.sum_ctas = ceil_div((long long)p.chunks * p.slabs, 8);
-    const long long ctas = p.sum_ctas + (a.accumulate ? 0 : ceil_div(a.vocabulary, 256));
+    p.zero_ctas = a.accumulate ? 0 : ceil_div(a.vocabulary, 256);
+    const long long ctas = p.zero_ctas + (long long)p.chunks * p.slabs;
+    FMB_REQUIRE(ctas < (1ll << 31), "fmb_embedding_gradient: too many sums");
     if (ctas > 0) {
-        if (packed(a)) k_embedding_sums<T, true, kPack><<<(unsigned)ctas, 256, 0, stream>>>(p);
-        else k_embedding_sums<T, false, 4><<<(unsigned)ctas, 256, 0, stream>>>(p);
+        if (packed(a)) k_embedding_sums<T, true, kPack><<<(unsigned)ctas, kThreads, 0, stream>>>(p);
+        else k_embedding_sums<T, false, 4><<<(unsigned)ctas, kThreads, 0, stream>>>(p);
         FMB_LAUNCH_CHECK();
     }
     if (p.chunks > 1) {

@@ -19,9 +19,10 @@ namespace fmb {
 
 namespace {
 
-constexpr int kWarps = 32, kThreads = kWarps * 32;
 constexpr int kKeys = 8;                                  // per lane
 constexpr int kRowsPerWarp = 32 * kKeys;
+constexpr int kWarps = 32;                                // of a CTA that groups; of one that sorts tokens also kFewWarps
+constexpr int kFewWarps = 8;
 constexpr int kRowsPerCta = kWarps * kRowsPerWarp;
 
 // A pass over some bits of keys that are too many for one table (sort_tokens): the row in place i is from[i], or i; a key that
@@ -87,9 +88,10 @@ __device__ __forceinline__ int warps_before(int mine, int& all) {
     return inclusive - mine;
 }
 
-template <typename K, bool DIGIT>
-__global__ void __launch_bounds__(kThreads)
+template <typename K, bool DIGIT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS)
 k_group_count(const K* __restrict__ keys, Digit d, long long rows, int groups, int32_t* __restrict__ table) {
+    constexpr int kThreads = 32 * WARPS, kRowsPerCta = WARPS * kRowsPerWarp;
     __shared__ int counts[FMB_MAX_GROUPS + 1];
     const int width = groups + 1;
     int g[kKeys];
@@ -134,8 +136,10 @@ k_group_scan(int32_t* __restrict__ table, int32_t* __restrict__ totals, int ctas
 }
 
 // starts[g] = sum of starts[0 .. g) for g < width, by the whole CTA
+template <int WARPS>
 __device__ __forceinline__ void exclusive_starts(int* starts, int width) {
-    __shared__ int warp_total[kWarps];
+    constexpr int kThreads = 32 * WARPS;
+    __shared__ int warp_total[WARPS];
     const int per = (width + kThreads - 1) / kThreads, begin = min(width, (int)threadIdx.x * per), end = min(width, begin + per);
     int sum = 0, all;
     for (int i = begin; i < end; ++i) sum += starts[i];
@@ -153,28 +157,33 @@ __device__ __forceinline__ void exclusive_starts(int* starts, int width) {
     __syncthreads();
 }
 
+// Distance of the warps' counts, odd: a warp reads one count of each (65,536 rows by the 512 values of nine bits: 32 us, and 9 so)
+__host__ __device__ constexpr int place_stride(int width) { return width | 1; }
+constexpr int place_smem(int width, int warps) { return (warps * place_stride(width) + 2 * width + warps * kRowsPerWarp) * 4; }
+
 // ALONE: the only CTA, which takes its own counts for the totals. The CTA's rows are put in order in shared memory first, so
 // that the rows of a group leave in one run.
-template <typename K, bool ALONE, bool DIGIT>
-__global__ void __launch_bounds__(kThreads, ALONE ? 1 : 2)
+template <typename K, bool ALONE, bool DIGIT, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, ALONE ? 1 : 64 / WARPS)
 k_group_place(const K* __restrict__ keys, Digit d, long long rows, int groups, int bits, const int32_t* __restrict__ table,
               const int32_t* __restrict__ totals, int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
-    extern __shared__ int counts[];                       // [kWarps][groups + 1], [groups + 1] starts of the CTA, [groups + 1] of all, rows
-    const int width = groups + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    int* const here = counts + kWarps * width;
+    constexpr int kThreads = 32 * WARPS, kRowsPerCta = WARPS * kRowsPerWarp;
+    extern __shared__ int counts[];                       // [WARPS][stride], [groups + 1] starts of the CTA, [groups + 1] of all, rows
+    const int width = groups + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stride = place_stride(width);
+    int* const here = counts + WARPS * stride;
     int* const starts = ALONE ? here : here + width;
     int* const sorted = here + 2 * width;                 // row of the CTA | group << 13
     const long long first = (long long)blockIdx.x * kRowsPerCta;
     int g[kKeys], rank[kKeys];
     load_keys<K, DIGIT>(keys, d, first + warp * kRowsPerWarp, rows, groups, g);
-    const int warps = ALONE ? (int)((rows + kRowsPerWarp - 1) / kRowsPerWarp) : kWarps;        // that have rows
-    for (int i = threadIdx.x; i < warps * width; i += kThreads) counts[i] = 0;
+    const int warps = ALONE ? (int)((rows + kRowsPerWarp - 1) / kRowsPerWarp) : WARPS;         // that have rows
+    for (int i = threadIdx.x; i < warps * stride; i += kThreads) counts[i] = 0;
     if (!ALONE)
         for (int q = threadIdx.x; q < width; q += kThreads) starts[q] = totals[q];
     unsigned same[kKeys];
     match_groups(g, bits, same);
     __syncthreads();
-    int* const mine = counts + warp * width;
+    int* const mine = counts + warp * stride;
 #pragma unroll
     for (int i = 0; i < kKeys; ++i) {
         const int before = g[i] >= 0 ? mine[g[i]] : 0, ahead = __popc(same[i] & ((1u << lane) - 1u));
@@ -184,15 +193,29 @@ k_group_place(const K* __restrict__ keys, Digit d, long long rows, int groups, i
         __syncwarp();
     }
     __syncthreads();
-    for (int q = warp; q < width; q += kWarps) {
-        int all;
-        const int before = warps_before(lane < warps ? counts[lane * width + q] : 0, all);
-        if (lane < warps) counts[lane * width + q] = before;
-        if (lane == 0) here[q] = all;
+    if (DIGIT && width >= kThreads / 4) {
+        // a thread per group, whose counts it reads one after the other (a warp for each waits 16 times for its shuffles at 512)
+        for (int q = threadIdx.x; q < width; q += kThreads) {
+            int all = 0;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) {
+                const int count = w < warps ? counts[w * stride + q] : 0;
+                if (w < warps) counts[w * stride + q] = all;
+                all += count;
+            }
+            here[q] = all;
+        }
+    } else {
+        for (int q = warp; q < width; q += WARPS) {
+            int all;
+            const int before = warps_before(lane < warps ? counts[lane * stride + q] : 0, all);
+            if (lane < warps) counts[lane * stride + q] = before;
+            if (lane == 0) here[q] = all;
+        }
     }
     __syncthreads();
-    exclusive_starts(here, width);
-    if (!ALONE) exclusive_starts(starts, width);
+    exclusive_starts<WARPS>(here, width);
+    if (!ALONE) exclusive_starts<WARPS>(starts, width);
     if (!DIGIT && blockIdx.x == 0)
         for (int q = threadIdx.x; q < width; q += kThreads) offsets[q] = starts[q];
 #pragma unroll
@@ -205,38 +228,50 @@ k_group_place(const K* __restrict__ keys, Digit d, long long rows, int groups, i
         __syncthreads();
     }
     const int count = (int)min((long long)kRowsPerCta, rows - first);
+    int32_t row[kKeys];
+    int to[kKeys];
 #pragma unroll
     for (int j = 0; j < kKeys; ++j) {
         const int i = threadIdx.x + j * kThreads, v = i < count ? sorted[i] : 0;
-        if (i >= count) continue;
-        const int to = (ALONE ? 0 : starts[v >> 13]) + i;
-        int32_t row = (int32_t)(first + (v & (kRowsPerCta - 1)));
-        if (DIGIT && d.from) row = d.from[row];
-        order[to] = row;
-        if (DIGIT && d.sorted_keys) d.sorted_keys[to] = group_of(keys[row], d.vocabulary);
+        to[j] = i < count ? (ALONE ? 0 : starts[v >> 13]) + i : -1;
+        row[j] = (int32_t)(first + (v & (kRowsPerCta - 1)));
+    }
+    if (DIGIT && d.from) {
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j)
+            if (to[j] >= 0) row[j] = d.from[row[j]];
+    }
+#pragma unroll
+    for (int j = 0; j < kKeys; ++j)
+        if (to[j] >= 0) order[to[j]] = row[j];
+    if (DIGIT && d.sorted_keys) {
+        K key[kKeys];
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j) key[j] = to[j] >= 0 ? keys[row[j]] : (K)0;
+#pragma unroll
+        for (int j = 0; j < kKeys; ++j)
+            if (to[j] >= 0) d.sorted_keys[to[j]] = group_of(key[j], d.vocabulary);
     }
 }
 
-constexpr int place_smem(int width) { return ((kWarps + 2) * width + kRowsPerCta) * 4; }
-
 // one stable pass: counts, their sums over the CTAs, places; a launch alone where one CTA takes all rows
-template <typename K, bool DIGIT>
+template <typename K, bool DIGIT, int WARPS>
 int sort_pass(const K* keys, const Digit& d, long long rows, int groups, int32_t* order, int32_t* offsets, int32_t* scratch, cudaStream_t stream) {
-    const int width = groups + 1, ctas = ceil_div(rows, kRowsPerCta);
-    const int smem = place_smem(width), bits = 32 - __builtin_clz(groups);
-    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, true, DIGIT>, place_smem(FMB_MAX_GROUPS + 1)));
-    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, false, DIGIT>, place_smem(FMB_MAX_GROUPS + 1)));
+    const int width = groups + 1, ctas = ceil_div(rows, WARPS * kRowsPerWarp);
+    const int smem = place_smem(width, WARPS), most = place_smem(FMB_MAX_GROUPS + 1, WARPS), bits = 32 - __builtin_clz(groups);
     if (ctas <= 1) {
-        k_group_place<K, true, DIGIT><<<1, kThreads, smem, stream>>>(keys, d, rows, groups, bits, nullptr, nullptr, order, offsets);
+        FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, true, DIGIT, WARPS>, most));
+        k_group_place<K, true, DIGIT, WARPS><<<1, 32 * WARPS, smem, stream>>>(keys, d, rows, groups, bits, nullptr, nullptr, order, offsets);
         FMB_LAUNCH_CHECK();
         return FMB_OK;
     }
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, false, DIGIT, WARPS>, most));
     int32_t* const totals = scratch + (long long)ctas * width;
-    k_group_count<K, DIGIT><<<ctas, kThreads, 0, stream>>>(keys, d, rows, groups, scratch);
+    k_group_count<K, DIGIT, WARPS><<<ctas, 32 * WARPS, 0, stream>>>(keys, d, rows, groups, scratch);
     FMB_LAUNCH_CHECK();
     k_group_scan<<<ceil_div(width, 32), 1024, 0, stream>>>(scratch, totals, ctas, width);
     FMB_LAUNCH_CHECK();
-    k_group_place<K, false, DIGIT><<<ctas, kThreads, smem, stream>>>(keys, d, rows, groups, bits, scratch, totals, order, offsets);
+    k_group_place<K, false, DIGIT, WARPS><<<ctas, 32 * WARPS, smem, stream>>>(keys, d, rows, groups, bits, scratch, totals, order, offsets);
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
@@ -244,15 +279,26 @@ int sort_pass(const K* keys, const Digit& d, long long rows, int groups, int32_t
 // Tokens by value: one pass where the table holds every value, else one over the lower half of their bits and one over the upper half,
 // which keeps the order that the first has made.
 int lower_bits(int vocabulary) { return vocabulary <= FMB_MAX_GROUPS ? 0 : (33 - __builtin_clz(vocabulary)) / 2; }
-long long table_size(long long rows, int width) { return rows <= kRowsPerCta ? 0 : ((rows + kRowsPerCta - 1) / kRowsPerCta + 1) * width; }
+// CTAs of eight warps, while that spreads the rows over more SMs: below, one CTA has them all without a second launch
+int warps_of(long long rows) { return rows > kRowsPerCta && rows <= 148ll * 2 * kFewWarps * kRowsPerWarp ? kFewWarps : kWarps; }
+long long table_size(long long rows, int width) {
+    const long long per_cta = warps_of(rows) * kRowsPerWarp;
+    return rows <= per_cta ? 0 : ((rows + per_cta - 1) / per_cta + 1) * width;
+}
+
+template <typename K>
+int sort_digit(const K* keys, const Digit& d, long long rows, int groups, int32_t* order, int32_t* scratch, cudaStream_t stream) {
+    return warps_of(rows) == kWarps ? sort_pass<K, true, kWarps>(keys, d, rows, groups, order, nullptr, scratch, stream)
+                                    : sort_pass<K, true, kFewWarps>(keys, d, rows, groups, order, nullptr, scratch, stream);
+}
 
 template <typename K>
 int sort_tokens(const K* tokens, long long rows, int vocabulary, int32_t* order, int32_t* keys, int32_t* scratch, cudaStream_t stream) {
     const int low = lower_bits(vocabulary);
-    if (low == 0) return sort_pass<K, true>(tokens, Digit{nullptr, keys, vocabulary, 0, -1}, rows, vocabulary, order, nullptr, scratch, stream);
+    if (low == 0) return sort_digit(tokens, Digit{nullptr, keys, vocabulary, 0, -1}, rows, vocabulary, order, scratch, stream);
     int32_t* const table = scratch + rows;
-    const int rc = sort_pass<K, true>(tokens, Digit{nullptr, nullptr, vocabulary, 0, (1 << low) - 1}, rows, (1 << low) - 1, scratch, nullptr, table, stream);
-    return rc ? rc : sort_pass<K, true>(tokens, Digit{scratch, keys, vocabulary, low, -1}, rows, vocabulary >> low, order, nullptr, table, stream);
+    const int rc = sort_digit(tokens, Digit{nullptr, nullptr, vocabulary, 0, (1 << low) - 1}, rows, (1 << low) - 1, scratch, table, stream);
+    return rc ? rc : sort_digit(tokens, Digit{scratch, keys, vocabulary, low, -1}, rows, vocabulary >> low, order, table, stream);
 }
 
 }  // namespace
@@ -274,8 +320,8 @@ extern "C" FMB_API int fmb_group_rows(const void* keys, int key_bytes, long long
     FMB_REQUIRE(scratch || fmb_group_rows_scratch(rows, groups) == 0, "fmb_group_rows: null scratch");
     FMB_REQUIRE(key_bytes == 4 || key_bytes == 8, "fmb_group_rows: keys of 4 or 8 bytes");
     if (key_bytes == 4)
-        return sort_pass<int32_t, false>((const int32_t*)keys, Digit{}, rows, groups, order, offsets, scratch, (cudaStream_t)stream);
-    return sort_pass<long long, false>((const long long*)keys, Digit{}, rows, groups, order, offsets, scratch, (cudaStream_t)stream);
+        return sort_pass<int32_t, false, kWarps>((const int32_t*)keys, Digit{}, rows, groups, order, offsets, scratch, (cudaStream_t)stream);
+    return sort_pass<long long, false, kWarps>((const long long*)keys, Digit{}, rows, groups, order, offsets, scratch, (cudaStream_t)stream);
 }
 
 extern "C" FMB_API long long fmb_sort_tokens_scratch(long long rows, int vocabulary) {
