@@ -8,9 +8,10 @@
 // a counter. A unit of the second kind waits for the first ones of its expert only; those were handed out before it, so they
 // are done or under way and the wait ends, however few CTAs run at a time.
 //
-// A unit is [64 columns] x [8 or 16 rows] over the whole depth, which the eight warps of a CTA share. Weights go from memory to the
-// registers that the tensor core reads them from: a lane loads eight neighbouring columns of as many rows of the matrix as a step has for
-// it, and two permutes make pairs along the depth of them. Columns of the matrix are the MMA's rows, tokens its columns, of which it
+// A unit is [64 columns] x [8 or 16 rows] over the whole depth, which the eight warps of a CTA share. Each warp has a ring of stages in
+// shared memory that asynchronous copies fill, without a barrier between warps; the ring does not run dry between units, since the first
+// stages of the next one are asked for before the results of the last are taken out and before a wait for what they multiply. Two
+// permutes make pairs along the depth of two rows of the matrix. Columns of the matrix are the MMA's rows, tokens its columns, of which it
 // has eight: mma.sync suits that shape (tcgen05 would take 128 columns from shared memory for the same bytes).
 //
 // Numbers: 16-bit products are exact in fp32. What passes between the products, h, is not rounded to the type of the weights: it is a pair of
@@ -116,36 +117,41 @@ k_route(fmb_route_t a, int wide, int rows) {
     }
     // (their shared memory lives until it has been read)
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank != 0 || threadIdx.x >= 32) return;
-    const int lane = threadIdx.x;
-    unsigned taken = 0;                          // of this lane's experts lane, lane + 32, ...
-    float first = 0.0f, total = 0.0f, mine = 0.0f;
-    int chosen = 0;
-    for (int j = 0; j < a.top; ++j) {
-        unsigned long long best = 0;             // logit, then the lowest number
-        for (int i = 0; i * 32 + lane < a.experts; ++i)
-            if (!(taken >> i & 1)) best = max(best, (unsigned long long)ordered(logits[i * 32 + lane]) << 32 | (0xffffffffu - (i * 32 + lane)));
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-        const int e = (int)(0xffffffffu - (uint32_t)best);
-        if ((e & 31) == lane) taken |= 1u << (e >> 5);
-        const float l = logits[e];
-        if (j == 0) first = l;
-        const float p = expf(l - first);
-        if (a.normalise) total += p;
-        if (lane == j) {
-            chosen = e;
-            mine = p;
+    if (rank != 0) return;
+    // An expert's place is the number of those before it (larger logit, or the same and a lower number): each thread counts for its own,
+    // which takes one wait where choosing one after the other takes one each. Numbers are made unlike by the expert's.
+    __shared__ unsigned long long order[FMB_MAX_GROUPS + 1];
+    __shared__ float best[FMB_MAX_TOP], warp_total[kWarps];
+    for (int e = threadIdx.x; e <= a.experts; e += kThreads)
+        order[e] = e < a.experts ? (unsigned long long)ordered(logits[e]) << 32 | (0xffffffffu - e) : 0;
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.experts; e += kThreads) {
+        const unsigned long long mine = order[e];
+        int before = 0;
+#pragma unroll 4
+        for (int f = 0; f < a.experts; f += 2) {
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(order + f);
+            before += (two.x > mine) + (two.y > mine);
+        }
+        if (before < a.top) {
+            best[before] = logits[e];
+            a.chosen[token * (long long)a.top + before] = e;
         }
     }
-    if (!a.normalise) {
-        for (int e = lane; e < a.experts; e += 32) total += expf(logits[e] - first);
+    __syncthreads();
+    const float first = best[0];
+    float total = 0.0f;
+    if (a.normalise) {
+        for (int j = 0; j < a.top; ++j) total += expf(best[j] - first);
+    } else {
+        for (int e = threadIdx.x; e < a.experts; e += kThreads) total += expf(logits[e] - first);
         total = warp_sum(total);
+        if ((threadIdx.x & 31) == 0) warp_total[threadIdx.x >> 5] = total;
+        __syncthreads();
+        total = 0.0f;
+        for (int w = 0; w < kWarps; ++w) total += warp_total[w];
     }
-    if (lane < a.top) {
-        a.chosen[token * (long long)a.top + lane] = chosen;
-        a.weights[token * (long long)a.top + lane] = mine / total;
-    }
+    if (threadIdx.x < a.top) a.weights[token * (long long)a.top + threadIdx.x] = expf(best[threadIdx.x] - first) / total;
 }
 
 // --------------------------------------------------------------------------------------------------------------- layer
@@ -172,283 +178,330 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
 }
 
-// What a lane brings of a step: kRows neighbouring rows of the matrix, eight columns of each. A step has 4 kRows rows.
-template <typename T> struct Step { static constexpr int kRows = sizeof(T) == 4 ? 4 : 8, kDepth = 4 * kRows, kWords = sizeof(T) == 4 ? 8 : 4; };
+// What a warp brings at a time, a stage: kDepth rows of the unit's 64 columns and as much of its rows of x or h. For the product a lane has
+// kRows neighbouring rows of the depth and eight columns, which are kPieces times 16 bytes, and of block n of the unit's rows one row, kRows
+// values of it. Stages lie in shared memory, a ring for each warp, so that no registers wait for them. Copies go along the rows of the
+// matrix: lanes that copy what lies side by side (64 bytes that went to lanes four apart came at 3.9 TB/s, and so at 6.9). Rows
+// that start at no multiple of 16 bytes (not WIDE) come as the pieces of 16 bytes that they lie in, for each half of the columns one
+// more than it fills.
+template <typename T, bool WIDE> struct Stage {
+    static constexpr int kRows = sizeof(T) == 4 ? 2 : 4, kDepth = 4 * kRows, kPieces = sizeof(T) / 2;
+    static constexpr int kHalf = WIDE ? 4 * kPieces : 4 * kPieces + 1;         // pieces of a half
+    static constexpr int kMatrixBytes = kDepth * 2 * kHalf * 16, kBytes = kMatrixBytes + 2 * 32 * 16;
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load_weights(const T* __restrict__ w, long long stride, int k, int depth, int live, uint32_t (&v)[Step<T>::kRows][Step<T>::kWords]) {
-#pragma unroll
-    for (int j = 0; j < Step<T>::kRows; ++j) {
-        const T* const at = w + (long long)j * stride;
-        const int here = k + j < depth ? live : 0;
-        if (WIDE) {
-            // (rows and columns by whole packs)
-#pragma unroll
-            for (int i = 0; i < Step<T>::kWords; i += 4) {
-                uint4 in = make_uint4(0, 0, 0, 0);
-                if (here > 0) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-                                           : "=r"(in.x), "=r"(in.y), "=r"(in.z), "=r"(in.w) : "l"(reinterpret_cast<const uint4*>(at) + i / 4));
-                v[j][i] = in.x; v[j][i + 1] = in.y; v[j][i + 2] = in.z; v[j][i + 3] = in.w;
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < Step<T>::kWords; ++i) {
-                if constexpr (sizeof(T) == 4) {
-                    v[j][i] = i < here ? __float_as_uint(__ldg((const float*)at + i)) : 0u;
-                } else {
-                    const uint32_t low = 2 * i < here ? __ldg((const uint16_t*)at + 2 * i) : 0u, high = 2 * i + 1 < here ? __ldg((const uint16_t*)at + 2 * i + 1) : 0u;
-                    v[j][i] = low | high << 16;
-                }
-            }
-        }
-    }
-}
-
-// A unit's rows for a step, of which a lane has Step::kRows of the depth, of one row per eight. Rows of x:
-template <typename T> struct RowsOfX {
-    static constexpr int kRegs = 4;
-    uint32_t v[kRegs];
-
-    __device__ __forceinline__ void load(const T* __restrict__ row, int k, int depth, bool wide) {
-        constexpr int kRows = Step<T>::kRows;
-        const int live = row ? depth - k : 0;
-        if (wide && live >= kRows) {
-            const uint4 in = __ldg(reinterpret_cast<const uint4*>(row + k));
-            v[0] = in.x; v[1] = in.y; v[2] = in.z; v[3] = in.w;
-        } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = i < live ? __float_as_uint(__ldg((const float*)row + k + i)) : 0u;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t low = 2 * i < live ? __ldg((const uint16_t*)row + k + 2 * i) : 0u;
-                const uint32_t high = 2 * i + 1 < live ? __ldg((const uint16_t*)row + k + 2 * i + 1) : 0u;
-                v[i] = low | high << 16;
-            }
-        }
+    // Where piece c of row kRows quad + j lies: so that the eight lanes that read at a time, of the four quads and pieces of two lanes' columns,
+    // find them on different banks.
+    __device__ static __forceinline__ int place(int quad, int j, int c) {
+        if (WIDE) return (quad * kRows + j) * 2 * kHalf + (c ^ (sizeof(T) == 2 ? 2 * quad : (quad & 1) * 4 + (quad >> 1)));
+        return (j * 4 + quad) * 2 * kHalf + c;
     }
 };
+constexpr int kStages = 3;
 
-// rows of h, which the other CTAs of this launch have written (so never by way of L1): for bfloat16 weights two bfloat16 a value, of
-// which the upper halves of eight values lie before their lower ones; else float32
-template <typename T> struct RowsOfH {
-    static constexpr int kRegs = Step<T>::kRows;
-    uint32_t v[kRegs];
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-    __device__ __forceinline__ void load(const float* __restrict__ row, int k, int, bool) {
-#pragma unroll
-        for (int i = 0; i < kRegs; i += 4) {
-            const uint4 in = row ? __ldcg(reinterpret_cast<const uint4*>(row + k + i)) : make_uint4(0, 0, 0, 0);
-            v[i] = in.x; v[i + 1] = in.y; v[i + 2] = in.z; v[i + 3] = in.w;
-        }
-    }
-};
-
-// acc[i][n]: columns 2 i and 2 i + 1 of the lanes' eight, rows of block n
-template <typename T, int NB>
-__device__ __forceinline__ void multiply_x(float (&acc)[4][NB][4], const uint32_t (&w)[Step<T>::kRows][Step<T>::kWords], const RowsOfX<T> (&x)[NB]) {
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t a[4] = {__byte_perm(w[4 * s][i], w[4 * s + 1][i], 0x5410), __byte_perm(w[4 * s][i], w[4 * s + 1][i], 0x7632),
-                                       __byte_perm(w[4 * s + 2][i], w[4 * s + 3][i], 0x5410), __byte_perm(w[4 * s + 2][i], w[4 * s + 3][i], 0x7632)};
-#pragma unroll
-                for (int n = 0; n < NB; ++n) mma_16(acc[i][n], a, x[n].v[2 * s], x[n].v[2 * s + 1], T());
-            }
-    } else {
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-            uint32_t b[NB][2][2];
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int q = 0; q < 2; ++q) split_tf32(__uint_as_float(x[n].v[2 * s + q]), b[n][0][q], b[n][1][q]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int q = 0; q < 4; ++q) split_tf32(__uint_as_float(w[2 * s + q / 2][2 * i + q % 2]), hi[q], lo[q]);
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    mma_tf32(acc[i][n], hi, b[n][1][0], b[n][1][1]);
-                    mma_tf32(acc[i][n], lo, b[n][0][0], b[n][0][1]);
-                    mma_tf32(acc[i][n], hi, b[n][0][0], b[n][0][1]);
-                }
-            }
-        }
-    }
+// 16 or 8 bytes, of which the first `bytes` are read and the others zero
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
+__device__ __forceinline__ void copy_8(uint32_t to, const void* from, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+// whole ones
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copy_8(uint32_t to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
-template <typename T, int NB>
-__device__ __forceinline__ void multiply_h(float (&acc)[4][NB][4], const uint32_t (&w)[Step<T>::kRows][Step<T>::kWords], const RowsOfH<T> (&h)[NB]) {
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t a[4] = {__byte_perm(w[4 * s][i], w[4 * s + 1][i], 0x5410), __byte_perm(w[4 * s][i], w[4 * s + 1][i], 0x7632),
-                                       __byte_perm(w[4 * s + 2][i], w[4 * s + 3][i], 0x5410), __byte_perm(w[4 * s + 2][i], w[4 * s + 3][i], 0x7632)};
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    mma_16(acc[i][n], a, h[n].v[4 + 2 * s], h[n].v[4 + 2 * s + 1], T());
-                    mma_16(acc[i][n], a, h[n].v[2 * s], h[n].v[2 * s + 1], T());
-                }
-            }
-    } else if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            uint32_t b[NB][2][2];
-#pragma unroll
-            for (int n = 0; n < NB; ++n)
-#pragma unroll
-                for (int q = 0; q < 2; ++q) split_tf32(__uint_as_float(h[n].v[2 * s + q]), b[n][0][q], b[n][1][q]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t a[4];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&w[2 * s + q][i]));
-                    a[2 * q] = __float_as_uint(two.x);
-                    a[2 * q + 1] = __float_as_uint(two.y);
-                }
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    mma_tf32(acc[i][n], a, b[n][1][0], b[n][1][1]);
-                    mma_tf32(acc[i][n], a, b[n][0][0], b[n][0][1]);
-                }
-            }
-        }
-    } else {
-        RowsOfX<T> x[NB];
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[n].v[i] = h[n].v[i];
-        multiply_x<T, NB>(acc, w, x);
-    }
+__device__ __forceinline__ uint4 load_16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ uint2 load_8(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
 }
 
 struct Layer {
     fmb_experts_t a;
-    int up_wide, down_wide, x_wide;
     int up_units, down_units;                    // of an expert
+    uint32_t up_inverse, down_inverse;           // 2^32 over them, rounded up
     long long h_stride, part_stride;             // floats of a row: the inner width, or the width, filled up to whole units
-    int32_t* control;                            // next unit, CTAs that gave up; units of each expert that are done; experts of each column unit
+    int32_t* control;                            // next unit; then of each active expert the units that are done, of each column unit the experts
+    int32_t* lists;                              // number of active experts, total of pairs; active[], first[], pair[]
     float* h;                                    // [tokens * top]
     float* parts;
+    void* x;                                     // rows that copies of 8 bytes take: the caller's, or copies of them
+    long long x_stride;
 };
-
-// rows a reduction keeps of a column: chosen so that the lanes' stores fall on different banks
-template <int NB> struct Turn { static constexpr int kStride = NB == 1 ? 8 : 24; };
-
-// The sums over the depth of 64 columns and 8 NB rows, left in turn[column][row] by all warps: columns 8 g + j at place 8 j + g.
-template <typename T, bool WIDE, int NB, bool UP>
-__device__ __forceinline__ void product(const Layer& p, const T* __restrict__ w, long long stride, int live, int depth, const void* const (&rows)[NB], float* turn) {
-    constexpr int kRows = Step<T>::kRows, kDepth = Step<T>::kDepth;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3;
-    using Rows = typename std::conditional<UP, RowsOfX<T>, RowsOfH<T>>::type;
-    using From = typename std::conditional<UP, T, float>::type;
-    float acc[4][NB][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) acc[i][n][q] = 0.0f;
-    uint32_t v[2][kRows][Step<T>::kWords];
-    Rows x[2][NB];
-    const int steps = (depth + kDepth - 1) / kDepth;
-    auto bring = [&](int step, int slot) {
-        const int k = step * kDepth + kRows * quad;
-        load_weights<T, WIDE>(w + k * stride, stride, k, step < steps ? depth : 0, live, v[slot]);
-#pragma unroll
-        for (int n = 0; n < NB; ++n) x[slot][n].load(step < steps ? (const From*)rows[n] : nullptr, k, depth, p.x_wide);
-    };
-    bring(warp, 0);
-#pragma unroll 2
-    for (int step = warp, slot = 0; step < steps; step += kWarps, slot ^= 1) {
-        bring(step + kWarps, slot ^ 1);
-        if constexpr (UP) multiply_x<T, NB>(acc, v[slot], x[slot]);
-        else multiply_h<T, NB>(acc, v[slot], x[slot]);
-    }
-    float* const mine = turn + warp * kUnit * Turn<NB>::kStride;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int n = 0; n < NB; ++n)
-#pragma unroll
-            for (int b = 0; b < 2; ++b)
-                *reinterpret_cast<float2*>(mine + ((2 * i + b) * 8 + (lane >> 2)) * Turn<NB>::kStride + 8 * n + 2 * quad) =
-                    make_float2(acc[i][n][2 * b], acc[i][n][2 * b + 1]);
-}
-
-template <int NB>
-__device__ __forceinline__ float sum_of(const float* turn, int place, int row) {
-    float sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += turn[(w * kUnit + place) * Turn<NB>::kStride + row];
-    return sum;
-}
 
 constexpr int kMaxPairs = FMB_MAX_LAYER_TOKENS * FMB_MAX_TOP;
-constexpr int kTurnFloats = kWarps * kUnit * 24;
 
-template <typename T>
+template <typename T, bool WIDE>
 struct Smem {
-    float turn[kTurnFloats];
-    int pair[kMaxPairs];                         // pairs of token and choice, by expert
-    int start[FMB_MAX_GROUPS + 1];
-    int active[FMB_MAX_GROUPS];                  // experts that have pairs
-    int warp_total[2][kWarps];
-    int ticket[2], actives, flag;
+    alignas(16) uint8_t ring[kWarps][kStages][Stage<T, WIDE>::kBytes];
+    float turn[kWarps][kUnit][8];                // results of eight rows on their way out
+    uint16_t pair[kMaxPairs];                    // pairs of token and choice, by expert
+    uint8_t token[kMaxPairs];
+    uint16_t active[FMB_MAX_GROUPS], first[FMB_MAX_GROUPS + 1];
+    int ticket, last[2];                         // last: of two units in turn, the columns that are complete with it, or -1
+    volatile int gave_up;
 };
 
-// Which pairs belong to which expert, and which experts have any. Pairs of one expert stand in any order: their results do not
-// depend on it.
-template <typename T>
-__device__ __forceinline__ void list_pairs(const Layer& p, Smem<T>& s) {
-    const int experts = p.a.experts, pairs = p.a.tokens * p.a.top, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int e = threadIdx.x; e <= experts; e += kThreads) s.start[e] = 0;
-    __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += kThreads) {
-        const int e = __ldg(p.a.chosen + i);
-        if (e >= 0 && e < experts) atomicAdd(s.start + e, 1);
+struct Unit {
+    int up, number, expert, block, first, end;
+};
+
+template <typename S>
+__device__ __forceinline__ Unit unit_of(const Layer& p, const S& s, int ticket, int ups) {
+    Unit u;
+    u.up = ticket < ups;
+    const int t = u.up ? ticket : ticket - ups, per = u.up ? p.up_units : p.down_units;
+    u.number = per == 1 ? t : (int)__umulhi((uint32_t)t, u.up ? p.up_inverse : p.down_inverse);
+    while (u.number * per > t) --u.number;       // (too large by one where the product is beyond 2^32)
+    u.block = t - u.number * per;
+    u.expert = s.active[u.number];
+    u.first = s.first[u.number];
+    u.end = s.first[u.number + 1];
+    return u;
+}
+
+// The matrix of a unit: 32 columns from its first row on, and 32 more `second` bytes behind them; how many bytes of each there are.
+struct Matrix {
+    const char* at;
+    long long second;
+    int stride, first_bytes, second_bytes, depth;                              // stride: bytes
+    // WIDE: where this lane's copies of the first stage begin, and whether there is something (Stage::kRows rows at once)
+    const char* lane_at;
+    bool lane_there;
+};
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ Matrix matrix_of(const Layer& p, const Unit& u) {
+    const fmb_experts_t& a = p.a;
+    constexpr int kSize = sizeof(T);
+    Matrix m;
+    auto bytes = [](int columns) { return max(0, min(columns, 32)) * kSize; };
+    if (u.up) {
+        m.at = (const char*)((const T*)a.w_up + u.expert * a.up_group_stride + 32 * u.block);
+        m.second = (long long)a.inner * kSize;
+        m.first_bytes = m.second_bytes = bytes(a.inner - 32 * u.block);
+        m.stride = (int)a.up_row_stride * kSize;
+        m.depth = a.width;
+    } else {
+        m.at = (const char*)((const T*)a.w_down + u.expert * a.down_group_stride + kUnit * u.block);
+        m.second = 32 * kSize;
+        m.first_bytes = bytes(a.width - kUnit * u.block);
+        m.second_bytes = bytes(a.width - kUnit * u.block - 32);
+        m.stride = (int)a.down_row_stride * kSize;
+        m.depth = a.inner;
     }
-    __syncthreads();
-    const int per = (experts + kThreads - 1) / kThreads, from = min(experts, (int)threadIdx.x * per), to = min(experts, from + per);
-    int sum = 0, some = 0;
-    for (int e = from; e < to; ++e) {
-        sum += s.start[e];
-        some += s.start[e] > 0;
+    if (WIDE) {
+        constexpr int kHalf = Stage<T, WIDE>::kHalf;
+        const int lane = threadIdx.x & 31, row = lane / (2 * kHalf), half = lane / kHalf & 1, piece = lane % kHalf;
+        m.lane_at = m.at + (long long)m.stride * row + (half ? m.second : 0) + piece * 16;
+        m.lane_there = piece * 16 < (half ? m.second_bytes : m.first_bytes);
     }
-    int sums = sum, somes = some;
+    return m;
+}
+
+// A lane's rows of the unit, up to two, from its first value of the first stage on, and whether they are rows of x
+struct Rows {
+    const char* at[2];
+    bool up;
+};
+
+// (Pieces of which a byte belongs to the row are mapped memory, since no piece crosses a page. What they hold beside it, and what is left
+// in shared memory where nothing is copied, goes into columns or rows that are not there, which nothing reads.)
+template <typename T, bool WIDE>
+__device__ __forceinline__ void bring_matrix(const Matrix& m, int step, uint32_t slot) {
+    using S = Stage<T, WIDE>;
+    const int lane = threadIdx.x & 31, live = m.depth - step * S::kDepth;
+    const long long offset = (long long)m.stride * (step * S::kDepth);
+    if constexpr (WIDE) {
+        // a copy takes kRows rows, those of a quad
+        constexpr int kOfRow = 2 * S::kHalf;
+        static_assert(kOfRow * S::kRows == 32, "a copy is kRows rows");
+        const char* const at = m.lane_at + offset;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int a = __shfl_up_sync(0xffffffffu, sums, o), b = __shfl_up_sync(0xffffffffu, somes, o);
-        if (lane >= o) sums += a, somes += b;
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t to = slot + S::place(i, lane / kOfRow, lane % kOfRow) * 16;
+            const char* const from = at + (long long)m.stride * (i * S::kRows);
+            if (live >= S::kDepth) {
+                if (m.lane_there) copy_16(to, from);
+            } else {
+                const bool here = m.lane_there && i * S::kRows + lane / kOfRow < live;
+                copy_16(to, here ? from : (const char*)((uintptr_t)m.at & ~(uintptr_t)15), here ? 16 : 0);
+            }
+        }
+    } else {
+        // the pieces that a half fills, kRows rows at a time as above, and then the one more of each row
+        constexpr int kOfRow = 8 * S::kPieces;
+        auto bring = [&](int r, int half, int piece) {
+            const char* const row = m.at + offset + (long long)m.stride * r + (half ? m.second : 0);
+            const int shift = (int)((uintptr_t)row & 15), bytes = half ? m.second_bytes : m.first_bytes;
+            const bool here = r < live && bytes > 0 && piece * 16 < shift + bytes;
+            copy_16(slot + S::place(r / S::kRows, r % S::kRows, half * S::kHalf + piece) * 16,
+                    here ? row - shift + piece * 16 : (const char*)((uintptr_t)m.at & ~(uintptr_t)15), here ? 16 : 0);
+        };
+#pragma unroll
+        for (int i = 0; i < 4; ++i) bring(i * S::kRows + lane / kOfRow, lane % kOfRow / (kOfRow / 2), lane % (kOfRow / 2));
+        if (lane < 2 * S::kDepth) bring(lane >> 1, lane & 1, S::kHalf - 1);
     }
-    if (lane == 31) s.warp_total[0][warp] = sums, s.warp_total[1][warp] = somes;
-    __syncthreads();
-    int before = sums - sum, number = somes - some;
-    for (int w = 0; w < warp; ++w) before += s.warp_total[0][w], number += s.warp_total[1][w];
-    for (int e = from; e < to; ++e) {
-        const int count = s.start[e];
-        if (count > 0) s.active[number++] = e;
-        before += count;
-        s.start[e] = before;                     // the end: places are taken from there downwards
+}
+
+// rows of x by kRows values, 8 bytes; of h, which is kept as float32 or, for bfloat16 weights, as four upper halves and then four lower ones
+template <typename T, bool WIDE, int NB>
+__device__ __forceinline__ void bring_rows(const Layer& p, const Rows& r, int depth, int step, uint32_t slot) {
+    using S = Stage<T, WIDE>;
+    const int lane = threadIdx.x & 31;
+    const uint32_t to = slot + S::kMatrixBytes + lane * 16;
+    const int offset = step * S::kDepth * (r.up ? (int)sizeof(T) : 4);
+    if ((step + 1) * S::kDepth <= depth) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            if (!r.at[n]) continue;
+            if (sizeof(T) == 2 && !r.up) copy_16(to + n * 512, r.at[n] + offset);
+            else copy_8(to + n * 512, r.at[n] + offset);
+        }
+        return;
     }
-    if (threadIdx.x == kThreads - 1) {
-        s.start[experts] = before;
-        s.actives = number;
+    const int most = depth - step * S::kDepth - S::kRows * (lane & 3);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+        const int live = r.at[n] ? max(0, min(S::kRows, most)) : 0;
+        const char* const from = live ? r.at[n] + offset : (const char*)p.h;
+        if (r.up) copy_8(to + n * 512, from, live * (int)sizeof(T));
+        else if (sizeof(T) == 2) copy_16(to + n * 512, from, live ? 16 : 0);
+        else copy_8(to + n * 512, from, live ? 8 : 0);
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < pairs; i += kThreads) {
-        const int e = __ldg(p.a.chosen + i);
-        if (e >= 0 && e < experts) s.pair[atomicSub(s.start + e, 1) - 1] = i;
+}
+
+// a row's eight values from the pieces they lie in: first by whole words, then by the half
+template <typename T>
+__device__ __forceinline__ void align_row(uint32_t from, const uint32_t (&v)[sizeof(T) * 2 + 4], uint32_t (&out)[sizeof(T) * 2]) {
+    constexpr int kWords = sizeof(T) * 2;
+    uint32_t a[kWords + 2], b[kWords + 1];
+#pragma unroll
+    for (int i = 0; i < kWords + 2; ++i) a[i] = from & 8 ? v[i + 2 < kWords + 4 ? i + 2 : i] : v[i];
+#pragma unroll
+    for (int i = 0; i < kWords + 1; ++i) b[i] = from & 4 ? a[i + 1] : a[i];
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) out[i] = sizeof(T) == 2 ? __funnelshift_r(b[i], b[i + 1], (from & 2) * 8) : b[i];
+}
+
+// The stage's product. Matrix columns are the MMA's rows, in the order of the lanes' eight: acc[i][n] has columns 2 i and 2 i + 1.
+template <typename T, bool WIDE, int NB, bool UP>
+__device__ __forceinline__ void multiply(float (&acc)[4][NB][4], const Matrix& m, int step, uint32_t slot) {
+    using S = Stage<T, WIDE>;
+    constexpr int kWords = sizeof(T) * 2;
+    const int lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
+    uint32_t w[S::kRows][kWords];
+#pragma unroll
+    for (int j = 0; j < S::kRows; ++j) {
+        if (WIDE) {
+#pragma unroll
+            for (int i = 0; i < S::kPieces; ++i) {
+                const uint4 v = load_16(slot + S::place(quad, j, g * S::kPieces + i) * 16);
+                w[j][4 * i] = v.x; w[j][4 * i + 1] = v.y; w[j][4 * i + 2] = v.z; w[j][4 * i + 3] = v.w;
+            }
+        } else {
+            uint32_t raw[kWords + 4];
+#pragma unroll
+            for (int i = 0; i <= S::kPieces; ++i) {
+                const uint4 v = load_16(slot + S::place(quad, j, (g >> 2) * S::kHalf + (g & 3) * S::kPieces + i) * 16);
+                raw[4 * i] = v.x; raw[4 * i + 1] = v.y; raw[4 * i + 2] = v.z; raw[4 * i + 3] = v.w;
+            }
+            align_row<T>(((uint32_t)(uintptr_t)m.at + (g >> 2 ? (uint32_t)m.second : 0u) + (uint32_t)m.stride * (step * S::kDepth + S::kRows * quad + j)) & 15, raw, w[j]);
+        }
     }
-    __syncthreads();
+    const uint32_t rows = slot + S::kMatrixBytes + lane * 16;
+    if constexpr (sizeof(T) == 2 && (UP || std::is_same<T, __nv_bfloat16>::value)) {
+        uint4 b[NB];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            if constexpr (UP) {
+                const uint2 two = load_8(rows + n * 512);
+                b[n] = make_uint4(two.x, two.y, 0, 0);
+            } else {
+                b[n] = load_16(rows + n * 512);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t a[4] = {__byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[0][i], w[1][i], 0x7632),
+                                   __byte_perm(w[2][i], w[3][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x7632)};
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                if (!UP) mma_16(acc[i][n], a, b[n].z, b[n].w, T());
+                mma_16(acc[i][n], a, b[n].x, b[n].y, T());
+            }
+        }
+    } else {
+        // float32 values as pairs of tf32, float16 weights as they are
+        float b[NB][S::kRows];
+#pragma unroll
+        for (int n = 0; n < NB; ++n) {
+            if constexpr (S::kRows == 4) {
+                const uint4 v = load_16(rows + n * 512);
+                b[n][0] = __uint_as_float(v.x); b[n][1] = __uint_as_float(v.y); b[n][2] = __uint_as_float(v.z); b[n][3] = __uint_as_float(v.w);
+            } else {
+                const uint2 v = load_8(rows + n * 512);
+                b[n][0] = __uint_as_float(v.x); b[n][1] = __uint_as_float(v.y);
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < S::kRows / 2; ++s) {
+            uint32_t hi[NB][2], lo[NB][2];
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) split_tf32(b[n][2 * s + q], hi[n][q], lo[n][q]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t a[4], rest[4];
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    if constexpr (sizeof(T) == 2) {
+                        const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&w[2 * s + q][i]));
+                        a[2 * q] = __float_as_uint(two.x);
+                        a[2 * q + 1] = __float_as_uint(two.y);
+                    } else {
+                        split_tf32(__uint_as_float(w[2 * s + q][2 * i]), a[2 * q], rest[2 * q]);
+                        split_tf32(__uint_as_float(w[2 * s + q][2 * i + 1]), a[2 * q + 1], rest[2 * q + 1]);
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    mma_tf32(acc[i][n], a, lo[n][0], lo[n][1]);
+                    if constexpr (sizeof(T) == 4) mma_tf32(acc[i][n], rest, hi[n][0], hi[n][1]);
+                    mma_tf32(acc[i][n], a, hi[n][0], hi[n][1]);
+                }
+            }
+        }
+    }
+}
+
+// The CTA's coming unit of the second matrix into the L2, so that memory does not wait for the first products with it: lines of
+// 128 bytes, up to 1,024 rows (at F = 1,024 the units of all CTAs are 38 MB).
+__device__ __forceinline__ void prefetch_unit(const Matrix& m) {
+    const int rows = min(m.depth, 1024);
+    for (int k = threadIdx.x; k < rows; k += kThreads) {
+        const char* const at = m.at + (long long)m.stride * k;
+        asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
+        const char* const last = at + (m.second_bytes > 0 ? m.second + m.second_bytes : m.first_bytes) - 1;
+        if (((uintptr_t)last ^ (uintptr_t)at) >> 7) asm volatile("prefetch.global.L2 [%0];" ::"l"(last));
+    }
+}
+
+// one more at a counter, behind what this CTA has written before its last barrier
+__device__ __forceinline__ void add_release(int32_t* at) { asm volatile("red.release.gpu.global.add.s32 [%0], 1;" ::"l"(at) : "memory"); }
+__device__ __forceinline__ int add_acquire_release(int32_t* at) {
+    int before;
+    asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(at) : "memory");
+    return before;
 }
 
 __device__ __forceinline__ int load_acquire(const int32_t* at) {
@@ -457,193 +510,412 @@ __device__ __forceinline__ int load_acquire(const int32_t* at) {
     return v;
 }
 
-// 32 gate columns and those they multiply, for `count` (up to 8 NB) pairs from `first` on
-template <typename T, bool WIDE, int NB>
-__device__ __forceinline__ void up_unit(const Layer& p, Smem<T>& s, int expert, int block, int first, int count) {
-    const fmb_experts_t& a = p.a;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c0 = 32 * block + 8 * (g & 3);
-    const void* rows[NB];
+// The state of a warp's ring between the units: the place of the next stage, and what has been asked for of the coming unit.
+struct Ring {
+    uint32_t base;
+    int place;
+
+    template <int BYTES> __device__ __forceinline__ uint32_t slot(int ahead) const {
+        const int at = place + ahead;
+        return base + (at >= kStages ? at - kStages : at) * BYTES;
+    }
+};
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ Rows rows_of(const Layer& p, const Smem<T, WIDE>& s, const Unit& u, int first) {
+    Rows r;
+    const int g = (threadIdx.x & 31) >> 2;
+    r.up = u.up;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) rows[n] = 8 * n + g < count ? (const T*)a.x + (s.pair[first + 8 * n + g] / a.top) * a.x_stride : nullptr;
-    const T* const w = (const T*)a.w_up + expert * a.up_group_stride + (g < 4 ? 0 : a.inner) + c0;
-    product<T, WIDE, NB, true>(p, w, a.up_row_stride, a.inner - c0, a.width, rows, s.turn);
-    __syncthreads();
-    // warp j: columns j, 8 + j, 16 + j, 24 + j of the 32; a lane has one of them and one row of each eight
-    const int column = 32 * block + 8 * (lane >> 3) + warp;
+    for (int n = 0; n < 2; ++n) {
+        const int at = first + 8 * n + g;
+        r.at[n] = nullptr;
+        if (at >= u.end) continue;
+        const int k = Stage<T, WIDE>::kRows * (threadIdx.x & 3);
+        r.at[n] = u.up ? (const char*)((const T*)p.x + s.token[at] * p.x_stride + k) : (const char*)(p.h + s.pair[at] * p.h_stride + k);
+    }
+    return r;
+}
+
+// one warp's first stages of a unit, the matrix or the rows or both; a group of copies each
+template <typename T, bool WIDE>
+__device__ __forceinline__ void begin(const Layer& p, const Ring& ring, const Matrix& m, const Rows& r, bool matrix, bool rows) {
+    using S = Stage<T, WIDE>;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-        const int row = 8 * n + (lane & 7);
-        const float gate = sum_of<NB>(s.turn, 8 * warp + (lane >> 3), row), up = sum_of<NB>(s.turn, 8 * warp + 4 + (lane >> 3), row);
-        if (row >= count) continue;
-        const float h = column < a.inner ? gate / (1.0f + expf(-gate)) * up : 0.0f;
-        float* const to = p.h + s.pair[first + row] * p.h_stride;
-        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-            const __nv_bfloat16 hi = __float2bfloat16_rn(h);
-            const float rest = fabsf(h) <= 3.3e38f ? h - __bfloat162float(hi) : 0.0f;
-            __nv_bfloat16* const eight = (__nv_bfloat16*)(to + (column & ~7));
-            eight[column & 7] = hi;
-            eight[8 + (column & 7)] = __float2bfloat16_rn(rest);
-        } else {
-            to[column] = h;
+    for (int i = 0; i < kStages - 1; ++i) {
+        const int step = (threadIdx.x >> 5) + i * kWarps;
+        const uint32_t slot = ring.template slot<S::kBytes>(i);
+        // (nothing is asked for past the end: it would not be waited for before its place is filled again)
+        if (step * S::kDepth < m.depth) {
+            if (matrix) bring_matrix<T, WIDE>(m, step, slot);
+            if (rows) bring_rows<T, WIDE, 2>(p, r, m.depth, step, slot);
         }
+        copies_end_group();
     }
 }
 
-template <typename T, bool WIDE, int NB>
-__device__ __forceinline__ void down_unit(const Layer& p, Smem<T>& s, int expert, int block, int first, int count) {
-    const fmb_experts_t& a = p.a;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c0 = kUnit * block + 8 * g;
-    const void* rows[NB];
+// The sums over the depth of a unit's 64 columns and up to 8 NB rows. All of the first stages have been asked for; `all`: only the wait
+// for every copy covers them.
+template <typename T, bool WIDE, int NB, bool UP>
+__device__ __forceinline__ void product(const Layer& p, Ring& ring, const Matrix& m, const Rows& r, bool all, float (&acc)[4][NB][4]) {
+    using S = Stage<T, WIDE>;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) rows[n] = 8 * n + g < count ? p.h + s.pair[first + 8 * n + g] * p.h_stride : nullptr;
-    product<T, WIDE, NB, false>(p, (const T*)a.w_down + expert * a.down_group_stride + c0, a.down_row_stride, a.width - c0, a.inner, rows, s.turn);
-    __syncthreads();
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+        for (int n = 0; n < NB; ++n)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            const int row = 8 * n + (lane & 7), at = 4 * q + (lane >> 3);
-            const float sum = sum_of<NB>(s.turn, 8 * warp + at, row);
-            if (row < count) p.parts[s.pair[first + row] * p.part_stride + kUnit * block + 8 * at + warp] = sum;
+            for (int q = 0; q < 4; ++q) acc[i][n][q] = 0.0f;
+    if (all) copies_wait<0>();
+    for (int step = threadIdx.x >> 5; step * S::kDepth < m.depth; step += kWarps) {
+        copies_wait<kStages - 2>();
+        __syncwarp();                            // every lane's copies of this stage are here, and the stage before has been read
+        const uint32_t next = ring.template slot<S::kBytes>(kStages - 1);
+        const int coming = step + (kStages - 1) * kWarps;
+        if (coming * S::kDepth < m.depth) {
+            bring_matrix<T, WIDE>(m, coming, next);
+            bring_rows<T, WIDE, NB>(p, r, m.depth, coming, next);
         }
+        copies_end_group();
+        multiply<T, WIDE, NB, UP>(acc, m, step, ring.template slot<S::kBytes>(0));
+        ring.place = ring.place + 1 == kStages ? 0 : ring.place + 1;
+    }
+    __syncwarp();
 }
 
-// y of 64 columns: what the experts of each token have given, in the order of its choices
+// Block n of the warps' sums: two columns of a row in each lane's hands. `then`: what is done when all warps have finished the product.
+template <int NB, typename G, typename F>
+__device__ __forceinline__ void turned(float (&turn)[kWarps][kUnit][8], const float (&acc)[4][NB][4], int n, G then, F take) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // column 8 g + j at place 8 j + g: the lanes' stores and loads fall on different banks
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+            *reinterpret_cast<float2*>(&turn[warp][(2 * i + b) * 8 + (lane >> 2)][2 * (lane & 3)]) = make_float2(acc[i][n][2 * b], acc[i][n][2 * b + 1]);
+    __syncthreads();
+    if (n == 0) then();
+    float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) sum[q] += turn[w][8 * warp + 4 * q + (lane >> 3)][lane & 7];
+    take(sum[0], sum[1]);
+    __syncthreads();                             // the sums have been read, and what they gave is written
+}
+
+// Results of a unit's block n. In lane l of warp j: columns 8 (l / 8) + j and that + 32, row l % 8.
+template <typename T, int NB, typename S, typename G>
+__device__ __forceinline__ void put_up(const Layer& p, S& s, const Unit& u, int first, const float (&acc)[4][NB][4], G then) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, column = 32 * u.block + 8 * (lane >> 3) + warp;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+        turned<NB>(s.turn, acc, n, then, [&](float gate, float up) {
+            const int at = first + 8 * n + (lane & 7);
+            if (at >= u.end) return;
+            const float h = column < p.a.inner ? gate / (1.0f + expf(-gate)) * up : 0.0f;
+            float* const to = p.h + s.pair[at] * p.h_stride;
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+                const float rest = fabsf(h) <= 3.3e38f ? h - __bfloat162float(hi) : 0.0f;
+                __nv_bfloat16* const four = (__nv_bfloat16*)(to + (column & ~3));
+                four[column & 3] = hi;
+                four[4 + (column & 3)] = __float2bfloat16_rn(rest);
+            } else {
+                to[column] = h;
+            }
+        });
+}
+
+template <int NB, typename S, typename G>
+__device__ __forceinline__ void put_down(const Layer& p, S& s, const Unit& u, int first, const float (&acc)[4][NB][4], G then) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, column = kUnit * u.block + 8 * (lane >> 3) + warp;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+        turned<NB>(s.turn, acc, n, then, [&](float low, float high) {
+            const int at = first + 8 * n + (lane & 7);
+            if (at >= u.end) return;
+            float* const to = p.parts + s.pair[at] * p.part_stride + column;
+            to[0] = low;
+            to[32] = high;
+        });
+}
+
+// y of 64 columns: what the experts of each token have given, in the order of its choices. Four columns a thread, 16 tokens at a time.
 template <typename T>
 __device__ __forceinline__ void combine(const Layer& p, int block) {
     const fmb_experts_t& a = p.a;
-    const int c = kUnit * block + (threadIdx.x & (kUnit - 1));
-    if (c >= a.width) return;
-    for (int t = threadIdx.x / kUnit; t < a.tokens; t += kThreads / kUnit) {
-        float sum = 0.0f;
+    const int c = kUnit * block + 4 * (threadIdx.x & 15);
+    for (int t = threadIdx.x >> 4; t < a.tokens; t += kThreads / 16) {
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         for (int j0 = 0; j0 < a.top; j0 += 4) {
-            float v[4];
+            float w[4];
+            float4 v[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int pair = t * a.top + j0 + j, e = j0 + j < a.top ? __ldg(a.chosen + pair) : -1;
-                v[j] = e >= 0 && e < a.experts ? __ldg(a.weights + pair) * __ldcg(p.parts + pair * p.part_stride + c) : 0.0f;
+                const int pair = t * a.top + j0 + j;
+                const bool there = j0 + j < a.top;
+                const int e = there ? __ldg(a.chosen + pair) : -1;
+                w[j] = there ? __ldg(a.weights + pair) : 0.0f;
+                // (of a choice that is no expert nothing has been written)
+                v[j] = there ? __ldcg(reinterpret_cast<const float4*>(p.parts + pair * p.part_stride + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if (e < 0 || e >= a.experts) w[j] = 0.0f, v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum += v[j];
+            for (int j = 0; j < 4; ++j) {
+                sum.x += w[j] * v[j].x;
+                sum.y += w[j] * v[j].y;
+                sum.z += w[j] * v[j].z;
+                sum.w += w[j] * v[j].w;
+            }
         }
-        ((T*)a.y)[t * a.y_stride + c] = rounded<T>(sum);
+        T* const y = (T*)a.y + t * a.y_stride + c;
+        const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (c + i < a.width) y[i] = rounded<T>(out[i]);
     }
+}
+
+// Which pairs belong to which expert, and which experts have any; the counters of the next launch become zero. Pairs of one expert stand in
+// any order: their results do not depend on it. The CTAs behind the first copy rows of x, where those do not begin at multiples
+// of 8 bytes.
+template <typename T>
+__global__ void __launch_bounds__(1024)
+k_list_pairs(const __grid_constant__ Layer p, int control, void* packed) {
+    const fmb_experts_t& a = p.a;
+    asm volatile("griddepcontrol.launch_dependents;");            // the next launch comes to the SMs meanwhile, and waits there
+    if (blockIdx.x > 0) {
+        const T* const from = (const T*)a.x + (blockIdx.x - 1) * a.x_stride;
+        T* const to = (T*)packed + (blockIdx.x - 1) * p.x_stride;
+        for (int c = threadIdx.x; c < p.x_stride; c += 1024) to[c] = c < a.width ? from[c] : zero<T>();
+        return;
+    }
+    __shared__ int start[FMB_MAX_GROUPS];
+    __shared__ int warp_total[2][32];
+    const int experts = a.experts, pairs = a.tokens * a.top, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
+    int32_t* const active = p.lists + 2;
+    int32_t* const first = active + experts;
+    int32_t* const pair = first + experts + 1;
+    for (int i = threadIdx.x; i < control; i += 1024) p.control[i] = 0;
+    start[e] = 0;
+    __syncthreads();
+    int chosen[kMaxPairs / 1024];
+#pragma unroll
+    for (int q = 0; q < kMaxPairs / 1024; ++q) {
+        const int i = threadIdx.x + 1024 * q;
+        chosen[q] = i < pairs ? __ldg(a.chosen + i) : -1;
+        if (chosen[q] >= experts) chosen[q] = -1;
+        if (chosen[q] >= 0) atomicAdd(start + chosen[q], 1);
+    }
+    __syncthreads();
+    const int count = start[e];
+    int sums = count, somes = count > 0;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, sums, o), y = __shfl_up_sync(0xffffffffu, somes, o);
+        if (lane >= o) sums += x, somes += y;
+    }
+    if (lane == 31) warp_total[0][warp] = sums, warp_total[1][warp] = somes;
+    __syncthreads();
+    int before = lane < warp ? warp_total[0][lane] : 0, number = lane < warp ? warp_total[1][lane] : 0;
+    before = warp_sum(before);
+    number = warp_sum(number);
+    const int begin = before + sums - count, place = number + somes - (count > 0);
+    start[e] = begin;
+    if (count > 0) {
+        active[place] = e;
+        first[place] = begin;
+    }
+    if (e == 1023) {
+        first[place + (count > 0)] = begin + count;
+        p.lists[0] = place + (count > 0);
+        p.lists[1] = begin + count;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < kMaxPairs / 1024; ++q)
+        if (chosen[q] >= 0) pair[atomicAdd(start + chosen[q], 1)] = threadIdx.x + 1024 * q;
 }
 
 template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads, 2)
 k_experts(const __grid_constant__ Layer p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    Smem<T>& s = *reinterpret_cast<Smem<T>*>(smem);
+    Smem<T, WIDE>& s = *reinterpret_cast<Smem<T, WIDE>*>(smem);
     const fmb_experts_t& a = p.a;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int32_t* const next = p.control;
-    int32_t* const done = p.control + 2;
+    int32_t* const done = p.control + 1;
     int32_t* const columns = done + a.experts;
-    if (threadIdx.x == 0) s.ticket[0] = atomicAdd(next, 1);
-    list_pairs(p, s);
-    const int actives = s.actives, ups = actives * p.up_units, units = ups + actives * p.down_units;
+    asm volatile("griddepcontrol.wait;" ::: "memory");            // for the lists
+    if (threadIdx.x == 0) {
+        s.ticket = atomicAdd(next, 1);
+        s.gave_up = 0;
+        s.last[1] = -1;
+    }
+    // (the lists' places, whether in use or not: their numbers need not be waited for)
+    const int actives = __ldg(p.lists), most = min(a.experts, a.tokens * a.top);
+    for (int i = threadIdx.x; i <= most; i += kThreads) {
+        if (i < most) s.active[i] = (uint16_t)__ldg(p.lists + 2 + i);
+        s.first[i] = (uint16_t)__ldg(p.lists + 2 + a.experts + i);
+    }
+    for (int i = threadIdx.x; i < a.tokens * a.top; i += kThreads) {
+        const uint32_t pair = (uint32_t)__ldg(p.lists + 3 + 2 * a.experts + i);
+        s.pair[i] = (uint16_t)pair;
+        s.token[i] = (uint8_t)(pair / a.top);
+    }
+    __syncthreads();
     if (actives == 0) {                          // no expert is one
         for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < (long long)a.tokens * a.width; i += (long long)gridDim.x * kThreads)
             ((T*)a.y)[i / a.width * a.y_stride + i % a.width] = zero<T>();
         return;
     }
-    for (int round = 0;; round ^= 1) {
-        const int unit = s.ticket[round];
-        if (unit >= units) return;
-        const bool up = unit < ups;
-        const int number = up ? unit / p.up_units : (unit - ups) / p.down_units;
-        const int block = up ? unit % p.up_units : (unit - ups) % p.down_units;
-        const int expert = s.active[number], first = s.start[expert];
-        // (the starts have been counted down to where each expert's pairs begin)
-        int end = s.start[a.experts];
-        if (number + 1 < actives) end = s.start[s.active[number + 1]];
-        if (threadIdx.x == 0) {
-            s.ticket[round ^ 1] = atomicAdd(next, 1);
-            int ready = 1;
-            if (!up) {
+    const int ups = actives * p.up_units, units = ups + actives * p.down_units;
+    int ticket = s.ticket;
+    if (ticket >= units) return;
+    Unit u = unit_of(p, s, ticket, ups);
+    Matrix m = matrix_of<T, WIDE>(p, u);
+    Rows r = rows_of<T, WIDE>(p, s, u, u.first);
+    Ring ring = {smem_at(s.ring[warp]), 0};
+    bool ready = u.up;                           // what the unit's rows are has been written
+    begin<T, WIDE>(p, ring, m, r, true, ready);
+    int round = 0;
+    for (;;) {
+        bool all = false;
+        if (!ready) {
+            if (lane == 0) {
                 long long spins = 0;
-                while (load_acquire(done + number) < p.up_units && ++spins < kSpins) __nanosleep(32);
-                ready = spins < kSpins;
-                if (!ready && a.status) atomicOr(a.status, (uint32_t)FMB_STATUS_TENSOR_TIMEOUT);
+                while (load_acquire(done + u.number) < p.up_units && !s.gave_up)
+                    if (++spins < kSpins) __nanosleep(32);
+                    else s.gave_up = 1;
+                if (s.gave_up && a.status) atomicOr(a.status, (uint32_t)FMB_STATUS_TENSOR_TIMEOUT);
             }
-            s.flag = ready;
+            __syncwarp();
+            begin<T, WIDE>(p, ring, m, r, false, true);
+            all = true;
         }
-        __syncthreads();
-        if (!s.flag) return;
-        for (int at = first; at < end; at += 16) {
-            const int count = min(16, end - at);
-            if (at > first) __syncthreads();
-            if (up) {
-                if (count <= 8) up_unit<T, WIDE, 1>(p, s, expert, block, at, count);
-                else up_unit<T, WIDE, 2>(p, s, expert, block, at, count);
-            } else {
-                if (count <= 8) down_unit<T, WIDE, 1>(p, s, expert, block, at, count);
-                else down_unit<T, WIDE, 2>(p, s, expert, block, at, count);
-            }
+        // The unit after this one: asked for now, when this one no longer waits for others, and needed at its end.
+        const int ahead = threadIdx.x == 0 ? atomicAdd(next, 1) : 0;
+        const Unit v = u;
+        for (int at = v.first; at < v.end; at += 16) {
+            const bool last = at + 16 >= v.end;
+            // behind the product: the first stages of the next unit, or of this one for its next rows. They are on their way while the
+            // results are taken out.
+            auto then = [&]() {
+                if (!last) {
+                    r = rows_of<T, WIDE>(p, s, v, at + 16);
+                    begin<T, WIDE>(p, ring, m, r, true, true);
+                    return;
+                }
+                ticket = s.ticket;
+                if (ticket >= units) return;
+                u = unit_of(p, s, ticket, ups);
+                m = matrix_of<T, WIDE>(p, u);
+                r = rows_of<T, WIDE>(p, s, u, u.first);
+                ready = u.up;
+                begin<T, WIDE>(p, ring, m, r, true, ready);
+                if (v.up && !u.up) prefetch_unit(m);
+            };
+            auto run = [&](auto blocks) {
+                constexpr int NB = decltype(blocks)::value;
+                float acc[4][NB][4];
+                if (v.up) product<T, WIDE, NB, true>(p, ring, m, r, all, acc);
+                else product<T, WIDE, NB, false>(p, ring, m, r, all, acc);
+                if (last && threadIdx.x == 0) s.ticket = ahead;
+                if (v.up) put_up<T, NB>(p, s, v, at, acc, then);
+                else put_down<NB>(p, s, v, at, acc, then);
+            };
+            if (v.end - at <= 8) run(std::integral_constant<int, 1>());
+            else run(std::integral_constant<int, 2>());
+            all = false;
         }
-        __syncthreads();
+        // Thread 0 tells the others that the unit is done, while its CTA goes on; whether the unit was the last of its columns the CTA
+        // looks at after the next one.
+        if (s.last[round ^ 1] >= 0) combine<T>(p, s.last[round ^ 1]);
         if (threadIdx.x == 0) {
-            __threadfence();
-            if (up) {
-                atomicAdd(done + number, 1);
-                s.flag = 0;
-            } else {
-                s.flag = atomicAdd(columns + block, 1) == actives - 1;
-                __threadfence();
-            }
+            s.last[round] = -1;
+            if (v.up) add_release(done + v.number);
+            else if (add_acquire_release(columns + v.block) == actives - 1) s.last[round] = v.block;
         }
-        __syncthreads();
-        if (s.flag) combine<T>(p, block);
-        __syncthreads();                         // the flag has been read
+        if (ticket >= units) break;
+        round ^= 1;
     }
+    __syncthreads();
+    if (s.last[round] >= 0) combine<T>(p, s.last[round]);
 }
 
 long long up_to(long long n, long long step) { return (n + step - 1) / step * step; }
 
 struct Sizes {
-    long long control, h, parts;                 // in floats
-    long long h_stride, part_stride;
+    long long control, lists, h, parts, x;       // in floats
+    long long h_stride, part_stride, x_stride;
 };
 
 Sizes sizes_of(const fmb_experts_t& a) {
     Sizes s;
-    s.control = up_to(2 + a.experts + ceil_div(a.width, kUnit), 64);
+    const long long pairs = (long long)a.tokens * a.top;
+    s.control = up_to(1 + a.experts + ceil_div(a.width, kUnit), 64);
+    s.lists = up_to(3 + 2 * a.experts + pairs, 64);
     s.h_stride = up_to(a.inner, 32);
     s.part_stride = up_to(a.width, kUnit);
-    s.h = up_to((long long)a.tokens * a.top * s.h_stride, 64);
-    s.parts = (long long)a.tokens * a.top * s.part_stride;
+    s.h = pairs * s.h_stride;
+    s.parts = pairs * s.part_stride;
+    s.x_stride = up_to(a.width, 8);
+    s.x = a.tokens * s.x_stride;
     return s;
 }
 
-bool fits(const void* base, long long stride, int bytes) { return ((uintptr_t)base & 15) == 0 && stride * bytes % 16 == 0; }
+// whether the rows of a matrix begin at multiples of `unit` bytes
+bool begin_at(const void* base, long long stride, int rows, int bytes, int unit) {
+    return (uintptr_t)base % unit == 0 && (rows <= 1 || stride * bytes % unit == 0);
+}
 
 template <typename T>
 int layer(const fmb_experts_t& a, cudaStream_t stream) {
     const Sizes size = sizes_of(a);
+    const int b = sizeof(T);
     Layer p;
     p.a = a;
     p.control = (int32_t*)a.scratch;
-    p.h = a.scratch + size.control;
+    p.lists = p.control + size.control;
+    p.h = a.scratch + size.control + size.lists;
     p.parts = p.h + size.h;
+    void* const packed = p.parts + size.parts;
     p.h_stride = size.h_stride;
     p.part_stride = size.part_stride;
     p.up_units = ceil_div(a.inner, 32);
     p.down_units = ceil_div(a.width, kUnit);
-    const int b = sizeof(T);
-    p.x_wide = fits(a.x, a.tokens > 1 ? a.x_stride : 8, b);
-    // whole packs of eight columns
-    const bool wide = a.inner % 8 == 0 && a.width % 8 == 0 && fits(a.w_up, a.up_row_stride, b) && fits(a.w_down, a.down_row_stride, b) &&
-                      (a.experts == 1 || (a.up_group_stride * b % 16 == 0 && a.down_group_stride * b % 16 == 0));
-    FMB_CUDA_CHECK(cudaMemsetAsync(p.control, 0, size.control * 4, stream));
-    const void* const kernel = wide ? (const void*)k_experts<T, true> : (const void*)k_experts<T, false>;
-    FMB_CUDA_CHECK(opt_in_shared_memory(kernel, sizeof(Smem<T>)));
+    p.up_inverse = (uint32_t)(((1ull << 32) + p.up_units - 1) / p.up_units);
+    p.down_inverse = (uint32_t)(((1ull << 32) + p.down_units - 1) / p.down_units);
+    const bool pack = !begin_at(a.x, a.x_stride, a.tokens, b, 8);
+    p.x = pack ? packed : const_cast<void*>(a.x);
+    p.x_stride = pack ? size.x_stride : a.x_stride;
+    k_list_pairs<T><<<pack ? a.tokens + 1 : 1, 1024, 0, stream>>>(p, (int)size.control, packed);
+    FMB_LAUNCH_CHECK();
+    // whole pieces of 16 bytes, at multiples of 16
+    auto pieces = [&](const void* base, long long row, long long group, int rows, int columns) {
+        return columns * b % 16 == 0 && begin_at(base, row, rows, b, 16) && begin_at(base, group, a.experts, b, 16);
+    };
+    const bool wide = pieces(a.w_up, a.up_row_stride, a.up_group_stride, a.width, a.inner) && pieces(a.w_down, a.down_row_stride, a.down_group_stride, a.inner, a.width);
     const long long most = std::min<long long>(a.experts, (long long)a.tokens * a.top) * (p.up_units + p.down_units);
     const int grid = (int)std::min<long long>(most, 2 * grp::sm_count());
-    if (wide) k_experts<T, true><<<grid, kThreads, sizeof(Smem<T>), stream>>>(p);
-    else k_experts<T, false><<<grid, kThreads, sizeof(Smem<T>), stream>>>(p);
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = wide ? sizeof(Smem<T, true>) : sizeof(Smem<T, false>);
+    config.stream = stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    FMB_CUDA_CHECK(opt_in_shared_memory(wide ? (const void*)k_experts<T, true> : (const void*)k_experts<T, false>, (int)config.dynamicSmemBytes));
+    FMB_CUDA_CHECK(wide ? cudaLaunchKernelEx(&config, k_experts<T, true>, p) : cudaLaunchKernelEx(&config, k_experts<T, false>, p));
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
+
+bool fits(const void* base, long long stride, int bytes) { return ((uintptr_t)base & 15) == 0 && stride * bytes % 16 == 0; }
 
 template <typename T>
 int route(const fmb_route_t& a, cudaStream_t stream) {
@@ -705,7 +977,7 @@ int check_layer(const fmb_experts_t* a) {
 extern "C" FMB_API long long fmb_expert_layer_scratch(const fmb_experts_t* a) {
     if (check_layer(a) || a->tokens == 0) return 0;
     const Sizes s = sizes_of(*a);
-    return s.control + s.h + s.parts;
+    return s.control + s.lists + s.h + s.parts + s.x;
 }
 
 extern "C" FMB_API int fmb_expert_layer(const fmb_experts_t* a, fmb_stream_t stream) {
@@ -713,6 +985,8 @@ extern "C" FMB_API int fmb_expert_layer(const fmb_experts_t* a, fmb_stream_t str
     if (rc || a->tokens == 0) return rc;
     FMB_REQUIRE(a->x && a->w_up && a->w_down && a->chosen && a->weights && a->y && a->scratch, "fmb_expert_layer: null argument");
     FMB_REQUIRE(a->tokens == 1 || (a->x_stride >= a->width && a->y_stride >= a->width), "fmb_expert_layer: rows overlap");
+    const long long far = (1ll << 31) / 4 - 1;
+    FMB_REQUIRE(a->up_row_stride >= 0 && a->up_row_stride <= far && a->down_row_stride >= 0 && a->down_row_stride <= far, "fmb_expert_layer: rows of weights more than 2^29 apart");
     FMB_REQUIRE(((uintptr_t)a->scratch & 15) == 0, "fmb_expert_layer: scratch starts at a multiple of 16 bytes");
     return a->type == FMB_TYPE_F32    ? layer<float>(*a, (cudaStream_t)stream)
            : a->type == FMB_TYPE_BF16 ? layer<__nv_bfloat16>(*a, (cudaStream_t)stream)
