@@ -273,7 +273,8 @@ struct Matrix {
     const char* at;
     long long second;
     int stride, first_bytes, second_bytes, depth;                              // stride: bytes
-    // WIDE: where this lane's copies of the first stage begin, and whether there is something (Stage::kRows rows at once)
+    // where this lane's copies of the first stage begin, of kRows rows at once, and whether there is something (not WIDE: the pieces that
+    // the halves fill; and the copy of one more piece of each row)
     const char* lane_at;
     bool lane_there;
 };
@@ -298,12 +299,10 @@ __device__ __forceinline__ Matrix matrix_of(const Layer& p, const Unit& u) {
         m.stride = (int)a.down_row_stride * kSize;
         m.depth = a.inner;
     }
-    if (WIDE) {
-        constexpr int kHalf = Stage<T, WIDE>::kHalf;
-        const int lane = threadIdx.x & 31, row = lane / (2 * kHalf), half = lane / kHalf & 1, piece = lane % kHalf;
-        m.lane_at = m.at + (long long)m.stride * row + (half ? m.second : 0) + piece * 16;
-        m.lane_there = piece * 16 < (half ? m.second_bytes : m.first_bytes);
-    }
+    constexpr int kHalf = 4 * Stage<T, WIDE>::kPieces;
+    const int lane = threadIdx.x & 31, row = lane / (2 * kHalf), half = lane / kHalf & 1, piece = lane % kHalf;
+    m.lane_at = m.at + (long long)m.stride * row + (half ? m.second : 0) + piece * 16;
+    m.lane_there = piece * 16 < (half ? m.second_bytes : m.first_bytes);
     return m;
 }
 
@@ -339,6 +338,18 @@ __device__ __forceinline__ void bring_matrix(const Matrix& m, int step, uint32_t
     } else {
         // the pieces that a half fills, kRows rows at a time as above, and then the one more of each row
         constexpr int kOfRow = 8 * S::kPieces;
+        if (live >= S::kDepth && m.second_bytes == 32 * (int)sizeof(T)) {
+            const char* const at = m.lane_at + offset;
+            const uint32_t to = slot + S::place(0, lane / kOfRow, lane % kOfRow / (kOfRow / 2) * S::kHalf + lane % (kOfRow / 2)) * 16;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                copy_16(to + S::place(i, 0, 0) * 16, (const char*)((uintptr_t)(at + (long long)m.stride * (i * S::kRows)) & ~(uintptr_t)15));
+            const char* const row = m.at + offset + (long long)m.stride * (lane >> 1) + (lane & 1 ? m.second : 0);
+            if (lane < 2 * S::kDepth && ((uintptr_t)row & 15))
+                copy_16(slot + S::place((lane >> 1) / S::kRows, (lane >> 1) % S::kRows, (lane & 1) * S::kHalf + S::kHalf - 1) * 16,
+                        (const char*)((uintptr_t)row & ~(uintptr_t)15) + (S::kHalf - 1) * 16);
+            return;
+        }
         auto bring = [&](int r, int half, int piece) {
             const char* const row = m.at + offset + (long long)m.stride * r + (half ? m.second : 0);
             const int shift = (int)((uintptr_t)row & 15), bytes = half ? m.second_bytes : m.first_bytes;
@@ -353,7 +364,7 @@ __device__ __forceinline__ void bring_matrix(const Matrix& m, int step, uint32_t
 }
 
 // rows of x by kRows values, 8 bytes; of h, which is kept as float32 or, for bfloat16 weights, as four upper halves and then four lower ones
-template <typename T, bool WIDE, int NB>
+template <typename T, bool WIDE>
 __device__ __forceinline__ void bring_rows(const Layer& p, const Rows& r, int depth, int step, uint32_t slot) {
     using S = Stage<T, WIDE>;
     const int lane = threadIdx.x & 31;
@@ -361,7 +372,7 @@ __device__ __forceinline__ void bring_rows(const Layer& p, const Rows& r, int de
     const int offset = step * S::kDepth * (r.up ? (int)sizeof(T) : 4);
     if ((step + 1) * S::kDepth <= depth) {
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
+        for (int n = 0; n < 2; ++n) {
             if (!r.at[n]) continue;
             if (sizeof(T) == 2 && !r.up) copy_16(to + n * 512, r.at[n] + offset);
             else copy_8(to + n * 512, r.at[n] + offset);
@@ -370,7 +381,7 @@ __device__ __forceinline__ void bring_rows(const Layer& p, const Rows& r, int de
     }
     const int most = depth - step * S::kDepth - S::kRows * (lane & 3);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
+    for (int n = 0; n < 2; ++n) {
         const int live = r.at[n] ? max(0, min(S::kRows, most)) : 0;
         const char* const from = live ? r.at[n] + offset : (const char*)p.h;
         if (r.up) copy_8(to + n * 512, from, live * (int)sizeof(T));
@@ -392,9 +403,11 @@ __device__ __forceinline__ void align_row(uint32_t from, const uint32_t (&v)[siz
     for (int i = 0; i < kWords; ++i) out[i] = sizeof(T) == 2 ? __funnelshift_r(b[i], b[i + 1], (from & 2) * 8) : b[i];
 }
 
-// The stage's product. Matrix columns are the MMA's rows, in the order of the lanes' eight: acc[i][n] has columns 2 i and 2 i + 1.
-template <typename T, bool WIDE, int NB, bool UP>
-__device__ __forceinline__ void multiply(float (&acc)[4][NB][4], const Matrix& m, int step, uint32_t slot) {
+// The stage's product, for rows of x (up) or h, one block of eight rows or two: branches that the whole warp takes, in one body, since with
+// a body for each case the code of a unit's end was waited for longer than it took. Matrix columns are the MMA's rows, in the order of
+// the lanes' eight: acc[i][n] has columns 2 i and 2 i + 1.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void multiply(float (&acc)[4][2][4], const Matrix& m, int step, uint32_t slot, bool up, bool two_blocks) {
     using S = Stage<T, WIDE>;
     constexpr int kWords = sizeof(T) * 2;
     const int lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
@@ -418,66 +431,63 @@ __device__ __forceinline__ void multiply(float (&acc)[4][NB][4], const Matrix& m
         }
     }
     const uint32_t rows = slot + S::kMatrixBytes + lane * 16;
-    if constexpr (sizeof(T) == 2 && (UP || std::is_same<T, __nv_bfloat16>::value)) {
-        uint4 b[NB];
+    if (sizeof(T) == 2 && (up || std::is_same<T, __nv_bfloat16>::value)) {
+        if constexpr (sizeof(T) == 2) {
+            uint32_t a[4][4];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
-            if constexpr (UP) {
-                const uint2 two = load_8(rows + n * 512);
-                b[n] = make_uint4(two.x, two.y, 0, 0);
-            } else {
-                b[n] = load_16(rows + n * 512);
+            for (int i = 0; i < 4; ++i) {
+                a[i][0] = __byte_perm(w[0][i], w[1][i], 0x5410);
+                a[i][1] = __byte_perm(w[0][i], w[1][i], 0x7632);
+                a[i][2] = __byte_perm(w[2][i], w[3][i], 0x5410);
+                a[i][3] = __byte_perm(w[2][i], w[3][i], 0x7632);
             }
-        }
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t a[4] = {__byte_perm(w[0][i], w[1][i], 0x5410), __byte_perm(w[0][i], w[1][i], 0x7632),
-                                   __byte_perm(w[2][i], w[3][i], 0x5410), __byte_perm(w[2][i], w[3][i], 0x7632)};
+            for (int n = 0; n < 2; ++n) {
+                if (n && !two_blocks) break;
+                const uint4 b = load_16(rows + n * 512);          // (of x the first half)
+                if (!up) {
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                if (!UP) mma_16(acc[i][n], a, b[n].z, b[n].w, T());
-                mma_16(acc[i][n], a, b[n].x, b[n].y, T());
+                    for (int i = 0; i < 4; ++i) mma_16(acc[i][n], a[i], b.z, b.w, T());
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mma_16(acc[i][n], a[i], b.x, b.y, T());
             }
         }
     } else {
         // float32 values as pairs of tf32, float16 weights as they are
-        float b[NB][S::kRows];
 #pragma unroll
-        for (int n = 0; n < NB; ++n) {
+        for (int n = 0; n < 2; ++n) {
+            if (n && !two_blocks) break;
+            float b[S::kRows];
             if constexpr (S::kRows == 4) {
                 const uint4 v = load_16(rows + n * 512);
-                b[n][0] = __uint_as_float(v.x); b[n][1] = __uint_as_float(v.y); b[n][2] = __uint_as_float(v.z); b[n][3] = __uint_as_float(v.w);
+                b[0] = __uint_as_float(v.x); b[1] = __uint_as_float(v.y); b[2] = __uint_as_float(v.z); b[3] = __uint_as_float(v.w);
             } else {
                 const uint2 v = load_8(rows + n * 512);
-                b[n][0] = __uint_as_float(v.x); b[n][1] = __uint_as_float(v.y);
+                b[0] = __uint_as_float(v.x); b[1] = __uint_as_float(v.y);
             }
-        }
 #pragma unroll
-        for (int s = 0; s < S::kRows / 2; ++s) {
-            uint32_t hi[NB][2], lo[NB][2];
+            for (int s = 0; s < S::kRows / 2; ++s) {
+                uint32_t hi[2], lo[2];
 #pragma unroll
-            for (int n = 0; n < NB; ++n)
+                for (int q = 0; q < 2; ++q) split_tf32(b[2 * s + q], hi[q], lo[q]);
 #pragma unroll
-                for (int q = 0; q < 2; ++q) split_tf32(b[n][2 * s + q], hi[n][q], lo[n][q]);
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t a[4], rest[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t a[4], rest[4];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) {
-                    if constexpr (sizeof(T) == 2) {
-                        const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&w[2 * s + q][i]));
-                        a[2 * q] = __float_as_uint(two.x);
-                        a[2 * q + 1] = __float_as_uint(two.y);
-                    } else {
-                        split_tf32(__uint_as_float(w[2 * s + q][2 * i]), a[2 * q], rest[2 * q]);
-                        split_tf32(__uint_as_float(w[2 * s + q][2 * i + 1]), a[2 * q + 1], rest[2 * q + 1]);
+                    for (int q = 0; q < 2; ++q) {
+                        if constexpr (sizeof(T) == 2) {
+                            const float2 two = __half22float2(*reinterpret_cast<const __half2*>(&w[2 * s + q][i]));
+                            a[2 * q] = __float_as_uint(two.x);
+                            a[2 * q + 1] = __float_as_uint(two.y);
+                        } else {
+                            split_tf32(__uint_as_float(w[2 * s + q][2 * i]), a[2 * q], rest[2 * q]);
+                            split_tf32(__uint_as_float(w[2 * s + q][2 * i + 1]), a[2 * q + 1], rest[2 * q + 1]);
+                        }
                     }
-                }
-#pragma unroll
-                for (int n = 0; n < NB; ++n) {
-                    mma_tf32(acc[i][n], a, lo[n][0], lo[n][1]);
-                    if constexpr (sizeof(T) == 4) mma_tf32(acc[i][n], rest, hi[n][0], hi[n][1]);
-                    mma_tf32(acc[i][n], a, hi[n][0], hi[n][1]);
+                    mma_tf32(acc[i][n], a, lo[0], lo[1]);
+                    if constexpr (sizeof(T) == 4) mma_tf32(acc[i][n], rest, hi[0], hi[1]);
+                    mma_tf32(acc[i][n], a, hi[0], hi[1]);
                 }
             }
         }
@@ -548,21 +558,21 @@ __device__ __forceinline__ void begin(const Layer& p, const Ring& ring, const Ma
         // (nothing is asked for past the end: it would not be waited for before its place is filled again)
         if (step * S::kDepth < m.depth) {
             if (matrix) bring_matrix<T, WIDE>(m, step, slot);
-            if (rows) bring_rows<T, WIDE, 2>(p, r, m.depth, step, slot);
+            if (rows) bring_rows<T, WIDE>(p, r, m.depth, step, slot);
         }
         copies_end_group();
     }
 }
 
-// The sums over the depth of a unit's 64 columns and up to 8 NB rows. All of the first stages have been asked for; `all`: only the wait
+// The sums over the depth of a unit's 64 columns and up to 16 rows. All of the first stages have been asked for; `all`: only the wait
 // for every copy covers them.
-template <typename T, bool WIDE, int NB, bool UP>
-__device__ __forceinline__ void product(const Layer& p, Ring& ring, const Matrix& m, const Rows& r, bool all, float (&acc)[4][NB][4]) {
+template <typename T, bool WIDE>
+__device__ __forceinline__ void product(const Layer& p, Ring& ring, const Matrix& m, const Rows& r, bool all, bool two_blocks, float (&acc)[4][2][4]) {
     using S = Stage<T, WIDE>;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
             for (int q = 0; q < 4; ++q) acc[i][n][q] = 0.0f;
     if (all) copies_wait<0>();
@@ -573,76 +583,60 @@ __device__ __forceinline__ void product(const Layer& p, Ring& ring, const Matrix
         const int coming = step + (kStages - 1) * kWarps;
         if (coming * S::kDepth < m.depth) {
             bring_matrix<T, WIDE>(m, coming, next);
-            bring_rows<T, WIDE, NB>(p, r, m.depth, coming, next);
+            bring_rows<T, WIDE>(p, r, m.depth, coming, next);
         }
         copies_end_group();
-        multiply<T, WIDE, NB, UP>(acc, m, step, ring.template slot<S::kBytes>(0));
+        multiply<T, WIDE>(acc, m, step, ring.template slot<S::kBytes>(0), r.up, two_blocks);
         ring.place = ring.place + 1 == kStages ? 0 : ring.place + 1;
     }
     __syncwarp();
 }
 
-// Block n of the warps' sums: two columns of a row in each lane's hands. `then`: what is done when all warps have finished the product.
-template <int NB, typename G, typename F>
-__device__ __forceinline__ void turned(float (&turn)[kWarps][kUnit][8], const float (&acc)[4][NB][4], int n, G then, F take) {
+// Block n of the warps' sums on its way out: column 8 g + j at place 8 j + g, so that the lanes' stores and loads fall on different banks
+__device__ __forceinline__ void turn_in(float (&turn)[kWarps][kUnit][8], const float (&acc)[4][2][4], int n) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    // column 8 g + j at place 8 j + g: the lanes' stores and loads fall on different banks
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int b = 0; b < 2; ++b)
-            *reinterpret_cast<float2*>(&turn[warp][(2 * i + b) * 8 + (lane >> 2)][2 * (lane & 3)]) = make_float2(acc[i][n][2 * b], acc[i][n][2 * b + 1]);
-    __syncthreads();
-    if (n == 0) then();
-    float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) sum[q] += turn[w][8 * warp + 4 * q + (lane >> 3)][lane & 7];
-    take(sum[0], sum[1]);
-    __syncthreads();                             // the sums have been read, and what they gave is written
+            *reinterpret_cast<float2*>(&turn[warp][(2 * i + b) * 8 + (lane >> 2)][2 * (lane & 3)]) =
+                n == 0 ? make_float2(acc[i][0][2 * b], acc[i][0][2 * b + 1]) : make_float2(acc[i][1][2 * b], acc[i][1][2 * b + 1]);
 }
 
-// Results of a unit's block n. In lane l of warp j: columns 8 (l / 8) + j and that + 32, row l % 8.
-template <typename T, int NB, typename S, typename G>
-__device__ __forceinline__ void put_up(const Layer& p, S& s, const Unit& u, int first, const float (&acc)[4][NB][4], G then) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, column = 32 * u.block + 8 * (lane >> 3) + warp;
+// Lane l of warp j takes columns 8 (l / 8) + j and that + 32 of row l % 8 out: the gate's result for h, or the two columns of a pair's part.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void turn_out(const Layer& p, const Smem<T, WIDE>& s, const Unit& u, int first) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = first + (lane & 7);
+    float low = 0.0f, high = 0.0f;
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
-        turned<NB>(s.turn, acc, n, then, [&](float gate, float up) {
-            const int at = first + 8 * n + (lane & 7);
-            if (at >= u.end) return;
-            const float h = column < p.a.inner ? gate / (1.0f + expf(-gate)) * up : 0.0f;
-            float* const to = p.h + s.pair[at] * p.h_stride;
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                const __nv_bfloat16 hi = __float2bfloat16_rn(h);
-                const float rest = fabsf(h) <= 3.3e38f ? h - __bfloat162float(hi) : 0.0f;
-                __nv_bfloat16* const four = (__nv_bfloat16*)(to + (column & ~3));
-                four[column & 3] = hi;
-                four[4 + (column & 3)] = __float2bfloat16_rn(rest);
-            } else {
-                to[column] = h;
-            }
-        });
-}
-
-template <int NB, typename S, typename G>
-__device__ __forceinline__ void put_down(const Layer& p, S& s, const Unit& u, int first, const float (&acc)[4][NB][4], G then) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, column = kUnit * u.block + 8 * (lane >> 3) + warp;
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-        turned<NB>(s.turn, acc, n, then, [&](float low, float high) {
-            const int at = first + 8 * n + (lane & 7);
-            if (at >= u.end) return;
-            float* const to = p.parts + s.pair[at] * p.part_stride + column;
-            to[0] = low;
-            to[32] = high;
-        });
+    for (int w = 0; w < kWarps; ++w) {
+        low += s.turn[w][8 * warp + (lane >> 3)][lane & 7];
+        high += s.turn[w][8 * warp + 4 + (lane >> 3)][lane & 7];
+    }
+    if (at >= u.end) return;
+    if (!u.up) {
+        float* const to = p.parts + s.pair[at] * p.part_stride + kUnit * u.block + 8 * (lane >> 3) + warp;
+        to[0] = low;
+        to[32] = high;
+        return;
+    }
+    const int column = 32 * u.block + 8 * (lane >> 3) + warp;
+    const float h = column < p.a.inner ? low / (1.0f + expf(-low)) * high : 0.0f;
+    float* const to = p.h + s.pair[at] * p.h_stride;
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const __nv_bfloat16 hi = __float2bfloat16_rn(h);
+        const float rest = fabsf(h) <= 3.3e38f ? h - __bfloat162float(hi) : 0.0f;
+        __nv_bfloat16* const four = (__nv_bfloat16*)(to + (column & ~3));
+        four[column & 3] = hi;
+        four[4 + (column & 3)] = __float2bfloat16_rn(rest);
+    } else {
+        to[column] = h;
+    }
 }
 
 // y of 64 columns: what the experts of each token have given, in the order of its choices. Four columns a thread, 16 tokens at a time.
 template <typename T>
-__device__ __forceinline__ void combine(const Layer& p, int block) {
+__device__ __noinline__ void combine(const Layer& p, int block) {
     const fmb_experts_t& a = p.a;
     const int c = kUnit * block + 4 * (threadIdx.x & 15);
     for (int t = threadIdx.x >> 4; t < a.tokens; t += kThreads / 16) {
@@ -797,37 +791,43 @@ k_experts(const __grid_constant__ Layer p) {
         // The unit after this one: asked for now, when this one no longer waits for others, and needed at its end.
         const int ahead = threadIdx.x == 0 ? atomicAdd(next, 1) : 0;
         const Unit v = u;
+        bool turning = false;
+        // the unit after this one and its first stages
+        auto go_on = [&]() {
+            if (ticket >= units) return;
+            u = unit_of(p, s, ticket, ups);
+            m = matrix_of<T, WIDE>(p, u);
+            r = rows_of<T, WIDE>(p, s, u, u.first);
+            ready = u.up;
+            begin<T, WIDE>(p, ring, m, r, true, ready);
+            if (turning) prefetch_unit(m);
+        };
         for (int at = v.first; at < v.end; at += 16) {
-            const bool last = at + 16 >= v.end;
-            // behind the product: the first stages of the next unit, or of this one for its next rows. They are on their way while the
-            // results are taken out.
-            auto then = [&]() {
-                if (!last) {
-                    r = rows_of<T, WIDE>(p, s, v, at + 16);
-                    begin<T, WIDE>(p, ring, m, r, true, true);
-                    return;
-                }
-                ticket = s.ticket;
-                if (ticket >= units) return;
-                u = unit_of(p, s, ticket, ups);
-                m = matrix_of<T, WIDE>(p, u);
-                r = rows_of<T, WIDE>(p, s, u, u.first);
-                ready = u.up;
-                begin<T, WIDE>(p, ring, m, r, true, ready);
-                if (v.up && !u.up) prefetch_unit(m);
-            };
-            auto run = [&](auto blocks) {
-                constexpr int NB = decltype(blocks)::value;
-                float acc[4][NB][4];
-                if (v.up) product<T, WIDE, NB, true>(p, ring, m, r, all, acc);
-                else product<T, WIDE, NB, false>(p, ring, m, r, all, acc);
-                if (last && threadIdx.x == 0) s.ticket = ahead;
-                if (v.up) put_up<T, NB>(p, s, v, at, acc, then);
-                else put_down<NB>(p, s, v, at, acc, then);
-            };
-            if (v.end - at <= 8) run(std::integral_constant<int, 1>());
-            else run(std::integral_constant<int, 2>());
+            const bool last = at + 16 >= v.end, two_blocks = v.end - at > 8;
+            float acc[4][2][4];
+            product<T, WIDE>(p, ring, m, r, all, two_blocks, acc);
             all = false;
+            if (last && threadIdx.x == 0) s.ticket = ahead;
+            turn_in(s.turn, acc, 0);
+            __syncthreads();
+            // Copies are on their way while results are taken out. Only where the next unit waits for first products, this one's are given
+            // to the others first: all CTAs come to that point at the same time.
+            if (last) {
+                ticket = s.ticket;
+                turning = v.up && ticket >= ups;
+                if (!turning) go_on();
+            } else {
+                r = rows_of<T, WIDE>(p, s, v, at + 16);
+                begin<T, WIDE>(p, ring, m, r, true, true);
+            }
+            turn_out<T, WIDE>(p, s, v, at);
+            __syncthreads();                     // the sums have been read, and what they gave is written
+            if (two_blocks) {
+                turn_in(s.turn, acc, 1);
+                __syncthreads();
+                turn_out<T, WIDE>(p, s, v, at + 8);
+                __syncthreads();
+            }
         }
         // Thread 0 tells the others that the unit is done, while its CTA goes on; whether the unit was the last of its columns the CTA
         // looks at after the next one.
@@ -837,6 +837,7 @@ k_experts(const __grid_constant__ Layer p) {
             if (v.up) add_release(done + v.number);
             else if (add_acquire_release(columns + v.block) == actives - 1) s.last[round] = v.block;
         }
+        if (turning) go_on();
         if (ticket >= units) break;
         round ^= 1;
     }
