@@ -6,12 +6,14 @@
 //   release:  x read back
 //
 // One pass each, bound by memory. A lane has eight neighbouring columns (16 bytes of a 16-bit type), four lanes a block of 32; where rows
-// do not start at multiples of eight values it has one column, and a warp a block. The largest of a block is a maximum over those
-// lanes, so the codes leave in the pass that reads the values. The arithmetic is in fp32 and every result is rounded once.
+// do not start at multiples of eight values a lane has one column of each of four blocks, and a warp a block, so that it reads and writes
+// side by side with the others. The largest of a block is a maximum over those lanes, so the codes leave in the pass that reads the
+// values. The arithmetic is in fp32 and every result is rounded once.
 
 #include "held.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fmb {
 namespace held {
@@ -27,15 +29,60 @@ struct Grid {
     int lanes, width, columns, parts;            // width: of a part
 };
 
+// A lane's N values as they are in memory, two to a word where they have 16 bits, so that what is on its way takes few registers
+template <typename T, int N> struct Raw {
+    static constexpr int kWords = (N * (int)sizeof(T) + 3) / 4;
+    uint32_t v[kWords];
+};
+
 template <typename T, int N>
-__device__ __forceinline__ void load(const T* __restrict__ at, int live, float (&x)[N]) {
-    if (live >= N) {
-        const Pack<T, N> in = *reinterpret_cast<const Pack<T, N>*>(at);
+__device__ __forceinline__ Raw<T, N> load(const T* __restrict__ at, int live) {
+    using R = Raw<T, N>;
+    R in = {};
+    if constexpr (N == 8) {
+        if (live >= N) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = to_float(in.v[i]);
+            for (int i = 0; i < R::kWords; i += 4) {
+                const uint4 four = __ldg(reinterpret_cast<const uint4*>(at) + i / 4);
+                in.v[i] = four.x; in.v[i + 1] = four.y; in.v[i + 2] = four.z; in.v[i + 3] = four.w;
+            }
+            return in;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i >= live) break;
+        if constexpr (sizeof(T) == 4) in.v[i] = __ldg(reinterpret_cast<const uint32_t*>(at) + i);
+        else in.v[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at) + i) << (16 * (i % 2));
+    }
+    return in;
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void unpack(const Raw<T, N>& in, float (&x)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t w = in.v[i * sizeof(T) / 4];
+        if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w);
+        else if constexpr (std::is_same<T, __nv_bfloat16>::value) x[i] = __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
+        else x[i] = __half2float(__ushort_as_half((uint16_t)(i % 2 ? w >> 16 : w & 0xffffu)));
+    }
+}
+
+// the largest of |x|, as the bits of a float; NaN and infinities are larger than what is finite
+template <typename T, int N>
+__device__ __forceinline__ uint32_t largest_of(const Raw<T, N>& in) {
+    uint32_t largest = 0;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) largest = max(largest, in.v[i] & 0x7fffffffu);
+        return largest;
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] = i < live ? to_float(at[i]) : 0.0f;
+        for (int i = 0; i < Raw<T, N>::kWords; ++i) largest = __vmaxu2(largest, in.v[i] & 0x7fff7fffu);
+        largest = max(largest >> 16, largest & 0xffffu);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return largest << 16;
+        else return __float_as_uint(__half2float(__ushort_as_half((uint16_t)largest)));
     }
 }
 
@@ -55,32 +102,50 @@ __device__ __forceinline__ void store(T* __restrict__ at, int live, const float 
 
 // Codes of this lane's values and the block's exponent, by all lanes of the warp; `live` of the values exist, the others are zero.
 template <typename T, int N>
-__device__ __forceinline__ void hold(const float (&x)[N], int live, bool block_exists, uint8_t* __restrict__ codes, uint8_t* __restrict__ exponent) {
+__device__ __forceinline__ void hold(const Raw<T, N>& raw, const float (&x)[N], int live, bool block_exists, uint8_t* __restrict__ codes,
+                                     uint8_t* __restrict__ exponent) {
     constexpr int kLanes = kBlock / N;
-    uint32_t largest = 0;
+    constexpr uint32_t kInfinity = 0x7f800000u;
+    auto over_block = [](uint32_t v) {
+        if constexpr (kLanes == 32) {
+            return __reduce_max_sync(0xffffffffu, v);
+        } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint32_t bits = __float_as_uint(x[i]) & 0x7fffffffu;
-        if (bits < 0x7f800000u) largest = max(largest, bits);
-    }
-#pragma unroll
-    for (int o = 1; o < kLanes; o <<= 1) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-    // largest = m 2^E: 448 = 1.75 x 2^8 units hold it at e = E - 8 where m <= 1.75
-    const int e = min(max((int)((largest + 0x1fffffu) >> 23) - kBias - 8, Units<T>::kLowest), Units<T>::kHighest);
-    const float inverse = unit_of(kBias - e), most = e == Units<T>::kHighest ? 240.0f : 448.0f;
-    uint32_t out[(N + 3) / 4];
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-        float v[2];
-        uint32_t nan = 0;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const float value = i + j < N ? x[i + j] : 0.0f;
-            if ((__float_as_uint(value) & 0x7fffffffu) >= 0x7f800000u) nan |= 0x7fu << (8 * j);
-            v[j] = fminf(fmaxf(value * inverse, -most), most);
+            for (int o = 1; o < kLanes; o <<= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+            return v;
         }
-        const uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(v[0], v[1]), __NV_SATFINITE, __NV_E4M3) | nan;
+    };
+    // largest = m 2^E: 448 = 1.75 x 2^8 units hold it at e = E - 8 where m <= 1.75
+    auto exponent_of = [](uint32_t largest) { return min(max((int)((largest + 0x1fffffu) >> 23) - kBias - 8, Units<T>::kLowest), Units<T>::kHighest); };
+    uint32_t largest = over_block(largest_of<T, N>(raw));
+    int e = exponent_of(largest);
+    uint32_t out[(N + 3) / 4];
+    auto put = [&](int i, uint32_t two) {
         if (i % 4 == 0) out[i / 4] = two; else out[i / 4] |= two << 16;
+    };
+    // What is not finite does not count for the unit and is NaN; in the highest unit codes end at 240. Neither is met often.
+    if (__any_sync(0xffffffffu, e == Units<T>::kHighest)) {
+        largest = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const uint32_t bits = __float_as_uint(x[i]) & 0x7fffffffu;
+            if (bits < kInfinity) largest = max(largest, bits);
+        }
+        e = exponent_of(over_block(largest));
+        const float inverse = unit_of(kBias - e), most = e == Units<T>::kHighest ? 240.0f : 448.0f;
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            const float y = i + 1 < N ? x[i + 1 < N ? i + 1 : i] : 0.0f;
+            uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(fminf(fmaxf(x[i] * inverse, -most), most), fminf(fmaxf(y * inverse, -most), most)), __NV_SATFINITE, __NV_E4M3);
+            if ((__float_as_uint(x[i]) & 0x7fffffffu) >= kInfinity) two |= 0x7f;
+            if ((__float_as_uint(y) & 0x7fffffffu) >= kInfinity) two |= 0x7f00;
+            put(i, two);
+        }
+    } else {
+        const float inverse = unit_of(kBias - e);
+#pragma unroll
+        for (int i = 0; i < N; i += 2)
+            put(i, __nv_cvt_float2_to_fp8x2(make_float2(x[i] * inverse, i + 1 < N ? x[i + 1 < N ? i + 1 : i] * inverse : 0.0f), __NV_SATFINITE, __NV_E4M3));
     }
     if (live >= N && N == 8) {
         *reinterpret_cast<uint2*>(codes) = make_uint2(out[0], out[(N + 3) / 4 - 1]);
@@ -92,37 +157,67 @@ __device__ __forceinline__ void hold(const float (&x)[N], int live, bool block_e
     if (block_exists && (threadIdx.x & (kLanes - 1)) == 0) *exponent = (uint8_t)(e + kBias);
 }
 
+// a lane's codes, and its values of them
+template <int N> struct Codes {
+    uint32_t v[(N + 3) / 4], byte;
+};
+
 template <int N>
-__device__ __forceinline__ void release(const uint8_t* __restrict__ codes, int live, int byte, float (&x)[N]) {
-    const float unit = unit_of(byte);
-    uint32_t in[(N + 3) / 4] = {};
+__device__ __forceinline__ Codes<N> load_codes(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponent, int live) {
+    Codes<N> in = {};
+    if (live <= 0) return in;
+    in.byte = __ldg(exponent);
     if (live >= N && N == 8) {
-        const uint2 v = *reinterpret_cast<const uint2*>(codes);
-        in[0] = v.x;
-        in[(N + 3) / 4 - 1] = v.y;
+        const uint2 v = __ldg(reinterpret_cast<const uint2*>(codes));
+        in.v[0] = v.x;
+        in.v[(N + 3) / 4 - 1] = v.y;
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
-            if (i < live) in[i / 4] |= (uint32_t)codes[i] << (8 * (i % 4));
+            if (i < live) in.v[i / 4] |= (uint32_t)__ldg(codes + i) << (8 * (i % 4));
     }
+    return in;
+}
+
+template <int N>
+__device__ __forceinline__ void release(const Codes<N>& in, float (&x)[N]) {
+    const float unit = unit_of(in.byte);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-        const float2 v = two_values(in[i / 4] >> (8 * (i % 4)));
+        const float2 v = two_values(in.v[i / 4] >> (8 * (i % 4)));
         x[i] = v.x * unit;
-        if (i + 1 < N) x[i + 1] = v.y * unit;
+        if (i + 1 < N) x[i + 1 < N ? i + 1 : i] = v.y * unit;
     }
 }
 
-// Rows of this thread, the same number for all threads of a CTA, and columns of each: what is past the last has none to load or store.
-template <typename F>
-__device__ __forceinline__ void walk(const Grid& g, long long rows, int n, F body) {
-    const int per_cta = kThreads / g.lanes, part = threadIdx.x & (g.lanes - 1), whole = blocks_of(g.width) * kBlock;
-    for (long long r0 = (long long)blockIdx.x * per_cta; r0 < rows; r0 += (long long)gridDim.x * per_cta) {
+// Places of a thread, whose loads are on their way together: N neighbouring columns of two rows, or one column of four blocks of a row
+template <int N> constexpr int kPlaces = N == 1 ? 4 : 2;
+
+struct Place {
+    long long row;
+    int column, live;                            // columns that exist from there on
+    bool exists;                                 // the block does
+};
+
+// The same number of rounds for all threads of a CTA; what is past the last row or block has nothing to load or store.
+template <int N, typename F>
+__device__ __forceinline__ void walk(const Grid& g, long long rows, F body) {
+    constexpr int kOfRow = N == 1 ? kPlaces<N> : 1, kRowsAtOnce = kPlaces<N> / kOfRow;
+    const int per_cta = kThreads / g.lanes, whole = blocks_of(g.width) * kBlock;
+    const int part = threadIdx.x & (g.lanes - 1), first = N == 1 ? part / 32 * 32 * kOfRow + part % 32 : part * N;
+    for (long long r0 = (long long)blockIdx.x * per_cta * kRowsAtOnce; r0 < rows; r0 += (long long)gridDim.x * per_cta * kRowsAtOnce) {
         const long long r = r0 + threadIdx.x / g.lanes;
-        for (int c0 = 0; c0 < whole; c0 += g.lanes * n) {
-            const int c = c0 + part * n;
-            const bool exists = r < rows && c < whole;
-            body(r, c, exists ? g.width - c : 0, exists);
+        for (int c0 = 0; c0 < whole; c0 += g.lanes * N * kOfRow) {
+            if (N == 1 && c0 + first - part % 32 >= whole) continue;             // (the same for a warp)
+            Place at[kPlaces<N>];
+#pragma unroll
+            for (int q = 0; q < kPlaces<N>; ++q) {
+                at[q].row = r + (N == 1 ? 0 : q * per_cta);
+                at[q].column = c0 + first + (N == 1 ? q * kBlock : 0);
+                at[q].exists = at[q].row < rows && at[q].column < whole;
+                at[q].live = at[q].exists ? g.width - at[q].column : 0;
+            }
+            body(at);
         }
     }
 }
@@ -131,12 +226,18 @@ template <typename T, int N>
 __global__ void __launch_bounds__(kThreads)
 k_hold(fmb_held_t a, Grid g) {
     const int blocks = blocks_of(g.width);
-    walk(g, (long long)a.rows * g.parts, N, [&](long long r, int c, int live, bool exists) {
-        const long long row = g.parts == 2 ? r >> 1 : r;
-        const int first = g.parts == 2 && (r & 1) ? g.width : 0;
-        float v[N];
-        load<T, N>((const T*)a.x + row * a.x_stride + first + c, live, v);
-        hold<T, N>(v, live, exists, a.codes + row * a.columns + first + c, a.exponents + r * blocks + c / kBlock);
+    walk<N>(g, (long long)a.rows * g.parts, [&](const Place (&at)[kPlaces<N>]) {
+        auto row = [&](const Place& p) { return g.parts == 2 ? p.row >> 1 : p.row; };
+        auto column = [&](const Place& p) { return (g.parts == 2 && (p.row & 1) ? g.width : 0) + p.column; };
+        Raw<T, N> raw[kPlaces<N>];
+#pragma unroll
+        for (int q = 0; q < kPlaces<N>; ++q) raw[q] = load<T, N>((const T*)a.x + row(at[q]) * a.x_stride + column(at[q]), at[q].live);
+#pragma unroll
+        for (int q = 0; q < kPlaces<N>; ++q) {
+            float x[N];
+            unpack<T, N>(raw[q], x);
+            hold<T, N>(raw[q], x, at[q].live, at[q].exists, a.codes + row(at[q]) * a.columns + column(at[q]), a.exponents + at[q].row * blocks + at[q].column / kBlock);
+        }
     });
 }
 
@@ -145,37 +246,58 @@ __global__ void __launch_bounds__(kThreads)
 k_release(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, int rows, int columns, T* __restrict__ out,
           long long stride, Grid g) {
     const int blocks = blocks_of(g.width);
-    walk(g, (long long)rows * g.parts, N, [&](long long r, int c, int live, bool exists) {
-        if (!exists) return;
-        const long long row = g.parts == 2 ? r >> 1 : r;
-        const int first = g.parts == 2 && (r & 1) ? g.width : 0;
-        float v[N];
-        release<N>(codes + row * columns + first + c, live, exponents[r * blocks + c / kBlock], v);
-        store<T, N>(out + row * stride + first + c, live, v);
+    walk<N>(g, (long long)rows * g.parts, [&](const Place (&at)[kPlaces<N>]) {
+        auto row = [&](const Place& p) { return g.parts == 2 ? p.row >> 1 : p.row; };
+        auto column = [&](const Place& p) { return (g.parts == 2 && (p.row & 1) ? g.width : 0) + p.column; };
+        Codes<N> in[kPlaces<N>];
+#pragma unroll
+        for (int q = 0; q < kPlaces<N>; ++q)
+            in[q] = load_codes<N>(codes + row(at[q]) * columns + column(at[q]), exponents + at[q].row * blocks + at[q].column / kBlock, at[q].live);
+#pragma unroll
+        for (int q = 0; q < kPlaces<N>; ++q) {
+            float x[N];
+            release<N>(in[q], x);
+            store<T, N>(out + row(at[q]) * stride + column(at[q]), at[q].live, x);
+        }
     });
 }
 
-// 1 / (1 + exp(-x)): in float32 to its last bits; where results have 16 bits, by the fast exponential and division
-template <typename T> __device__ __forceinline__ float sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(-x)); }
+// 1 / (1 + exp(-x)): in float32 to its last bits; where results have 16 bits, by the approximate exponential and reciprocal (2 and 1 ulp, and
+// |x| 2^-24 for x log2 e)
+template <typename T> __device__ __forceinline__ float sigmoid(float x) {
+    float power, s;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(power) : "f"(x * -1.44269504088896341f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(s) : "f"(1.0f + power));
+    return s;
+}
 template <> __device__ __forceinline__ float sigmoid<float>(float x) { return 1.0f / (1.0f + expf(-x)); }
 
 template <typename T, int N, bool HOLD>
 __global__ void __launch_bounds__(kThreads)
 k_gate(fmb_held_t a, Grid g) {
     const int blocks = blocks_of(g.width);
-    walk(g, a.rows, N, [&](long long r, int c, int live, bool exists) {
-        const T* const u = (const T*)a.x + r * a.x_stride + c;
-        float x[N], y[N], h[N];
-        load<T, N>(u, live, x);
-        load<T, N>(u + g.width, live, y);
+    walk<N>(g, a.rows, [&](const Place (&at)[kPlaces<N>]) {
+        Raw<T, N> raw[kPlaces<N>][2];
 #pragma unroll
-        for (int i = 0; i < N; ++i) h[i] = x[i] * sigmoid<T>(x[i]) * y[i];
-        store<T, N>((T*)a.h + r * a.h_stride + c, live, h);
-        if (HOLD) {
-            uint8_t* const codes = a.codes + r * a.columns + c;
-            uint8_t* const exponents = a.exponents + 2 * r * blocks + c / kBlock;
-            hold<T, N>(x, live, exists, codes, exponents);
-            hold<T, N>(y, live, exists, codes + g.width, exponents + blocks);
+        for (int q = 0; q < kPlaces<N>; ++q) {
+            const T* const u = (const T*)a.x + at[q].row * a.x_stride + at[q].column;
+            raw[q][0] = load<T, N>(u, at[q].live);
+            raw[q][1] = load<T, N>(u + g.width, at[q].live);
+        }
+#pragma unroll
+        for (int q = 0; q < kPlaces<N>; ++q) {
+            float x[N], y[N], h[N];
+            unpack<T, N>(raw[q][0], x);
+            unpack<T, N>(raw[q][1], y);
+#pragma unroll
+            for (int i = 0; i < N; ++i) h[i] = x[i] * sigmoid<T>(x[i]) * y[i];
+            store<T, N>((T*)a.h + at[q].row * a.h_stride + at[q].column, at[q].live, h);
+            if (HOLD) {
+                uint8_t* const codes = a.codes + at[q].row * a.columns + at[q].column;
+                uint8_t* const exponents = a.exponents + 2 * at[q].row * blocks + at[q].column / kBlock;
+                hold<T, N>(raw[q][0], x, at[q].live, at[q].exists, codes, exponents);
+                hold<T, N>(raw[q][1], y, at[q].live, at[q].exists, codes + g.width, exponents + blocks);
+            }
         }
     });
 }
@@ -184,31 +306,46 @@ template <typename T, int N, bool HELD>
 __global__ void __launch_bounds__(kThreads)
 k_gate_gradient(fmb_held_t a, Grid g) {
     const int blocks = blocks_of(g.width);
-    walk(g, a.rows, N, [&](long long r, int c, int live, bool exists) {
-        if (!exists) return;
-        float x[N], y[N], dh[N], h[N];
-        load<T, N>((const T*)a.dh + r * a.dh_stride + c, live, dh);
-        if (HELD) {
-            const uint8_t* const codes = a.codes + r * a.columns + c;
-            const uint8_t* const exponents = a.exponents + 2 * r * blocks + c / kBlock;
-            release<N>(codes, live, exponents[0], x);
-            release<N>(codes + g.width, live, exponents[blocks], y);
-        } else {
-            const T* const u = (const T*)a.x + r * a.x_stride + c;
-            load<T, N>(u, live, x);
-            load<T, N>(u + g.width, live, y);
+    walk<N>(g, a.rows, [&](const Place (&at)[kPlaces<N>]) {
+        Raw<T, N> dh_raw[kPlaces<N>], raw[kPlaces<N>][2];
+        Codes<N> codes[kPlaces<N>][2];
+#pragma unroll
+        for (int q = 0; q < kPlaces<N>; ++q) {
+            dh_raw[q] = load<T, N>((const T*)a.dh + at[q].row * a.dh_stride + at[q].column, at[q].live);
+            if (HELD) {
+                const uint8_t* const from = a.codes + at[q].row * a.columns + at[q].column;
+                const uint8_t* const exponents = a.exponents + 2 * at[q].row * blocks + at[q].column / kBlock;
+                codes[q][0] = load_codes<N>(from, exponents, at[q].live);
+                codes[q][1] = load_codes<N>(from + g.width, exponents + blocks, at[q].live);
+            } else {
+                const T* const u = (const T*)a.x + at[q].row * a.x_stride + at[q].column;
+                raw[q][0] = load<T, N>(u, at[q].live);
+                raw[q][1] = load<T, N>(u + g.width, at[q].live);
+            }
         }
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float s = sigmoid<T>(x[i]), silu = x[i] * s;
-            h[i] = silu * y[i];
-            y[i] = dh[i] * y[i] * s * (1.0f + x[i] * (1.0f - s));
-            x[i] = dh[i] * silu;
+        for (int q = 0; q < kPlaces<N>; ++q) {
+            float x[N], y[N], dh[N], h[N];
+            unpack<T, N>(dh_raw[q], dh);
+            if (HELD) {
+                release<N>(codes[q][0], x);
+                release<N>(codes[q][1], y);
+            } else {
+                unpack<T, N>(raw[q][0], x);
+                unpack<T, N>(raw[q][1], y);
+            }
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const float s = sigmoid<T>(x[i]), silu = x[i] * s;
+                h[i] = silu * y[i];
+                y[i] = dh[i] * y[i] * s * (1.0f + x[i] * (1.0f - s));
+                x[i] = dh[i] * silu;
+            }
+            T* const du = (T*)a.du + at[q].row * a.du_stride + at[q].column;
+            store<T, N>(du, at[q].live, y);
+            store<T, N>(du + g.width, at[q].live, x);
+            if (a.h) store<T, N>((T*)a.h + at[q].row * a.h_stride + at[q].column, at[q].live, h);
         }
-        T* const du = (T*)a.du + r * a.du_stride + c;
-        store<T, N>(du, live, y);
-        store<T, N>(du + g.width, live, x);
-        if (a.h) store<T, N>((T*)a.h + r * a.h_stride + c, live, h);
     });
 }
 
@@ -222,7 +359,8 @@ Grid grid_of(int columns, int parts, int n) {
     g.parts = parts;
     g.width = columns / parts;
     g.lanes = kBlock / n;
-    while (g.lanes < kThreads && g.lanes * n < g.width) g.lanes *= 2;
+    const int columns_of_lane = n == 1 ? kPlaces<1> : n;
+    while (g.lanes < kThreads && g.lanes * columns_of_lane < g.width) g.lanes *= 2;
     return g;
 }
 
