@@ -5,10 +5,11 @@
 //   gradient: da = dh b s (1 + a (1 - s)), db = dh a s with s = 1 / (1 + exp(-a)), from held u (or u itself), and h anew
 //   release:  x read back
 //
-// One pass each, bound by memory. A lane has eight neighbouring columns (16 bytes of a 16-bit type), four lanes a block of 32; where rows
-// do not start at multiples of eight values a lane has one column of each of four blocks, and a warp a block, so that it reads and writes
-// side by side with the others. The largest of a block is a maximum over those lanes, so the codes leave in the pass that reads the
-// values. The arithmetic is in fp32 and every result is rounded once.
+// One pass each, bound by memory. A lane has eight neighbouring columns of two rows, 16 bytes of a 16-bit type, four lanes a block of 32;
+// where rows do not start at multiples of eight values (not WIDE) it takes them by the words and halves that they lie in (a column a
+// lane, side by side with the others, takes four times the instructions: 20,000 rows of 2 x 1,001 in 80 us). The largest of
+// a block is a maximum over its lanes, so the codes leave in the pass that reads the values. The arithmetic is in fp32 and
+// every result is rounded once.
 
 #include "held.cuh"
 
@@ -22,35 +23,50 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <typename T, int N> struct alignas(N * sizeof(T) < 16 ? N * sizeof(T) : 16) Pack { T v[N]; };
+constexpr int kEach = 8;                         // columns of a lane
+constexpr int kLanes = kBlock / kEach;
 
 // A CTA's threads by rows: `lanes` (a power of two, whole blocks) for the columns of one, 256 / lanes rows at a time.
 struct Grid {
     int lanes, width, columns, parts;            // width: of a part
 };
 
-// A lane's N values as they are in memory, two to a word where they have 16 bits, so that what is on its way takes few registers
-template <typename T, int N> struct Raw {
-    static constexpr int kWords = (N * (int)sizeof(T) + 3) / 4;
+// A lane's values as they are in memory, two to a word where they have 16 bits, so that what is on its way takes few registers
+template <typename T> struct Raw {
+    static constexpr int kWords = kEach * (int)sizeof(T) / 4;
     uint32_t v[kWords];
 };
 
-template <typename T, int N>
-__device__ __forceinline__ Raw<T, N> load(const T* __restrict__ at, int live) {
-    using R = Raw<T, N>;
-    R in = {};
-    if constexpr (N == 8) {
-        if (live >= N) {
+template <typename T, bool WIDE>
+__device__ __forceinline__ Raw<T> load(const T* __restrict__ at, int live) {
+    Raw<T> in = {};
+    if (live >= kEach) {
+        if constexpr (WIDE) {
 #pragma unroll
-            for (int i = 0; i < R::kWords; i += 4) {
+            for (int i = 0; i < Raw<T>::kWords; i += 4) {
                 const uint4 four = __ldg(reinterpret_cast<const uint4*>(at) + i / 4);
                 in.v[i] = four.x; in.v[i + 1] = four.y; in.v[i + 2] = four.z; in.v[i + 3] = four.w;
             }
-            return in;
+        } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < kEach; ++i) in.v[i] = __ldg(reinterpret_cast<const uint32_t*>(at) + i);
+        } else if ((uintptr_t)at & 2) {
+            // three words between two halves
+            const uint32_t* const words = reinterpret_cast<const uint32_t*>(reinterpret_cast<const uint16_t*>(at) + 1);
+            const uint32_t first = __ldg(reinterpret_cast<const uint16_t*>(at)), last = __ldg(reinterpret_cast<const uint16_t*>(at) + 7);
+            const uint32_t a = __ldg(words), b = __ldg(words + 1), c = __ldg(words + 2);
+            in.v[0] = first | a << 16;
+            in.v[1] = __funnelshift_r(a, b, 16);
+            in.v[2] = __funnelshift_r(b, c, 16);
+            in.v[3] = c >> 16 | last << 16;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) in.v[i] = __ldg(reinterpret_cast<const uint32_t*>(at) + i);
         }
+        return in;
     }
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < kEach; ++i) {
         if (i >= live) break;
         if constexpr (sizeof(T) == 4) in.v[i] = __ldg(reinterpret_cast<const uint32_t*>(at) + i);
         else in.v[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at) + i) << (16 * (i % 2));
@@ -58,10 +74,10 @@ __device__ __forceinline__ Raw<T, N> load(const T* __restrict__ at, int live) {
     return in;
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void unpack(const Raw<T, N>& in, float (&x)[N]) {
+template <typename T>
+__device__ __forceinline__ void unpack(const Raw<T>& in, float (&x)[kEach]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
+    for (int i = 0; i < kEach; ++i) {
         const uint32_t w = in.v[i * sizeof(T) / 4];
         if constexpr (sizeof(T) == 4) x[i] = __uint_as_float(w);
         else if constexpr (std::is_same<T, __nv_bfloat16>::value) x[i] = __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
@@ -69,129 +85,163 @@ __device__ __forceinline__ void unpack(const Raw<T, N>& in, float (&x)[N]) {
     }
 }
 
+template <typename T, bool WIDE>
+__device__ __forceinline__ void store(T* __restrict__ at, int live, const float (&x)[kEach]) {
+    uint32_t v[Raw<T>::kWords];
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kWords; ++i) {
+        if constexpr (sizeof(T) == 4) v[i] = __float_as_uint(x[i]);
+        else v[i] = two_of<T>(x[2 * i], x[2 * i + 1]);
+    }
+    if (live >= kEach) {
+        if constexpr (WIDE) {
+#pragma unroll
+            for (int i = 0; i < Raw<T>::kWords; i += 4) *(reinterpret_cast<uint4*>(at) + i / 4) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+        } else if (sizeof(T) == 2 && (uintptr_t)at & 2) {
+            uint16_t* const halves = reinterpret_cast<uint16_t*>(at);
+            uint32_t* const words = reinterpret_cast<uint32_t*>(halves + 1);
+            halves[0] = (uint16_t)v[0];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) words[i] = __funnelshift_r(v[i], v[i + 1 < Raw<T>::kWords ? i + 1 : i], 16);
+            halves[7] = (uint16_t)(v[3] >> 16);
+        } else {
+#pragma unroll
+            for (int i = 0; i < Raw<T>::kWords; ++i) reinterpret_cast<uint32_t*>(at)[i] = v[i];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+        if (i >= live) break;
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(at)[i] = v[i];
+        else reinterpret_cast<uint16_t*>(at)[i] = (uint16_t)(v[i / 2] >> (16 * (i % 2)));
+    }
+}
+
+// eight codes, by words, halves and bytes as they lie
+template <bool WIDE>
+__device__ __forceinline__ void store_codes(uint8_t* __restrict__ at, int live, uint32_t low, uint32_t high) {
+    const unsigned from = (unsigned)(uintptr_t)at & 3;
+    if (live >= kEach && WIDE) {
+        *reinterpret_cast<uint2*>(at) = make_uint2(low, high);
+    } else if (live >= kEach && from == 0) {
+        reinterpret_cast<uint32_t*>(at)[0] = low;
+        reinterpret_cast<uint32_t*>(at)[1] = high;
+    } else if (live >= kEach) {
+        // up to the next word; a word; what is left
+        const unsigned before = 4 - from;        // bytes, 1 to 3
+        if (before & 1) at[0] = (uint8_t)low;
+        if (before & 2) *reinterpret_cast<uint16_t*>(at + (before & 1)) = (uint16_t)(low >> (8 * (before & 1)));
+        *reinterpret_cast<uint32_t*>(at + before) = __funnelshift_r(low, high, 8 * before);
+        const uint32_t rest = high >> (8 * before);               // 4 - before bytes
+        if (from & 2) *reinterpret_cast<uint16_t*>(at + before + 4) = (uint16_t)rest;
+        if (from & 1) at[before + 4 + (from & 2)] = (uint8_t)(rest >> (8 * (from & 2)));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (i < live) at[i] = (uint8_t)((i < 4 ? low : high) >> (8 * (i % 4)));
+    }
+}
+
 // the largest of |x|, as the bits of a float; NaN and infinities are larger than what is finite
-template <typename T, int N>
-__device__ __forceinline__ uint32_t largest_of(const Raw<T, N>& in) {
+template <typename T>
+__device__ __forceinline__ uint32_t largest_of(const Raw<T>& in) {
     uint32_t largest = 0;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < N; ++i) largest = max(largest, in.v[i] & 0x7fffffffu);
+        for (int i = 0; i < kEach; ++i) largest = max(largest, in.v[i] & 0x7fffffffu);
         return largest;
     } else {
 #pragma unroll
-        for (int i = 0; i < Raw<T, N>::kWords; ++i) largest = __vmaxu2(largest, in.v[i] & 0x7fff7fffu);
+        for (int i = 0; i < Raw<T>::kWords; ++i) largest = __vmaxu2(largest, in.v[i] & 0x7fff7fffu);
         largest = max(largest >> 16, largest & 0xffffu);
         if constexpr (std::is_same<T, __nv_bfloat16>::value) return largest << 16;
         else return __float_as_uint(__half2float(__ushort_as_half((uint16_t)largest)));
     }
 }
 
-template <typename T, int N>
-__device__ __forceinline__ void store(T* __restrict__ at, int live, const float (&x)[N]) {
-    if (live >= N) {
-        Pack<T, N> out;
-#pragma unroll
-        for (int i = 0; i < N; ++i) out.v[i] = rounded<T>(x[i]);
-        *reinterpret_cast<Pack<T, N>*>(at) = out;
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < live) at[i] = rounded<T>(x[i]);
-    }
-}
-
 // Codes of this lane's values and the block's exponent, by all lanes of the warp; `live` of the values exist, the others are zero.
-template <typename T, int N>
-__device__ __forceinline__ void hold(const Raw<T, N>& raw, const float (&x)[N], int live, bool block_exists, uint8_t* __restrict__ codes,
+template <typename T, bool WIDE>
+__device__ __forceinline__ void hold(const Raw<T>& raw, const float (&x)[kEach], int live, bool block_exists, uint8_t* __restrict__ codes,
                                      uint8_t* __restrict__ exponent) {
-    constexpr int kLanes = kBlock / N;
     constexpr uint32_t kInfinity = 0x7f800000u;
     auto over_block = [](uint32_t v) {
-        if constexpr (kLanes == 32) {
-            return __reduce_max_sync(0xffffffffu, v);
-        } else {
 #pragma unroll
-            for (int o = 1; o < kLanes; o <<= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-            return v;
-        }
+        for (int o = 1; o < kLanes; o <<= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
     };
     // largest = m 2^E: 448 = 1.75 x 2^8 units hold it at e = E - 8 where m <= 1.75
     auto exponent_of = [](uint32_t largest) { return min(max((int)((largest + 0x1fffffu) >> 23) - kBias - 8, Units<T>::kLowest), Units<T>::kHighest); };
-    uint32_t largest = over_block(largest_of<T, N>(raw));
+    uint32_t largest = over_block(largest_of<T>(raw));
     int e = exponent_of(largest);
-    uint32_t out[(N + 3) / 4];
-    auto put = [&](int i, uint32_t two) {
-        if (i % 4 == 0) out[i / 4] = two; else out[i / 4] |= two << 16;
-    };
+    uint32_t two[kEach / 2];
     // What is not finite does not count for the unit and is NaN; in the highest unit codes end at 240. Neither is met often.
     if (__any_sync(0xffffffffu, e == Units<T>::kHighest)) {
         largest = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
+        for (int i = 0; i < kEach; ++i) {
             const uint32_t bits = __float_as_uint(x[i]) & 0x7fffffffu;
             if (bits < kInfinity) largest = max(largest, bits);
         }
         e = exponent_of(over_block(largest));
         const float inverse = unit_of(kBias - e), most = e == Units<T>::kHighest ? 240.0f : 448.0f;
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            const float y = i + 1 < N ? x[i + 1 < N ? i + 1 : i] : 0.0f;
-            uint32_t two = __nv_cvt_float2_to_fp8x2(make_float2(fminf(fmaxf(x[i] * inverse, -most), most), fminf(fmaxf(y * inverse, -most), most)), __NV_SATFINITE, __NV_E4M3);
-            if ((__float_as_uint(x[i]) & 0x7fffffffu) >= kInfinity) two |= 0x7f;
-            if ((__float_as_uint(y) & 0x7fffffffu) >= kInfinity) two |= 0x7f00;
-            put(i, two);
+        for (int i = 0; i < kEach; i += 2) {
+            two[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(fminf(fmaxf(x[i] * inverse, -most), most), fminf(fmaxf(x[i + 1] * inverse, -most), most)),
+                                                  __NV_SATFINITE, __NV_E4M3);
+            if ((__float_as_uint(x[i]) & 0x7fffffffu) >= kInfinity) two[i / 2] |= 0x7f;
+            if ((__float_as_uint(x[i + 1]) & 0x7fffffffu) >= kInfinity) two[i / 2] |= 0x7f00;
         }
     } else {
         const float inverse = unit_of(kBias - e);
 #pragma unroll
-        for (int i = 0; i < N; i += 2)
-            put(i, __nv_cvt_float2_to_fp8x2(make_float2(x[i] * inverse, i + 1 < N ? x[i + 1 < N ? i + 1 : i] * inverse : 0.0f), __NV_SATFINITE, __NV_E4M3));
+        for (int i = 0; i < kEach; i += 2) two[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(x[i] * inverse, x[i + 1] * inverse), __NV_SATFINITE, __NV_E4M3);
     }
-    if (live >= N && N == 8) {
-        *reinterpret_cast<uint2*>(codes) = make_uint2(out[0], out[(N + 3) / 4 - 1]);
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < live) codes[i] = (uint8_t)(out[i / 4] >> (8 * (i % 4)));
-    }
+    store_codes<WIDE>(codes, live, two[0] | two[1] << 16, two[2] | two[3] << 16);
     if (block_exists && (threadIdx.x & (kLanes - 1)) == 0) *exponent = (uint8_t)(e + kBias);
 }
 
 // a lane's codes, and its values of them
-template <int N> struct Codes {
-    uint32_t v[(N + 3) / 4], byte;
+struct Codes {
+    uint32_t low, high, byte;
 };
 
-template <int N>
-__device__ __forceinline__ Codes<N> load_codes(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponent, int live) {
-    Codes<N> in = {};
+template <bool WIDE>
+__device__ __forceinline__ Codes load_codes(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponent, int live) {
+    Codes in = {};
     if (live <= 0) return in;
     in.byte = __ldg(exponent);
-    if (live >= N && N == 8) {
+    if (live >= kEach && WIDE) {
         const uint2 v = __ldg(reinterpret_cast<const uint2*>(codes));
-        in.v[0] = v.x;
-        in.v[(N + 3) / 4 - 1] = v.y;
+        in.low = v.x;
+        in.high = v.y;
+    } else if (live >= kEach) {
+        // the words that they lie in: the outer two hold bytes of them, so they are there
+        const unsigned from = (unsigned)(uintptr_t)codes & 3;
+        const uint32_t* const words = reinterpret_cast<const uint32_t*>(codes - from);
+        const uint32_t a = __ldg(words), b = __ldg(words + 1), c = from ? __ldg(words + 2) : 0u;
+        in.low = __funnelshift_r(a, b, 8 * from);
+        in.high = __funnelshift_r(b, c, 8 * from);
     } else {
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-            if (i < live) in.v[i / 4] |= (uint32_t)__ldg(codes + i) << (8 * (i % 4));
+        for (int i = 0; i < kEach; ++i)
+            if (i < live) (i < 4 ? in.low : in.high) |= (uint32_t)__ldg(codes + i) << (8 * (i % 4));
     }
     return in;
 }
 
-template <int N>
-__device__ __forceinline__ void release(const Codes<N>& in, float (&x)[N]) {
+__device__ __forceinline__ void release(const Codes& in, float (&x)[kEach]) {
     const float unit = unit_of(in.byte);
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {
-        const float2 v = two_values(in.v[i / 4] >> (8 * (i % 4)));
+    for (int i = 0; i < kEach; i += 2) {
+        const float2 v = two_values((i < 4 ? in.low : in.high) >> (8 * (i % 4)));
         x[i] = v.x * unit;
-        if (i + 1 < N) x[i + 1 < N ? i + 1 : i] = v.y * unit;
+        x[i + 1] = v.y * unit;
     }
 }
 
-// Places of a thread, whose loads are on their way together: N neighbouring columns of two rows, or one column of four blocks of a row
-template <int N> constexpr int kPlaces = N == 1 ? 4 : 2;
+// Places of a thread, whose loads are on their way together: kEach neighbouring columns of two rows
+constexpr int kPlaces = 2;
 
 struct Place {
     long long row;
@@ -200,20 +250,17 @@ struct Place {
 };
 
 // The same number of rounds for all threads of a CTA; what is past the last row or block has nothing to load or store.
-template <int N, typename F>
+template <typename F>
 __device__ __forceinline__ void walk(const Grid& g, long long rows, F body) {
-    constexpr int kOfRow = N == 1 ? kPlaces<N> : 1, kRowsAtOnce = kPlaces<N> / kOfRow;
-    const int per_cta = kThreads / g.lanes, whole = blocks_of(g.width) * kBlock;
-    const int part = threadIdx.x & (g.lanes - 1), first = N == 1 ? part / 32 * 32 * kOfRow + part % 32 : part * N;
-    for (long long r0 = (long long)blockIdx.x * per_cta * kRowsAtOnce; r0 < rows; r0 += (long long)gridDim.x * per_cta * kRowsAtOnce) {
+    const int per_cta = kThreads / g.lanes, whole = blocks_of(g.width) * kBlock, first = (threadIdx.x & (g.lanes - 1)) * kEach;
+    for (long long r0 = (long long)blockIdx.x * per_cta * kPlaces; r0 < rows; r0 += (long long)gridDim.x * per_cta * kPlaces) {
         const long long r = r0 + threadIdx.x / g.lanes;
-        for (int c0 = 0; c0 < whole; c0 += g.lanes * N * kOfRow) {
-            if (N == 1 && c0 + first - part % 32 >= whole) continue;             // (the same for a warp)
-            Place at[kPlaces<N>];
+        for (int c0 = 0; c0 < whole; c0 += g.lanes * kEach) {
+            Place at[kPlaces];
 #pragma unroll
-            for (int q = 0; q < kPlaces<N>; ++q) {
-                at[q].row = r + (N == 1 ? 0 : q * per_cta);
-                at[q].column = c0 + first + (N == 1 ? q * kBlock : 0);
+            for (int q = 0; q < kPlaces; ++q) {
+                at[q].row = r + q * per_cta;
+                at[q].column = c0 + first;
                 at[q].exists = at[q].row < rows && at[q].column < whole;
                 at[q].live = at[q].exists ? g.width - at[q].column : 0;
             }
@@ -222,42 +269,42 @@ __device__ __forceinline__ void walk(const Grid& g, long long rows, F body) {
     }
 }
 
-template <typename T, int N>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads)
 k_hold(fmb_held_t a, Grid g) {
     const int blocks = blocks_of(g.width);
-    walk<N>(g, (long long)a.rows * g.parts, [&](const Place (&at)[kPlaces<N>]) {
+    walk(g, (long long)a.rows * g.parts, [&](const Place (&at)[kPlaces]) {
         auto row = [&](const Place& p) { return g.parts == 2 ? p.row >> 1 : p.row; };
         auto column = [&](const Place& p) { return (g.parts == 2 && (p.row & 1) ? g.width : 0) + p.column; };
-        Raw<T, N> raw[kPlaces<N>];
+        Raw<T> raw[kPlaces];
 #pragma unroll
-        for (int q = 0; q < kPlaces<N>; ++q) raw[q] = load<T, N>((const T*)a.x + row(at[q]) * a.x_stride + column(at[q]), at[q].live);
+        for (int q = 0; q < kPlaces; ++q) raw[q] = load<T, WIDE>((const T*)a.x + row(at[q]) * a.x_stride + column(at[q]), at[q].live);
 #pragma unroll
-        for (int q = 0; q < kPlaces<N>; ++q) {
-            float x[N];
-            unpack<T, N>(raw[q], x);
-            hold<T, N>(raw[q], x, at[q].live, at[q].exists, a.codes + row(at[q]) * a.columns + column(at[q]), a.exponents + at[q].row * blocks + at[q].column / kBlock);
+        for (int q = 0; q < kPlaces; ++q) {
+            float x[kEach];
+            unpack<T>(raw[q], x);
+            hold<T, WIDE>(raw[q], x, at[q].live, at[q].exists, a.codes + row(at[q]) * a.columns + column(at[q]), a.exponents + at[q].row * blocks + at[q].column / kBlock);
         }
     });
 }
 
-template <typename T, int N>
+template <typename T, bool WIDE>
 __global__ void __launch_bounds__(kThreads)
 k_release(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponents, int rows, int columns, T* __restrict__ out,
           long long stride, Grid g) {
     const int blocks = blocks_of(g.width);
-    walk<N>(g, (long long)rows * g.parts, [&](const Place (&at)[kPlaces<N>]) {
+    walk(g, (long long)rows * g.parts, [&](const Place (&at)[kPlaces]) {
         auto row = [&](const Place& p) { return g.parts == 2 ? p.row >> 1 : p.row; };
         auto column = [&](const Place& p) { return (g.parts == 2 && (p.row & 1) ? g.width : 0) + p.column; };
-        Codes<N> in[kPlaces<N>];
+        Codes in[kPlaces];
 #pragma unroll
-        for (int q = 0; q < kPlaces<N>; ++q)
-            in[q] = load_codes<N>(codes + row(at[q]) * columns + column(at[q]), exponents + at[q].row * blocks + at[q].column / kBlock, at[q].live);
+        for (int q = 0; q < kPlaces; ++q)
+            in[q] = load_codes<WIDE>(codes + row(at[q]) * columns + column(at[q]), exponents + at[q].row * blocks + at[q].column / kBlock, at[q].live);
 #pragma unroll
-        for (int q = 0; q < kPlaces<N>; ++q) {
-            float x[N];
-            release<N>(in[q], x);
-            store<T, N>(out + row(at[q]) * stride + column(at[q]), at[q].live, x);
+        for (int q = 0; q < kPlaces; ++q) {
+            float x[kEach];
+            release(in[q], x);
+            store<T, WIDE>(out + row(at[q]) * stride + column(at[q]), at[q].live, x);
         }
     });
 }
@@ -272,79 +319,79 @@ template <typename T> __device__ __forceinline__ float sigmoid(float x) {
 }
 template <> __device__ __forceinline__ float sigmoid<float>(float x) { return 1.0f / (1.0f + expf(-x)); }
 
-template <typename T, int N, bool HOLD>
+template <typename T, bool WIDE, bool HOLD>
 __global__ void __launch_bounds__(kThreads)
 k_gate(fmb_held_t a, Grid g) {
     const int blocks = blocks_of(g.width);
-    walk<N>(g, a.rows, [&](const Place (&at)[kPlaces<N>]) {
-        Raw<T, N> raw[kPlaces<N>][2];
+    walk(g, a.rows, [&](const Place (&at)[kPlaces]) {
+        Raw<T> raw[kPlaces][2];
 #pragma unroll
-        for (int q = 0; q < kPlaces<N>; ++q) {
+        for (int q = 0; q < kPlaces; ++q) {
             const T* const u = (const T*)a.x + at[q].row * a.x_stride + at[q].column;
-            raw[q][0] = load<T, N>(u, at[q].live);
-            raw[q][1] = load<T, N>(u + g.width, at[q].live);
+            raw[q][0] = load<T, WIDE>(u, at[q].live);
+            raw[q][1] = load<T, WIDE>(u + g.width, at[q].live);
         }
 #pragma unroll
-        for (int q = 0; q < kPlaces<N>; ++q) {
-            float x[N], y[N], h[N];
-            unpack<T, N>(raw[q][0], x);
-            unpack<T, N>(raw[q][1], y);
+        for (int q = 0; q < kPlaces; ++q) {
+            float x[kEach], y[kEach], h[kEach];
+            unpack<T>(raw[q][0], x);
+            unpack<T>(raw[q][1], y);
 #pragma unroll
-            for (int i = 0; i < N; ++i) h[i] = x[i] * sigmoid<T>(x[i]) * y[i];
-            store<T, N>((T*)a.h + at[q].row * a.h_stride + at[q].column, at[q].live, h);
+            for (int i = 0; i < kEach; ++i) h[i] = x[i] * sigmoid<T>(x[i]) * y[i];
+            store<T, WIDE>((T*)a.h + at[q].row * a.h_stride + at[q].column, at[q].live, h);
             if (HOLD) {
                 uint8_t* const codes = a.codes + at[q].row * a.columns + at[q].column;
                 uint8_t* const exponents = a.exponents + 2 * at[q].row * blocks + at[q].column / kBlock;
-                hold<T, N>(raw[q][0], x, at[q].live, at[q].exists, codes, exponents);
-                hold<T, N>(raw[q][1], y, at[q].live, at[q].exists, codes + g.width, exponents + blocks);
+                hold<T, WIDE>(raw[q][0], x, at[q].live, at[q].exists, codes, exponents);
+                hold<T, WIDE>(raw[q][1], y, at[q].live, at[q].exists, codes + g.width, exponents + blocks);
             }
         }
     });
 }
 
-template <typename T, int N, bool HELD>
+template <typename T, bool WIDE, bool HELD>
 __global__ void __launch_bounds__(kThreads)
 k_gate_gradient(fmb_held_t a, Grid g) {
     const int blocks = blocks_of(g.width);
-    walk<N>(g, a.rows, [&](const Place (&at)[kPlaces<N>]) {
-        Raw<T, N> dh_raw[kPlaces<N>], raw[kPlaces<N>][2];
-        Codes<N> codes[kPlaces<N>][2];
+    walk(g, a.rows, [&](const Place (&at)[kPlaces]) {
+        Raw<T> dh_raw[kPlaces], raw[kPlaces][2];
+        Codes codes[kPlaces][2];
 #pragma unroll
-        for (int q = 0; q < kPlaces<N>; ++q) {
-            dh_raw[q] = load<T, N>((const T*)a.dh + at[q].row * a.dh_stride + at[q].column, at[q].live);
+        for (int q = 0; q < kPlaces; ++q) {
+            dh_raw[q] = load<T, WIDE>((const T*)a.dh + at[q].row * a.dh_stride + at[q].column, at[q].live);
             if (HELD) {
                 const uint8_t* const from = a.codes + at[q].row * a.columns + at[q].column;
                 const uint8_t* const exponents = a.exponents + 2 * at[q].row * blocks + at[q].column / kBlock;
-                codes[q][0] = load_codes<N>(from, exponents, at[q].live);
-                codes[q][1] = load_codes<N>(from + g.width, exponents + blocks, at[q].live);
+                codes[q][0] = load_codes<WIDE>(from, exponents, at[q].live);
+                codes[q][1] = load_codes<WIDE>(from + g.width, exponents + blocks, at[q].live);
             } else {
                 const T* const u = (const T*)a.x + at[q].row * a.x_stride + at[q].column;
-                raw[q][0] = load<T, N>(u, at[q].live);
-                raw[q][1] = load<T, N>(u + g.width, at[q].live);
+                raw[q][0] = load<T, WIDE>(u, at[q].live);
+                raw[q][1] = load<T, WIDE>(u + g.width, at[q].live);
             }
         }
 #pragma unroll
-        for (int q = 0; q < kPlaces<N>; ++q) {
-            float x[N], y[N], dh[N], h[N];
-            unpack<T, N>(dh_raw[q], dh);
+        for (int q = 0; q < kPlaces; ++q) {
+            float x[kEach], y[kEach], dh[kEach], h[kEach];
+            unpack<T>(dh_raw[q], dh);
             if (HELD) {
-                release<N>(codes[q][0], x);
-                release<N>(codes[q][1], y);
+                release(codes[q][0], x);
+                release(codes[q][1], y);
             } else {
-                unpack<T, N>(raw[q][0], x);
-                unpack<T, N>(raw[q][1], y);
+                unpack<T>(raw[q][0], x);
+                unpack<T>(raw[q][1], y);
             }
 #pragma unroll
-            for (int i = 0; i < N; ++i) {
+            for (int i = 0; i < kEach; ++i) {
                 const float s = sigmoid<T>(x[i]), silu = x[i] * s;
                 h[i] = silu * y[i];
                 y[i] = dh[i] * y[i] * s * (1.0f + x[i] * (1.0f - s));
                 x[i] = dh[i] * silu;
             }
             T* const du = (T*)a.du + at[q].row * a.du_stride + at[q].column;
-            store<T, N>(du, at[q].live, y);
-            store<T, N>(du + g.width, at[q].live, x);
-            if (a.h) store<T, N>((T*)a.h + at[q].row * a.h_stride + at[q].column, at[q].live, h);
+            store<T, WIDE>(du, at[q].live, y);
+            store<T, WIDE>(du + g.width, at[q].live, x);
+            if (a.h) store<T, WIDE>((T*)a.h + at[q].row * a.h_stride + at[q].column, at[q].live, h);
         }
     });
 }
@@ -353,35 +400,37 @@ bool by_eight(const void* base, long long stride, int bytes) {
     return ((uintptr_t)base & (uintptr_t)(std::min(16, 8 * bytes) - 1)) == 0 && stride % 8 == 0;
 }
 
-Grid grid_of(int columns, int parts, int n) {
+Grid grid_of(int columns, int parts) {
     Grid g;
     g.columns = columns;
     g.parts = parts;
     g.width = columns / parts;
-    g.lanes = kBlock / n;
-    const int columns_of_lane = n == 1 ? kPlaces<1> : n;
-    while (g.lanes < kThreads && g.lanes * columns_of_lane < g.width) g.lanes *= 2;
+    g.lanes = kLanes;
+    while (g.lanes < kThreads && g.lanes * kEach < g.width) g.lanes *= 2;
     return g;
 }
 
-unsigned ctas(const Grid& g, long long rows) { return (unsigned)std::min<long long>((rows + kThreads / g.lanes - 1) / (kThreads / g.lanes), 1 << 20); }
+unsigned ctas(const Grid& g, long long rows) {
+    const int rows_at_once = kThreads / g.lanes * kPlaces;
+    return (unsigned)std::min<long long>((rows + rows_at_once - 1) / rows_at_once, 1 << 20);
+}
 
 struct Launch {
     const fmb_held_t& a;
     bool wide;
     cudaStream_t stream;
 
-    template <typename T, int N>
+    template <typename T, bool WIDE>
     void go(int what) const {
-        const Grid g = grid_of(a.columns, what == 0 ? a.parts : 2, N);
+        const Grid g = grid_of(a.columns, what == 0 ? a.parts : 2);
         const long long rows = (long long)a.rows * (what == 0 ? a.parts : 1);
-        if (what == 0) k_hold<T, N><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
-        else if (what == 1 && a.codes) k_gate<T, N, true><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
-        else if (what == 1) k_gate<T, N, false><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
-        else if (a.codes) k_gate_gradient<T, N, true><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
-        else k_gate_gradient<T, N, false><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
+        if (what == 0) k_hold<T, WIDE><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
+        else if (what == 1 && a.codes) k_gate<T, WIDE, true><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
+        else if (what == 1) k_gate<T, WIDE, false><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
+        else if (a.codes) k_gate_gradient<T, WIDE, true><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
+        else k_gate_gradient<T, WIDE, false><<<ctas(g, rows), kThreads, 0, stream>>>(a, g);
     }
-    template <typename T> void typed(int what) const { wide ? go<T, 8>(what) : go<T, 1>(what); }
+    template <typename T> void typed(int what) const { wide ? go<T, true>(what) : go<T, false>(what); }
 
     int operator()(int what) const {
         if (a.type == FMB_TYPE_F32) typed<float>(what);
@@ -413,10 +462,10 @@ bool wide(const fmb_held_t& a) {
 template <typename T>
 void release_typed(const uint8_t* codes, const uint8_t* exponents, int rows, int columns, int parts, void* out, long long stride, cudaStream_t stream) {
     const bool eight = columns / parts % 8 == 0 && by_eight(out, stride, sizeof(T)) && ((uintptr_t)codes & 7) == 0;
-    const Grid g = grid_of(columns, parts, eight ? 8 : 1);
+    const Grid g = grid_of(columns, parts);
     const long long all = (long long)rows * parts;
-    if (eight) k_release<T, 8><<<ctas(g, all), kThreads, 0, stream>>>(codes, exponents, rows, columns, (T*)out, stride, g);
-    else k_release<T, 1><<<ctas(g, all), kThreads, 0, stream>>>(codes, exponents, rows, columns, (T*)out, stride, g);
+    if (eight) k_release<T, true><<<ctas(g, all), kThreads, 0, stream>>>(codes, exponents, rows, columns, (T*)out, stride, g);
+    else k_release<T, false><<<ctas(g, all), kThreads, 0, stream>>>(codes, exponents, rows, columns, (T*)out, stride, g);
 }
 
 }  // namespace
