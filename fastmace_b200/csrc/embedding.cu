@@ -10,6 +10,7 @@
 //
 // Bound by memory: every row is read once and every row of the table written once.
 
+#include "early.cuh"
 #include "grouped.cuh"
 
 #include <algorithm>
@@ -237,6 +238,8 @@ __device__ __forceinline__ void write_sums(const Sums& p, int slab, float* out, 
 template <typename T, bool VEC, int N>
 __global__ void __launch_bounds__(kThreads, 3)
 k_embedding_sums(Sums p) {
+    let_next_come();
+    kernels_before();
     if (blockIdx.x < p.zero_ctas) {              // the first, since their searches take long and their writes little
         write_zeros(p);
         return;
@@ -355,6 +358,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 k_embedding_join(Sums p) {
     __shared__ int list[kJoinList], count;
     __shared__ float4 sums[kJoinWarps][32];
+    kernels_before();
     const fmb_embedding_t& a = p.a;
     const int32_t* const keys = (const int32_t*)a.tokens;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -444,12 +448,11 @@ int gradient(const fmb_embedding_t& a, cudaStream_t stream) {
     const long long ctas = p.zero_ctas + (long long)p.chunks * p.slabs;
     FMB_REQUIRE(ctas < (1ll << 31), "fmb_embedding_gradient: too many sums");
     if (ctas > 0) {
-        if (packed(a)) k_embedding_sums<T, true, kPack><<<(unsigned)ctas, kThreads, 0, stream>>>(p);
-        else k_embedding_sums<T, false, 4><<<(unsigned)ctas, kThreads, 0, stream>>>(p);
+        FMB_CUDA_CHECK(launch_early(packed(a) ? k_embedding_sums<T, true, kPack> : k_embedding_sums<T, false, 4>, (unsigned)ctas, kThreads, 0, stream, p));
         FMB_LAUNCH_CHECK();
     }
     if (p.chunks > 1) {
-        k_embedding_join<<<std::min(p.chunks, 148), kJoinWarps * 32, 0, stream>>>(p);
+        FMB_CUDA_CHECK(launch_early(k_embedding_join, std::min(p.chunks, 148), kJoinWarps * 32, 0, stream, p));
         FMB_LAUNCH_CHECK();
     }
     return FMB_OK;

@@ -18,6 +18,7 @@
 // bfloat16 (17 bits, any float32's range) against bfloat16 weights, a pair of tf32 against float16 ones, which are exact in tf32.
 // float32 operands are pairs of tf32 (22 bits), of whose four products the smallest is left out.
 
+#include "early.cuh"
 #include "grouped.cuh"
 
 #include <algorithm>
@@ -70,6 +71,7 @@ __global__ void __launch_bounds__(kThreads)
 k_route(fmb_route_t a, int wide, int rows) {
     __shared__ float sums[kThreads * 8];
     __shared__ float logits[FMB_MAX_GROUPS];
+    let_next_come();
     const int token = blockIdx.x / kCluster, rank = blockIdx.x % kCluster, packs = (a.experts + 7) / 8;
     const int pack = threadIdx.x % packs, row = threadIdx.x / packs;
     const T* const x = (const T*)a.x + token * a.x_stride;
@@ -677,7 +679,8 @@ template <typename T>
 __global__ void __launch_bounds__(1024)
 k_list_pairs(const __grid_constant__ Layer p, int control, void* packed) {
     const fmb_experts_t& a = p.a;
-    asm volatile("griddepcontrol.launch_dependents;");            // the next launch comes to the SMs meanwhile, and waits there
+    let_next_come();
+    kernels_before();                            // what the rows and the choices come from
     if (blockIdx.x > 0) {
         const T* const from = (const T*)a.x + (blockIdx.x - 1) * a.x_stride;
         T* const to = (T*)packed + (blockIdx.x - 1) * p.x_stride;
@@ -741,7 +744,7 @@ k_experts(const __grid_constant__ Layer p) {
     int32_t* const next = p.control;
     int32_t* const done = p.control + 1;
     int32_t* const columns = done + a.experts;
-    asm volatile("griddepcontrol.wait;" ::: "memory");            // for the lists
+    kernels_before();                            // for the lists
     if (threadIdx.x == 0) {
         s.ticket = atomicAdd(next, 1);
         s.gave_up = 0;
@@ -891,7 +894,7 @@ int layer(const fmb_experts_t& a, cudaStream_t stream) {
     const bool pack = !begin_at(a.x, a.x_stride, a.tokens, b, 8);
     p.x = pack ? packed : const_cast<void*>(a.x);
     p.x_stride = pack ? size.x_stride : a.x_stride;
-    k_list_pairs<T><<<pack ? a.tokens + 1 : 1, 1024, 0, stream>>>(p, (int)size.control, packed);
+    FMB_CUDA_CHECK(launch_early(k_list_pairs<T>, pack ? a.tokens + 1 : 1, 1024, 0, stream, p, (int)size.control, packed));
     FMB_LAUNCH_CHECK();
     // whole pieces of 16 bytes, at multiples of 16
     auto pieces = [&](const void* base, long long row, long long group, int rows, int columns) {
@@ -900,18 +903,10 @@ int layer(const fmb_experts_t& a, cudaStream_t stream) {
     const bool wide = pieces(a.w_up, a.up_row_stride, a.up_group_stride, a.width, a.inner) && pieces(a.w_down, a.down_row_stride, a.down_group_stride, a.inner, a.width);
     const long long most = std::min<long long>(a.experts, (long long)a.tokens * a.top) * (p.up_units + p.down_units);
     const int grid = (int)std::min<long long>(most, 2 * grp::sm_count());
-    cudaLaunchConfig_t config = {};
-    cudaLaunchAttribute early;
-    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    early.val.programmaticStreamSerializationAllowed = 1;
-    config.gridDim = dim3(grid);
-    config.blockDim = dim3(kThreads);
-    config.dynamicSmemBytes = wide ? sizeof(Smem<T, true>) : sizeof(Smem<T, false>);
-    config.stream = stream;
-    config.attrs = &early;
-    config.numAttrs = 1;
-    FMB_CUDA_CHECK(opt_in_shared_memory(wide ? (const void*)k_experts<T, true> : (const void*)k_experts<T, false>, (int)config.dynamicSmemBytes));
-    FMB_CUDA_CHECK(wide ? cudaLaunchKernelEx(&config, k_experts<T, true>, p) : cudaLaunchKernelEx(&config, k_experts<T, false>, p));
+    const auto kernel = wide ? k_experts<T, true> : k_experts<T, false>;
+    const int smem = wide ? sizeof(Smem<T, true>) : sizeof(Smem<T, false>);
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)kernel, smem));
+    FMB_CUDA_CHECK(launch_early(kernel, grid, kThreads, smem, stream, p));
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }

@@ -11,7 +11,7 @@
 // both passes of `place`; one at a time, each waited for, 1,944 rows took 14 us. A call: 1,944 rows by 2 keys 11 us (one launch of
 // one CTA, of which the launch is most), 2,100,003 rows by 128 keys 35 us (three launches; 17 MB, 2.6 us of memory).
 
-#include "fmb_common.cuh"
+#include "early.cuh"
 
 #include <algorithm>
 
@@ -94,6 +94,10 @@ k_group_count(const K* __restrict__ keys, Digit d, long long rows, int groups, i
     constexpr int kThreads = 32 * WARPS, kRowsPerCta = WARPS * kRowsPerWarp;
     __shared__ int counts[FMB_MAX_GROUPS + 1];
     const int width = groups + 1;
+    if (DIGIT) {
+        let_next_come();
+        kernels_before();
+    }
     int g[kKeys];
     load_keys<K, DIGIT>(keys, d, (long long)blockIdx.x * kRowsPerCta + (threadIdx.x >> 5) * kRowsPerWarp, rows, groups, g);
     for (int q = threadIdx.x; q < width; q += kThreads) counts[q] = 0;
@@ -107,8 +111,13 @@ k_group_count(const K* __restrict__ keys, Digit d, long long rows, int groups, i
 
 // table[cta][g] becomes the rows of g in the CTAs before; totals[g]. A CTA takes 32 groups, its 32 warps a share of the
 // table's rows each.
+template <bool DIGIT>
 __global__ void __launch_bounds__(1024)
 k_group_scan(int32_t* __restrict__ table, int32_t* __restrict__ totals, int ctas, int width) {
+    if (DIGIT) {
+        let_next_come();
+        kernels_before();
+    }
     __shared__ int part[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.x * 32 + lane;
     const int share = (ctas + 31) / 32, begin = warp * share, end = min(ctas, begin + share);
@@ -174,6 +183,10 @@ k_group_place(const K* __restrict__ keys, Digit d, long long rows, int groups, i
     int* const starts = ALONE ? here : here + width;
     int* const sorted = here + 2 * width;                 // row of the CTA | group << 13
     const long long first = (long long)blockIdx.x * kRowsPerCta;
+    if (DIGIT) {
+        let_next_come();
+        kernels_before();
+    }
     int g[kKeys], rank[kKeys];
     load_keys<K, DIGIT>(keys, d, first + warp * kRowsPerWarp, rows, groups, g);
     const int warps = ALONE ? (int)((rows + kRowsPerWarp - 1) / kRowsPerWarp) : WARPS;         // that have rows
@@ -254,24 +267,31 @@ k_group_place(const K* __restrict__ keys, Digit d, long long rows, int groups, i
     }
 }
 
-// one stable pass: counts, their sums over the CTAs, places; a launch alone where one CTA takes all rows
+// one stable pass: counts, their sums over the CTAs, places; a launch alone where one CTA takes all rows. The passes of tokens, of which there
+// are two and more behind them, come early.
 template <typename K, bool DIGIT, int WARPS>
 int sort_pass(const K* keys, const Digit& d, long long rows, int groups, int32_t* order, int32_t* offsets, int32_t* scratch, cudaStream_t stream) {
     const int width = groups + 1, ctas = ceil_div(rows, WARPS * kRowsPerWarp);
     const int smem = place_smem(width, WARPS), most = place_smem(FMB_MAX_GROUPS + 1, WARPS), bits = 32 - __builtin_clz(groups);
+    auto launch = [&](auto kernel, int grid, int threads, int bytes, auto... arguments) -> cudaError_t {
+        if constexpr (DIGIT) return launch_early(kernel, grid, threads, bytes, stream, arguments...);
+        kernel<<<grid, threads, bytes, stream>>>(arguments...);
+        return cudaGetLastError();
+    };
+    const int32_t* none = nullptr;
     if (ctas <= 1) {
         FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, true, DIGIT, WARPS>, most));
-        k_group_place<K, true, DIGIT, WARPS><<<1, 32 * WARPS, smem, stream>>>(keys, d, rows, groups, bits, nullptr, nullptr, order, offsets);
+        FMB_CUDA_CHECK(launch(k_group_place<K, true, DIGIT, WARPS>, 1, 32 * WARPS, smem, keys, d, rows, groups, bits, none, none, order, offsets));
         FMB_LAUNCH_CHECK();
         return FMB_OK;
     }
     FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, false, DIGIT, WARPS>, most));
     int32_t* const totals = scratch + (long long)ctas * width;
-    k_group_count<K, DIGIT, WARPS><<<ctas, 32 * WARPS, 0, stream>>>(keys, d, rows, groups, scratch);
+    FMB_CUDA_CHECK(launch(k_group_count<K, DIGIT, WARPS>, ctas, 32 * WARPS, 0, keys, d, rows, groups, scratch));
     FMB_LAUNCH_CHECK();
-    k_group_scan<<<ceil_div(width, 32), 1024, 0, stream>>>(scratch, totals, ctas, width);
+    FMB_CUDA_CHECK(launch(k_group_scan<DIGIT>, ceil_div(width, 32), 1024, 0, scratch, totals, ctas, width));
     FMB_LAUNCH_CHECK();
-    k_group_place<K, false, DIGIT, WARPS><<<ctas, 32 * WARPS, smem, stream>>>(keys, d, rows, groups, bits, scratch, totals, order, offsets);
+    FMB_CUDA_CHECK(launch(k_group_place<K, false, DIGIT, WARPS>, ctas, 32 * WARPS, smem, keys, d, rows, groups, bits, scratch, totals, order, offsets));
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
@@ -280,7 +300,7 @@ int sort_pass(const K* keys, const Digit& d, long long rows, int groups, int32_t
 // which keeps the order that the first has made.
 int lower_bits(int vocabulary) { return vocabulary <= FMB_MAX_GROUPS ? 0 : (33 - __builtin_clz(vocabulary)) / 2; }
 // CTAs of eight warps, while that spreads the rows over more SMs: below, one CTA has them all without a second launch
-int warps_of(long long rows) { return rows > kRowsPerCta && rows <= 148ll * 2 * kFewWarps * kRowsPerWarp ? kFewWarps : kWarps; }
+int warps_of(long long rows) { return rows > kRowsPerCta && rows <= 148ll * 8 * kFewWarps * kRowsPerWarp ? kFewWarps : kWarps; }
 long long table_size(long long rows, int width) {
     const long long per_cta = warps_of(rows) * kRowsPerWarp;
     return rows <= per_cta ? 0 : ((rows + per_cta - 1) / per_cta + 1) * width;
