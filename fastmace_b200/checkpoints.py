@@ -26,6 +26,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
+from .embedding import _empty
 from .grouped import TYPES, RowGroups, _launch, _matrix, _on_device, _shares_memory, _weight_gradient, _written
 
 BLOCK = _lib.HELD_BLOCK
@@ -72,26 +73,21 @@ def _held(what: str, held: HeldRows, parts: int | None = None):
 
 
 def _new_held(rows: int, columns: int, parts: int, like: torch.Tensor) -> HeldRows:
-    return HeldRows(torch.empty((rows, columns), dtype=torch.float8_e4m3fn, device=like.device),
-                    torch.empty((rows, _blocks(columns, parts)), dtype=torch.uint8, device=like.device), like.dtype, parts)
+    device = like.device
+    return HeldRows(_empty(rows, columns, torch.float8_e4m3fn, device), _empty(rows, _blocks(columns, parts), torch.uint8, device), like.dtype, parts)
 
 
-def _struct(kind: int, rows: int, columns: int, parts: int, held: HeldRows | None, **matrices) -> "_lib.HeldStruct":
-    """``matrices``: x, h, dh, du as (tensor, row stride), or None."""
-    a = _lib.HeldStruct(kind, rows, columns, parts)
-    if held is not None:
-        a.codes, a.exponents = held.codes.data_ptr(), held.exponents.data_ptr()
-    for name, matrix in matrices.items():
-        if matrix is not None:
-            setattr(a, name, matrix[0].data_ptr())
-            setattr(a, name + "_stride", matrix[1])
-    return a
+def _struct(kind: int, rows: int, columns: int, parts: int, held: HeldRows | None, x=(None, 0), h=(None, 0), dh=(None, 0), du=(None, 0)):
+    """The C call's arguments; x, h, dh, du as (tensor, row stride)."""
+    at = [t if t is None else t.data_ptr() for t, _ in (x, h, dh, du)]
+    codes, exponents = (None, None) if held is None else (held[0].data_ptr(), held[1].data_ptr())
+    return _lib.HeldStruct(kind, rows, columns, parts, at[0], codes, exponents, *at[1:], x[1], h[1], dh[1], du[1])
 
 
 def _given(what: str, name: str, out: torch.Tensor | None, rows: int, columns: int, like: torch.Tensor, dtype: torch.dtype, *operands):
     """(output, row stride): one that is given, checked, or a new one."""
     if out is None:
-        return torch.empty((rows, columns), dtype=dtype, device=like.device), columns
+        return _empty(rows, columns, dtype, like.device), columns
     stride = _matrix(what, name, out, columns, rows)[2]
     if out.dtype != dtype:
         raise ValueError(f"{what}: {name} must be {dtype}")
@@ -165,10 +161,10 @@ def gated_rows_gradient(u: HeldRows | torch.Tensor, dh: torch.Tensor, out: torch
         raise ValueError(f"{what}: dh must have the rows' type, {dtype}")
     index = _on_device(what, dh, *operands)
     du, du_stride = _given(what, "out", out, rows, columns, dh, dtype, dh, *operands)
-    h = torch.empty((rows, columns // 2), dtype=dtype, device=dh.device) if recompute else None
+    h = _empty(rows, columns // 2, dtype, dh.device) if recompute else None
     if rows:
         a = _struct(TYPES[dtype], rows, columns, 2, None if source else u, dh=(dh, dh_stride), du=(du, du_stride),
-                    h=(h, columns // 2) if recompute else None, **source)
+                    h=(h, columns // 2), **source)
         _lib.check(_launch(index, _lib.load().fmb_gated_rows_gradient, ctypes.byref(a)), "fmb_gated_rows_gradient")
         if out is not None:
             _written(out)

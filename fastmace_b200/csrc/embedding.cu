@@ -356,6 +356,7 @@ constexpr int kJoinWarps = 32, kJoinList = 64;
 
 __global__ void __launch_bounds__(kJoinWarps * 32)
 k_embedding_join(Sums p) {
+    constexpr int kThreads = 32 * kJoinWarps;
     __shared__ int list[kJoinList], count;
     __shared__ float4 sums[kJoinWarps][32];
     kernels_before();
@@ -381,8 +382,13 @@ k_embedding_join(Sums p) {
         }
         __syncthreads();
         for (int q = 0; q < count; ++q) {
-            const int chunk = list[q], end = (chunk + 1) * p.chunk, key = __ldg(keys + end - 1);
-            const int parts = (lower_bound(keys, end, a.rows, key + 1) - 1) / p.chunk - chunk + 1;
+            const int chunk = list[q], key = __ldg(keys + (chunk + 1) * p.chunk - 1);
+            // the chunks behind it that begin with the run, 1,024 looked at together
+            int parts = 1;
+            for (int first = chunk + 1, some = kThreads; some == kThreads; first += kThreads) {
+                some = __syncthreads_count(first + (int)threadIdx.x < p.chunks && __ldg(keys + (long long)(first + threadIdx.x) * p.chunk) == key);
+                parts += some;
+            }
             for (int s0 = 0; s0 < slabs; s0 += kJoinWarps / shares) {
                 const int slab = s0 + warp / shares, part = warp % shares, c = slab * 128 + 4 * lane;
                 float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

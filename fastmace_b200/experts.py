@@ -24,6 +24,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
+from .embedding import _empty, _scratch
 from .grouped import MAX_GROUPS, TYPES, _launch, _matrix, _on_device, _shares_memory, _status_pointer, _weights, _written
 
 MAX_TOP = _lib.MAX_TOP
@@ -55,8 +56,7 @@ def route_rows(x: torch.Tensor, router: torch.Tensor, top: int, normalise: bool 
     if not 1 <= int(top) <= min(MAX_TOP, count):
         raise ValueError(f"{what}: 1 to {min(MAX_TOP, count)} choices")
     index = _on_device(what, x, router)
-    routes = Routes(torch.empty((tokens, int(top)), dtype=torch.int32, device=x.device),
-                    torch.empty((tokens, int(top)), dtype=torch.float32, device=x.device))
+    routes = Routes(_empty(tokens, int(top), torch.int32, x.device), _empty(tokens, int(top), torch.float32, x.device))
     if tokens:
         a = _lib.RouteStruct(kind, tokens, width, count, int(top), bool(normalise), x.data_ptr(), router.data_ptr(),
                              routes.experts.data_ptr(), routes.weights.data_ptr(), stride, router_stride)
@@ -90,14 +90,14 @@ def expert_layer(x: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, rout
         if any(_shares_memory(out, t) for t in (x, w_up, w_down, chosen, weights)):
             raise ValueError(f"{what}: out shares memory with an operand")
     else:
-        out, out_stride = x.new_empty((tokens, width)), width
+        out, out_stride = _empty(tokens, width, x.dtype, x.device), width
     if tokens:
         lib = _lib.load()
         a = _lib.ExpertsStruct(kind, tokens, count, chosen.shape[1], width, inner, x.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
                                chosen.data_ptr(), weights.data_ptr(), out.data_ptr(), stride, out_stride, up_group, up_row, down_group,
                                down_row, None, _status_pointer(index))
         call = ctypes.byref(a)
-        scratch = torch.empty(lib.fmb_expert_layer_scratch(call), dtype=torch.float32, device=x.device)
+        scratch = _scratch(lib.fmb_expert_layer_scratch(call), torch.float32, x.device)
         a.scratch = scratch.data_ptr()
         _lib.check(_launch(index, lib.fmb_expert_layer, call), "fmb_expert_layer")
         if given:
