@@ -487,9 +487,19 @@ __device__ __forceinline__ void multiply(float (&acc)[4][2][4], const Matrix& m,
                             split_tf32(__uint_as_float(w[2 * s + q][2 * i + 1]), a[2 * q + 1], rest[2 * q + 1]);
                         }
                     }
-                    mma_tf32(acc[i][n], a, lo[0], lo[1]);
-                    if constexpr (sizeof(T) == 4) mma_tf32(acc[i][n], rest, hi[0], hi[1]);
-                    mma_tf32(acc[i][n], a, hi[0], hi[1]);
+                    if constexpr (sizeof(T) == 4) {
+                        // The tensor core cuts its sums off, which adds up along the depth (float32 results were 8e-6 off at a depth of
+                        // 4,096): each stage's sum begins at zero and is added with rounding.
+                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma_tf32(sum, a, lo[0], lo[1]);
+                        mma_tf32(sum, rest, hi[0], hi[1]);
+                        mma_tf32(sum, a, hi[0], hi[1]);
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) acc[i][n][q] += sum[q];
+                    } else {
+                        mma_tf32(acc[i][n], a, lo[0], lo[1]);
+                        mma_tf32(acc[i][n], a, hi[0], hi[1]);
+                    }
                 }
             }
         }
