@@ -149,7 +149,7 @@ struct Sums {
     int chunk, chunks, slabs;                    // rows of a CTA's chunk, kWarps shares of them
     int wide_out;                                // rows of the table start at multiples of 16 bytes
     long long part_stride;                       // floats of a part in scratch: the width, filled up to a multiple of four
-    unsigned zero_ctas;                          // CTAs that write zeros, before those that sum
+    unsigned zero_ctas, zero_shares;             // CTAs that write zeros, before those that sum, and of how many they share a row's columns
 };
 
 // first place from `low` on whose key is not less than v, by a warp: 32 places of what is left at a time
@@ -167,41 +167,44 @@ __device__ __forceinline__ int lower_bound(const int32_t* __restrict__ keys, int
     return low;
 }
 
-// Zeros for the tokens without rows, of 256 at a time: the rows' keys from the first of them on say which have some.
+// Zeros for the tokens without rows: kZeroTokens of them and a share of the columns by a CTA. Warp 0 finds out which have rows.
+constexpr int kZeroTokens = 32;
+
 __device__ __forceinline__ void write_zeros(const Sums& p) {
-    __shared__ uint32_t present[kWarps];
+    __shared__ uint32_t present;
     const fmb_embedding_t& a = p.a;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int32_t* const keys = (const int32_t*)a.tokens;
-    const int first = (int)blockIdx.x * 256, last = min(first + 256, a.vocabulary);
-    if (threadIdx.x < kWarps) present[threadIdx.x] = 0;
-    __syncthreads();
-    // every warp takes 32 of them: its rows lie between two bounds, and a lane looks at every 32nd
-    const int mine = first + 32 * warp;
-    if (mine < last) {
-        const int from = lower_bound(keys, 0, a.rows, mine), to = lower_bound(keys, from, a.rows, min(mine + 32, last));
+    const int first = (int)(blockIdx.x / p.zero_shares) * kZeroTokens, last = min(first + kZeroTokens, a.vocabulary);
+    if (warp == 0) {
+        const int from = lower_bound(keys, 0, a.rows, first), to = lower_bound(keys, from, a.rows, last);
         uint32_t seen = 0;
         if (to - from > 256) {
             // tokens of many rows: a lane looks for its own
-            int low = from, high = mine + lane < last ? to : from;
+            int low = from, high = first + lane < last ? to : from;
             while (low < high) {
                 const int mid = (int)(((unsigned)low + (unsigned)high) >> 1);
-                if (__ldg(keys + mid) < mine + lane) low = mid + 1; else high = mid;
+                if (__ldg(keys + mid) < first + lane) low = mid + 1; else high = mid;
             }
-            seen = __ballot_sync(0xffffffffu, mine + lane < last && low < to && __ldg(keys + low) == mine + lane);
+            seen = __ballot_sync(0xffffffffu, first + lane < last && low < to && __ldg(keys + low) == first + lane);
         } else {
-            for (int at = from + lane; at < to; at += 32) seen |= 1u << ((__ldg(keys + at) - mine) & 31);
+            for (int at = from + lane; at < to; at += 32) seen |= 1u << ((__ldg(keys + at) - first) & 31);
             seen = __reduce_or_sync(0xffffffffu, seen);
         }
-        if (lane == 0) present[warp] = seen;
+        if (lane == 0) present = seen;
     }
     __syncthreads();
+    const int share = blockIdx.x % p.zero_shares, units = p.wide_out ? a.width / 4 : a.width;
+    const int begin = (int)((long long)units * share / p.zero_shares), end = (int)((long long)units * (share + 1) / p.zero_shares);
     for (int v = first + warp; v < last; v += kWarps) {
-        if (present[(v - first) >> 5] >> ((v - first) & 31) & 1) continue;
+        if (present >> (v - first) & 1) continue;
         float* const out = (float*)a.out + v * a.out_stride;
-        const int packs = p.wide_out ? a.width / 4 : 0;
-        for (int c = lane; c < packs; c += 32) reinterpret_cast<float4*>(out)[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int c = 4 * packs + lane; c < a.width; c += 32) out[c] = 0.0f;
+        if (p.wide_out) {
+            for (int c = begin + lane; c < end; c += 32) reinterpret_cast<float4*>(out)[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (share == p.zero_shares - 1 && lane < a.width % 4) out[4 * units + lane] = 0.0f;
+        } else {
+            for (int c = begin + lane; c < end; c += 32) out[c] = 0.0f;
+        }
     }
 }
 
@@ -450,7 +453,10 @@ int gradient(const fmb_embedding_t& a, cudaStream_t stream) {
     p.chunks = ceil_div(a.rows, p.chunk);
     p.wide_out = starts_at(a.out, a.out_stride, 4, 4);
     p.part_stride = (a.width + 3) / 4 * 4;
-    p.zero_ctas = a.accumulate ? 0 : ceil_div(a.vocabulary, 256);
+    // two CTAs for every SM, as far as a share keeps 512 columns
+    const int zero_groups = ceil_div(a.vocabulary, kZeroTokens);
+    p.zero_shares = std::max(1, std::min(ceil_div(2 * 148, zero_groups), a.width / 512));
+    p.zero_ctas = a.accumulate ? 0 : zero_groups * p.zero_shares;
     const long long ctas = p.zero_ctas + (long long)p.chunks * p.slabs;
     FMB_REQUIRE(ctas < (1ll << 31), "fmb_embedding_gradient: too many sums");
     if (ctas > 0) {

@@ -278,12 +278,13 @@ int sort_pass(const K* keys, const Digit& d, long long rows, int groups, int32_t
         kernel<<<grid, threads, bytes, stream>>>(arguments...);
         return cudaGetLastError();
     };
-    const int32_t* none = nullptr;
-    if (ctas <= 1) {
-        FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, true, DIGIT, WARPS>, most));
-        FMB_CUDA_CHECK(launch(k_group_place<K, true, DIGIT, WARPS>, 1, 32 * WARPS, smem, keys, d, rows, groups, bits, none, none, order, offsets));
-        FMB_LAUNCH_CHECK();
-        return FMB_OK;
+    if constexpr (!DIGIT) {                      // (fewer tokens are ranked)
+        if (ctas <= 1) {
+            FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, true, false, WARPS>, most));
+            k_group_place<K, true, false, WARPS><<<1, 32 * WARPS, smem, stream>>>(keys, d, rows, groups, bits, nullptr, nullptr, order, offsets);
+            FMB_LAUNCH_CHECK();
+            return FMB_OK;
+        }
     }
     FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_group_place<K, false, DIGIT, WARPS>, most));
     int32_t* const totals = scratch + (long long)ctas * width;
@@ -299,11 +300,11 @@ int sort_pass(const K* keys, const Digit& d, long long rows, int groups, int32_t
 // Tokens by value: one pass where the table holds every value, else one over the lower half of their bits and one over the upper half,
 // which keeps the order that the first has made.
 int lower_bits(int vocabulary) { return vocabulary <= FMB_MAX_GROUPS ? 0 : (33 - __builtin_clz(vocabulary)) / 2; }
-// CTAs of eight warps, while that spreads the rows over more SMs: below, one CTA has them all without a second launch
-int warps_of(long long rows) { return rows > kRowsPerCta && rows <= 148ll * 8 * kFewWarps * kRowsPerWarp ? kFewWarps : kWarps; }
+// CTAs of eight warps, while that spreads the rows over more SMs
+int warps_of(long long rows) { return rows <= 148ll * 8 * kFewWarps * kRowsPerWarp ? kFewWarps : kWarps; }
 long long table_size(long long rows, int width) {
     const long long per_cta = warps_of(rows) * kRowsPerWarp;
-    return rows <= per_cta ? 0 : ((rows + per_cta - 1) / per_cta + 1) * width;
+    return ((rows + per_cta - 1) / per_cta + 1) * width;
 }
 
 template <typename K>
@@ -312,8 +313,46 @@ int sort_digit(const K* keys, const Digit& d, long long rows, int groups, int32_
                                     : sort_pass<K, true, kFewWarps>(keys, d, rows, groups, order, nullptr, scratch, stream);
 }
 
+// Few rows: the place of each is the number of those before it, for which eight lanes count a row's share of all, four at a time. One launch
+// for any vocabulary, each CTA with 32 rows (1,928 rows by two passes of one CTA: 8 us more; by one CTA alone 75 us more).
+constexpr int kFewRows = kRowsPerCta, kRankRows = 32;
+
+template <typename K>
+__global__ void __launch_bounds__(8 * kRankRows)
+k_rank_tokens(const K* __restrict__ tokens, int rows, int vocabulary, int32_t* __restrict__ order, int32_t* __restrict__ keys) {
+    __shared__ int4 all[kFewRows / 4];
+    let_next_come();
+    kernels_before();
+    int* const key = reinterpret_cast<int*>(all);
+    const int quads = (rows + 3) / 4;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < 4 * quads; i += 8 * kRankRows) key[i] = i < rows ? group_of(tokens[i], vocabulary) : 0x7fffffff;
+    __syncthreads();
+    const int i = blockIdx.x * kRankRows + (threadIdx.x >> 3), mine = i < rows ? key[i] : 0, own = i / 4;
+    int before = 0;
+    // a key as large as this one counts where its row comes before
+#pragma unroll 4
+    for (int q = threadIdx.x & 7; q < quads; q += 8) {
+        const int4 k = all[q];
+        const int bound = mine + (q < own);
+        before += (k.x < bound) + (k.y < bound) + (k.z < bound) + (k.w < bound);
+        if (q == own) before += (i % 4 > 0 && k.x == mine) + (i % 4 > 1 && k.y == mine) + (i % 4 > 2 && k.z == mine);
+    }
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (i < rows && (threadIdx.x & 7) == 0) {
+        order[before] = i;
+        keys[before] = mine;
+    }
+}
+
 template <typename K>
 int sort_tokens(const K* tokens, long long rows, int vocabulary, int32_t* order, int32_t* keys, int32_t* scratch, cudaStream_t stream) {
+    if (rows <= kFewRows) {
+        FMB_CUDA_CHECK(launch_early(k_rank_tokens<K>, ceil_div(rows, kRankRows), 8 * kRankRows, 0, stream, tokens, (int)rows, vocabulary, order, keys));
+        FMB_LAUNCH_CHECK();
+        return FMB_OK;
+    }
     const int low = lower_bits(vocabulary);
     if (low == 0) return sort_digit(tokens, Digit{nullptr, keys, vocabulary, 0, -1}, rows, vocabulary, order, scratch, stream);
     int32_t* const table = scratch + rows;
@@ -345,7 +384,7 @@ extern "C" FMB_API int fmb_group_rows(const void* keys, int key_bytes, long long
 }
 
 extern "C" FMB_API long long fmb_sort_tokens_scratch(long long rows, int vocabulary) {
-    if (rows < 1 || vocabulary < 1 || vocabulary > FMB_MAX_VOCABULARY) return 0;
+    if (rows <= kFewRows || vocabulary < 1 || vocabulary > FMB_MAX_VOCABULARY) return 0;
     const int low = lower_bits(vocabulary);
     if (low == 0) return table_size(rows, vocabulary + 1);
     return rows + table_size(rows, std::max(1 << low, (vocabulary >> low) + 1));

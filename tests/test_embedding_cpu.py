@@ -66,6 +66,6 @@ def test_scratch_covers_both_passes():
             low = 0 if vocabulary <= 1024 else (vocabulary.bit_length() + 1) // 2
             widths = [vocabulary + 1] if not low else [1 << low, (vocabulary >> low) + 1]
             assert max(widths) <= 1025                     # what a table in shared memory holds
-            per_cta = 2048 if 8192 < rows <= 148 * 8 * 2048 else 8192
-            tables = 0 if rows <= 8192 else (-(-rows // per_cta) + 1) * max(widths)
-            assert lib.fmb_sort_tokens_scratch(rows, vocabulary) == tables + (rows if low else 0)
+            per_cta = 2048 if rows <= 148 * 8 * 2048 else 8192
+            tables = (-(-rows // per_cta) + 1) * max(widths)
+            assert lib.fmb_sort_tokens_scratch(rows, vocabulary) == (0 if rows <= 8192 else tables + (rows if low else 0))

@@ -41,7 +41,8 @@ def _rounding(t):
 SHAPES = [(1, 1, 1, "even", 1), (1, 5, 128, "one", 1), (33, 89, 128, "even", 4), (500, 3, 65, "uneven", 1), (257, 1024, 4, "even", 1),
           (700, 1025, 200, "uneven", 2), (300, 40_000, 515, "even", 1), (64, 20, 130, "none", 1), (8192, 70_000, 64, "uneven", 1),
           (8193, 700, 33, "uneven", 3), (9000, 100_003, 96, "even", 1), (30_000, 2, 128, "even", 1), (20_000, 5000, 1032, "uneven", 1),
-          (5000, 1, 2500, "one", 1), (12_345, 1_000_000, 7, "uneven", 1)]
+          (5000, 1, 2500, "one", 1), (12_345, 1_000_000, 7, "uneven", 1), (8191, 1, 40, "one", 1), (8192, 50_000, 40, "uneven", 1), (255, 1_048_575, 3, "even", 1),
+          (90, 381, 4096, "uneven", 1)]
 
 
 @pytest.mark.parametrize("tokens_type", [torch.int32, torch.int64])
