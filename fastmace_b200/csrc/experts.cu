@@ -3,10 +3,10 @@
 //   route:   l = x R; the `top` largest of each token, ties to the lowest number; weights softmax(l) of the chosen, or of all
 //   layer:   y[t] = sum_j w[t, j] (silu(x Wg) * (x Wu)) Wd of expert e(t, j)
 //
-// What bounds the layer is the weights of the experts that are chosen, read once from memory. One launch does both products:
-// units of 32 gate columns with the 32 columns they multiply, then units of 64 columns of the second matrix, handed out in that order by
-// a counter. A unit of the second kind waits for the first ones of its expert only; those were handed out before it, so they
-// are done or under way and the wait ends, however few CTAs run at a time.
+// What bounds the layer is the weights of the experts that are chosen, read once from memory. One launch does it all: units of 32 gate
+// columns with the 32 columns they multiply, then units of 64 columns of the second matrix, then units of y, handed out in that order by
+// a counter. A unit of the second kind waits for the first ones of its expert, one of y for the second ones of its columns; those were
+// handed out before it, so they are done or under way and the wait ends, however few CTAs run at a time.
 //
 // A unit is [64 columns] x [8 or 16 rows] over the whole depth, which the eight warps of a CTA share. Each warp has a ring of stages in
 // shared memory that asynchronous copies fill, without a barrier between warps; the ring does not run dry between units, since the first
@@ -228,13 +228,20 @@ __device__ __forceinline__ uint2 load_8(uint32_t at) {
 
 struct Layer {
     fmb_experts_t a;
-    int up_units, down_units;                    // of an expert
-    uint32_t up_inverse, down_inverse;           // 2^32 over them, rounded up
+    // Of each of the two products: blocks of columns of an expert, groups of 64 columns in a block, which have kWarps / groups warps each for the
+    // depth, and units that share the depth of a block
+    struct Shape {
+        int blocks, log_groups, splits;
+        uint32_t inverse;                        // 2^32 / (blocks splits), rounded up
+    } up, down;
+    int up_share, down_share;                    // stages of a unit
     long long h_stride, part_stride;             // floats of a row: the inner width, or the width, filled up to whole units
-    int32_t* control;                            // next unit; then of each active expert the units that are done, of each column unit the experts
+    int32_t* control;                            // next unit; of each active expert the blocks that are done; of each block of the second matrix the
+                                                 // units; of each block of an active expert's first the units, where they share the depth
     int32_t* lists;                              // number of active experts, total of pairs; active[], first[], pair[]
     float* h;                                    // [tokens * top]
-    float* parts;
+    float* parts;                                // [down.splits][tokens * top]
+    float* up_parts;                             // [up.splits][tokens * top] of h_stride gates and as many they multiply
     void* x;                                     // rows that copies of 8 bytes take: the caller's, or copies of them
     long long x_stride;
 };
@@ -248,29 +255,36 @@ struct Smem {
     uint16_t pair[kMaxPairs];                    // pairs of token and choice, by expert
     uint8_t token[kMaxPairs];
     uint16_t active[FMB_MAX_GROUPS], first[FMB_MAX_GROUPS + 1];
-    int ticket, last[2];                         // last: of two units in turn, the columns that are complete with it, or -1
+    int ticket, joins;
     volatile int gave_up;
 };
 
 struct Unit {
-    int up, number, expert, block, first, end;
+    int up, number, expert, block, part, first, end;
 };
 
 template <typename S>
 __device__ __forceinline__ Unit unit_of(const Layer& p, const S& s, int ticket, int ups) {
     Unit u;
     u.up = ticket < ups;
-    const int t = u.up ? ticket : ticket - ups, per = u.up ? p.up_units : p.down_units;
-    u.number = per == 1 ? t : (int)__umulhi((uint32_t)t, u.up ? p.up_inverse : p.down_inverse);
+    const Layer::Shape& shape = u.up ? p.up : p.down;
+    const int t = u.up ? ticket : ticket - ups, per = shape.blocks * shape.splits;
+    u.number = per == 1 ? t : (int)__umulhi((uint32_t)t, shape.inverse);
     while (u.number * per > t) --u.number;       // (too large by one where the product is beyond 2^32)
     u.block = t - u.number * per;
+    u.part = 0;
+    if (shape.splits > 1) {
+        u.part = u.block % shape.splits;
+        u.block /= shape.splits;
+    }
     u.expert = s.active[u.number];
     u.first = s.first[u.number];
     u.end = s.first[u.number + 1];
     return u;
 }
 
-// The matrix of a unit: 32 columns from its first row on, and 32 more `second` bytes behind them; how many bytes of each there are.
+// The matrix of a unit as a warp sees it: 32 columns from its first row on, and 32 more `second` bytes behind them; how many bytes of each there
+// are; the warp's stages: from `step` to `end`, every hop-th.
 struct Matrix {
     const char* at;
     long long second;
@@ -279,6 +293,7 @@ struct Matrix {
     // the halves fill; and the copy of one more piece of each row)
     const char* lane_at;
     bool lane_there;
+    int step, end, hop;
 };
 
 template <typename T, bool WIDE>
@@ -287,20 +302,27 @@ __device__ __forceinline__ Matrix matrix_of(const Layer& p, const Unit& u) {
     constexpr int kSize = sizeof(T);
     Matrix m;
     auto bytes = [](int columns) { return max(0, min(columns, 32)) * kSize; };
+    const Layer::Shape& shape = u.up ? p.up : p.down;
+    const int warp = threadIdx.x >> 5;
+    m.hop = kWarps >> shape.log_groups;
+    const int group = (u.block << shape.log_groups) + (warp >> (3 - shape.log_groups));
     if (u.up) {
-        m.at = (const char*)((const T*)a.w_up + u.expert * a.up_group_stride + 32 * u.block);
+        m.at = (const char*)((const T*)a.w_up + u.expert * a.up_group_stride + 32 * group);
         m.second = (long long)a.inner * kSize;
-        m.first_bytes = m.second_bytes = bytes(a.inner - 32 * u.block);
+        m.first_bytes = m.second_bytes = bytes(a.inner - 32 * group);
         m.stride = (int)a.up_row_stride * kSize;
         m.depth = a.width;
     } else {
-        m.at = (const char*)((const T*)a.w_down + u.expert * a.down_group_stride + kUnit * u.block);
+        m.at = (const char*)((const T*)a.w_down + u.expert * a.down_group_stride + kUnit * group);
         m.second = 32 * kSize;
-        m.first_bytes = bytes(a.width - kUnit * u.block);
-        m.second_bytes = bytes(a.width - kUnit * u.block - 32);
+        m.first_bytes = bytes(a.width - kUnit * group);
+        m.second_bytes = bytes(a.width - kUnit * group - 32);
         m.stride = (int)a.down_row_stride * kSize;
         m.depth = a.inner;
     }
+    const int stages = (m.depth + Stage<T, WIDE>::kDepth - 1) / Stage<T, WIDE>::kDepth, share = u.up ? p.up_share : p.down_share;
+    m.step = u.part * share + (warp & (m.hop - 1));
+    m.end = m.first_bytes > 0 ? min(stages, (u.part + 1) * share) : 0;
     constexpr int kHalf = 4 * Stage<T, WIDE>::kPieces;
     const int lane = threadIdx.x & 31, row = lane / (2 * kHalf), half = lane / kHalf & 1, piece = lane % kHalf;
     m.lane_at = m.at + (long long)m.stride * row + (half ? m.second : 0) + piece * 16;
@@ -509,8 +531,9 @@ __device__ __forceinline__ void multiply(float (&acc)[4][2][4], const Matrix& m,
 // The CTA's coming unit of the second matrix into the L2, so that memory does not wait for the first products with it: lines of
 // 128 bytes, up to 1,024 rows (at F = 1,024 the units of all CTAs are 38 MB).
 __device__ __forceinline__ void prefetch_unit(const Matrix& m) {
+    if (m.first_bytes == 0) return;
     const int rows = min(m.depth, 1024);
-    for (int k = threadIdx.x; k < rows; k += kThreads) {
+    for (int k = ((threadIdx.x >> 5) & (m.hop - 1)) * 32 + (threadIdx.x & 31); k < rows; k += m.hop * 32) {
         const char* const at = m.at + (long long)m.stride * k;
         asm volatile("prefetch.global.L2 [%0];" ::"l"(at));
         const char* const last = at + (m.second_bytes > 0 ? m.second + m.second_bytes : m.first_bytes) - 1;
@@ -524,6 +547,12 @@ __device__ __forceinline__ int add_acquire_release(int32_t* at) {
     int before;
     asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(before) : "l"(at) : "memory");
     return before;
+}
+
+__device__ __forceinline__ int load_relaxed(const int32_t* at) {
+    int v;
+    asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(at) : "memory");
+    return v;
 }
 
 __device__ __forceinline__ int load_acquire(const int32_t* at) {
@@ -565,10 +594,10 @@ __device__ __forceinline__ void begin(const Layer& p, const Ring& ring, const Ma
     using S = Stage<T, WIDE>;
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) {
-        const int step = (threadIdx.x >> 5) + i * kWarps;
+        const int step = m.step + i * m.hop;
         const uint32_t slot = ring.template slot<S::kBytes>(i);
         // (nothing is asked for past the end: it would not be waited for before its place is filled again)
-        if (step * S::kDepth < m.depth) {
+        if (step < m.end) {
             if (matrix) bring_matrix<T, WIDE>(m, step, slot);
             if (rows) bring_rows<T, WIDE>(p, r, m.depth, step, slot);
         }
@@ -588,12 +617,12 @@ __device__ __forceinline__ void product(const Layer& p, Ring& ring, const Matrix
 #pragma unroll
             for (int q = 0; q < 4; ++q) acc[i][n][q] = 0.0f;
     if (all) copies_wait<0>();
-    for (int step = threadIdx.x >> 5; step * S::kDepth < m.depth; step += kWarps) {
+    for (int step = m.step; step < m.end; step += m.hop) {
         copies_wait<kStages - 2>();
         __syncwarp();                            // every lane's copies of this stage are here, and the stage before has been read
         const uint32_t next = ring.template slot<S::kBytes>(kStages - 1);
-        const int coming = step + (kStages - 1) * kWarps;
-        if (coming * S::kDepth < m.depth) {
+        const int coming = step + (kStages - 1) * m.hop;
+        if (coming < m.end) {
             bring_matrix<T, WIDE>(m, coming, next);
             bring_rows<T, WIDE>(p, r, m.depth, coming, next);
         }
@@ -615,26 +644,10 @@ __device__ __forceinline__ void turn_in(float (&turn)[kWarps][kUnit][8], const f
                 n == 0 ? make_float2(acc[i][0][2 * b], acc[i][0][2 * b + 1]) : make_float2(acc[i][1][2 * b], acc[i][1][2 * b + 1]);
 }
 
-// Lane l of warp j takes columns 8 (l / 8) + j and that + 32 of row l % 8 out: the gate's result for h, or the two columns of a pair's part.
-template <typename T, bool WIDE>
-__device__ __forceinline__ void turn_out(const Layer& p, const Smem<T, WIDE>& s, const Unit& u, int first) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = first + (lane & 7);
-    float low = 0.0f, high = 0.0f;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        low += s.turn[w][8 * warp + (lane >> 3)][lane & 7];
-        high += s.turn[w][8 * warp + 4 + (lane >> 3)][lane & 7];
-    }
-    if (at >= u.end) return;
-    if (!u.up) {
-        float* const to = p.parts + s.pair[at] * p.part_stride + kUnit * u.block + 8 * (lane >> 3) + warp;
-        to[0] = low;
-        to[32] = high;
-        return;
-    }
-    const int column = 32 * u.block + 8 * (lane >> 3) + warp;
-    const float h = column < p.a.inner ? low / (1.0f + expf(-low)) * high : 0.0f;
-    float* const to = p.h + s.pair[at] * p.h_stride;
+template <typename T>
+__device__ __forceinline__ void put_h(const Layer& p, int pair, int column, float gate, float up) {
+    const float h = column < p.a.inner ? gate / (1.0f + expf(-gate)) * up : 0.0f;
+    float* const to = p.h + pair * p.h_stride;
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
         const __nv_bfloat16 hi = __float2bfloat16_rn(h);
         const float rest = fabsf(h) <= 3.3e38f ? h - __bfloat162float(hi) : 0.0f;
@@ -646,40 +659,110 @@ __device__ __forceinline__ void turn_out(const Layer& p, const Smem<T, WIDE>& s,
     }
 }
 
-// y of 64 columns: what the experts of each token have given, in the order of its choices. Four columns a thread, 16 tokens at a time.
-template <typename T>
-__device__ __noinline__ void combine(const Layer& p, int block) {
-    const fmb_experts_t& a = p.a;
-    const int c = kUnit * block + 4 * (threadIdx.x & 15);
-    for (int t = threadIdx.x >> 4; t < a.tokens; t += kThreads / 16) {
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int j0 = 0; j0 < a.top; j0 += 4) {
-            float w[4];
-            float4 v[4];
+// Lane l of warp j takes columns 8 (l / 8) + j and that + 32 of row l % 8 out, of each group of 64: the gate's result for h, or the two columns
+// of a pair's part.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void turn_out(const Layer& p, const Smem<T, WIDE>& s, const Unit& u, int first) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = first + (lane & 7);
+    const Layer::Shape& shape = u.up ? p.up : p.down;
+    const int warps = kWarps >> shape.log_groups;
+    const long long pairs = (long long)p.a.tokens * p.a.top;
+    for (int q = 0; q < 1 << shape.log_groups; ++q) {
+        float low = 0.0f, high = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int pair = t * a.top + j0 + j;
-                const bool there = j0 + j < a.top;
-                const int e = there ? __ldg(a.chosen + pair) : -1;
-                w[j] = there ? __ldg(a.weights + pair) : 0.0f;
-                // (of a choice that is no expert nothing has been written)
-                v[j] = there ? __ldcg(reinterpret_cast<const float4*>(p.parts + pair * p.part_stride + c)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                if (e < 0 || e >= a.experts) w[j] = 0.0f, v[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                sum.x += w[j] * v[j].x;
-                sum.y += w[j] * v[j].y;
-                sum.z += w[j] * v[j].z;
-                sum.w += w[j] * v[j].w;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w >= warps) break;
+            low += s.turn[q * warps + w][8 * warp + (lane >> 3)][lane & 7];
+            high += s.turn[q * warps + w][8 * warp + 4 + (lane >> 3)][lane & 7];
+        }
+        if (at >= u.end) continue;
+        const int group = (u.block << shape.log_groups) + q, place = 8 * (lane >> 3) + warp, pair = s.pair[at];
+        if (!u.up) {
+            if (kUnit * group >= p.part_stride) continue;
+            float* const to = p.parts + (u.part * pairs + pair) * p.part_stride + kUnit * group + place;
+            to[0] = low;
+            to[32] = high;
+        } else if (32 * group < p.h_stride) {
+            if (shape.splits > 1) {
+                float* const to = p.up_parts + (u.part * pairs + pair) * 2 * p.h_stride + 32 * group + place;
+                to[0] = low;
+                to[p.h_stride] = high;
+            } else {
+                put_h<T>(p, pair, 32 * group + place, low, high);
             }
         }
-        T* const y = (T*)a.y + t * a.y_stride + c;
-        const float out[4] = {sum.x, sum.y, sum.z, sum.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c + i < a.width) y[i] = rounded<T>(out[i]);
     }
+}
+
+// h of a block whose depth units have shared, by the one that was done last
+template <typename T, bool WIDE>
+__device__ __noinline__ void join_up(const Layer& p, const Smem<T, WIDE>& s, const Unit& u) {
+    const int columns = 32 << p.up.log_groups, first = u.block * columns;
+    const long long pairs = (long long)p.a.tokens * p.a.top;
+    for (int i = threadIdx.x; i < (u.end - u.first) * columns; i += kThreads) {
+        const int pair = s.pair[u.first + i / columns], column = first + i % columns;
+        if (column >= p.h_stride) continue;
+        float gate = 0.0f, up = 0.0f;
+#pragma unroll 4
+        for (int part = 0; part < p.up.splits; ++part) {
+            const float* const from = p.up_parts + (part * pairs + pair) * 2 * p.h_stride + column;
+            gate += __ldcg(from);
+            up += __ldcg(from + p.h_stride);
+        }
+        put_h<T>(p, pair, column, gate, up);
+    }
+}
+
+// y of 64 columns and kCombined tokens: what the experts of each token have given, in the order of its choices. Four columns a thread. The
+// weights are asked for before the wait for the parts (`await`).
+constexpr int kCombined = kThreads / 16;
+
+template <typename T, typename F>
+__device__ __forceinline__ void combine(const Layer& p, int group, int tokens, F await) {
+    const fmb_experts_t& a = p.a;
+    const long long pairs = (long long)a.tokens * a.top;
+    const int c = kUnit * group + 4 * (threadIdx.x & 15), t = tokens * kCombined + (threadIdx.x >> 4);
+    const bool exists = c < a.width && t < a.tokens;
+    float w[FMB_MAX_TOP];
+    unsigned live = 0;                           // choices that are experts: of the others nothing has been written
+#pragma unroll
+    for (int j = 0; j < FMB_MAX_TOP; ++j) {
+        const bool there = exists && j < a.top;
+        const int e = there ? __ldg(a.chosen + t * a.top + j) : -1;
+        w[j] = there ? __ldg(a.weights + t * a.top + j) : 0.0f;
+        if (e >= 0 && e < a.experts) live |= 1u << j;
+    }
+    await();
+    if (!exists) return;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int j0 = 0; j0 < FMB_MAX_TOP; j0 += 8) {
+        if (j0 >= a.top) break;
+        float4 v[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float* const from = p.parts + (t * a.top + j0 + j) * p.part_stride + c;
+            const bool there = live >> (j0 + j) & 1;
+            v[j] = there ? __ldcg(reinterpret_cast<const float4*>(from)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int part = 1; part < p.down.splits && there; ++part) {
+                const float4 more = __ldcg(reinterpret_cast<const float4*>(from + part * pairs * p.part_stride));
+                v[j].x += more.x; v[j].y += more.y; v[j].z += more.z; v[j].w += more.w;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if (!(live >> (j0 + j) & 1)) continue;
+            sum.x += w[j0 + j] * v[j].x;
+            sum.y += w[j0 + j] * v[j].y;
+            sum.z += w[j0 + j] * v[j].z;
+            sum.w += w[j0 + j] * v[j].w;
+        }
+    }
+    T* const y = (T*)a.y + t * a.y_stride + c;
+    const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (c + i < a.width) y[i] = rounded<T>(out[i]);
 }
 
 // Which pairs belong to which expert, and which experts have any; the counters of the next launch become zero. Pairs of one expert stand in
@@ -758,7 +841,6 @@ k_experts(const __grid_constant__ Layer p) {
     if (threadIdx.x == 0) {
         s.ticket = atomicAdd(next, 1);
         s.gave_up = 0;
-        s.last[1] = -1;
     }
     // (the lists' places, whether in use or not: their numbers need not be waited for)
     const int actives = __ldg(p.lists), most = min(a.experts, a.tokens * a.top);
@@ -777,44 +859,50 @@ k_experts(const __grid_constant__ Layer p) {
             ((T*)a.y)[i / a.width * a.y_stride + i % a.width] = zero<T>();
         return;
     }
-    const int ups = actives * p.up_units, units = ups + actives * p.down_units;
+    // three kinds of units, of which each waits for ones of the kind before: h, the parts of y, and y
+    const int ups = actives * p.up.blocks * p.up.splits, downs = ups + actives * p.down.blocks * p.down.splits;
+    const int groups = (a.width + kUnit - 1) / kUnit, units = downs + groups * ((a.tokens + kCombined - 1) / kCombined);
+    int32_t* const shared = columns + p.down.blocks;
+    // Thread 0 waits for a counter, with a limit, after which all waits end at once and the results are said to be none; the others wait for it
+    // (2,048 warps that ask for the same eight counters hold up those that count)
+    auto await = [&](const int32_t* counter, int value) {
+        if (threadIdx.x == 0) {
+            long long spins = 0;
+            while (load_relaxed(counter) < value && !s.gave_up)
+                if (++spins < kSpins) __nanosleep(20);
+                else s.gave_up = 1;
+            (void)load_acquire(counter);
+            if (s.gave_up && a.status) atomicOr(a.status, (uint32_t)FMB_STATUS_TENSOR_TIMEOUT);
+        }
+        __syncthreads();
+    };
     int ticket = s.ticket;
-    if (ticket >= units) return;
-    Unit u = unit_of(p, s, ticket, ups);
-    Matrix m = matrix_of<T, WIDE>(p, u);
-    Rows r = rows_of<T, WIDE>(p, s, u, u.first);
+    Unit u;
+    Matrix m;
+    Rows r;
     Ring ring = {smem_at(s.ring[warp]), 0};
-    bool ready = u.up;                           // what the unit's rows are has been written
-    begin<T, WIDE>(p, ring, m, r, true, ready);
-    int round = 0;
-    for (;;) {
+    bool ready = false, turning = false;         // ready: what the unit's rows are has been written
+    // the unit of the ticket, if it is one of a product, and its first stages
+    auto go_on = [&]() {
+        if (ticket >= downs) return;
+        u = unit_of(p, s, ticket, ups);
+        m = matrix_of<T, WIDE>(p, u);
+        r = rows_of<T, WIDE>(p, s, u, u.first);
+        ready = u.up;
+        begin<T, WIDE>(p, ring, m, r, true, ready);
+        if (turning) prefetch_unit(m);
+    };
+    go_on();
+    while (ticket < downs) {
         bool all = false;
         if (!ready) {
-            if (lane == 0) {
-                long long spins = 0;
-                while (load_acquire(done + u.number) < p.up_units && !s.gave_up)
-                    if (++spins < kSpins) __nanosleep(32);
-                    else s.gave_up = 1;
-                if (s.gave_up && a.status) atomicOr(a.status, (uint32_t)FMB_STATUS_TENSOR_TIMEOUT);
-            }
-            __syncwarp();
+            await(done + u.number, p.up.blocks);
             begin<T, WIDE>(p, ring, m, r, false, true);
             all = true;
         }
         // The unit after this one: asked for now, when this one no longer waits for others, and needed at its end.
         const int ahead = threadIdx.x == 0 ? atomicAdd(next, 1) : 0;
         const Unit v = u;
-        bool turning = false;
-        // the unit after this one and its first stages
-        auto go_on = [&]() {
-            if (ticket >= units) return;
-            u = unit_of(p, s, ticket, ups);
-            m = matrix_of<T, WIDE>(p, u);
-            r = rows_of<T, WIDE>(p, s, u, u.first);
-            ready = u.up;
-            begin<T, WIDE>(p, ring, m, r, true, ready);
-            if (turning) prefetch_unit(m);
-        };
         for (int at = v.first; at < v.end; at += 16) {
             const bool last = at + 16 >= v.end, two_blocks = v.end - at > 8;
             float acc[4][2][4];
@@ -842,38 +930,64 @@ k_experts(const __grid_constant__ Layer p) {
                 __syncthreads();
             }
         }
-        // Thread 0 tells the others that the unit is done, while its CTA goes on; whether the unit was the last of its columns the CTA
-        // looks at after the next one.
-        if (s.last[round ^ 1] >= 0) combine<T>(p, s.last[round ^ 1]);
-        if (threadIdx.x == 0) {
-            s.last[round] = -1;
-            if (v.up) add_release(done + v.number);
-            else if (add_acquire_release(columns + v.block) == actives - 1) s.last[round] = v.block;
+        bool tells = true;                       // thread 0, while its CTA goes on
+        if (v.up && p.up.splits > 1) {
+            if (threadIdx.x == 0) s.joins = add_acquire_release(shared + v.number * p.up.blocks + v.block) == p.up.splits - 1;
+            __syncthreads();
+            tells = s.joins;
+            if (tells) join_up<T, WIDE>(p, s, v);
+            __syncthreads();
         }
+        if (threadIdx.x == 0 && tells) add_release(v.up ? done + v.number : columns + v.block);
         if (turning) go_on();
-        if (ticket >= units) break;
-        round ^= 1;
     }
-    __syncthreads();
-    if (s.last[round] >= 0) combine<T>(p, s.last[round]);
+    while (ticket < units) {
+        const int group = (ticket - downs) % groups, tokens = (ticket - downs) / groups;
+        // (the barrier of the wait: the ticket has been read)
+        combine<T>(p, group, tokens, [&]() { await(columns + (group >> p.down.log_groups), actives * p.down.splits); });
+        if (threadIdx.x == 0) s.ticket = atomicAdd(next, 1);
+        __syncthreads();
+        ticket = s.ticket;
+    }
 }
 
 long long up_to(long long n, long long step) { return (n + step - 1) / step * step; }
 
+// How a product with `columns` (32 or 64 a group) and `depth` is cut for the experts that tokens choose at most.
+Layer::Shape shape_of(int experts, int columns, int of_group, int depth, int stage_depth) {
+    constexpr int kCtas = 2 * 148;
+    Layer::Shape s;
+    const int stages = ceil_div(depth, stage_depth);
+    s.log_groups = 0;
+    s.splits = 1;
+    while (s.log_groups < 3 && stages << s.log_groups < 8 * kWarps && (long long)experts * ceil_div(columns, of_group << (s.log_groups + 1)) >= 2 * kCtas) ++s.log_groups;
+    s.blocks = ceil_div(columns, of_group << s.log_groups);
+    const long long units = (long long)experts * s.blocks;
+    if (2 * units <= kCtas) s.splits = (int)std::max<long long>(1, std::min<long long>({8, kCtas / units, stages / (2 * kWarps)}));
+    s.inverse = (uint32_t)(((1ull << 32) + s.blocks * s.splits - 1) / (s.blocks * s.splits));
+    return s;
+}
+
 struct Sizes {
-    long long control, lists, h, parts, x;       // in floats
+    Layer::Shape up, down;
+    long long control, lists, h, parts, up_parts, x;              // in floats
     long long h_stride, part_stride, x_stride;
 };
 
+// wide: whether the matrices' rows are whole pieces of 16 bytes (their stages are alike: the plan does not depend on it)
 Sizes sizes_of(const fmb_experts_t& a) {
     Sizes s;
     const long long pairs = (long long)a.tokens * a.top;
-    s.control = up_to(1 + a.experts + ceil_div(a.width, kUnit), 64);
+    const int experts = (int)std::min<long long>(a.experts, pairs), stage = a.type == FMB_TYPE_F32 ? Stage<float, true>::kDepth : Stage<__half, true>::kDepth;
+    s.up = shape_of(experts, a.inner, 32, a.width, stage);
+    s.down = shape_of(experts, a.width, kUnit, a.inner, stage);
+    s.control = up_to(1 + a.experts + s.down.blocks + (s.up.splits > 1 ? (long long)experts * s.up.blocks : 0), 64);
     s.lists = up_to(3 + 2 * a.experts + pairs, 64);
     s.h_stride = up_to(a.inner, 32);
     s.part_stride = up_to(a.width, kUnit);
     s.h = pairs * s.h_stride;
-    s.parts = pairs * s.part_stride;
+    s.parts = s.down.splits * pairs * s.part_stride;
+    s.up_parts = s.up.splits > 1 ? s.up.splits * pairs * 2 * s.h_stride : 0;
     s.x_stride = up_to(a.width, 8);
     s.x = a.tokens * s.x_stride;
     return s;
@@ -894,13 +1008,15 @@ int layer(const fmb_experts_t& a, cudaStream_t stream) {
     p.lists = p.control + size.control;
     p.h = a.scratch + size.control + size.lists;
     p.parts = p.h + size.h;
-    void* const packed = p.parts + size.parts;
+    p.up_parts = p.parts + size.parts;
+    void* const packed = p.up_parts + size.up_parts;
     p.h_stride = size.h_stride;
     p.part_stride = size.part_stride;
-    p.up_units = ceil_div(a.inner, 32);
-    p.down_units = ceil_div(a.width, kUnit);
-    p.up_inverse = (uint32_t)(((1ull << 32) + p.up_units - 1) / p.up_units);
-    p.down_inverse = (uint32_t)(((1ull << 32) + p.down_units - 1) / p.down_units);
+    p.up = size.up;
+    p.down = size.down;
+    const int stage = sizeof(T) == 4 ? Stage<float, true>::kDepth : Stage<__half, true>::kDepth;
+    p.up_share = ceil_div(ceil_div(a.width, stage), p.up.splits);
+    p.down_share = ceil_div(ceil_div(a.inner, stage), p.down.splits);
     const bool pack = !begin_at(a.x, a.x_stride, a.tokens, b, 8);
     p.x = pack ? packed : const_cast<void*>(a.x);
     p.x_stride = pack ? size.x_stride : a.x_stride;
@@ -911,7 +1027,7 @@ int layer(const fmb_experts_t& a, cudaStream_t stream) {
         return columns * b % 16 == 0 && begin_at(base, row, rows, b, 16) && begin_at(base, group, a.experts, b, 16);
     };
     const bool wide = pieces(a.w_up, a.up_row_stride, a.up_group_stride, a.width, a.inner) && pieces(a.w_down, a.down_row_stride, a.down_group_stride, a.inner, a.width);
-    const long long most = std::min<long long>(a.experts, (long long)a.tokens * a.top) * (p.up_units + p.down_units);
+    const long long most = std::min<long long>(a.experts, (long long)a.tokens * a.top) * (p.up.blocks * p.up.splits + p.down.blocks * p.down.splits);
     const int grid = (int)std::min<long long>(most, 2 * grp::sm_count());
     const auto kernel = wide ? k_experts<T, true> : k_experts<T, false>;
     const int smem = wide ? sizeof(Smem<T, true>) : sizeof(Smem<T, false>);
@@ -983,7 +1099,7 @@ int check_layer(const fmb_experts_t* a) {
 extern "C" FMB_API long long fmb_expert_layer_scratch(const fmb_experts_t* a) {
     if (check_layer(a) || a->tokens == 0) return 0;
     const Sizes s = sizes_of(*a);
-    return s.control + s.lists + s.h + s.parts + s.x;
+    return s.control + s.lists + s.h + s.parts + s.up_parts + s.x;
 }
 
 extern "C" FMB_API int fmb_expert_layer(const fmb_experts_t* a, fmb_stream_t stream) {

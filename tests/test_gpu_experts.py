@@ -76,8 +76,10 @@ def test_layer_against_float64(shape, dtype):
     y = experts.expert_layer(_wide(x, stride), up, down, routes)
     _check(y, x, up, down, chosen, weights)
     assert torch.equal(y, experts.expert_layer(x, up, down, routes))                     # the same bits again
-    one = experts.expert_layer(x[t - 1:], up, down, experts.Routes(chosen[t - 1:], weights[t - 1:]))
-    assert torch.equal(one, y[t - 1:])                                                    # whatever the other tokens are
+    others, elsewhere = torch.randn(x.shape, generator=g, device="cuda").to(dtype), torch.roll(chosen, 1, 0)
+    others[t - 1], elsewhere[t - 1] = x[t - 1], chosen[t - 1]
+    one = experts.expert_layer(others, up, down, experts.Routes(elsewhere, weights))
+    assert torch.equal(one[t - 1], y[t - 1])                                              # whatever the other tokens are
     given = torch.full((t, 3, width), 7.0, device="cuda", dtype=dtype)
     experts.expert_layer(x, up, down, routes, out=given[:, 1])
     assert torch.equal(given[:, 1], y) and bool((given[:, 0] == 7).all()) and bool((given[:, 2] == 7).all())
