@@ -42,21 +42,38 @@ template <typename T> __device__ __forceinline__ T zero() { return T(0.0f); }
 
 // --------------------------------------------------------------------------------------------------------------- route
 
-constexpr int kCluster = 8;                      // CTAs that share the depth of a token's logits
 
-// eight values from `at` on, of which `live` exist
+constexpr int kRouteChunk = 512;                 // of a CTA's depth, whose values of x lie in shared memory
+
+// eight values as they are in memory, and as floats
+template <typename T> struct Eight { uint32_t v[2 * sizeof(T)]; };
+
 template <typename T>
-__device__ __forceinline__ void load_eight(const T* __restrict__ at, int live, bool wide, float (&v)[8]) {
+__device__ __forceinline__ Eight<T> load_eight(const T* __restrict__ at, int live, bool wide) {
+    Eight<T> in = {};
     if (wide && live >= 8) {
-        uint4 in[sizeof(T) / 2];
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) in[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = to_float(reinterpret_cast<const T*>(in)[i]);
+        for (int i = 0; i < 2 * (int)sizeof(T); i += 4) {
+            const uint4 four = __ldg(reinterpret_cast<const uint4*>(at) + i / 4);
+            in.v[i] = four.x; in.v[i + 1] = four.y; in.v[i + 2] = four.z; in.v[i + 3] = four.w;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < live ? to_float(at[i]) : 0.0f;
+        for (int i = 0; i < 8; ++i) {
+            if (i >= live) break;
+            if constexpr (sizeof(T) == 4) in.v[i] = __ldg(reinterpret_cast<const uint32_t*>(at) + i);
+            else in.v[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(at) + i) << (16 * (i % 2));
+        }
     }
+    return in;
+}
+
+template <typename T>
+__device__ __forceinline__ float value(const Eight<T>& in, int i) {
+    const uint32_t w = in.v[i * sizeof(T) / 4];
+    if constexpr (sizeof(T) == 4) return __uint_as_float(w);
+    else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(i % 2 ? w & 0xffff0000u : w << 16);
+    else return __half2float(__ushort_as_half((uint16_t)(i % 2 ? w >> 16 : w)));
 }
 
 // floats in an order of unsigned numbers; NaN below all
@@ -65,95 +82,131 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return x != x ? 0u : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-// A cluster per token: each CTA takes an eighth of the depth, threads by packs of eight experts and rows of R.
-template <typename T>
+// CLUSTER CTAs for TOKENS tokens: each takes its share of the depth, threads by packs of eight experts and rows of R, which all tokens share; then
+// CTA c the choices of tokens c, c + CLUSTER, ... A cluster of eight for a token each where there are few (1 token of 2,048, 64 experts: 5.2 us),
+// for two to eight tokens where they would read much of R one by one, and a CTA alone beyond 128 tokens.
+template <typename T, int TOKENS, int CLUSTER>
 __global__ void __launch_bounds__(kThreads)
 k_route(fmb_route_t a, int wide, int rows) {
-    __shared__ float sums[kThreads * 8];
-    __shared__ float logits[FMB_MAX_GROUPS];
+    extern __shared__ float sums[];              // [kRouteChunk][TOKENS] values of x; then [TOKENS][rows][packs of eight]
     let_next_come();
-    const int token = blockIdx.x / kCluster, rank = blockIdx.x % kCluster, packs = (a.experts + 7) / 8;
+    const int first_token = blockIdx.x / CLUSTER * TOKENS, rank = blockIdx.x % CLUSTER, packs = (a.experts + 7) / 8;
     const int pack = threadIdx.x % packs, row = threadIdx.x / packs;
-    const T* const x = (const T*)a.x + token * a.x_stride;
-    const int begin = (int)((long long)a.width * rank / kCluster), end = (int)((long long)a.width * (rank + 1) / kCluster);
-    float sum[8] = {};
-    if (row < rows) {
-        for (int k0 = begin + row; k0 < end; k0 += 4 * rows) {
-            float w[4][8], v[4];
+    const int begin = (int)((long long)a.width * rank / CLUSTER), end = (int)((long long)a.width * (rank + 1) / CLUSTER);
+    const T* const x = (const T*)a.x + first_token * a.x_stride;
+    constexpr int kDeep = sizeof(T) == 4 ? 4 : 8;                 // rows of R on their way
+    float sum[TOKENS][8] = {};
+    for (int c0 = begin; c0 < end; c0 += kRouteChunk) {
+        const int count = min(kRouteChunk, end - c0);
+        if (c0 > begin) __syncthreads();
+        for (int i = threadIdx.x; i < TOKENS * count; i += kThreads) {
+            const int t = i / count, k = i - t * count;
+            sums[k * TOKENS + t] = first_token + t < a.tokens ? to_float(x[t * a.x_stride + c0 + k]) : 0.0f;
+        }
+        __syncthreads();
+        if (row >= rows) continue;
+        for (int k0 = row; k0 < count; k0 += kDeep * rows) {
+            Eight<T> w[kDeep];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < kDeep; ++j) {
                 const int k = k0 + j * rows;
-                v[j] = k < end ? to_float(x[k]) : 0.0f;
-                load_eight((const T*)a.router + k * a.router_stride + 8 * pack, k < end ? a.experts - 8 * pack : 0, wide, w[j]);
+                w[j] = load_eight((const T*)a.router + (c0 + k) * a.router_stride + 8 * pack, k < count ? a.experts - 8 * pack : 0, wide);
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < kDeep; ++j) {
+                const int k = k0 + j * rows;
+                if (k >= count) break;
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (k0 + j * rows < end) sum[i] = fmaf(v[j], w[j][i], sum[i]);
+                for (int t = 0; t < TOKENS; ++t) {
+                    const float v = sums[k * TOKENS + t];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) sum[t][i] = fmaf(v, value(w[j], i), sum[t][i]);
+                }
+            }
         }
+    }
+    __syncthreads();
+    if (row < rows) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sums[row * packs * 8 + 8 * pack + i] = sum[i];
+        for (int t = 0; t < TOKENS; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sums[(t * rows + row) * packs * 8 + 8 * pack + i] = sum[t][i];
     }
     for (int half = rows / 2; half > 0; half /= 2) {
         __syncthreads();
-        for (int i = threadIdx.x; i < half * packs * 8; i += kThreads) sums[i] += sums[i + half * packs * 8];
-    }
-    // the CTAs' sums, in their order, by the first
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank == 0) {
-        const uint32_t here = (uint32_t)__cvta_generic_to_shared(sums);
-        for (int e = threadIdx.x; e < a.experts; e += kThreads) {
-            float part[kCluster];
-#pragma unroll
-            for (int c = 0; c < kCluster; ++c) {
-                uint32_t there;
-                asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here + 4 * e), "r"(c));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[c]) : "r"(there) : "memory");
-            }
-            float all = part[0];
-#pragma unroll
-            for (int c = 1; c < kCluster; ++c) all += part[c];
-            logits[e] = all;
+        const int size = half * packs * 8;
+        for (int i = threadIdx.x; i < TOKENS * size; i += kThreads) {
+            const int t = TOKENS == 1 ? 0 : i / size, at = t * rows * packs * 8 + i - t * size;
+            sums[at] += sums[at + size];
         }
     }
-    // (their shared memory lives until it has been read)
-    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    if (rank != 0) return;
+    auto meet = []() {
+        if constexpr (CLUSTER > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else __syncthreads();
+    };
+    meet();
     // An expert's place is the number of those before it (larger logit, or the same and a lower number): each thread counts for its own,
     // which takes one wait where choosing one after the other takes one each. Numbers are made unlike by the expert's.
-    __shared__ unsigned long long order[FMB_MAX_GROUPS + 1];
-    __shared__ float best[FMB_MAX_TOP], warp_total[kWarps];
-    for (int e = threadIdx.x; e <= a.experts; e += kThreads)
-        order[e] = e < a.experts ? (unsigned long long)ordered(logits[e]) << 32 | (0xffffffffu - e) : 0;
-    __syncthreads();
-    for (int e = threadIdx.x; e < a.experts; e += kThreads) {
-        const unsigned long long mine = order[e];
-        int before = 0;
-#pragma unroll 4
-        for (int f = 0; f < a.experts; f += 2) {
-            const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(order + f);
-            before += (two.x > mine) + (two.y > mine);
+    __shared__ alignas(16) unsigned long long order[FMB_MAX_GROUPS + 2];
+    __shared__ float logits[FMB_MAX_GROUPS], best[FMB_MAX_TOP], warp_total[kWarps];
+    for (int own = rank; own < TOKENS; own += CLUSTER) {
+        const long long token = first_token + own;
+        if (token >= a.tokens) break;            // (the same for the CTA)
+        for (int e = threadIdx.x; e <= a.experts; e += kThreads) {
+            // the CTAs' sums, in their order
+            float all = 0.0f;
+            if (e < a.experts) {
+                const float* const mine = sums + own * rows * packs * 8 + e;
+                if constexpr (CLUSTER > 1) {
+                    const uint32_t here = (uint32_t)__cvta_generic_to_shared(mine);
+                    float part[CLUSTER];
+#pragma unroll
+                    for (int c = 0; c < CLUSTER; ++c) {
+                        uint32_t there;
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(c));
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[c]) : "r"(there) : "memory");
+                    }
+                    all = part[0];
+#pragma unroll
+                    for (int c = 1; c < CLUSTER; ++c) all += part[c];
+                } else {
+                    all = *mine;
+                }
+                logits[e] = all;
+            }
+            order[e] = e < a.experts ? (unsigned long long)ordered(all) << 32 | (0xffffffffu - e) : 0;
         }
-        if (before < a.top) {
-            best[before] = logits[e];
-            a.chosen[token * (long long)a.top + before] = e;
-        }
-    }
-    __syncthreads();
-    const float first = best[0];
-    float total = 0.0f;
-    if (a.normalise) {
-        for (int j = 0; j < a.top; ++j) total += expf(best[j] - first);
-    } else {
-        for (int e = threadIdx.x; e < a.experts; e += kThreads) total += expf(logits[e] - first);
-        total = warp_sum(total);
-        if ((threadIdx.x & 31) == 0) warp_total[threadIdx.x >> 5] = total;
         __syncthreads();
-        total = 0.0f;
-        for (int w = 0; w < kWarps; ++w) total += warp_total[w];
+        for (int e = threadIdx.x; e < a.experts; e += kThreads) {
+            const unsigned long long mine = order[e];
+            int before = 0;
+#pragma unroll 4
+            for (int f = 0; f < a.experts; f += 2) {
+                const ulonglong2 two = *reinterpret_cast<const ulonglong2*>(order + f);
+                before += (two.x > mine) + (two.y > mine);
+            }
+            if (before < a.top) {
+                best[before] = logits[e];
+                a.chosen[token * a.top + before] = e;
+            }
+        }
+        __syncthreads();
+        const float first = best[0];
+        float total = 0.0f;
+        if (a.normalise) {
+            for (int j = 0; j < a.top; ++j) total += expf(best[j] - first);
+        } else {
+            for (int e = threadIdx.x; e < a.experts; e += kThreads) total += expf(logits[e] - first);
+            total = warp_sum(total);
+            if ((threadIdx.x & 31) == 0) warp_total[threadIdx.x >> 5] = total;
+            __syncthreads();
+            total = 0.0f;
+            for (int w = 0; w < kWarps; ++w) total += warp_total[w];
+        }
+        if (threadIdx.x < a.top) a.weights[token * a.top + threadIdx.x] = expf(best[threadIdx.x] - first) / total;
+        if (CLUSTER < TOKENS) __syncthreads();
     }
-    if (threadIdx.x < a.top) a.weights[token * (long long)a.top + threadIdx.x] = expf(best[threadIdx.x] - first) / total;
+    if (CLUSTER > 1) meet();                     // shared memory lives until it has been read
 }
 
 // --------------------------------------------------------------------------------------------------------------- layer
@@ -1039,25 +1092,36 @@ int layer(const fmb_experts_t& a, cudaStream_t stream) {
 
 bool fits(const void* base, long long stride, int bytes) { return ((uintptr_t)base & 15) == 0 && stride * bytes % 16 == 0; }
 
-template <typename T>
+template <typename T, int TOKENS, int CLUSTER>
 int route(const fmb_route_t& a, cudaStream_t stream) {
-    const int packs = (a.experts + 7) / 8;
     int rows = 1;
-    while (2 * rows * packs <= kThreads) rows *= 2;
+    while (2 * rows * ((a.experts + 7) / 8) <= kThreads) rows *= 2;
+    const int smem = TOKENS * std::max(kRouteChunk, rows * ((a.experts + 7) / 8) * 8) * (int)sizeof(float);
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_route<T, TOKENS, CLUSTER>, TOKENS * kThreads * 8 * (int)sizeof(float)));
     cudaLaunchConfig_t config = {};
     cudaLaunchAttribute cluster;
     cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = kCluster;
+    cluster.val.clusterDim.x = CLUSTER;
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    config.gridDim = dim3((unsigned)a.tokens * kCluster);
+    config.gridDim = dim3((unsigned)ceil_div(a.tokens, TOKENS) * CLUSTER);
     config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = smem;
     config.stream = stream;
     config.attrs = &cluster;
-    config.numAttrs = 1;
-    const int wide = fits(a.router, a.router_stride, sizeof(T));
-    FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_route<T>, a, wide, rows));
+    config.numAttrs = CLUSTER > 1;
+    FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_route<T, TOKENS, CLUSTER>, a, (int)fits(a.router, a.router_stride, sizeof(T)), rows));
     FMB_LAUNCH_CHECK();
     return FMB_OK;
+}
+
+template <typename T>
+int route(const fmb_route_t& a, cudaStream_t stream) {
+    // by what the tokens would read of R one by one (us with one, two, four, eight tokens a cluster: 64 tokens and 32 experts of 4,096: 7.7, -, 10.9, -;
+    // 64 and 256: -, -, 24, -; 128 and 256: 56, -, -, 35)
+    if (a.tokens > 128) return route<T, 8, 1>(a, stream);
+    const int logits = a.tokens * a.experts;
+    return logits <= 4096 ? route<T, 1, 8>(a, stream) : logits <= 8192 ? route<T, 2, 8>(a, stream)
+           : logits <= 16384 ? route<T, 4, 8>(a, stream) : route<T, 8, 8>(a, stream);
 }
 
 }  // namespace
