@@ -11,9 +11,10 @@
 // Bound by memory: every row is read once and every row of the table written once.
 
 #include "early.cuh"
-#include "grouped.cuh"
+#include "eight.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace fmb {
 namespace emb {
@@ -29,39 +30,76 @@ template <> __device__ __forceinline__ float rounded<float>(float x) { return x;
 // N values side by side in one load or store of up to 16 bytes
 template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T v[N]; };
 
+// (what is written is not read again soon: 200,000 rows of 512 fp16 values 71 us, and 61 so)
+template <typename T, int N>
+__device__ __forceinline__ void store_streaming(T* to, const Pack<T, N>& v) {
+    if constexpr (N * sizeof(T) == 16) __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&v));
+    else if constexpr (N * sizeof(T) == 8) __stcs(reinterpret_cast<uint2*>(to), *reinterpret_cast<const uint2*>(&v));
+    else *reinterpret_cast<Pack<T, N>*>(to) = v;
+}
+
 // -------------------------------------------------------------------------------------------------------------- lookup
 
-// Lanes that share a row: as many as it has packs, a power of two up to 32; a warp has 32 / lanes rows at a time and four packs a lane
-// on their way. N = 1 where rows do not start at multiples of a pack.
-template <typename T, typename O, typename K, int N>
+// Lanes that share a row: as many as it has packs of N values, a power of two up to 32; a warp has ROWS times 32 / lanes rows at a time, and a
+// lane four packs on their way. WIDE: rows start at multiples of a pack; else a pack is eight values by the words that they lie in.
+template <typename T, typename O, typename K, int N, int ROWS, bool WIDE>
 __global__ void __launch_bounds__(256)
 k_embedding(fmb_embedding_t a, int lanes) {
+    constexpr int kOfRow = 4 / ROWS;             // packs of a row on their way
+    static_assert(WIDE || N == eight::kEach, "eight values by words");
+    using In = typename std::conditional<WIDE, Pack<T, N>, eight::Raw<T>>::type;
     const int lane = threadIdx.x & 31, part = lane & (lanes - 1), per_warp = 32 / lanes;
     const long long warp = (blockIdx.x * 256ll + threadIdx.x) >> 5, warps = gridDim.x * 8ll;
     const float scale = (float)a.scale;
     const int packs = a.width / N;
-    for (long long r = warp * per_warp + lane / lanes; r < a.rows; r += warps * per_warp) {
-        const K token = ((const K*)a.tokens)[r];
-        const bool live = token >= 0 && token < (K)a.vocabulary;
-        if (!live && !a.zero_rest) continue;
-        const T* const from = (const T*)a.source + (live ? (long long)token : 0) * a.source_stride;
-        O* const to = (O*)a.out + r * a.out_stride;
-        for (int c = part; c < packs; c += 4 * lanes) {
-            Pack<T, N> in[4];
+    for (long long r0 = warp * per_warp * ROWS + lane / lanes; r0 < a.rows; r0 += warps * per_warp * ROWS) {
+        K token[ROWS];
+        bool live[ROWS];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (live && c + j * lanes < packs) in[j] = *reinterpret_cast<const Pack<T, N>*>(from + (c + j * lanes) * N);
+        for (int q = 0; q < ROWS; ++q) token[q] = r0 + q * per_warp < a.rows ? ((const K*)a.tokens)[r0 + q * per_warp] : (K)-1;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (c + j * lanes >= packs) break;
-                Pack<O, N> out;
+        for (int q = 0; q < ROWS; ++q) live[q] = token[q] >= 0 && token[q] < (K)a.vocabulary;
+        auto from = [&](int q) { return (const T*)a.source + (live[q] ? (long long)token[q] : 0) * a.source_stride; };
+        auto to = [&](int q) { return (O*)a.out + (r0 + q * per_warp) * a.out_stride; };
+        auto written = [&](int q) { return r0 + q * per_warp < a.rows && (live[q] || a.zero_rest); };
+        for (int c = part; c < packs; c += kOfRow * lanes) {
+            In in[ROWS][kOfRow];
 #pragma unroll
-                for (int i = 0; i < N; ++i) out.v[i] = rounded<O>(live ? scale * to_float(in[j].v[i]) : 0.0f);
-                *reinterpret_cast<Pack<O, N>*>(to + (c + j * lanes) * N) = out;
+            for (int q = 0; q < ROWS; ++q)
+#pragma unroll
+                for (int j = 0; j < kOfRow; ++j) {
+                    if (live[q] && c + j * lanes < packs) {
+                        if constexpr (WIDE) in[q][j] = *reinterpret_cast<const In*>(from(q) + (c + j * lanes) * N);
+                        else in[q][j] = eight::load<T, false>(from(q) + (c + j * lanes) * N, N);
+                    }
+                }
+#pragma unroll
+            for (int q = 0; q < ROWS; ++q) {
+                if (!written(q)) continue;
+#pragma unroll
+                for (int j = 0; j < kOfRow; ++j) {
+                    if (c + j * lanes >= packs) break;
+                    O* const at = to(q) + (c + j * lanes) * N;
+                    if constexpr (WIDE) {
+                        Pack<O, N> out;
+#pragma unroll
+                        for (int i = 0; i < N; ++i) out.v[i] = rounded<O>(live[q] ? scale * to_float(in[q][j].v[i]) : 0.0f);
+                        store_streaming<O, N>(at, out);
+                    } else {
+                        float x[N] = {};
+                        if (live[q]) eight::unpack<T>(in[q][j], x);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) x[i] = live[q] ? scale * x[i] : 0.0f;
+                        eight::store<O, false>(at, N, x);
+                    }
+                }
             }
         }
         // the columns behind the last whole pack
-        for (int c = packs * N + part; c < a.width; c += lanes) to[c] = rounded<O>(live ? scale * to_float(from[c]) : 0.0f);
+        for (int c = packs * N + part; c < a.width; c += lanes)
+#pragma unroll
+            for (int q = 0; q < ROWS; ++q)
+                if (written(q)) to(q)[c] = rounded<O>(live[q] ? scale * to_float(from(q)[c]) : 0.0f);
     }
 }
 
@@ -69,18 +107,26 @@ bool starts_at(const void* base, long long stride, int bytes, int values) {
     return ((uintptr_t)base & (uintptr_t)(bytes * values - 1)) == 0 && stride % values == 0;
 }
 
+template <typename T, typename O, typename K, int N, bool WIDE>
+int lookup_by(const fmb_embedding_t& a, cudaStream_t stream) {
+    const int packs = std::max(1, a.width / N);
+    int lanes = 1;
+    while (lanes < 32 && lanes < packs) lanes *= 2;
+    // rows at a time: as many as give a lane four packs, where that leaves work for every SM (300,000 rows of 128 values: 82 us with one, 27 with four)
+    const int of_lane = ceil_div(packs, lanes), rows = of_lane > 2 || (long long)a.rows * lanes < 148 * 2048 ? 1 : of_lane > 1 ? 2 : 4;
+    const int grid = std::min(ceil_div((long long)ceil_div(a.rows, rows) * lanes, 256), 1 << 20);
+    const auto kernel = rows == 1 ? k_embedding<T, O, K, N, 1, WIDE> : rows == 2 ? k_embedding<T, O, K, N, 2, WIDE> : k_embedding<T, O, K, N, 4, WIDE>;
+    kernel<<<grid, 256, 0, stream>>>(a, lanes);
+    FMB_LAUNCH_CHECK();
+    return FMB_OK;
+}
+
+// packs of 16 bytes of the larger type where rows start at multiples of them, of four values where they start at those
 template <typename T, typename O, typename K>
 int lookup(const fmb_embedding_t& a, cudaStream_t stream) {
     constexpr int kPack = sizeof(T) == 4 || sizeof(O) == 4 ? 4 : 8;
-    const bool wide = starts_at(a.source, a.source_stride, sizeof(T), kPack) && starts_at(a.out, a.out_stride, sizeof(O), kPack);
-    const int packs = wide ? std::max(1, a.width / kPack) : a.width;
-    int lanes = 1;
-    while (lanes < 32 && lanes < packs) lanes *= 2;
-    const int grid = std::min(ceil_div((long long)a.rows * lanes, 256), 1 << 20);
-    if (wide) k_embedding<T, O, K, kPack><<<grid, 256, 0, stream>>>(a, lanes);
-    else k_embedding<T, O, K, 1><<<grid, 256, 0, stream>>>(a, lanes);
-    FMB_LAUNCH_CHECK();
-    return FMB_OK;
+    auto by = [&](int n) { return starts_at(a.source, a.source_stride, sizeof(T), n) && starts_at(a.out, a.out_stride, sizeof(O), n); };
+    return by(kPack) ? lookup_by<T, O, K, kPack, true>(a, stream) : by(4) ? lookup_by<T, O, K, 4, true>(a, stream) : lookup_by<T, O, K, 8, false>(a, stream);
 }
 
 template <typename T, typename O>

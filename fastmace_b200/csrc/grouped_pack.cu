@@ -118,7 +118,7 @@ __device__ __forceinline__ uint4 held_eight(const uint8_t* __restrict__ codes, c
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 two = held::two_values(v[i / 2] >> (16 * (i % 2)));
-        out[i] = held::two_of<T>(two.x * unit, two.y * unit);
+        out[i] = eight::two_of<T>(two.x * unit, two.y * unit);
     }
     return make_uint4(out[0], out[1], out[2], out[3]);
 }

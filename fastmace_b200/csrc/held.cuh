@@ -7,7 +7,7 @@
 // not finite is held as NaN, and does not count for the unit.
 #pragma once
 
-#include "grouped.cuh"
+#include "eight.cuh"
 
 #include <cuda_fp8.h>
 
@@ -22,28 +22,12 @@ __host__ __device__ __forceinline__ constexpr int blocks_of(int columns) { retur
 template <typename T> struct Units { static constexpr int kLowest = -117, kHighest = 120; };
 template <> struct Units<__half> { static constexpr int kLowest = -15, kHighest = 8; };
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-template <typename T> __device__ __forceinline__ T rounded(float x) { return grp::from_float<T>(x); }
-template <> __device__ __forceinline__ float rounded<float>(float x) { return x; }
-
 // 2^(byte - 127) for bytes from 1 to 254
 __device__ __forceinline__ float unit_of(int byte) { return __uint_as_float((uint32_t)byte << 23); }
 
 // two codes, the first in the lower byte
 __device__ __forceinline__ float2 two_values(uint32_t codes) {
     return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)codes, __NV_E4M3)));
-}
-
-template <typename T> __device__ __forceinline__ uint32_t two_of(float x, float y);
-template <> __device__ __forceinline__ uint32_t two_of<__nv_bfloat16>(float x, float y) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <> __device__ __forceinline__ uint32_t two_of<__half>(float x, float y) {
-    const __half2 v = __floats2half2_rn(x, y);
-    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
 // rows read back, [rows][columns], row_stride apart (checkpoints.cu)
