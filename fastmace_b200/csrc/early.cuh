@@ -6,8 +6,14 @@
 
 namespace fmb {
 
-// ahead of the first read or write of global memory
-__device__ __forceinline__ void kernels_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Ahead of the first read or write of global memory. What is read of what the kernels before have written is read by way of pointers that have
+// been named here: the compiler takes a load of what a kernel never writes (__ldg, const __restrict__) for one that may come at any time, and
+// could move it before the wait, but not before its address is there.
+template <typename... Pointers>
+__device__ __forceinline__ void kernels_before(Pointers&... pointers) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    ((void)([&] { asm volatile("" : "+l"(pointers) : : "memory"); }()), ...);
+}
 // once every CTA of a launch has said so, the next one's may come
 __device__ __forceinline__ void let_next_come() { asm volatile("griddepcontrol.launch_dependents;"); }
 

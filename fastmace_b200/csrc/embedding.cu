@@ -288,7 +288,7 @@ template <typename T, bool VEC, int N>
 __global__ void __launch_bounds__(kThreads, 3)
 k_embedding_sums(Sums p) {
     let_next_come();
-    kernels_before();
+    kernels_before(p.a.tokens, p.a.order, p.a.source);
     if (blockIdx.x < p.zero_ctas) {              // the first, since their searches take long and their writes little
         write_zeros(p);
         return;
@@ -408,7 +408,7 @@ k_embedding_join(Sums p) {
     constexpr int kThreads = 32 * kJoinWarps;
     __shared__ int list[kJoinList], count;
     __shared__ float4 sums[kJoinWarps][32];
-    kernels_before();
+    kernels_before(p.a.tokens, p.a.scratch);
     const fmb_embedding_t& a = p.a;
     const int32_t* const keys = (const int32_t*)a.tokens;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;

@@ -8,7 +8,8 @@
 // a counter. A unit of the second kind waits for the first ones of its expert, one of y for the second ones of its columns; those were
 // handed out before it, so they are done or under way and the wait ends, however few CTAs run at a time.
 //
-// A unit is [64 columns] x [8 or 16 rows] over the whole depth, which the eight warps of a CTA share. Each warp has a ring of stages in
+// A unit is 64 columns and 8 or 16 rows over the whole depth, which the eight warps of a CTA share; by sizes (shape_of) several groups of 64
+// columns with fewer warps each, or a part of the depth. Each warp has a ring of stages in
 // shared memory that asynchronous copies fill, without a barrier between warps; the ring does not run dry between units, since the first
 // stages of the next one are asked for before the results of the last are taken out and before a wait for what they multiply. Two
 // permutes make pairs along the depth of two rows of the matrix. Columns of the matrix are the MMA's rows, tokens its columns, of which it
@@ -31,14 +32,13 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 constexpr int kUnit = 64;                        // columns of a unit
-constexpr long long kSpins = 1ll << 22;          // polls of a wait, each of 32 ns or more, before a CTA gives up
+constexpr int kSpins = 1 << 22;                  // polls of a wait, each of 20 ns or more, before a CTA gives up
 
 __device__ __forceinline__ float to_float(float x) { return x; }
 __device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 template <typename T> __device__ __forceinline__ T rounded(float x) { return grp::from_float<T>(x); }
 template <> __device__ __forceinline__ float rounded<float>(float x) { return x; }
-template <typename T> __device__ __forceinline__ T zero() { return T(0.0f); }
 
 // --------------------------------------------------------------------------------------------------------------- route
 
@@ -291,7 +291,7 @@ struct Layer {
     long long h_stride, part_stride;             // floats of a row: the inner width, or the width, filled up to whole units
     int32_t* control;                            // next unit; of each active expert the blocks that are done; of each block of the second matrix the
                                                  // units; of each block of an active expert's first the units, where they share the depth
-    int32_t* lists;                              // number of active experts, total of pairs; active[], first[], pair[]
+    int32_t* lists;                              // number of active experts; active[experts], first[experts + 1], pair[]
     float* h;                                    // [tokens * top]
     float* parts;                                // [down.splits][tokens * top]
     float* up_parts;                             // [up.splits][tokens * top] of h_stride gates and as many they multiply
@@ -781,8 +781,8 @@ __device__ __forceinline__ void combine(const Layer& p, int group, int tokens, F
 #pragma unroll
     for (int j = 0; j < FMB_MAX_TOP; ++j) {
         const bool there = exists && j < a.top;
-        const int e = there ? __ldg(a.chosen + t * a.top + j) : -1;
-        w[j] = there ? __ldg(a.weights + t * a.top + j) : 0.0f;
+        const int e = there ? __ldcg(a.chosen + t * a.top + j) : -1;
+        w[j] = there ? __ldcg(a.weights + t * a.top + j) : 0.0f;
         if (e >= 0 && e < a.experts) live |= 1u << j;
     }
     await();
@@ -823,20 +823,20 @@ __device__ __forceinline__ void combine(const Layer& p, int group, int tokens, F
 // of 8 bytes.
 template <typename T>
 __global__ void __launch_bounds__(1024)
-k_list_pairs(const __grid_constant__ Layer p, int control, void* packed) {
+k_list_pairs(Layer p, int control, void* packed) {
     const fmb_experts_t& a = p.a;
     let_next_come();
-    kernels_before();                            // what the rows and the choices come from
+    kernels_before(p.a.x, p.a.chosen);           // what the rows and the choices come from
     if (blockIdx.x > 0) {
         const T* const from = (const T*)a.x + (blockIdx.x - 1) * a.x_stride;
         T* const to = (T*)packed + (blockIdx.x - 1) * p.x_stride;
-        for (int c = threadIdx.x; c < p.x_stride; c += 1024) to[c] = c < a.width ? from[c] : zero<T>();
+        for (int c = threadIdx.x; c < p.x_stride; c += 1024) to[c] = c < a.width ? from[c] : T(0.0f);
         return;
     }
     __shared__ int start[FMB_MAX_GROUPS];
     __shared__ int warp_total[2][32];
     const int experts = a.experts, pairs = a.tokens * a.top, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, e = threadIdx.x;
-    int32_t* const active = p.lists + 2;
+    int32_t* const active = p.lists + 1;
     int32_t* const first = active + experts;
     int32_t* const pair = first + experts + 1;
     for (int i = threadIdx.x; i < control; i += 1024) p.control[i] = 0;
@@ -872,7 +872,6 @@ k_list_pairs(const __grid_constant__ Layer p, int control, void* packed) {
     if (e == 1023) {
         first[place + (count > 0)] = begin + count;
         p.lists[0] = place + (count > 0);
-        p.lists[1] = begin + count;
     }
     __syncthreads();
 #pragma unroll
@@ -886,30 +885,30 @@ k_experts(const __grid_constant__ Layer p) {
     extern __shared__ __align__(16) uint8_t smem[];
     Smem<T, WIDE>& s = *reinterpret_cast<Smem<T, WIDE>*>(smem);
     const fmb_experts_t& a = p.a;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int32_t* const next = p.control;
     int32_t* const done = p.control + 1;
     int32_t* const columns = done + a.experts;
-    kernels_before();                            // for the lists
+    const int32_t* lists = p.lists;
+    kernels_before(lists);
     if (threadIdx.x == 0) {
         s.ticket = atomicAdd(next, 1);
         s.gave_up = 0;
     }
     // (the lists' places, whether in use or not: their numbers need not be waited for)
-    const int actives = __ldg(p.lists), most = min(a.experts, a.tokens * a.top);
+    const int actives = __ldg(lists), most = min(a.experts, a.tokens * a.top);
     for (int i = threadIdx.x; i <= most; i += kThreads) {
-        if (i < most) s.active[i] = (uint16_t)__ldg(p.lists + 2 + i);
-        s.first[i] = (uint16_t)__ldg(p.lists + 2 + a.experts + i);
+        if (i < most) s.active[i] = (uint16_t)__ldg(lists + 1 + i);
+        s.first[i] = (uint16_t)__ldg(lists + 1 + a.experts + i);
     }
     for (int i = threadIdx.x; i < a.tokens * a.top; i += kThreads) {
-        const uint32_t pair = (uint32_t)__ldg(p.lists + 3 + 2 * a.experts + i);
+        const uint32_t pair = (uint32_t)__ldg(lists + 2 + 2 * a.experts + i);
         s.pair[i] = (uint16_t)pair;
         s.token[i] = (uint8_t)(pair / a.top);
     }
     __syncthreads();
     if (actives == 0) {                          // no expert is one
         for (long long i = blockIdx.x * (long long)kThreads + threadIdx.x; i < (long long)a.tokens * a.width; i += (long long)gridDim.x * kThreads)
-            ((T*)a.y)[i / a.width * a.y_stride + i % a.width] = zero<T>();
+            ((T*)a.y)[i / a.width * a.y_stride + i % a.width] = T(0.0f);
         return;
     }
     // three kinds of units, of which each waits for ones of the kind before: h, the parts of y, and y
@@ -920,7 +919,7 @@ k_experts(const __grid_constant__ Layer p) {
     // (2,048 warps that ask for the same eight counters hold up those that count)
     auto await = [&](const int32_t* counter, int value) {
         if (threadIdx.x == 0) {
-            long long spins = 0;
+            int spins = 0;
             while (load_relaxed(counter) < value && !s.gave_up)
                 if (++spins < kSpins) __nanosleep(20);
                 else s.gave_up = 1;
@@ -933,9 +932,9 @@ k_experts(const __grid_constant__ Layer p) {
     Unit u;
     Matrix m;
     Rows r;
-    Ring ring = {smem_at(s.ring[warp]), 0};
+    Ring ring = {smem_at(s.ring[threadIdx.x >> 5]), 0};
     bool ready = false, turning = false;         // ready: what the unit's rows are has been written
-    // the unit of the ticket, if it is one of a product, and its first stages
+    // the ticket's unit, if it is one of a product, and its first stages
     auto go_on = [&]() {
         if (ticket >= downs) return;
         u = unit_of(p, s, ticket, ups);
@@ -1027,7 +1026,6 @@ struct Sizes {
     long long h_stride, part_stride, x_stride;
 };
 
-// wide: whether the matrices' rows are whole pieces of 16 bytes (their stages are alike: the plan does not depend on it)
 Sizes sizes_of(const fmb_experts_t& a) {
     Sizes s;
     const long long pairs = (long long)a.tokens * a.top;
@@ -1035,7 +1033,7 @@ Sizes sizes_of(const fmb_experts_t& a) {
     s.up = shape_of(experts, a.inner, 32, a.width, stage);
     s.down = shape_of(experts, a.width, kUnit, a.inner, stage);
     s.control = up_to(1 + a.experts + s.down.blocks + (s.up.splits > 1 ? (long long)experts * s.up.blocks : 0), 64);
-    s.lists = up_to(3 + 2 * a.experts + pairs, 64);
+    s.lists = up_to(2 + 2 * a.experts + pairs, 64);
     s.h_stride = up_to(a.inner, 32);
     s.part_stride = up_to(a.width, kUnit);
     s.h = pairs * s.h_stride;

@@ -90,13 +90,13 @@ __device__ __forceinline__ int warps_before(int mine, int& all) {
 
 template <typename K, bool DIGIT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS)
-k_group_count(const K* __restrict__ keys, Digit d, long long rows, int groups, int32_t* __restrict__ table) {
+k_group_count(const K* keys, Digit d, long long rows, int groups, int32_t* __restrict__ table) {
     constexpr int kThreads = 32 * WARPS, kRowsPerCta = WARPS * kRowsPerWarp;
     __shared__ int counts[FMB_MAX_GROUPS + 1];
     const int width = groups + 1;
     if (DIGIT) {
         let_next_come();
-        kernels_before();
+        kernels_before(keys, d.from);
     }
     int g[kKeys];
     load_keys<K, DIGIT>(keys, d, (long long)blockIdx.x * kRowsPerCta + (threadIdx.x >> 5) * kRowsPerWarp, rows, groups, g);
@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(1024)
 k_group_scan(int32_t* __restrict__ table, int32_t* __restrict__ totals, int ctas, int width) {
     if (DIGIT) {
         let_next_come();
-        kernels_before();
+        kernels_before(table);
     }
     __shared__ int part[32][33];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = blockIdx.x * 32 + lane;
@@ -174,8 +174,8 @@ constexpr int place_smem(int width, int warps) { return (warps * place_stride(wi
 // that the rows of a group leave in one run.
 template <typename K, bool ALONE, bool DIGIT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, ALONE ? 1 : 64 / WARPS)
-k_group_place(const K* __restrict__ keys, Digit d, long long rows, int groups, int bits, const int32_t* __restrict__ table,
-              const int32_t* __restrict__ totals, int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
+k_group_place(const K* keys, Digit d, long long rows, int groups, int bits, const int32_t* table, const int32_t* totals,
+              int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
     constexpr int kThreads = 32 * WARPS, kRowsPerCta = WARPS * kRowsPerWarp;
     extern __shared__ int counts[];                       // [WARPS][stride], [groups + 1] starts of the CTA, [groups + 1] of all, rows
     const int width = groups + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stride = place_stride(width);
@@ -185,7 +185,7 @@ k_group_place(const K* __restrict__ keys, Digit d, long long rows, int groups, i
     const long long first = (long long)blockIdx.x * kRowsPerCta;
     if (DIGIT) {
         let_next_come();
-        kernels_before();
+        kernels_before(keys, d.from, table, totals);
     }
     int g[kKeys], rank[kKeys];
     load_keys<K, DIGIT>(keys, d, first + warp * kRowsPerWarp, rows, groups, g);
@@ -319,10 +319,10 @@ constexpr int kFewRows = kRowsPerCta, kRankRows = 32;
 
 template <typename K>
 __global__ void __launch_bounds__(8 * kRankRows)
-k_rank_tokens(const K* __restrict__ tokens, int rows, int vocabulary, int32_t* __restrict__ order, int32_t* __restrict__ keys) {
+k_rank_tokens(const K* tokens, int rows, int vocabulary, int32_t* __restrict__ order, int32_t* __restrict__ keys) {
     __shared__ int4 all[kFewRows / 4];
     let_next_come();
-    kernels_before();
+    kernels_before(tokens);
     int* const key = reinterpret_cast<int*>(all);
     const int quads = (rows + 3) / 4;
 #pragma unroll 4

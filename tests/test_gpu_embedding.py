@@ -93,6 +93,29 @@ def test_rows_and_gradient_against_float64(shape, dtype):
     assert torch.equal(more[count == 0], base[count == 0])
 
 
+@pytest.mark.parametrize("vocabulary", [1000, 100_003])
+def test_millions_of_rows(vocabulary):
+    """Sorting CTAs of 32 warps, and a run over more chunks than are looked at together."""
+    from fastmace_b200 import embedding
+    rows, width = 2_600_000, 8
+    g = torch.Generator(device="cuda").manual_seed(vocabulary)
+    t = torch.randint(0, vocabulary, (rows,), generator=g, device="cuda")
+    t = torch.where(torch.rand(rows, generator=g, device="cuda") < 0.9, 7, t)
+    order = embedding.sort_tokens(t, vocabulary)
+    keys, at = torch.sort(t, stable=True)
+    assert torch.equal(order.keys, keys.to(torch.int32)) and torch.equal(order.rows, at.to(torch.int32))
+    dy = torch.randn(rows, width, generator=g, device="cuda")
+    grad = embedding.embedding_gradient(dy, order, vocabulary, 0.5)
+    total = torch.cat([torch.zeros(1, width, dtype=torch.float64, device="cuda"), dy[at].double().cumsum(0)])
+    edge = torch.searchsorted(keys, torch.arange(vocabulary + 1, device="cuda"))
+    ref = (total[edge[1:]] - total[edge[:-1]]) * 0.5
+    size = torch.cat([torch.zeros(1, width, dtype=torch.float64, device="cuda"), dy[at].double().abs().cumsum(0)])
+    size = (size[edge[1:]] - size[edge[:-1]]) * 0.5
+    assert bool(((grad.double() - ref).abs() <= ((edge[1:] - edge[:-1])[:, None] + 8) * 2.0 ** -24 * size + 1e-9).all())
+    # sums of at most 256 rows a warp, of 8 of those, and of those: the error of the long run is that of far fewer additions in a row
+    assert float((grad[7].double() - ref[7]).norm() / size[7].norm()) < 400 * 2.0 ** -24
+
+
 def test_given_rows_keep_what_no_token_writes():
     from fastmace_b200 import embedding
     t = torch.tensor([2, -1, 0, 3, 2 ** 40], device="cuda")

@@ -168,3 +168,76 @@ def test_a_captured_step_with_adamw():
         assert torch.equal(eager.master[k], captured.master[k]) and torch.equal(eager.copies[k], captured.copies[k])
         assert not torch.equal(captured.master[k], Model(BF16, 4).master[k])
     grouped.check_status()
+
+
+def test_launches_that_come_early_read_what_was_written_before():
+    """Calls one behind the other, each on what the kernels right before it have written, without a wait in between."""
+    from fastmace_b200 import embedding, experts
+    g = torch.Generator(device="cuda").manual_seed(7)
+    model = Model(BF16, 6)
+    rounds = [(torch.randint(-3, V, (9000,), generator=g, device="cuda"), torch.randn(9000, 40, generator=g, device="cuda"),
+               torch.randn(30, D, generator=g, device="cuda").to(BF16)) for _ in range(12)]
+    big = torch.randn(2048, 2048, device="cuda")
+
+    def one(tokens, dy, x, wait):
+        busy = big @ big                                    # so that the launches behind it queue up
+        t, d, rows = tokens.clone(), dy * 2.0, x.roll(1, 0).clone()
+        if wait:
+            torch.cuda.synchronize()
+        grad = embedding.embedding_gradient(d, embedding.sort_tokens(t, V), V)
+        few = embedding.embedding_gradient(d[:500], embedding.sort_tokens(t[:500], V), V)
+        routes = experts.route_rows(rows, model.router, TOP)
+        y = experts.expert_layer(rows, model.copies["up"], model.copies["down"], routes)
+        t.fill_(0), d.zero_(), rows.zero_()                 # what comes behind does not come too early
+        return grad, few, y, routes.weights, busy
+
+    want = [one(*r, True) for r in rounds]
+    torch.cuda.synchronize()
+    got = [one(*r, False) for r in rounds]
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a[:4], b[:4]))
+
+
+def test_captured_behind_copies_and_other_streams():
+    """In a graph the launch before is not always a kernel, nor is there always just one."""
+    from fastmace_b200 import embedding, experts, grouped
+    model = Model(F32, 8)
+    tokens, x = torch.empty_like(model.tokens), torch.empty(20, D, device="cuda")
+    table = torch.empty_like(model.master["table"])
+    g = torch.Generator(device="cuda").manual_seed(9)
+    sources = [(torch.randint(-3, V, (T,), generator=g, device="cuda"), torch.randn(20, D, generator=g, device="cuda"), torch.randn(V, D, generator=g, device="cuda"))
+               for _ in range(3)]
+    now = [t.clone() for t in sources[0]]
+    dy = model.target
+
+    def work(other):
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            x.copy_(now[1])
+            routes = experts.route_rows(x, model.router, TOP)
+        tokens.copy_(now[0])                                # a copy of memory right before
+        order = embedding.sort_tokens(tokens, V)
+        table.copy_(now[2])
+        torch.cuda.current_stream().wait_stream(other)
+        y = experts.expert_layer(x, model.copies["up"], model.copies["down"], routes)
+        return embedding.embedding(tokens, table, 2.0), embedding.embedding_gradient(dy, order, V), y
+
+    other, side = torch.cuda.Stream(), torch.cuda.Stream()
+    work(other)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            got = work(other)
+    for source in sources:
+        for a, b in zip(now, source):
+            a.copy_(b)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        kept = [t.clone() for t in got]
+        want = work(other)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(kept, want))
+    grouped.check_status()
