@@ -233,6 +233,13 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
 }
 
+// The same for a weight, of which there are many: in integers, since conversions run at a quarter of the rate (6 tokens, 50 experts of 1,024 x 1,024:
+// 74 us by conversions); the rest of an infinity is NaN. What lies below a tf32's bits is cut off: less than 2^-21 |x|.
+__device__ __forceinline__ void split_weight(uint32_t x, uint32_t& hi, uint32_t& lo) {
+    hi = (x + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(__uint_as_float(x) - __uint_as_float(hi)) & 0xffffe000u;
+}
+
 // What a warp brings at a time, a stage: kDepth rows of the unit's 64 columns and as much of its rows of x or h. For the product a lane has
 // kRows neighbouring rows of the depth and eight columns, which are kPieces times 16 bytes, and of block n of the unit's rows one row, kRows
 // values of it. Stages lie in shared memory, a ring for each warp, so that no registers wait for them. Copies go along the rows of the
@@ -532,22 +539,24 @@ __device__ __forceinline__ void multiply(float (&acc)[4][2][4], const Matrix& m,
         }
     } else {
         // float32 values as pairs of tf32, float16 weights as they are
+        auto add = [&](auto blocks) {
+            constexpr int NB = decltype(blocks)::value;
+            uint32_t hi[NB][S::kRows], lo[NB][S::kRows];
 #pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            if (n && !two_blocks) break;
-            float b[S::kRows];
-            if constexpr (S::kRows == 4) {
-                const uint4 v = load_16(rows + n * 512);
-                b[0] = __uint_as_float(v.x); b[1] = __uint_as_float(v.y); b[2] = __uint_as_float(v.z); b[3] = __uint_as_float(v.w);
-            } else {
-                const uint2 v = load_8(rows + n * 512);
-                b[0] = __uint_as_float(v.x); b[1] = __uint_as_float(v.y);
+            for (int n = 0; n < NB; ++n) {
+                float b[S::kRows];
+                if constexpr (S::kRows == 4) {
+                    const uint4 v = load_16(rows + n * 512);
+                    b[0] = __uint_as_float(v.x); b[1] = __uint_as_float(v.y); b[2] = __uint_as_float(v.z); b[3] = __uint_as_float(v.w);
+                } else {
+                    const uint2 v = load_8(rows + n * 512);
+                    b[0] = __uint_as_float(v.x); b[1] = __uint_as_float(v.y);
+                }
+#pragma unroll
+                for (int q = 0; q < S::kRows; ++q) split_tf32(b[q], hi[n][q], lo[n][q]);
             }
 #pragma unroll
-            for (int s = 0; s < S::kRows / 2; ++s) {
-                uint32_t hi[2], lo[2];
-#pragma unroll
-                for (int q = 0; q < 2; ++q) split_tf32(b[2 * s + q], hi[q], lo[q]);
+            for (int s = 0; s < S::kRows / 2; ++s)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t a[4], rest[4];
@@ -558,26 +567,30 @@ __device__ __forceinline__ void multiply(float (&acc)[4][2][4], const Matrix& m,
                             a[2 * q] = __float_as_uint(two.x);
                             a[2 * q + 1] = __float_as_uint(two.y);
                         } else {
-                            split_tf32(__uint_as_float(w[2 * s + q][2 * i]), a[2 * q], rest[2 * q]);
-                            split_tf32(__uint_as_float(w[2 * s + q][2 * i + 1]), a[2 * q + 1], rest[2 * q + 1]);
+                            split_weight(w[2 * s + q][2 * i], a[2 * q], rest[2 * q]);
+                            split_weight(w[2 * s + q][2 * i + 1], a[2 * q + 1], rest[2 * q + 1]);
                         }
                     }
-                    if constexpr (sizeof(T) == 4) {
-                        // The tensor core cuts its sums off, which adds up along the depth (float32 results were 8e-6 off at a depth of
-                        // 4,096): each stage's sum begins at zero and is added with rounding.
-                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma_tf32(sum, a, lo[0], lo[1]);
-                        mma_tf32(sum, rest, hi[0], hi[1]);
-                        mma_tf32(sum, a, hi[0], hi[1]);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) acc[i][n][q] += sum[q];
-                    } else {
-                        mma_tf32(acc[i][n], a, lo[0], lo[1]);
-                        mma_tf32(acc[i][n], a, hi[0], hi[1]);
+                    for (int n = 0; n < NB; ++n) {
+                        if constexpr (sizeof(T) == 4) {
+                            // The tensor core cuts its sums off, which adds up along the depth (float32 results were 8e-6 off at a depth
+                            // of 4,096): each stage's sum begins at zero and is added with rounding.
+                            float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma_tf32(sum, a, lo[n][2 * s], lo[n][2 * s + 1]);
+                            mma_tf32(sum, rest, hi[n][2 * s], hi[n][2 * s + 1]);
+                            mma_tf32(sum, a, hi[n][2 * s], hi[n][2 * s + 1]);
+#pragma unroll
+                            for (int q = 0; q < 4; ++q) acc[i][n][q] += sum[q];
+                        } else {
+                            mma_tf32(acc[i][n], a, lo[n][2 * s], lo[n][2 * s + 1]);
+                            mma_tf32(acc[i][n], a, hi[n][2 * s], hi[n][2 * s + 1]);
+                        }
                     }
                 }
-            }
-        }
+        };
+        if (two_blocks) add(std::integral_constant<int, 2>());
+        else add(std::integral_constant<int, 1>());
     }
 }
 
