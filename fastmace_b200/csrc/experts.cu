@@ -832,7 +832,7 @@ __device__ __forceinline__ void combine(const Layer& p, int group, int tokens, F
 }
 
 // Which pairs belong to which expert, and which experts have any; the counters of the next launch become zero. Pairs of one expert stand in
-// any order: their results do not depend on it. The CTAs behind the first copy rows of x, where those do not begin at multiples
+// any order: their results do not depend on it. A thread for every expert and every two pairs. The CTAs behind the first copy rows of x, where those do not begin at multiples
 // of 8 bytes.
 template <typename T>
 __global__ void __launch_bounds__(1024)
@@ -843,7 +843,7 @@ k_list_pairs(Layer p, int control, void* packed) {
     if (blockIdx.x > 0) {
         const T* const from = (const T*)a.x + (blockIdx.x - 1) * a.x_stride;
         T* const to = (T*)packed + (blockIdx.x - 1) * p.x_stride;
-        for (int c = threadIdx.x; c < p.x_stride; c += 1024) to[c] = c < a.width ? from[c] : T(0.0f);
+        for (int c = threadIdx.x; c < p.x_stride; c += blockDim.x) to[c] = c < a.width ? from[c] : T(0.0f);
         return;
     }
     __shared__ int start[FMB_MAX_GROUPS];
@@ -852,13 +852,13 @@ k_list_pairs(Layer p, int control, void* packed) {
     int32_t* const active = p.lists + 1;
     int32_t* const first = active + experts;
     int32_t* const pair = first + experts + 1;
-    for (int i = threadIdx.x; i < control; i += 1024) p.control[i] = 0;
+    for (int i = threadIdx.x; i < control; i += blockDim.x) p.control[i] = 0;
     start[e] = 0;
     __syncthreads();
-    int chosen[kMaxPairs / 1024];
+    int chosen[2];
 #pragma unroll
-    for (int q = 0; q < kMaxPairs / 1024; ++q) {
-        const int i = threadIdx.x + 1024 * q;
+    for (int q = 0; q < 2; ++q) {
+        const int i = threadIdx.x + blockDim.x * q;
         chosen[q] = i < pairs ? __ldg(a.chosen + i) : -1;
         if (chosen[q] >= experts) chosen[q] = -1;
         if (chosen[q] >= 0) atomicAdd(start + chosen[q], 1);
@@ -882,14 +882,14 @@ k_list_pairs(Layer p, int control, void* packed) {
         active[place] = e;
         first[place] = begin;
     }
-    if (e == 1023) {
+    if (e == blockDim.x - 1) {
         first[place + (count > 0)] = begin + count;
         p.lists[0] = place + (count > 0);
     }
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < kMaxPairs / 1024; ++q)
-        if (chosen[q] >= 0) pair[atomicAdd(start + chosen[q], 1)] = threadIdx.x + 1024 * q;
+    for (int q = 0; q < 2; ++q)
+        if (chosen[q] >= 0) pair[atomicAdd(start + chosen[q], 1)] = threadIdx.x + blockDim.x * q;
 }
 
 template <typename T, bool WIDE>
@@ -1084,7 +1084,9 @@ int layer(const fmb_experts_t& a, cudaStream_t stream) {
     const bool pack = !begin_at(a.x, a.x_stride, a.tokens, b, 8);
     p.x = pack ? packed : const_cast<void*>(a.x);
     p.x_stride = pack ? size.x_stride : a.x_stride;
-    FMB_CUDA_CHECK(launch_early(k_list_pairs<T>, pack ? a.tokens + 1 : 1, 1024, 0, stream, p, (int)size.control, packed));
+    static_assert(kMaxPairs <= 2 * 1024 && FMB_MAX_GROUPS <= 1024, "a thread for every expert and every two pairs");
+    const int list_threads = (int)up_to(std::max({a.experts, (a.tokens * a.top + 1) / 2, pack ? 256 : 1}), 32);
+    FMB_CUDA_CHECK(launch_early(k_list_pairs<T>, pack ? a.tokens + 1 : 1, list_threads, 0, stream, p, (int)size.control, packed));
     FMB_LAUNCH_CHECK();
     // whole pieces of 16 bytes, at multiples of 16
     auto pieces = [&](const void* base, long long row, long long group, int rows, int columns) {
