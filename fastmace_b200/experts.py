@@ -38,9 +38,10 @@ class Routes(NamedTuple):
     weights: torch.Tensor
 
 
-def _kind(what: str, *operands: torch.Tensor) -> int:
-    kind = TYPES.get(operands[0].dtype)
-    if kind is None or any(t.dtype != operands[0].dtype for t in operands):
+def _kind(what: str, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor) -> int:
+    dtype = x.dtype
+    kind = TYPES.get(dtype)
+    if kind is None or a.dtype != dtype or b.dtype != dtype:
         raise ValueError(f"{what}: the operands must have the same type, float32, bfloat16 or float16")
     return kind
 
@@ -51,15 +52,16 @@ def route_rows(x: torch.Tensor, router: torch.Tensor, top: int, normalise: bool 
     what = "route_rows"
     tokens, width, stride = _matrix(what, "x", x)
     _, count, router_stride = _matrix(what, "router", router, rows=width)
-    kind = _kind(what, x, router)
+    kind = _kind(what, x, router, router)
     if count > MAX_GROUPS:
         raise ValueError(f"{what}: more than {MAX_GROUPS} experts")
-    if not 1 <= int(top) <= min(MAX_TOP, count):
+    top = int(top)
+    if not 1 <= top <= MAX_TOP or top > count:
         raise ValueError(f"{what}: 1 to {min(MAX_TOP, count)} choices")
-    index = _on_device(what, x, router)
-    routes = Routes(_empty(tokens, int(top), torch.int32, x.device), _empty(tokens, int(top), torch.float32, x.device))
+    index, device = _on_device(what, x, router), x.device
+    routes = Routes(_empty(tokens, top, torch.int32, device), _empty(tokens, top, torch.float32, device))
     if tokens:
-        a = _lib.RouteStruct(kind, tokens, width, count, int(top), bool(normalise), x.data_ptr(), router.data_ptr(),
+        a = _lib.RouteStruct(kind, tokens, width, count, top, bool(normalise), x.data_ptr(), router.data_ptr(),
                              routes.experts.data_ptr(), routes.weights.data_ptr(), stride, router_stride)
         _lib.check(_launch(index, _lib.load().fmb_route_rows, ctypes.byref(a)), "fmb_route_rows")
     return routes
@@ -78,8 +80,9 @@ def expert_layer(x: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, rout
     chosen, weights = routes
     if tokens > MAX_TOKENS:
         raise ValueError(f"{what}: {tokens} tokens, of {MAX_TOKENS} at most: grouped_linear is for more")
-    if chosen.dtype != torch.int32 or weights.dtype != torch.float32 or chosen.dim() != 2 or chosen.shape != weights.shape or \
-            chosen.shape[0] != tokens or not 1 <= chosen.shape[1] <= MAX_TOP or not chosen.is_contiguous() or not weights.is_contiguous():
+    shape = chosen.shape
+    if chosen.dtype != torch.int32 or weights.dtype != torch.float32 or len(shape) != 2 or shape != weights.shape or \
+            shape[0] != tokens or not 1 <= shape[1] <= MAX_TOP or not chosen.is_contiguous() or not weights.is_contiguous():
         raise ValueError(f"{what}: routes must be as route_rows returns them, for {tokens} tokens and 1 to {MAX_TOP} choices")
     index = _on_device(what, x, w_up, w_down, chosen, weights)
     given = out is not None
@@ -94,7 +97,7 @@ def expert_layer(x: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor, rout
         out, out_stride = _empty(tokens, width, x.dtype, x.device), width
     if tokens:
         lib = _lib.load()
-        a = _lib.ExpertsStruct(kind, tokens, count, chosen.shape[1], width, inner, x.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
+        a = _lib.ExpertsStruct(kind, tokens, count, shape[1], width, inner, x.data_ptr(), w_up.data_ptr(), w_down.data_ptr(),
                                chosen.data_ptr(), weights.data_ptr(), out.data_ptr(), stride, out_stride, up_group, up_row, down_group,
                                down_row, None, _status_pointer(index))
         call = ctypes.byref(a)
