@@ -40,6 +40,31 @@ __device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
 template <typename T> __device__ __forceinline__ T rounded(float x) { return grp::from_float<T>(x); }
 template <> __device__ __forceinline__ float rounded<float>(float x) { return x; }
 
+__device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+// 16 or 8 bytes, of which the first `bytes` are read and the others zero
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copy_8(uint32_t to, const void* from, int bytes) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+// whole ones
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copy_8(uint32_t to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory"); }
+__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // --------------------------------------------------------------------------------------------------------------- route
 
 
@@ -84,7 +109,7 @@ __device__ __forceinline__ uint32_t ordered(float x) {
 
 // CLUSTER CTAs for TOKENS tokens: each takes its share of the depth, threads by packs of eight experts and rows of R, which all tokens share; then
 // CTA c the choices of tokens c, c + CLUSTER, ... A cluster of eight for a token each where there are few (1 token of 2,048, 64 experts: 5.2 us),
-// for two to eight tokens where they would read much of R one by one, and a CTA alone beyond 128 tokens.
+// for two to eight tokens where they would read much of R one by one, and a CTA alone beyond 128 tokens of float32.
 template <typename T, int TOKENS, int CLUSTER>
 __global__ void __launch_bounds__(kThreads)
 k_route(fmb_route_t a, int wide, int rows) {
@@ -209,17 +234,220 @@ k_route(fmb_route_t a, int wide, int rows) {
     if (CLUSTER > 1) meet();                     // shared memory lives until it has been read
 }
 
+// Many tokens of 16-bit types, by matrix instructions: a CTA has 16 MT tokens and all experts, COLUMNS of them at a time, its eight warps MT blocks of
+// 16 tokens by 8 / MT shares of the columns. A ring of asynchronous copies brings 64 of the depth at a time; their sums start at zero and are added
+// to those before with rounding, since the tensor core cuts its sums off. Where blocks of tokens are few, the CTAs of a cluster share the depth,
+// and each then has every so many of the tokens. A warp chooses for up to four tokens side by side: rounds of the largest of all, which a lane holds a 32nd
+// of. 16,384 tokens of 2,048 and 64 experts: 28 us with one choice, 34 with eight (10 for the bytes; instructions issue in half of the cycles).
+constexpr int kRouteDepth = 64, kMaxCluster = 8;
+
+template <int COLUMNS> constexpr int kRouteStages = COLUMNS == 256 ? 3 : 4;
+template <int MT, int COLUMNS> constexpr int kRouteRing = kRouteStages<COLUMNS> * kRouteDepth * (16 * MT + COLUMNS) * 2;
+__host__ __device__ constexpr int route_row(int experts) { return (experts + 31) / 32 * 32 + 8; }   // floats of a token's logits, for the banks
+
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void load_turned(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+// eight values to shared memory, of which the first `live` are read and the others zero
+template <typename T>
+__device__ __forceinline__ void bring_eight(uint32_t to, const T* from, int live, bool wide) {
+    if (wide) {
+        copy_16(to, from, 2 * min(live, 8));
+    } else {
+        const Eight<T> in = load_eight(from, live, false);
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(in.v[0]), "r"(in.v[1]), "r"(in.v[2]), "r"(in.v[3]) : "memory");
+    }
+}
+
+template <typename T, int MT, int COLUMNS, int KEYS>
+__global__ void __launch_bounds__(kThreads)
+k_route_many(fmb_route_t a, int x_wide, int r_wide, int cluster) {
+    constexpr int kTokens = 16 * MT, kShare = COLUMNS * MT / kWarps, kBlocks = kShare / 16, kRing = kRouteStages<COLUMNS>;
+    constexpr int kStageBytes = kRouteDepth * (kTokens + COLUMNS) * 2, kXBytes = kTokens * kRouteDepth * 2, kRowPieces = COLUMNS / 8;
+    constexpr bool kOver = KEYS * 32 <= COLUMNS; // the logits take the ring's place
+    extern __shared__ __align__(128) uint8_t shared[];
+    let_next_come();
+    const int rank = blockIdx.x % cluster, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const long long first_token = (long long)(blockIdx.x / cluster) * kTokens;
+    const int tokens = (int)min((long long)kTokens, a.tokens - first_token), stages = (a.width + kRouteDepth - 1) / kRouteDepth;
+    const int begin = (int)((long long)stages * rank / cluster), end = (int)((long long)stages * (rank + 1) / cluster);
+    const T* const x = (const T*)a.x + first_token * a.x_stride;
+    const T* const r = (const T*)a.router;
+    float* const logits = reinterpret_cast<float*>(shared + (kOver ? 0 : kRouteRing<MT, COLUMNS>));
+    const int row_floats = route_row(a.experts);
+    const uint32_t ring = smem_at(shared);
+    const int block = warp % MT, share = warp / MT * kShare;      // of the warp: tokens, columns of a pass
+    const int at_row = lane & 15, at_piece = lane >> 4;
+
+    // of the thread: one piece of every 32nd row of x, and one of every kRowStep-th of R
+    constexpr int kRowStep = kThreads / kRowPieces;
+    const int x_row = threadIdx.x / 8, x_piece = threadIdx.x % 8, r_row = threadIdx.x / kRowPieces, r_piece = threadIdx.x % kRowPieces;
+    const uint32_t x_to = x_row * 128 + (x_piece ^ (x_row & 7)) * 16, r_to = kXBytes + r_row * (2 * COLUMNS) + (r_piece ^ (r_row & 7)) * 16;
+    static_assert(kRowStep % 8 == 0 && kTokens % 32 == 0, "rows of a thread have one place in their eight");
+    const T* x_from[kTokens / 32];
+#pragma unroll
+    for (int i = 0; i < kTokens / 32; ++i) x_from[i] = x + min(x_row + 32 * i, tokens - 1) * a.x_stride + 8 * x_piece;   // (rows behind the last: anything)
+    const bool wide = x_wide && r_wide;
+
+    for (int pass = 0; pass < a.experts; pass += COLUMNS) {
+        const int columns = min(COLUMNS, a.experts - pass), r_live = columns - 8 * r_piece, r_bytes = 2 * min(r_live, 8);
+        const T* const r_from = r + pass + 8 * r_piece + r_row * a.router_stride;
+        auto bring = [&](int s, uint32_t to) {
+            const int k0 = s * kRouteDepth;
+            if (s >= end) {
+            } else if (wide && k0 + kRouteDepth <= a.width) {
+#pragma unroll
+                for (int i = 0; i < kTokens / 32; ++i) copy_16(to + x_to + i * 32 * 128, x_from[i] + k0);
+                if (r_live > 0) {
+                    const T* from = r_from + k0 * a.router_stride;
+#pragma unroll
+                    for (int i = 0; i < kRouteDepth / kRowStep; ++i, from += kRowStep * a.router_stride) copy_16(to + r_to + i * kRowStep * 2 * COLUMNS, from, r_bytes);
+                }
+            } else {
+                const int x_live = a.width - k0 - 8 * x_piece;
+#pragma unroll 1
+                for (int i = 0; i < kTokens / 32; ++i) bring_eight(to + x_to + i * 32 * 128, x_live > 0 ? x_from[i] + k0 : x, max(x_live, 0), x_wide);
+#pragma unroll 1
+                for (int i = 0; i < kRouteDepth / kRowStep; ++i) {
+                    const int k = r_row + i * kRowStep, live = k0 + k < a.width ? max(r_live, 0) : 0;
+                    bring_eight(to + r_to + i * kRowStep * 2 * COLUMNS, live ? r_from + (k0 + i * kRowStep) * a.router_stride : r, live, r_wide);
+                }
+            }
+            copies_end_group();
+        };
+        float sum[2 * kBlocks][4] = {};
+        for (int s = 0; s < kRing - 1; ++s) bring(begin + s, ring + s * kStageBytes);
+        uint32_t slot = 0;
+        for (int s = begin; s < end; ++s) {
+            copies_wait<kRing - 2>();
+            __syncthreads();
+            bring(s + kRing - 1, ring + (slot == 0 ? kRing - 1 : slot - 1) * kStageBytes);
+            const uint32_t x_at = ring + slot * kStageBytes + (16 * block + at_row) * 128, r_at = ring + slot * kStageBytes + kXBytes + at_row * (2 * COLUMNS);
+            slot = slot == kRing - 1 ? 0 : slot + 1;
+            uint32_t rows[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) load_matrices(rows[k], x_at + ((2 * k + at_piece) ^ (at_row & 7)) * 16);
+#pragma unroll
+            for (int n = 0; n < kBlocks; ++n) {
+                float part[2][4] = {};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t b[4];
+                    load_turned(b, r_at + k * 16 * (2 * COLUMNS) + (((share + 16 * n) / 8 + at_piece) ^ (at_row & 7)) * 16);
+                    mma_16(part[0], rows[k], b[0], b[1], T());
+                    mma_16(part[1], rows[k], b[2], b[3], T());
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[2 * n][i] += part[0][i], sum[2 * n + 1][i] += part[1][i];
+            }
+        }
+        copies_wait<0>();
+        __syncthreads();                         // the ring is free: for the logits, or for the next pass
+#pragma unroll
+        for (int n = 0; n < 2 * kBlocks; ++n) {
+            if (share + 8 * n >= columns) break;
+            float* const to = logits + (16 * block + lane / 4) * row_floats + pass + share + 8 * n + lane % 4 * 2;
+            *reinterpret_cast<float2*>(to) = make_float2(sum[n][0], sum[n][1]);
+            *reinterpret_cast<float2*>(to + 8 * row_floats) = make_float2(sum[n][2], sum[n][3]);
+        }
+    }
+    auto meet = [&]() {
+        if (cluster > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        else __syncthreads();
+    };
+    meet();
+    // keys: an order of numbers above 0, which stands for none: NaN 1
+    auto number = [](uint32_t key) {
+        const uint32_t bits = key - 1;
+        return bits == 0 ? __uint_as_float(0x7fffffffu) : __uint_as_float(bits & 0x80000000u ? bits & 0x7fffffffu : ~bits);
+    };
+    constexpr int kAtOnce = KEYS > 8 ? 1 : 4;    // tokens of a warp, whose rounds wait side by side
+    for (int t0 = warp; rank + t0 * cluster < tokens; t0 += kWarps * kAtOnce) {
+        uint32_t key[kAtOnce][KEYS];
+        int token[kAtOnce];
+#pragma unroll
+        for (int b = 0; b < kAtOnce; ++b) {
+            token[b] = rank + (t0 + b * kWarps) * cluster;
+            const float* const mine = logits + min(token[b], tokens - 1) * row_floats;
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) {
+                const int e = 32 * i + lane;
+                float all = 0.0f;
+                if (cluster == 1) {
+                    all = e < a.experts ? mine[e] : 0.0f;
+                } else if (e < a.experts && token[b] < tokens) {
+                    // the CTAs' sums, in their order
+                    float part[kMaxCluster];
+#pragma unroll
+                    for (int c = 0; c < kMaxCluster; ++c) {
+                        uint32_t there;
+                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(smem_at(mine + e)), "r"(c < cluster ? c : 0));
+                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[c]) : "r"(there) : "memory");
+                    }
+#pragma unroll
+                    for (int c = 0; c < kMaxCluster; ++c) all += c < cluster ? part[c] : 0.0f;
+                }
+                key[b][i] = e < a.experts ? ordered(all) + 1 : 0;
+            }
+        }
+        float first[kAtOnce], total[kAtOnce], own[kAtOnce];
+        int chosen[kAtOnce];
+#pragma unroll
+        for (int b = 0; b < kAtOnce; ++b) {
+            uint32_t best = 0;
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) best = max(best, key[b][i]);
+            first[b] = number(__reduce_max_sync(0xffffffffu, best));
+            total[b] = 0.0f;
+            if (a.normalise) continue;
+#pragma unroll
+            for (int i = 0; i < KEYS; ++i) total[b] += key[b][i] ? expf(number(key[b][i]) - first[b]) : 0.0f;
+        }
+        for (int j = 0; j < a.top; ++j) {
+            uint32_t best[kAtOnce];
+            int e[kAtOnce];
+#pragma unroll
+            for (int b = 0; b < kAtOnce; ++b) {
+                best[b] = 0;
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) best[b] = max(best[b], key[b][i]);
+                best[b] = __reduce_max_sync(0xffffffffu, best[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < kAtOnce; ++b) {
+                // the lowest of those that have it
+                e[b] = FMB_MAX_GROUPS;
+#pragma unroll
+                for (int i = KEYS - 1; i >= 0; --i) e[b] = key[b][i] == best[b] ? 32 * i + lane : e[b];
+                e[b] = __reduce_min_sync(0xffffffffu, e[b]);
+            }
+#pragma unroll
+            for (int b = 0; b < kAtOnce; ++b) {
+#pragma unroll
+                for (int i = 0; i < KEYS; ++i) key[b][i] = 32 * i + lane == e[b] ? 0 : key[b][i];
+                own[b] = lane == j ? number(best[b]) : own[b];
+                chosen[b] = lane == j ? e[b] : chosen[b];
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < kAtOnce; ++b) {
+            own[b] = lane < a.top ? expf(own[b] - first[b]) : 0.0f;
+            total[b] = warp_sum(a.normalise ? own[b] : total[b]);
+            if (lane < a.top && token[b] < tokens) {
+                const long long to = (first_token + token[b]) * a.top + lane;
+                a.chosen[to] = chosen[b];
+                a.weights[to] = own[b] / total[b];
+            }
+        }
+    }
+    if (cluster > 1) meet();                     // shared memory lives until it has been read
+}
+
 // --------------------------------------------------------------------------------------------------------------- layer
-
-__device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-__device__ __forceinline__ void mma_16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
 
 __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -259,21 +487,6 @@ template <typename T, bool WIDE> struct Stage {
     }
 };
 constexpr int kStages = 3;
-
-__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-// 16 or 8 bytes, of which the first `bytes` are read and the others zero
-__device__ __forceinline__ void copy_16(uint32_t to, const void* from, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void copy_8(uint32_t to, const void* from, int bytes) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
-}
-// whole ones
-__device__ __forceinline__ void copy_16(uint32_t to, const void* from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
-__device__ __forceinline__ void copy_8(uint32_t to, const void* from) { asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to), "l"(from) : "memory"); }
-__device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ uint4 load_16(uint32_t at) {
     uint4 v;
@@ -1127,14 +1340,55 @@ int route(const fmb_route_t& a, cudaStream_t stream) {
     return FMB_OK;
 }
 
+template <typename T, int MT, int COLUMNS, int KEYS>
+int route_many(const fmb_route_t& a, cudaStream_t stream) {
+    const auto kernel = k_route_many<T, MT, COLUMNS, KEYS>;
+    constexpr int kRing = kRouteRing<MT, COLUMNS>, kLogits = 16 * MT * route_row(32 * KEYS) * (int)sizeof(float);
+    constexpr int kSmem = KEYS * 32 <= COLUMNS ? std::max(kRing, kLogits) : kRing + kLogits;
+    static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)kernel, kSmem));
+    const int blocks = ceil_div(a.tokens, 16 * MT), stages = ceil_div(a.width, kRouteDepth);
+    // CTAs that share the depth, while there are SMs for them, for two each where they fit (8,192 tokens of 2,048, 64 experts: 18.9 us, and 20.6 with
+    // one each)
+    constexpr int kResident = std::min(2, 227 * 1024 / kSmem);
+    int share = 1;
+    while (share < kMaxCluster && 2 * share * blocks <= kResident * grp::sm_count() && 2 * share <= stages) share *= 2;
+    cudaLaunchConfig_t config = {};
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = share;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.gridDim = dim3((unsigned)(blocks * share));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kSmem;
+    config.stream = stream;
+    config.attrs = &cluster;
+    config.numAttrs = share > 1;
+    FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, kernel, a, (int)fits(a.x, a.x_stride, sizeof(T)), (int)fits(a.router, a.router_stride, sizeof(T)), share));
+    FMB_LAUNCH_CHECK();
+    return FMB_OK;
+}
+
 template <typename T>
 int route(const fmb_route_t& a, cudaStream_t stream) {
-    // by what the tokens would read of R one by one (us with one, two, four, eight tokens a cluster: 64 tokens and 32 experts of 4,096: 7.7, -, 10.9, -;
-    // 64 and 256: -, -, 24, -; 128 and 256: 56, -, -, 35)
-    if (a.tokens > 128) return route<T, 8, 1>(a, stream);
-    const int logits = a.tokens * a.experts;
-    return logits <= 4096 ? route<T, 1, 8>(a, stream) : logits <= 8192 ? route<T, 2, 8>(a, stream)
-           : logits <= 16384 ? route<T, 4, 8>(a, stream) : route<T, 8, 8>(a, stream);
+    const int logits = a.tokens <= 128 ? a.tokens * a.experts : 128 * FMB_MAX_GROUPS;
+    if constexpr (sizeof(T) == 2) {
+        // by matrix instructions (us, and without, bf16: 64 tokens and 64 experts of 2,048 8.7, 7.1; 64 and 128 of 4,096 13.7, 12.2; 8 and 256 20, 13; 64 and
+        // 256 21, 24; 128 and 256 21, 34; 4 and 1,024 of 2,048 28, 51; 16,384 and 64 28, 361)
+        if (logits > 8192 || a.experts > 256) {
+            return a.experts <= 64    ? route_many<T, 4, 64, 2>(a, stream)
+                   : a.experts <= 128 ? route_many<T, 4, 128, 4>(a, stream)
+                   : a.experts <= 256 ? route_many<T, 4, 256, 8>(a, stream)
+                                      : route_many<T, 2, 128, 32>(a, stream);
+        }
+        return logits <= 4096 ? route<T, 1, 8>(a, stream) : route<T, 2, 8>(a, stream);
+    } else {
+        // by what the tokens would read of R one by one (us with one, two, four, eight tokens a cluster, bf16: 64 tokens and 32 experts of 4,096: 7.7, -,
+        // 10.9, -; 64 and 256: -, -, 24, -; 128 and 256: 56, -, -, 35)
+        if (a.tokens > 128) return route<T, 8, 1>(a, stream);
+        return logits <= 4096 ? route<T, 1, 8>(a, stream) : logits <= 8192 ? route<T, 2, 8>(a, stream)
+               : logits <= 16384 ? route<T, 4, 8>(a, stream) : route<T, 8, 8>(a, stream);
+    }
 }
 
 }  // namespace

@@ -144,6 +144,68 @@ def test_infinities_and_nan_stay_with_their_tokens():
         assert torch.equal(y[keep], want[keep]) and bool(y[3].isnan().all()) and not bool(y[9].isfinite().any())
 
 
+def _check_routes(x, router, top, normalise, given):
+    from fastmace_b200 import experts
+    (t, width), count = x.shape, router.shape[1]
+    routes = experts.route_rows(given, router, top, normalise)
+    logits, size = x.double() @ router.double(), x.double().abs() @ router.double().abs()
+    order = torch.sort(logits, dim=1, descending=True, stable=True).indices[:, :top]
+    got = torch.gather(logits, 1, routes.experts.long())
+    # sums in float32: width additions of half a step, and what the tensor core cuts off
+    tol = (width + 8) * 2.0 ** -24 * size.amax(1, keepdim=True)
+    assert bool(((got - torch.gather(logits, 1, order)).abs() <= 2 * tol).all())
+    assert all(len(set(row)) == top for row in routes.experts.tolist())
+    p = torch.softmax(got if normalise else logits, 1)
+    p = p if normalise else torch.gather(p, 1, routes.experts.long())
+    assert bool(((routes.weights.double() - p).abs() <= p * (4 * tol + (count + 16) * 2.0 ** -24) + 1e-30).all())
+    again = experts.route_rows(x.contiguous(), router, top, normalise)
+    assert torch.equal(again.experts, routes.experts) and torch.equal(again.weights, routes.weights)
+
+
+@pytest.mark.parametrize("normalise", [True, False])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("shape", [(129, 64, 8, 64), (130, 300, 16, 192), (257, 1024, 4, 72), (3, 1000, 5, 2000), (4097, 65, 5, 520), (140, 256, 16, 1),
+                                   (150, 9, 2, 4096), (129, 128, 1, 63), (10001, 17, 3, 129), (128, 250, 8, 1000), (40000, 8, 2, 96)])
+def test_routes_of_many_tokens(shape, dtype, normalise):
+    t, count, top, width = shape
+    g = torch.Generator(device="cuda").manual_seed(t + count)
+    x = torch.randn(t, width, generator=g, device="cuda").to(dtype)
+    router = (torch.randn(width, count, generator=g, device="cuda") / width ** 0.5).to(dtype)
+    for extra in (0, 3, 8):                      # rows side by side, odd and at whole pieces of 16 bytes
+        held = [torch.full((m.shape[0], m.shape[1] + extra), float("nan"), dtype=dtype, device="cuda") for m in (x, router)]
+        for h, m in zip(held, (x, router)):
+            h[:, :m.shape[1]] = m
+        _check_routes(x, held[1][:, :count], top, normalise, held[0][:, :width])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("tokens", [130, 20000])
+def test_routes_of_many_tokens_with_equal_and_bad_logits(dtype, tokens):
+    from fastmace_b200 import experts
+    inf, nan = float("inf"), float("nan")
+    x = torch.zeros(tokens, 64, device="cuda", dtype=dtype)
+    x[:, 0] = 1
+    router = torch.zeros(64, 70, device="cuda", dtype=dtype)
+    router[0] = torch.tensor([1.0, -0.0, 0.0, 2.0, 1.0, 2.0] + [0.5] * 64, device="cuda").to(dtype)
+    routes = experts.route_rows(x, router, 6)
+    assert bool((routes.experts == torch.tensor([3, 5, 0, 4, 6, 7], device="cuda")).all())
+    router[0, 3], router[0, 9] = nan, -inf       # infinities times the zeros of x are nowhere else
+    routes = experts.route_rows(x, router, 6)
+    assert bool((routes.experts == torch.tensor([5, 0, 4, 6, 7, 8], device="cuda")).all()) and bool(routes.weights.isfinite().all())
+    assert bool(experts.route_rows(x, router, 6, normalise=False).weights.isnan().all())
+    # one bad token: its own row alone
+    router[0, 3] = 2.0
+    want = experts.route_rows(x, router, 6)
+    x[77] = nan
+    routes = experts.route_rows(x, router, 6)
+    assert routes.experts[77].tolist() == [0, 1, 2, 3, 4, 5] and bool(routes.weights[77].isnan().all())
+    rest = torch.arange(tokens, device="cuda") != 77
+    assert torch.equal(routes.experts[rest], want.experts[rest]) and torch.equal(routes.weights[rest], want.weights[rest])
+    # all choices are NaN, in their order
+    router[0] = nan
+    assert bool((experts.route_rows(x, router, 6).experts == torch.arange(6, device="cuda")).all())
+
+
 @pytest.mark.parametrize("normalise", [True, False])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("shape", [(1, 1, 1, 1), (3, 64, 8, 256), (40, 7, 7, 65), (200, 40, 3, 1001), (5, 1024, 16, 128), (2, 9, 2, 4096), (1000, 128, 8, 64)])
