@@ -65,9 +65,15 @@ __device__ __forceinline__ void copy_8(uint32_t to, const void* from) { asm vola
 __device__ __forceinline__ void copies_end_group() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+__device__ __forceinline__ uint4 load_16(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+    return v;
+}
 // --------------------------------------------------------------------------------------------------------------- route
 
 
+constexpr int kMaxCluster = 8;
 constexpr int kRouteChunk = 512;                 // of a CTA's depth, whose values of x lie in shared memory
 
 // eight values as they are in memory, and as floats
@@ -107,12 +113,13 @@ __device__ __forceinline__ uint32_t ordered(float x) {
     return x != x ? 0u : bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
 
-// CLUSTER CTAs for TOKENS tokens: each takes its share of the depth, threads by packs of eight experts and rows of R, which all tokens share; then
-// CTA c the choices of tokens c, c + CLUSTER, ... A cluster of eight for a token each where there are few (1 token of 2,048, 64 experts: 5.2 us),
-// for two to eight tokens where they would read much of R one by one, and a CTA alone beyond 128 tokens of float32.
-template <typename T, int TOKENS, int CLUSTER>
+// A few tokens. A cluster of eight CTAs for TOKENS tokens: each takes its share of the depth, threads by packs of eight experts and rows of R, which
+// all tokens share; then CTA c the choices of token c. A cluster for a token each where there are few (1 token of 2,048, 64 experts: 5.2
+// us), for two to eight tokens where they would read much of R one by one.
+template <typename T, int TOKENS>
 __global__ void __launch_bounds__(kThreads)
 k_route(fmb_route_t a, int wide, int rows) {
+    constexpr int CLUSTER = kMaxCluster;
     extern __shared__ float sums[];              // [kRouteChunk][TOKENS] values of x; then [TOKENS][rows][packs of eight]
     let_next_come();
     const int first_token = blockIdx.x / CLUSTER * TOKENS, rank = blockIdx.x % CLUSTER, packs = (a.experts + 7) / 8;
@@ -165,38 +172,31 @@ k_route(fmb_route_t a, int wide, int rows) {
             sums[at] += sums[at + size];
         }
     }
-    auto meet = []() {
-        if constexpr (CLUSTER > 1) asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-        else __syncthreads();
-    };
+    auto meet = []() { asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory"); };
     meet();
     // An expert's place is the number of those before it (larger logit, or the same and a lower number): each thread counts for its own,
     // which takes one wait where choosing one after the other takes one each. Numbers are made unlike by the expert's.
     __shared__ alignas(16) unsigned long long order[FMB_MAX_GROUPS + 2];
     __shared__ float logits[FMB_MAX_GROUPS], best[FMB_MAX_TOP], warp_total[kWarps];
-    for (int own = rank; own < TOKENS; own += CLUSTER) {
-        const long long token = first_token + own;
-        if (token >= a.tokens) break;            // (the same for the CTA)
+    static_assert(TOKENS <= CLUSTER, "a CTA for each token's choices");
+    const long long token = first_token + rank;
+    if (rank < TOKENS && token < a.tokens) {
         for (int e = threadIdx.x; e <= a.experts; e += kThreads) {
             // the CTAs' sums, in their order
             float all = 0.0f;
             if (e < a.experts) {
-                const float* const mine = sums + own * rows * packs * 8 + e;
-                if constexpr (CLUSTER > 1) {
-                    const uint32_t here = (uint32_t)__cvta_generic_to_shared(mine);
-                    float part[CLUSTER];
+                const float* const mine = sums + rank * rows * packs * 8 + e;
+                const uint32_t here = (uint32_t)__cvta_generic_to_shared(mine);
+                float part[CLUSTER];
 #pragma unroll
-                    for (int c = 0; c < CLUSTER; ++c) {
-                        uint32_t there;
-                        asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(c));
-                        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[c]) : "r"(there) : "memory");
-                    }
-                    all = part[0];
-#pragma unroll
-                    for (int c = 1; c < CLUSTER; ++c) all += part[c];
-                } else {
-                    all = *mine;
+                for (int c = 0; c < CLUSTER; ++c) {
+                    uint32_t there;
+                    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(here), "r"(c));
+                    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(part[c]) : "r"(there) : "memory");
                 }
+                all = part[0];
+#pragma unroll
+                for (int c = 1; c < CLUSTER; ++c) all += part[c];
                 logits[e] = all;
             }
             order[e] = e < a.experts ? (unsigned long long)ordered(all) << 32 | (0xffffffffu - e) : 0;
@@ -229,20 +229,21 @@ k_route(fmb_route_t a, int wide, int rows) {
             for (int w = 0; w < kWarps; ++w) total += warp_total[w];
         }
         if (threadIdx.x < a.top) a.weights[token * a.top + threadIdx.x] = expf(best[threadIdx.x] - first) / total;
-        if (CLUSTER < TOKENS) __syncthreads();
     }
-    if (CLUSTER > 1) meet();                     // shared memory lives until it has been read
+    meet();                                      // shared memory lives until it has been read
 }
 
-// Many tokens of 16-bit types, by matrix instructions: a CTA has 16 MT tokens and all experts, COLUMNS of them at a time, its eight warps MT blocks of
-// 16 tokens by 8 / MT shares of the columns. A ring of asynchronous copies brings 64 of the depth at a time; their sums start at zero and are added
-// to those before with rounding, since the tensor core cuts its sums off. Where blocks of tokens are few, the CTAs of a cluster share the depth,
-// and each then has every so many of the tokens. A warp chooses for up to four tokens side by side: rounds of the largest of all, which a lane holds a 32nd
-// of. 16,384 tokens of 2,048 and 64 experts: 28 us with one choice, 34 with eight (10 for the bytes; instructions issue in half of the cycles).
-constexpr int kRouteDepth = 64, kMaxCluster = 8;
+// Many tokens. A CTA has 16 MT of them and all experts, COLUMNS at a time; a ring of asynchronous copies brings 128 bytes of each row of x and the
+// rows of R that they multiply. 16-bit types by matrix instructions, eight warps as MT blocks of 16 tokens by 8 / MT shares of the columns; the sums of a
+// stage start at zero and are added to those before with rounding, since the tensor core cuts its sums off. float32 by fused multiply-adds, in which
+// all bits count, MT tokens by COLUMNS / 16 columns a thread. Where blocks of tokens are few, the CTAs of a cluster share the depth, and each
+// then has every so many of the tokens. A warp chooses for up to four tokens side by side: rounds of the largest of all, which a lane holds a 32nd of.
+// 16,384 tokens of 2,048 and 64 experts: bf16 28 us with one choice, 34 with eight (10 for the bytes; instructions issue in half of the cycles),
+// fp32 137 (60 for the multiply-adds).
+template <typename T> constexpr int kRouteDepth = 128 / sizeof(T);
 
 template <int COLUMNS> constexpr int kRouteStages = COLUMNS == 256 ? 3 : 4;
-template <int MT, int COLUMNS> constexpr int kRouteRing = kRouteStages<COLUMNS> * kRouteDepth * (16 * MT + COLUMNS) * 2;
+template <int MT, int COLUMNS> constexpr int kRouteRing = kRouteStages<COLUMNS> * 128 * (16 * MT + COLUMNS);
 __host__ __device__ constexpr int route_row(int experts) { return (experts + 31) / 32 * 32 + 8; }   // floats of a token's logits, for the banks
 
 __device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t at) {
@@ -252,13 +253,14 @@ __device__ __forceinline__ void load_turned(uint32_t (&r)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
 
-// eight values to shared memory, of which the first `live` are read and the others zero
+// 16 bytes of values to shared memory, of which the first `live` values are read and the others zero
 template <typename T>
-__device__ __forceinline__ void bring_eight(uint32_t to, const T* from, int live, bool wide) {
+__device__ __forceinline__ void bring_piece(uint32_t to, const T* from, int live, bool wide) {
+    constexpr int kValues = 16 / sizeof(T);
     if (wide) {
-        copy_16(to, from, 2 * min(live, 8));
+        copy_16(to, from, (int)sizeof(T) * min(live, kValues));
     } else {
-        const Eight<T> in = load_eight(from, live, false);
+        const Eight<T> in = load_eight(from, min(live, kValues), false);
         asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(in.v[0]), "r"(in.v[1]), "r"(in.v[2]), "r"(in.v[3]) : "memory");
     }
 }
@@ -266,93 +268,142 @@ __device__ __forceinline__ void bring_eight(uint32_t to, const T* from, int live
 template <typename T, int MT, int COLUMNS, int KEYS>
 __global__ void __launch_bounds__(kThreads)
 k_route_many(fmb_route_t a, int x_wide, int r_wide, int cluster) {
-    constexpr int kTokens = 16 * MT, kShare = COLUMNS * MT / kWarps, kBlocks = kShare / 16, kRing = kRouteStages<COLUMNS>;
-    constexpr int kStageBytes = kRouteDepth * (kTokens + COLUMNS) * 2, kXBytes = kTokens * kRouteDepth * 2, kRowPieces = COLUMNS / 8;
+    constexpr int kTokens = 16 * MT, kRing = kRouteStages<COLUMNS>, kDepth = kRouteDepth<T>, kValues = 16 / sizeof(T);
+    constexpr int kXBytes = kTokens * 128, kStageBytes = kXBytes + COLUMNS * 128, kRowBytes = COLUMNS * sizeof(T), kRowPieces = kRowBytes / 16;
+    constexpr bool kMatrix = sizeof(T) == 2;
     constexpr bool kOver = KEYS * 32 <= COLUMNS; // the logits take the ring's place
     extern __shared__ __align__(128) uint8_t shared[];
     let_next_come();
     const int rank = blockIdx.x % cluster, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const long long first_token = (long long)(blockIdx.x / cluster) * kTokens;
-    const int tokens = (int)min((long long)kTokens, a.tokens - first_token), stages = (a.width + kRouteDepth - 1) / kRouteDepth;
+    const int tokens = (int)min((long long)kTokens, a.tokens - first_token), stages = (a.width + kDepth - 1) / kDepth;
     const int begin = (int)((long long)stages * rank / cluster), end = (int)((long long)stages * (rank + 1) / cluster);
     const T* const x = (const T*)a.x + first_token * a.x_stride;
     const T* const r = (const T*)a.router;
     float* const logits = reinterpret_cast<float*>(shared + (kOver ? 0 : kRouteRing<MT, COLUMNS>));
     const int row_floats = route_row(a.experts);
     const uint32_t ring = smem_at(shared);
-    const int block = warp % MT, share = warp / MT * kShare;      // of the warp: tokens, columns of a pass
-    const int at_row = lane & 15, at_piece = lane >> 4;
 
     // of the thread: one piece of every 32nd row of x, and one of every kRowStep-th of R
     constexpr int kRowStep = kThreads / kRowPieces;
     const int x_row = threadIdx.x / 8, x_piece = threadIdx.x % 8, r_row = threadIdx.x / kRowPieces, r_piece = threadIdx.x % kRowPieces;
-    const uint32_t x_to = x_row * 128 + (x_piece ^ (x_row & 7)) * 16, r_to = kXBytes + r_row * (2 * COLUMNS) + (r_piece ^ (r_row & 7)) * 16;
-    static_assert(kRowStep % 8 == 0 && kTokens % 32 == 0, "rows of a thread have one place in their eight");
+    const uint32_t x_to = x_row * 128 + (x_piece ^ (x_row & 7)) * 16, r_to = kXBytes + r_row * kRowBytes + (kMatrix ? r_piece ^ (r_row & 7) : r_piece) * 16;
+    static_assert((!kMatrix || kRowStep % 8 == 0) && kTokens % 32 == 0, "rows of a thread have one place in their eight");
     const T* x_from[kTokens / 32];
 #pragma unroll
-    for (int i = 0; i < kTokens / 32; ++i) x_from[i] = x + min(x_row + 32 * i, tokens - 1) * a.x_stride + 8 * x_piece;   // (rows behind the last: anything)
+    for (int i = 0; i < kTokens / 32; ++i) x_from[i] = x + min(x_row + 32 * i, tokens - 1) * a.x_stride + kValues * x_piece;   // (rows behind the last: anything)
     const bool wide = x_wide && r_wide;
 
     for (int pass = 0; pass < a.experts; pass += COLUMNS) {
-        const int columns = min(COLUMNS, a.experts - pass), r_live = columns - 8 * r_piece, r_bytes = 2 * min(r_live, 8);
-        const T* const r_from = r + pass + 8 * r_piece + r_row * a.router_stride;
+        const int columns = min(COLUMNS, a.experts - pass), r_live = columns - kValues * r_piece, r_bytes = (int)sizeof(T) * min(r_live, kValues);
+        const T* const r_from = r + pass + kValues * r_piece + r_row * a.router_stride;
         auto bring = [&](int s, uint32_t to) {
-            const int k0 = s * kRouteDepth;
+            const int k0 = s * kDepth;
             if (s >= end) {
-            } else if (wide && k0 + kRouteDepth <= a.width) {
+            } else if (wide && k0 + kDepth <= a.width) {
 #pragma unroll
                 for (int i = 0; i < kTokens / 32; ++i) copy_16(to + x_to + i * 32 * 128, x_from[i] + k0);
                 if (r_live > 0) {
                     const T* from = r_from + k0 * a.router_stride;
 #pragma unroll
-                    for (int i = 0; i < kRouteDepth / kRowStep; ++i, from += kRowStep * a.router_stride) copy_16(to + r_to + i * kRowStep * 2 * COLUMNS, from, r_bytes);
+                    for (int i = 0; i < kDepth / kRowStep; ++i, from += kRowStep * a.router_stride) copy_16(to + r_to + i * kRowStep * kRowBytes, from, r_bytes);
                 }
             } else {
-                const int x_live = a.width - k0 - 8 * x_piece;
+                const int x_live = a.width - k0 - kValues * x_piece;
 #pragma unroll 1
-                for (int i = 0; i < kTokens / 32; ++i) bring_eight(to + x_to + i * 32 * 128, x_live > 0 ? x_from[i] + k0 : x, max(x_live, 0), x_wide);
+                for (int i = 0; i < kTokens / 32; ++i) bring_piece(to + x_to + i * 32 * 128, x_live > 0 ? x_from[i] + k0 : x, max(x_live, 0), x_wide);
 #pragma unroll 1
-                for (int i = 0; i < kRouteDepth / kRowStep; ++i) {
+                for (int i = 0; i < kDepth / kRowStep; ++i) {
                     const int k = r_row + i * kRowStep, live = k0 + k < a.width ? max(r_live, 0) : 0;
-                    bring_eight(to + r_to + i * kRowStep * 2 * COLUMNS, live ? r_from + (k0 + i * kRowStep) * a.router_stride : r, live, r_wide);
+                    bring_piece(to + r_to + i * kRowStep * kRowBytes, live ? r_from + (k0 + i * kRowStep) * a.router_stride : r, live, r_wide);
                 }
             }
             copies_end_group();
         };
-        float sum[2 * kBlocks][4] = {};
         for (int s = 0; s < kRing - 1; ++s) bring(begin + s, ring + s * kStageBytes);
         uint32_t slot = 0;
-        for (int s = begin; s < end; ++s) {
+        auto next = [&](int s) {
             copies_wait<kRing - 2>();
             __syncthreads();
             bring(s + kRing - 1, ring + (slot == 0 ? kRing - 1 : slot - 1) * kStageBytes);
-            const uint32_t x_at = ring + slot * kStageBytes + (16 * block + at_row) * 128, r_at = ring + slot * kStageBytes + kXBytes + at_row * (2 * COLUMNS);
+            const uint32_t at = ring + slot * kStageBytes;
             slot = slot == kRing - 1 ? 0 : slot + 1;
-            uint32_t rows[4][4];
+            return at;
+        };
+        auto ring_free = [] {                    // for the logits, or for the next pass
+            copies_wait<0>();
+            __syncthreads();
+        };
+        if constexpr (kMatrix) {
+            constexpr int kShare = COLUMNS * MT / kWarps, kBlocks = kShare / 16;
+            const int block = warp % MT, share = warp / MT * kShare;                    // of the warp: tokens, columns of the pass
+            const int at_row = lane & 15, at_piece = lane >> 4;
+            float sum[2 * kBlocks][4] = {};
+            for (int s = begin; s < end; ++s) {
+                const uint32_t at = next(s), x_at = at + (16 * block + at_row) * 128, r_at = at + kXBytes + at_row * kRowBytes;
+                uint32_t rows[4][4];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) load_matrices(rows[k], x_at + ((2 * k + at_piece) ^ (at_row & 7)) * 16);
+                for (int k = 0; k < 4; ++k) load_matrices(rows[k], x_at + ((2 * k + at_piece) ^ (at_row & 7)) * 16);
 #pragma unroll
-            for (int n = 0; n < kBlocks; ++n) {
-                float part[2][4] = {};
+                for (int n = 0; n < kBlocks; ++n) {
+                    float part[2][4] = {};
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    uint32_t b[4];
-                    load_turned(b, r_at + k * 16 * (2 * COLUMNS) + (((share + 16 * n) / 8 + at_piece) ^ (at_row & 7)) * 16);
-                    mma_16(part[0], rows[k], b[0], b[1], T());
-                    mma_16(part[1], rows[k], b[2], b[3], T());
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t b[4];
+                        load_turned(b, r_at + k * 16 * kRowBytes + (((share + 16 * n) / 8 + at_piece) ^ (at_row & 7)) * 16);
+                        mma_16(part[0], rows[k], b[0], b[1], T());
+                        mma_16(part[1], rows[k], b[2], b[3], T());
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sum[2 * n][i] += part[0][i], sum[2 * n + 1][i] += part[1][i];
                 }
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum[2 * n][i] += part[0][i], sum[2 * n + 1][i] += part[1][i];
             }
-        }
-        copies_wait<0>();
-        __syncthreads();                         // the ring is free: for the logits, or for the next pass
+            ring_free();
 #pragma unroll
-        for (int n = 0; n < 2 * kBlocks; ++n) {
-            if (share + 8 * n >= columns) break;
-            float* const to = logits + (16 * block + lane / 4) * row_floats + pass + share + 8 * n + lane % 4 * 2;
-            *reinterpret_cast<float2*>(to) = make_float2(sum[n][0], sum[n][1]);
-            *reinterpret_cast<float2*>(to + 8 * row_floats) = make_float2(sum[n][2], sum[n][3]);
+            for (int n = 0; n < 2 * kBlocks; ++n) {
+                if (share + 8 * n >= columns) break;
+                float* const to = logits + (16 * block + lane / 4) * row_floats + pass + share + 8 * n + lane % 4 * 2;
+                *reinterpret_cast<float2*>(to) = make_float2(sum[n][0], sum[n][1]);
+                *reinterpret_cast<float2*>(to + 8 * row_floats) = make_float2(sum[n][2], sum[n][3]);
+            }
+        } else {
+            // MT tokens, 16 apart, by groups of four columns, 64 apart
+            constexpr int kGroups = COLUMNS / 64;
+            const int own = threadIdx.x / 16, four = threadIdx.x % 16;
+            float sum[MT][kGroups][4] = {};
+            for (int s = begin; s < end; ++s) {
+                const uint32_t at = next(s), x_at = at + own * 128, r_at = at + kXBytes + four * 16;
+#pragma unroll 2
+                for (int k = 0; k < 8; ++k) {
+                    uint4 v[MT];
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) v[t] = load_16(x_at + t * 16 * 128 + (k ^ (own & 7)) * 16);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+                        for (int n = 0; n < kGroups; ++n) {
+                            const uint4 w = load_16(r_at + (4 * k + i) * kRowBytes + n * 256);
+#pragma unroll
+                            for (int t = 0; t < MT; ++t) {
+                                const float x = __uint_as_float(i == 0 ? v[t].x : i == 1 ? v[t].y : i == 2 ? v[t].z : v[t].w);
+                                sum[t][n][0] = fmaf(x, __uint_as_float(w.x), sum[t][n][0]);
+                                sum[t][n][1] = fmaf(x, __uint_as_float(w.y), sum[t][n][1]);
+                                sum[t][n][2] = fmaf(x, __uint_as_float(w.z), sum[t][n][2]);
+                                sum[t][n][3] = fmaf(x, __uint_as_float(w.w), sum[t][n][3]);
+                            }
+                        }
+                    }
+                }
+            }
+            ring_free();
+#pragma unroll
+            for (int n = 0; n < kGroups; ++n) {
+                if (64 * n + 4 * four >= columns) break;
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+                    *reinterpret_cast<float4*>(logits + (16 * t + own) * row_floats + pass + 64 * n + 4 * four) =
+                        make_float4(sum[t][n][0], sum[t][n][1], sum[t][n][2], sum[t][n][3]);
+            }
         }
     }
     auto meet = [&]() {
@@ -488,11 +539,6 @@ template <typename T, bool WIDE> struct Stage {
 };
 constexpr int kStages = 3;
 
-__device__ __forceinline__ uint4 load_16(uint32_t at) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
-    return v;
-}
 __device__ __forceinline__ uint2 load_8(uint32_t at) {
     uint2 v;
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
@@ -1318,24 +1364,24 @@ int layer(const fmb_experts_t& a, cudaStream_t stream) {
 
 bool fits(const void* base, long long stride, int bytes) { return ((uintptr_t)base & 15) == 0 && stride * bytes % 16 == 0; }
 
-template <typename T, int TOKENS, int CLUSTER>
+template <typename T, int TOKENS>
 int route(const fmb_route_t& a, cudaStream_t stream) {
     int rows = 1;
     while (2 * rows * ((a.experts + 7) / 8) <= kThreads) rows *= 2;
     const int smem = TOKENS * std::max(kRouteChunk, rows * ((a.experts + 7) / 8) * 8) * (int)sizeof(float);
-    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_route<T, TOKENS, CLUSTER>, TOKENS * kThreads * 8 * (int)sizeof(float)));
+    FMB_CUDA_CHECK(opt_in_shared_memory((const void*)k_route<T, TOKENS>, TOKENS * kThreads * 8 * (int)sizeof(float)));
     cudaLaunchConfig_t config = {};
     cudaLaunchAttribute cluster;
     cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = CLUSTER;
+    cluster.val.clusterDim.x = kMaxCluster;
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    config.gridDim = dim3((unsigned)ceil_div(a.tokens, TOKENS) * CLUSTER);
+    config.gridDim = dim3((unsigned)ceil_div(a.tokens, TOKENS) * kMaxCluster);
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = smem;
     config.stream = stream;
     config.attrs = &cluster;
-    config.numAttrs = CLUSTER > 1;
-    FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_route<T, TOKENS, CLUSTER>, a, (int)fits(a.router, a.router_stride, sizeof(T)), rows));
+    config.numAttrs = 1;
+    FMB_CUDA_CHECK(cudaLaunchKernelEx(&config, k_route<T, TOKENS>, a, (int)fits(a.router, a.router_stride, sizeof(T)), rows));
     FMB_LAUNCH_CHECK();
     return FMB_OK;
 }
@@ -1347,7 +1393,7 @@ int route_many(const fmb_route_t& a, cudaStream_t stream) {
     constexpr int kSmem = KEYS * 32 <= COLUMNS ? std::max(kRing, kLogits) : kRing + kLogits;
     static_assert(kSmem <= 227 * 1024, "shared memory of a CTA");
     FMB_CUDA_CHECK(opt_in_shared_memory((const void*)kernel, kSmem));
-    const int blocks = ceil_div(a.tokens, 16 * MT), stages = ceil_div(a.width, kRouteDepth);
+    const int blocks = ceil_div(a.tokens, 16 * MT), stages = ceil_div(a.width, kRouteDepth<T>);
     // CTAs that share the depth, while there are SMs for them, for two each where they fit (8,192 tokens of 2,048, 64 experts: 18.9 us, and 20.6 with
     // one each)
     constexpr int kResident = std::min(2, 227 * 1024 / kSmem);
@@ -1371,24 +1417,20 @@ int route_many(const fmb_route_t& a, cudaStream_t stream) {
 
 template <typename T>
 int route(const fmb_route_t& a, cudaStream_t stream) {
-    const int logits = a.tokens <= 128 ? a.tokens * a.experts : 128 * FMB_MAX_GROUPS;
-    if constexpr (sizeof(T) == 2) {
-        // by matrix instructions (us, and without, bf16: 64 tokens and 64 experts of 2,048 8.7, 7.1; 64 and 128 of 4,096 13.7, 12.2; 8 and 256 20, 13; 64 and
-        // 256 21, 24; 128 and 256 21, 34; 4 and 1,024 of 2,048 28, 51; 16,384 and 64 28, 361)
-        if (logits > 8192 || a.experts > 256) {
-            return a.experts <= 64    ? route_many<T, 4, 64, 2>(a, stream)
-                   : a.experts <= 128 ? route_many<T, 4, 128, 4>(a, stream)
-                   : a.experts <= 256 ? route_many<T, 4, 256, 8>(a, stream)
-                                      : route_many<T, 2, 128, 32>(a, stream);
-        }
-        return logits <= 4096 ? route<T, 1, 8>(a, stream) : route<T, 2, 8>(a, stream);
-    } else {
-        // by what the tokens would read of R one by one (us with one, two, four, eight tokens a cluster, bf16: 64 tokens and 32 experts of 4,096: 7.7, -,
-        // 10.9, -; 64 and 256: -, -, 24, -; 128 and 256: 56, -, -, 35)
-        if (a.tokens > 128) return route<T, 8, 1>(a, stream);
-        return logits <= 4096 ? route<T, 1, 8>(a, stream) : logits <= 8192 ? route<T, 2, 8>(a, stream)
-               : logits <= 16384 ? route<T, 4, 8>(a, stream) : route<T, 8, 8>(a, stream);
-    }
+    // us by blocks of many tokens, and by clusters for a few, bf16: 64 tokens and 64 experts of 2,048 8.7, 7.1; 64 and 128 of 4,096 13.7, 12.2; 8 and 256 20,
+    // 13; 64 and 256 21, 24; 128 and 256 21, 34; 4 and 1,024 of 2,048 28, 51 (rows at whole pieces of 16 bytes; 1 and 300 of 4,096, which are not, 66 by
+    // blocks). fp32: 128 and 256 of 4,096 72, 37; 1,024 and 64 of 2,048 23, 45
+    const bool pieces = fits(a.x, a.x_stride, sizeof(T)) && fits(a.router, a.router_stride, sizeof(T));
+    if (a.tokens > 128 || (sizeof(T) == 2 && pieces && (a.tokens * a.experts > 8192 || a.experts > 256)))
+        return a.experts <= 64    ? route_many<T, 4, 64, 2>(a, stream)
+               : a.experts <= 128 ? route_many<T, 4, 128, 4>(a, stream)
+               : a.experts <= 256 ? route_many<T, 4, 256, 8>(a, stream)
+                                  : route_many<T, 2, 128, 32>(a, stream);
+    // by what the tokens would read of R one by one (us with one, two, four, eight tokens a cluster: 64 tokens and 32 experts of 4,096: 7.7, -, 10.9, -;
+    // 64 and 256: -, -, 24, -; 128 and 256: 56, -, -, 35)
+    const int logits = a.tokens * a.experts;
+    return logits <= 4096 ? route<T, 1>(a, stream) : logits <= 8192 ? route<T, 2>(a, stream)
+           : logits <= 16384 ? route<T, 4>(a, stream) : route<T, 8>(a, stream);
 }
 
 }  // namespace

@@ -163,7 +163,7 @@ def _check_routes(x, router, top, normalise, given):
 
 
 @pytest.mark.parametrize("normalise", [True, False])
-@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("shape", [(129, 64, 8, 64), (130, 300, 16, 192), (257, 1024, 4, 72), (3, 1000, 5, 2000), (4097, 65, 5, 520), (140, 256, 16, 1),
                                    (150, 9, 2, 4096), (129, 128, 1, 63), (10001, 17, 3, 129), (128, 250, 8, 1000), (40000, 8, 2, 96)])
 def test_routes_of_many_tokens(shape, dtype, normalise):
@@ -171,14 +171,14 @@ def test_routes_of_many_tokens(shape, dtype, normalise):
     g = torch.Generator(device="cuda").manual_seed(t + count)
     x = torch.randn(t, width, generator=g, device="cuda").to(dtype)
     router = (torch.randn(width, count, generator=g, device="cuda") / width ** 0.5).to(dtype)
-    for extra in (0, 3, 8):                      # rows side by side, odd and at whole pieces of 16 bytes
+    for extra in (0, 3, 8):                  # rows side by side, odd and at whole pieces of 16 bytes
         held = [torch.full((m.shape[0], m.shape[1] + extra), float("nan"), dtype=dtype, device="cuda") for m in (x, router)]
         for h, m in zip(held, (x, router)):
             h[:, :m.shape[1]] = m
         _check_routes(x, held[1][:, :count], top, normalise, held[0][:, :width])
 
 
-@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("tokens", [130, 20000])
 def test_routes_of_many_tokens_with_equal_and_bad_logits(dtype, tokens):
     from fastmace_b200 import experts
