@@ -206,6 +206,32 @@ def test_routes_of_many_tokens_with_equal_and_bad_logits(dtype, tokens):
     assert bool((experts.route_rows(x, router, 6).experts == torch.arange(6, device="cuda")).all())
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tokens", [300, 12000])
+def test_routes_of_many_tokens_captured_and_on_two_streams(tokens, dtype):
+    from fastmace_b200 import experts
+    g = torch.Generator(device="cuda").manual_seed(tokens)
+    xs = [torch.randn(tokens, 520, generator=g, device="cuda").to(dtype) for _ in range(4)]
+    router = torch.randn(520, 130, generator=g, device="cuda").to(dtype)
+    want = [experts.route_rows(x, router, 6) for x in xs]
+    x = xs[0].clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = experts.route_rows(x, router, 6)
+    for given, routes in zip(xs, want):
+        x.copy_(given)
+        graph.replay()
+        assert torch.equal(held.experts, routes.experts) and torch.equal(held.weights, routes.weights)
+    streams, got = [torch.cuda.Stream() for _ in range(2)], []
+    torch.cuda.synchronize()
+    for n, given in enumerate(xs):
+        with torch.cuda.stream(streams[n % 2]):
+            got.append(experts.route_rows(given, router, 6))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a.experts, b.experts) and torch.equal(a.weights, b.weights) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("normalise", [True, False])
 @pytest.mark.parametrize("dtype", [F32, BF16, F16])
 @pytest.mark.parametrize("shape", [(1, 1, 1, 1), (3, 64, 8, 256), (40, 7, 7, 65), (200, 40, 3, 1001), (5, 1024, 16, 128), (2, 9, 2, 4096), (1000, 128, 8, 64)])
