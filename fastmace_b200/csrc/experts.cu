@@ -238,7 +238,7 @@ k_route(fmb_route_t a, int wide, int rows) {
 // stage start at zero and are added to those before with rounding, since the tensor core cuts its sums off. float32 by fused multiply-adds, in which
 // all bits count, MT tokens by COLUMNS / 16 columns a thread. Where blocks of tokens are few, the CTAs of a cluster share the depth, and each
 // then has every so many of the tokens. A warp chooses for up to four tokens side by side: rounds of the largest of all, which a lane holds a 32nd of.
-// 16,384 tokens of 2,048 and 64 experts: bf16 28 us with one choice, 34 with eight (10 for the bytes; instructions issue in half of the cycles),
+// 16,384 tokens of 2,048 and 64 experts: bf16 28 us with one choice, 34 with eight (10 for the bytes; issue slots 44 % full, most SMs with two of 256 blocks),
 // fp32 137 (60 for the multiply-adds).
 template <typename T> constexpr int kRouteDepth = 128 / sizeof(T);
 
