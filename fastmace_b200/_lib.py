@@ -232,9 +232,7 @@ def load() -> ctypes.CDLL:
     lib.fmb_sort_tokens_scratch.argtypes = [ctypes.c_longlong, c_int]
     lib.fmb_sort_tokens.argtypes = [P, c_int, ctypes.c_longlong, c_int, P, P, P, P]
     lib.fmb_embedding_gradient_scratch.argtypes = [POINTER(EmbeddingStruct)]
-    for name in ("fmb_sort_tokens_scratch", "fmb_embedding_gradient_scratch",
-           "fmb_hold_rows", "fmb_release_rows", "fmb_gated_rows", "fmb_gated_rows_gradient", "fmb_held_weight_gradient",
-           "fmb_held_weight_gradient_scratch", "fmb_route_rows", "fmb_expert_layer", "fmb_expert_layer_scratch"):
+    for name in ("fmb_sort_tokens_scratch", "fmb_embedding_gradient_scratch", "fmb_held_weight_gradient_scratch", "fmb_expert_layer_scratch"):
         getattr(lib, name).restype = ctypes.c_longlong
     for name in ("fmb_embedding", "fmb_embedding_gradient"):
         getattr(lib, name).argtypes = [POINTER(EmbeddingStruct), P]
@@ -242,11 +240,9 @@ def load() -> ctypes.CDLL:
         getattr(lib, name).argtypes = [POINTER(HeldStruct), P]
     lib.fmb_held_weight_gradient.argtypes = [POINTER(GroupedStruct), P, P]
     lib.fmb_held_weight_gradient_scratch.argtypes = [POINTER(GroupedStruct)]
-    lib.fmb_held_weight_gradient_scratch.restype = ctypes.c_longlong
     lib.fmb_route_rows.argtypes = [POINTER(RouteStruct), P]
     lib.fmb_expert_layer.argtypes = [POINTER(ExpertsStruct), P]
     lib.fmb_expert_layer_scratch.argtypes = [POINTER(ExpertsStruct)]
-    lib.fmb_expert_layer_scratch.restype = ctypes.c_longlong
     lib.fmb_adamw_step.argtypes = [POINTER(AdamwStruct), POINTER(AdamwTensorStruct), c_int, P]
     _LIB = lib
     return lib
