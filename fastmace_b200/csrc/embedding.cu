@@ -477,9 +477,10 @@ k_embedding_join(Sums p) {
 }
 
 // Rows per chunk: kWarps shares that make enough warps for 24 on every SM, and as few parts as that leaves; a share has between 8 rows,
-// what a warp has on their way, and 256.
-int chunk_rows(const fmb_embedding_t& a, int slabs) {
-    const long long rows = (long long)a.rows * slabs / (148 * 24) + 1;
+// what a warp has on their way, and 256. By sizes and type alone, with the slabs of rows at multiples of 16 bytes: the order of the sums and the
+// room for their parts do not depend on where the rows lie.
+int chunk_rows(const fmb_embedding_t& a) {
+    const long long rows = (long long)a.rows * ceil_div(a.width, a.type == FMB_TYPE_F32 ? 128 : 256) / (148 * 24) + 1;
     return kWarps * (int)std::min(256ll, std::max(8ll, (rows + 7) / 8 * 8));
 }
 
@@ -487,15 +488,13 @@ bool packed(const fmb_embedding_t& a) {
     return starts_at(a.source, a.source_stride, a.type == FMB_TYPE_F32 ? 4 : 2, a.type == FMB_TYPE_F32 ? 4 : 8);
 }
 
-int slabs_of(const fmb_embedding_t& a) { return ceil_div(a.width, a.type == FMB_TYPE_F32 ? 128 : packed(a) ? 256 : 128); }
-
 template <typename T>
 int gradient(const fmb_embedding_t& a, cudaStream_t stream) {
     constexpr int kPack = 16 / sizeof(T);
     Sums p;
     p.a = a;
-    p.slabs = slabs_of(a);
-    p.chunk = chunk_rows(a, p.slabs);
+    p.slabs = ceil_div(a.width, a.type != FMB_TYPE_F32 && packed(a) ? 256 : 128);
+    p.chunk = chunk_rows(a);
     p.chunks = ceil_div(a.rows, p.chunk);
     p.wide_out = starts_at(a.out, a.out_stride, 4, 4);
     p.part_stride = (a.width + 3) / 4 * 4;
@@ -549,7 +548,7 @@ extern "C" FMB_API int fmb_embedding(const fmb_embedding_t* a, fmb_stream_t stre
 
 extern "C" FMB_API long long fmb_embedding_gradient_scratch(const fmb_embedding_t* a) {
     if (!a || a->rows < 1 || a->width < 1 || a->type < FMB_TYPE_F32 || a->type > FMB_TYPE_F16) return 0;
-    const int chunk = chunk_rows(*a, slabs_of(*a));
+    const int chunk = chunk_rows(*a);
     return a->rows <= chunk ? 0 : 2ll * ceil_div(a->rows, chunk) * ((a->width + 3) / 4 * 4);
 }
 
