@@ -13,8 +13,8 @@ further rounding: the products with it are those of ``grouped_linear_weight_grad
 and 2^120, in float16 2^-15 and 2^8; in the highest, codes end at 240. What is not finite is held as NaN, and
 leaves the others of its block as they are.
 
-Rows: float32, bfloat16 or float16, possibly further apart than they are long. Gates are computed in float32 and rounded once. Calls run
-on the current stream of the operands' device and allocate their outputs and scratch from torch's allocator, so they can be captured
+Rows: float32, bfloat16 or float16, up to 2^30 of up to 2^20 columns, possibly further apart than they are long. Gates are computed in
+float32 and rounded once. Calls run on the current stream of the operands' device and allocate their outputs and scratch from torch's allocator, so they can be captured
 (``held_weight_gradient`` after one call of its kind outside a capture). Nothing synchronises. There is no autograd and no CPU path.
 """
 
@@ -26,7 +26,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .embedding import _empty
+from .embedding import _empty, _limits
 from .grouped import TYPES, RowGroups, _launch, _matrix, _on_device, _shares_memory, _weight_gradient, _written
 
 BLOCK = _lib.HELD_BLOCK
@@ -64,6 +64,7 @@ def _held(what: str, held: HeldRows, parts: int | None = None):
             not exponents.is_contiguous() or codes.shape[1] < 1:
         raise ValueError(f"{what}: held rows must be as hold_rows returns them")
     rows, columns = codes.shape
+    _limits(what, rows, columns)
     _parts(what, columns, held.parts)
     if parts is not None and held.parts != parts:
         raise ValueError(f"{what}: rows held in {parts} part{'s' if parts > 1 else ''} are expected, these have {held.parts}")
@@ -102,6 +103,7 @@ def hold_rows(x: torch.Tensor, parts: int = 1) -> HeldRows:
     what = "hold_rows"
     rows, columns, stride = _matrix(what, "x", x)
     kind = _kind(what, x.dtype)
+    _limits(what, rows, columns)
     _parts(what, columns, parts)
     index = _on_device(what, x)
     held = _new_held(rows, columns, parts, x)
@@ -131,6 +133,7 @@ def gated_rows(u: torch.Tensor, hold: bool = False, out: torch.Tensor | None = N
     what = "gated_rows"
     rows, columns, stride = _matrix(what, "u", u)
     kind = _kind(what, u.dtype)
+    _limits(what, rows, columns)
     _parts(what, columns, 2)
     index = _on_device(what, u)
     h, h_stride = _given(what, "out", out, rows, columns // 2, u, u.dtype, u)
@@ -154,6 +157,7 @@ def gated_rows_gradient(u: HeldRows | torch.Tensor, dh: torch.Tensor, out: torch
     else:
         rows, columns, stride = _matrix(what, "u", u)
         _kind(what, u.dtype)
+        _limits(what, rows, columns)
         _parts(what, columns, 2)
         operands, dtype, source = (u,), u.dtype, {"x": (u, stride)}
     dh_stride = _matrix(what, "dh", dh, columns // 2, rows)[2]

@@ -7,8 +7,8 @@
 
 ``tokens``: int32 or int64, one per row. A token that is no row of the table (negative, as padding has it, or >= the vocabulary) gives
 a row of zeros in an output the call allocates, leaves the row as it was in one that is given, and takes no part in a gradient. Table,
-rows and ``dy``: float32, bfloat16 or float16, rows possibly further apart than they are long. The product with ``scale`` is made in
-float32 and rounded once. The gradient is float32 whatever the rows' type, summed in float32 without atomics: the same call gives the
+rows and ``dy``: float32, bfloat16 or float16, up to 2^30 rows and 2^20 columns, rows possibly further apart than they are long. The
+product with ``scale`` is made in float32 and rounded once. The gradient is float32 whatever the rows' type, summed in float32 without atomics: the same call gives the
 same bits. It is the whole table's, with zeros where a token has no rows, as ``optimiser.AdamW`` takes it; with ``accumulate`` the rows
 of such tokens are not touched.
 
@@ -27,6 +27,7 @@ from . import _lib
 from .grouped import TYPES, _launch, _matrix, _on_device, _shares_memory, _written
 
 MAX_VOCABULARY = _lib.MAX_VOCABULARY
+MAX_ROWS, MAX_COLUMNS = 1 << 30, 1 << 20
 
 
 def _empty(rows: int, columns: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
@@ -36,6 +37,11 @@ def _empty(rows: int, columns: int, dtype: torch.dtype, device: torch.device) ->
 
 def _scratch(size: int, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
     return torch.empty_strided((size,), (1,), dtype=dtype, device=device)
+
+
+def _limits(what: str, rows: int, columns: int, most: int = MAX_ROWS) -> None:
+    if rows > most or columns > MAX_COLUMNS:
+        raise ValueError(f"{what}: {rows} x {columns}, of {most} rows and {MAX_COLUMNS} columns at most")
 
 
 class TokenOrder(NamedTuple):
@@ -82,6 +88,7 @@ def embedding(tokens: torch.Tensor, table: torch.Tensor, scale: float = 1.0, out
     dtype = dtype if dtype is not None else out.dtype if out is not None else table.dtype
     if kind is None or dtype not in TYPES:
         raise ValueError(f"{what}: table and rows must be float32, bfloat16 or float16")
+    _limits(what, tokens.shape[0] if tokens.dim() else 0, width)
     index = _on_device(what, tokens, table)
     tokens = _tokens(what, tokens)
     rows, given = tokens.shape[0], out is not None
@@ -110,6 +117,7 @@ def embedding_gradient(dy: torch.Tensor, order: TokenOrder, vocabulary: int, sca
     ``order``: as ``sort_tokens`` gives it for the same vocabulary. ``accumulate=True`` adds to ``out``."""
     what = "embedding_gradient"
     rows, width, stride = _matrix(what, "dy", dy)
+    _limits(what, rows, width)
     vocabulary = _vocabulary(what, vocabulary)
     kind = TYPES.get(dy.dtype)
     if kind is None:

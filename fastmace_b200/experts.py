@@ -25,11 +25,12 @@ from typing import NamedTuple
 import torch
 
 from . import _lib
-from .embedding import _empty, _scratch
+from .embedding import _empty, _limits, _scratch
 from .grouped import MAX_GROUPS, TYPES, _launch, _matrix, _on_device, _shares_memory, _status_pointer, _weights, _written
 
 MAX_TOP = _lib.MAX_TOP
 MAX_TOKENS = _lib.MAX_LAYER_TOKENS
+MAX_ROUTED = 1 << 24                          # tokens of route_rows
 
 
 class Routes(NamedTuple):
@@ -48,11 +49,12 @@ def _kind(what: str, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor) -> int:
 
 def route_rows(x: torch.Tensor, router: torch.Tensor, top: int, normalise: bool = True) -> Routes:
     """The ``top`` experts with the largest logits ``x router`` of each token, in falling order, equal ones by number (NaN is chosen last),
-    and their weights: the softmax over the chosen logits, or over all (``normalise=False``). Any number of tokens."""
+    and their weights: the softmax over the chosen logits, or over all (``normalise=False``). Up to 2^24 tokens."""
     what = "route_rows"
     tokens, width, stride = _matrix(what, "x", x)
     _, count, router_stride = _matrix(what, "router", router, rows=width)
     kind = _kind(what, x, router, router)
+    _limits(what, tokens, width, MAX_ROUTED)
     if count > MAX_GROUPS:
         raise ValueError(f"{what}: more than {MAX_GROUPS} experts")
     top = int(top)

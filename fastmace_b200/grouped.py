@@ -30,6 +30,7 @@ from . import _lib
 
 MAX_GROUPS = _lib.MAX_GROUPS
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+MOST = 2 ** 31 - 1                            # what an entry's 32 bits hold; a larger number would lose its upper ones on the way
 
 
 class RowGroups(NamedTuple):
@@ -123,6 +124,8 @@ def _matrix(what: str, name: str, t: torch.Tensor, columns: int | None = None, r
         raise ValueError(f"{what}: {name} is {m} x {n}, expected {m if rows is None else rows} x {n if columns is None else columns}")
     if n < 1:
         raise ValueError(f"{what}: {name} has empty rows")
+    if m > MOST or n > MOST:
+        raise ValueError(f"{what}: {name} is {m} x {n}, of {MOST} rows and columns at most")
     if (n > 1 and near != 1) or (m > 1 and far < n):
         raise ValueError(f"{what}: {name} must have contiguous rows that do not overlap")
     return m, n, far if m > 1 else n
@@ -152,6 +155,8 @@ def _weights(what: str, name: str, t: torch.Tensor):
     (g, k, n), (between, far, near) = t.shape, t.stride()
     if n > 1 and near != 1:
         raise ValueError(f"{what}: the columns of {name} must be contiguous")
+    if k > MOST or n > MOST:
+        raise ValueError(f"{what}: {name} is {k} x {n}, of {MOST} rows and columns at most")
     return g, k, n, between, far
 
 
