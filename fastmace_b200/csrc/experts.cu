@@ -32,6 +32,7 @@ namespace {
 
 constexpr int kThreads = 256, kWarps = 8;
 constexpr int kUnit = 64;                        // columns of a unit
+const float kInfinity = __builtin_huge_valf();
 constexpr int kSpins = 1 << 22;                  // polls of a wait, each of 20 ns or more, before a CTA gives up
 
 __device__ __forceinline__ float to_float(float x) { return x; }
@@ -505,11 +506,11 @@ __device__ __forceinline__ void mma_tf32(float (&c)[4], const uint32_t (&a)[4], 
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo + less than 2^-22 |x|; an infinity or NaN stays in hi alone
+// x = hi + lo + at most 2^-23 |x|: hi is off by 2^12 steps of x's 24 bits at most, of which lo's 11 hold all but the last. The rest of an infinity is
+// NaN (plain_up, plain_down).
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
     asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-    const float rest = fabsf(x) <= 3.4e38f ? x - __uint_as_float(hi) : 0.0f;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(rest));
+    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
 }
 
 // The same for a weight, of which there are many: in integers, since conversions run at a quarter of the rate (6 tokens, 50 experts of 1,024 x 1,024:
@@ -974,8 +975,9 @@ __device__ __forceinline__ void put_h(const Layer& p, int pair, int column, floa
     const float h = column < p.a.inner ? gate / (1.0f + expf(-gate)) * up : 0.0f;
     float* const to = p.h + pair * p.h_stride;
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const __nv_bfloat16 hi = __float2bfloat16_rn(h);
-        const float rest = fabsf(h) <= 3.3e38f ? h - __bfloat162float(hi) : 0.0f;
+        // (what would be rounded past bfloat16's largest number is cut off instead)
+        const __nv_bfloat16 hi = fabsf(h) <= 3.3e38f ? __float2bfloat16_rn(h) : __float2bfloat16_rz(h);
+        const float rest = fabsf(h) < kInfinity ? h - __bfloat162float(hi) : 0.0f;
         __nv_bfloat16* const four = (__nv_bfloat16*)(to + (column & ~3));
         four[column & 3] = hi;
         four[4 + (column & 3)] = __float2bfloat16_rn(rest);
@@ -984,10 +986,71 @@ __device__ __forceinline__ void put_h(const Layer& p, int pair, int column, floa
     }
 }
 
-// Lane l of warp j takes columns 8 (l / 8) + j and that + 32 of row l % 8 out, of each group of 64: the gate's result for h, or the two columns
-// of a pair's part.
+// h as put_h has kept it
+template <typename T>
+__device__ __forceinline__ float get_h(const float* h, int column) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const uint16_t* const four = (const uint16_t*)(h + (column & ~3));
+        return __uint_as_float((uint32_t)__ldcg(four + (column & 3)) << 16) + __uint_as_float((uint32_t)__ldcg(four + 4 + (column & 3)) << 16);
+    } else {
+        return __ldcg(h + column);
+    }
+}
+
+// Where operands are split in parts, an infinite one is multiplied with another's zero rest, and one near the largest number is rounded to
+// infinity. Such a sum is not finite, so what is not is asked of a plain product, by a thread alone: slow, and not met where numbers are.
+// In the first product those are sums of float32 (x and weights of 16 bits are multiplied as they are), by the CTA whose unit they are, after it;
 template <typename T, bool WIDE>
-__device__ __forceinline__ void turn_out(const Layer& p, const Smem<T, WIDE>& s, const Unit& u, int first) {
+__device__ __noinline__ void plain_up(const Layer& p, const Smem<T, WIDE>& s, const Unit& u) {
+    const int columns = 32 << p.up.log_groups, share = p.up_share * Stage<T, WIDE>::kDepth, begin = u.part * share, end = min(p.a.width, begin + share);
+    const long long pairs = (long long)p.a.tokens * p.a.top, stride = p.a.up_row_stride;
+    for (int i = threadIdx.x; i < (u.end - u.first) * columns; i += kThreads) {
+        const int at = u.first + i / columns, pair = s.pair[at], column = u.block * columns + i % columns;
+        if (column >= p.a.inner) continue;
+        float* const parts = p.up_parts + (u.part * pairs + pair) * 2 * p.h_stride + column;
+        const bool shared = p.up.splits > 1;
+        if (fabsf(shared ? parts[0] + parts[p.h_stride] : p.h[pair * p.h_stride + column]) < kInfinity) continue;
+        const T* const x = (const T*)p.x + s.token[at] * p.x_stride;
+        const T* const w = (const T*)p.a.w_up + u.expert * p.a.up_group_stride + column;
+        float gate = 0.0f, up = 0.0f;
+#pragma unroll 4
+        for (int k = begin; k < end; ++k) {
+            gate = fmaf(to_float(x[k]), to_float(w[k * stride]), gate);
+            up = fmaf(to_float(x[k]), to_float(w[k * stride + p.a.inner]), up);
+        }
+        if (shared) parts[0] = gate, parts[p.h_stride] = up;
+        else put_h<T>(p, pair, column, gate, up);
+    }
+}
+
+// in the second all, found by their weighted sum: a column of y with what is not finite of its parts anew.
+template <typename T>
+__device__ __noinline__ float plain_down(const Layer& p, int t, int column) {
+    const fmb_experts_t& a = p.a;
+    const long long pairs = (long long)a.tokens * a.top;
+    float sum = 0.0f;
+    for (int j = 0; j < a.top; ++j) {
+        const long long pair = (long long)t * a.top + j;
+        const int e = __ldcg(a.chosen + pair);
+        if (e < 0 || e >= a.experts) continue;
+        float v = 0.0f;
+        for (int part = 0; part < p.down.splits; ++part) v += __ldcg(p.parts + (part * pairs + pair) * p.part_stride + column);
+        if (!(fabsf(v) < kInfinity)) {
+            const T* const w = (const T*)a.w_down + e * a.down_group_stride + column;
+            const float* const h = p.h + pair * p.h_stride;
+            v = 0.0f;
+#pragma unroll 4
+            for (int k = 0; k < a.inner; ++k) v = fmaf(get_h<T>(h, k), to_float(w[k * a.down_row_stride]), v);
+        }
+        sum += __ldcg(a.weights + pair) * v;
+    }
+    return sum;
+}
+
+// Lane l of warp j takes columns 8 (l / 8) + j and that + 32 of row l % 8 out, of each group of 64: the gate's result for h, or the two columns
+// of a pair's part. `finite`: whether this thread's sums of float32 for h still are.
+template <typename T, bool WIDE>
+__device__ __forceinline__ void turn_out(const Layer& p, const Smem<T, WIDE>& s, const Unit& u, int first, bool& finite) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, at = first + (lane & 7);
     const Layer::Shape& shape = u.up ? p.up : p.down;
     const int warps = kWarps >> shape.log_groups;
@@ -1008,6 +1071,7 @@ __device__ __forceinline__ void turn_out(const Layer& p, const Smem<T, WIDE>& s,
             to[0] = low;
             to[32] = high;
         } else if (32 * group < p.h_stride) {
+            if (sizeof(T) == 4) finite &= fabsf(low + high) < kInfinity || 32 * group + place >= p.a.inner;
             if (shape.splits > 1) {
                 float* const to = p.up_parts + (u.part * pairs + pair) * 2 * p.h_stride + 32 * group + place;
                 to[0] = low;
@@ -1084,10 +1148,13 @@ __device__ __forceinline__ void combine(const Layer& p, int group, int tokens, F
         }
     }
     T* const y = (T*)a.y + t * a.y_stride + c;
-    const float out[4] = {sum.x, sum.y, sum.z, sum.w};
+    float out[4] = {sum.x, sum.y, sum.z, sum.w};
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        if (c + i < a.width) y[i] = rounded<T>(out[i]);
+    for (int i = 0; i < 4; ++i) {
+        if (c + i >= a.width) break;
+        if (!(fabsf(out[i]) < kInfinity)) out[i] = plain_down<T>(p, t, c + i);
+        y[i] = rounded<T>(out[i]);
+    }
 }
 
 // Which pairs belong to which expert, and which experts have any; the counters of the next launch become zero. Pairs of one expert stand in
@@ -1227,6 +1294,7 @@ k_experts(const __grid_constant__ Layer p) {
         // The unit after this one: asked for now, when this one no longer waits for others, and needed at its end.
         const int ahead = threadIdx.x == 0 ? atomicAdd(next, 1) : 0;
         const Unit v = u;
+        bool finite = true;
         for (int at = v.first; at < v.end; at += 16) {
             const bool last = at + 16 >= v.end, two_blocks = v.end - at > 8;
             float acc[4][2][4];
@@ -1245,14 +1313,18 @@ k_experts(const __grid_constant__ Layer p) {
                 r = rows_of<T, WIDE>(p, s, v, at + 16);
                 begin<T, WIDE>(p, ring, m, r, true, true);
             }
-            turn_out<T, WIDE>(p, s, v, at);
+            turn_out<T, WIDE>(p, s, v, at, finite);
             __syncthreads();                     // the sums have been read, and what they gave is written
             if (two_blocks) {
                 turn_in(s.turn, acc, 1);
                 __syncthreads();
-                turn_out<T, WIDE>(p, s, v, at + 8);
+                turn_out<T, WIDE>(p, s, v, at + 8, finite);
                 __syncthreads();
             }
+        }
+        if (sizeof(T) == 4 && v.up && !__syncthreads_and(finite)) {
+            plain_up<T, WIDE>(p, s, v);
+            __syncthreads();
         }
         bool tells = true;                       // thread 0, while its CTA goes on
         if (v.up && p.up.splits > 1) {
