@@ -1,10 +1,40 @@
-"""What the expert layer keeps of its numbers."""
+"""What the expert layer keeps of its numbers.
+
+Between the products h = silu(a) b has 17 bits with bfloat16 weights (two bfloat16, each off by half a step: 2^-9 2^-9 of h) and 23 with the others (two
+tf32, of 11 bits with a sign between them: a step of 24 bits). The tests' a are 64, where silu(a) = a in float32, and their b are sums of powers of two that
+float32 holds; a column of the second matrix takes one h less another, so y is their difference, off by what the two lose, and rounded once.
+"""
 import pytest
 import torch
 
 pytestmark = pytest.mark.gpu
 
 F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("tokens,width,inner,columns", [(1, 8, 2, 8), (9, 40, 70, 64), (17, 264, 1032, 136), (33, 33, 515, 101)])
+def test_what_passes_the_gate_keeps_its_bits(tokens, width, inner, columns, dtype):
+    from fastmace_b200 import experts
+    width = max(width, columns)
+    x = torch.zeros(tokens, width, device="cuda")
+    x[:, 0], x[:, 1], x[:, 2] = 1.0, 2.0 ** -9, 2.0 ** -20
+    x *= torch.exp2(torch.arange(tokens, device="cuda") % 3).unsqueeze(1)       # b by token: 1, 2 or 4 times
+    up = torch.zeros(1, width, 2 * inner, device="cuda")
+    up[:, 0, :inner] = 64.0
+    up[:, :2, inner:] = 1.0                                                       # b = 1 + 2^-9, and 2^-20 more in every second column
+    up[:, 2, inner::2] = 1.0
+    down = torch.zeros(1, inner, width, device="cuda")
+    for c in range(columns):
+        down[0, 2 * c % (inner - inner % 2), c] = 1.0
+        down[0, (2 * c * 7 + 1) % (inner - inner % 2), c] = -1.0
+    routes = experts.Routes(torch.zeros(tokens, 1, dtype=torch.int32, device="cuda"), torch.ones(tokens, 1, device="cuda"))
+    y = experts.expert_layer(x.to(dtype), up.to(dtype), down.to(dtype), routes)[:, :columns].double()
+    scale = torch.exp2(torch.arange(tokens, device="cuda") % 3).double().unsqueeze(1)
+    h = 64.0 * scale * scale                                                      # (a is 64 times as large as well)
+    want = h * 2.0 ** -20
+    lost = 2.0 ** -18 if dtype == BF16 else 2.0 ** -23
+    assert bool(((y - want).abs() <= 2 * h * 1.01 * lost + torch.finfo(dtype).eps / 2 * want).all()), (float(y.min()), float(y.max()))
 
 
 def _like(y, ref, off):
@@ -94,3 +124,25 @@ def test_numbers_near_the_largest_stay_finite():
         want = gate / (1 + float(torch.exp(torch.tensor(-gate, dtype=torch.float64)))) * (held[0] * held[2]) * held[3]
         y = layer(dtype, *held)
         assert bool(((y - want).abs() <= (torch.finfo(dtype).eps / 2 + 2.0 ** -17) * abs(want)).all()), (dtype, x, a, b, w, float(y[0]), want)
+
+
+@pytest.mark.parametrize("tokens,experts,top,width,inner", [(17, 12, 4, 4096, 128), (5, 3, 2, 1024, 4100), (8, 4, 2, 4096, 4096), (33, 9, 3, 515, 1001),
+                                                            (64, 4, 2, 512, 256), (1, 64, 8, 2048, 1024)])
+def test_float32_layers_are_as_near_as_float32_is(tokens, experts, top, width, inner):
+    """Each product's terms are off by 2^-21 of themselves at most (two operands by 2^-23 each, the product of their rests, 2^-22, left out), in either
+    direction alike, and so is their sum, of terms of either sign, on the norm; roundings of a sum in stages are less. Two products behind one
+    another, whose errors are independent: 2^-20.5."""
+    from fastmace_b200 import experts as m
+    g = torch.Generator(device="cuda").manual_seed(width + inner)
+    x = torch.randn(tokens, width, generator=g, device="cuda")
+    up = torch.randn(experts, width, 2 * inner, generator=g, device="cuda") / width ** 0.5
+    down = torch.randn(experts, inner, width, generator=g, device="cuda") / inner ** 0.5
+    chosen = torch.stack([torch.randperm(experts, generator=g, device="cuda")[:top] for _ in range(tokens)]).to(torch.int32)
+    weights = torch.rand(tokens, top, generator=g, device="cuda")
+    y = m.expert_layer(x, up, down, m.Routes(chosen, weights)).double()
+    ref = torch.zeros_like(y)
+    for e in range(experts):
+        t, j = torch.nonzero(chosen == e, as_tuple=True)
+        a, b = (x[t].double() @ up[e].double()).chunk(2, 1)
+        ref.index_add_(0, t, (a / (1 + torch.exp(-a)) * b) @ down[e].double() * weights[t, j].double()[:, None])
+    assert float((y - ref).norm() / ref.norm()) < 2.0 ** -20.5
