@@ -83,3 +83,20 @@ def test_layers_of_many_experts_and_short_depths(tokens, count, top, width, inne
     _check(y, x, up, down, chosen, weights)
     assert torch.equal(y, experts.expert_layer(_beside(x, 1), up, down, routes))
     grouped.check_status()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_long_sums_do_not_lose_what_is_small(dtype):
+    """A token in 900,000 places: a row of ones in 256, the others below half a step of float32 beside it, so that each is lost where they are added one
+    after the other. By eights (3 additions), the eights of a warp's 256 rows (32), the warps of a chunk (8), the 440 chunks by 32 warps (14)
+    and those (32) a term goes through 89 additions, each off by half a step of what there is."""
+    from fastmace_b200 import embedding
+    rows, width = 900_000, 8
+    dy = torch.full((rows, width), 63.0 * 2.0 ** -20, device="cuda")
+    dy[::256] = 1024.0
+    dy = dy.to(dtype)
+    tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    grad = embedding.embedding_gradient(dy, embedding.sort_tokens(tokens, 3), 3)
+    want = dy.double().sum(0)
+    assert bool(((grad[0].double() - want).abs() <= 89 * 2.0 ** -24 * want).all()), float(((grad[0].double() - want) / want).abs().max() * 2 ** 24)
+    assert bool((grad[1:] == 0).all())
