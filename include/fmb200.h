@@ -588,7 +588,8 @@ typedef struct {
     long long router_stride;
 } fmb_route_t;
 
-/* The `top` largest of the logits x router of each token in falling order, equal ones by number, NaN last, and their weights; sums in fp32 */
+/* The `top` largest of the logits x router of each token in falling order, equal ones by number, NaN last, and their weights; sums in fp32, in
+ * an order that the sizes fix and, up to 128 tokens in 16 bits, whether rows of x and router begin at multiples of 16 bytes */
 FMB_API int fmb_route_rows(const fmb_route_t* args, fmb_stream_t stream);
 
 typedef struct {
