@@ -225,7 +225,7 @@ k_release(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exponen
 }
 
 // 1 / (1 + exp(-x)): in float32 to its last bits; where results have 16 bits, by the approximate exponential and reciprocal (2 and 1 ulp, and
-// |x| 2^-24 for x log2 e)
+// |x| 2^-24 for x log2 e; below 2^-126, for x under -87.3, it is zero, and x times it less than 2e-36 off)
 template <typename T> __device__ __forceinline__ float sigmoid(float x) {
     float power, s;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(power) : "f"(x * -1.44269504088896341f));

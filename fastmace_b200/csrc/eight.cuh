@@ -11,6 +11,12 @@ namespace eight {
 
 constexpr int kEach = 8;
 
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+template <typename T> __device__ __forceinline__ T rounded(float x) { return grp::from_float<T>(x); }
+template <> __device__ __forceinline__ float rounded<float>(float x) { return x; }
+
 template <typename T> __device__ __forceinline__ uint32_t two_of(float x, float y);
 template <> __device__ __forceinline__ uint32_t two_of<__nv_bfloat16>(float x, float y) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);

@@ -21,11 +21,8 @@ namespace emb {
 
 namespace {
 
-__device__ __forceinline__ float to_float(float x) { return x; }
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-template <typename T> __device__ __forceinline__ T rounded(float x) { return grp::from_float<T>(x); }
-template <> __device__ __forceinline__ float rounded<float>(float x) { return x; }
+using eight::rounded;
+using eight::to_float;
 
 // N values side by side in one load or store of up to 16 bytes
 template <typename T, int N> struct alignas(N * sizeof(T)) Pack { T v[N]; };

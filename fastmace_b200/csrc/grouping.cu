@@ -176,6 +176,7 @@ template <typename K, bool ALONE, bool DIGIT, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, ALONE ? 1 : 64 / WARPS)
 k_group_place(const K* keys, Digit d, long long rows, int groups, int bits, const int32_t* table, const int32_t* totals,
               int32_t* __restrict__ order, int32_t* __restrict__ offsets) {
+    static_assert(!(ALONE && DIGIT), "rows of one CTA are ranked, not sorted by digits");
     constexpr int kThreads = 32 * WARPS, kRowsPerCta = WARPS * kRowsPerWarp;
     extern __shared__ int counts[];                       // [WARPS][stride], [groups + 1] starts of the CTA, [groups + 1] of all, rows
     const int width = groups + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, stride = place_stride(width);
@@ -212,8 +213,8 @@ k_group_place(const K* keys, Digit d, long long rows, int groups, int bits, cons
             int all = 0;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
-                const int count = w < warps ? counts[w * stride + q] : 0;
-                if (w < warps) counts[w * stride + q] = all;
+                const int count = counts[w * stride + q];
+                counts[w * stride + q] = all;
                 all += count;
             }
             here[q] = all;
