@@ -8,14 +8,15 @@ per 32 columns, the gate of an expert's two matrices, and the backward pass from
     dw = held_weight_gradient(held, dy, groups)                    # dW[g] = sum over its rows of x[r]^T dy[r], fp32
 
 A block's unit is the smallest power of two with |x| <= 448 units, so a value is off by at most 2^-4 of itself, or by half of the smallest
-code (2^-10 units) where it is far below its block's largest. Read back, a held value is a number of its own type with no
-further rounding: the products with it are those of ``grouped_linear_weight_gradient`` with ``release_rows(held)``. Units are between 2^-117
-and 2^120, in float16 2^-15 and 2^8; in the highest, codes end at 240. What is not finite is held as NaN, and
-leaves the others of its block as they are.
+code (2^-10 units) where it is far below its block's largest. Read back, a held value is a number of its own type with no further rounding:
+the products with it are those of ``grouped_linear_weight_gradient`` with ``release_rows(held)`` (the same bits where k is a multiple of 8).
+Units are between 2^-117 and 2^120, in float16 2^-15 and 2^8; in the highest, codes end at 240. What is not finite is held as NaN, and leaves
+the others of its block as they are.
 
 Rows: float32, bfloat16 or float16, up to 2^30 of up to 2^20 columns, possibly further apart than they are long. Gates are computed in
-float32 and rounded once. Calls run on the current stream of the operands' device and allocate their outputs and scratch from torch's allocator, so they can be captured
-(``held_weight_gradient`` after one call of its kind outside a capture). Nothing synchronises. There is no autograd and no CPU path.
+float32 and rounded once. Calls run on the current stream of the operands' device and allocate their outputs and scratch from torch's
+allocator, so they can be captured (``held_weight_gradient`` after one call of its kind outside a capture). Nothing synchronises. There is no
+autograd and no CPU path.
 """
 
 from __future__ import annotations
