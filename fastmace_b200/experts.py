@@ -6,7 +6,8 @@
 
 x ``[tokens, width]``, router ``[width, experts]``, w_up ``[experts, width, 2 inner]`` with the gate's columns first, w_down ``[experts,
 inner, width]``, y as x: float32, bfloat16 or float16, the same for all operands of a call; x and y possibly with rows further apart than
-they are long, the weights any views with contiguous columns. Up to 1,024 experts, 16 choices and, in ``expert_layer``, 128 tokens.
+they are long, the weights any views with contiguous columns. Up to 1,024 experts, 16 choices and, in ``expert_layer``, 128 tokens
+and widths of 2^17 (in ``route_rows`` 2^24 and 2^20).
 Sums are in float32 and y is rounded once: what passes between the two products keeps 17 bits with bfloat16 weights, 23 with the others. A
 product of two float32 is off by 2^-21 of itself at most. A choice that is no expert (negative, as padding has it, or >= the number of
 experts) gives nothing. The same call gives the same bits, and a token's result does not depend on what the other tokens are; how many they
