@@ -9,10 +9,12 @@ inner, width]``, y as x: float32, bfloat16 or float16, the same for all operands
 they are long, the weights any views with contiguous columns. Up to 1,024 experts, 16 choices and, in ``expert_layer``, 128 tokens
 and widths of 2^17 (in ``route_rows`` 2^24 and 2^20).
 Sums are in float32 and y is rounded once: what passes between the two products keeps 17 bits with bfloat16 weights, 23 with the others. A
-product of two float32 is off by 2^-21 of itself at most. A choice that is no expert (negative, as padding has it, or >= the number of
-experts) gives nothing. The same call gives the same bits, and a token's result does not depend on what the other tokens are; how many they
-are fixes the order of the sums with the other sizes. ``route_rows`` of up to 128 tokens in 16 bits also goes by whether the rows of x and router
-begin at multiples of 16 bytes: where logits are nearer than float32 sums are exact, a view's choices can be others than its copy's.
+product of two float32 is off by 2^-21 of itself at most where both are 2^-112 or more, and by more where they are less: what lies below
+2^-136 is lost. A choice that is no expert (negative, as padding has it, or >= the number of experts) gives nothing.
+
+The same call gives the same bits, and a token's result does not depend on what the other tokens are; how many they are fixes the order of
+the sums with the other sizes. ``route_rows`` of up to 128 tokens in 16 bits also goes by whether the rows of x and router begin at multiples of
+16 bytes: where logits are nearer than float32 sums are exact, a view's choices can be others than its copy's.
 
 Calls run on the current stream of the operands' device and allocate their outputs and scratch from torch's allocator, so they can be
 captured, ``expert_layer`` after one call outside a capture (or ``grouped.prepare_device``). Nothing synchronises. A kernel that gives up

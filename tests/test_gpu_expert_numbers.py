@@ -146,3 +146,28 @@ def test_float32_layers_are_as_near_as_float32_is(tokens, experts, top, width, i
         a, b = (x[t].double() @ up[e].double()).chunk(2, 1)
         ref.index_add_(0, t, (a / (1 + torch.exp(-a)) * b) @ down[e].double() * weights[t, j].double()[:, None])
     assert float((y - ref).norm() / ref.norm()) < 2.0 ** -20.5
+
+
+@pytest.mark.parametrize("small", ["x", "up", "down"])
+def test_float32_layers_at_the_end_of_their_range(small):
+    """A tf32's smallest step is 2^-136, which an operand loses at most beside what operands of any size do; from 2^-112 on that is no more than the last
+    of its 24 bits. Weights here are smaller, by the root of the depth: 2^-116 and 2^-115.5 of the norm, so that the step is 2^-20 and 2^-20.5 of
+    them, and as much of their sums' norm, added to the 2^-20.5 of two products."""
+    from fastmace_b200 import experts
+    tokens, width, inner, scale = 9, 264, 136, 2.0 ** -112
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = torch.randn(tokens, width, generator=g, device="cuda")
+    up = torch.randn(1, width, 2 * inner, generator=g, device="cuda") / width ** 0.5
+    down = torch.randn(1, inner, width, generator=g, device="cuda") / inner ** 0.5
+    if small == "x":
+        x, up = x * scale, up / scale
+    elif small == "up":
+        x, up = x / scale, up * scale
+    else:
+        up[:, :, inner:] /= scale
+        down *= scale
+    y = experts.expert_layer(x, up, down, experts.Routes(torch.zeros(tokens, 1, dtype=torch.int32, device="cuda"), torch.ones(tokens, 1, device="cuda")))
+    ref, _ = _plain(x, up, down)
+    operand = {"x": x, "up": up[:, :, :inner], "down": down}[small].double()
+    step = 2.0 ** -136 / float(operand.square().mean().sqrt())
+    assert float((y.double() - ref).norm() / ref.norm()) < 2.0 ** -20.5 + step
